@@ -413,6 +413,89 @@ int lkv_decode_gemm(const void* x, int64_t x_row, const void* w, int64_t w_row, 
                     int m, int64_t n_rows, int64_t k, int mode, int32_t* error_word, int* splits,
                     void* stream);
 
+/* ------------------------------------------------------------------ int8 rows
+ * bf16 rows to int8 with fp32 group scales, the activations of lkv_w4_linear_q8:
+ * a row's columns are cut into groups of `group` = 32, 64 or 128 (the last may
+ * be short); with y the row's fp32 values, a group keeps s = max|y| / 127 and
+ * q = round-to-nearest-even(y / s) (zeros where s = 0) and stands for q * s.
+ *   lkv_rmsnorm_q8:  h = x (+ residual, then residual_out = bf16(h)),
+ *                    y = h * rsqrt(mean(h^2) + eps) * weight, in fp32 throughout
+ *                    (residual and residual_out may be the same rows);
+ *                    hidden <= 32768
+ *   lkv_silu_mul_q8: gate_up rows [gate (ffn) | up (ffn)], y = silu(gate) * up
+ *   lkv_quantize_q8: y = x
+ *   lkv_dequantize_q8: out = bf16(q * s)
+ * Widths are multiples of 8; bf16 rows 16-byte aligned, q rows 8-byte aligned,
+ * row strides in elements; scale [rows, >= ceil(width / group)].  A group that
+ * holds an infinity or a NaN gets that as its scale and zeros (its values are
+ * NaN).  The norm replaces the reference's fused_add_rms_norm and the SiLU its
+ * silu_and_mul (vllm/src/lastkv/vllm/vllm_model.py:756-789) where the
+ * projections take int8 rows. */
+int lkv_rmsnorm_q8(const void* x, int64_t x_row, const void* residual, int64_t residual_row,
+                   void* residual_out, int64_t residual_out_row, const void* weight, float eps,
+                   int8_t* q, int64_t q_row, float* scale, int64_t scale_row, int64_t rows, int hidden,
+                   int group, void* stream);
+int lkv_silu_mul_q8(const void* gate_up, int64_t gate_up_row, int8_t* q, int64_t q_row, float* scale,
+                    int64_t scale_row, int64_t rows, int ffn, int group, void* stream);
+int lkv_quantize_q8(const void* x, int64_t x_row, int8_t* q, int64_t q_row, float* scale, int64_t scale_row,
+                    int64_t rows, int cols, int group, void* stream);
+int lkv_dequantize_q8(const int8_t* q, int64_t q_row, const float* scale, int64_t scale_row, void* out,
+                      int64_t out_row, int64_t rows, int cols, int group, void* stream);
+
+/* ------------------------------------------------------------------ 4-bit weights
+ * y[t, n] = sum_k x[t, k] * s[n, k / group] * (u[n, k] - 8) (+ bias[n]), bf16 out,
+ * for a weight of 4-bit codes u with bf16 group scales s along k: the model's
+ * projections (modeling.py decoder layer) with 4-bit weights.  x is bf16
+ * (lkv_w4_linear) or int8 rows with fp32 group scales of the same `group`
+ * (lkv_w4_linear_q8).  Sums inside a group are unscaled (exact int32 for int8
+ * rows, fp32 for bf16 rows), group sums are scaled and added in fp32; no weight
+ * is rounded beyond its 4 bits.
+ *   lkv_w4_bytes: bytes of the packed weight (0: unsupported shape or group)
+ *   lkv_w4_pack:  codes uint8 [n, >= k / 2], column 2i in the low half of byte i
+ *                 and 2i + 1 in the high half; scales bf16 [n, >= ceil(k / group)];
+ *                 packed: lkv_w4_bytes bytes, 16-byte aligned, laid out once per weight
+ * n >= 1 any; k a multiple of 8 (the last group may be short); group 32, 64 or
+ * 128; any number of tokens.  x rows 16-byte (bf16) or 8-byte (int8) aligned,
+ * strides in elements; bias bf16 [n] or NULL.  No workspace; one launch;
+ * sums in a fixed order (deterministic). */
+size_t lkv_w4_bytes(int64_t n, int64_t k, int group);
+int lkv_w4_pack(const uint8_t* codes, int64_t codes_row, const void* scales, int64_t scales_row, int64_t n,
+                int64_t k, int group, void* packed, void* stream);
+int lkv_w4_linear(const void* x, int64_t x_row, const void* packed, const void* bias, void* y, int64_t y_row,
+                  int64_t tokens, int64_t n, int64_t k, int group, int32_t* error_word, void* stream);
+int lkv_w4_linear_q8(const int8_t* q, int64_t q_row, const float* scale, int64_t scale_row, const void* packed,
+                     const void* bias, void* y, int64_t y_row, int64_t tokens, int64_t n, int64_t k, int group,
+                     int32_t* error_word, void* stream);
+
+/* ------------------------------------------------------------------ step plan
+ * The host plan of a step on the merged pool (_row_plan + _merged_fill,
+ * vllm/.../rmarin_flashinfer/fastpath.py:373-454, and the boundary commits of
+ * batching.py:1099-1144) built on the device from request lengths, for steps
+ * that run in a CUDA graph without the host.  Row b has num_computed[b] tokens
+ * in session slot slots[b] and num_new[b] >= 1 new ones, a span inside one
+ * chunk.  Writes every element of
+ *   block_tables int32 [num_layers, batch, width]: every layer's table
+ *       (lkv_build_layer_block_tables of the host plan's rows)
+ *   seq_k int32 [batch], cu_q int32 [batch + 1]
+ *   positions, ring_slots (relative to a layer's ring), src_slots int64
+ *       [max_tokens]; tokens past cu_q[batch] get position 0 and scratch slots
+ *   commit_raw, commit_ring int32 [batch, chunk / 16], commit_count int32 [1]:
+ *       the lkv_rope_norm_append_commit lists of the chunks that end where a
+ *       row's span begins (num_computed a positive multiple of chunk), in row order
+ * src_table int32 [num_slots, >= ceil(max_sequence_tokens / 16)]: the shared
+ * pages of each slot; ring_base int32 [num_layers]; width >= ceil(max_sequence_tokens / 16).
+ * A row with slot < 0 is padding: one token on the scratch pages (its lengths are
+ * not read).  A row that breaks these rules (or the max_tokens of the buffers) runs
+ * on the scratch pages and is recorded in error_word (may be NULL).  All lengths
+ * are read on the device; one launch (PDL). */
+int lkv_plan_step(const int32_t* num_computed, const int32_t* num_new, const int32_t* slots, int batch,
+                  const int32_t* src_table, int64_t src_table_stride, int num_slots, int max_sequence_tokens,
+                  int chunk, const int32_t* ring_base, int num_layers, int scratch_src_page,
+                  int scratch_ring_page, int width, int max_tokens, int32_t* block_tables, int32_t* seq_k,
+                  int32_t* cu_q, int64_t* positions, int64_t* ring_slots, int64_t* src_slots,
+                  int32_t* commit_raw, int32_t* commit_ring, int32_t* commit_count, int32_t* error_word,
+                  void* stream);
+
 /* ------------------------------------------------------------------ context-parallel combine
  * Exchange + LSE merge of sequence-sharded decode partials over NVLink peer
  * memory, replacing the all-gather of the partials and lkv_merge_partials for

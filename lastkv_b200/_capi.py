@@ -54,6 +54,16 @@ _SIGNATURES = {
     "lkv_rmsnorm": (I32, [P, I64, P, I64, P, I64, P, P, I64, I32, I32, F32, P]),
     "lkv_silu_mul": (I32, [P, I64, P, I64, I64, I32, P]),
     "lkv_argmax_rows": (I32, [P, I64, I32, I32, P, P]),
+    "lkv_rmsnorm_q8": (I32, [P, I64, P, I64, P, I64, P, F32, P, I64, P, I64, I64, I32, I32, P]),
+    "lkv_silu_mul_q8": (I32, [P, I64, P, I64, P, I64, I64, I32, I32, P]),
+    "lkv_quantize_q8": (I32, [P, I64, P, I64, P, I64, I64, I32, I32, P]),
+    "lkv_dequantize_q8": (I32, [P, I64, P, I64, P, I64, I64, I32, I32, P]),
+    "lkv_w4_bytes": (SZ, [I64, I64, I32]),
+    "lkv_w4_pack": (I32, [P, I64, P, I64, I64, I64, I32, P, P]),
+    "lkv_w4_linear": (I32, [P, I64, P, P, P, I64, I64, I64, I64, I32, P, P]),
+    "lkv_w4_linear_q8": (I32, [P, I64, P, I64, P, P, P, I64, I64, I64, I64, I32, P, P]),
+    "lkv_plan_step": (I32, [P, P, P, I32, P, I64, I32, I32, I32, P, I32, I32, I32, I32, I32,
+                            P, P, P, P, P, P, P, P, P, P, P]),
     "lkv_decode_gemm_plan": (I32, [I64, I64, I32, P, P, P]),
     "lkv_cp_combine_sizes": (I32, [I64, I32, I32, P, P]),
     "lkv_cp_combine": (I32, [P, P, I32, I32, P, I64, I32, I32, P, P, I64, P, P]),

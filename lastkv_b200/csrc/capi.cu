@@ -501,6 +501,90 @@ int lkv_argmax_rows(const void* x, int64_t row_stride, int rows, int cols, int64
   return lkv::argmax_rows(x, row_stride, rows, cols, out, static_cast<cudaStream_t>(stream));
 }
 
+int lkv_rmsnorm_q8(const void* x, int64_t x_row, const void* residual, int64_t residual_row, void* residual_out,
+                   int64_t residual_out_row, const void* weight, float eps, int8_t* q, int64_t q_row, float* scale,
+                   int64_t scale_row, int64_t rows, int hidden, int group, void* stream) {
+  return lkv::rmsnorm_q8(x, x_row, residual, residual_row, residual_out, residual_out_row, weight, eps,
+                         lkv::Q8RowsArgs{q, q_row, scale, scale_row, rows, hidden, group},
+                         static_cast<cudaStream_t>(stream));
+}
+
+int lkv_silu_mul_q8(const void* gate_up, int64_t gate_up_row, int8_t* q, int64_t q_row, float* scale,
+                    int64_t scale_row, int64_t rows, int ffn, int group, void* stream) {
+  return lkv::rows_q8(gate_up, gate_up_row, 1, lkv::Q8RowsArgs{q, q_row, scale, scale_row, rows, ffn, group},
+                      static_cast<cudaStream_t>(stream));
+}
+
+int lkv_quantize_q8(const void* x, int64_t x_row, int8_t* q, int64_t q_row, float* scale, int64_t scale_row,
+                    int64_t rows, int cols, int group, void* stream) {
+  return lkv::rows_q8(x, x_row, 0, lkv::Q8RowsArgs{q, q_row, scale, scale_row, rows, cols, group},
+                      static_cast<cudaStream_t>(stream));
+}
+
+int lkv_dequantize_q8(const int8_t* q, int64_t q_row, const float* scale, int64_t scale_row, void* out,
+                      int64_t out_row, int64_t rows, int cols, int group, void* stream) {
+  return lkv::dequantize_q8(lkv::Q8RowsArgs{const_cast<int8_t*>(q), q_row, const_cast<float*>(scale), scale_row,
+                                            rows, cols, group},
+                            out, out_row, static_cast<cudaStream_t>(stream));
+}
+
+size_t lkv_w4_bytes(int64_t n, int64_t k, int group) { return lkv::w4_bytes(n, k, group); }
+
+int lkv_w4_pack(const uint8_t* codes, int64_t codes_row, const void* scales, int64_t scales_row, int64_t n,
+                int64_t k, int group, void* packed, void* stream) {
+  return lkv::w4_pack(codes, codes_row, scales, scales_row, n, k, group, packed, static_cast<cudaStream_t>(stream));
+}
+
+int lkv_w4_linear(const void* x, int64_t x_row, const void* packed, const void* bias, void* y, int64_t y_row,
+                  int64_t tokens, int64_t n, int64_t k, int group, int32_t* error_word, void* stream) {
+  return lkv::w4_linear(lkv::W4Args{x, x_row, nullptr, 0, packed, bias, y, y_row, tokens, n, k, group, error_word},
+                        static_cast<cudaStream_t>(stream));
+}
+
+int lkv_w4_linear_q8(const int8_t* q, int64_t q_row, const float* scale, int64_t scale_row, const void* packed,
+                     const void* bias, void* y, int64_t y_row, int64_t tokens, int64_t n, int64_t k, int group,
+                     int32_t* error_word, void* stream) {
+  if (tokens != 0 && !scale) return LKV_ERR_INVALID_ARGUMENT;
+  return lkv::w4_linear(
+      lkv::W4Args{q, q_row, scale, scale_row, packed, bias, y, y_row, tokens, n, k, group, error_word},
+      static_cast<cudaStream_t>(stream));
+}
+
+int lkv_plan_step(const int32_t* num_computed, const int32_t* num_new, const int32_t* slots, int batch,
+                  const int32_t* src_table, int64_t src_table_stride, int num_slots, int max_sequence_tokens,
+                  int chunk, const int32_t* ring_base, int num_layers, int scratch_src_page, int scratch_ring_page,
+                  int width, int max_tokens, int32_t* block_tables, int32_t* seq_k, int32_t* cu_q,
+                  int64_t* positions, int64_t* ring_slots, int64_t* src_slots, int32_t* commit_raw,
+                  int32_t* commit_ring, int32_t* commit_count, int32_t* error_word, void* stream) {
+  lkv::PlanArgs a{};
+  a.num_computed = num_computed;
+  a.num_new = num_new;
+  a.slots = slots;
+  a.batch = batch;
+  a.src_table = src_table;
+  a.src_table_stride = src_table_stride;
+  a.num_slots = num_slots;
+  a.max_sequence_tokens = max_sequence_tokens;
+  a.chunk = chunk;
+  a.ring_base = ring_base;
+  a.num_layers = num_layers;
+  a.scratch_src_page = scratch_src_page;
+  a.scratch_ring_page = scratch_ring_page;
+  a.width = width;
+  a.max_tokens = max_tokens;
+  a.block_tables = block_tables;
+  a.seq_k = seq_k;
+  a.cu_q = cu_q;
+  a.positions = positions;
+  a.ring_slots = ring_slots;
+  a.src_slots = src_slots;
+  a.commit_raw = commit_raw;
+  a.commit_ring = commit_ring;
+  a.commit_count = commit_count;
+  a.error_word = error_word;
+  return lkv::plan_step(a, static_cast<cudaStream_t>(stream));
+}
+
 int lkv_cp_combine_sizes(int64_t rows, int head_dim, int world, int64_t* send_floats, int64_t* recv_words) {
   if (rows < 1 || head_dim < 1 || world < 1 || world > lkv::kCpMaxRanks) return LKV_ERR_INVALID_ARGUMENT;
   if (send_floats) *send_floats = (rows * (head_dim + 1) + 3) / 4 * 4;

@@ -19,6 +19,7 @@ enum DevErr : int {
   DEVERR_WAIT_TIMEOUT = 1,  // an mbarrier wait gave up (TMA never landed / peer never arrived)
   DEVERR_BAD_PAGE = 2,      // a block-table entry was outside the pool (its keys were skipped)
   DEVERR_BAD_SLOT = 3,      // an append slot was outside the pool (the store was skipped)
+  DEVERR_BAD_SPAN = 4,      // a planned row broke the plan's rules (it runs on the scratch pages)
 };
 
 __device__ __forceinline__ void report_error(int* err, int code, int kernel, int detail) {
@@ -170,6 +171,35 @@ __device__ __forceinline__ uint64_t policy_evict_last() {
   uint64_t p;
   asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
   return p;
+}
+
+// ---------------------------------------------------------------- clusters
+
+__device__ __forceinline__ void cluster_sync_all() {
+  __syncwarp();  // the barrier is .aligned: every warp arrives converged
+  asm volatile(
+      "barrier.cluster.arrive.release.aligned;\n"
+      "barrier.cluster.wait.acquire.aligned;" ::
+          : "memory");
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+// Address of the same shared-memory location in CTA `rank` of this cluster.
+__device__ __forceinline__ uint32_t dsmem_map(uint32_t saddr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+  return r;
+}
+
+__device__ __forceinline__ float dsmem_ld(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
 }
 
 // ---------------------------------------------------------------- fragments

@@ -185,4 +185,59 @@ int decode_gemm_plan(int64_t n_rows, int64_t k, int mode, int* tiles, int* split
 int decode_gemm(const void* x, int64_t x_row, const void* w, int64_t w_row, void* y, int64_t y_row, int m,
                 int64_t n_rows, int64_t k, int mode, int32_t* error_word, cudaStream_t stream, int* splits_out);
 
+// int8 rows with fp32 group scales (rows_q8.cu); strides in elements
+struct Q8RowsArgs {
+  int8_t* q;
+  int64_t q_row;
+  float* scale;
+  int64_t scale_row;
+  int64_t rows;
+  int cols, group;
+};
+int rmsnorm_q8(const void* x, int64_t x_row, const void* residual, int64_t residual_row, void* residual_out,
+               int64_t residual_out_row, const void* weight, float eps, const Q8RowsArgs& a, cudaStream_t stream);
+int rows_q8(const void* x, int64_t x_row, int silu, const Q8RowsArgs& a, cudaStream_t stream);
+int dequantize_q8(const Q8RowsArgs& a, void* out, int64_t out_row, cudaStream_t stream);
+
+// products with 4-bit weights (w4.cu); x_scale NULL: x is bf16, else int8 rows with group scales
+size_t w4_bytes(int64_t n, int64_t k, int group);
+int w4_pack(const uint8_t* codes, int64_t codes_row, const void* scales, int64_t scales_row, int64_t n, int64_t k,
+            int group, void* packed, cudaStream_t stream);
+struct W4Args {
+  const void* x;
+  int64_t x_row;
+  const float* x_scale;
+  int64_t x_scale_row;
+  const void* packed;
+  const void* bias;  // bf16 [n] or NULL
+  void* y;
+  int64_t y_row;
+  int64_t tokens, n, k;
+  int group;
+  int32_t* error_word;
+};
+int w4_linear(const W4Args& a, cudaStream_t stream);
+
+// a step's tables from request lengths (plan.cu); passed to the kernel by value
+struct PlanArgs {
+  const int32_t* num_computed;
+  const int32_t* num_new;
+  const int32_t* slots;
+  const int32_t* src_table;
+  int64_t src_table_stride;
+  const int32_t* ring_base;
+  int batch, max_tokens, num_layers, num_slots, max_sequence_tokens, chunk, scratch_src_page, scratch_ring_page, width;
+  int32_t* block_tables;
+  int32_t* seq_k;
+  int32_t* cu_q;
+  int64_t* positions;
+  int64_t* ring_slots;
+  int64_t* src_slots;
+  int32_t* commit_raw;
+  int32_t* commit_ring;
+  int32_t* commit_count;
+  int32_t* error_word;
+};
+int plan_step(const PlanArgs& a, cudaStream_t stream);
+
 }  // namespace lkv

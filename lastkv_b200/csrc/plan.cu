@@ -1,0 +1,200 @@
+// A step's block tables, slot maps, positions and boundary commits from request lengths,
+// in one launch (sm_100a): the device form of the host plan of the merged pool
+// (vllm/src/lastkv/vllm/backends/rmarin_flashinfer/fastpath.py:373-454), for steps that
+// are captured in a CUDA graph and advance without the host.
+//
+// For row b with p0 computed tokens, n new ones and session slot s (C the chunk, P = 16,
+// RP = 2C / P ring pages per slot):
+//   last = p0 + n - 1, cur = floor(last / C) C, rec = max(0, cur - C), ns = rec / P,
+//   np = ceil((last + 1 - rec) / P)
+//   table[l, b, j] = src_table[s, j]                                    j < ns
+//                  = ring_base[l] + s RP + (ns % RP + j - ns) % RP      ns <= j < ns + np
+//                  = ring_base[l]                                       beyond
+//   seq_k[b] = last + 1;  token p of the row: position p, ring slot s 2C + p % 2C,
+//   shared slot src_table[s, p / P] P + p % P
+//   a commit of chunk [p0 - C, p0) where n > 0, p0 > 0 and p0 % C = 0: the step is the
+//   first after that chunk (spans never cross a boundary, so each chunk gets exactly one)
+// A row with slot < 0 is padding: one token on the scratch pages.  A row that breaks the
+// plan's rules (a span over a chunk boundary, past the capacity, a slot that is not
+// there, n < 1, more tokens than the buffers hold) is recorded in the error word and runs
+// on the scratch pages too.
+//
+// Writing L x B x W table words is the floor.  grid = (rows + 1) x parts: a block takes
+// one part of a row's columns, computes each column once and stores it for every layer;
+// the extra row fills the unused tokens and commit rows.  Every block scans the rows'
+// lengths itself (a few KB from L2), which costs less than a second launch.
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "launch.cuh"
+
+namespace lkv {
+
+namespace {
+
+constexpr int kPlanThreads = 256;
+constexpr int kPlanKernelId = 12;
+
+struct Row {
+  int p0, n, slot;  // slot < 0: padding, runs on the scratch pages
+  int tokens;       // token slots that the row takes in the buffers
+  bool bad;
+};
+
+__device__ __forceinline__ Row load_row(const PlanArgs& a, int b) {
+  Row r;
+  r.p0 = a.num_computed[b];
+  r.n = a.num_new[b];
+  r.slot = a.slots[b];
+  r.bad = false;
+  if (r.slot < 0) {
+    r.p0 = 0;
+    r.n = 1;
+  } else {
+    const int64_t end = (int64_t)r.p0 + r.n;
+    r.bad = r.slot >= a.num_slots || r.p0 < 0 || r.n < 1 || end > a.max_sequence_tokens ||
+            r.p0 / a.chunk != (int)((end - 1) / a.chunk);
+  }
+  r.tokens = max(0, min(r.n, a.max_tokens));
+  return r;
+}
+
+__device__ __forceinline__ bool row_commits(const PlanArgs& a, const Row& r) {
+  return !r.bad && r.slot >= 0 && r.p0 > 0 && r.p0 % a.chunk == 0;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.x, part = blockIdx.y, parts = gridDim.y;
+  const bool tail = b == a.batch;
+  // tokens and commits of the rows before this one, and of all rows (saturating: a sum
+  // past the buffers is past them)
+  __shared__ int64_t s_tok[2][kPlanThreads / 32];
+  __shared__ int s_com[2][kPlanThreads / 32];
+  int64_t tok[2] = {0, 0};
+  int com[2] = {0, 0};
+  for (int i = threadIdx.x; i < a.batch; i += kPlanThreads) {
+    const Row r = load_row(a, i);
+    const int c = row_commits(a, r) ? 1 : 0;
+    tok[1] += r.tokens;
+    com[1] += c;
+    if (i < b) {
+      tok[0] += r.tokens;
+      com[0] += c;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      tok[k] += __shfl_xor_sync(0xffffffffu, tok[k], o);
+      com[k] += __shfl_xor_sync(0xffffffffu, com[k], o);
+    }
+    if ((threadIdx.x & 31) == 0) {
+      s_tok[k][threadIdx.x >> 5] = tok[k];
+      s_com[k][threadIdx.x >> 5] = com[k];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    tok[k] = 0;
+    com[k] = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+      tok[k] += s_tok[k][w];
+      com[k] += s_com[k][w];
+    }
+  }
+  const int64_t first_tok = tok[0] < a.max_tokens ? tok[0] : a.max_tokens;
+  const int64_t all_tok = tok[1] < a.max_tokens ? tok[1] : a.max_tokens;
+  const int ppc = a.chunk / LKV_PAGE_SIZE, ring_pages = 2 * ppc;
+  const int gtid = part * kPlanThreads + threadIdx.x, gsize = parts * kPlanThreads;
+  const int64_t pad_ring = (int64_t)a.scratch_ring_page * LKV_PAGE_SIZE;
+  const int64_t pad_src = (int64_t)a.scratch_src_page * LKV_PAGE_SIZE;
+
+  if (tail) {
+    for (int64_t t = all_tok + gtid; t < a.max_tokens; t += gsize) {
+      a.positions[t] = 0;
+      a.ring_slots[t] = pad_ring;
+      a.src_slots[t] = pad_src;
+    }
+    for (int64_t i = (int64_t)com[1] * ppc + gtid; i < (int64_t)a.batch * ppc; i += gsize) {
+      a.commit_raw[i] = 0;
+      a.commit_ring[i] = 0;
+    }
+    if (gtid == 0) {
+      a.cu_q[a.batch] = (int)all_tok;
+      a.commit_count[0] = com[1];
+    }
+    return;
+  }
+
+  const Row r = load_row(a, b);
+  const bool over = tok[0] + r.tokens > a.max_tokens;
+  const bool real = r.slot >= 0 && !r.bad && !over;
+  if (gtid == 0) {
+    if (r.bad || over) report_error(a.error_word, DEVERR_BAD_SPAN, kPlanKernelId, b);
+    a.cu_q[b] = (int)first_tok;
+    a.seq_k[b] = real ? r.p0 + r.n : max(1, (int)(min(first_tok + r.tokens, (int64_t)a.max_tokens) - first_tok));
+  }
+  const int last = r.p0 + r.n - 1;
+  const int rec = max(0, last / a.chunk * a.chunk - a.chunk);
+  const int ns = real ? rec / LKV_PAGE_SIZE : 0;
+  const int np = real ? (last + LKV_PAGE_SIZE - rec) / LKV_PAGE_SIZE : 0;
+  const int32_t* src = a.src_table + (int64_t)(real ? r.slot : 0) * a.src_table_stride;
+  for (int j = gtid; j < a.width; j += gsize) {
+    int v = 0;
+    if (j < ns)
+      v = src[j];
+    else if (j < ns + np)
+      v = r.slot * ring_pages + (ns % ring_pages + j - ns) % ring_pages;
+    else if (!real && j == 0)
+      v = a.scratch_ring_page;
+    int32_t* dst = a.block_tables + (int64_t)b * a.width + j;
+    const int64_t layer = (int64_t)a.batch * a.width;
+    for (int l = 0; l < a.num_layers; ++l) dst[l * layer] = j < ns ? v : v + a.ring_base[l];
+  }
+  for (int i = gtid; i < r.tokens; i += gsize) {
+    const int64_t t = first_tok + i;
+    if (t >= a.max_tokens) break;
+    const int p = r.p0 + i;
+    a.positions[t] = real ? p : 0;
+    a.ring_slots[t] = real ? (int64_t)r.slot * 2 * a.chunk + p % (2 * a.chunk) : pad_ring;
+    a.src_slots[t] = real ? (int64_t)src[p / LKV_PAGE_SIZE] * LKV_PAGE_SIZE + p % LKV_PAGE_SIZE : pad_src;
+  }
+  if (row_commits(a, r)) {
+    const int page = (r.p0 - a.chunk) / LKV_PAGE_SIZE;
+    const int32_t* own = a.src_table + (int64_t)r.slot * a.src_table_stride;
+    for (int i = gtid; i < ppc; i += gsize) {
+      a.commit_raw[(int64_t)com[0] * ppc + i] = own[page + i];
+      a.commit_ring[(int64_t)com[0] * ppc + i] = a.ring_base[0] + r.slot * ring_pages + page % ring_pages + i;
+    }
+  }
+}
+
+}  // namespace
+
+int plan_step(const PlanArgs& a, cudaStream_t stream) {
+  if (a.batch < 0 || a.max_tokens < 0 || a.num_layers < 1 || a.num_slots < 1 || a.max_sequence_tokens < 1 ||
+      a.chunk < LKV_PAGE_SIZE || a.chunk % LKV_PAGE_SIZE || a.chunk > (1 << 29))
+    return LKV_ERR_INVALID_ARGUMENT;
+  const int pages = (int)(((int64_t)a.max_sequence_tokens + LKV_PAGE_SIZE - 1) / LKV_PAGE_SIZE);
+  // a row uses ceil((last + 1) / 16) columns: older pages and ring pages together
+  if (a.src_table_stride < pages || a.width < pages) return LKV_ERR_INVALID_ARGUMENT;
+  if (a.batch == 0) return LKV_OK;
+  if (!a.num_computed || !a.num_new || !a.slots || !a.src_table || !a.ring_base || !a.block_tables || !a.seq_k ||
+      !a.cu_q || !a.positions || !a.ring_slots || !a.src_slots || !a.commit_raw || !a.commit_ring ||
+      !a.commit_count)
+    return LKV_ERR_INVALID_ARGUMENT;
+  const int parts = std::max(1, std::min((a.width + kPlanThreads - 1) / kPlanThreads, 65535));
+  return launch_pdl(plan_step_kernel, dim3((unsigned)a.batch + 1, (unsigned)parts), dim3(kPlanThreads), 0, stream,
+                    a) == cudaSuccess
+             ? LKV_OK
+             : LKV_ERR_CUDA;
+}
+
+}  // namespace lkv

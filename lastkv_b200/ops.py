@@ -16,7 +16,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _capi
-from .contract import PAGE_SIZE, RMarinBackendContractError, require_heads
+from .contract import PAGE_SIZE, RMarinBackendContractError, require_chunk_size, require_heads
 
 
 # lkv_decode_paged / lkv_decode_paged_cp flags (include/lastkv_b200.h): the tables predate the PDL chain;
@@ -586,6 +586,284 @@ def decode_gemm(x, weight, *, silu_mul: bool = False, out=None, error_word=None)
                                      out.data_ptr(), n_out, M, N, K, mode, _ptr(error_word), None, _stream())
     _capi.check(st, "lkv_decode_gemm")
     return out
+
+
+# ------------------------------------------------------------------ int8 rows, 4-bit weights
+
+Q8_GROUPS = (32, 64, 128)
+
+
+class Q8Rows(NamedTuple):
+    """int8 rows with fp32 group scales: ``q`` [rows, K] stands for ``q * scale`` per group of
+    ``group`` columns; ``scale`` [rows, ceil(K / group)].  ``shape`` is the activations' shape."""
+
+    q: torch.Tensor
+    scale: torch.Tensor
+    group: int
+    lead: Optional[tuple] = None  # leading dimensions of the rows they came from (None: q's)
+
+    @classmethod
+    def empty(cls, lead: tuple, cols: int, group: int, device) -> "Q8Rows":
+        rows = 1
+        for n in lead:
+            rows *= n
+        pitch = -(-cols // 16) * 16  # 16-byte rows, whatever the width
+        q = torch.empty((rows, pitch), dtype=torch.int8, device=device)
+        return cls(q if pitch == cols else q[:, :cols],
+                   torch.empty((rows, -(-cols // group)), dtype=torch.float32, device=device), group, tuple(lead))
+
+
+def _check_group(group) -> None:
+    _require(group in Q8_GROUPS, f"group must be one of {Q8_GROUPS}, got {group!r}")
+
+
+def _check_q8(r: Q8Rows, what: str) -> None:
+    _check_group(r.group)
+    _require(r.q.is_cuda and r.q.dtype == torch.int8 and r.q.dim() == 2 and r.q.stride(1) == 1,
+             f"{what}.q must be CUDA int8 [rows, K] rows")
+    _require(r.scale.is_cuda and r.scale.dtype == torch.float32 and r.scale.dim() == 2 and r.scale.stride(1) == 1
+             and r.scale.shape == (r.q.shape[0], -(-r.q.shape[1] // r.group)),
+             f"{what}.scale must be CUDA fp32 [rows, ceil(K / group)] rows")
+
+
+def _q8_out(out, x, cols: int, group: int) -> Q8Rows:
+    _check_group(group)
+    if out is None:
+        return Q8Rows.empty(tuple(x.shape[:-1]), cols, group, x.device)
+    _check_q8(out, "out")
+    _require(out.group == group and out.q.shape == (x.numel() // max(x.shape[-1], 1), cols), "out layout")
+    return out
+
+
+def _out2d(t, cols: int, name: str):
+    """An output's rows, written in place: 2-D rows of any stride, or contiguous."""
+    _require(t.is_cuda and t.dtype == torch.bfloat16 and t.dim() >= 1 and t.shape[-1] == cols
+             and ((t.dim() == 2 and t.stride(1) == 1) or t.is_contiguous()),
+             f"{name} must be CUDA bf16 [..., {cols}], contiguous or 2-D rows")
+    return t if t.dim() == 2 else t.view(-1, cols)
+
+
+def _row_stride(t) -> int:
+    """Row stride of a 2-D tensor as the kernels take it (one row has no stride to speak of)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+@_traced
+def rmsnorm_q8(x, weight, eps: float, residual=None, *, group: int = 128, out: Optional[Q8Rows] = None,
+               residual_out=None):
+    """RMSNorm rows as int8 with group scales (lkv_rmsnorm_q8), all in fp32 before the int8.
+
+    x bf16 [..., H] rows.  With ``residual`` the kernel first forms ``h = x + residual`` and
+    returns ``(h, rows)``, h rounded to bf16 (``residual_out`` may be ``residual`` itself);
+    otherwise ``rows`` (:class:`Q8Rows`).
+    """
+    x2 = _rows2d(x, "x")
+    H = x2.shape[1]
+    _require(weight.is_cuda and weight.dtype == torch.bfloat16 and weight.is_contiguous() and weight.numel() == H,
+             "weight must be CUDA bf16 [H]")
+    rows = _q8_out(out, x, H, group)
+    r2 = ro2 = None
+    if residual is not None:
+        r2 = _rows2d(residual, "residual")
+        _require(r2.shape == x2.shape, "residual must match x")
+        if residual_out is None:
+            residual_out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
+        ro2 = _out2d(residual_out, H, "residual_out")
+        _require(ro2.shape == x2.shape, "residual_out must match x")
+    st = _capi.lib().lkv_rmsnorm_q8(
+        x2.data_ptr(), _row_stride(x2), _ptr(r2), _row_stride(r2) if r2 is not None else 0, _ptr(ro2),
+        _row_stride(ro2) if ro2 is not None else 0, weight.data_ptr(), float(eps), rows.q.data_ptr(),
+        _row_stride(rows.q), rows.scale.data_ptr(), _row_stride(rows.scale), x2.shape[0], H, group, _stream())
+    _capi.check(st, "lkv_rmsnorm_q8")
+    return rows if residual is None else (residual_out, rows)
+
+
+@_traced
+def silu_mul_q8(gate_up, *, group: int = 128, out: Optional[Q8Rows] = None) -> Q8Rows:
+    """``silu(gate) * up`` for bf16 [..., 2F] rows of [gate | up], as int8 rows (lkv_silu_mul_q8)."""
+    x2 = _rows2d(gate_up, "gate_up")
+    _require(x2.shape[1] % 2 == 0, "gate_up must be [..., 2F]")
+    rows = _q8_out(out, gate_up, x2.shape[1] // 2, group)
+    st = _capi.lib().lkv_silu_mul_q8(x2.data_ptr(), _row_stride(x2), rows.q.data_ptr(), _row_stride(rows.q),
+                                     rows.scale.data_ptr(), _row_stride(rows.scale), x2.shape[0], x2.shape[1] // 2,
+                                     group, _stream())
+    _capi.check(st, "lkv_silu_mul_q8")
+    return rows
+
+
+@_traced
+def quantize_q8(x, *, group: int = 128, out: Optional[Q8Rows] = None) -> Q8Rows:
+    """bf16 [..., K] rows as int8 rows with group scales (lkv_quantize_q8)."""
+    x2 = _rows2d(x, "x")
+    rows = _q8_out(out, x, x2.shape[1], group)
+    st = _capi.lib().lkv_quantize_q8(x2.data_ptr(), _row_stride(x2), rows.q.data_ptr(), _row_stride(rows.q),
+                                     rows.scale.data_ptr(), _row_stride(rows.scale), x2.shape[0], x2.shape[1], group,
+                                     _stream())
+    _capi.check(st, "lkv_quantize_q8")
+    return rows
+
+
+@_traced
+def dequantize_q8(rows: Q8Rows, out=None):
+    """The bf16 values [..., K] that int8 rows stand for (lkv_dequantize_q8)."""
+    _check_q8(rows, "rows")
+    T, K = rows.q.shape
+    shape = (*(rows.lead if rows.lead is not None else (T,)), K)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=rows.q.device)
+    o2 = _out2d(out, K, "out")
+    _require(o2.shape[0] == T, "out must have the rows' count")
+    st = _capi.lib().lkv_dequantize_q8(rows.q.data_ptr(), _row_stride(rows.q), rows.scale.data_ptr(),
+                                       _row_stride(rows.scale), o2.data_ptr(), _row_stride(o2), T, K, rows.group,
+                                       _stream())
+    _capi.check(st, "lkv_dequantize_q8")
+    return out
+
+
+class W4Weight(NamedTuple):
+    """A weight [n, k] of 4-bit codes with bf16 group scales, in the kernels' layout (``w4_pack``)."""
+
+    packed: torch.Tensor
+    n: int
+    k: int
+    group: int
+
+
+@_traced
+def w4_pack(codes, scales, group: int = 128) -> W4Weight:
+    """Lay out a 4-bit weight for ``w4_linear`` (once per weight; lkv_w4_pack).
+
+    codes uint8 [n, k / 2]: codes u of value u - 8, column 2i in the low half of byte i and
+    2i + 1 in the high half; scales bf16 [n, ceil(k / group)].
+    """
+    _check_group(group)
+    _require(codes.is_cuda and codes.dtype == torch.uint8 and codes.dim() == 2 and codes.stride(1) == 1,
+             "codes must be CUDA uint8 [n, k / 2]")
+    n, k = codes.shape[0], 2 * codes.shape[1]
+    _require(scales.is_cuda and scales.dtype == torch.bfloat16 and scales.dim() == 2 and scales.stride(1) == 1
+             and scales.shape == (n, -(-k // group)), "scales must be CUDA bf16 [n, ceil(k / group)]")
+    nbytes = _capi.lib().lkv_w4_bytes(n, k, group)
+    _require(nbytes > 0, f"4-bit weights need n >= 1 and k a positive multiple of 8, got [{n}, {k}]")
+    packed = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
+    st = _capi.lib().lkv_w4_pack(codes.data_ptr(), _row_stride(codes), scales.data_ptr(), _row_stride(scales), n, k,
+                                 group, packed.data_ptr(), _stream())
+    _capi.check(st, "lkv_w4_pack")
+    return W4Weight(packed, n, k, group)
+
+
+def w4_quantize(weight, group: int = 128) -> W4Weight:
+    """A [n, k] weight rounded to 4 bits: per group s = bf16(max|w| / 7), code = rne(w / s) in -8 .. 7."""
+    _check_group(group)
+    _require(weight.dim() == 2 and weight.is_floating_point(), "weight must be a floating-point [n, k] matrix")
+    n, k = weight.shape
+    _require(k % 8 == 0, f"k must be a multiple of 8, got {k}")
+    w = torch.nn.functional.pad(weight.detach().float(), (0, -k % group)).view(n, -1, group)
+    scales = (w.abs().amax(-1) / 7).to(torch.bfloat16)
+    s = scales.float()[..., None]
+    u = (torch.where(s == 0, torch.zeros_like(w), w / s).round_().clamp_(-8, 7) + 8).to(torch.uint8)
+    u = u.view(n, -1)[:, :k]
+    return w4_pack((u[:, 0::2] | (u[:, 1::2] << 4)).contiguous(), scales, group)
+
+
+@_traced
+def w4_linear(x, weight: W4Weight, bias=None, *, out=None, error_word=None):
+    """``x @ w.T (+ bias)`` for a 4-bit weight: x bf16 [..., k] or :class:`Q8Rows` of the
+    weight's group; bf16 out [..., n], any number of rows (lkv_w4_linear, lkv_w4_linear_q8)."""
+    n, k = weight.n, weight.k
+    q8 = isinstance(x, Q8Rows)
+    if q8:
+        _check_q8(x, "x")
+        _require(x.group == weight.group, f"rows of groups of {x.group} against a weight of groups of {weight.group}")
+        x2, lead = x.q, x.lead if x.lead is not None else (x.q.shape[0],)
+    else:
+        x2, lead = _rows2d(x, "x"), tuple(x.shape[:-1])
+    _require(x2.shape[1] == k, f"x has {x2.shape[1]} columns, the weight {k}")
+    if out is None:
+        out = torch.empty((*lead, n), dtype=torch.bfloat16, device=x2.device)
+    o2 = _out2d(out, n, "out")
+    _require(o2.shape[0] == x2.shape[0], "out must have the rows of x")
+    if bias is not None:
+        _require(bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == n and bias.is_cuda,
+                 "bias must be bf16 [n]")
+    T = x2.shape[0]
+    if q8:
+        st = _capi.lib().lkv_w4_linear_q8(x2.data_ptr(), _row_stride(x2), x.scale.data_ptr(), _row_stride(x.scale),
+                                          weight.packed.data_ptr(), _ptr(bias), o2.data_ptr(), _row_stride(o2), T, n,
+                                          k, weight.group, _ptr(error_word), _stream())
+    else:
+        st = _capi.lib().lkv_w4_linear(x2.data_ptr(), _row_stride(x2), weight.packed.data_ptr(), _ptr(bias),
+                                       o2.data_ptr(), _row_stride(o2), T, n, k, weight.group, _ptr(error_word),
+                                       _stream())
+    _capi.check(st, "lkv_w4_linear_q8" if q8 else "lkv_w4_linear")
+    return out
+
+
+# ------------------------------------------------------------------ step plan
+
+
+class StepPlan:
+    """A step's tables, built on the device from request lengths (lkv_plan_step).
+
+    Holds the static buffers of steps of ``batch`` rows and at most ``max_tokens`` new tokens
+    over a merged pool: ``src_table`` int32 [slots, pages] (the shared pages of every session
+    slot), ``ring_base`` int32 [layers].  ``run(num_computed, num_new, slots)`` (int32 [batch]
+    on the device; slot -1 pads a row) fills ``block_tables`` [layers, batch, width],
+    ``seq_k``, ``cu_q``, ``positions``, ``ring_slots`` (relative to a layer's ring),
+    ``src_slots`` and the boundary commits ``commit_raw`` / ``commit_ring`` /
+    ``commit_count`` that the step's first append carries.  Rows that break the plan's rules
+    run on the scratch pages and set ``error_word``.  Capturable in CUDA graphs.
+    """
+
+    def __init__(self, batch: int, max_tokens: int, src_table, ring_base, *, chunk_size: int,
+                 max_sequence_tokens: int, scratch_src_page: int, scratch_ring_page: int,
+                 width: int | None = None, error_word=None):
+        require_chunk_size(chunk_size)
+        _require(batch >= 1 and max_tokens >= 1, "a step has at least one row and one token")
+        _require(src_table.is_cuda and src_table.dtype == torch.int32 and src_table.dim() == 2
+                 and src_table.stride(1) == 1, "src_table must be CUDA int32 [slots, pages]")
+        _require(ring_base.is_cuda and ring_base.dtype == torch.int32 and ring_base.is_contiguous()
+                 and ring_base.dim() == 1 and ring_base.numel() >= 1, "ring_base must be CUDA int32 [layers]")
+        pages = -(-max_sequence_tokens // PAGE_SIZE)
+        _require(max_sequence_tokens >= 1 and src_table.shape[1] >= pages,
+                 "src_table must hold ceil(max_sequence_tokens / 16) pages per slot")
+        self.width = int(width) if width is not None else src_table.shape[1] + 2 * chunk_size // PAGE_SIZE
+        _require(self.width >= pages, "width must hold ceil(max_sequence_tokens / 16) pages")
+        dev, ppc = src_table.device, chunk_size // PAGE_SIZE
+        self.batch, self.max_tokens, self.chunk_size = int(batch), int(max_tokens), chunk_size
+        self.max_sequence_tokens = int(max_sequence_tokens)
+        self.src_table, self.ring_base = src_table, ring_base
+
+        def i32(*shape):
+            return torch.zeros(shape, dtype=torch.int32, device=dev)
+
+        self.block_tables = i32(ring_base.numel(), batch, self.width)
+        self.seq_k, self.cu_q = i32(batch), i32(batch + 1)
+        self.positions, self.ring_slots, self.src_slots = (
+            torch.zeros(max_tokens, dtype=torch.int64, device=dev) for _ in range(3))
+        self.commit_raw, self.commit_ring, self.commit_count = i32(batch, ppc), i32(batch, ppc), i32(1)
+        self.error_word = error_word if error_word is not None else i32(4)
+        # everything after the lengths is the same in every call
+        self._rest = (self.batch, src_table.data_ptr(), _row_stride(src_table), src_table.shape[0],
+                      self.max_sequence_tokens, chunk_size, ring_base.data_ptr(), ring_base.numel(),
+                      int(scratch_src_page), int(scratch_ring_page), self.width, self.max_tokens,
+                      *(t.data_ptr() for t in (self.block_tables, self.seq_k, self.cu_q, self.positions,
+                                               self.ring_slots, self.src_slots, self.commit_raw, self.commit_ring,
+                                               self.commit_count, self.error_word)))
+
+    def run(self, num_computed, num_new, slots) -> "StepPlan":
+        for name, t in (("num_computed", num_computed), ("num_new", num_new), ("slots", slots)):
+            _require(t.is_cuda and t.dtype == torch.int32 and t.is_contiguous() and t.numel() == self.batch,
+                     f"{name} must be CUDA int32 [{self.batch}]")
+        st = _capi.lib().lkv_plan_step(num_computed.data_ptr(), num_new.data_ptr(), slots.data_ptr(), *self._rest,
+                                       _stream())
+        _capi.check(st, "lkv_plan_step")
+        return self
+
+    def check_errors(self) -> None:
+        """Raise if a planned row broke the rules (synchronises)."""
+        e = self.error_word.cpu().tolist()
+        if e[0]:
+            raise RMarinBackendContractError(f"device error word set: step plan {e}")
 
 
 def cp_combine_sizes(rows: int, head_dim: int, world: int) -> dict:
