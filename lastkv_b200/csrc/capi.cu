@@ -87,21 +87,33 @@ int make_query_tensor_map(CUtensorMap* map, const void* q, int64_t total_q, int6
 // 2-D map over a row-major bf16 matrix [rows, cols] (row stride in elements),
 // copying (box_rows x 64 columns) tiles of 128-byte rows, 128-byte swizzled: a
 // K-major UMMA operand tile.  Reads past the matrix fill zeros.
-int make_matrix_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t row_stride,
-                           int box_rows) {
+namespace {
+int matrix_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t row_stride, int box_rows,
+               CUtensorMapDataType type, int elem) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return LKV_ERR_TENSOR_MAP;
   if ((reinterpret_cast<uintptr_t>(base) & 15) || rows < 1 || cols < 1 || rows > (int64_t)0x7fffffff ||
-      cols > (int64_t)0x7fffffff || row_stride < cols || (row_stride * 2) % 16 || box_rows < 1 || box_rows > 256)
+      cols > (int64_t)0x7fffffff || row_stride < cols || (row_stride * elem) % 16 || box_rows < 1 || box_rows > 256)
     return LKV_ERR_INVALID_ARGUMENT;
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)row_stride * 2};
-  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  cuuint64_t strides[1] = {(cuuint64_t)row_stride * elem};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / elem), (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+  CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? LKV_OK : LKV_ERR_TENSOR_MAP;
+}
+}  // namespace
+
+int make_matrix_tensor_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t row_stride,
+                           int box_rows) {
+  return matrix_map(map, base, rows, cols, row_stride, box_rows, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2);
+}
+
+int make_matrix_tensor_map_s8(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t row_stride,
+                              int box_rows) {
+  return matrix_map(map, base, rows, cols, row_stride, box_rows, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1);
 }
 
 }  // namespace lkv

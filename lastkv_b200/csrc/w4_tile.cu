@@ -1,0 +1,590 @@
+// Products with 4-bit weights for more than a few tokens, on tcgen05 (sm_100a).
+//
+// Tile: 128 output rows (the MMA's M side) x TN tokens (N side).  Per 128 bytes of k (128
+// columns of int8 rows, 64 of bf16 rows) one stage of shared memory holds the A operand -
+// the codes, expanded from 4 bits to int8 (16 c) or bf16 (c, exact) by the four dequant
+// warps - and the B operand, the rows as they are, by TMA; both K-major, 128-byte swizzled.
+//
+// Group scales stay out of the operands: a group's MMAs sum into one of two TMEM buffers
+// from zero (int32 or fp32), and the eight drain warps add each finished group into fp32
+// registers, scaled by the weight's scale of their lane's row and, for int8 rows, by the
+// tokens' scales, while the tensor core sums the next group into the other buffer.  So
+// int8 x 4-bit group sums are exact and no weight is rounded, at the price of reading
+// 128 x TN sums from TMEM per group.
+//
+// Roles of the 512 threads (one CTA per SM, persistent over the tiles):
+//   warp 0  rows and weight scales by TMA       warp 1     tcgen05.mma issue, TMEM
+//   warp 2  the tokens' scales (int8 rows)      warp 3     codes by bulk copies
+//   warps 4-7    codes -> A tiles               warps 8-15 drain, epilogue
+// Where the tiles alone do not fill the GPU, k is split over the CTAs of a cluster, whose
+// partial tiles meet in shared memory (added in split order).
+
+#include <algorithm>
+#include <mutex>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "launch.cuh"
+#include "tcgen05.cuh"
+#include "w4.cuh"
+
+namespace lkv {
+
+namespace {
+
+constexpr int kM = 128;
+constexpr int kDrainWgs = 2;
+constexpr int kThreads = 256 + 128 * kDrainWgs;
+constexpr int kKernelId = 13;
+constexpr int kAStage = kM * 128;
+constexpr int kMaxSplits = 8;
+
+struct TileParams {
+  const uint8_t* packed;
+  const float* x_scale;
+  int64_t x_scale_row;
+  const __nv_bfloat16* bias;
+  __nv_bfloat16* y;
+  int64_t y_row;
+  int tokens, n, k, kblocks, row_blocks, tok_tiles, tiles, splits;
+  int* err;
+};
+
+// Ring depths: A stages (16 KB, filled in the CTA), B stages (TN x 128 bytes, from L2).
+template <int TN>
+__host__ __device__ constexpr int a_stages() {
+  return TN == 256 ? 3 : 4;
+}
+template <int TN>
+__host__ __device__ constexpr int b_stages() {
+  return TN == 256 ? 4 : TN == 128 ? 6 : TN == 64 ? 8 : 12;
+}
+
+// 128-column blocks of codes (8 KB for the tile's 128 rows) in flight
+template <int TN>
+__host__ __device__ constexpr int code_slots() {
+  return TN == 256 ? 3 : TN == 128 ? 5 : TN == 64 ? 8 : 10;
+}
+
+
+template <int TN>
+__host__ __device__ constexpr int ring_bytes() {
+  return a_stages<TN>() * kAStage + b_stages<TN>() * TN * 128 + code_slots<TN>() * 2 * kCodeBytes;
+}
+
+constexpr int kWsSlots = 4;
+constexpr int kXsGroups = 8;  // one 32-byte sector of a token's scales
+
+template <bool INT8, int G, int TN>
+struct Shared {
+  uint64_t a_full[a_stages<TN>()], a_empty[a_stages<TN>()];
+  uint64_t b_full[b_stages<TN>()], b_empty[b_stages<TN>()];
+  uint64_t d_full[2];
+  uint64_t d_empty[2];
+  uint64_t done;
+  uint64_t c_full[code_slots<TN>()], c_empty[code_slots<TN>()];
+  uint64_t ws_full[kWsSlots], ws_empty[kWsSlots];
+  uint64_t xs_full[2], xs_empty[2];
+  uint32_t tmem;
+  alignas(16) uint8_t ws[kWsSlots][2][kTileRows * 2 * (kTileK / G)];  // the weight's scales of a 128-column block
+  alignas(16) float xs[INT8 ? 2 : 1][kXsGroups][INT8 ? TN : 4];      // the tokens' scales of eight groups
+};
+
+template <bool INT8, int G, int TN>
+constexpr int smem_bytes() {
+  return 1024 + ring_bytes<TN>() + (int)sizeof(Shared<INT8, G, TN>);
+}
+
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+__device__ __forceinline__ void st_shared8(uint32_t addr, uint32_t a, uint32_t b) {
+  asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+}
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// Two int32 below 2^22 in magnitude (128 x 127 x 128 < 2^21) to fp32, exactly: 1.5 * 2^23 + v
+// has v in its low mantissa bits.  Two adds on the fp32 pipes; the conversion instruction
+// runs at an eighth of their rate.
+__device__ __forceinline__ float2 int_float2(uint32_t a, uint32_t b) {
+  return __fadd2_rn(make_float2(__uint_as_float(a + 0x4b400000u), __uint_as_float(b + 0x4b400000u)),
+                    make_float2(-12582912.f, -12582912.f));
+}
+
+template <bool INT8, int G, int TN>
+__global__ void __launch_bounds__(kThreads, 1)
+    w4_tile_kernel(const __grid_constant__ CUtensorMap tmx, const TileParams p) {
+  constexpr int SA = a_stages<TN>(), SB = b_stages<TN>(), C = code_slots<TN>(), kBStage = TN * 128;
+  constexpr int kSpb = INT8 ? 1 : 2;               // stages per 128-column block
+  constexpr int kMpg = INT8 ? G / 32 : G / 16;     // MMAs per group
+  constexpr int kGpb = kTileK / G;                 // groups per block
+  constexpr int kCols = TN / kDrainWgs;            // tokens of one drain warpgroup
+  constexpr int kLd = kCols < 16 ? kCols : 16;     // columns per TMEM load
+  constexpr uint32_t kIdesc = INT8 ? umma_idesc_s8(kM, TN) : umma_idesc_bf16(kM, TN, 0, 0);
+  constexpr uint32_t kTmemCols = 2 * TN;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  using Sh = Shared<INT8, G, TN>;
+  uint8_t* b_ring = smem + SA * kAStage;
+  uint8_t* codes = b_ring + SB * kBStage;  // [C][2][kCodeBytes]
+  Sh* sh = reinterpret_cast<Sh*>(smem + ring_bytes<TN>());
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = blockIdx.y;
+  const int kb0 = (int)((int64_t)p.kblocks * split / p.splits);
+  const int kb1 = (int)((int64_t)p.kblocks * (split + 1) / p.splits);
+  const int nkb = kb1 - kb0;
+  pdl_launch_dependents();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < SA; ++s) {
+      mbar_init(&sh->a_full[s], 4);
+      mbar_init(&sh->a_empty[s], 1);
+    }
+    for (int s = 0; s < SB; ++s) {
+      mbar_init(&sh->b_full[s], 1);
+      mbar_init(&sh->b_empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sh->d_full[b], 1);
+      mbar_init(&sh->d_empty[b], 4 * kDrainWgs);
+    }
+    mbar_init(&sh->done, 1);
+    for (int b = 0; b < C; ++b) {
+      mbar_init(&sh->c_full[b], 1);
+      mbar_init(&sh->c_empty[b], 4);
+    }
+    for (int b = 0; b < kWsSlots; ++b) {
+      mbar_init(&sh->ws_full[b], 1);
+      mbar_init(&sh->ws_empty[b], 4 * kDrainWgs);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sh->xs_full[b], 1);
+      mbar_init(&sh->xs_empty[b], 4 * kDrainWgs);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sh->tmem, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem;
+
+  if (warp < 4) {
+    regs_dec<40>();
+    if (warp == 0) {
+      if (lane == 0) {
+        // ------------------------------------------------------------ rows by TMA
+        tma_prefetch_desc(&tmx);
+        pdl_wait();
+        uint32_t it = 0, blk = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
+          const int tok0 = tile % p.tok_tiles * TN, rb = tile / p.tok_tiles * 2;
+          for (int kb = 0; ok && kb < nkb; ++kb, ++blk) {
+            const int b = blk % kWsSlots;
+            ok = mbar_wait(&sh->ws_empty[b], ((blk / kWsSlots) & 1) ^ 1);
+            if (!ok) break;
+            constexpr uint32_t kWs = sizeof(sh->ws[0][0]);
+            const int halves = min(2, p.row_blocks - rb);
+            mbar_arrive_expect_tx(&sh->ws_full[b], kWs * halves);
+            for (int h = 0; h < halves; ++h)
+              bulk_load(sh->ws[b][h],
+                        p.packed + ((int64_t)(rb + h) * p.kblocks + kb0 + kb) * block_bytes(G) + kCodeBytes, kWs,
+                        &sh->ws_full[b]);
+            for (int i = 0; i < kSpb; ++i, ++it) {
+              const int s = it % SB;
+              ok = mbar_wait(&sh->b_empty[s], ((it / SB) & 1) ^ 1);
+              if (!ok) break;
+              mbar_arrive_expect_tx(&sh->b_full[s], kBStage);
+              tma_load_2d(b_ring + s * kBStage, &tmx, &sh->b_full[s],
+                          ((kb0 + kb) * kSpb + i) * (INT8 ? 128 : 64), tok0);
+            }
+          }
+        }
+        if (!ok) {  // no copy may still be in flight when the CTA leaves
+          report_error(p.err, DEVERR_WAIT_TIMEOUT, kKernelId, (int)it);
+          for (uint32_t i = it > SB ? it - SB : 0; i < it; ++i) mbar_wait(&sh->b_full[i % SB], (i / SB) & 1);
+          for (uint32_t i = blk > kWsSlots ? blk - kWsSlots : 0; i < blk; ++i)
+            mbar_wait(&sh->ws_full[i % kWsSlots], (i / kWsSlots) & 1);
+        }
+      }
+    } else if (warp == 1) {
+      // -------------------------------------------------------------- MMA issue
+      const uint32_t base = smem_u32(smem);
+      uint32_t it = 0, grp = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
+        for (int kb = 0; ok && kb < nkb; ++kb) {
+#pragma unroll
+          for (int m = 0; m < 4 * kSpb; ++m) {
+            const int sa = it % SA, sb = it % SB;
+            if (m % 4 == 0)
+              ok = ok && mbar_wait(&sh->a_full[sa], (it / SA) & 1) && mbar_wait(&sh->b_full[sb], (it / SB) & 1);
+            if (m % kMpg == 0) ok = ok && mbar_wait(&sh->d_empty[grp & 1], ((grp >> 1) & 1) ^ 1);
+            if (m % 4 == 0 || m % kMpg == 0) {
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              tc_fence_after();
+            }
+            if (elect_one()) {
+              const uint64_t da = umma_sdesc_sw128(base + sa * kAStage + (m % 4) * 32, 16, 1024);
+              const uint64_t db = umma_sdesc_sw128(base + SA * kAStage + sb * kBStage + (m % 4) * 32, 16, 1024);
+              const uint32_t d = tmem + (grp & 1) * TN;
+              if (INT8)
+                umma_s8_ss(d, da, db, kIdesc, m % kMpg != 0);
+              else
+                umma_bf16_ss(d, da, db, kIdesc, m % kMpg != 0);
+              if (m % 4 == 3) {
+                umma_commit(&sh->a_empty[sa]);
+                umma_commit(&sh->b_empty[sb]);
+              }
+              if (m % kMpg == kMpg - 1) umma_commit(&sh->d_full[grp & 1]);
+            }
+            __syncwarp();
+            if (m % 4 == 3) ++it;
+            if (m % kMpg == kMpg - 1) ++grp;
+          }
+        }
+      }
+      if (!ok && lane == 0) report_error(p.err, DEVERR_WAIT_TIMEOUT, kKernelId, 1000000 + (int)it);
+      if (elect_one()) umma_commit(&sh->done);
+      __syncwarp();
+      mbar_wait(&sh->done, 0);  // no MMA may still be in flight when TMEM is freed
+    } else if (warp == 3) {
+      // -------------------------------------------------------------- codes by bulk copies
+      if (lane == 0) {  // before the previous kernel has finished: the weights do not depend on it
+        uint32_t blk = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
+          const int rb = tile / p.tok_tiles * 2, halves = min(2, p.row_blocks - rb);
+          const uint8_t* src = p.packed + ((int64_t)rb * p.kblocks + kb0) * block_bytes(G);
+          for (int kb = 0; kb < nkb; ++kb, ++blk, src += block_bytes(G)) {
+            const int b = blk % C;
+            ok = mbar_wait(&sh->c_empty[b], ((blk / C) & 1) ^ 1);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&sh->c_full[b], kCodeBytes * halves);
+            for (int h = 0; h < halves; ++h)
+              bulk_load(codes + (b * 2 + h) * kCodeBytes, src + (int64_t)h * p.kblocks * block_bytes(G), kCodeBytes,
+                        &sh->c_full[b]);
+          }
+        }
+        if (!ok) {
+          report_error(p.err, DEVERR_WAIT_TIMEOUT, kKernelId, 5000000 + (int)blk);
+          for (uint32_t i = blk > C ? blk - C : 0; i < blk; ++i) mbar_wait(&sh->c_full[i % C], (i / C) & 1);
+        }
+      }
+    } else if (INT8) {
+      // -------------------------------------------------------------- the tokens' scales, transposed
+      pdl_wait();
+      const int groups = (p.k + G - 1) / G, g0 = kb0 * kGpb, g1 = kb1 * kGpb;
+      const bool wide = (reinterpret_cast<uintptr_t>(p.x_scale) & 15) == 0 && p.x_scale_row % 4 == 0 && g0 % 4 == 0;
+      uint32_t slot = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
+        const int tok0 = tile % p.tok_tiles * TN;
+        for (int gr = g0; ok && gr < g1; gr += kXsGroups, ++slot) {
+          const int b = slot & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh->xs_empty[b], ((slot >> 1) & 1) ^ 1));
+          if (!ok) break;
+          for (int c = lane; c < TN; c += 32) {
+            float v[kXsGroups];
+            const float* src = p.x_scale + (int64_t)(tok0 + c) * p.x_scale_row + gr;
+            if (tok0 + c < p.tokens && wide && gr + kXsGroups <= groups) {
+              const float4 lo = *reinterpret_cast<const float4*>(src), hi = *reinterpret_cast<const float4*>(src + 4);
+              v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w;
+              v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+            } else {
+#pragma unroll
+              for (int e = 0; e < kXsGroups; ++e) v[e] = tok0 + c < p.tokens && gr + e < groups ? src[e] : 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < kXsGroups; ++e) sh->xs[b][e][c] = v[e];
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->xs_full[b]);
+        }
+      }
+      if (!ok && lane == 0) report_error(p.err, DEVERR_WAIT_TIMEOUT, kKernelId, 4000000 + (int)slot);
+    }
+  } else if (warp < 8) {
+    // ---------------------------------------------------------------- codes -> A tiles
+    // the block launches with 128 registers a thread: 40 + 88 + 2 x 192 = 4 x 128
+    regs_dec<88>();
+    constexpr int kN = INT8 ? 4 : 2;  // 16-byte pieces (rows g and g + 8 of a sub-tile, two 32-column steps) per lane
+    // Piece of lane 4 g + t.  A phase of eight lanes reads all eight 16-byte banks of its 128
+    // bytes (t and the parity of g) and stores to all eight swizzled chunks (chunk ^ g): the
+    // rows of a phase are g and g ^ 5; phases in the order 0, 2, 1, 3 also keep the 8-byte
+    // stores of half a warp apart.
+    const int w = warp - 4, t = lane & 3, q3 = lane >> 3;
+    const int g = ((q3 & 1) << 1 | q3 >> 1) ^ ((lane & 4) ? 5 : 0);
+    uint32_t it = 0, blk = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
+      const int halves = min(2, p.row_blocks - tile / p.tok_tiles * 2);
+      for (int kb = 0; ok && kb < nkb; ++kb, ++blk) {
+        const int b = blk % C;
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh->c_full[b], (blk / C) & 1));
+        if (!ok) break;
+        const uint8_t* src = codes + b * 2 * kCodeBytes + (4 * g + t) * 16;
+#pragma unroll
+        for (int i = 0; i < kSpb; ++i, ++it) {
+          uint4 v[kN];
+#pragma unroll
+          for (int q = 0; q < kN; ++q) {
+            const int c = w * kN + q;  // int8: (half, r, j); bf16: (half, r), j from the stage
+            const int hb = INT8 ? c >> 3 : c >> 2, r = INT8 ? (c >> 1) & 3 : c & 3, j = INT8 ? c & 1 : i;
+            v[q] = hb < halves ? *reinterpret_cast<const uint4*>(src + hb * kCodeBytes + r * 1024 + j * 512)
+                               : make_uint4(0, 0, 0, 0);
+          }
+          if (i == kSpb - 1) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->c_empty[b]);
+          }
+          const int s = it % SA;
+          ok = ok && __all_sync(0xffffffffu, mbar_wait(&sh->a_empty[s], ((it / SA) & 1) ^ 1));
+          if (!ok) break;
+          const uint32_t a = smem_u32(smem + s * kAStage);
+#pragma unroll
+          for (int q = 0; q < kN; ++q) {
+            const int c = w * kN + q;
+            const int hb = INT8 ? c >> 3 : c >> 2, r = INT8 ? (c >> 1) & 3 : c & 3, j = INT8 ? c & 1 : 0;
+            const uint32_t words[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t row = a + (hb * 64 + 16 * r + 8 * (e & 1) + g) * 128;
+              const uint32_t u = words[e];
+              if (INT8) {
+                const int chunk = 2 * (2 * j + (e >> 1)) + (t >> 1);
+                st_shared8(row + ((chunk ^ g) << 4) + 8 * (t & 1), u << 4 & 0xf0f0f0f0u, u & 0xf0f0f0f0u);
+              } else {
+                const uint32_t c02 = codes_bf16<0>(u), c46 = codes_bf16<1>(u), c13 = codes_bf16<2>(u),
+                               c57 = codes_bf16<3>(u);
+                const int chunk = 4 * (e >> 1) + t;
+                st_shared16(row + ((chunk ^ g) << 4), __byte_perm(c02, c13, 0x5410), __byte_perm(c02, c13, 0x7632),
+                            __byte_perm(c46, c57, 0x5410), __byte_perm(c46, c57, 0x7632));
+              }
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->a_full[s]);
+        }
+      }
+    }
+    if (!ok && lane == 0) report_error(p.err, DEVERR_WAIT_TIMEOUT, kKernelId, 2000000 + (int)it);
+  } else {
+    // ---------------------------------------------------------------- drain, epilogue
+    regs_inc<192>();
+    const int wg = (warp - 8) >> 2, tid = threadIdx.x & 127, sub = warp & 3;
+    const uint32_t lanes = (uint32_t)(sub * 32) << 16;
+    // scale of row 16 r + 8 h + g of a 64-row block at 2 (8 g + 2 r + h)
+    const int ws_off = 2 * (8 * (tid & 7) + 2 * ((tid >> 4) & 3) + ((tid >> 3) & 1));
+    pdl_wait();  // before any global write
+    uint32_t grp = 0, blk = 0, slot = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
+      const int tok0 = tile % p.tok_tiles * TN + wg * kCols;
+      const int row = (tile / p.tok_tiles) * kM + tid;
+      const bool live_row = tile / p.tok_tiles * 2 + (tid >> 6) < p.row_blocks;
+      float2 acc[kCols / 2];
+#pragma unroll
+      for (int c = 0; c < kCols / 2; ++c) acc[c] = make_float2(0.f, 0.f);
+      int gt = 0;  // group of this tile's range
+      for (int kb = 0; ok && kb < nkb; ++kb, ++blk) {
+        const int b = blk % kWsSlots;
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh->ws_full[b], (blk / kWsSlots) & 1));
+        if (!ok) break;
+#pragma unroll 1
+        for (int gi = 0; gi < kGpb; ++gi, ++gt) {
+          const int buf = grp & 1;
+          float w1 = live_row ? __uint_as_float((uint32_t)*reinterpret_cast<const unsigned short*>(
+                                                    &sh->ws[b][tid >> 6][gi * 128 + ws_off])
+                                                << 16)
+                              : 0.f;
+          if (INT8) w1 *= 0.0625f;  // int8 codes stand at 16 c
+          const float2 ws = make_float2(w1, w1);
+          const float* xs = &sh->xs[INT8 ? slot & 1 : 0][gt % kXsGroups][INT8 ? wg * kCols : 0];
+          if (INT8 && gt % kXsGroups == 0) ok = mbar_wait(&sh->xs_full[slot & 1], (slot >> 1) & 1);
+          ok = ok && mbar_wait(&sh->d_full[buf], (grp >> 1) & 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t at = tmem + lanes + buf * TN + wg * kCols;
+#pragma unroll
+          for (int c0 = 0; c0 < kCols; c0 += kLd) {
+            uint32_t u[16];
+            if constexpr (kLd == 16)
+              tmem_ld16(at + c0, u);
+            else
+              tmem_ld8(at + c0, u);
+            tmem_wait_ld16(u);
+            if (c0 + kLd == kCols) {  // the buffer is read: the tensor core may sum the next group but one
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sh->d_empty[buf]);
+            }
+#pragma unroll
+            for (int c = 0; c < kLd; c += 4) {
+              float2 s0 = ws, s1 = ws, v0, v1;
+              if (INT8) {
+                const float4 x4 = *reinterpret_cast<const float4*>(xs + c0 + c);
+                s0 = __fmul2_rn(ws, make_float2(x4.x, x4.y));
+                s1 = __fmul2_rn(ws, make_float2(x4.z, x4.w));
+                v0 = int_float2(u[c], u[c + 1]);
+                v1 = int_float2(u[c + 2], u[c + 3]);
+              } else {
+                v0 = make_float2(__uint_as_float(u[c]), __uint_as_float(u[c + 1]));
+                v1 = make_float2(__uint_as_float(u[c + 2]), __uint_as_float(u[c + 3]));
+              }
+              acc[(c0 + c) / 2] = __ffma2_rn(v0, s0, acc[(c0 + c) / 2]);
+              acc[(c0 + c) / 2 + 1] = __ffma2_rn(v1, s1, acc[(c0 + c) / 2 + 1]);
+            }
+          }
+          ++grp;
+          if (INT8 && (gt % kXsGroups == kXsGroups - 1 || gt == nkb * kGpb - 1)) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->xs_empty[slot & 1]);
+            ++slot;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->ws_empty[b]);
+      }
+      if (!ok) break;
+      if (p.splits == 1) {
+        const float b = p.bias && row < p.n ? __bfloat162float(p.bias[row]) : 0.f;
+        __nv_bfloat16* y = p.y + (int64_t)tok0 * p.y_row + row;
+#pragma unroll
+        for (int c = 0; c < kCols / 2; ++c) {
+          if (row < p.n) {
+            if (tok0 + 2 * c < p.tokens) y[(int64_t)(2 * c) * p.y_row] = __float2bfloat16_rn(acc[c].x + b);
+            if (tok0 + 2 * c + 1 < p.tokens) y[(int64_t)(2 * c + 1) * p.y_row] = __float2bfloat16_rn(acc[c].y + b);
+          }
+        }
+      } else {
+        // one tile per cluster: every stage has been consumed, their memory takes the partial [token][row]
+        float* part = reinterpret_cast<float*>(smem) + wg * kCols * kM;
+#pragma unroll
+        for (int c = 0; c < kCols / 2; ++c) {
+          part[(2 * c) * kM + tid] = acc[c].x;
+          part[(2 * c + 1) * kM + tid] = acc[c].y;
+        }
+      }
+    }
+    if (!ok && lane == 0) report_error(p.err, DEVERR_WAIT_TIMEOUT, kKernelId, 3000000 + (int)grp);
+  }
+
+  __syncwarp();
+  if (p.splits > 1) {
+    cluster_sync_all();  // every split has published its partial
+    const int tile = blockIdx.x;
+    const int tok0 = tile % p.tok_tiles * TN, row0 = tile / p.tok_tiles * kM;
+    const int live = min(TN, p.tokens - tok0) * kM;
+    const uint32_t base = smem_u32(smem);
+    for (int i = (int)cluster_rank() * kThreads + threadIdx.x; i < live; i += p.splits * kThreads) {
+      const int r = row0 + i % kM;
+      float v[kMaxSplits];
+#pragma unroll
+      for (int s = 0; s < kMaxSplits; ++s) v[s] = s < p.splits ? dsmem_ld(dsmem_map(base, s) + i * 4) : 0.f;
+      float sum = 0.f;
+#pragma unroll
+      for (int s = 0; s < kMaxSplits; ++s) sum += v[s];
+      if (r < p.n) {
+        if (p.bias) sum += __bfloat162float(p.bias[r]);
+        p.y[(int64_t)(tok0 + i / kM) * p.y_row + r] = __float2bfloat16_rn(sum);
+      }
+    }
+    cluster_sync_all();  // the partials stay readable until every CTA has read them
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+template <bool INT8, int G, int TN>
+int launch(const CUtensorMap& map, const TileParams& p, int sms, cudaStream_t stream) {
+  static std::once_flag once[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return LKV_ERR_CUDA;
+  static cudaError_t set[64];
+  std::call_once(once[dev], [&] {
+    set[dev] = cudaFuncSetAttribute(w4_tile_kernel<INT8, G, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    smem_bytes<INT8, G, TN>());
+  });
+  if (set[dev] != cudaSuccess) return LKV_ERR_CUDA;
+  const dim3 grid(std::min(p.tiles, std::max(1, sms / p.splits)), p.splits);
+  return launch_pdl_cluster(w4_tile_kernel<INT8, G, TN>, grid, dim3(kThreads), smem_bytes<INT8, G, TN>(), stream,
+                            dim3(1, p.splits, 1), map, p) == cudaSuccess
+             ? LKV_OK
+             : LKV_ERR_CUDA;
+}
+
+template <bool INT8, int G>
+int by_tokens(int tn, const CUtensorMap& map, const TileParams& p, int sms, cudaStream_t stream) {
+  switch (tn) {
+    case 32: return launch<INT8, G, 32>(map, p, sms, stream);
+    case 64: return launch<INT8, G, 64>(map, p, sms, stream);
+    case 128: return launch<INT8, G, 128>(map, p, sms, stream);
+    default: return launch<INT8, G, 256>(map, p, sms, stream);
+  }
+}
+
+}  // namespace
+
+bool w4_tile_aligned(const W4Args& a) {
+  const int elem = a.x_scale ? 1 : 2;
+  return (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && (a.x_row * elem) % 16 == 0;
+}
+
+int w4_tile(const W4Args& a, int sms, cudaStream_t stream) {
+  const bool int8 = a.x_scale != nullptr;
+  TileParams p{};
+  p.packed = static_cast<const uint8_t*>(a.packed);
+  p.x_scale = a.x_scale;
+  p.x_scale_row = a.x_scale_row;
+  p.bias = static_cast<const __nv_bfloat16*>(a.bias);
+  p.y = static_cast<__nv_bfloat16*>(a.y);
+  p.y_row = a.y_row;
+  p.tokens = (int)a.tokens;
+  p.n = (int)a.n;
+  p.k = (int)a.k;
+  p.kblocks = (int)((a.k + kTileK - 1) / kTileK);
+  p.row_blocks = (int)((a.n + kTileRows - 1) / kTileRows);
+  p.err = a.error_word;
+  const int tn = a.tokens <= 32 ? 32 : a.tokens <= 64 ? 64 : a.tokens <= 128 ? 128 : 256;
+  p.tok_tiles = (int)((a.tokens + tn - 1) / tn);
+  const int64_t tiles = (a.n + kM - 1) / kM * p.tok_tiles;
+  if (tiles > 0x7fffffff) return LKV_ERR_UNSUPPORTED;
+  p.tiles = (int)tiles;
+  // a power of two of splits, while every CTA of every cluster still has an SM and two blocks of k
+  p.splits = 1;
+  while (p.splits < kMaxSplits && p.tiles * p.splits * 2 <= sms && p.kblocks >= p.splits * 4) p.splits *= 2;
+  CUtensorMap map;
+  const int st = int8 ? make_matrix_tensor_map_s8(&map, a.x, a.tokens, a.k, a.x_row, tn)
+                      : make_matrix_tensor_map(&map, a.x, a.tokens, a.k, a.x_row, tn);
+  if (st != LKV_OK) return st;
+  if (int8)
+    return a.group == 32   ? by_tokens<true, 32>(tn, map, p, sms, stream)
+           : a.group == 64 ? by_tokens<true, 64>(tn, map, p, sms, stream)
+                           : by_tokens<true, 128>(tn, map, p, sms, stream);
+  return a.group == 32   ? by_tokens<false, 32>(tn, map, p, sms, stream)
+         : a.group == 64 ? by_tokens<false, 64>(tn, map, p, sms, stream)
+                         : by_tokens<false, 128>(tn, map, p, sms, stream);
+}
+
+}  // namespace lkv
