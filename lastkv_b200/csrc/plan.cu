@@ -184,7 +184,7 @@ int plan_step(const PlanArgs& a, cudaStream_t stream) {
     return LKV_ERR_INVALID_ARGUMENT;
   const int pages = (int)(((int64_t)a.max_sequence_tokens + LKV_PAGE_SIZE - 1) / LKV_PAGE_SIZE);
   // a row uses ceil((last + 1) / 16) columns: older pages and ring pages together
-  if (a.src_table_stride < pages || a.width < pages) return LKV_ERR_INVALID_ARGUMENT;
+  if ((a.num_slots > 1 && a.src_table_stride < pages) || a.width < pages) return LKV_ERR_INVALID_ARGUMENT;
   if (a.batch == 0) return LKV_OK;
   if (!a.num_computed || !a.num_new || !a.slots || !a.src_table || !a.ring_base || !a.block_tables || !a.seq_k ||
       !a.cu_q || !a.positions || !a.ring_slots || !a.src_slots || !a.commit_raw || !a.commit_ring ||

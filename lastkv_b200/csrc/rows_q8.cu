@@ -197,12 +197,14 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-bool rows_ok(const void* p, int64_t row, int64_t cols, int elem, int align) {
-  return p && (reinterpret_cast<uintptr_t>(p) % align) == 0 && row >= cols && (row * elem) % align == 0;
+// `count` rows at p, `row` elements apart (a single row has no distance to speak of)
+bool rows_ok(const void* p, int64_t count, int64_t row, int64_t cols, int elem, int align) {
+  return p && (reinterpret_cast<uintptr_t>(p) % align) == 0 &&
+         (count == 1 || (row >= cols && (row * elem) % align == 0));
 }
 
 bool q8_ok(const Q8RowsArgs& a) {
-  return rows_ok(a.q, a.q_row, a.cols, 1, 8) && rows_ok(a.scale, a.scale_row, (a.cols + a.group - 1) / a.group, 4, 4);
+  return rows_ok(a.q, a.rows, a.q_row, a.cols, 1, 8) && rows_ok(a.scale, a.rows, a.scale_row, (a.cols + a.group - 1) / a.group, 4, 4);
 }
 
 int q8_shape(const Q8RowsArgs& a) {
@@ -222,10 +224,10 @@ int rmsnorm_q8(const void* x, int64_t x_row, const void* residual, int64_t resid
   if (st != LKV_OK) return st;
   if (a.cols > 512 * 8 * kVec) return LKV_ERR_UNSUPPORTED;
   if (a.rows == 0) return LKV_OK;
-  if (!rows_ok(x, x_row, a.cols, 2, 16) || !rows_ok(weight, a.cols, a.cols, 2, 16) || !q8_ok(a))
+  if (!rows_ok(x, a.rows, x_row, a.cols, 2, 16) || !rows_ok(weight, 1, a.cols, a.cols, 2, 16) || !q8_ok(a))
     return LKV_ERR_INVALID_ARGUMENT;
-  if (residual && (!rows_ok(residual, residual_row, a.cols, 2, 16) ||
-                   !rows_ok(residual_out, residual_out_row, a.cols, 2, 16)))
+  if (residual && (!rows_ok(residual, a.rows, residual_row, a.cols, 2, 16) ||
+                   !rows_ok(residual_out, a.rows, residual_out_row, a.cols, 2, 16)))
     return LKV_ERR_INVALID_ARGUMENT;
   NormQ8Params p{static_cast<const __nv_bfloat16*>(x),
                  x_row,
@@ -255,7 +257,7 @@ int rows_q8(const void* x, int64_t x_row, int silu, const Q8RowsArgs& a, cudaStr
   const int st = q8_shape(a);
   if (st != LKV_OK) return st;
   if (a.rows == 0) return LKV_OK;
-  if (!rows_ok(x, x_row, silu ? 2 * (int64_t)a.cols : a.cols, 2, 16) || !q8_ok(a)) return LKV_ERR_INVALID_ARGUMENT;
+  if (!rows_ok(x, a.rows, x_row, silu ? 2 * (int64_t)a.cols : a.cols, 2, 16) || !q8_ok(a)) return LKV_ERR_INVALID_ARGUMENT;
   const int blocks = row_blocks(a.rows * ((a.cols + 255) / 256));
   return launch_pdl(silu ? rows_q8_kernel<true> : rows_q8_kernel<false>, dim3(blocks), dim3(256), 0, stream,
                     static_cast<const __nv_bfloat16*>(x), x_row, a.q, a.q_row, a.scale, a.scale_row, a.rows, a.cols,
@@ -268,7 +270,7 @@ int dequantize_q8(const Q8RowsArgs& a, void* out, int64_t out_row, cudaStream_t 
   const int st = q8_shape(a);
   if (st != LKV_OK) return st;
   if (a.rows == 0) return LKV_OK;
-  if (!q8_ok(a) || !rows_ok(out, out_row, a.cols, 2, 16)) return LKV_ERR_INVALID_ARGUMENT;
+  if (!q8_ok(a) || !rows_ok(out, a.rows, out_row, a.cols, 2, 16)) return LKV_ERR_INVALID_ARGUMENT;
   const int blocks = row_blocks((a.rows * (a.cols / kVec) + 31) / 32);
   return launch_pdl(dequantize_q8_kernel, dim3(blocks), dim3(256), 0, stream, static_cast<const int8_t*>(a.q),
                     a.q_row, static_cast<const float*>(a.scale), a.scale_row, static_cast<__nv_bfloat16*>(out),

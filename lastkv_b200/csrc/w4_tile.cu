@@ -33,6 +33,7 @@ namespace lkv {
 namespace {
 
 constexpr int kM = 128;
+constexpr int kQuarters = kM / kTileRows;  // packed row blocks of a tile
 constexpr int kDrainWgs = 2;
 constexpr int kThreads = 256 + 128 * kDrainWgs;
 constexpr int kKernelId = 13;
@@ -69,7 +70,7 @@ __host__ __device__ constexpr int code_slots() {
 
 template <int TN>
 __host__ __device__ constexpr int ring_bytes() {
-  return a_stages<TN>() * kAStage + b_stages<TN>() * TN * 128 + code_slots<TN>() * 2 * kCodeBytes;
+  return a_stages<TN>() * kAStage + b_stages<TN>() * TN * 128 + code_slots<TN>() * kQuarters * kCodeBytes;
 }
 
 constexpr int kWsSlots = 4;
@@ -86,7 +87,7 @@ struct Shared {
   uint64_t ws_full[kWsSlots], ws_empty[kWsSlots];
   uint64_t xs_full[2], xs_empty[2];
   uint32_t tmem;
-  alignas(16) uint8_t ws[kWsSlots][2][kTileRows * 2 * (kTileK / G)];  // the weight's scales of a 128-column block
+  alignas(16) uint8_t ws[kWsSlots][kQuarters][kTileRows * 2 * (kTileK / G)];  // the weight's scales of a 128-column block
   alignas(16) float xs[INT8 ? 2 : 1][kXsGroups][INT8 ? TN : 4];      // the tokens' scales of eight groups
 };
 
@@ -135,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   using Sh = Shared<INT8, G, TN>;
   uint8_t* b_ring = smem + SA * kAStage;
-  uint8_t* codes = b_ring + SB * kBStage;  // [C][2][kCodeBytes]
+  uint8_t* codes = b_ring + SB * kBStage;  // [C][kQuarters][kCodeBytes]
   Sh* sh = reinterpret_cast<Sh*>(smem + ring_bytes<TN>());
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.y;
@@ -191,15 +192,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t it = 0, blk = 0;
         bool ok = true;
         for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
-          const int tok0 = tile % p.tok_tiles * TN, rb = tile / p.tok_tiles * 2;
+          const int tok0 = tile % p.tok_tiles * TN, rb = tile / p.tok_tiles * kQuarters;
           for (int kb = 0; ok && kb < nkb; ++kb, ++blk) {
             const int b = blk % kWsSlots;
             ok = mbar_wait(&sh->ws_empty[b], ((blk / kWsSlots) & 1) ^ 1);
             if (!ok) break;
             constexpr uint32_t kWs = sizeof(sh->ws[0][0]);
-            const int halves = min(2, p.row_blocks - rb);
-            mbar_arrive_expect_tx(&sh->ws_full[b], kWs * halves);
-            for (int h = 0; h < halves; ++h)
+            const int quarters = min(kQuarters, p.row_blocks - rb);
+            mbar_arrive_expect_tx(&sh->ws_full[b], kWs * quarters);
+            for (int h = 0; h < quarters; ++h)
               bulk_load(sh->ws[b][h],
                         p.packed + ((int64_t)(rb + h) * p.kblocks + kb0 + kb) * block_bytes(G) + kCodeBytes, kWs,
                         &sh->ws_full[b]);
@@ -268,15 +269,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t blk = 0;
         bool ok = true;
         for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
-          const int rb = tile / p.tok_tiles * 2, halves = min(2, p.row_blocks - rb);
+          const int rb = tile / p.tok_tiles * kQuarters, quarters = min(kQuarters, p.row_blocks - rb);
           const uint8_t* src = p.packed + ((int64_t)rb * p.kblocks + kb0) * block_bytes(G);
           for (int kb = 0; kb < nkb; ++kb, ++blk, src += block_bytes(G)) {
             const int b = blk % C;
             ok = mbar_wait(&sh->c_empty[b], ((blk / C) & 1) ^ 1);
             if (!ok) break;
-            mbar_arrive_expect_tx(&sh->c_full[b], kCodeBytes * halves);
-            for (int h = 0; h < halves; ++h)
-              bulk_load(codes + (b * 2 + h) * kCodeBytes, src + (int64_t)h * p.kblocks * block_bytes(G), kCodeBytes,
+            mbar_arrive_expect_tx(&sh->c_full[b], kCodeBytes * quarters);
+            for (int h = 0; h < quarters; ++h)
+              bulk_load(codes + (b * kQuarters + h) * kCodeBytes, src + (int64_t)h * p.kblocks * block_bytes(G), kCodeBytes,
                         &sh->c_full[b]);
           }
         }
@@ -332,20 +333,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t it = 0, blk = 0;
     bool ok = true;
     for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
-      const int halves = min(2, p.row_blocks - tile / p.tok_tiles * 2);
+      const int quarters = min(kQuarters, p.row_blocks - tile / p.tok_tiles * kQuarters);
       for (int kb = 0; ok && kb < nkb; ++kb, ++blk) {
         const int b = blk % C;
         ok = __all_sync(0xffffffffu, mbar_wait(&sh->c_full[b], (blk / C) & 1));
         if (!ok) break;
-        const uint8_t* src = codes + b * 2 * kCodeBytes + (4 * g + t) * 16;
+        const uint8_t* src = codes + b * kQuarters * kCodeBytes + (4 * g + t) * 16;
 #pragma unroll
         for (int i = 0; i < kSpb; ++i, ++it) {
           uint4 v[kN];
 #pragma unroll
           for (int q = 0; q < kN; ++q) {
-            const int c = w * kN + q;  // int8: (half, r, j); bf16: (half, r), j from the stage
-            const int hb = INT8 ? c >> 3 : c >> 2, r = INT8 ? (c >> 1) & 3 : c & 3, j = INT8 ? c & 1 : i;
-            v[q] = hb < halves ? *reinterpret_cast<const uint4*>(src + hb * kCodeBytes + r * 1024 + j * 512)
+            // warp w expands row block w: int8 pieces (r, j), bf16 pieces r, j from the stage
+            const int r = INT8 ? q >> 1 : q, j = INT8 ? q & 1 : i;
+            v[q] = w < quarters ? *reinterpret_cast<const uint4*>(src + w * kCodeBytes + r * 1024 + j * 512)
                                : make_uint4(0, 0, 0, 0);
           }
           if (i == kSpb - 1) {
@@ -358,12 +359,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t a = smem_u32(smem + s * kAStage);
 #pragma unroll
           for (int q = 0; q < kN; ++q) {
-            const int c = w * kN + q;
-            const int hb = INT8 ? c >> 3 : c >> 2, r = INT8 ? (c >> 1) & 3 : c & 3, j = INT8 ? c & 1 : 0;
+            const int r = INT8 ? q >> 1 : q, j = INT8 ? q & 1 : 0;
             const uint32_t words[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const uint32_t row = a + (hb * 64 + 16 * r + 8 * (e & 1) + g) * 128;
+              const uint32_t row = a + (w * kTileRows + 16 * r + 8 * (e & 1) + g) * 128;
               const uint32_t u = words[e];
               if (INT8) {
                 const int chunk = 2 * (2 * j + (e >> 1)) + (t >> 1);
@@ -389,15 +389,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     regs_inc<192>();
     const int wg = (warp - 8) >> 2, tid = threadIdx.x & 127, sub = warp & 3;
     const uint32_t lanes = (uint32_t)(sub * 32) << 16;
-    // scale of row 16 r + 8 h + g of a 64-row block at 2 (8 g + 2 r + h)
-    const int ws_off = 2 * (8 * (tid & 7) + 2 * ((tid >> 4) & 3) + ((tid >> 3) & 1));
+    // scale of row 16 r + 8 h + g of a row block at 2 (4 g + 2 r + h)
+    const int ws_off = 2 * (4 * (tid & 7) + 2 * ((tid >> 4) & 1) + ((tid >> 3) & 1));
     pdl_wait();  // before any global write
     uint32_t grp = 0, blk = 0, slot = 0;
     bool ok = true;
     for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
       const int tok0 = tile % p.tok_tiles * TN + wg * kCols;
       const int row = (tile / p.tok_tiles) * kM + tid;
-      const bool live_row = tile / p.tok_tiles * 2 + (tid >> 6) < p.row_blocks;
+      const bool live_row = tile / p.tok_tiles * kQuarters + (tid >> 5) < p.row_blocks;
       float2 acc[kCols / 2];
 #pragma unroll
       for (int c = 0; c < kCols / 2; ++c) acc[c] = make_float2(0.f, 0.f);
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int gi = 0; gi < kGpb; ++gi, ++gt) {
           const int buf = grp & 1;
           float w1 = live_row ? __uint_as_float((uint32_t)*reinterpret_cast<const unsigned short*>(
-                                                    &sh->ws[b][tid >> 6][gi * 128 + ws_off])
+                                                    &sh->ws[b][tid >> 5][gi * 64 + ws_off])
                                                 << 16)
                               : 0.f;
           if (INT8) w1 *= 0.0625f;  // int8 codes stand at 16 c

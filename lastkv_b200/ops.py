@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import os
 from typing import NamedTuple, Optional
 
@@ -32,7 +33,8 @@ def _ptr(t):
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    # the current stream's handle, without building a torch.cuda.Stream object for it
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _require(cond: bool, msg: str) -> None:
@@ -589,63 +591,76 @@ def decode_gemm(x, weight, *, silu_mul: bool = False, out=None, error_word=None)
 
 
 # ------------------------------------------------------------------ int8 rows, 4-bit weights
+#
+# At decode sizes these calls cost the host more than the GPU, so the checks of a call are a
+# few comparisons and its messages are built only when one fails.
 
 Q8_GROUPS = (32, 64, 128)
+_BF16, _I8, _F32 = torch.bfloat16, torch.int8, torch.float32
 
 
 class Q8Rows(NamedTuple):
     """int8 rows with fp32 group scales: ``q`` [rows, K] stands for ``q * scale`` per group of
-    ``group`` columns; ``scale`` [rows, ceil(K / group)].  ``shape`` is the activations' shape."""
+    ``group`` columns; ``scale`` [rows, ceil(K / group)]."""
 
     q: torch.Tensor
     scale: torch.Tensor
     group: int
-    lead: Optional[tuple] = None  # leading dimensions of the rows they came from (None: q's)
+    lead: Optional[tuple] = None  # leading dimensions of the activations (None: [rows])
 
     @classmethod
-    def empty(cls, lead: tuple, cols: int, group: int, device) -> "Q8Rows":
-        rows = 1
-        for n in lead:
-            rows *= n
-        pitch = -(-cols // 16) * 16  # 16-byte rows, whatever the width
-        q = torch.empty((rows, pitch), dtype=torch.int8, device=device)
-        return cls(q if pitch == cols else q[:, :cols],
-                   torch.empty((rows, -(-cols // group)), dtype=torch.float32, device=device), group, tuple(lead))
+    def empty_for(cls, x, cols: int, group: int) -> "Q8Rows":
+        """Rows of ``cols`` columns for the leading dimensions and the device of ``x``."""
+        lead = tuple(x.shape[:-1])
+        rows = lead[0] if len(lead) == 1 else math.prod(lead)
+        pitch = (cols + 15) & -16  # 16-byte rows, whatever the width
+        q = x.new_empty((rows, pitch), dtype=_I8)
+        return cls(q if pitch == cols else q[:, :cols], x.new_empty((rows, -(-cols // group)), dtype=_F32), group, lead)
 
 
-def _check_group(group) -> None:
-    _require(group in Q8_GROUPS, f"group must be one of {Q8_GROUPS}, got {group!r}")
+def _fail(msg: str):
+    raise RMarinBackendContractError(msg)
 
 
-def _check_q8(r: Q8Rows, what: str) -> None:
-    _check_group(r.group)
-    _require(r.q.is_cuda and r.q.dtype == torch.int8 and r.q.dim() == 2 and r.q.stride(1) == 1,
-             f"{what}.q must be CUDA int8 [rows, K] rows")
-    _require(r.scale.is_cuda and r.scale.dtype == torch.float32 and r.scale.dim() == 2 and r.scale.stride(1) == 1
-             and r.scale.shape == (r.q.shape[0], -(-r.q.shape[1] // r.group)),
-             f"{what}.scale must be CUDA fp32 [rows, ceil(K / group)] rows")
-
-
-def _q8_out(out, x, cols: int, group: int) -> Q8Rows:
-    _check_group(group)
-    if out is None:
-        return Q8Rows.empty(tuple(x.shape[:-1]), cols, group, x.device)
-    _check_q8(out, "out")
-    _require(out.group == group and out.q.shape == (x.numel() // max(x.shape[-1], 1), cols), "out layout")
-    return out
+def _in2d(t, name: str):
+    """CUDA bf16 rows with unit column stride, as a 2-D view (or copy) of [..., cols]."""
+    if t.dtype != _BF16 or not t.is_cuda or t.dim() < 1 or t.stride(-1) != 1:
+        _fail(f"{name} must be CUDA bf16 with unit stride")
+    return t if t.dim() == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
 
 
 def _out2d(t, cols: int, name: str):
     """An output's rows, written in place: 2-D rows of any stride, or contiguous."""
-    _require(t.is_cuda and t.dtype == torch.bfloat16 and t.dim() >= 1 and t.shape[-1] == cols
-             and ((t.dim() == 2 and t.stride(1) == 1) or t.is_contiguous()),
-             f"{name} must be CUDA bf16 [..., {cols}], contiguous or 2-D rows")
-    return t if t.dim() == 2 else t.view(-1, cols)
+    if t.dtype != _BF16 or not t.is_cuda or t.dim() < 1 or t.shape[-1] != cols \
+            or not (t.is_contiguous() or (t.dim() == 2 and t.stride(1) == 1)):
+        _fail(f"{name} must be CUDA bf16 [..., {cols}], contiguous or 2-D rows")
+    return t if t.dim() == 2 else t.view(math.prod(t.shape[:-1]), cols)
 
 
-def _row_stride(t) -> int:
-    """Row stride of a 2-D tensor as the kernels take it (one row has no stride to speak of)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+def _check_group(group) -> None:
+    if group not in Q8_GROUPS:
+        _fail(f"group must be one of {Q8_GROUPS}, got {group!r}")
+
+
+def _check_q8(r: Q8Rows, what: str) -> None:
+    q, scale = r.q, r.scale
+    _check_group(r.group)
+    if q.dtype != _I8 or not q.is_cuda or q.dim() != 2 or q.stride(1) != 1:
+        _fail(f"{what}.q must be CUDA int8 [rows, K] rows")
+    rows, cols = q.shape
+    if scale.dtype != _F32 or not scale.is_cuda or scale.dim() != 2 or scale.stride(1) != 1 \
+            or scale.shape != (rows, -(-cols // r.group)):
+        _fail(f"{what}.scale must be CUDA fp32 [rows, ceil(K / group)] rows")
+
+
+def _q8_out(out, x, rows: int, cols: int, group: int) -> Q8Rows:
+    if out is None:
+        _check_group(group)
+        return Q8Rows.empty_for(x, cols, group)
+    _check_q8(out, "out")
+    if out.group != group or out.q.shape != (rows, cols):
+        _fail(f"out must be Q8Rows [{rows}, {cols}] of groups of {group}")
+    return out
 
 
 @_traced
@@ -657,49 +672,60 @@ def rmsnorm_q8(x, weight, eps: float, residual=None, *, group: int = 128, out: O
     returns ``(h, rows)``, h rounded to bf16 (``residual_out`` may be ``residual`` itself);
     otherwise ``rows`` (:class:`Q8Rows`).
     """
-    x2 = _rows2d(x, "x")
-    H = x2.shape[1]
-    _require(weight.is_cuda and weight.dtype == torch.bfloat16 and weight.is_contiguous() and weight.numel() == H,
-             "weight must be CUDA bf16 [H]")
-    rows = _q8_out(out, x, H, group)
-    r2 = ro2 = None
-    if residual is not None:
-        r2 = _rows2d(residual, "residual")
-        _require(r2.shape == x2.shape, "residual must match x")
-        if residual_out is None:
-            residual_out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
-        ro2 = _out2d(residual_out, H, "residual_out")
-        _require(ro2.shape == x2.shape, "residual_out must match x")
-    st = _capi.lib().lkv_rmsnorm_q8(
-        x2.data_ptr(), _row_stride(x2), _ptr(r2), _row_stride(r2) if r2 is not None else 0, _ptr(ro2),
-        _row_stride(ro2) if ro2 is not None else 0, weight.data_ptr(), float(eps), rows.q.data_ptr(),
-        _row_stride(rows.q), rows.scale.data_ptr(), _row_stride(rows.scale), x2.shape[0], H, group, _stream())
-    _capi.check(st, "lkv_rmsnorm_q8")
-    return rows if residual is None else (residual_out, rows)
+    x2 = _in2d(x, "x")
+    T, H = x2.shape
+    if weight.dtype != _BF16 or not weight.is_cuda or weight.numel() != H or not weight.is_contiguous():
+        _fail("weight must be CUDA bf16 [H]")
+    rows = _q8_out(out, x, T, H, group)
+    q, scale = rows.q, rows.scale
+    if residual is None:
+        st = _capi.lib().lkv_rmsnorm_q8(x2.data_ptr(), x2.stride(0), None, 0, None, 0, weight.data_ptr(), eps,
+                                        q.data_ptr(), q.stride(0), scale.data_ptr(), scale.stride(0), T, H, group,
+                                        _stream())
+        if st:
+            _capi.check(st, "lkv_rmsnorm_q8")
+        return rows
+    r2 = _in2d(residual, "residual")
+    if residual_out is None:
+        residual_out = x.new_empty(x.shape)
+    ro2 = _out2d(residual_out, H, "residual_out")
+    if r2.shape != x2.shape or ro2.shape != x2.shape:
+        _fail("residual and residual_out must match x")
+    st = _capi.lib().lkv_rmsnorm_q8(x2.data_ptr(), x2.stride(0), r2.data_ptr(), r2.stride(0), ro2.data_ptr(),
+                                    ro2.stride(0), weight.data_ptr(), eps, q.data_ptr(), q.stride(0),
+                                    scale.data_ptr(), scale.stride(0), T, H, group, _stream())
+    if st:
+        _capi.check(st, "lkv_rmsnorm_q8")
+    return residual_out, rows
 
 
 @_traced
 def silu_mul_q8(gate_up, *, group: int = 128, out: Optional[Q8Rows] = None) -> Q8Rows:
     """``silu(gate) * up`` for bf16 [..., 2F] rows of [gate | up], as int8 rows (lkv_silu_mul_q8)."""
-    x2 = _rows2d(gate_up, "gate_up")
-    _require(x2.shape[1] % 2 == 0, "gate_up must be [..., 2F]")
-    rows = _q8_out(out, gate_up, x2.shape[1] // 2, group)
-    st = _capi.lib().lkv_silu_mul_q8(x2.data_ptr(), _row_stride(x2), rows.q.data_ptr(), _row_stride(rows.q),
-                                     rows.scale.data_ptr(), _row_stride(rows.scale), x2.shape[0], x2.shape[1] // 2,
-                                     group, _stream())
-    _capi.check(st, "lkv_silu_mul_q8")
+    x2 = _in2d(gate_up, "gate_up")
+    T, F2 = x2.shape
+    if F2 % 2:
+        _fail("gate_up must be [..., 2F]")
+    rows = _q8_out(out, gate_up, T, F2 // 2, group)
+    q, scale = rows.q, rows.scale
+    st = _capi.lib().lkv_silu_mul_q8(x2.data_ptr(), x2.stride(0), q.data_ptr(), q.stride(0), scale.data_ptr(),
+                                     scale.stride(0), T, F2 // 2, group, _stream())
+    if st:
+        _capi.check(st, "lkv_silu_mul_q8")
     return rows
 
 
 @_traced
 def quantize_q8(x, *, group: int = 128, out: Optional[Q8Rows] = None) -> Q8Rows:
     """bf16 [..., K] rows as int8 rows with group scales (lkv_quantize_q8)."""
-    x2 = _rows2d(x, "x")
-    rows = _q8_out(out, x, x2.shape[1], group)
-    st = _capi.lib().lkv_quantize_q8(x2.data_ptr(), _row_stride(x2), rows.q.data_ptr(), _row_stride(rows.q),
-                                     rows.scale.data_ptr(), _row_stride(rows.scale), x2.shape[0], x2.shape[1], group,
-                                     _stream())
-    _capi.check(st, "lkv_quantize_q8")
+    x2 = _in2d(x, "x")
+    T, K = x2.shape
+    rows = _q8_out(out, x, T, K, group)
+    q, scale = rows.q, rows.scale
+    st = _capi.lib().lkv_quantize_q8(x2.data_ptr(), x2.stride(0), q.data_ptr(), q.stride(0), scale.data_ptr(),
+                                     scale.stride(0), T, K, group, _stream())
+    if st:
+        _capi.check(st, "lkv_quantize_q8")
     return rows
 
 
@@ -707,16 +733,17 @@ def quantize_q8(x, *, group: int = 128, out: Optional[Q8Rows] = None) -> Q8Rows:
 def dequantize_q8(rows: Q8Rows, out=None):
     """The bf16 values [..., K] that int8 rows stand for (lkv_dequantize_q8)."""
     _check_q8(rows, "rows")
-    T, K = rows.q.shape
-    shape = (*(rows.lead if rows.lead is not None else (T,)), K)
+    q, scale = rows.q, rows.scale
+    T, K = q.shape
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=rows.q.device)
+        out = q.new_empty((T, K) if rows.lead is None else (*rows.lead, K), dtype=_BF16)
     o2 = _out2d(out, K, "out")
-    _require(o2.shape[0] == T, "out must have the rows' count")
-    st = _capi.lib().lkv_dequantize_q8(rows.q.data_ptr(), _row_stride(rows.q), rows.scale.data_ptr(),
-                                       _row_stride(rows.scale), o2.data_ptr(), _row_stride(o2), T, K, rows.group,
-                                       _stream())
-    _capi.check(st, "lkv_dequantize_q8")
+    if o2.shape[0] != T:
+        _fail("out must have the rows' count")
+    st = _capi.lib().lkv_dequantize_q8(q.data_ptr(), q.stride(0), scale.data_ptr(), scale.stride(0), o2.data_ptr(),
+                                       o2.stride(0), T, K, rows.group, _stream())
+    if st:
+        _capi.check(st, "lkv_dequantize_q8")
     return out
 
 
@@ -737,16 +764,18 @@ def w4_pack(codes, scales, group: int = 128) -> W4Weight:
     2i + 1 in the high half; scales bf16 [n, ceil(k / group)].
     """
     _check_group(group)
-    _require(codes.is_cuda and codes.dtype == torch.uint8 and codes.dim() == 2 and codes.stride(1) == 1,
-             "codes must be CUDA uint8 [n, k / 2]")
+    if not (codes.is_cuda and codes.dtype == torch.uint8 and codes.dim() == 2 and codes.stride(1) == 1):
+        _fail("codes must be CUDA uint8 [n, k / 2]")
     n, k = codes.shape[0], 2 * codes.shape[1]
-    _require(scales.is_cuda and scales.dtype == torch.bfloat16 and scales.dim() == 2 and scales.stride(1) == 1
-             and scales.shape == (n, -(-k // group)), "scales must be CUDA bf16 [n, ceil(k / group)]")
+    if not (scales.is_cuda and scales.dtype == _BF16 and scales.dim() == 2 and scales.stride(1) == 1
+            and scales.shape == (n, -(-k // group))):
+        _fail("scales must be CUDA bf16 [n, ceil(k / group)]")
     nbytes = _capi.lib().lkv_w4_bytes(n, k, group)
-    _require(nbytes > 0, f"4-bit weights need n >= 1 and k a positive multiple of 8, got [{n}, {k}]")
+    if nbytes == 0:
+        _fail(f"4-bit weights need n >= 1 and k a positive multiple of 8, got [{n}, {k}]")
     packed = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
-    st = _capi.lib().lkv_w4_pack(codes.data_ptr(), _row_stride(codes), scales.data_ptr(), _row_stride(scales), n, k,
-                                 group, packed.data_ptr(), _stream())
+    st = _capi.lib().lkv_w4_pack(codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0), n, k, group,
+                                 packed.data_ptr(), _stream())
     _capi.check(st, "lkv_w4_pack")
     return W4Weight(packed, n, k, group)
 
@@ -769,32 +798,37 @@ def w4_quantize(weight, group: int = 128) -> W4Weight:
 def w4_linear(x, weight: W4Weight, bias=None, *, out=None, error_word=None):
     """``x @ w.T (+ bias)`` for a 4-bit weight: x bf16 [..., k] or :class:`Q8Rows` of the
     weight's group; bf16 out [..., n], any number of rows (lkv_w4_linear, lkv_w4_linear_q8)."""
-    n, k = weight.n, weight.k
-    q8 = isinstance(x, Q8Rows)
+    packed, n, k, group = weight
+    q8 = type(x) is Q8Rows
     if q8:
         _check_q8(x, "x")
-        _require(x.group == weight.group, f"rows of groups of {x.group} against a weight of groups of {weight.group}")
-        x2, lead = x.q, x.lead if x.lead is not None else (x.q.shape[0],)
+        if x.group != group:
+            _fail(f"rows of groups of {x.group} against a weight of groups of {group}")
+        x2 = x.q
+        lead = x.lead
     else:
-        x2, lead = _rows2d(x, "x"), tuple(x.shape[:-1])
-    _require(x2.shape[1] == k, f"x has {x2.shape[1]} columns, the weight {k}")
+        x2 = _in2d(x, "x")
+        lead = None if x2 is x else x.shape[:-1]
+    T, cols = x2.shape
+    if cols != k:
+        _fail(f"x has {cols} columns, the weight {k}")
     if out is None:
-        out = torch.empty((*lead, n), dtype=torch.bfloat16, device=x2.device)
+        out = x2.new_empty((T, n) if lead is None else (*lead, n), dtype=_BF16)
     o2 = _out2d(out, n, "out")
-    _require(o2.shape[0] == x2.shape[0], "out must have the rows of x")
-    if bias is not None:
-        _require(bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == n and bias.is_cuda,
-                 "bias must be bf16 [n]")
-    T = x2.shape[0]
+    if o2.shape[0] != T:
+        _fail("out must have the rows of x")
+    if bias is not None and not (bias.dtype == _BF16 and bias.is_contiguous() and bias.numel() == n and bias.is_cuda):
+        _fail("bias must be CUDA bf16 [n]")
     if q8:
-        st = _capi.lib().lkv_w4_linear_q8(x2.data_ptr(), _row_stride(x2), x.scale.data_ptr(), _row_stride(x.scale),
-                                          weight.packed.data_ptr(), _ptr(bias), o2.data_ptr(), _row_stride(o2), T, n,
-                                          k, weight.group, _ptr(error_word), _stream())
+        scale = x.scale
+        st = _capi.lib().lkv_w4_linear_q8(x2.data_ptr(), x2.stride(0), scale.data_ptr(), scale.stride(0),
+                                          packed.data_ptr(), _ptr(bias), o2.data_ptr(), o2.stride(0), T, n, k, group,
+                                          _ptr(error_word), _stream())
     else:
-        st = _capi.lib().lkv_w4_linear(x2.data_ptr(), _row_stride(x2), weight.packed.data_ptr(), _ptr(bias),
-                                       o2.data_ptr(), _row_stride(o2), T, n, k, weight.group, _ptr(error_word),
-                                       _stream())
-    _capi.check(st, "lkv_w4_linear_q8" if q8 else "lkv_w4_linear")
+        st = _capi.lib().lkv_w4_linear(x2.data_ptr(), x2.stride(0), packed.data_ptr(), _ptr(bias), o2.data_ptr(),
+                                       o2.stride(0), T, n, k, group, _ptr(error_word), _stream())
+    if st:
+        _capi.check(st, "lkv_w4_linear_q8" if q8 else "lkv_w4_linear")
     return out
 
 
@@ -843,7 +877,7 @@ class StepPlan:
         self.commit_raw, self.commit_ring, self.commit_count = i32(batch, ppc), i32(batch, ppc), i32(1)
         self.error_word = error_word if error_word is not None else i32(4)
         # everything after the lengths is the same in every call
-        self._rest = (self.batch, src_table.data_ptr(), _row_stride(src_table), src_table.shape[0],
+        self._rest = (self.batch, src_table.data_ptr(), src_table.stride(0), src_table.shape[0],
                       self.max_sequence_tokens, chunk_size, ring_base.data_ptr(), ring_base.numel(),
                       int(scratch_src_page), int(scratch_ring_page), self.width, self.max_tokens,
                       *(t.data_ptr() for t in (self.block_tables, self.seq_k, self.cu_q, self.positions,
@@ -851,12 +885,13 @@ class StepPlan:
                                                self.commit_count, self.error_word)))
 
     def run(self, num_computed, num_new, slots) -> "StepPlan":
-        for name, t in (("num_computed", num_computed), ("num_new", num_new), ("slots", slots)):
-            _require(t.is_cuda and t.dtype == torch.int32 and t.is_contiguous() and t.numel() == self.batch,
-                     f"{name} must be CUDA int32 [{self.batch}]")
+        for t in (num_computed, num_new, slots):
+            if t.dtype != torch.int32 or not t.is_cuda or t.numel() != self.batch or not t.is_contiguous():
+                _fail(f"num_computed, num_new and slots must be CUDA int32 [{self.batch}]")
         st = _capi.lib().lkv_plan_step(num_computed.data_ptr(), num_new.data_ptr(), slots.data_ptr(), *self._rest,
                                        _stream())
-        _capi.check(st, "lkv_plan_step")
+        if st:
+            _capi.check(st, "lkv_plan_step")
         return self
 
     def check_errors(self) -> None:

@@ -145,7 +145,7 @@ def test_refusals():
                  lambda: ops.quantize_q8(x[:, :12]),             # not a multiple of 8
                  lambda: ops.quantize_q8(x[:, 1:33]),            # rows off the 16-byte grid
                  lambda: ops.quantize_q8(x.t()),
-                 lambda: ops.quantize_q8(x, out=ops.Q8Rows.empty((3,), 64, 128, "cuda")),
+                 lambda: ops.quantize_q8(x, out=ops.Q8Rows.empty_for(x[:3], 64, 128)),
                  lambda: ops.silu_mul_q8(x[:, :24]),             # 12 columns
                  lambda: ops.rmsnorm_q8(x, w[:32], 1e-6),
                  lambda: ops.rmsnorm_q8(x, w.float(), 1e-6),
