@@ -24,10 +24,11 @@ namespace {
 
 __global__ void __launch_bounds__(256)
     w4_pack_kernel(const uint8_t* __restrict__ codes, int64_t codes_row, const __nv_bfloat16* __restrict__ scales,
-                   int64_t scales_row, int64_t n, int64_t k, int group, int64_t kblocks, uint8_t* __restrict__ packed) {
-  const int64_t block = blockIdx.x;  // (row tile, k block)
-  const int64_t row0 = block / kblocks * kTileRows, k0 = block % kblocks * kTileK;
-  uint8_t* dst = packed + block * block_bytes(group);
+                   int64_t scales_row, int64_t n, int64_t k, int group, int kblocks, int row_blocks,
+                   uint8_t* __restrict__ packed) {
+  const int64_t rb = blockIdx.x / kblocks, kb = blockIdx.x % kblocks;
+  const int64_t row0 = rb * kTileRows, k0 = kb * kTileK;
+  uint8_t* dst = packed + block_offset(rb, kb, kblocks, row_blocks, group);
   for (int w = threadIdx.x; w < kCodeBytes / 4; w += blockDim.x) {
     const int i = w & 3, lane = (w >> 2) & 31, j = (w >> 7) & 1, r = w >> 8;
     const int64_t row = row0 + 16 * r + (lane >> 2) + 8 * (i & 1);
@@ -52,6 +53,11 @@ __global__ void __launch_bounds__(256)
     reinterpret_cast<__nv_bfloat16*>(dst + kCodeBytes)[i] = in ? scales[row * scales_row + g] : __float2bfloat16(0.f);
   }
 }
+
+// Launched after w4_pack_kernel: the products read their weights before their launch's
+// dependency wait (PDL), which a plain kernel in between makes safe - it starts once the
+// packing has completed and its writes are visible, and the product's launch after it.
+__global__ void w4_packed_kernel() {}
 
 // ---------------------------------------------------------------- few tokens
 
@@ -217,7 +223,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) w4_skinny_kernel(const SkinnyP
     if (lt >= p.tiles) return;
     if (lane == 0) {
       mbar_arrive_expect_tx(&sh->full[warp][slot], block_bytes(G));
-      bulk_load_hint(sh->ring[warp][slot], p.packed + ((int64_t)lt * p.kblocks + lk) * block_bytes(G), block_bytes(G),
+      bulk_load_hint(sh->ring[warp][slot], p.packed + block_offset(lt, lk, p.kblocks, p.tiles, G), block_bytes(G),
                      &sh->full[warp][slot], policy_evict_first());
     }
     if (++lk == k1) {
@@ -416,8 +422,9 @@ int w4_pack(const uint8_t* codes, int64_t codes_row, const void* scales, int64_t
   const int64_t kblocks = (k + kTileK - 1) / kTileK, blocks = (n + kTileRows - 1) / kTileRows * kblocks;
   if (blocks > 0x7fffffff) return LKV_ERR_UNSUPPORTED;
   w4_pack_kernel<<<(unsigned)blocks, 256, 0, stream>>>(codes, codes_row, static_cast<const __nv_bfloat16*>(scales),
-                                                       scales_row, n, k, group, kblocks,
+                                                       scales_row, n, k, group, (int)kblocks, (int)(blocks / kblocks),
                                                        static_cast<uint8_t*>(packed));
+  w4_packed_kernel<<<1, 1, 0, stream>>>();
   return cudaGetLastError() == cudaSuccess ? LKV_OK : LKV_ERR_CUDA;
 }
 

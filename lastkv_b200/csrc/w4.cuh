@@ -1,7 +1,8 @@
 // The packed 4-bit weight and its codes, shared by the kernels that read it (w4.cu, w4_tile.cu).
 //
-// Packed weight (lkv_w4_pack, laid out once): blocks of 32 output rows x 128 columns, a row
-// block's blocks contiguous along k.  A block is 2 sub-tiles of 16 rows x 128 columns (1 KB
+// Packed weight (lkv_w4_pack, laid out once): blocks of 32 output rows x 128 columns; the
+// four row blocks of 128 rows (the last ones may be fewer) lie side by side, then the next
+// 128 columns, so a tile of 128 rows reads 128 columns with one copy.  A block is 2 sub-tiles of 16 rows x 128 columns (1 KB
 // each, in the order of the mma.sync A fragments) followed by its scales:
 //   word (r, j, lane, i) at r * 1024 + j * 512 + lane * 16 + i * 4 holds
 //     row 16 r + lane / 4 + 8 (i & 1), columns 32 (2 j + i / 2) + 8 (lane & 3) .. + 7,
@@ -22,6 +23,14 @@ constexpr int kTileK = 128;
 constexpr int kCodeBytes = kTileRows * kTileK / 2;
 
 __host__ __device__ constexpr int block_bytes(int group) { return kCodeBytes + kTileRows * 2 * (kTileK / group); }
+
+// First byte of block (rb, kb).
+__host__ __device__ __forceinline__ int64_t block_offset(int64_t rb, int64_t kb, int kblocks, int row_blocks,
+                                                         int group) {
+  const int64_t first = rb & ~int64_t(3);
+  const int64_t wide = row_blocks - first < 4 ? row_blocks - first : 4;
+  return (first * kblocks + kb * wide + (rb - first)) * block_bytes(group);
+}
 
 // Two of a word's codes (I = 0: columns 0, 2; 1: 4, 6; 2: 1, 3; 3: 5, 7) as exact bf16:
 // 128 + (c + 8) by its mantissa bits, minus 136.

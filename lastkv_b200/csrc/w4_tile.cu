@@ -13,8 +13,8 @@
 // 128 x TN sums from TMEM per group.
 //
 // Roles of the 512 threads (one CTA per SM, persistent over the tiles):
-//   warp 0  rows and weight scales by TMA       warp 1     tcgen05.mma issue, TMEM
-//   warp 2  the tokens' scales (int8 rows)      warp 3     codes by bulk copies
+//   warp 0  rows by TMA                         warp 1     tcgen05.mma issue, TMEM
+//   warp 2  the tokens' scales (int8 rows)      warp 3     codes, weight scales by bulk copies
 //   warps 4-7    codes -> A tiles               warps 8-15 drain, epilogue
 // Where the tiles alone do not fill the GPU, k is split over the CTAs of a cluster, whose
 // partial tiles meet in shared memory (added in split order).
@@ -61,20 +61,24 @@ __host__ __device__ constexpr int b_stages() {
   return TN == 256 ? 4 : TN == 128 ? 6 : TN == 64 ? 8 : 12;
 }
 
-// 128-column blocks of codes (8 KB for the tile's 128 rows) in flight
+// 128-column blocks of packed weights (8 KB and the scales for the tile's 128 rows) in flight
 template <int TN>
 __host__ __device__ constexpr int code_slots() {
-  return TN == 256 ? 3 : TN == 128 ? 5 : TN == 64 ? 8 : 10;
+  return TN == 256 ? 3 : TN == 128 ? 4 : TN == 64 ? 8 : 10;
 }
 
 
-template <int TN>
+template <int G, int TN>
 __host__ __device__ constexpr int ring_bytes() {
-  return a_stages<TN>() * kAStage + b_stages<TN>() * TN * 128 + code_slots<TN>() * kQuarters * kCodeBytes;
+  return a_stages<TN>() * kAStage + b_stages<TN>() * TN * 128 + code_slots<TN>() * kQuarters * block_bytes(G);
 }
 
-constexpr int kWsSlots = 4;
-constexpr int kXsGroups = 8;  // one 32-byte sector of a token's scales
+// blocks of weight scales in flight: as many as the codes run ahead of the drain
+template <int G, int TN>
+__host__ __device__ constexpr int scale_slots() {
+  return TN == 256 ? (G == 32 ? 4 : 8) : 16;
+}
+constexpr int kXsGroups = 4;  // groups of the tokens' scales per slot: one 16-byte load
 
 template <bool INT8, int G, int TN>
 struct Shared {
@@ -84,16 +88,16 @@ struct Shared {
   uint64_t d_empty[2];
   uint64_t done;
   uint64_t c_full[code_slots<TN>()], c_empty[code_slots<TN>()];
-  uint64_t ws_full[kWsSlots], ws_empty[kWsSlots];
+  uint64_t ws_full[scale_slots<G, TN>()], ws_empty[scale_slots<G, TN>()];
   uint64_t xs_full[2], xs_empty[2];
   uint32_t tmem;
-  alignas(16) uint8_t ws[kWsSlots][kQuarters][kTileRows * 2 * (kTileK / G)];  // the weight's scales of a 128-column block
-  alignas(16) float xs[INT8 ? 2 : 1][kXsGroups][INT8 ? TN : 4];      // the tokens' scales of eight groups
+  alignas(16) uint8_t ws[scale_slots<G, TN>()][kQuarters][kTileRows * 2 * (kTileK / G)];  // the weight's scales of a 128-column block
+  alignas(16) float xs[INT8 ? 2 : 1][kXsGroups][2][INT8 ? TN : 4];  // x, and -1.5 * 2^23 x, for the tokens' scales x
 };
 
 template <bool INT8, int G, int TN>
 constexpr int smem_bytes() {
-  return 1024 + ring_bytes<TN>() + (int)sizeof(Shared<INT8, G, TN>);
+  return 1024 + ring_bytes<G, TN>() + (int)sizeof(Shared<INT8, G, TN>);
 }
 
 template <int N>
@@ -112,23 +116,15 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t 
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-// Two int32 below 2^22 in magnitude (128 x 127 x 128 < 2^21) to fp32, exactly: 1.5 * 2^23 + v
-// has v in its low mantissa bits.  Two adds on the fp32 pipes; the conversion instruction
-// runs at an eighth of their rate.
-__device__ __forceinline__ float2 int_float2(uint32_t a, uint32_t b) {
-  return __fadd2_rn(make_float2(__uint_as_float(a + 0x4b400000u), __uint_as_float(b + 0x4b400000u)),
-                    make_float2(-12582912.f, -12582912.f));
-}
-
 template <bool INT8, int G, int TN>
 __global__ void __launch_bounds__(kThreads, 1)
     w4_tile_kernel(const __grid_constant__ CUtensorMap tmx, const TileParams p) {
+  constexpr int kWsSlots = scale_slots<G, TN>();
   constexpr int SA = a_stages<TN>(), SB = b_stages<TN>(), C = code_slots<TN>(), kBStage = TN * 128;
   constexpr int kSpb = INT8 ? 1 : 2;               // stages per 128-column block
   constexpr int kMpg = INT8 ? G / 32 : G / 16;     // MMAs per group
   constexpr int kGpb = kTileK / G;                 // groups per block
   constexpr int kCols = TN / kDrainWgs;            // tokens of one drain warpgroup
-  constexpr int kLd = kCols < 16 ? kCols : 16;     // columns per TMEM load
   constexpr uint32_t kIdesc = INT8 ? umma_idesc_s8(kM, TN) : umma_idesc_bf16(kM, TN, 0, 0);
   constexpr uint32_t kTmemCols = 2 * TN;
 
@@ -136,8 +132,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   using Sh = Shared<INT8, G, TN>;
   uint8_t* b_ring = smem + SA * kAStage;
-  uint8_t* codes = b_ring + SB * kBStage;  // [C][kQuarters][kCodeBytes]
-  Sh* sh = reinterpret_cast<Sh*>(smem + ring_bytes<TN>());
+  uint8_t* codes = b_ring + SB * kBStage;  // [C][kQuarters][block_bytes(G)]
+  Sh* sh = reinterpret_cast<Sh*>(smem + ring_bytes<G, TN>());
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.y;
   const int kb0 = (int)((int64_t)p.kblocks * split / p.splits);
@@ -164,7 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sh->c_empty[b], 4);
     }
     for (int b = 0; b < kWsSlots; ++b) {
-      mbar_init(&sh->ws_full[b], 1);
+      mbar_init(&sh->ws_full[b], 4);
       mbar_init(&sh->ws_empty[b], 4 * kDrainWgs);
     }
     for (int b = 0; b < 2; ++b) {
@@ -189,74 +185,73 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ------------------------------------------------------------ rows by TMA
         tma_prefetch_desc(&tmx);
         pdl_wait();
-        uint32_t it = 0, blk = 0;
+        uint32_t it = 0;
         bool ok = true;
         for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
-          const int tok0 = tile % p.tok_tiles * TN, rb = tile / p.tok_tiles * kQuarters;
-          for (int kb = 0; ok && kb < nkb; ++kb, ++blk) {
-            const int b = blk % kWsSlots;
-            ok = mbar_wait(&sh->ws_empty[b], ((blk / kWsSlots) & 1) ^ 1);
+          const int tok0 = tile % p.tok_tiles * TN;
+          for (int i = 0; i < nkb * kSpb; ++i, ++it) {
+            const int s = it % SB;
+            ok = mbar_wait(&sh->b_empty[s], ((it / SB) & 1) ^ 1);
             if (!ok) break;
-            constexpr uint32_t kWs = sizeof(sh->ws[0][0]);
-            const int quarters = min(kQuarters, p.row_blocks - rb);
-            mbar_arrive_expect_tx(&sh->ws_full[b], kWs * quarters);
-            for (int h = 0; h < quarters; ++h)
-              bulk_load(sh->ws[b][h],
-                        p.packed + ((int64_t)(rb + h) * p.kblocks + kb0 + kb) * block_bytes(G) + kCodeBytes, kWs,
-                        &sh->ws_full[b]);
-            for (int i = 0; i < kSpb; ++i, ++it) {
-              const int s = it % SB;
-              ok = mbar_wait(&sh->b_empty[s], ((it / SB) & 1) ^ 1);
-              if (!ok) break;
-              mbar_arrive_expect_tx(&sh->b_full[s], kBStage);
-              tma_load_2d(b_ring + s * kBStage, &tmx, &sh->b_full[s],
-                          ((kb0 + kb) * kSpb + i) * (INT8 ? 128 : 64), tok0);
-            }
+            mbar_arrive_expect_tx(&sh->b_full[s], kBStage);
+            tma_load_2d(b_ring + s * kBStage, &tmx, &sh->b_full[s], (kb0 * kSpb + i) * (INT8 ? 128 : 64), tok0);
           }
         }
         if (!ok) {  // no copy may still be in flight when the CTA leaves
           report_error(p.err, DEVERR_WAIT_TIMEOUT, kKernelId, (int)it);
           for (uint32_t i = it > SB ? it - SB : 0; i < it; ++i) mbar_wait(&sh->b_full[i % SB], (i / SB) & 1);
-          for (uint32_t i = blk > kWsSlots ? blk - kWsSlots : 0; i < blk; ++i)
-            mbar_wait(&sh->ws_full[i % kWsSlots], (i / kWsSlots) & 1);
         }
       }
     } else if (warp == 1) {
       // -------------------------------------------------------------- MMA issue
-      const uint32_t base = smem_u32(smem);
-      uint32_t it = 0, grp = 0;
+      // One MMA of a 256-token tile takes 128 cycles, so the loop is kept short: stages and
+      // phases are counted, descriptors are additions to two bases, and the MMAs of a stage
+      // (or of a group inside one) go out together.
+      constexpr int kRun = kMpg < 4 ? kMpg : 4;        // MMAs between two waits
+      constexpr int kStagesPerGroup = kMpg / kRun;     // 1, or 2 (bf16 rows in groups of 128)
+      const uint64_t desc_a = umma_sdesc_sw128(smem_u32(smem), 16, 1024);
+      const uint64_t desc_b = umma_sdesc_sw128(smem_u32(b_ring), 16, 1024);
+      uint32_t it = 0, sa = 0, sb = 0, pa = 0, pb = 0, buf = 0, pd = 1, in_group = 0;
       bool ok = true;
       for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
-        for (int kb = 0; ok && kb < nkb; ++kb) {
+        for (int i = 0; i < nkb * kSpb; ++i, ++it) {
+          ok = mbar_wait(&sh->a_full[sa], pa) && mbar_wait(&sh->b_full[sb], pb);
+          const uint64_t da = desc_a + sa * (kAStage >> 4), db = desc_b + sb * (kBStage >> 4);
 #pragma unroll
-          for (int m = 0; m < 4 * kSpb; ++m) {
-            const int sa = it % SA, sb = it % SB;
-            if (m % 4 == 0)
-              ok = ok && mbar_wait(&sh->a_full[sa], (it / SA) & 1) && mbar_wait(&sh->b_full[sb], (it / SB) & 1);
-            if (m % kMpg == 0) ok = ok && mbar_wait(&sh->d_empty[grp & 1], ((grp >> 1) & 1) ^ 1);
-            if (m % 4 == 0 || m % kMpg == 0) {
-              ok = __all_sync(0xffffffffu, ok);
-              if (!ok) break;
-              tc_fence_after();
-            }
+          for (int r = 0; r < 4 / kRun; ++r) {
+            if (in_group == 0) ok = ok && mbar_wait(&sh->d_empty[buf], pd);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const bool last = in_group == kStagesPerGroup - 1;
             if (elect_one()) {
-              const uint64_t da = umma_sdesc_sw128(base + sa * kAStage + (m % 4) * 32, 16, 1024);
-              const uint64_t db = umma_sdesc_sw128(base + SA * kAStage + sb * kBStage + (m % 4) * 32, 16, 1024);
-              const uint32_t d = tmem + (grp & 1) * TN;
-              if (INT8)
-                umma_s8_ss(d, da, db, kIdesc, m % kMpg != 0);
-              else
-                umma_bf16_ss(d, da, db, kIdesc, m % kMpg != 0);
-              if (m % 4 == 3) {
+              const uint32_t d = tmem + buf * TN;
+#pragma unroll
+              for (int m = 0; m < kRun; ++m) {
+                const int at = 2 * (r * kRun + m);  // 32 bytes of k, in descriptor units
+                if (INT8)
+                  umma_s8_ss(d, da + at, db + at, kIdesc, m > 0 || in_group > 0);
+                else
+                  umma_bf16_ss(d, da + at, db + at, kIdesc, m > 0 || in_group > 0);
+              }
+              if (r == 4 / kRun - 1) {
                 umma_commit(&sh->a_empty[sa]);
                 umma_commit(&sh->b_empty[sb]);
               }
-              if (m % kMpg == kMpg - 1) umma_commit(&sh->d_full[grp & 1]);
+              if (last) umma_commit(&sh->d_full[buf]);
             }
             __syncwarp();
-            if (m % 4 == 3) ++it;
-            if (m % kMpg == kMpg - 1) ++grp;
+            if (last) {
+              in_group = 0;
+              buf ^= 1;
+              if (buf == 0) pd ^= 1;
+            } else {
+              ++in_group;
+            }
           }
+          if (!ok) break;
+          if (++sa == SA) sa = 0, pa ^= 1;
+          if (++sb == SB) sb = 0, pb ^= 1;
         }
       }
       if (!ok && lane == 0) report_error(p.err, DEVERR_WAIT_TIMEOUT, kKernelId, 1000000 + (int)it);
@@ -264,21 +259,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       mbar_wait(&sh->done, 0);  // no MMA may still be in flight when TMEM is freed
     } else if (warp == 3) {
-      // -------------------------------------------------------------- codes by bulk copies
+      // -------------------------------------------------------------- packed weights by bulk copies
       if (lane == 0) {  // before the previous kernel has finished: the weights do not depend on it
         uint32_t blk = 0;
         bool ok = true;
         for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
           const int rb = tile / p.tok_tiles * kQuarters, quarters = min(kQuarters, p.row_blocks - rb);
-          const uint8_t* src = p.packed + ((int64_t)rb * p.kblocks + kb0) * block_bytes(G);
-          for (int kb = 0; kb < nkb; ++kb, ++blk, src += block_bytes(G)) {
+          const uint32_t bytes = quarters * block_bytes(G);
+          const uint8_t* src = p.packed + block_offset(rb, kb0, p.kblocks, p.row_blocks, G);
+          for (int kb = 0; kb < nkb; ++kb, ++blk, src += bytes) {
             const int b = blk % C;
             ok = mbar_wait(&sh->c_empty[b], ((blk / C) & 1) ^ 1);
             if (!ok) break;
-            mbar_arrive_expect_tx(&sh->c_full[b], kCodeBytes * quarters);
-            for (int h = 0; h < quarters; ++h)
-              bulk_load(codes + (b * kQuarters + h) * kCodeBytes, src + (int64_t)h * p.kblocks * block_bytes(G), kCodeBytes,
-                        &sh->c_full[b]);
+            mbar_arrive_expect_tx(&sh->c_full[b], bytes);
+            bulk_load(codes + b * kQuarters * block_bytes(G), src, bytes, &sh->c_full[b]);
           }
         }
         if (!ok) {
@@ -303,15 +297,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             float v[kXsGroups];
             const float* src = p.x_scale + (int64_t)(tok0 + c) * p.x_scale_row + gr;
             if (tok0 + c < p.tokens && wide && gr + kXsGroups <= groups) {
-              const float4 lo = *reinterpret_cast<const float4*>(src), hi = *reinterpret_cast<const float4*>(src + 4);
-              v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w;
-              v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+              const float4 q = *reinterpret_cast<const float4*>(src);
+              v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
             } else {
 #pragma unroll
               for (int e = 0; e < kXsGroups; ++e) v[e] = tok0 + c < p.tokens && gr + e < groups ? src[e] : 0.f;
             }
 #pragma unroll
-            for (int e = 0; e < kXsGroups; ++e) sh->xs[b][e][c] = v[e];
+            for (int e = 0; e < kXsGroups; ++e) {
+              // 22 significant bits (truncated), so that 1.5 * 2^23 times it is exact too; 2^-20 keeps that finite
+              const float x = __uint_as_float(__float_as_uint(v[e]) & ~3u) * 0x1p-20f;
+              sh->xs[b][e][0][c] = x;
+              sh->xs[b][e][1][c] = -12582912.f * x;
+            }
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh->xs_full[b]);
@@ -335,10 +333,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
       const int quarters = min(kQuarters, p.row_blocks - tile / p.tok_tiles * kQuarters);
       for (int kb = 0; ok && kb < nkb; ++kb, ++blk) {
-        const int b = blk % C;
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh->c_full[b], (blk / C) & 1));
+        const int b = blk % C, e = blk % kWsSlots;
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh->c_full[b], (blk / C) & 1) &&
+                                         mbar_wait(&sh->ws_empty[e], ((blk / kWsSlots) & 1) ^ 1));
         if (!ok) break;
-        const uint8_t* src = codes + b * kQuarters * kCodeBytes + (4 * g + t) * 16;
+        const uint8_t* src = codes + (b * kQuarters + w) * block_bytes(G);
+        // the row block's scales, for the drain
+        for (int i = lane; i < kGpb * 16; i += 32)
+          reinterpret_cast<uint32_t*>(sh->ws[e][w])[i] = reinterpret_cast<const uint32_t*>(src + kCodeBytes)[i];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->ws_full[e]);
 #pragma unroll
         for (int i = 0; i < kSpb; ++i, ++it) {
           uint4 v[kN];
@@ -346,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int q = 0; q < kN; ++q) {
             // warp w expands row block w: int8 pieces (r, j), bf16 pieces r, j from the stage
             const int r = INT8 ? q >> 1 : q, j = INT8 ? q & 1 : i;
-            v[q] = w < quarters ? *reinterpret_cast<const uint4*>(src + w * kCodeBytes + r * 1024 + j * 512)
+            v[q] = w < quarters ? *reinterpret_cast<const uint4*>(src + r * 1024 + j * 512 + (4 * g + t) * 16)
                                : make_uint4(0, 0, 0, 0);
           }
           if (i == kSpb - 1) {
@@ -387,20 +391,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ---------------------------------------------------------------- drain, epilogue
     regs_inc<192>();
-    const int wg = (warp - 8) >> 2, tid = threadIdx.x & 127, sub = warp & 3;
+    // A lane holds, of each 8 tokens, two neighbours (2 q, 2 q + 1) in four rows (g, + 8, + 16,
+    // + 24 of the warp's 32): a group's token scales are one 8-byte load for eight sums, where
+    // a lane per row would need one for two and wait for shared memory.
+    const int wg = (warp - 8) >> 2, sub = warp & 3, g = lane >> 2, q = lane & 3;
     const uint32_t lanes = (uint32_t)(sub * 32) << 16;
-    // scale of row 16 r + 8 h + g of a row block at 2 (4 g + 2 r + h)
-    const int ws_off = 2 * (4 * (tid & 7) + 2 * ((tid >> 4) & 1) + ((tid >> 3) & 1));
-    pdl_wait();  // before any global write
     uint32_t grp = 0, blk = 0, slot = 0;
     bool ok = true;
+    pdl_wait();  // before any global write
     for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
       const int tok0 = tile % p.tok_tiles * TN + wg * kCols;
-      const int row = (tile / p.tok_tiles) * kM + tid;
-      const bool live_row = tile / p.tok_tiles * kQuarters + (tid >> 5) < p.row_blocks;
-      float2 acc[kCols / 2];
+      const int row0 = (tile / p.tok_tiles) * kM + sub * kTileRows;
+      const bool live = row0 < p.row_blocks * kTileRows;
+      float2 acc[2][kCols / 8][2];  // [16 rows][8 tokens][8 rows]
 #pragma unroll
-      for (int c = 0; c < kCols / 2; ++c) acc[c] = make_float2(0.f, 0.f);
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < kCols / 8; ++c) acc[h][c][0] = acc[h][c][1] = make_float2(0.f, 0.f);
       int gt = 0;  // group of this tile's range
       for (int kb = 0; ok && kb < nkb; ++kb, ++blk) {
         const int b = blk % kWsSlots;
@@ -409,13 +416,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int gi = 0; gi < kGpb; ++gi, ++gt) {
           const int buf = grp & 1;
-          float w1 = live_row ? __uint_as_float((uint32_t)*reinterpret_cast<const unsigned short*>(
-                                                    &sh->ws[b][tid >> 5][gi * 64 + ws_off])
-                                                << 16)
-                              : 0.f;
-          if (INT8) w1 *= 0.0625f;  // int8 codes stand at 16 c
-          const float2 ws = make_float2(w1, w1);
-          const float* xs = &sh->xs[INT8 ? slot & 1 : 0][gt % kXsGroups][INT8 ? wg * kCols : 0];
+          // scales of rows 16 h + 8 e + g at 2 (4 g + 2 h + e); int8 codes stand at 16 c, the tokens' scales at 2^-20
+          const uint2 w4 = live ? *reinterpret_cast<const uint2*>(&sh->ws[b][sub][gi * 64 + g * 8]) : make_uint2(0, 0);
+          constexpr float kUnit = INT8 ? 0x1p16f : 1.f;
+          const float ws[2][2] = {{bf16_lo(w4.x) * kUnit, bf16_hi(w4.x) * kUnit},
+                                  {bf16_lo(w4.y) * kUnit, bf16_hi(w4.y) * kUnit}};
+          const float* xs = &sh->xs[INT8 ? slot & 1 : 0][gt % kXsGroups][0][INT8 ? wg * kCols : 0] + 2 * q;
           if (INT8 && gt % kXsGroups == 0) ok = mbar_wait(&sh->xs_full[slot & 1], (slot >> 1) & 1);
           ok = ok && mbar_wait(&sh->d_full[buf], (grp >> 1) & 1);
           ok = __all_sync(0xffffffffu, ok);
@@ -423,33 +429,37 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
           const uint32_t at = tmem + lanes + buf * TN + wg * kCols;
 #pragma unroll
-          for (int c0 = 0; c0 < kCols; c0 += kLd) {
-            uint32_t u[16];
-            if constexpr (kLd == 16)
-              tmem_ld16(at + c0, u);
-            else
-              tmem_ld8(at + c0, u);
+          for (int c0 = 0; c0 < kCols; c0 += 16) {
+            uint32_t u[2][8];
+            tmem_ld_16x16(at + c0, u[0]);
+            tmem_ld_16x16(at + (16u << 16) + c0, u[1]);
             tmem_wait_ld16(u);
-            if (c0 + kLd == kCols) {  // the buffer is read: the tensor core may sum the next group but one
+            if (c0 + 16 == kCols) {  // the buffer is read: the tensor core may sum the next group but one
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(&sh->d_empty[buf]);
             }
 #pragma unroll
-            for (int c = 0; c < kLd; c += 4) {
-              float2 s0 = ws, s1 = ws, v0, v1;
+            for (int c = 0; c < 2; ++c) {
+              float2 x, y;
               if (INT8) {
-                const float4 x4 = *reinterpret_cast<const float4*>(xs + c0 + c);
-                s0 = __fmul2_rn(ws, make_float2(x4.x, x4.y));
-                s1 = __fmul2_rn(ws, make_float2(x4.z, x4.w));
-                v0 = int_float2(u[c], u[c + 1]);
-                v1 = int_float2(u[c + 2], u[c + 3]);
-              } else {
-                v0 = make_float2(__uint_as_float(u[c]), __uint_as_float(u[c + 1]));
-                v1 = make_float2(__uint_as_float(u[c + 2]), __uint_as_float(u[c + 3]));
+                x = *reinterpret_cast<const float2*>(xs + c0 + 8 * c);
+                y = *reinterpret_cast<const float2*>(xs + TN + c0 + 8 * c);
               }
-              acc[(c0 + c) / 2] = __ffma2_rn(v0, s0, acc[(c0 + c) / 2]);
-              acc[(c0 + c) / 2 + 1] = __ffma2_rn(v1, s1, acc[(c0 + c) / 2 + 1]);
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const uint32_t lo = u[h][4 * c + 2 * e], hi = u[h][4 * c + 2 * e + 1];
+                  float2 v;
+                  if (INT8)  // 1.5 * 2^23 + sum as fp32 bits (exact: 128 x 127 x 128 < 2^21), then
+                             // (1.5 * 2^23 + sum) x - 1.5 * 2^23 x, rounded once
+                    v = __ffma2_rn(make_float2(__uint_as_float(lo + 0x4b400000u), __uint_as_float(hi + 0x4b400000u)), x, y);
+                  else
+                    v = make_float2(__uint_as_float(lo), __uint_as_float(hi));
+                  float2& a = acc[h][c0 / 8 + c][e];
+                  a = __ffma2_rn(v, make_float2(ws[h][e], ws[h][e]), a);
+                }
             }
           }
           ++grp;
@@ -464,23 +474,42 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       if (p.splits == 1) {
-        const float b = p.bias && row < p.n ? __bfloat162float(p.bias[row]) : 0.f;
-        __nv_bfloat16* y = p.y + (int64_t)tok0 * p.y_row + row;
+        // 8 rows x 8 tokens at a time through a register transpose: a lane then stores two
+        // neighbouring rows of one token
+        const bool words = ((reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)(p.y_row * 2)) & 3) == 0;
 #pragma unroll
-        for (int c = 0; c < kCols / 2; ++c) {
-          if (row < p.n) {
-            if (tok0 + 2 * c < p.tokens) y[(int64_t)(2 * c) * p.y_row] = __float2bfloat16_rn(acc[c].x + b);
-            if (tok0 + 2 * c + 1 < p.tokens) y[(int64_t)(2 * c + 1) * p.y_row] = __float2bfloat16_rn(acc[c].y + b);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = row0 + 16 * h + 8 * e;
+            const float bias = p.bias && r + g < p.n ? __bfloat162float(p.bias[r + g]) : 0.f;
+            const int f = r + 2 * q;
+#pragma unroll
+            for (int c = 0; c < kCols / 8; ++c) {
+              const uint32_t v = movmatrix_trans(pack_bf16(acc[h][c][e].x + bias, acc[h][c][e].y + bias));
+              const int tok = tok0 + 8 * c + g;
+              if (tok >= p.tokens) continue;
+              __nv_bfloat16* y = p.y + (int64_t)tok * p.y_row + f;
+              if (words && f + 1 < p.n) {
+                *reinterpret_cast<uint32_t*>(y) = v;
+              } else {
+                if (f < p.n) y[0] = __ushort_as_bfloat16((unsigned short)v);
+                if (f + 1 < p.n) y[1] = __ushort_as_bfloat16((unsigned short)(v >> 16));
+              }
+            }
           }
-        }
       } else {
         // one tile per cluster: every stage has been consumed, their memory takes the partial [token][row]
-        float* part = reinterpret_cast<float*>(smem) + wg * kCols * kM;
+        float* part = reinterpret_cast<float*>(smem) + (wg * kCols + 2 * q) * kM + sub * kTileRows + g;
 #pragma unroll
-        for (int c = 0; c < kCols / 2; ++c) {
-          part[(2 * c) * kM + tid] = acc[c].x;
-          part[(2 * c + 1) * kM + tid] = acc[c].y;
-        }
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int c = 0; c < kCols / 8; ++c)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              part[8 * c * kM + 16 * h + 8 * e] = acc[h][c][e].x;
+              part[(8 * c + 1) * kM + 16 * h + 8 * e] = acc[h][c][e].y;
+            }
       }
     }
     if (!ok && lane == 0) report_error(p.err, DEVERR_WAIT_TIMEOUT, kKernelId, 3000000 + (int)grp);
@@ -518,6 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <bool INT8, int G, int TN>
 int launch(const CUtensorMap& map, const TileParams& p, int sms, cudaStream_t stream) {
+  static_assert(smem_bytes<INT8, G, TN>() <= 227 * 1024, "shared memory of a CTA");
   static std::once_flag once[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return LKV_ERR_CUDA;
