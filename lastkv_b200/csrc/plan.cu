@@ -19,10 +19,12 @@
 // there, n < 1, more tokens than the buffers hold) is recorded in the error word and runs
 // on the scratch pages too.
 //
-// Writing L x B x W table words is the floor.  grid = (rows + 1) x parts: a block takes
-// one part of a row's columns, computes each column once and stores it for every layer;
-// the extra row fills the unused tokens and commit rows.  Every block scans the rows'
-// lengths itself (a few KB from L2), which costs less than a second launch.
+// Writing L x B x W table words is the floor.  grid = (rows + 1) x parts x layer runs: a
+// block takes one part of a row's columns (four neighbours per thread where the width allows
+// 16-byte stores), computes each once and stores it for its run of layers; few rows and
+// columns get more runs, so that the GPU is filled.  The extra row fills the unused tokens
+// and commit rows.  Every block scans the rows' lengths itself (a few KB from L2), which
+// costs less than a second launch.
 
 #include <algorithm>
 
@@ -65,11 +67,15 @@ __device__ __forceinline__ bool row_commits(const PlanArgs& a, const Row& r) {
   return !r.bad && r.slot >= 0 && r.p0 > 0 && r.p0 % a.chunk == 0;
 }
 
+template <int VEC>
 __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   const int b = blockIdx.x, part = blockIdx.y, parts = gridDim.y;
-  const bool tail = b == a.batch;
+  const bool tail = b == a.batch, once = blockIdx.z == 0;  // what a row has once: by the first layer run
+  const int l0 = (int)((int64_t)a.num_layers * blockIdx.z / gridDim.z);
+  const int l1 = (int)((int64_t)a.num_layers * (blockIdx.z + 1) / gridDim.z);
+  if (tail && !once) return;
   // tokens and commits of the rows before this one, and of all rows (saturating: a sum
   // past the buffers is past them)
   __shared__ int64_t s_tok[2][kPlanThreads / 32];
@@ -136,7 +142,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs 
   const Row r = load_row(a, b);
   const bool over = tok[0] + r.tokens > a.max_tokens;
   const bool real = r.slot >= 0 && !r.bad && !over;
-  if (gtid == 0) {
+  if (once && gtid == 0) {
     if (r.bad || over) report_error(a.error_word, DEVERR_BAD_SPAN, kPlanKernelId, b);
     a.cu_q[b] = (int)first_tok;
     a.seq_k[b] = real ? r.p0 + r.n : max(1, (int)(min(first_tok + r.tokens, (int64_t)a.max_tokens) - first_tok));
@@ -146,18 +152,36 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs 
   const int ns = real ? rec / LKV_PAGE_SIZE : 0;
   const int np = real ? (last + LKV_PAGE_SIZE - rec) / LKV_PAGE_SIZE : 0;
   const int32_t* src = a.src_table + (int64_t)(real ? r.slot : 0) * a.src_table_stride;
-  for (int j = gtid; j < a.width; j += gsize) {
-    int v = 0;
-    if (j < ns)
-      v = src[j];
-    else if (j < ns + np)
-      v = r.slot * ring_pages + (ns % ring_pages + j - ns) % ring_pages;
-    else if (!real && j == 0)
-      v = a.scratch_ring_page;
-    int32_t* dst = a.block_tables + (int64_t)b * a.width + j;
-    const int64_t layer = (int64_t)a.batch * a.width;
-    for (int l = 0; l < a.num_layers; ++l) dst[l * layer] = j < ns ? v : v + a.ring_base[l];
+  const int64_t layer = (int64_t)a.batch * a.width;
+  for (int j0 = gtid * VEC; j0 < a.width; j0 += gsize * VEC) {
+    int v[VEC];
+    int ring = j0 < ns + np ? (ns % ring_pages + max(j0 - ns, 0)) % ring_pages : 0;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int j = j0 + e;
+      v[e] = 0;
+      if (j < ns) {
+        v[e] = src[j];
+      } else if (j < ns + np) {
+        v[e] = r.slot * ring_pages + ring;
+        if (++ring == ring_pages) ring = 0;
+      } else if (!real && j == 0) {
+        v[e] = a.scratch_ring_page;
+      }
+    }
+    int32_t* dst = a.block_tables + (int64_t)b * a.width + j0;
+    for (int l = l0; l < l1; ++l) {
+      const int base = a.ring_base[l];
+      if constexpr (VEC == 4) {
+        *reinterpret_cast<int4*>(dst + l * layer) =
+            make_int4(j0 < ns ? v[0] : v[0] + base, j0 + 1 < ns ? v[1] : v[1] + base,
+                      j0 + 2 < ns ? v[2] : v[2] + base, j0 + 3 < ns ? v[3] : v[3] + base);
+      } else {
+        dst[l * layer] = j0 < ns ? v[0] : v[0] + base;
+      }
+    }
   }
+  if (!once) return;
   for (int i = gtid; i < r.tokens; i += gsize) {
     const int64_t t = first_tok + i;
     if (t >= a.max_tokens) break;
@@ -190,8 +214,14 @@ int plan_step(const PlanArgs& a, cudaStream_t stream) {
       !a.cu_q || !a.positions || !a.ring_slots || !a.src_slots || !a.commit_raw || !a.commit_ring ||
       !a.commit_count)
     return LKV_ERR_INVALID_ARGUMENT;
-  const int parts = std::max(1, std::min((a.width + kPlanThreads - 1) / kPlanThreads, 65535));
-  return launch_pdl(plan_step_kernel, dim3((unsigned)a.batch + 1, (unsigned)parts), dim3(kPlanThreads), 0, stream,
+  const bool wide = a.width % 4 == 0 && (reinterpret_cast<uintptr_t>(a.block_tables) & 15) == 0;
+  const int per_block = kPlanThreads * (wide ? 4 : 1);
+  const int parts = std::max(1, std::min((a.width + per_block - 1) / per_block, 65535));
+  // two blocks per SM, if the layers allow
+  const int64_t blocks = ((int64_t)a.batch + 1) * parts;
+  const int runs = (int)std::min<int64_t>(std::min(a.num_layers, 65535), std::max<int64_t>(1, 2 * 148 / blocks));
+  return launch_pdl(wide ? plan_step_kernel<4> : plan_step_kernel<1>,
+                    dim3((unsigned)a.batch + 1, (unsigned)parts, (unsigned)runs), dim3(kPlanThreads), 0, stream,
                     a) == cudaSuccess
              ? LKV_OK
              : LKV_ERR_CUDA;

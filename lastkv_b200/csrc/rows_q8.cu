@@ -9,9 +9,10 @@
 //   plain  y = x
 // A group that holds an infinity or a NaN gets that scale and zeros: its values are NaN.
 //
-// Group maxima compare the bit patterns of |y|, which order like the values and put
-// NaN on top.  The quotient is y * (127 / max), one division per group; a group whose
-// maximum is below 1e-30 divides by s instead, where the reciprocal would overflow.
+// The quotient is y * (127 / max), one division per group, rounded to the integer by the
+// addition that puts it into the low byte of 1.5 * 2^23 + q (no conversion instruction, which
+// runs at an eighth of the rate); a group whose maximum is below 1e-30 divides by s instead,
+// where the reciprocal would overflow.
 
 #include <algorithm>
 
@@ -34,32 +35,38 @@ __device__ __forceinline__ void unpack8(const uint4& v, float* f) {
   }
 }
 
+// max that keeps a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
 // Group scale and quantised values of this lane's 8 columns; `lanes` = G / 8 neighbouring
 // lanes share a group.  The whole warp calls it.  Returns the 8 int8 values, packed.
 __device__ __forceinline__ uint2 quantise8(const float* y, int lanes, float* scale) {
-  uint32_t top = 0;
+  float amax = fabsf(y[0]);
 #pragma unroll
-  for (int j = 0; j < kVec; ++j) top = max(top, __float_as_uint(y[j]) & 0x7fffffffu);
-  for (int o = lanes >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float amax = __uint_as_float(top);
+  for (int j = 1; j < kVec; ++j) amax = max_nan(amax, fabsf(y[j]));
+  for (int o = lanes >> 1; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   const float s = amax / 127.0f;
   *scale = s;
-  int q[kVec];
-  if (top >= 0x7f800000u || s == 0.f) {
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) q[j] = 0;
-  } else if (amax >= 1e-30f) {
+  if (!(amax < INFINITY) || s == 0.f) return make_uint2(0, 0);
+  uint32_t q[kVec];
+  if (amax >= 1e-30f) {
     const float inv = 127.0f / amax;
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) q[j] = __float2int_rn(y[j] * inv);
+    for (int j = 0; j < kVec; ++j) q[j] = __float_as_uint(fmaf(y[j], inv, 12582912.0f));
   } else {
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) q[j] = max(-127, min(127, __float2int_rn(y[j] / s)));
+    for (int j = 0; j < kVec; ++j) q[j] = (uint32_t)max(-127, min(127, __float2int_rn(y[j] / s)));
   }
-  uint2 r;
-  r.x = (q[0] & 0xff) | (q[1] & 0xff) << 8 | (q[2] & 0xff) << 16 | (uint32_t)q[3] << 24;
-  r.y = (q[4] & 0xff) | (q[5] & 0xff) << 8 | (q[6] & 0xff) << 16 | (uint32_t)q[7] << 24;
-  return r;
+  return make_uint2(low_bytes(q[0], q[1], q[2], q[3]), low_bytes(q[4], q[5], q[6], q[7]));
 }
 
 struct NormQ8Params {
@@ -74,126 +81,165 @@ struct NormQ8Params {
   int64_t q_row;
   float* scale;
   int64_t scale_row;
+  int64_t rows;
   int hidden, group;
   float eps;
 };
 
-// One CTA per row, the row in registers (V vectors of 8 columns per thread): one pass
-// over memory, one barrier for the sum of squares.
-template <int V>
-__global__ void __launch_bounds__(V <= 2 ? 1024 : 512) rmsnorm_q8_kernel(const NormQ8Params p) {
+// A CTA takes whole rows, a row in registers (V vectors of 8 columns per thread): one pass
+// over memory, one barrier per row for the sum of squares.  The CTAs are persistent (at most
+// 1536 threads per SM): the next row's loads are in flight while a row is reduced and stored.
+// The weight stays in registers, loaded before the previous kernel has finished.  (Rows of
+// more than 16384 columns, V = 8, leave no registers for either.)
+template <int V, int THREADS>
+__global__ void __launch_bounds__(THREADS) rmsnorm_q8_kernel(const NormQ8Params p) {
   pdl_launch_dependents();
-  const int64_t row = blockIdx.x;
   const int nvec = p.hidden / kVec;
   const uint4 zero = make_uint4(0, 0, 0, 0);
   const uint4* w4 = reinterpret_cast<const uint4*>(p.weight);
-  uint4 wv[V];
+  constexpr bool kAhead = V <= 2;
+  uint4 wv[kAhead ? V : 1], xv[V], rv[V];
+  if (kAhead) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {  // the weight does not depend on the previous kernel
-    const int c = threadIdx.x + i * blockDim.x;
-    wv[i] = c < nvec ? w4[c] : zero;
+    for (int i = 0; i < V; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      wv[kAhead ? i : 0] = c < nvec ? w4[c] : zero;
+    }
   }
   pdl_wait();
-  const uint4* x = reinterpret_cast<const uint4*>(p.x + row * p.x_row);
-  const uint4* r = p.residual ? reinterpret_cast<const uint4*>(p.residual + row * p.residual_row) : nullptr;
-  float h[V][kVec];
-  float ss = 0.f;
+  auto load = [&](int64_t row) {
+    const uint4* x = reinterpret_cast<const uint4*>(p.x + row * p.x_row);
+    const uint4* r = reinterpret_cast<const uint4*>(p.residual + row * p.residual_row);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = threadIdx.x + i * blockDim.x;
-    unpack8(c < nvec ? x[c] : zero, h[i]);
-    if (r && c < nvec) {
-      float rv[kVec];
-      unpack8(r[c], rv);
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) h[i][j] += rv[j];
-      reinterpret_cast<uint4*>(p.residual_out + row * p.residual_out_row)[c] =
-          make_uint4(pack_bf16(h[i][0], h[i][1]), pack_bf16(h[i][2], h[i][3]), pack_bf16(h[i][4], h[i][5]),
-                     pack_bf16(h[i][6], h[i][7]));
+    for (int i = 0; i < V; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      xv[i] = c < nvec ? x[c] : zero;
+      rv[i] = p.residual && c < nvec ? r[c] : zero;
     }
+  };
+  __shared__ float red[2][32];  // two buffers: a row's barrier is the only one
+  const int warps = blockDim.x >> 5, lanes = p.group / kVec;
+  int buf = 0;
+  if (kAhead) load(blockIdx.x);
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, buf ^= 1) {
+    if (!kAhead) load(row);
+    float h[V][kVec];
+    float ss = 0.f;
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) ss = fmaf(h[i][j], h[i][j], ss);
-  }
-  __shared__ float red[32];
+    for (int i = 0; i < V; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      float r[kVec];
+      unpack8(xv[i], h[i]);
+      unpack8(rv[i], r);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const int warps = blockDim.x >> 5;
-  if (warps > 1) {
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
-    __syncthreads();
-    ss = (threadIdx.x & 31) < warps ? red[threadIdx.x & 31] : 0.f;
+      for (int j = 0; j < kVec; ++j) {
+        h[i][j] += r[j];
+        ss = fmaf(h[i][j], h[i][j], ss);
+      }
+      if (p.residual && c < nvec)
+        reinterpret_cast<uint4*>(p.residual_out + row * p.residual_out_row)[c] =
+            make_uint4(pack_bf16(h[i][0], h[i][1]), pack_bf16(h[i][2], h[i][3]), pack_bf16(h[i][4], h[i][5]),
+                       pack_bf16(h[i][6], h[i][7]));
+    }
+    if (kAhead && row + gridDim.x < p.rows) load(row + gridDim.x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  }
-  const float rs = 1.0f / sqrtf(ss / (float)p.hidden + p.eps);
-  const int lanes = p.group / kVec;
+    if (warps > 1) {
+      if ((threadIdx.x & 31) == 0) red[buf][threadIdx.x >> 5] = ss;
+      __syncthreads();
+      ss = (threadIdx.x & 31) < warps ? red[buf][threadIdx.x & 31] : 0.f;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = threadIdx.x + i * blockDim.x;
-    float w[kVec], y[kVec], s;
-    unpack8(wv[i], w);
+      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    }
+    const float rs = 1.0f / sqrtf(ss / (float)p.hidden + p.eps);
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) y[j] = h[i][j] * rs * w[j];
-    const uint2 q = quantise8(y, lanes, &s);
-    if (c < nvec) {
-      *reinterpret_cast<uint2*>(p.q + row * p.q_row + (int64_t)c * kVec) = q;
-      if ((c & (lanes - 1)) == 0) p.scale[row * p.scale_row + c / lanes] = s;
+    for (int i = 0; i < V; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      float w[kVec], y[kVec], s;
+      unpack8(kAhead ? wv[kAhead ? i : 0] : c < nvec ? w4[c] : zero, w);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) y[j] = h[i][j] * rs * w[j];
+      const uint2 q = quantise8(y, lanes, &s);
+      if (c < nvec) {
+        *reinterpret_cast<uint2*>(p.q + row * p.q_row + (int64_t)c * kVec) = q;
+        if ((c & (lanes - 1)) == 0) p.scale[row * p.scale_row + c / lanes] = s;
+      }
     }
   }
 }
 
-// One warp per 256 columns of a row (whole groups), one 8-column vector per lane.
-template <bool SILU>
+// One warp per 256 columns of a row (whole groups), one 8-column vector per lane; with many
+// rows U such chunks' loads are in flight per warp.
+template <bool SILU, int U>
 __global__ void __launch_bounds__(256)
     rows_q8_kernel(const __nv_bfloat16* __restrict__ x, int64_t x_row, int8_t* __restrict__ q, int64_t q_row,
                    float* __restrict__ scale, int64_t scale_row, int64_t rows, int cols, int group) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, lanes = group / kVec, nvec = cols / kVec;
-  const int chunks = (cols + 255) / 256;
-  const int64_t total = rows * chunks;
-  for (int64_t i = blockIdx.x * (int64_t)(blockDim.x >> 5) + (threadIdx.x >> 5); i < total;
-       i += (int64_t)gridDim.x * (blockDim.x >> 5)) {
-    const int64_t row = i / chunks;
-    const int c = (int)(i - row * chunks) * 32 + lane;
-    const uint4* src = reinterpret_cast<const uint4*>(x + row * x_row);
-    float y[kVec], s;
-    unpack8(c < nvec ? src[c] : make_uint4(0, 0, 0, 0), y);
-    if (SILU) {
-      float u[kVec];
-      unpack8(c < nvec ? src[nvec + c] : make_uint4(0, 0, 0, 0), u);
+  const uint32_t chunks = (cols + 255) / 256, total = (uint32_t)rows * chunks;
+  const uint32_t stride = gridDim.x * (blockDim.x >> 5);
+  for (uint32_t i0 = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i0 < total; i0 += U * stride) {
+    uint4 g[U], up[U];
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) y[j] = y[j] / (1.0f + expf(-y[j])) * u[j];
+    for (int k = 0; k < U; ++k) {
+      const uint32_t i = i0 + k * stride, row = i / chunks, c = (i - row * chunks) * 32 + lane;
+      const uint4* src = reinterpret_cast<const uint4*>(x + (int64_t)row * x_row);
+      const bool in = i < total && c < nvec;
+      g[k] = in ? src[c] : make_uint4(0, 0, 0, 0);
+      if (SILU) up[k] = in ? src[nvec + c] : make_uint4(0, 0, 0, 0);
     }
-    const uint2 v = quantise8(y, lanes, &s);
-    if (c < nvec) {
-      *reinterpret_cast<uint2*>(q + row * q_row + (int64_t)c * kVec) = v;
-      if ((c & (lanes - 1)) == 0) scale[row * scale_row + c / lanes] = s;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const uint32_t i = i0 + k * stride, row = i / chunks, c = (i - row * chunks) * 32 + lane;
+      float y[kVec], s;
+      unpack8(g[k], y);
+      if (SILU) {
+        float u[kVec];
+        unpack8(up[k], u);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) y[j] = __fdividef(y[j], 1.0f + expf(-y[j])) * u[j];
+      }
+      const uint2 v = quantise8(y, lanes, &s);
+      if (i < total && c < nvec) {
+        *reinterpret_cast<uint2*>(q + row * q_row + (int64_t)c * kVec) = v;
+        if ((c & (lanes - 1)) == 0) scale[row * scale_row + c / lanes] = s;
+      }
     }
   }
 }
 
+template <int U>
 __global__ void __launch_bounds__(256)
     dequantize_q8_kernel(const int8_t* __restrict__ q, int64_t q_row, const float* __restrict__ scale,
                          int64_t scale_row, __nv_bfloat16* __restrict__ out, int64_t out_row, int64_t rows, int cols,
                          int group) {
   pdl_launch_dependents();
   pdl_wait();
-  const int nvec = cols / kVec;
-  const int64_t total = rows * nvec;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t row = i / nvec;
-    const int c = (int)(i - row * nvec) * kVec;
-    const uint2 v = *reinterpret_cast<const uint2*>(q + row * q_row + c);
-    const float s = scale[row * scale_row + c / group];
-    float f[kVec];
+  const uint32_t nvec = cols / kVec, total = (uint32_t)rows * nvec, stride = gridDim.x * blockDim.x;
+  for (uint32_t i0 = blockIdx.x * blockDim.x + threadIdx.x; i0 < total; i0 += U * stride) {
+    uint2 v[U];
+    float s[U];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f[j] = (float)(int8_t)(v.x >> (8 * j)) * s;
-      f[j + 4] = (float)(int8_t)(v.y >> (8 * j)) * s;
+    for (int k = 0; k < U; ++k) {
+      const uint32_t i = i0 + k * stride, row = i / nvec, c = (i - row * nvec) * kVec;
+      v[k] = i < total ? *reinterpret_cast<const uint2*>(q + row * q_row + c) : make_uint2(0, 0);
+      s[k] = i < total ? scale[row * scale_row + c / group] : 0.f;
     }
-    *reinterpret_cast<uint4*>(out + row * out_row + c) =
-        make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const uint32_t i = i0 + k * stride, row = i / nvec, c = (i - row * nvec) * kVec;
+      if (i >= total) break;
+      const uint32_t lo = v[k].x ^ 0x80808080u, hi = v[k].y ^ 0x80808080u;  // q + 128 as a byte
+      float f[kVec];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // the byte under the exponent of 2^23 is 2^23 + q + 128
+        f[j] = (__uint_as_float(__byte_perm(lo, 0x4b000000u, 0x7440 | j)) - 8388736.0f) * s[k];
+        f[j + 4] = (__uint_as_float(__byte_perm(hi, 0x4b000000u, 0x7440 | j)) - 8388736.0f) * s[k];
+      }
+      *reinterpret_cast<uint4*>(out + row * out_row + c) =
+          make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+    }
   }
 }
 
@@ -210,7 +256,8 @@ bool q8_ok(const Q8RowsArgs& a) {
 int q8_shape(const Q8RowsArgs& a) {
   if (a.group != 32 && a.group != 64 && a.group != 128) return LKV_ERR_UNSUPPORTED;
   if (a.rows < 0 || a.rows > 0x7fffffff || a.cols <= 0 || a.cols % kVec) return LKV_ERR_INVALID_ARGUMENT;
-  return LKV_OK;
+  // work items are counted in 32 bits
+  return a.rows * (a.cols / kVec) <= 0x7fffffff ? LKV_OK : LKV_ERR_UNSUPPORTED;
 }
 
 // CTAs of 256 threads for `warps` warps of work: at most 16 waves of a full GPU, then strides.
@@ -240,16 +287,18 @@ int rmsnorm_q8(const void* x, int64_t x_row, const void* residual, int64_t resid
                  a.q_row,
                  a.scale,
                  a.scale_row,
+                 a.rows,
                  a.cols,
                  a.group,
                  eps};
   const int nvec = a.cols / kVec;
-  const int v = nvec <= 1024 ? 1 : nvec <= 2048 ? 2 : 8;
+  const int v = nvec > 2048 ? 8 : nvec <= 1024 ? 1 : 2;
   const int threads = ((nvec + v - 1) / v + 31) / 32 * 32;
-  void (*kernel)(const NormQ8Params) = v == 1   ? rmsnorm_q8_kernel<1>
-                                       : v == 2 ? rmsnorm_q8_kernel<2>
-                                                : rmsnorm_q8_kernel<8>;
-  return launch_pdl(kernel, dim3((unsigned)a.rows), dim3(threads), 0, stream, p) == cudaSuccess ? LKV_OK
+  void (*kernel)(const NormQ8Params) = v == 1   ? rmsnorm_q8_kernel<1, 1024>
+                                       : v == 2 ? rmsnorm_q8_kernel<2, 1024>
+                                                : rmsnorm_q8_kernel<8, 512>;
+  const int64_t ctas = std::min<int64_t>(a.rows, 148 * std::max(1, 1536 / threads));
+  return launch_pdl(kernel, dim3((unsigned)ctas), dim3(threads), 0, stream, p) == cudaSuccess ? LKV_OK
                                                                                                  : LKV_ERR_CUDA;
 }
 
@@ -258,8 +307,12 @@ int rows_q8(const void* x, int64_t x_row, int silu, const Q8RowsArgs& a, cudaStr
   if (st != LKV_OK) return st;
   if (a.rows == 0) return LKV_OK;
   if (!rows_ok(x, a.rows, x_row, silu ? 2 * (int64_t)a.cols : a.cols, 2, 16) || !q8_ok(a)) return LKV_ERR_INVALID_ARGUMENT;
-  const int blocks = row_blocks(a.rows * ((a.cols + 255) / 256));
-  return launch_pdl(silu ? rows_q8_kernel<true> : rows_q8_kernel<false>, dim3(blocks), dim3(256), 0, stream,
+  const int64_t warps = a.rows * ((a.cols + 255) / 256);
+  const bool many = warps > 148 * 64;  // more than the GPU runs at once
+  const int blocks = row_blocks(many ? (warps + 3) / 4 : warps);
+  return launch_pdl(silu ? (many ? rows_q8_kernel<true, 4> : rows_q8_kernel<true, 1>)
+                         : (many ? rows_q8_kernel<false, 4> : rows_q8_kernel<false, 1>),
+                    dim3(blocks), dim3(256), 0, stream,
                     static_cast<const __nv_bfloat16*>(x), x_row, a.q, a.q_row, a.scale, a.scale_row, a.rows, a.cols,
                     a.group) == cudaSuccess
              ? LKV_OK
@@ -271,8 +324,10 @@ int dequantize_q8(const Q8RowsArgs& a, void* out, int64_t out_row, cudaStream_t 
   if (st != LKV_OK) return st;
   if (a.rows == 0) return LKV_OK;
   if (!q8_ok(a) || !rows_ok(out, a.rows, out_row, a.cols, 2, 16)) return LKV_ERR_INVALID_ARGUMENT;
-  const int blocks = row_blocks((a.rows * (a.cols / kVec) + 31) / 32);
-  return launch_pdl(dequantize_q8_kernel, dim3(blocks), dim3(256), 0, stream, static_cast<const int8_t*>(a.q),
+  const int64_t warps = (a.rows * (a.cols / kVec) + 31) / 32;
+  const bool many = warps > 148 * 64;
+  return launch_pdl(many ? dequantize_q8_kernel<4> : dequantize_q8_kernel<1>,
+                    dim3(row_blocks(many ? (warps + 3) / 4 : warps)), dim3(256), 0, stream, static_cast<const int8_t*>(a.q),
                     a.q_row, static_cast<const float*>(a.scale), a.scale_row, static_cast<__nv_bfloat16*>(out),
                     out_row, a.rows, a.cols, a.group) == cudaSuccess
              ? LKV_OK

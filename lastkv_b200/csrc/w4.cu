@@ -189,7 +189,6 @@ __device__ __forceinline__ void add_group(float (&acc)[2][NT][4], const WeightBl
 // last read the last one's row (their sums are not stored).
 constexpr int kDepth = 3;
 constexpr int kSkinnyKernelId = 14;
-constexpr int kSkinnyTokens = 16;  // above, the tcgen05 kernel takes over
 
 template <int G, int NT, int W>
 struct SkinnyShared {
@@ -403,6 +402,15 @@ int device_sms(int* sms) {
   return LKV_OK;
 }
 
+// The streaming kernel reads the weight again for every 16 tokens (from L2), so it takes up to
+// 32 tokens, and more where its CTAs still fit the GPU at once; the tcgen05 kernel the rest.
+// int8 / bf16 rows, streaming against tcgen05: 32 tokens 4096 x 4096 6.16 / 7.80 against 9.04 /
+// 11.5 us, 28672 x 4096 35.4 / 48.3 against 33.8 / 52.0 us; 64 tokens 1003 x 1544 2.95 / 3.34
+// against 7.28 / 7.32 us, 4096 x 4096 (512 CTAs) 10.9 / 14.3 against 10.2 / 12.5 us.
+bool few_tokens(const W4Args& a, int sms) {
+  return a.tokens <= 32 || (a.n + kTileRows - 1) / kTileRows * ((a.tokens + 15) / 16) <= 2 * (int64_t)sms;
+}
+
 bool shape_ok(int64_t n, int64_t k) { return n >= 1 && n <= 0x7fffff00 && k >= 8 && k <= 0x7fffff00 && k % 8 == 0; }
 
 }  // namespace
@@ -443,7 +451,7 @@ int w4_linear(const W4Args& a, cudaStream_t stream) {
   int sms = 0;
   const int st = device_sms(&sms);
   if (st != LKV_OK) return st;
-  if (a.tokens > kSkinnyTokens && w4_tile_aligned(a)) return w4_tile(a, sms, stream);
+  if (!few_tokens(a, sms) && w4_tile_aligned(a)) return w4_tile(a, sms, stream);
   SkinnyParams p{};
   p.packed = static_cast<const uint8_t*>(a.packed);
   p.x = a.x;

@@ -2,15 +2,20 @@
 //
 // Tile: 128 output rows (the MMA's M side) x TN tokens (N side).  Per 128 bytes of k (128
 // columns of int8 rows, 64 of bf16 rows) one stage of shared memory holds the A operand -
-// the codes, expanded from 4 bits to int8 (16 c) or bf16 (c, exact) by the four dequant
-// warps - and the B operand, the rows as they are, by TMA; both K-major, 128-byte swizzled.
+// the codes, expanded from 4 bits to int8 (16 c) or bf16 (c, exact) - and the B operand, the
+// rows as they are, by TMA; both K-major, 128-byte swizzled.
 //
-// Group scales stay out of the operands: a group's MMAs sum into one of two TMEM buffers
+// Group scales stay out of the operands: a group's MMAs sum into one of two or four TMEM buffers
 // from zero (int32 or fp32), and the eight drain warps add each finished group into fp32
-// registers, scaled by the weight's scale of their lane's row and, for int8 rows, by the
-// tokens' scales, while the tensor core sums the next group into the other buffer.  So
+// registers, scaled by the weight's scale of the row and, for int8 rows, by the token's,
+// while the tensor core sums the next groups into the other buffers.  So
 // int8 x 4-bit group sums are exact and no weight is rounded, at the price of reading
-// 128 x TN sums from TMEM per group.
+// 128 x TN sums from TMEM per group, which is what bounds it: 2048 tokens x 28672 x 4096 in
+// groups of 128 take 457 us with bf16 rows (1053 TFLOP/s, 0.63 of the measured bf16 peak) and
+// 565 us with int8 rows, whose sums need a second multiply-add each; in groups of 64 and 32
+// (4096 x 4096) 72 -> 102 -> 167 us and 90 -> 151 -> 274 us.  Four drain warpgroups (567 us),
+// a second expanding one (narrow tiles 65 against 58 us), 32-column loads (482 us) and waits
+// with a suspend hint (482 / 580 us) were no faster.
 //
 // Roles of the 512 threads (one CTA per SM, persistent over the tiles):
 //   warp 0  rows by TMA                         warp 1     tcgen05.mma issue, TMEM
@@ -58,19 +63,24 @@ __host__ __device__ constexpr int a_stages() {
 }
 template <int TN>
 __host__ __device__ constexpr int b_stages() {
-  return TN == 256 ? 4 : TN == 128 ? 6 : TN == 64 ? 8 : 12;
+  return TN == 256 ? 4 : TN == 128 ? 6 : 8;
 }
 
 // 128-column blocks of packed weights (8 KB and the scales for the tile's 128 rows) in flight
 template <int TN>
 __host__ __device__ constexpr int code_slots() {
-  return TN == 256 ? 3 : TN == 128 ? 4 : TN == 64 ? 8 : 10;
+  return TN == 256 ? 3 : TN == 128 ? 4 : 8;
 }
-
 
 template <int G, int TN>
 __host__ __device__ constexpr int ring_bytes() {
   return a_stages<TN>() * kAStage + b_stages<TN>() * TN * 128 + code_slots<TN>() * kQuarters * block_bytes(G);
+}
+
+// TMEM buffers of group sums: two 256-token tiles fill its 512 columns
+template <int TN>
+__host__ __device__ constexpr int d_buffers() {
+  return TN == 256 ? 2 : 4;
 }
 
 // blocks of weight scales in flight: as many as the codes run ahead of the drain
@@ -84,8 +94,7 @@ template <bool INT8, int G, int TN>
 struct Shared {
   uint64_t a_full[a_stages<TN>()], a_empty[a_stages<TN>()];
   uint64_t b_full[b_stages<TN>()], b_empty[b_stages<TN>()];
-  uint64_t d_full[2];
-  uint64_t d_empty[2];
+  uint64_t d_full[d_buffers<TN>()], d_empty[d_buffers<TN>()];
   uint64_t done;
   uint64_t c_full[code_slots<TN>()], c_empty[code_slots<TN>()];
   uint64_t ws_full[scale_slots<G, TN>()], ws_empty[scale_slots<G, TN>()];
@@ -116,17 +125,27 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t 
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// 1.5 * 2^23 + v for an int32 |v| < 2^22 (128 x 127 x 128 < 2^21 here), exactly: the integer sum
+// of v and the bits of 1.5 * 2^23, which masking and flipping bit 22 give for either sign.
+// (A logic instruction: the add goes to the fp32 pipe, which the drain fills already, and a
+// conversion runs at an eighth of their rate.)
+__device__ __forceinline__ float int_bits(uint32_t v) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(v), "r"(0x007fffffu), "r"(0x4b400000u));
+  return __uint_as_float(r);
+}
+
 template <bool INT8, int G, int TN>
 __global__ void __launch_bounds__(kThreads, 1)
     w4_tile_kernel(const __grid_constant__ CUtensorMap tmx, const TileParams p) {
   constexpr int kWsSlots = scale_slots<G, TN>();
-  constexpr int SA = a_stages<TN>(), SB = b_stages<TN>(), C = code_slots<TN>(), kBStage = TN * 128;
+  constexpr int SA = a_stages<TN>(), SB = b_stages<TN>(), C = code_slots<TN>(), kBStage = TN * 128, ND = d_buffers<TN>();
   constexpr int kSpb = INT8 ? 1 : 2;               // stages per 128-column block
   constexpr int kMpg = INT8 ? G / 32 : G / 16;     // MMAs per group
   constexpr int kGpb = kTileK / G;                 // groups per block
   constexpr int kCols = TN / kDrainWgs;            // tokens of one drain warpgroup
   constexpr uint32_t kIdesc = INT8 ? umma_idesc_s8(kM, TN) : umma_idesc_bf16(kM, TN, 0, 0);
-  constexpr uint32_t kTmemCols = 2 * TN;
+  constexpr uint32_t kTmemCols = ND * TN;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -150,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sh->b_full[s], 1);
       mbar_init(&sh->b_empty[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < ND; ++b) {
       mbar_init(&sh->d_full[b], 1);
       mbar_init(&sh->d_empty[b], 4 * kDrainWgs);
     }
@@ -243,8 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (last) {
               in_group = 0;
-              buf ^= 1;
-              if (buf == 0) pd ^= 1;
+              if (++buf == ND) buf = 0, pd ^= 1;
             } else {
               ++in_group;
             }
@@ -328,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // stores of half a warp apart.
     const int w = warp - 4, t = lane & 3, q3 = lane >> 3;
     const int g = ((q3 & 1) << 1 | q3 >> 1) ^ ((lane & 4) ? 5 : 0);
-    uint32_t it = 0, blk = 0;
+    uint32_t blk = 0;
     bool ok = true;
     for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
       const int quarters = min(kQuarters, p.row_blocks - tile / p.tok_tiles * kQuarters);
@@ -344,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->ws_full[e]);
 #pragma unroll
-        for (int i = 0; i < kSpb; ++i, ++it) {
+        for (int i = 0; i < kSpb; ++i) {
           uint4 v[kN];
 #pragma unroll
           for (int q = 0; q < kN; ++q) {
@@ -357,6 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh->c_empty[b]);
           }
+          const uint32_t it = blk * kSpb + i;
           const int s = it % SA;
           ok = ok && __all_sync(0xffffffffu, mbar_wait(&sh->a_empty[s], ((it / SA) & 1) ^ 1));
           if (!ok) break;
@@ -387,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    if (!ok && lane == 0) report_error(p.err, DEVERR_WAIT_TIMEOUT, kKernelId, 2000000 + (int)it);
+    if (!ok && lane == 0) report_error(p.err, DEVERR_WAIT_TIMEOUT, kKernelId, 2000000 + (int)blk);
   } else {
     // ---------------------------------------------------------------- drain, epilogue
     regs_inc<192>();
@@ -415,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
 #pragma unroll 1
         for (int gi = 0; gi < kGpb; ++gi, ++gt) {
-          const int buf = grp & 1;
+          const int buf = grp % ND;
           // scales of rows 16 h + 8 e + g at 2 (4 g + 2 h + e); int8 codes stand at 16 c, the tokens' scales at 2^-20
           const uint2 w4 = live ? *reinterpret_cast<const uint2*>(&sh->ws[b][sub][gi * 64 + g * 8]) : make_uint2(0, 0);
           constexpr float kUnit = INT8 ? 0x1p16f : 1.f;
@@ -423,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                   {bf16_lo(w4.y) * kUnit, bf16_hi(w4.y) * kUnit}};
           const float* xs = &sh->xs[INT8 ? slot & 1 : 0][gt % kXsGroups][0][INT8 ? wg * kCols : 0] + 2 * q;
           if (INT8 && gt % kXsGroups == 0) ok = mbar_wait(&sh->xs_full[slot & 1], (slot >> 1) & 1);
-          ok = ok && mbar_wait(&sh->d_full[buf], (grp >> 1) & 1);
+          ok = ok && mbar_wait(&sh->d_full[buf], (grp / ND) & 1);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
@@ -452,9 +471,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int e = 0; e < 2; ++e) {
                   const uint32_t lo = u[h][4 * c + 2 * e], hi = u[h][4 * c + 2 * e + 1];
                   float2 v;
-                  if (INT8)  // 1.5 * 2^23 + sum as fp32 bits (exact: 128 x 127 x 128 < 2^21), then
-                             // (1.5 * 2^23 + sum) x - 1.5 * 2^23 x, rounded once
-                    v = __ffma2_rn(make_float2(__uint_as_float(lo + 0x4b400000u), __uint_as_float(hi + 0x4b400000u)), x, y);
+                  if (INT8)  // (1.5 * 2^23 + sum) x - 1.5 * 2^23 x, rounded once
+                    v = __ffma2_rn(make_float2(int_bits(lo), int_bits(hi)), x, y);
                   else
                     v = make_float2(__uint_as_float(lo), __uint_as_float(hi));
                   float2& a = acc[h][c0 / 8 + c][e];
@@ -567,7 +585,6 @@ int launch(const CUtensorMap& map, const TileParams& p, int sms, cudaStream_t st
 template <bool INT8, int G>
 int by_tokens(int tn, const CUtensorMap& map, const TileParams& p, int sms, cudaStream_t stream) {
   switch (tn) {
-    case 32: return launch<INT8, G, 32>(map, p, sms, stream);
     case 64: return launch<INT8, G, 64>(map, p, sms, stream);
     case 128: return launch<INT8, G, 128>(map, p, sms, stream);
     default: return launch<INT8, G, 256>(map, p, sms, stream);
@@ -596,7 +613,7 @@ int w4_tile(const W4Args& a, int sms, cudaStream_t stream) {
   p.kblocks = (int)((a.k + kTileK - 1) / kTileK);
   p.row_blocks = (int)((a.n + kTileRows - 1) / kTileRows);
   p.err = a.error_word;
-  const int tn = a.tokens <= 32 ? 32 : a.tokens <= 64 ? 64 : a.tokens <= 128 ? 128 : 256;
+  const int tn = a.tokens <= 64 ? 64 : a.tokens <= 128 ? 128 : 256;
   p.tok_tiles = (int)((a.tokens + tn - 1) / tn);
   const int64_t tiles = (a.n + kM - 1) / kM * p.tok_tiles;
   if (tiles > 0x7fffffff) return LKV_ERR_UNSUPPORTED;
