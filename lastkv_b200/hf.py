@@ -138,6 +138,46 @@ class RMSNorm(nn.Module):
         h = x if residual is None else x + residual
         return h, self(h)
 
+    def fused_q8(self, x, residual=None, group=128):
+        """``fused`` with int8 rows of ``group`` columns as the norm's output (``ops.rmsnorm_q8``)."""
+        w = self.weight.detach()
+        if residual is None:
+            return x, ops.rmsnorm_q8(x, w, self.variance_epsilon, group=group)
+        return ops.rmsnorm_q8(x, w, self.variance_epsilon, residual, group=group)
+
+
+@dataclass
+class QuantizedLinears:
+    """Projections with 4-bit weights (``quantize_projections_``): one weight for linears that
+    share their input, its bias, and whether their input comes as int8 rows."""
+
+    weight: ops.W4Weight
+    bias: torch.Tensor | None
+    int8: bool
+
+    @classmethod
+    def of(cls, linears, group: int, int8: bool, release: bool) -> "QuantizedLinears":
+        """Round the linears' weights, side by side along the outputs, to 4 bits with group scales.
+        ``release`` frees the bf16 weights (the modules keep empty ones)."""
+        for lin in linears:
+            w = lin.weight
+            if not (w.is_cuda and w.dtype == torch.bfloat16 and w.dim() == 2 and w.numel()):
+                raise RMarinBackendContractError("4-bit projections are made from bf16 CUDA weights")
+        weight = ops.w4_quantize(torch.cat([lin.weight.detach() for lin in linears], 0), group)
+        bias = None
+        if linears[0].bias is not None:
+            bias = torch.cat([lin.bias.detach() for lin in linears], 0).contiguous()
+        if release:
+            for lin in linears:
+                lin.weight = nn.Parameter(lin.weight.new_empty((0, lin.in_features)), requires_grad=False)
+        return cls(weight, bias, int8)
+
+    def __call__(self, x):
+        """The projections of x: bf16 [..., k], rounded to int8 rows first where they are taken, or int8 rows."""
+        if self.int8 and not isinstance(x, ops.Q8Rows):
+            x = ops.quantize_q8(x, group=self.weight.group)
+        return ops.w4_linear(x, self.weight, self.bias)
+
 
 def _fuse_linears(linears) -> tuple[torch.Tensor, torch.Tensor | None]:
     """Concatenate the weights (and biases) of ``linears`` along the output dim and
@@ -191,6 +231,13 @@ class MLP(nn.Module):
         self.up_proj = nn.Linear(config.hidden_size, config.intermediate_size, bias=False)
         self.down_proj = nn.Linear(config.intermediate_size, config.hidden_size, bias=False)
         self._gate_up = None
+        self._w4 = None
+
+    def quantize_(self, group: int, int8: bool, release: bool):
+        """4-bit [gate | up] and down projections."""
+        self._w4 = (QuantizedLinears.of([self.gate_proj, self.up_proj], group, int8, release),
+                    QuantizedLinears.of([self.down_proj], group, int8, release))
+        return self
 
     def fuse_(self):
         """One [gate | up] GEMM + the SiLU-and-mul kernel instead of two GEMMs and two elementwise ops."""
@@ -198,6 +245,10 @@ class MLP(nn.Module):
         return self
 
     def forward(self, x):
+        if self._w4 is not None:
+            gate_up, down = self._w4
+            h = gate_up(x)
+            return down(ops.silu_mul_q8(h, group=down.weight.group) if down.int8 else ops.silu_mul(h))
         if x.is_cuda and x.dtype == torch.bfloat16 and _fused_ok(self._gate_up, [self.gate_proj, self.up_proj]):
             w = self._gate_up[0]
             h = _decode_linear(x, w, silu_mul=True)
@@ -454,7 +505,15 @@ class LastKVAttention(nn.Module):
             self.q_norm = RMSNorm(d, config.rms_norm_eps)
             self.k_norm = RMSNorm(d, config.rms_norm_eps)
         self._qkv = None
+        self._w4 = None
         self._consts = (None, None)
+
+    def quantize_(self, group: int, int8: bool, release: bool):
+        """4-bit [q | k | v] and output projections."""
+        self._w4 = (QuantizedLinears.of([self.q_proj, self.k_proj, self.v_proj], group, int8, release),
+                    QuantizedLinears.of([self.o_proj], group, int8, release))
+        self._qkv = None
+        return self
 
     def fuse_qkv_(self):
         """One [q | k | v] GEMM per call; the three projections become views of its weight."""
@@ -495,11 +554,15 @@ class LastKVAttention(nn.Module):
         return self.prev_chunk_alphas.detach().to(kv_dtype).sigmoid().float()
 
     def forward(self, hidden_states, position_embeddings, cache: PagedLastKVCache):
-        B, L, _ = hidden_states.shape
+        """``hidden_states`` [B, L, hidden], or its int8 rows (4-bit projections)."""
+        B, L = hidden_states.lead if isinstance(hidden_states, ops.Q8Rows) else hidden_states.shape[:2]
         D, Hq, Hkv = self.head_dim, self.num_heads, self.num_key_value_heads
         meta = cache._meta if cache._meta is not None and cache._meta["n"] == L else cache.plan(L)
-        fast = _fused_ok(self._qkv, [self.q_proj, self.k_proj, self.v_proj])
-        if fast:
+        fast = self._w4 is None and _fused_ok(self._qkv, [self.q_proj, self.k_proj, self.v_proj])
+        if self._w4 is not None:
+            qkv = self._w4[0](hidden_states).reshape(B * L, (Hq + 2 * Hkv) * D)
+            q, k, v = qkv[:, : Hq * D], qkv[:, Hq * D: (Hq + Hkv) * D], qkv[:, (Hq + Hkv) * D:]
+        elif fast:
             qkv = _decode_linear(hidden_states, *self._qkv)
             if qkv is None:
                 qkv = F.linear(hidden_states, *self._qkv)
@@ -544,7 +607,10 @@ class LastKVAttention(nn.Module):
         else:
             out = ops.prefill_paged(q_out, cache.pool_k, cache.pool_v, bt, meta["seq_k"], meta["cu_q"], L,
                                     out_scale=out_scale, error_word=cache.error_word, max_pages=meta["W"])
-        out = out.view(B, L, Hq * D).to(hidden_states.dtype)
+        out = out.view(B, L, Hq * D)
+        if self._w4 is not None:
+            return self._w4[1](out)
+        out = out.to(hidden_states.dtype)
         y = _decode_linear(out, self.o_proj.weight, self.o_proj.bias) if fast else None
         return y if y is not None else self.o_proj(out)
 
@@ -568,9 +634,20 @@ class LastKVDecoderLayer(nn.Module):
         with each residual add done inside the following RMSNorm kernel; the MLP
         output is returned un-added so the next layer's norm can absorb it.
         """
+        w4 = self.self_attn._w4
+        if w4 is not None and w4[0].int8:  # the norms write the int8 rows that the projections take
+            group = w4[0].weight.group
+            h, x = self.input_layernorm.fused_q8(residual, delta, group)
+            h, x = self.post_attention_layernorm.fused_q8(h, self.self_attn(x, position_embeddings, cache), group)
+            return h, self.mlp(x)
         h, x = self.input_layernorm.fused(residual, delta)
         h, x = self.post_attention_layernorm.fused(h, self.self_attn(x, position_embeddings, cache))
         return h, self.mlp(x)
+
+    def quantize_projections_(self, group: int, int8: bool, release: bool):
+        self.self_attn.quantize_(group, int8, release)
+        self.mlp.quantize_(group, int8, release)
+        return self
 
     def fuse_projections_(self):
         self.self_attn.fuse_qkv_()
@@ -657,6 +734,20 @@ class LastKVForCausalLM(nn.Module):
         model (a later move falls back to the module path)."""
         for layer in self.model.layers:
             layer.fuse_projections_()
+        return self
+
+    def quantize_projections_(self, group: int = 128, activations: str = "int8", release: bool = False):
+        """4-bit projections: every layer's q/k/v, output, gate/up and down weights are rounded
+        to 4 bits with a bf16 scale per ``group`` (32, 64 or 128) input columns and run on
+        ``ops.w4_linear``, for decode steps and prefill alike.  ``activations``: ``"int8"``
+        (the norms, SiLU-and-mul and the attention output leave int8 rows with a scale per
+        group) or ``"bf16"``.  Embedding, norms and LM head stay bf16.  Call it on a bf16 CUDA
+        model with its weights loaded; ``release`` frees the bf16 projection weights (the
+        state dict then no longer holds them).  Later changes of the weights are not seen."""
+        if activations not in ("int8", "bf16"):
+            raise RMarinBackendContractError(f"activations must be 'int8' or 'bf16', got {activations!r}")
+        for layer in self.model.layers:
+            layer.quantize_projections_(group, activations == "int8", release)
         return self
 
     def new_cache(self, batch: int, max_tokens: int, **kw) -> PagedLastKVCache:

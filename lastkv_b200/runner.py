@@ -11,6 +11,11 @@ chunk-boundary commit runs inside the first layer's append of the next step:
 a second graph, captured with that fused launch over static page lists,
 replays for the step after each boundary.  All sequences of the batch advance
 together (equal positions), as in ``generate``.
+
+With ``device_plan=True`` the prologue runs inside the graph as well
+(``ops.StepPlan``): the tables, slots, positions and commit lists of a step are
+built on the device from the lengths there, which the step advances itself, so a
+step is one graph launch and copies nothing from the host.
 """
 
 from __future__ import annotations
@@ -25,7 +30,7 @@ from .hf import LastKVForCausalLM, PagedLastKVCache
 class GraphDecodeRunner:
     NSETS = 4
 
-    def __init__(self, model: LastKVForCausalLM, cache: PagedLastKVCache):
+    def __init__(self, model: LastKVForCausalLM, cache: PagedLastKVCache, *, device_plan: bool = False):
         self.model, self.cache = model, cache
         dev = cache.device
         B, L = cache.batch, cache.num_layers
@@ -55,10 +60,35 @@ class GraphDecodeRunner:
         ppc = cache.chunk_size // PAGE_SIZE
         self.c_raw = torch.zeros((B, ppc), dtype=torch.int32, device=dev)
         self.c_ring = torch.zeros((B, ppc), dtype=torch.int32, device=dev)
+        self.plan = None
+        if device_plan:
+            # the step's lengths, advanced by the graph; the plan's buffers take the place of the staged ones
+            self.computed = torch.zeros(B, dtype=torch.int32, device=dev)
+            self.new_tokens = torch.ones(B, dtype=torch.int32, device=dev)
+            self.slots = torch.arange(B, dtype=torch.int32, device=dev)
+            self._computed_host = None  # what the device's lengths are known to be
+            scratch = cache.ring_pages * B  # each layer's spare ring page (no row of this runner uses it)
+            self.plan = ops.StepPlan(B, B, cache.src_table_dev, cache.ring_base_dev, chunk_size=cache.chunk_size,
+                                     max_sequence_tokens=cache.max_tokens, scratch_src_page=cache.src_pages + scratch,
+                                     scratch_ring_page=scratch, width=self.W, error_word=cache.error_word)
+            p = self.plan
+            self.bt_all, self.seq_k, self.ring_tok, self.src_slot = p.block_tables, p.seq_k, p.ring_slots, p.src_slots
+            self.pos = p.positions[:1].view(1, 1)
+            self.c_raw, self.c_ring = p.commit_raw, p.commit_ring
 
     def _prepare(self):
         """Host plan of the next token -> static device buffers (stream-ordered copies)."""
         cache = self.cache
+        if self.plan is not None:
+            if cache.seen_tokens >= cache.max_tokens:
+                raise RMarinBackendContractError(f"cache capacity {cache.max_tokens} exceeded")
+            if cache.pages_per_seq + cache.ring_pages != self.W or cache.src_table_dev is not self.plan.src_table:
+                raise RMarinBackendContractError("the cache has grown since the runner planned its steps")
+            if self._computed_host != cache.seen_tokens:  # a prefill or another runner has moved the cache
+                self.computed.fill_(cache.seen_tokens)
+                self._computed_host = cache.seen_tokens
+            self._fresh_meta()
+            return
         h = cache.plan_host(1)
         self._set = (self._set + 1) % self.NSETS
         st = self._h[self._set]
@@ -99,6 +129,9 @@ class GraphDecodeRunner:
 
     def _body(self):
         m = self.model.model
+        if self.plan is not None:
+            # first, so that the embedding (a plain launch) lies between the tables and the PDL chain
+            self.plan.run(self.computed, self.new_tokens, self.slots)
         hidden = m.embed_tokens(self.ids)
         pe = m.rotary_emb(hidden, self.pos)
         logits = self.model.lm_head(m.run_layers(hidden, pe, self.cache)[:, -1])
@@ -106,6 +139,8 @@ class GraphDecodeRunner:
             ops.argmax_rows(logits, out=self.ids.view(-1))  # torch.argmax order, one launch
         else:
             self.ids.copy_(logits.float().argmax(-1, keepdim=True))
+        if self.plan is not None:
+            self.computed.add_(self.new_tokens)
 
     def capture(self):
         """Capture one decode step at the current position (the warm-up runs do not advance),
@@ -121,6 +156,8 @@ class GraphDecodeRunner:
         with torch.cuda.stream(s):
             for i in range(3 if fused else 2):
                 self.ids.copy_(saved)
+                if self.plan is not None:
+                    self.computed.fill_(cache.seen_tokens)
                 self._fresh_meta()
                 if i == 2:  # loads the fused append kernel before its capture; commits nothing
                     cache._pending = ops.Commit(cache.pool_k, cache.pool_v, empty, empty, cache.ring_stride,
@@ -145,6 +182,9 @@ class GraphDecodeRunner:
                 cache._pending = None
             self.graph_commit = gc
         self.ids.copy_(saved)
+        if self.plan is not None:
+            self.computed.fill_(cache.seen_tokens)
+            self._computed_host = cache.seen_tokens
 
     def step(self):
         """One greedy token for every sequence; returns the device tensor of new ids [B, 1]."""
@@ -160,12 +200,15 @@ class GraphDecodeRunner:
             pending = None
         self._prepare()
         if pending is not None:
-            self.c_raw.copy_(pending.raw_pages)
-            self.c_ring.copy_(pending.ring_pages)
+            if self.plan is None:  # (the device plan makes the same lists)
+                self.c_raw.copy_(pending.raw_pages)
+                self.c_ring.copy_(pending.ring_pages)
             self.graph_commit.replay()
         else:
             self.graph.replay()
         cache.seen_tokens += 1
+        if self.plan is not None:
+            self._computed_host = cache.seen_tokens
         cache._meta = None
         if cache.seen_tokens % cache.chunk_size == 0:
             cache.commit(self.alpha)

@@ -50,7 +50,8 @@ def _gen(*key):
 
 SHAPES = [(1, 64, 128), (1, 1, 8), (3, 100, 72), (8, 768, 768), (8, 4096, 4096), (9, 130, 1544), (16, 2055, 264),
           (17, 64, 4096), (33, 1003, 1544), (40, 4096, 136), (64, 6144, 512), (65, 300, 2048), (128, 129, 1160),
-          (200, 1000, 776), (256, 768, 2048), (300, 2048, 768), (1030, 520, 392)]
+          (200, 1000, 776), (256, 768, 2048), (300, 2048, 768), (1030, 520, 392), (70, 3000, 1544),
+          (100, 2055, 392), (50, 5000, 136), (400, 1500, 8), (129, 2600, 4096), (2000, 257, 264)]
 
 
 @pytest.mark.parametrize("t,n,k", SHAPES)
@@ -68,13 +69,15 @@ def test_matches_definition(t, n, k, group, int8):
     assert err.tolist() == [0, 0, 0, 0]
 
 
-@pytest.mark.parametrize("t", [1, 8, 20, 90, 300])
+@pytest.mark.parametrize("t,n", [(1, 203), (8, 203), (20, 203), (90, 203), (300, 203),
+                                 (60, 2403), (100, 2402), (300, 2403), (290, 2402)])
 @pytest.mark.parametrize("int8", [False, True])
-def test_bias_strides_and_untouched_neighbours(t, int8):
+@pytest.mark.parametrize("off", [8, 16])
+def test_bias_strides_and_untouched_neighbours(t, n, int8, off):
     from lastkv_b200 import ops
 
-    n, k, group = 203, 1032, 64
-    g = _gen(t, int8)
+    k, group = 1032, 64
+    g = _gen(t, int8, n, off)
     codes, scales, w64 = make_weight(n, k, group, g)
     wide_c = torch.zeros((n, k // 2 + 7), dtype=torch.uint8, device="cuda")
     wide_c[:, : k // 2] = codes
@@ -83,26 +86,26 @@ def test_bias_strides_and_untouched_neighbours(t, int8):
     x, x64 = make_x(t, k, group, int8, g)
     if int8:
         q = torch.full((t, k + 40), 55, dtype=torch.int8, device="cuda")
-        q[:, 8:k + 8] = x.q
+        q[:, off:k + off] = x.q
         s = torch.full((t, x.scale.shape[1] + 3), float("nan"), device="cuda")
         s[:, :-3] = x.scale
-        x = ops.Q8Rows(q[:, 8:k + 8], s[:, :-3], group)
+        x = ops.Q8Rows(q[:, off:k + off], s[:, :-3], group)
     else:
         xw = torch.full((t, k + 24), float("nan"), dtype=torch.bfloat16, device="cuda")
-        xw[:, 8:k + 8] = x
-        x = xw[:, 8:k + 8]
+        xw[:, off:k + off] = x
+        x = xw[:, off:k + off]
     out = torch.full((t + 1, n + 5), 7.0, dtype=torch.bfloat16, device="cuda")
     y = ops.w4_linear(x, w, bias, out=out[:t, 1:n + 1])
     check(y, x64, w64, group, bias)
     assert bool((out[t] == 7).all()) and bool((out[:, 0] == 7).all()) and bool((out[:, n + 1:] == 7).all())
 
 
-@pytest.mark.parametrize("t", [1, 12, 100])
-def test_every_code_and_column_is_its_own(t):
+@pytest.mark.parametrize("t,n", [(1, 80), (12, 80), (100, 80), (60, 4000), (100, 3000), (264, 1200)])
+def test_every_code_and_column_is_its_own(t, n):
     """One-hot rows read single weights: code, scale and place of each."""
     from lastkv_b200 import ops
 
-    n, k, group = 80, 264, 32
+    k, group = 264, 32
     g = _gen(t, 3)
     codes, scales, w64 = make_weight(n, k, group, g)
     w = ops.w4_pack(codes, scales, group)
@@ -115,12 +118,12 @@ def test_every_code_and_column_is_its_own(t):
     torch.testing.assert_close(ops.w4_linear(q, w), want, rtol=0, atol=0)
 
 
-@pytest.mark.parametrize("t", [2, 40, 130])
-def test_non_finite_rows_stay_their_own(t):
+@pytest.mark.parametrize("t,n", [(2, 192), (40, 192), (130, 192), (60, 3000), (130, 2000), (300, 1000)])
+def test_non_finite_rows_stay_their_own(t, n):
     from lastkv_b200 import ops
 
-    g = _gen(t, 4)
-    codes, scales, w64 = make_weight(192, 512, 128, g)
+    g = _gen(t, 4, n)
+    codes, scales, w64 = make_weight(n, 512, 128, g)
     w = ops.w4_pack(codes, scales, 128)
     x, x64 = make_x(t, 512, 128, False, g)
     x[0, 3] = float("nan")
@@ -135,6 +138,23 @@ def test_non_finite_rows_stay_their_own(t):
     rows = ops.quantize_q8(x)
     y = ops.w4_linear(rows, w)
     assert bool(torch.isnan(y[:2]).all()) and bool(torch.isfinite(y[2:]).all())
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e33])
+@pytest.mark.parametrize("t,n", [(4, 64), (300, 1000)])
+def test_scales_far_from_one(scale, t, n):
+    """int8 rows whose values reach the ends of bf16's range, times weights that bring them back."""
+    from lastkv_b200 import ops
+
+    g = _gen(t, 9)
+    codes, scales, w64 = make_weight(n, 512, 128, g)
+    unit = 1e-4 if scale > 1 else 1.0
+    w = ops.w4_pack(codes, (scales.float() * unit).bfloat16())
+    w64 = (w64 / scales.double().repeat_interleave(128, 1)) * (scales.float() * unit).bfloat16().double().repeat_interleave(128, 1)
+    x, x64 = make_x(t, 512, 128, True, g)
+    x = ops.Q8Rows(x.q, x.scale * scale, 128)
+    x64 = x.q.double() * x.scale.double().repeat_interleave(128, 1)
+    check(ops.w4_linear(x, w), x64, w64, 128)
 
 
 @pytest.mark.parametrize("t", [1, 8, 50, 200])
