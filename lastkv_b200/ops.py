@@ -610,12 +610,9 @@ class Q8Rows(NamedTuple):
 
     @classmethod
     def empty_for(cls, x, cols: int, group: int) -> "Q8Rows":
-        """Rows of ``cols`` columns for the leading dimensions and the device of ``x``."""
-        lead = tuple(x.shape[:-1])
-        rows = lead[0] if len(lead) == 1 else math.prod(lead)
-        pitch = (cols + 15) & -16  # 16-byte rows, whatever the width
-        q = x.new_empty((rows, pitch), dtype=_I8)
-        return cls(q if pitch == cols else q[:, :cols], x.new_empty((rows, -(-cols // group)), dtype=_F32), group, lead)
+        """Rows of ``cols`` columns for the leading dimensions and the device of ``x`` (16-byte
+        rows, whatever the width), to pass as ``out``."""
+        return _q8_out(None, x, math.prod(x.shape[:-1]), cols, group)[0]
 
 
 def _fail(msg: str):
@@ -653,14 +650,20 @@ def _check_q8(r: Q8Rows, what: str) -> None:
         _fail(f"{what}.scale must be CUDA fp32 [rows, ceil(K / group)] rows")
 
 
-def _q8_out(out, x, rows: int, cols: int, group: int) -> Q8Rows:
+def _q8_out(out, x, rows: int, cols: int, group: int):
+    """``out`` checked, or new rows for x: (rows, q's and the scales' row strides)."""
     if out is None:
         _check_group(group)
-        return Q8Rows.empty_for(x, cols, group)
+        pitch, groups = (cols + 15) & -16, -(-cols // group)
+        q = x.new_empty((rows, pitch), dtype=_I8)
+        scale = x.new_empty((rows, groups), dtype=_F32)
+        shape = x.shape
+        lead = (rows,) if len(shape) == 2 else tuple(shape[:-1])
+        return Q8Rows(q if pitch == cols else q[:, :cols], scale, group, lead), pitch, groups
     _check_q8(out, "out")
     if out.group != group or out.q.shape != (rows, cols):
         _fail(f"out must be Q8Rows [{rows}, {cols}] of groups of {group}")
-    return out
+    return out, out.q.stride(0), out.scale.stride(0)
 
 
 @_traced
@@ -676,27 +679,27 @@ def rmsnorm_q8(x, weight, eps: float, residual=None, *, group: int = 128, out: O
     T, H = x2.shape
     if weight.dtype != _BF16 or not weight.is_cuda or weight.numel() != H or not weight.is_contiguous():
         _fail("weight must be CUDA bf16 [H]")
-    rows = _q8_out(out, x, T, H, group)
-    q, scale = rows.q, rows.scale
-    if residual is None:
-        st = _capi.lib().lkv_rmsnorm_q8(x2.data_ptr(), x2.stride(0), None, 0, None, 0, weight.data_ptr(), eps,
-                                        q.data_ptr(), q.stride(0), scale.data_ptr(), scale.stride(0), T, H, group,
-                                        _stream())
-        if st:
-            _capi.check(st, "lkv_rmsnorm_q8")
-        return rows
-    r2 = _in2d(residual, "residual")
-    if residual_out is None:
-        residual_out = x.new_empty(x.shape)
-    ro2 = _out2d(residual_out, H, "residual_out")
-    if r2.shape != x2.shape or ro2.shape != x2.shape:
-        _fail("residual and residual_out must match x")
-    st = _capi.lib().lkv_rmsnorm_q8(x2.data_ptr(), x2.stride(0), r2.data_ptr(), r2.stride(0), ro2.data_ptr(),
-                                    ro2.stride(0), weight.data_ptr(), eps, q.data_ptr(), q.stride(0),
-                                    scale.data_ptr(), scale.stride(0), T, H, group, _stream())
+    rows, q_row, s_row = _q8_out(out, x, T, H, group)
+    r = r_row = ro = ro_row = None
+    if residual is not None:
+        r2 = _in2d(residual, "residual")
+        if r2.shape != x2.shape:
+            _fail("residual must match x")
+        r, r_row = r2.data_ptr(), r2.stride(0)
+        if residual_out is None:
+            residual_out = x.new_empty(x.shape)
+            ro, ro_row = residual_out.data_ptr(), H
+        else:
+            ro2 = _out2d(residual_out, H, "residual_out")
+            if ro2.shape != x2.shape:
+                _fail("residual_out must match x")
+            ro, ro_row = ro2.data_ptr(), ro2.stride(0)
+    st = _capi.lib().lkv_rmsnorm_q8(x2.data_ptr(), x2.stride(0), r, r_row or 0, ro, ro_row or 0, weight.data_ptr(),
+                                    eps, rows.q.data_ptr(), q_row, rows.scale.data_ptr(), s_row, T, H, group,
+                                    _stream())
     if st:
         _capi.check(st, "lkv_rmsnorm_q8")
-    return residual_out, rows
+    return rows if residual is None else (residual_out, rows)
 
 
 @_traced
@@ -706,10 +709,9 @@ def silu_mul_q8(gate_up, *, group: int = 128, out: Optional[Q8Rows] = None) -> Q
     T, F2 = x2.shape
     if F2 % 2:
         _fail("gate_up must be [..., 2F]")
-    rows = _q8_out(out, gate_up, T, F2 // 2, group)
-    q, scale = rows.q, rows.scale
-    st = _capi.lib().lkv_silu_mul_q8(x2.data_ptr(), x2.stride(0), q.data_ptr(), q.stride(0), scale.data_ptr(),
-                                     scale.stride(0), T, F2 // 2, group, _stream())
+    rows, q_row, s_row = _q8_out(out, gate_up, T, F2 // 2, group)
+    st = _capi.lib().lkv_silu_mul_q8(x2.data_ptr(), x2.stride(0), rows.q.data_ptr(), q_row, rows.scale.data_ptr(),
+                                     s_row, T, F2 // 2, group, _stream())
     if st:
         _capi.check(st, "lkv_silu_mul_q8")
     return rows
@@ -720,10 +722,9 @@ def quantize_q8(x, *, group: int = 128, out: Optional[Q8Rows] = None) -> Q8Rows:
     """bf16 [..., K] rows as int8 rows with group scales (lkv_quantize_q8)."""
     x2 = _in2d(x, "x")
     T, K = x2.shape
-    rows = _q8_out(out, x, T, K, group)
-    q, scale = rows.q, rows.scale
-    st = _capi.lib().lkv_quantize_q8(x2.data_ptr(), x2.stride(0), q.data_ptr(), q.stride(0), scale.data_ptr(),
-                                     scale.stride(0), T, K, group, _stream())
+    rows, q_row, s_row = _q8_out(out, x, T, K, group)
+    st = _capi.lib().lkv_quantize_q8(x2.data_ptr(), x2.stride(0), rows.q.data_ptr(), q_row, rows.scale.data_ptr(),
+                                     s_row, T, K, group, _stream())
     if st:
         _capi.check(st, "lkv_quantize_q8")
     return rows
@@ -733,15 +734,18 @@ def quantize_q8(x, *, group: int = 128, out: Optional[Q8Rows] = None) -> Q8Rows:
 def dequantize_q8(rows: Q8Rows, out=None):
     """The bf16 values [..., K] that int8 rows stand for (lkv_dequantize_q8)."""
     _check_q8(rows, "rows")
-    q, scale = rows.q, rows.scale
+    q, scale, group, lead = rows
     T, K = q.shape
     if out is None:
-        out = q.new_empty((T, K) if rows.lead is None else (*rows.lead, K), dtype=_BF16)
-    o2 = _out2d(out, K, "out")
-    if o2.shape[0] != T:
-        _fail("out must have the rows' count")
+        out = o2 = q.new_empty((T, K) if lead is None else (*lead, K), dtype=_BF16)
+        o_row = K
+    else:
+        o2 = _out2d(out, K, "out")
+        if o2.shape[0] != T:
+            _fail("out must have the rows' count")
+        o_row = o2.stride(0)
     st = _capi.lib().lkv_dequantize_q8(q.data_ptr(), q.stride(0), scale.data_ptr(), scale.stride(0), o2.data_ptr(),
-                                       o2.stride(0), T, K, rows.group, _stream())
+                                       o_row, T, K, group, _stream())
     if st:
         _capi.check(st, "lkv_dequantize_q8")
     return out
@@ -799,36 +803,40 @@ def w4_linear(x, weight: W4Weight, bias=None, *, out=None, error_word=None):
     """``x @ w.T (+ bias)`` for a 4-bit weight: x bf16 [..., k] or :class:`Q8Rows` of the
     weight's group; bf16 out [..., n], any number of rows (lkv_w4_linear, lkv_w4_linear_q8)."""
     packed, n, k, group = weight
-    q8 = type(x) is Q8Rows
-    if q8:
+    if type(x) is Q8Rows:
         _check_q8(x, "x")
-        if x.group != group:
-            _fail(f"rows of groups of {x.group} against a weight of groups of {group}")
-        x2 = x.q
-        lead = x.lead
+        x2, scale, x_group, lead = x
+        if x_group != group:
+            _fail(f"rows of groups of {x_group} against a weight of groups of {group}")
     else:
-        x2 = _in2d(x, "x")
-        lead = None if x2 is x else x.shape[:-1]
+        x2, scale, lead = _in2d(x, "x"), None, None
+        if x2 is not x:
+            lead = x.shape[:-1]
     T, cols = x2.shape
     if cols != k:
         _fail(f"x has {cols} columns, the weight {k}")
     if out is None:
-        out = x2.new_empty((T, n) if lead is None else (*lead, n), dtype=_BF16)
-    o2 = _out2d(out, n, "out")
-    if o2.shape[0] != T:
-        _fail("out must have the rows of x")
-    if bias is not None and not (bias.dtype == _BF16 and bias.is_contiguous() and bias.numel() == n and bias.is_cuda):
-        _fail("bias must be CUDA bf16 [n]")
-    if q8:
-        scale = x.scale
-        st = _capi.lib().lkv_w4_linear_q8(x2.data_ptr(), x2.stride(0), scale.data_ptr(), scale.stride(0),
-                                          packed.data_ptr(), _ptr(bias), o2.data_ptr(), o2.stride(0), T, n, k, group,
-                                          _ptr(error_word), _stream())
+        out = o2 = x2.new_empty((T, n) if lead is None else (*lead, n), dtype=_BF16)
+        o_row = n
     else:
-        st = _capi.lib().lkv_w4_linear(x2.data_ptr(), x2.stride(0), packed.data_ptr(), _ptr(bias), o2.data_ptr(),
-                                       o2.stride(0), T, n, k, group, _ptr(error_word), _stream())
+        o2 = _out2d(out, n, "out")
+        if o2.shape[0] != T:
+            _fail("out must have the rows of x")
+        o_row = o2.stride(0)
+    b = None
+    if bias is not None:
+        if bias.dtype != _BF16 or not bias.is_cuda or bias.numel() != n or not bias.is_contiguous():
+            _fail("bias must be CUDA bf16 [n]")
+        b = bias.data_ptr()
+    err = None if error_word is None else error_word.data_ptr()
+    if scale is not None:
+        st = _capi.lib().lkv_w4_linear_q8(x2.data_ptr(), x2.stride(0), scale.data_ptr(), scale.stride(0),
+                                          packed.data_ptr(), b, o2.data_ptr(), o_row, T, n, k, group, err, _stream())
+    else:
+        st = _capi.lib().lkv_w4_linear(x2.data_ptr(), x2.stride(0), packed.data_ptr(), b, o2.data_ptr(), o_row, T, n,
+                                       k, group, err, _stream())
     if st:
-        _capi.check(st, "lkv_w4_linear_q8" if q8 else "lkv_w4_linear")
+        _capi.check(st, "lkv_w4_linear" if scale is None else "lkv_w4_linear_q8")
     return out
 
 
