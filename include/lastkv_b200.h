@@ -455,9 +455,12 @@ int lkv_dequantize_q8(const int8_t* q, int64_t q_row, const float* scale, int64_
  *                 and 2i + 1 in the high half; scales bf16 [n, >= ceil(k / group)];
  *                 packed: lkv_w4_bytes bytes, 16-byte aligned, laid out once per weight
  * n >= 1 any; k a multiple of 8 (the last group may be short); group 32, 64 or
- * 128; any number of tokens.  x rows 16-byte (bf16) or 8-byte (int8) aligned,
+ * 128; tokens 0 .. 2^20 - 1.  x rows 16-byte (bf16) or 8-byte (int8) aligned,
  * strides in elements; bias bf16 [n] or NULL.  No workspace; one launch;
- * sums in a fixed order (deterministic). */
+ * sums in a fixed order (deterministic).  error_word (NULL or 4 words) records
+ * a pipeline wait that gave up.  The packed weight is read before the launch's
+ * dependency wait (programmatic dependent launch): write it with lkv_w4_pack, or
+ * with at least one plain kernel or copy after its last dependent launch. */
 size_t lkv_w4_bytes(int64_t n, int64_t k, int group);
 int lkv_w4_pack(const uint8_t* codes, int64_t codes_row, const void* scales, int64_t scales_row, int64_t n,
                 int64_t k, int group, void* packed, void* stream);

@@ -21,7 +21,7 @@ INCLUDE = os.path.join(ROOT, "include")
 LIBDIR = os.path.join(PKG, "_lib")
 LIB = os.path.join(LIBDIR, "liblastkv_b200.so")
 SOURCES = ["capi.cu", "decode.cu", "append.cu", "prefill.cu", "decode_noalloc.cu", "dense.cu", "gemm.cu", "cp_combine.cu",
-           "fp32.cu", "rows_q8.cu", "w4.cu", "w4_tile.cu", "w4_wide.cu", "plan.cu"]
+           "fp32.cu", "rows_q8.cu", "w4.cu", "w4_tile.cu", "plan.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -46,7 +46,6 @@ __device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {
 // More tokens than the skinny kernel takes well: tcgen05 tiles (w4_tile.cu).  LKV_ERR_UNSUPPORTED
 // where the rows' alignment rules a TMA copy out.
 bool w4_tile_aligned(const W4Args& a);
-int w4_tile(const W4Args& a, int sms, cudaStream_t stream);  // int8 rows
-int w4_wide(const W4Args& a, int sms, cudaStream_t stream);  // bf16 rows (w4_wide.cu)
+int w4_tile(const W4Args& a, int sms, cudaStream_t stream);
 
 }  // namespace lkv

@@ -11,16 +11,17 @@
 // while the tensor core sums the next groups into the other buffers.  So
 // int8 x 4-bit group sums are exact and no weight is rounded, at the price of reading
 // 128 x TN sums from TMEM per group, which is what bounds it: 2048 tokens x 28672 x 4096 in
-// groups of 128 take 457 us with bf16 rows (1053 TFLOP/s, 0.63 of the measured bf16 peak) and
-// 565 us with int8 rows, whose sums need a second multiply-add each; in groups of 64 and 32
-// (4096 x 4096) 72 -> 102 -> 167 us and 90 -> 151 -> 274 us.  Four drain warpgroups (567 us),
-// a second expanding one (narrow tiles 65 against 58 us), 32-column loads (482 us) and waits
-// with a suspend hint (482 / 580 us) were no faster.
+// groups of 128 take 457 us with bf16 rows (1052 TFLOP/s, 0.63 of the measured bf16 peak) and
+// 562 us with int8 rows, whose sums need a second multiply-add each; in groups of 64 and 32
+// (4096 x 4096) 70 -> 102 -> 167 us and 90 -> 151 -> 274 us.  Weights s * c rounded to bf16
+// need no group sums (376 and 59 us), but are off by up to 2^-8 each.  Four drain warpgroups
+// (567 us), a second expanding one (narrow tiles 65 against 58 us), 32-column loads (482 us)
+// and waits with a suspend hint (482 / 580 us) were no faster.
 //
 // Roles of the 512 threads (one CTA per SM, persistent over the tiles):
-//   warp 0  rows by TMA                         warp 1     tcgen05.mma issue, TMEM
-//   warp 2  the tokens' scales (int8 rows)      warp 3     codes, weight scales by bulk copies
-//   warps 4-7    codes -> A tiles               warps 8-15 drain, epilogue
+//   warp 0  rows by TMA                     warp 1     tcgen05.mma issue, TMEM
+//   warp 2  the tokens' scales (int8 rows)  warp 3     codes, weight scales by bulk copies
+//   warps 4-7  codes -> A tiles, weight scales -> their own slots     warps 8-15 drain, epilogue
 // Where the tiles alone do not fill the GPU, k is split over the CTAs of a cluster, whose
 // partial tiles meet in shared memory (added in split order).
 

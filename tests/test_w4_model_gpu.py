@@ -75,6 +75,20 @@ def test_model_matches_its_four_bit_values(activations, group, bias):
     assert off < LIMIT[activations]
 
 
+@pytest.mark.parametrize("activations", ["bf16", "int8"])
+def test_long_spans(activations):
+    """Long spans run on bf16 activations; the compared model has the weights rounded to bf16."""
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    tokens = torch.randint(0, 512, (2, 600), generator=gen, device="cuda")
+    segments = [590, 10]
+    model = build(chunk_size=512)
+    got = run(model.quantize_projections_(64, activations), tokens, segments)
+    want = run(four_bit_values(build(chunk_size=512), 64), tokens, segments)
+    off = float((got[:, :512] - want[:, :512]).norm() / want[:, :512].norm())
+    print(f"{activations}: {off:.4f} of the logits' norm")
+    assert off < LIMIT["bf16"]
+
+
 def test_release_frees_the_weights_and_changes_nothing():
     gen = torch.Generator(device="cuda").manual_seed(2)
     tokens = torch.randint(0, 512, (1, 40), generator=gen, device="cuda")
