@@ -91,6 +91,10 @@ struct NormQ8Params {
 // 1536 threads per SM): the next row's loads are in flight while a row is reduced and stored.
 // The weight stays in registers, loaded before the previous kernel has finished.  (Rows of
 // more than 16384 columns, V = 8, leave no registers for either.)
+// Bound by HBM for long rows, by the launch and one trip to memory for a few: with a residual,
+// 1 x 4096 1.8 us; 2048 x 4096 17.3 us (3.4 TB/s, 0.52 of the measured copy), 2048 x 8192 28.0,
+// 2048 x 16384 46.1 us (0.78), 512 x 32768 41.9 us.  A CTA per row instead of persistent ones:
+// 20.1, 43.4 and 62.8 us.
 template <int V, int THREADS>
 __global__ void __launch_bounds__(THREADS) rmsnorm_q8_kernel(const NormQ8Params p) {
   pdl_launch_dependents();
@@ -168,9 +172,13 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_q8_kernel(const NormQ8Params 
   }
 }
 
-// One warp per 256 columns of a row (whole groups), one 8-column vector per lane; with many
-// rows U such chunks' loads are in flight per warp.
-template <bool SILU, int U>
+// One warp per 256 columns of a row (whole groups), one 8-column vector per lane.  One pass;
+// SiLU 8 x 14336 2.2 us, 2048 x 14336 43 us (3.4 TB/s; issue slots: about 250 instructions per
+// 256 columns), plain 2048 x 4096 9.9 us (2.6 TB/s), 1000 x 1544 in groups of 32 3.1 us.  Four
+// chunks' loads in flight per warp: 42, 9.5 and 5.0 us, SiLU 256 x 14336 8.4 against 6.7 us.
+// __fdividef: the quotient's last bits are far below the int8 step (a denominator past 2^126
+// gives 0 for |silu| < 1e-35).
+template <bool SILU>
 __global__ void __launch_bounds__(256)
     rows_q8_kernel(const __nv_bfloat16* __restrict__ x, int64_t x_row, int8_t* __restrict__ q, int64_t q_row,
                    float* __restrict__ scale, int64_t scale_row, int64_t rows, int cols, int group) {
@@ -179,37 +187,29 @@ __global__ void __launch_bounds__(256)
   const int lane = threadIdx.x & 31, lanes = group / kVec, nvec = cols / kVec;
   const uint32_t chunks = (cols + 255) / 256, total = (uint32_t)rows * chunks;
   const uint32_t stride = gridDim.x * (blockDim.x >> 5);
-  for (uint32_t i0 = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i0 < total; i0 += U * stride) {
-    uint4 g[U], up[U];
+  for (uint32_t i = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < total; i += stride) {
+    const uint32_t row = i / chunks, c = (i - row * chunks) * 32 + lane;
+    const uint4* src = reinterpret_cast<const uint4*>(x + (int64_t)row * x_row);
+    const bool in = c < nvec;
+    const uint4 zero = make_uint4(0, 0, 0, 0), g = in ? src[c] : zero, up = SILU && in ? src[nvec + c] : zero;
+    float y[kVec], s;
+    unpack8(g, y);
+    if (SILU) {
+      float u[kVec];
+      unpack8(up, u);
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const uint32_t i = i0 + k * stride, row = i / chunks, c = (i - row * chunks) * 32 + lane;
-      const uint4* src = reinterpret_cast<const uint4*>(x + (int64_t)row * x_row);
-      const bool in = i < total && c < nvec;
-      g[k] = in ? src[c] : make_uint4(0, 0, 0, 0);
-      if (SILU) up[k] = in ? src[nvec + c] : make_uint4(0, 0, 0, 0);
+      for (int j = 0; j < kVec; ++j) y[j] = __fdividef(y[j], 1.0f + expf(-y[j])) * u[j];
     }
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const uint32_t i = i0 + k * stride, row = i / chunks, c = (i - row * chunks) * 32 + lane;
-      float y[kVec], s;
-      unpack8(g[k], y);
-      if (SILU) {
-        float u[kVec];
-        unpack8(up[k], u);
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) y[j] = __fdividef(y[j], 1.0f + expf(-y[j])) * u[j];
-      }
-      const uint2 v = quantise8(y, lanes, &s);
-      if (i < total && c < nvec) {
-        *reinterpret_cast<uint2*>(q + row * q_row + (int64_t)c * kVec) = v;
-        if ((c & (lanes - 1)) == 0) scale[row * scale_row + c / lanes] = s;
-      }
+    const uint2 v = quantise8(y, lanes, &s);
+    if (in) {
+      *reinterpret_cast<uint2*>(q + row * q_row + (int64_t)c * kVec) = v;
+      if ((c & (lanes - 1)) == 0) scale[row * scale_row + c / lanes] = s;
     }
   }
 }
 
-template <int U>
+// One 8-column vector per thread: 2048 x 4096 7.5 us (3.4 TB/s), 1000 x 1544 2.8 us; four
+// vectors in flight 8.5 and 4.1 us.
 __global__ void __launch_bounds__(256)
     dequantize_q8_kernel(const int8_t* __restrict__ q, int64_t q_row, const float* __restrict__ scale,
                          int64_t scale_row, __nv_bfloat16* __restrict__ out, int64_t out_row, int64_t rows, int cols,
@@ -217,29 +217,19 @@ __global__ void __launch_bounds__(256)
   pdl_launch_dependents();
   pdl_wait();
   const uint32_t nvec = cols / kVec, total = (uint32_t)rows * nvec, stride = gridDim.x * blockDim.x;
-  for (uint32_t i0 = blockIdx.x * blockDim.x + threadIdx.x; i0 < total; i0 += U * stride) {
-    uint2 v[U];
-    float s[U];
+  for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < total; i += stride) {
+    const uint32_t row = i / nvec, c = (i - row * nvec) * kVec;
+    const uint2 v = *reinterpret_cast<const uint2*>(q + row * q_row + c);
+    const float s = scale[row * scale_row + c / group];
+    const uint32_t lo = v.x ^ 0x80808080u, hi = v.y ^ 0x80808080u;  // q + 128 as a byte
+    float f[kVec];
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const uint32_t i = i0 + k * stride, row = i / nvec, c = (i - row * nvec) * kVec;
-      v[k] = i < total ? *reinterpret_cast<const uint2*>(q + row * q_row + c) : make_uint2(0, 0);
-      s[k] = i < total ? scale[row * scale_row + c / group] : 0.f;
+    for (int j = 0; j < 4; ++j) {  // the byte under the exponent of 2^23 is 2^23 + q + 128
+      f[j] = (__uint_as_float(__byte_perm(lo, 0x4b000000u, 0x7440 | j)) - 8388736.0f) * s;
+      f[j + 4] = (__uint_as_float(__byte_perm(hi, 0x4b000000u, 0x7440 | j)) - 8388736.0f) * s;
     }
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const uint32_t i = i0 + k * stride, row = i / nvec, c = (i - row * nvec) * kVec;
-      if (i >= total) break;
-      const uint32_t lo = v[k].x ^ 0x80808080u, hi = v[k].y ^ 0x80808080u;  // q + 128 as a byte
-      float f[kVec];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {  // the byte under the exponent of 2^23 is 2^23 + q + 128
-        f[j] = (__uint_as_float(__byte_perm(lo, 0x4b000000u, 0x7440 | j)) - 8388736.0f) * s[k];
-        f[j + 4] = (__uint_as_float(__byte_perm(hi, 0x4b000000u, 0x7440 | j)) - 8388736.0f) * s[k];
-      }
-      *reinterpret_cast<uint4*>(out + row * out_row + c) =
-          make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
-    }
+    *reinterpret_cast<uint4*>(out + row * out_row + c) =
+        make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
   }
 }
 
@@ -308,11 +298,7 @@ int rows_q8(const void* x, int64_t x_row, int silu, const Q8RowsArgs& a, cudaStr
   if (a.rows == 0) return LKV_OK;
   if (!rows_ok(x, a.rows, x_row, silu ? 2 * (int64_t)a.cols : a.cols, 2, 16) || !q8_ok(a)) return LKV_ERR_INVALID_ARGUMENT;
   const int64_t warps = a.rows * ((a.cols + 255) / 256);
-  const bool many = warps > 148 * 64;  // more than the GPU runs at once
-  const int blocks = row_blocks(many ? (warps + 3) / 4 : warps);
-  return launch_pdl(silu ? (many ? rows_q8_kernel<true, 4> : rows_q8_kernel<true, 1>)
-                         : (many ? rows_q8_kernel<false, 4> : rows_q8_kernel<false, 1>),
-                    dim3(blocks), dim3(256), 0, stream,
+  return launch_pdl(silu ? rows_q8_kernel<true> : rows_q8_kernel<false>, dim3(row_blocks(warps)), dim3(256), 0, stream,
                     static_cast<const __nv_bfloat16*>(x), x_row, a.q, a.q_row, a.scale, a.scale_row, a.rows, a.cols,
                     a.group) == cudaSuccess
              ? LKV_OK
@@ -325,11 +311,9 @@ int dequantize_q8(const Q8RowsArgs& a, void* out, int64_t out_row, cudaStream_t 
   if (a.rows == 0) return LKV_OK;
   if (!q8_ok(a) || !rows_ok(out, a.rows, out_row, a.cols, 2, 16)) return LKV_ERR_INVALID_ARGUMENT;
   const int64_t warps = (a.rows * (a.cols / kVec) + 31) / 32;
-  const bool many = warps > 148 * 64;
-  return launch_pdl(many ? dequantize_q8_kernel<4> : dequantize_q8_kernel<1>,
-                    dim3(row_blocks(many ? (warps + 3) / 4 : warps)), dim3(256), 0, stream, static_cast<const int8_t*>(a.q),
-                    a.q_row, static_cast<const float*>(a.scale), a.scale_row, static_cast<__nv_bfloat16*>(out),
-                    out_row, a.rows, a.cols, a.group) == cudaSuccess
+  return launch_pdl(dequantize_q8_kernel, dim3(row_blocks(warps)), dim3(256), 0, stream,
+                    static_cast<const int8_t*>(a.q), a.q_row, static_cast<const float*>(a.scale), a.scale_row,
+                    static_cast<__nv_bfloat16*>(out), out_row, a.rows, a.cols, a.group) == cudaSuccess
              ? LKV_OK
              : LKV_ERR_CUDA;
 }

@@ -45,6 +45,7 @@ constexpr int kThreads = 256 + 128 * kDrainWgs;
 constexpr int kKernelId = 13;
 constexpr int kAStage = kM * 128;
 constexpr int kMaxSplits = 8;
+constexpr int kPartRow = kM + 4;  // of a partial tile: 4 keeps the stores of neighbouring tokens off each other's banks
 
 struct TileParams {
   const uint8_t* packed;
@@ -519,15 +520,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
       } else {
         // one tile per cluster: every stage has been consumed, their memory takes the partial [token][row]
-        float* part = reinterpret_cast<float*>(smem) + (wg * kCols + 2 * q) * kM + sub * kTileRows + g;
+        float* part = reinterpret_cast<float*>(smem) + (wg * kCols + 2 * q) * kPartRow + sub * kTileRows + g;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int c = 0; c < kCols / 8; ++c)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              part[8 * c * kM + 16 * h + 8 * e] = acc[h][c][e].x;
-              part[(8 * c + 1) * kM + 16 * h + 8 * e] = acc[h][c][e].y;
+              part[8 * c * kPartRow + 16 * h + 8 * e] = acc[h][c][e].x;
+              part[(8 * c + 1) * kPartRow + 16 * h + 8 * e] = acc[h][c][e].y;
             }
       }
     }
@@ -539,19 +540,38 @@ __global__ void __launch_bounds__(kThreads, 1)
     cluster_sync_all();  // every split has published its partial
     const int tile = blockIdx.x;
     const int tok0 = tile % p.tok_tiles * TN, row0 = tile / p.tok_tiles * kM;
-    const int live = min(TN, p.tokens - tok0) * kM;
+    const bool words = ((reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)(p.y_row * 2)) & 3) == 0;
     const uint32_t base = smem_u32(smem);
-    for (int i = (int)cluster_rank() * kThreads + threadIdx.x; i < live; i += p.splits * kThreads) {
-      const int r = row0 + i % kM;
-      float v[kMaxSplits];
+    // A warp takes a token, a lane four rows of it: 16-byte loads, the splits' in flight together.
+    // (4-byte loads: 256 bf16 rows x 6144 x 4096, two splits, 29.5 against 23.4 us.)
+    constexpr int kWarps = kThreads / 32;
+    const int tokens = min(TN, p.tokens - tok0), r = row0 + 4 * lane;
+#pragma unroll 1
+    for (int t = (int)cluster_rank() * kWarps + warp; t < tokens; t += p.splits * kWarps) {
+      const uint32_t at = (uint32_t)(t * kPartRow + 4 * lane) * 4;
+      float4 v[kMaxSplits];
 #pragma unroll
-      for (int s = 0; s < kMaxSplits; ++s) v[s] = s < p.splits ? dsmem_ld(dsmem_map(base, s) + i * 4) : 0.f;
-      float sum = 0.f;
+      for (int s = 0; s < kMaxSplits; ++s)
+        v[s] = s < p.splits ? dsmem_ld4(dsmem_map(base, s) + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+      float sum[4] = {};
 #pragma unroll
-      for (int s = 0; s < kMaxSplits; ++s) sum += v[s];
-      if (r < p.n) {
-        if (p.bias) sum += __bfloat162float(p.bias[r]);
-        p.y[(int64_t)(tok0 + i / kM) * p.y_row + r] = __float2bfloat16_rn(sum);
+      for (int s = 0; s < kMaxSplits; ++s) {
+        sum[0] += v[s].x;
+        sum[1] += v[s].y;
+        sum[2] += v[s].z;
+        sum[3] += v[s].w;
+      }
+      __nv_bfloat16* y = p.y + (int64_t)(tok0 + t) * p.y_row + r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (p.bias && r + e < p.n) sum[e] += __bfloat162float(p.bias[r + e]);
+      if (words && r + 3 < p.n) {
+        reinterpret_cast<uint32_t*>(y)[0] = pack_bf16(sum[0], sum[1]);
+        reinterpret_cast<uint32_t*>(y)[1] = pack_bf16(sum[2], sum[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (r + e < p.n) y[e] = __float2bfloat16_rn(sum[e]);
       }
     }
     cluster_sync_all();  // the partials stay readable until every CTA has read them
@@ -567,6 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <bool INT8, int G, int TN>
 int launch(const CUtensorMap& map, const TileParams& p, int sms, cudaStream_t stream) {
   static_assert(smem_bytes<INT8, G, TN>() <= 227 * 1024, "shared memory of a CTA");
+  static_assert(TN * kPartRow * 4 <= ring_bytes<G, TN>(), "partial tile");
   static std::once_flag once[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return LKV_ERR_CUDA;
@@ -614,14 +635,27 @@ int w4_tile(const W4Args& a, int sms, cudaStream_t stream) {
   p.kblocks = (int)((a.k + kTileK - 1) / kTileK);
   p.row_blocks = (int)((a.n + kTileRows - 1) / kTileRows);
   p.err = a.error_word;
-  const int tn = a.tokens <= 64 ? 64 : a.tokens <= 128 ? 128 : 256;
-  p.tok_tiles = (int)((a.tokens + tn - 1) / tn);
-  const int64_t tiles = (a.n + kM - 1) / kM * p.tok_tiles;
-  if (tiles > 0x7fffffff) return LKV_ERR_UNSUPPORTED;
-  p.tiles = (int)tiles;
+  const int64_t row_tiles = (a.n + kM - 1) / kM;
+  auto tiles = [&](int tn) { return row_tiles * ((a.tokens + tn - 1) / tn); };
   // a power of two of splits, while every CTA of every cluster still has an SM and two blocks of k
-  p.splits = 1;
-  while (p.splits < kMaxSplits && p.tiles * p.splits * 2 <= sms && p.kblocks >= p.splits * 4) p.splits *= 2;
+  auto splits = [&](int tn) {
+    int s = 1;
+    while (s < kMaxSplits && tiles(tn) * s * 2 <= sms && p.kblocks >= s * 4) s *= 2;
+    return s;
+  };
+  // Tokens of a tile: 256 take 1.64 (int8) or 1.23 (bf16) times a 128-token tile's time, which the
+  // rounds of tiles over the SMs may cost.  256 against 128, int8 / bf16 rows: 1024 tokens x 28672
+  // x 4096 (7 against 13 rounds) 302 / 237 against 344 / 357 us, x 6144 (2, 3) 89 / 70 against
+  // 82 / 87 us; 384 tokens x 6144 (1, 1) 46 / 37 against 29 / 32 us, x 28672 (4, 5) 177 / 136
+  // against 136 / 143 us.
+  auto rounds = [&](int tn) { return (double)((tiles(tn) + sms - 1) / sms) / splits(tn); };
+  const int tn = a.tokens <= 64                                                         ? 64
+                 : a.tokens <= 128 || rounds(128) < rounds(256) * (int8 ? 1.64 : 1.23) ? 128
+                                                                                        : 256;
+  if (tiles(tn) > 0x7fffffff) return LKV_ERR_UNSUPPORTED;
+  p.tok_tiles = (int)((a.tokens + tn - 1) / tn);
+  p.tiles = (int)tiles(tn);
+  p.splits = splits(tn);
   CUtensorMap map;
   const int st = int8 ? make_matrix_tensor_map_s8(&map, a.x, a.tokens, a.k, a.x_row, tn)
                       : make_matrix_tensor_map(&map, a.x, a.tokens, a.k, a.x_row, tn);
