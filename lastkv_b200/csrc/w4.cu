@@ -72,6 +72,7 @@ struct SkinnyParams {
   int64_t y_row;
   int tokens, n, k, kblocks, splits, tiles;
   int* err;
+  Never never;
 };
 
 __device__ __forceinline__ void mma_s8_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -92,10 +93,17 @@ struct WeightBlock {
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) w[r][j] = *reinterpret_cast<const uint4*>(block + r * 1024 + j * 512 + lane * 16);
+      for (int j = 0; j < 2; ++j) w[r][j] = ld_shared16(block + r * 1024 + j * 512 + lane * 16);
 #pragma unroll
     for (int g = 0; g < kTileK / G; ++g)
-      s[g] = *reinterpret_cast<const uint2*>(block + kCodeBytes + g * 64 + (lane >> 2) * 8);
+      s[g] = ld_shared8(block + kCodeBytes + g * 64 + (lane >> 2) * 8);
+  }
+  // of every load's result
+  __device__ __forceinline__ uint32_t mix() const {
+    uint32_t v = w[0][0].x ^ w[0][1].x ^ w[1][0].x ^ w[1][1].x;
+#pragma unroll
+    for (int g = 0; g < kTileK / G; ++g) v ^= s[g].x;
+    return v;
   }
   __device__ __forceinline__ uint32_t word(int r, int step, int half) const {
     const uint4& v = w[r][step >> 1];
@@ -283,7 +291,8 @@ __global__ void __launch_bounds__(W * 32, 16 / W) w4_skinny_kernel(const SkinnyP
       ok = ok && mbar_wait(&sh->full[warp][slot], phase);
       WeightBlock<G> w;
       w.read(sh->ring[warp][slot], lane);
-      __syncwarp();  // the block is in registers: its slot may be filled again
+      // every lane's block is in registers: its slot may be filled again
+      ok = !__any_sync(0xffffffffu, !ok || p.never.is(w.mix()));
       if (ok) load(slot);
       if (++slot == kDepth) {
         slot = 0;

@@ -32,6 +32,16 @@ __host__ __device__ __forceinline__ int64_t block_offset(int64_t rb, int64_t kb,
   return (first * kblocks + kb * wide + (rb - first)) * block_bytes(group);
 }
 
+// A condition that no value meets, which the compiler does not know.  A slot of shared memory
+// that bulk copies refill may be released only once the values read from it have arrived in
+// registers.  An mbarrier arrival or __syncwarp behind the loads does not see to that: loads
+// whose results are used later were overtaken by the next copy, 64-byte pieces of which then
+// stood in the block.  A vote on the loaded values waits for them in every lane.
+struct Never {
+  uint32_t a = 0, b = 1;
+  __device__ __forceinline__ bool is(uint32_t v) const { return v == a && v == b; }
+};
+
 // Two of a word's codes (I = 0: columns 0, 2; 1: 4, 6; 2: 1, 3; 3: 5, 7) as exact bf16:
 // 128 + (c + 8) by its mantissa bits, minus 136.
 template <int I>

@@ -56,6 +56,7 @@ struct TileParams {
   int64_t y_row;
   int tokens, n, k, kblocks, row_blocks, tok_tiles, tiles, splits;
   int* err;
+  Never never;
 };
 
 // Ring depths: A stages (16 KB, filled in the CTA), B stages (TN x 128 bytes, from L2).
@@ -360,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint8_t* src = codes + (b * kQuarters + w) * block_bytes(G);
         // the row block's scales, for the drain
         for (int i = lane; i < kGpb * 16; i += 32)
-          reinterpret_cast<uint32_t*>(sh->ws[e][w])[i] = reinterpret_cast<const uint32_t*>(src + kCodeBytes)[i];
+          reinterpret_cast<uint32_t*>(sh->ws[e][w])[i] = ld_shared4(src + kCodeBytes + 4 * i);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->ws_full[e]);
 #pragma unroll
@@ -370,12 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int q = 0; q < kN; ++q) {
             // warp w expands row block w: int8 pieces (r, j), bf16 pieces r, j from the stage
             const int r = INT8 ? q >> 1 : q, j = INT8 ? q & 1 : i;
-            v[q] = w < quarters ? *reinterpret_cast<const uint4*>(src + r * 1024 + j * 512 + (4 * g + t) * 16)
-                               : make_uint4(0, 0, 0, 0);
-          }
-          if (i == kSpb - 1) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh->c_empty[b]);
+            v[q] = w < quarters ? ld_shared16(src + r * 1024 + j * 512 + (4 * g + t) * 16) : make_uint4(0, 0, 0, 0);
           }
           const uint32_t it = blk * kSpb + i;
           const int s = it % SA;
@@ -404,7 +400,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sh->a_full[s]);
+          if (lane == 0) {
+            mbar_arrive(&sh->a_full[s]);
+            // Not before the stores above, which need the loaded values: an arrival right after
+            // the loads lets the next copy overwrite the block before they have read it.
+            if (i == kSpb - 1) mbar_arrive(&sh->c_empty[b]);
+          }
         }
       }
     }
@@ -438,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int gi = 0; gi < kGpb; ++gi, ++gt) {
           const int buf = grp % ND;
           // scales of rows 16 h + 8 e + g at 2 (4 g + 2 h + e); int8 codes stand at 16 c, the tokens' scales at 2^-20
-          const uint2 w4 = live ? *reinterpret_cast<const uint2*>(&sh->ws[b][sub][gi * 64 + g * 8]) : make_uint2(0, 0);
+          const uint2 w4 = live ? ld_shared8(&sh->ws[b][sub][gi * 64 + g * 8]) : make_uint2(0, 0);
           constexpr float kUnit = INT8 ? 0x1p16f : 1.f;
           const float ws[2][2] = {{bf16_lo(w4.x) * kUnit, bf16_hi(w4.x) * kUnit},
                                   {bf16_lo(w4.y) * kUnit, bf16_hi(w4.y) * kUnit}};
@@ -464,8 +465,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c = 0; c < 2; ++c) {
               float2 x, y;
               if (INT8) {
-                x = *reinterpret_cast<const float2*>(xs + c0 + 8 * c);
-                y = *reinterpret_cast<const float2*>(xs + TN + c0 + 8 * c);
+                const uint2 ux = ld_shared8(xs + c0 + 8 * c), uy = ld_shared8(xs + TN + c0 + 8 * c);
+                x = make_float2(__uint_as_float(ux.x), __uint_as_float(ux.y));
+                y = make_float2(__uint_as_float(uy.x), __uint_as_float(uy.y));
               }
 #pragma unroll
               for (int h = 0; h < 2; ++h)
@@ -484,8 +486,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           ++grp;
           if (INT8 && (gt % kXsGroups == kXsGroups - 1 || gt == nkb * kGpb - 1)) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh->xs_empty[slot & 1]);
+            // the vote needs the last sums, and so the scales, in registers (see Never)
+            if (!__any_sync(0xffffffffu, p.never.is(__float_as_uint(acc[1][kCols / 8 - 1][1].x))) && lane == 0)
+              mbar_arrive(&sh->xs_empty[slot & 1]);
             ++slot;
           }
         }

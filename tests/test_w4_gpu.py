@@ -225,3 +225,23 @@ def test_no_rows_and_refusals():
                  lambda: ops.w4_quantize(codes)):
         with pytest.raises(RMarinBackendContractError):
             call()
+
+
+@pytest.mark.parametrize("t,n,k,group,int8", [
+    (20, 10075, 9992, 128, False), (32, 28672, 4096, 128, False), (45, 1508, 8400, 64, False), (14, 18754, 11568, 32, True),
+    (8, 28672, 4096, 128, True), (141, 24819, 1032, 128, True), (141, 24819, 1032, 32, True), (256, 6144, 4096, 32, True),
+    (141, 24819, 1032, 64, False), (300, 6144, 4096, 128, False), (300, 28672, 4096, 128, True)])
+def test_many_blocks_in_flight(t, n, k, group, int8):
+    """Weights past the rings' depth, over and over: each call gives the first one's bits, and those are right."""
+    from lastkv_b200 import ops
+
+    g = _gen(t, n, k, group)
+    codes, scales, w64 = make_weight(n, k, group, g)
+    x, x64 = make_x(t, k, group, int8, g)
+    w = ops.w4_pack(codes, scales, group)
+    err = torch.zeros(4, dtype=torch.int32, device="cuda")
+    first = ops.w4_linear(x, w, error_word=err)
+    check(first, x64, w64, group)
+    for _ in range(60):
+        assert torch.equal(ops.w4_linear(x, w, error_word=err), first)
+    assert err.tolist() == [0, 0, 0, 0]
