@@ -194,10 +194,11 @@ __device__ __forceinline__ void add_group(float (&acc)[2][NT][4], const WeightBl
 // splits' sums (a cluster's CTAs, then one tile per CTA) over the cluster's, always in the
 // same order.  Without splits the CTAs are persistent over the row tiles.  Tokens past the
 // last read the last one's row (their sums are not stored).
-// Bound by the expansion of the codes (issue slots) and, for small weights, by the launch and
-// the memory's latency, before HBM.  8 tokens, groups of 128, int8 / bf16 rows: 28672 x 4096
-// 14.0 / 19.9 us (4.3 / 3.1 TB/s of 6.5), 4096 x 14336 8.1 / 10.5 us, 4096 x 4096 3.6 / 4.5 us;
-// 1 token, 6144 x 4096 3.9 / 5.8 us.  Loads into registers instead of the ring: 15.9 / 23.3 us
+// What it waits for, before HBM, is the expansion of the codes and the products' dependent
+// steps (issue slots half used, four warps a scheduler) and, for small weights, the launch and
+// the memory's latency.  8 tokens, groups of 128, int8 / bf16 rows: 28672 x 4096 14.6 / 20.2 us
+// (4.2 / 3.0 TB/s of the 6.5 measured), 4096 x 14336 8.0 / 10.3 us, 4096 x 4096 3.6 / 4.3 us;
+// 1 token, 6144 x 4096 4.0 / 5.9 us.  Loads into registers instead of the ring: 15.9 / 23.3 us
 // for the first.
 constexpr int kDepth = 3;
 constexpr int kSkinnyKernelId = 14;
@@ -417,9 +418,9 @@ int device_sms(int* sms) {
 
 // The streaming kernel reads the weight again for every 16 tokens (from L2), so it takes up to
 // 32 tokens, and more where its CTAs still fit the GPU at once; the tcgen05 kernel the rest.
-// int8 / bf16 rows, streaming against tcgen05: 32 tokens 4096 x 4096 6.16 / 7.80 against 9.04 /
-// 11.5 us, 28672 x 4096 35.4 / 48.3 against 33.8 / 52.0 us; 64 tokens 1003 x 1544 2.95 / 3.34
-// against 7.28 / 7.32 us, 4096 x 4096 (512 CTAs) 10.9 / 14.3 against 10.2 / 12.5 us.
+// int8 / bf16 rows, streaming against tcgen05: 32 tokens 4096 x 4096 6.1 / 7.8 against 9.5 /
+// 11.6 us, 28672 x 4096 34.7 / 48.7 against 36.9 / 53.0 us; 64 tokens 1003 x 1544 2.7 / 3.3
+// against 5.9 / 6.9 us, 4096 x 4096 (512 CTAs) 10.9 / 14.3 against 9.9 / 12.0 us.
 bool few_tokens(const W4Args& a, int sms) {
   return a.tokens <= 32 || (a.n + kTileRows - 1) / kTileRows * ((a.tokens + 15) / 16) <= 2 * (int64_t)sms;
 }

@@ -11,12 +11,12 @@
 // while the tensor core sums the next groups into the other buffers.  So
 // int8 x 4-bit group sums are exact and no weight is rounded, at the price of reading
 // 128 x TN sums from TMEM per group, which is what bounds it: 2048 tokens x 28672 x 4096 in
-// groups of 128 take 457 us with bf16 rows (1052 TFLOP/s, 0.63 of the measured bf16 peak) and
-// 562 us with int8 rows, whose sums need a second multiply-add each; in groups of 64 and 32
-// (4096 x 4096) 70 -> 102 -> 167 us and 90 -> 151 -> 274 us.  Weights s * c rounded to bf16
-// need no group sums (376 and 59 us), but are off by up to 2^-8 each.  Four drain warpgroups
-// (567 us), a second expanding one (narrow tiles 65 against 58 us), 32-column loads (482 us)
-// and waits with a suspend hint (482 / 580 us) were no faster.
+// groups of 128 take 471 us with bf16 rows (1020 TFLOP/s, 0.61 of the measured bf16 peak) and
+// 540 us with int8 rows (890 TOP/s), whose sums need a second multiply-add each (timed without
+// it, and without the conversion, 410 us); in groups of 64 and 32 (4096 x 4096) 73 -> 112 ->
+// 182 us and 86 -> 148 -> 268 us.  Weights s * c rounded to bf16 need no group sums (376 and
+// 59 us), but are off by up to 2^-8 each.  Four drain warpgroups, a second expanding one,
+// 32-column loads, loads one chunk ahead and waits with a suspend hint were no faster.
 //
 // Roles of the 512 threads (one CTA per SM, persistent over the tiles):
 //   warp 0  rows by TMA                     warp 1     tcgen05.mma issue, TMEM
@@ -646,14 +646,14 @@ int w4_tile(const W4Args& a, int sms, cudaStream_t stream) {
     while (s < kMaxSplits && tiles(tn) * s * 2 <= sms && p.kblocks >= s * 4) s *= 2;
     return s;
   };
-  // Tokens of a tile: 256 take 1.64 (int8) or 1.23 (bf16) times a 128-token tile's time, which the
-  // rounds of tiles over the SMs may cost.  256 against 128, int8 / bf16 rows: 1024 tokens x 28672
-  // x 4096 (7 against 13 rounds) 302 / 237 against 344 / 357 us, x 6144 (2, 3) 89 / 70 against
-  // 82 / 87 us; 384 tokens x 6144 (1, 1) 46 / 37 against 29 / 32 us, x 28672 (4, 5) 177 / 136
-  // against 136 / 143 us.
+  // Tokens of a tile: 256 take 1.85 (int8) or 1.35 (bf16) times a 128-token tile's time, which the
+  // rounds of tiles over the SMs may cost.  256 against 128, int8 / bf16 rows: 2048 tokens x 28672
+  // x 4096 (13 against 25 rounds) 540 / 471 against 561 / 670 us; 1024 x 6144 (2, 3) 86 / 73 against
+  // 71 / 85 us; 384 x 6144 (1, 1) 45 / 38 against 26 / 31 us; 512 x 28672 (4, 7) 168 / 143 against
+  // 159 / 191 us.
   auto rounds = [&](int tn) { return (double)((tiles(tn) + sms - 1) / sms) / splits(tn); };
   const int tn = a.tokens <= 64                                                         ? 64
-                 : a.tokens <= 128 || rounds(128) < rounds(256) * (int8 ? 1.64 : 1.23) ? 128
+                 : a.tokens <= 128 || rounds(128) < rounds(256) * (int8 ? 1.85 : 1.35) ? 128
                                                                                         : 256;
   if (tiles(tn) > 0x7fffffff) return LKV_ERR_UNSUPPORTED;
   p.tok_tiles = (int)((a.tokens + tn - 1) / tn);

@@ -640,6 +640,8 @@ def _check_group(group) -> None:
 
 
 def _check_q8(r: Q8Rows, what: str) -> None:
+    if not isinstance(r, Q8Rows):
+        _fail(f"{what} must be Q8Rows")
     q, scale = r.q, r.scale
     _check_group(r.group)
     if q.dtype != _I8 or not q.is_cuda or q.dim() != 2 or q.stride(1) != 1:

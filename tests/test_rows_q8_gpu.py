@@ -155,3 +155,13 @@ def test_refusals():
                  lambda: ops.dequantize_q8(ops.quantize_q8(x), out=x[:2])):
         with pytest.raises(RMarinBackendContractError):
             call()
+
+
+def test_rows_must_be_q8rows():
+    from lastkv_b200 import ops
+    from lastkv_b200.contract import RMarinBackendContractError
+
+    x = torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda")
+    for call in (lambda: ops.dequantize_q8(x), lambda: ops.quantize_q8(x, out=x)):
+        with pytest.raises(RMarinBackendContractError):
+            call()
