@@ -198,7 +198,8 @@ __device__ __forceinline__ void add_group(float (&acc)[2][NT][4], const WeightBl
 // steps (issue slots half used, four warps a scheduler) and, for small weights, the launch and
 // the memory's latency.  8 tokens, groups of 128, int8 / bf16 rows: 28672 x 4096 14.6 / 20.2 us
 // (4.2 / 3.0 TB/s of the 6.5 measured), 4096 x 14336 8.0 / 10.3 us, 4096 x 4096 3.6 / 4.3 us;
-// 1 token, 6144 x 4096 4.0 / 5.9 us.  Loads into registers instead of the ring: 15.9 / 23.3 us
+// 1 token, 6144 x 4096 4.0 / 5.9 us.  Three CTAs per SM (85 registers) were no faster,
+// the round that 896 tiles begin on 296 CTAs costs 0.9 / 1.6 us.  Loads into registers instead of the ring: 15.9 / 23.3 us
 // for the first.
 constexpr int kDepth = 3;
 constexpr int kSkinnyKernelId = 14;

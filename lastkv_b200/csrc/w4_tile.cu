@@ -11,9 +11,9 @@
 // while the tensor core sums the next groups into the other buffers.  So
 // int8 x 4-bit group sums are exact and no weight is rounded, at the price of reading
 // 128 x TN sums from TMEM per group, which is what bounds it: 2048 tokens x 28672 x 4096 in
-// groups of 128 take 471 us with bf16 rows (1020 TFLOP/s, 0.61 of the measured bf16 peak) and
+// groups of 128 take 460 us with bf16 rows (1045 TFLOP/s, 0.63 of the measured bf16 peak) and
 // 540 us with int8 rows (890 TOP/s), whose sums need a second multiply-add each (timed without
-// it, and without the conversion, 410 us); in groups of 64 and 32 (4096 x 4096) 73 -> 112 ->
+// it, and without the conversion, 410 us); in groups of 64 and 32 (4096 x 4096) 71 -> 112 ->
 // 182 us and 86 -> 148 -> 268 us.  Weights s * c rounded to bf16 need no group sums (376 and
 // 59 us), but are off by up to 2^-8 each.  Four drain warpgroups, a second expanding one,
 // 32-column loads, loads one chunk ahead and waits with a suspend hint were no faster.
@@ -364,15 +364,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           reinterpret_cast<uint32_t*>(sh->ws[e][w])[i] = ld_shared4(src + kCodeBytes + 4 * i);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->ws_full[e]);
+        uint4 v[kSpb][kN];  // the whole block at once: 2048 bf16 rows x 4096 x 4096 71.4 us, a stage at a time 73.3
 #pragma unroll
-        for (int i = 0; i < kSpb; ++i) {
-          uint4 v[kN];
+        for (int i = 0; i < kSpb; ++i)
 #pragma unroll
           for (int q = 0; q < kN; ++q) {
             // warp w expands row block w: int8 pieces (r, j), bf16 pieces r, j from the stage
             const int r = INT8 ? q >> 1 : q, j = INT8 ? q & 1 : i;
-            v[q] = w < quarters ? ld_shared16(src + r * 1024 + j * 512 + (4 * g + t) * 16) : make_uint4(0, 0, 0, 0);
+            v[i][q] = w < quarters ? ld_shared16(src + r * 1024 + j * 512 + (4 * g + t) * 16) : make_uint4(0, 0, 0, 0);
           }
+#pragma unroll
+        for (int i = 0; i < kSpb; ++i) {
           const uint32_t it = blk * kSpb + i;
           const int s = it % SA;
           ok = ok && __all_sync(0xffffffffu, mbar_wait(&sh->a_empty[s], ((it / SA) & 1) ^ 1));
@@ -381,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int q = 0; q < kN; ++q) {
             const int r = INT8 ? q >> 1 : q, j = INT8 ? q & 1 : 0;
-            const uint32_t words[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+            const uint32_t words[4] = {v[i][q].x, v[i][q].y, v[i][q].z, v[i][q].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const uint32_t row = a + (w * kTileRows + 16 * r + 8 * (e & 1) + g) * 128;
@@ -648,7 +650,7 @@ int w4_tile(const W4Args& a, int sms, cudaStream_t stream) {
   };
   // Tokens of a tile: 256 take 1.85 (int8) or 1.35 (bf16) times a 128-token tile's time, which the
   // rounds of tiles over the SMs may cost.  256 against 128, int8 / bf16 rows: 2048 tokens x 28672
-  // x 4096 (13 against 25 rounds) 540 / 471 against 561 / 670 us; 1024 x 6144 (2, 3) 86 / 73 against
+  // x 4096 (13 against 25 rounds) 540 / 460 against 561 / 670 us; 1024 x 6144 (2, 3) 86 / 73 against
   // 71 / 85 us; 384 x 6144 (1, 1) 45 / 38 against 26 / 31 us; 512 x 28672 (4, 7) 168 / 143 against
   // 159 / 191 us.
   auto rounds = [&](int tn) { return (double)((tiles(tn) + sms - 1) / sms) / splits(tn); };

@@ -173,7 +173,7 @@ class QuantizedLinears:
         return cls(weight, bias, int8)
 
     # From here on bf16 rows are the faster ones, int8 against bf16 at 28672 x 4096: 128 rows 50
-    # and 60 us, 192 rows 87 and 74 us, 2048 rows 540 and 471 us.
+    # and 60 us, 192 rows 87 and 74 us, 2048 rows 540 and 460 us.
     MANY_ROWS = 192
 
     def takes_int8(self, rows: int) -> bool:
