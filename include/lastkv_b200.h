@@ -455,7 +455,7 @@ int lkv_dequantize_q8(const int8_t* q, int64_t q_row, const float* scale, int64_
  *                 and 2i + 1 in the high half; scales bf16 [n, >= ceil(k / group)];
  *                 packed: lkv_w4_bytes bytes, 16-byte aligned, laid out once per weight
  * n >= 1 any; k a multiple of 8 (the last group may be short); group 32, 64 or
- * 128; tokens 0 .. 2^20 - 1.  x rows 16-byte (bf16) or 8-byte (int8) aligned,
+ * 128; tokens 0 .. 16 x 65535.  x rows 16-byte (bf16) or 8-byte (int8) aligned,
  * strides in elements; bias bf16 [n] or NULL.  No workspace; one launch;
  * sums in a fixed order (deterministic).  error_word (NULL or 4 words) records
  * a pipeline wait that gave up.  The packed weight is read before the launch's

@@ -199,8 +199,10 @@ __device__ __forceinline__ void add_group(float (&acc)[2][NT][4], const WeightBl
 // the memory's latency.  8 tokens, groups of 128, int8 / bf16 rows: 28672 x 4096 14.6 / 20.2 us
 // (4.2 / 3.0 TB/s of the 6.5 measured), 4096 x 14336 8.0 / 10.3 us, 4096 x 4096 3.6 / 4.3 us;
 // 1 token, 6144 x 4096 4.0 / 5.9 us.  Three CTAs per SM (85 registers) were no faster,
-// the round that 896 tiles begin on 296 CTAs costs 0.9 / 1.6 us.  Loads into registers instead of the ring: 15.9 / 23.3 us
-// for the first.
+// the round that 896 tiles begin on 296 CTAs costs 0.9 / 1.6 us.
+// Loads into registers instead of the ring: 15.9 / 23.3 us for the first.
+// kDepth: three blocks of 16 warps are 101 KB in flight per SM, above what the latency asks for
+// (6.5 TB/s x 1 us / 148 SMs = 44 KB).
 constexpr int kDepth = 3;
 constexpr int kSkinnyKernelId = 14;
 
@@ -426,6 +428,8 @@ bool few_tokens(const W4Args& a, int sms) {
   return a.tokens <= 32 || (a.n + kTileRows - 1) / kTileRows * ((a.tokens + 15) / 16) <= 2 * (int64_t)sms;
 }
 
+constexpr int64_t kMaxTokens = 16 * 65535;  // the streaming kernel's grid
+
 bool shape_ok(int64_t n, int64_t k) { return n >= 1 && n <= 0x7fffff00 && k >= 8 && k <= 0x7fffff00 && k % 8 == 0; }
 
 }  // namespace
@@ -453,7 +457,7 @@ int w4_pack(const uint8_t* codes, int64_t codes_row, const void* scales, int64_t
 
 int w4_linear(const W4Args& a, cudaStream_t stream) {
   if (a.group != 32 && a.group != 64 && a.group != 128) return LKV_ERR_UNSUPPORTED;
-  if (!shape_ok(a.n, a.k) || a.tokens < 0 || a.tokens > 0xfffff) return LKV_ERR_INVALID_ARGUMENT;
+  if (!shape_ok(a.n, a.k) || a.tokens < 0 || a.tokens > kMaxTokens) return LKV_ERR_INVALID_ARGUMENT;
   if (a.tokens == 0) return LKV_OK;
   const bool int8 = a.x_scale != nullptr;
   const int align = int8 ? 8 : 16, elem = int8 ? 1 : 2;
