@@ -89,8 +89,9 @@ struct NormQ8Params {
 // A CTA takes whole rows, a row in registers (V vectors of 8 columns per thread): one pass
 // over memory, one barrier per row for the sum of squares.  The CTAs are persistent (at most
 // 1536 threads per SM): the next row's loads are in flight while a row is reduced and stored.
-// The weight stays in registers, loaded before the previous kernel has finished.  (Rows of
-// more than 16384 columns, V = 8, leave no registers for either.)
+// The weight is loaded once, beside the first row, and stays in registers.  (Rows of more than
+// 16384 columns, V = 8, leave no registers for either.)  It is read after the dependency wait
+// like the rows: it may be the previous kernel's output.
 // Bound by HBM for long rows, by the launch and one trip to memory for a few: with a residual,
 // 1 x 4096 1.8 us; 2048 x 4096 17.3 us (3.4 TB/s, 0.52 of the measured copy), 2048 x 8192 28.0,
 // 2048 x 16384 46.1 us (0.78), 512 x 32768 41.9 us.  A CTA per row instead of persistent ones:
@@ -103,13 +104,6 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_q8_kernel(const NormQ8Params 
   const uint4* w4 = reinterpret_cast<const uint4*>(p.weight);
   constexpr bool kAhead = V <= 2;
   uint4 wv[kAhead ? V : 1], xv[V], rv[V];
-  if (kAhead) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = threadIdx.x + i * blockDim.x;
-      wv[kAhead ? i : 0] = c < nvec ? w4[c] : zero;
-    }
-  }
   pdl_wait();
   auto load = [&](int64_t row) {
     const uint4* x = reinterpret_cast<const uint4*>(p.x + row * p.x_row);
@@ -124,7 +118,14 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_q8_kernel(const NormQ8Params 
   __shared__ float red[2][32];  // two buffers: a row's barrier is the only one
   const int warps = blockDim.x >> 5, lanes = p.group / kVec;
   int buf = 0;
-  if (kAhead) load(blockIdx.x);
+  if (kAhead) {
+    load(blockIdx.x);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      wv[kAhead ? i : 0] = c < nvec ? w4[c] : zero;
+    }
+  }
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, buf ^= 1) {
     if (!kAhead) load(row);
     float h[V][kVec];
