@@ -244,6 +244,7 @@ class MLP(nn.Module):
         """4-bit [gate | up] and down projections."""
         self._w4 = (QuantizedLinears.of([self.gate_proj, self.up_proj], group, int8, release),
                     QuantizedLinears.of([self.down_proj], group, int8, release))
+        self._gate_up = None  # fuse_'s [gate | up] tensor: the projections' weights are views of it
         return self
 
     def fuse_(self):

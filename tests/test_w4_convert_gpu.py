@@ -1,0 +1,37 @@
+"""Converting a model's projections to 4 bits: what is freed, what is refused, what is left as it was."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def build(layers=2, **kw):
+    from lastkv_b200.hf import LastKVConfig, LastKVForCausalLM
+    from lastkv_b200.runner import init_random_
+
+    cfg = LastKVConfig(**{**dict(hidden_size=512, intermediate_size=1032, num_attention_heads=8, num_key_value_heads=2,
+                                 num_hidden_layers=layers, head_dim=64, vocab_size=512, chunk_size=32), **kw})
+    model = LastKVForCausalLM(cfg).cuda().to(torch.bfloat16).eval()
+    init_random_(model, seed=5)
+    return model
+
+
+def projections(layer):
+    a, m = layer.self_attn, layer.mlp
+    return [a.q_proj, a.k_proj, a.v_proj, a.o_proj, m.gate_proj, m.up_proj, m.down_proj]
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_release_frees_the_bf16_weights(fused):
+    """Fused projections first, as examples/w4_decode.py has them, or not."""
+    model = build(hidden_size=1024, intermediate_size=4096, num_attention_heads=16)
+    if fused:
+        model.fuse_projections_()
+    weights = sum(lin.weight.numel() * 2 for layer in model.model.layers for lin in projections(layer))
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    model.quantize_projections_(release=True)
+    torch.cuda.synchronize()
+    # 4 bits and a bf16 scale per 128 columns take the place of 16 bits; 1 MB for the allocations' rounding
+    assert torch.cuda.memory_allocated() - before <= weights * (4 + 16 / 128) / 16 - weights + 2 ** 20
