@@ -754,12 +754,45 @@ def dequantize_q8(rows: Q8Rows, out=None):
 
 
 class W4Weight(NamedTuple):
-    """A weight [n, k] of 4-bit codes with bf16 group scales, in the kernels' layout (``w4_pack``)."""
+    """A weight [n, k] of 4-bit codes with bf16 group scales, in the kernels' layout (``w4_pack``).
+
+    ``w4_linear`` reads ``packed`` before the kernels in front of it have finished.  ``w4_pack``
+    allows for that; a packed weight that is written in another way (a copy on the GPU, say)
+    needs one more kernel or copy of torch's, or a synchronisation, between the write and the call."""
 
     packed: torch.Tensor
     n: int
     k: int
     group: int
+
+
+@functools.lru_cache(maxsize=None)
+def _w4_bytes(n: int, k: int, group: int) -> int:
+    return _capi.lib().lkv_w4_bytes(n, k, group)
+
+
+def _check_w4(weight, x) -> None:
+    """The kernels read lkv_w4_bytes(n, k, group) bytes at ``packed``, whatever the tensor holds."""
+    if not isinstance(weight, W4Weight):
+        _fail("weight must be a W4Weight")
+    packed, n, k, group = weight
+    _check_group(group)
+    if packed.dtype != torch.uint8 or not packed.is_contiguous() or packed.numel() != _w4_bytes(n, k, group) \
+            or packed.numel() == 0:
+        _fail(f"weight.packed must be the {_w4_bytes(n, k, group)} contiguous bytes that w4_pack lays out for "
+              f"[{n}, {k}] in groups of {group}, got {packed.dtype} {tuple(packed.shape)}")
+    if not packed.is_cuda or packed.device != x.device:
+        _fail(f"weight.packed must be on x's GPU, got {packed.device} for x on {x.device}")
+
+
+def _err_ptr(error_word):
+    """Address of a device error word (int32 [4]), None for none."""
+    if error_word is None:
+        return None
+    if error_word.dtype != torch.int32 or not error_word.is_cuda or error_word.numel() < 4 \
+            or not error_word.is_contiguous():
+        _fail("error_word must be CUDA int32 [4]")
+    return error_word.data_ptr()
 
 
 @_traced
@@ -776,7 +809,7 @@ def w4_pack(codes, scales, group: int = 128) -> W4Weight:
     if not (scales.is_cuda and scales.dtype == _BF16 and scales.dim() == 2 and scales.stride(1) == 1
             and scales.shape == (n, -(-k // group))):
         _fail("scales must be CUDA bf16 [n, ceil(k / group)]")
-    nbytes = _capi.lib().lkv_w4_bytes(n, k, group)
+    nbytes = _w4_bytes(n, k, group)
     if nbytes == 0:
         _fail(f"4-bit weights need n >= 1 and k a positive multiple of 8, got [{n}, {k}]")
     packed = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
@@ -804,6 +837,7 @@ def w4_quantize(weight, group: int = 128) -> W4Weight:
 def w4_linear(x, weight: W4Weight, bias=None, *, out=None, error_word=None):
     """``x @ w.T (+ bias)`` for a 4-bit weight: x bf16 [..., k] or :class:`Q8Rows` of the
     weight's group; bf16 out [..., n], any number of rows (lkv_w4_linear, lkv_w4_linear_q8)."""
+    _check_w4(weight, x.q if type(x) is Q8Rows else x)
     packed, n, k, group = weight
     if type(x) is Q8Rows:
         _check_q8(x, "x")
@@ -830,7 +864,7 @@ def w4_linear(x, weight: W4Weight, bias=None, *, out=None, error_word=None):
         if bias.dtype != _BF16 or not bias.is_cuda or bias.numel() != n or not bias.is_contiguous():
             _fail("bias must be CUDA bf16 [n]")
         b = bias.data_ptr()
-    err = None if error_word is None else error_word.data_ptr()
+    err = _err_ptr(error_word)
     if scale is not None:
         st = _capi.lib().lkv_w4_linear_q8(x2.data_ptr(), x2.stride(0), scale.data_ptr(), scale.stride(0),
                                           packed.data_ptr(), b, o2.data_ptr(), o_row, T, n, k, group, err, _stream())
@@ -886,6 +920,7 @@ class StepPlan:
             torch.zeros(max_tokens, dtype=torch.int64, device=dev) for _ in range(3))
         self.commit_raw, self.commit_ring, self.commit_count = i32(batch, ppc), i32(batch, ppc), i32(1)
         self.error_word = error_word if error_word is not None else i32(4)
+        _err_ptr(self.error_word)
         # everything after the lengths is the same in every call
         self._rest = (self.batch, src_table.data_ptr(), src_table.stride(0), src_table.shape[0],
                       self.max_sequence_tokens, chunk_size, ring_base.data_ptr(), ring_base.numel(),
