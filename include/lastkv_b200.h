@@ -456,7 +456,7 @@ int lkv_dequantize_q8(const int8_t* q, int64_t q_row, const float* scale, int64_
  *                 packed: lkv_w4_bytes bytes, 16-byte aligned, laid out once per weight
  * n >= 1 any; k a multiple of 8 (the last group may be short); group 32, 64 or
  * 128; tokens 0 .. 16 x 65535.  x rows 16-byte (bf16) or 8-byte (int8) aligned,
- * strides in elements; bias bf16 [n] or NULL.  No workspace; one launch;
+ * scales, y and bias by their elements, strides in elements; bias bf16 [n] or NULL.  No workspace; one launch;
  * sums in a fixed order (deterministic).  error_word (NULL or 4 words) records
  * a pipeline wait that gave up.  The packed weight is read before the launch's
  * dependency wait (programmatic dependent launch): write it with lkv_w4_pack, or

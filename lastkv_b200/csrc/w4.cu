@@ -462,7 +462,8 @@ int w4_linear(const W4Args& a, cudaStream_t stream) {
   const bool int8 = a.x_scale != nullptr;
   const int align = int8 ? 8 : 16, elem = int8 ? 1 : 2;
   if (!a.x || !a.packed || !a.y || (reinterpret_cast<uintptr_t>(a.packed) & 15) ||
-      (reinterpret_cast<uintptr_t>(a.x) % align))
+      (reinterpret_cast<uintptr_t>(a.x) % align) || (reinterpret_cast<uintptr_t>(a.y) & 1) ||
+      (reinterpret_cast<uintptr_t>(a.bias) & 1) || (reinterpret_cast<uintptr_t>(a.x_scale) & 3))
     return LKV_ERR_INVALID_ARGUMENT;
   if (a.tokens > 1 && ((a.x_row * elem) % align || a.x_row < a.k || a.y_row < a.n ||
                        (int8 && a.x_scale_row < (a.k + a.group - 1) / a.group)))
