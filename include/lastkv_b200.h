@@ -489,7 +489,7 @@ int lkv_w4_linear_q8(const int8_t* q, int64_t q_row, const float* scale, int64_t
  * pages of each slot; ring_base int32 [num_layers]; width >= ceil(max_sequence_tokens / 16).
  * A row with slot < 0 is padding: one token on the scratch pages (its lengths are
  * not read).  A row that breaks these rules (or the max_tokens of the buffers) runs
- * on the scratch pages and is recorded in error_word (may be NULL).  All lengths
+ * on the scratch pages, commits nothing and is recorded in error_word (may be NULL).  All lengths
  * are read on the device; one launch (PDL). */
 int lkv_plan_step(const int32_t* num_computed, const int32_t* num_new, const int32_t* slots, int batch,
                   const int32_t* src_table, int64_t src_table_stride, int num_slots, int max_sequence_tokens,

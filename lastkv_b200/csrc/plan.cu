@@ -117,6 +117,32 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs 
       com[k] += s_com[k][w];
     }
   }
+  // A row that does not fit the buffers runs on the scratch pages and comes again in another step,
+  // which commits its chunk: not this one (a commit blends in place).  After the first such row
+  // none fits.
+  int fits = a.batch;
+  if (tok[1] > a.max_tokens) {
+    __shared__ int s_fits[3];
+    if (threadIdx.x == 0) {
+      int64_t sum = 0;
+      int i = 0, before = 0, listed = 0;
+      for (; i < a.batch; ++i) {
+        const Row r = load_row(a, i);
+        sum += r.tokens;
+        if (sum > a.max_tokens) break;
+        const int c = row_commits(a, r) ? 1 : 0;
+        listed += c;
+        before += i < b ? c : 0;
+      }
+      s_fits[0] = i;
+      s_fits[1] = before;
+      s_fits[2] = listed;
+    }
+    __syncthreads();
+    fits = s_fits[0];
+    com[0] = s_fits[1];
+    com[1] = s_fits[2];
+  }
   const int64_t first_tok = tok[0] < a.max_tokens ? tok[0] : a.max_tokens;
   const int64_t all_tok = tok[1] < a.max_tokens ? tok[1] : a.max_tokens;
   const int ppc = a.chunk / LKV_PAGE_SIZE, ring_pages = 2 * ppc;
@@ -142,7 +168,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs 
   }
 
   const Row r = load_row(a, b);
-  const bool over = tok[0] + r.tokens > a.max_tokens;
+  const bool over = b >= fits;
   const bool real = r.slot >= 0 && !r.bad && !over;
   if (once && gtid == 0) {
     if (r.bad || over) report_error(a.error_word, DEVERR_BAD_SPAN, kPlanKernelId, b);
@@ -192,7 +218,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs 
     a.ring_slots[t] = real ? (int64_t)r.slot * 2 * a.chunk + p % (2 * a.chunk) : pad_ring;
     a.src_slots[t] = real ? (int64_t)src[p / LKV_PAGE_SIZE] * LKV_PAGE_SIZE + p % LKV_PAGE_SIZE : pad_src;
   }
-  if (row_commits(a, r)) {
+  if (!over && row_commits(a, r)) {
     const int page = (r.p0 - a.chunk) / LKV_PAGE_SIZE;
     const int32_t* own = a.src_table + (int64_t)r.slot * a.src_table_stride;
     for (int i = gtid; i < ppc; i += gsize) {

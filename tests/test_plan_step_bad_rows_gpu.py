@@ -1,0 +1,50 @@
+"""Rows of a device step plan that break its rules: they run on the scratch pages alone and commit nothing."""
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def make_pool(slots, max_tokens, chunk, layers):
+    from lastkv_b200.vllm_backend import SharedKVPool
+
+    pages = -(-max_tokens // 16)
+    return SharedKVPool(num_layers=layers, num_slots=slots, max_sequence_tokens=max_tokens, chunk_size=chunk,
+                        num_kv_heads=1, head_dim=64, page_order=np.random.default_rng(3).permutation(slots * pages))
+
+
+def make_plan(pool, batch, tokens, **kw):
+    from lastkv_b200 import ops
+
+    return ops.StepPlan(batch, tokens, torch.from_numpy(pool.src_table).cuda(), pool.ring_base_dev,
+                        chunk_size=pool.chunk_size, max_sequence_tokens=pool.max_sequence_tokens,
+                        scratch_src_page=pool.scratch_src_page, scratch_ring_page=pool.scratch_ring_page, **kw)
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("rows,most", [(4, 5), (4, 3), (700, 900)])
+def test_rows_past_the_buffers_commit_nothing(rows, most):
+    """Every row starts at a chunk's start; those that do not fit come again, so their commits must not run now."""
+    chunk, pool = 32, make_pool(rows, 200, 32, 2)
+    plan = make_plan(pool, rows, most)
+    computed, new, slots = [chunk * (1 + i % 5) for i in range(rows)], [2] * rows, list(range(rows))
+    plan.run(i32(computed), i32(new), i32(slots))
+    fits = most // 2
+    assert plan.error_word.tolist()[0] == 4
+    assert plan.commit_count.tolist() == [fits]
+    ring = 2 * chunk // 16
+    for i in range(fits):
+        page = (computed[i] - chunk) // 16
+        assert plan.commit_raw[i].tolist() == pool.src_table[slots[i], page:page + 2].tolist()
+        assert plan.commit_ring[i].tolist() == [pool.ring_base(0) + slots[i] * ring + page % ring + j for j in (0, 1)]
+    assert not bool(plan.commit_raw[fits:].any()) and not bool(plan.commit_ring[fits:].any())
+    if fits < rows:  # the same rows in a step of their own: each commit is there, once
+        rest = make_plan(pool, rows - fits, 2 * (rows - fits))
+        rest.run(i32(computed[fits:]), i32(new[fits:]), i32(slots[fits:]))
+        rest.check_errors()
+        assert rest.commit_count.tolist() == [rows - fits]
