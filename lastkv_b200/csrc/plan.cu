@@ -58,7 +58,7 @@ __device__ __forceinline__ Row load_row(const PlanArgs& a, int b) {
     r.n = 1;
   } else {
     const int64_t end = (int64_t)r.p0 + r.n;
-    r.bad = r.slot >= a.num_slots || r.p0 < 0 || r.n < 1 || end > a.max_sequence_tokens ||
+    r.bad = r.slot >= a.num_slots || r.p0 < 0 || r.n < 1 || r.n > a.max_tokens || end > a.max_sequence_tokens ||
             r.p0 / a.chunk != (int)((end - 1) / a.chunk);
   }
   r.tokens = max(0, min(r.n, a.max_tokens));

@@ -48,3 +48,18 @@ def test_rows_past_the_buffers_commit_nothing(rows, most):
         rest.run(i32(computed[fits:]), i32(new[fits:]), i32(slots[fits:]))
         rest.check_errors()
         assert rest.commit_count.tolist() == [rows - fits]
+
+
+@pytest.mark.parametrize("computed,new", [([0, 64], [9, 1]), ([3, 64], [2 ** 31 - 1, 1]), ([64, 3], [9, 1]), ([64], [9])])
+def test_a_row_longer_than_the_buffers(computed, new):
+    """The first row alone has more tokens than the buffers: it is reported, and so are the rows behind it."""
+    pool = make_pool(2, 200, 32, 2)
+    plan = make_plan(pool, len(new), 8)
+    plan.run(i32(computed), i32(new), i32(list(range(len(new)))))
+    assert plan.error_word.tolist()[0] == 4
+    assert plan.commit_count.tolist() == [0]
+    assert plan.cu_q.tolist() == [0, 8, 8][:len(new) + 1]
+    assert plan.positions.tolist() == [0] * 8
+    assert plan.ring_slots.tolist() == [pool.scratch_ring_page * 16] * 8
+    assert plan.src_slots.tolist() == [pool.scratch_src_page * 16] * 8
+    assert plan.seq_k.tolist() == [8, 1][:len(new)]
