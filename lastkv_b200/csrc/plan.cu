@@ -17,7 +17,7 @@
 // A row with slot < 0 is padding: one token on the scratch pages.  A row that breaks the
 // plan's rules (a span over a chunk boundary, past the capacity, a slot that is not
 // there, n < 1, more tokens than the buffers hold) is recorded in the error word and runs
-// on the scratch pages too.
+// on the scratch pages too: it reads no other page, however long, and commits nothing.
 //
 // Writing L x B x W table words is the floor.  grid = (rows + 1) x parts x layer runs: a
 // block takes one part of a row's columns (four neighbours per thread where the width allows
@@ -170,10 +170,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs 
   const Row r = load_row(a, b);
   const bool over = b >= fits;
   const bool real = r.slot >= 0 && !r.bad && !over;
+  // a row on the scratch pages is as long as its tokens, every page of it the scratch page
+  const int len = real ? r.p0 + r.n : max(1, (int)(min(first_tok + r.tokens, (int64_t)a.max_tokens) - first_tok));
+  const int scratch = real ? 0 : (len - 1) / LKV_PAGE_SIZE + 1;
   if (once && gtid == 0) {
     if (r.bad || over) report_error(a.error_word, DEVERR_BAD_SPAN, kPlanKernelId, b);
     a.cu_q[b] = (int)first_tok;
-    a.seq_k[b] = real ? r.p0 + r.n : max(1, (int)(min(first_tok + r.tokens, (int64_t)a.max_tokens) - first_tok));
+    a.seq_k[b] = len;
   }
   const int last = r.p0 + r.n - 1;
   const int rec = max(0, last / a.chunk * a.chunk - a.chunk);
@@ -193,7 +196,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs 
       } else if (j < ns + np) {
         v[e] = r.slot * ring_pages + ring;
         if (++ring == ring_pages) ring = 0;
-      } else if (!real && j == 0) {
+      } else if (j < scratch) {
         v[e] = a.scratch_ring_page;
       }
     }

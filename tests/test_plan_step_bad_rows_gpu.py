@@ -63,3 +63,45 @@ def test_a_row_longer_than_the_buffers(computed, new):
     assert plan.ring_slots.tolist() == [pool.scratch_ring_page * 16] * 8
     assert plan.src_slots.tolist() == [pool.scratch_src_page * 16] * 8
     assert plan.seq_k.tolist() == [8, 1][:len(new)]
+
+
+@pytest.mark.parametrize("new", [1, 15, 16, 17, 40, 130])
+@pytest.mark.parametrize("why", ["slot", "boundary", "over"])
+def test_bad_rows_read_no_sessions_pages(new, why):
+    """Every page that the row's length reaches is the layer's scratch page, also past its first 16 tokens."""
+    pool = make_pool(3, 300, 64, 3)
+    plan = make_plan(pool, 3, 132 if why != "over" else new + 1)
+    row = {"slot": (0, 3), "boundary": (63, 1), "over": (0, 1)}[why]
+    n = new if why != "boundary" else max(new, 2)
+    plan.run(i32([5, row[0], 7]), i32([1 if why != "over" else 2, n, 1]), i32([0, row[1], 2]))
+    assert plan.error_word.tolist()[0] == 4
+    tokens = n if why != "over" else n - 1
+    assert int(plan.seq_k[1]) == max(1, tokens)
+    pages = (max(1, tokens) + 15) // 16
+    for layer in range(3):
+        base = int(pool.ring_base(layer))
+        assert plan.block_tables[layer, 1, :pages].tolist()[: plan.width] == \
+            [base + pool.scratch_ring_page] * min(pages, plan.width)
+
+
+def test_bad_rows_leave_the_sessions_alone():
+    """Appending and attending as planned: the bad row's span writes and reads the scratch page alone, so its
+    output does not depend on what the sessions hold, and theirs stays."""
+    from lastkv_b200 import ops
+
+    pool = make_pool(2, 300, 64, 1)
+    plan = make_plan(pool, 2, 41)
+    plan.run(i32([5, 0]), i32([1, 40]), i32([0, 9]))
+    g = torch.Generator(device="cuda").manual_seed(4)
+    q = torch.randn((41, 1, 64), generator=g, device="cuda").bfloat16()
+    outs = []
+    for fill in (1.0, 50.0):
+        pool.pool_k.fill_(fill)
+        pool.pool_v.fill_(fill)
+        page = int(pool.ring_base(0)) + pool.scratch_ring_page
+        pool.pool_k[page] = 0.5
+        pool.pool_v[page] = 0.25
+        outs.append(ops.prefill_paged(q, pool.pool_k, pool.pool_v, plan.block_tables[0], plan.seq_k, plan.cu_q, 40,
+                                      max_pages=plan.width))
+    assert torch.equal(outs[0][1:], outs[1][1:])
+    assert not torch.equal(outs[0][0], outs[1][0])
