@@ -179,11 +179,11 @@ class QuantizedLinears:
     def takes_int8(self, rows: int) -> bool:
         return self.int8 and rows < self.MANY_ROWS
 
-    def __call__(self, x):
+    def __call__(self, x, error_word=None):
         """The projections of x: int8 rows, or bf16 [..., k], rounded to int8 rows first where those are taken."""
         if not isinstance(x, ops.Q8Rows) and self.takes_int8(x.numel() // x.shape[-1]):
             x = ops.quantize_q8(x, group=self.weight.group)
-        return ops.w4_linear(x, self.weight, self.bias)
+        return ops.w4_linear(x, self.weight, self.bias, error_word=error_word)
 
 
 def _fuse_linears(linears) -> tuple[torch.Tensor, torch.Tensor | None]:
@@ -252,12 +252,13 @@ class MLP(nn.Module):
         self._gate_up = _fuse_linears([self.gate_proj, self.up_proj])
         return self
 
-    def forward(self, x):
+    def forward(self, x, error_word=None):
+        """``error_word`` records what goes wrong in 4-bit products (the cache's, inside a model)."""
         if self._w4 is not None:
             gate_up, down = self._w4
-            h = gate_up(x)
+            h = gate_up(x, error_word)
             int8 = down.takes_int8(h.numel() // h.shape[-1])
-            return down(ops.silu_mul_q8(h, group=down.weight.group) if int8 else ops.silu_mul(h))
+            return down(ops.silu_mul_q8(h, group=down.weight.group) if int8 else ops.silu_mul(h), error_word)
         if x.is_cuda and x.dtype == torch.bfloat16 and _fused_ok(self._gate_up, [self.gate_proj, self.up_proj]):
             w = self._gate_up[0]
             h = _decode_linear(x, w, silu_mul=True)
@@ -481,7 +482,7 @@ class PagedLastKVCache:
         e = self.error_word.cpu().tolist()
         w = self.workspace.error() if self.workspace is not None else [0, 0, 0, 0]
         if e[0] or w[0]:
-            raise RMarinBackendContractError(f"device error word set: append/blend {e}, decode {w}")
+            raise RMarinBackendContractError(f"device error word set: append/blend/products {e}, decode {w}")
 
 
 # ----------------------------------------------------------------------- attention
@@ -569,7 +570,7 @@ class LastKVAttention(nn.Module):
         meta = cache._meta if cache._meta is not None and cache._meta["n"] == L else cache.plan(L)
         fast = self._w4 is None and _fused_ok(self._qkv, [self.q_proj, self.k_proj, self.v_proj])
         if self._w4 is not None:
-            qkv = self._w4[0](hidden_states).reshape(B * L, (Hq + 2 * Hkv) * D)
+            qkv = self._w4[0](hidden_states, cache.error_word).reshape(B * L, (Hq + 2 * Hkv) * D)
             q, k, v = qkv[:, : Hq * D], qkv[:, Hq * D: (Hq + Hkv) * D], qkv[:, (Hq + Hkv) * D:]
         elif fast:
             qkv = _decode_linear(hidden_states, *self._qkv)
@@ -618,7 +619,7 @@ class LastKVAttention(nn.Module):
                                     out_scale=out_scale, error_word=cache.error_word, max_pages=meta["W"])
         out = out.view(B, L, Hq * D)
         if self._w4 is not None:
-            return self._w4[1](out)
+            return self._w4[1](out, cache.error_word)
         out = out.to(hidden_states.dtype)
         y = _decode_linear(out, self.o_proj.weight, self.o_proj.bias) if fast else None
         return y if y is not None else self.o_proj(out)
@@ -649,10 +650,10 @@ class LastKVDecoderLayer(nn.Module):
             group = w4[0].weight.group
             h, x = self.input_layernorm.fused_q8(residual, delta, group)
             h, x = self.post_attention_layernorm.fused_q8(h, self.self_attn(x, position_embeddings, cache), group)
-            return h, self.mlp(x)
+            return h, self.mlp(x, cache.error_word)
         h, x = self.input_layernorm.fused(residual, delta)
         h, x = self.post_attention_layernorm.fused(h, self.self_attn(x, position_embeddings, cache))
-        return h, self.mlp(x)
+        return h, self.mlp(x) if w4 is None else self.mlp(x, cache.error_word)
 
     def quantize_projections_(self, group: int, int8: bool, release: bool):
         self.self_attn.quantize_(group, int8, release)
