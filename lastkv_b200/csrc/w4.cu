@@ -14,6 +14,7 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "launch.cuh"
+#include "ring.cuh"
 #include "w4.cuh"
 
 namespace lkv {
@@ -234,8 +235,10 @@ __global__ void __launch_bounds__(W * 32, 16 / W) w4_skinny_kernel(const SkinnyP
   __syncwarp();
   // load cursor: a tile's blocks [k0, k1), then the CTA's next tile
   int lt = k0 < k1 ? (int)blockIdx.x : p.tiles, lk = k0;
-  auto load = [&](int slot) {
+  Ring<kDepth> ring;
+  auto load = [&] {
     if (lt >= p.tiles) return;
+    const int slot = ring.fill();
     if (lane == 0) {
       mbar_arrive_expect_tx(&sh->full[warp][slot], block_bytes(G));
       bulk_load_hint(sh->ring[warp][slot], p.packed + block_offset(lt, lk, p.kblocks, p.tiles, G), block_bytes(G),
@@ -247,7 +250,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) w4_skinny_kernel(const SkinnyP
     }
   };
 #pragma unroll
-  for (int d = 0; d < kDepth; ++d) load(d);  // the weights do not depend on the previous kernel
+  for (int d = 0; d < kDepth; ++d) load();  // the weights do not depend on the previous kernel
   const uint8_t* xp[NT];
   const float* sp[NT][2];
 #pragma unroll
@@ -259,12 +262,10 @@ __global__ void __launch_bounds__(W * 32, 16 / W) w4_skinny_kernel(const SkinnyP
   }
   pdl_wait();
 
-  int slot = 0;
-  uint32_t phase = 0;
   bool ok = true;
   for (int tile = blockIdx.x, buf = 0; tile < p.tiles; tile += gridDim.x, buf ^= 1) {
     float acc[2][NT][4] = {};
-    for (int kb = k0; kb < k1; ++kb) {
+    for (int kb = k0; ok && kb < k1; ++kb) {
       const int64_t at = (int64_t)kb * kTileK * kElem;
       XFrag<INT8> x[NT][4];
       float xs[NT][kTileK / G][2];
@@ -292,16 +293,14 @@ __global__ void __launch_bounds__(W * 32, 16 / W) w4_skinny_kernel(const SkinnyP
               xs[nt][gi][h] = INT8 && gi * G < left ? sp[nt][h][kb * (kTileK / G) + gi] : 0.f;
         }
       }
-      ok = ok && mbar_wait(&sh->full[warp][slot], phase);
+      ok = mbar_wait(&sh->full[warp][ring.slot], ring.phase);
       WeightBlock<G> w;
-      w.read(sh->ring[warp][slot], lane);
+      w.read(sh->ring[warp][ring.slot], lane);
       // every lane's block is in registers: its slot may be filled again
       ok = !__any_sync(0xffffffffu, !ok || p.never.is(w.mix()));
-      if (ok) load(slot);
-      if (++slot == kDepth) {
-        slot = 0;
-        phase ^= 1;
-      }
+      if (!ok) break;  // this block's copy, and those behind it, are still in flight
+      ring.next();
+      load();
 #pragma unroll
       for (int gi = 0; gi < kTileK / G; ++gi) {
         XFrag<INT8> xg[NT][kSteps];
@@ -341,8 +340,8 @@ __global__ void __launch_bounds__(W * 32, 16 / W) w4_skinny_kernel(const SkinnyP
   }
   if (!ok) {
     if (lane == 0) report_error(p.err, DEVERR_WAIT_TIMEOUT, kSkinnyKernelId, warp);
-    // no copy may still be in flight when the CTA leaves: every slot was filled again after its last full wait
-    for (int d = 0; d < kDepth; ++d) mbar_wait(&sh->full[warp][d], d < slot ? phase ^ 1 : phase);
+    // no copy may still be in flight when the CTA leaves
+    for (; ring.flying > 0; ring.next()) mbar_wait(&sh->full[warp][ring.slot], ring.phase);
   }
   if (p.splits > 1) {
     const int tile = blockIdx.x;
