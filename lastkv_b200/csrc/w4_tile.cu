@@ -219,10 +219,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_2d(b_ring + s * kBStage, &tmx, &sh->b_full[s], (kb0 * kSpb + i) * (INT8 ? 128 : 64), tok0);
           }
         }
-        if (!ok) {  // no copy may still be in flight when the CTA leaves
-          report_error(p.err, DEVERR_WAIT_TIMEOUT, kKernelId, (int)it);
-          for (uint32_t i = it > SB ? it - SB : 0; i < it; ++i) mbar_wait(&sh->b_full[i % SB], (i / SB) & 1);
-        }
+        if (!ok) report_error(p.err, DEVERR_WAIT_TIMEOUT, kKernelId, (int)it);
+        // No copy may still be in flight when the CTA leaves, whichever warp's wait gave up.
+        for (uint32_t i = it > SB ? it - SB : 0; i < it; ++i) mbar_wait(&sh->b_full[i % SB], (i / SB) & 1);
       }
     } else if (warp == 1) {
       // -------------------------------------------------------------- MMA issue
@@ -296,10 +295,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             bulk_load(codes + b * kQuarters * block_bytes(G), src, bytes, &sh->c_full[b]);
           }
         }
-        if (!ok) {
-          report_error(p.err, DEVERR_WAIT_TIMEOUT, kKernelId, 5000000 + (int)blk);
-          for (uint32_t i = blk > C ? blk - C : 0; i < blk; ++i) mbar_wait(&sh->c_full[i % C], (i / C) & 1);
-        }
+        if (!ok) report_error(p.err, DEVERR_WAIT_TIMEOUT, kKernelId, 5000000 + (int)blk);
+        for (uint32_t i = blk > C ? blk - C : 0; i < blk; ++i) mbar_wait(&sh->c_full[i % C], (i / C) & 1);
       }
     } else if (INT8) {
       // -------------------------------------------------------------- the tokens' scales, transposed
