@@ -11,10 +11,10 @@
 // while the tensor core sums the next groups into the other buffers.  So
 // int8 x 4-bit group sums are exact and no weight is rounded, at the price of reading
 // 128 x TN sums from TMEM per group, which is what bounds it: 2048 tokens x 28672 x 4096 in
-// groups of 128 take 460 us with bf16 rows (1045 TFLOP/s, 0.63 of the measured bf16 peak) and
-// 540 us with int8 rows (890 TOP/s), whose sums need a second multiply-add each (timed without
-// it, and without the conversion, 410 us); in groups of 64 and 32 (4096 x 4096) 71 -> 112 ->
-// 182 us and 86 -> 148 -> 268 us.  Weights s * c rounded to bf16 need no group sums (376 and
+// groups of 128 take 452 us with bf16 rows (1064 TFLOP/s, 0.64 of the measured bf16 peak) and
+// 536 us with int8 rows (897 TOP/s), whose sums need a second multiply-add each (timed without
+// it, and without the conversion, 410 us); in groups of 64 and 32 (4096 x 4096) 77 -> 113 ->
+// 181 us and 85 -> 145 -> 263 us.  Weights s * c rounded to bf16 need no group sums (376 and
 // 59 us), but are off by up to 2^-8 each.  Four drain warpgroups, a second expanding one,
 // 32-column loads, loads one chunk ahead and waits with a suspend hint were no faster.
 //
@@ -27,6 +27,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -45,6 +46,7 @@ constexpr int kThreads = 256 + 128 * kDrainWgs;
 constexpr int kKernelId = 13;
 constexpr int kAStage = kM * 128;
 constexpr int kMaxSplits = 8;
+constexpr float kBias = 12582912.f;  // 1.5 * 2^23
 constexpr int kPartRow = kM + 4;  // of a partial tile: 4 keeps the stores of neighbouring tokens off each other's banks
 
 struct TileParams {
@@ -104,7 +106,7 @@ struct Shared {
   uint64_t xs_full[2], xs_empty[2];
   uint32_t tmem;
   alignas(16) uint8_t ws[scale_slots<G, TN>()][kQuarters][kTileRows * 2 * (kTileK / G)];  // the weight's scales of a 128-column block
-  alignas(16) float xs[INT8 ? 2 : 1][kXsGroups][2][INT8 ? TN : 4];  // x, and -1.5 * 2^23 x, for the tokens' scales x
+  alignas(16) float xs[INT8 ? 2 : 1][kXsGroups][INT8 ? TN : 4];  // the tokens' scales
 };
 
 template <bool INT8, int G, int TN>
@@ -322,12 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int e = 0; e < kXsGroups; ++e) v[e] = tok0 + c < p.tokens && gr + e < groups ? src[e] : 0.f;
             }
 #pragma unroll
-            for (int e = 0; e < kXsGroups; ++e) {
-              // 22 significant bits (truncated), so that 1.5 * 2^23 times it is exact too; 2^-20 keeps that finite
-              const float x = __uint_as_float(__float_as_uint(v[e]) & ~3u) * 0x1p-20f;
-              sh->xs[b][e][0][c] = x;
-              sh->xs[b][e][1][c] = -12582912.f * x;
-            }
+            for (int e = 0; e < kXsGroups; ++e) sh->xs[b][e][c] = v[e];
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh->xs_full[b]);
@@ -437,52 +434,72 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int gi = 0; gi < kGpb; ++gi, ++gt) {
           const int buf = grp % ND;
-          // scales of rows 16 h + 8 e + g at 2 (4 g + 2 h + e); int8 codes stand at 16 c, the tokens' scales at 2^-20
+          // scales of rows 16 h + 8 e + g at 2 (4 g + 2 h + e); int8 codes stand at 16 c.  With w such a scale
+          // (8 bits) over 16, 1.5 * 2^23 w is exact too, so (1.5 * 2^23 + sum) w - 1.5 * 2^23 w is sum * w,
+          // rounded once; the token's scale, with all its bits, multiplies that.
           const uint2 w4 = live ? ld_shared8(&sh->ws[b][sub][gi * 64 + g * 8]) : make_uint2(0, 0);
-          constexpr float kUnit = INT8 ? 0x1p16f : 1.f;
+          constexpr float kUnit = INT8 ? 0.0625f : 1.f;
           const float ws[2][2] = {{bf16_lo(w4.x) * kUnit, bf16_hi(w4.x) * kUnit},
                                   {bf16_lo(w4.y) * kUnit, bf16_hi(w4.y) * kUnit}};
-          const float* xs = &sh->xs[INT8 ? slot & 1 : 0][gt % kXsGroups][0][INT8 ? wg * kCols : 0] + 2 * q;
+          const float* xs = &sh->xs[INT8 ? slot & 1 : 0][gt % kXsGroups][INT8 ? wg * kCols : 0] + 2 * q;
           if (INT8 && gt % kXsGroups == 0) ok = mbar_wait(&sh->xs_full[slot & 1], (slot >> 1) & 1);
           ok = ok && mbar_wait(&sh->d_full[buf], (grp / ND) & 1);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
           const uint32_t at = tmem + lanes + buf * TN + wg * kCols;
-#pragma unroll
-          for (int c0 = 0; c0 < kCols; c0 += 16) {
-            uint32_t u[2][8];
+          uint32_t u[2][8];
+          auto load = [&](int c0) {
             tmem_ld_16x16(at + c0, u[0]);
             tmem_ld_16x16(at + (16u << 16) + c0, u[1]);
-            tmem_wait_ld16(u);
-            if (c0 + 16 == kCols) {  // the buffer is read: the tensor core may sum the next group but one
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&sh->d_empty[buf]);
-            }
+          };
+          load(0);  // before the vote: 128 tokens x 28672 x 4096 48.9 us, 51.5 behind it
+          // From about 2^104 on those products leave fp32's range: such a warp converts its sums first.
+          const bool far = INT8 && __any_sync(0xffffffffu, fmaxf(fmaxf(fabsf(ws[0][0]), fabsf(ws[0][1])),
+                                                                 fmaxf(fabsf(ws[1][0]), fabsf(ws[1][1]))) >= 0x1p100f);
+          auto drain = [&](auto converts) {
+            constexpr bool kConverts = decltype(converts)::value;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float2 x, y;
-              if (INT8) {
-                const uint2 ux = ld_shared8(xs + c0 + 8 * c), uy = ld_shared8(xs + TN + c0 + 8 * c);
-                x = make_float2(__uint_as_float(ux.x), __uint_as_float(ux.y));
-                y = make_float2(__uint_as_float(uy.x), __uint_as_float(uy.y));
+            for (int c0 = 0; c0 < kCols; c0 += 16) {
+              if (c0 > 0) load(c0);
+              tmem_wait_ld16(u);
+              if (c0 + 16 == kCols) {  // the buffer is read: the tensor core may sum the next group but one
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->d_empty[buf]);
               }
 #pragma unroll
-              for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const uint32_t lo = u[h][4 * c + 2 * e], hi = u[h][4 * c + 2 * e + 1];
-                  float2 v;
-                  if (INT8)  // (1.5 * 2^23 + sum) x - 1.5 * 2^23 x, rounded once
-                    v = __ffma2_rn(make_float2(int_bits(lo), int_bits(hi)), x, y);
-                  else
-                    v = make_float2(__uint_as_float(lo), __uint_as_float(hi));
-                  float2& a = acc[h][c0 / 8 + c][e];
-                  a = __ffma2_rn(v, make_float2(ws[h][e], ws[h][e]), a);
+              for (int c = 0; c < 2; ++c) {
+                float2 x = make_float2(1.f, 1.f);
+                if (INT8) {
+                  const uint2 ux = ld_shared8(xs + c0 + 8 * c);
+                  x = make_float2(__uint_as_float(ux.x), __uint_as_float(ux.y));
                 }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    const uint32_t lo = u[h][4 * c + 2 * e], hi = u[h][4 * c + 2 * e + 1];
+                    const float w = ws[h][e];
+                    float2& a = acc[h][c0 / 8 + c][e];
+                    if (!INT8) {
+                      a = __ffma2_rn(make_float2(__uint_as_float(lo), __uint_as_float(hi)), make_float2(w, w), a);
+                    } else if (kConverts) {
+                      a.x = fmaf(int_bits(lo) - kBias, w * x.x, a.x);
+                      a.y = fmaf(int_bits(hi) - kBias, w * x.y, a.y);
+                    } else {
+                      const float2 v = __ffma2_rn(make_float2(int_bits(lo), int_bits(hi)), make_float2(w, w),
+                                                  make_float2(-kBias * w, -kBias * w));
+                      a = __ffma2_rn(v, x, a);
+                    }
+                  }
+              }
             }
-          }
+          };
+          if (far)
+            drain(std::true_type{});
+          else
+            drain(std::false_type{});
           ++grp;
           if (INT8 && (gt % kXsGroups == kXsGroups - 1 || gt == nkb * kGpb - 1)) {
             // the vote needs the last sums, and so the scales, in registers (see Never)
