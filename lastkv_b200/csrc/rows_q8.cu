@@ -69,6 +69,15 @@ __device__ __forceinline__ uint2 quantise8(const float* y, int lanes, float* sca
   return make_uint2(low_bytes(q[0], q[1], q[2], q[3]), low_bytes(q[4], q[5], q[6], q[7]));
 }
 
+// silu(g) * u for any gate.  Below -87, where 1 + exp(-g) is or nears infinity, silu(g) is
+// g exp(g) to the last bit, and the product with a large u may still be an ordinary number: the
+// exponential's halves go on either side of it.
+__device__ __forceinline__ float silu_mul_far(float g, float u) {
+  if (!(g < -87.f)) return g / (1.0f + expf(-g)) * u;
+  const float half = expf(0.5f * g);
+  return g * half * u * half;
+}
+
 struct NormQ8Params {
   const __nv_bfloat16* x;
   int64_t x_row;
@@ -174,11 +183,13 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_q8_kernel(const NormQ8Params 
 }
 
 // One warp per 256 columns of a row (whole groups), one 8-column vector per lane.  One pass;
-// SiLU 8 x 14336 2.2 us, 2048 x 14336 43 us (3.4 TB/s; issue slots: about 250 instructions per
-// 256 columns), plain 2048 x 4096 9.9 us (2.6 TB/s), 1000 x 1544 in groups of 32 3.1 us.  Four
-// chunks' loads in flight per warp: 42, 9.5 and 5.0 us, SiLU 256 x 14336 8.4 against 6.7 us.
-// __fdividef: the quotient's last bits are far below the int8 step (a denominator past 2^126
-// gives 0 for |silu| < 1e-35).
+// SiLU 8 x 14336 1.7 us, 2048 x 14336 41 us (3.6 TB/s), plain 2048 x 4096 8.7 us (2.9 TB/s), 1000
+// x 1544 in groups of 32 3.1 us.  Bound by its instructions more than by memory: an IEEE division in
+// SiLU makes 46 us of the 41, an exact quotient by s in the rounding (two products and a rare
+// division) 11.0 of the 8.7.  Four chunks' loads in flight per warp: SiLU 2048 rows 1 us less,
+// 256 rows 8.4 against 6.7 us.
+// __fdividef: the quotient's last bits are far below the int8 step.  Its denominator has to stay
+// below 2^126; the test for gates past that costs 1.4 us of the 41.
 template <bool SILU>
 __global__ void __launch_bounds__(256)
     rows_q8_kernel(const __nv_bfloat16* __restrict__ x, int64_t x_row, int8_t* __restrict__ q, int64_t q_row,
@@ -198,8 +209,16 @@ __global__ void __launch_bounds__(256)
     if (SILU) {
       float u[kVec];
       unpack8(up, u);
+      float least = y[0];
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) y[j] = __fdividef(y[j], 1.0f + expf(-y[j])) * u[j];
+      for (int j = 1; j < kVec; ++j) least = fminf(least, y[j]);
+      if (least < -87.f) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) y[j] = silu_mul_far(y[j], u[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) y[j] = __fdividef(y[j], 1.0f + expf(-y[j])) * u[j];
+      }
     }
     const uint2 v = quantise8(y, lanes, &s);
     if (in) {
