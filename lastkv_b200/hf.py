@@ -155,14 +155,23 @@ class QuantizedLinears:
     bias: torch.Tensor | None
     int8: bool
 
-    @classmethod
-    def of(cls, linears, group: int, int8: bool, release: bool) -> "QuantizedLinears":
-        """Round the linears' weights, side by side along the outputs, to 4 bits with group scales.
-        ``release`` frees the bf16 weights (the modules keep empty ones)."""
+    @staticmethod
+    def check(linears, group: int) -> None:
+        """Refuse what ``of`` cannot convert, before anything is converted."""
+        if group not in ops.Q8_GROUPS:
+            raise RMarinBackendContractError(f"group must be one of {ops.Q8_GROUPS}, got {group!r}")
         for lin in linears:
             w = lin.weight
             if not (w.is_cuda and w.dtype == torch.bfloat16 and w.dim() == 2 and w.numel()):
                 raise RMarinBackendContractError("4-bit projections are made from bf16 CUDA weights")
+            if w.shape[1] % 8:
+                raise RMarinBackendContractError(f"4-bit projections need inputs of a multiple of 8, got {w.shape[1]}")
+
+    @classmethod
+    def of(cls, linears, group: int, int8: bool, release: bool) -> "QuantizedLinears":
+        """Round the linears' weights, side by side along the outputs, to 4 bits with group scales.
+        ``release`` frees the bf16 weights (the modules keep empty ones)."""
+        cls.check(linears, group)
         weight = ops.w4_quantize(torch.cat([lin.weight.detach() for lin in linears], 0), group)
         bias = None
         if linears[0].bias is not None:
@@ -240,10 +249,13 @@ class MLP(nn.Module):
         self._gate_up = None
         self._w4 = None
 
+    def projections(self):
+        """The linears of each 4-bit weight: [gate | up] and down."""
+        return [self.gate_proj, self.up_proj], [self.down_proj]
+
     def quantize_(self, group: int, int8: bool, release: bool):
         """4-bit [gate | up] and down projections."""
-        self._w4 = (QuantizedLinears.of([self.gate_proj, self.up_proj], group, int8, release),
-                    QuantizedLinears.of([self.down_proj], group, int8, release))
+        self._w4 = tuple(QuantizedLinears.of(linears, group, int8, release) for linears in self.projections())
         self._gate_up = None  # fuse_'s [gate | up] tensor: the projections' weights are views of it
         return self
 
@@ -518,10 +530,13 @@ class LastKVAttention(nn.Module):
         self._w4 = None
         self._consts = (None, None)
 
+    def projections(self):
+        """The linears of each 4-bit weight: [q | k | v] and the output."""
+        return [self.q_proj, self.k_proj, self.v_proj], [self.o_proj]
+
     def quantize_(self, group: int, int8: bool, release: bool):
         """4-bit [q | k | v] and output projections."""
-        self._w4 = (QuantizedLinears.of([self.q_proj, self.k_proj, self.v_proj], group, int8, release),
-                    QuantizedLinears.of([self.o_proj], group, int8, release))
+        self._w4 = tuple(QuantizedLinears.of(linears, group, int8, release) for linears in self.projections())
         self._qkv = None
         return self
 
@@ -655,7 +670,12 @@ class LastKVDecoderLayer(nn.Module):
         h, x = self.post_attention_layernorm.fused(h, self.self_attn(x, position_embeddings, cache))
         return h, self.mlp(x) if w4 is None else self.mlp(x, cache.error_word)
 
+    def check_projections(self, group: int) -> None:
+        for linears in (*self.self_attn.projections(), *self.mlp.projections()):
+            QuantizedLinears.check(linears, group)
+
     def quantize_projections_(self, group: int, int8: bool, release: bool):
+        self.check_projections(group)
         self.self_attn.quantize_(group, int8, release)
         self.mlp.quantize_(group, int8, release)
         return self
@@ -758,6 +778,8 @@ class LastKVForCausalLM(nn.Module):
         state dict then no longer holds them).  Later changes of the weights are not seen."""
         if activations not in ("int8", "bf16"):
             raise RMarinBackendContractError(f"activations must be 'int8' or 'bf16', got {activations!r}")
+        for layer in self.model.layers:  # all of them first: a refusal leaves the model as it was
+            layer.check_projections(group)
         for layer in self.model.layers:
             layer.quantize_projections_(group, activations == "int8", release)
         return self

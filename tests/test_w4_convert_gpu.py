@@ -35,3 +35,27 @@ def test_release_frees_the_bf16_weights(fused):
     torch.cuda.synchronize()
     # 4 bits and a bf16 scale per 128 columns take the place of 16 bits; 1 MB for the allocations' rounding
     assert torch.cuda.memory_allocated() - before <= weights * (4 + 16 / 128) / 16 - weights + 2 ** 20
+
+
+@pytest.mark.parametrize("why", ["width", "type", "device", "released", "group"])
+def test_a_refusal_leaves_the_model_as_it_was(why):
+    """The last layer's down projection cannot be converted: no weight of the model is touched."""
+    from lastkv_b200.contract import RMarinBackendContractError
+
+    model = build(intermediate_size=1028 if why == "width" else 1032)
+    group = 48 if why == "group" else 128
+    down = model.model.layers[-1].mlp.down_proj
+    if why == "type":
+        down.weight.data = down.weight.data.float()
+    elif why == "device":
+        down.weight.data = down.weight.data.cpu()
+    elif why == "released":
+        down.weight = torch.nn.Parameter(down.weight.new_empty((0, down.in_features)), requires_grad=False)
+    before = [[lin.weight for lin in projections(layer)] for layer in model.model.layers]
+    kept = [[w.detach().clone() for w in layer] for layer in before]
+    with pytest.raises(RMarinBackendContractError):
+        model.quantize_projections_(group, release=True)
+    for layer, weights, values in zip(model.model.layers, before, kept):
+        assert layer.self_attn._w4 is None and layer.mlp._w4 is None
+        for lin, w, v in zip(projections(layer), weights, values):
+            assert lin.weight is w and torch.equal(w, v)
