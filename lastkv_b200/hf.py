@@ -146,14 +146,20 @@ class RMSNorm(nn.Module):
         return ops.rmsnorm_q8(x, w, self.variance_epsilon, residual, group=group)
 
 
-@dataclass
-class QuantizedLinears:
+class QuantizedLinears(nn.Module):
     """Projections with 4-bit weights (``quantize_projections_``): one weight for linears that
-    share their input, its bias, and whether their input comes as int8 rows."""
+    share their input, its bias, and whether their input comes as int8 rows.  The packed weight
+    moves with the model (``.to``) and stays out of its state dict."""
 
-    weight: ops.W4Weight
-    bias: torch.Tensor | None
-    int8: bool
+    def __init__(self, weight: ops.W4Weight, bias: torch.Tensor | None, int8: bool):
+        super().__init__()
+        self.register_buffer("packed", weight.packed, persistent=False)
+        self.register_buffer("bias", bias, persistent=False)
+        self.n, self.k, self.group, self.int8 = weight.n, weight.k, weight.group, int8
+
+    @property
+    def weight(self) -> ops.W4Weight:
+        return ops.W4Weight(self.packed, self.n, self.k, self.group)
 
     @staticmethod
     def check(linears, group: int) -> None:
@@ -188,10 +194,10 @@ class QuantizedLinears:
     def takes_int8(self, rows: int) -> bool:
         return self.int8 and rows < self.MANY_ROWS
 
-    def __call__(self, x, error_word=None):
+    def forward(self, x, error_word=None):
         """The projections of x: int8 rows, or bf16 [..., k], rounded to int8 rows first where those are taken."""
         if not isinstance(x, ops.Q8Rows) and self.takes_int8(x.numel() // x.shape[-1]):
-            x = ops.quantize_q8(x, group=self.weight.group)
+            x = ops.quantize_q8(x, group=self.group)
         return ops.w4_linear(x, self.weight, self.bias, error_word=error_word)
 
 
@@ -255,7 +261,7 @@ class MLP(nn.Module):
 
     def quantize_(self, group: int, int8: bool, release: bool):
         """4-bit [gate | up] and down projections."""
-        self._w4 = tuple(QuantizedLinears.of(linears, group, int8, release) for linears in self.projections())
+        self._w4 = nn.ModuleList(QuantizedLinears.of(linears, group, int8, release) for linears in self.projections())
         self._gate_up = None  # fuse_'s [gate | up] tensor: the projections' weights are views of it
         return self
 
@@ -270,7 +276,7 @@ class MLP(nn.Module):
             gate_up, down = self._w4
             h = gate_up(x, error_word)
             int8 = down.takes_int8(h.numel() // h.shape[-1])
-            return down(ops.silu_mul_q8(h, group=down.weight.group) if int8 else ops.silu_mul(h), error_word)
+            return down(ops.silu_mul_q8(h, group=down.group) if int8 else ops.silu_mul(h), error_word)
         if x.is_cuda and x.dtype == torch.bfloat16 and _fused_ok(self._gate_up, [self.gate_proj, self.up_proj]):
             w = self._gate_up[0]
             h = _decode_linear(x, w, silu_mul=True)
@@ -536,7 +542,7 @@ class LastKVAttention(nn.Module):
 
     def quantize_(self, group: int, int8: bool, release: bool):
         """4-bit [q | k | v] and output projections."""
-        self._w4 = tuple(QuantizedLinears.of(linears, group, int8, release) for linears in self.projections())
+        self._w4 = nn.ModuleList(QuantizedLinears.of(linears, group, int8, release) for linears in self.projections())
         self._qkv = None
         return self
 
@@ -662,7 +668,7 @@ class LastKVDecoderLayer(nn.Module):
         w4 = self.self_attn._w4
         if w4 is not None and w4[0].takes_int8(residual.numel() // residual.shape[-1]):
             # the norms write the int8 rows that the projections take
-            group = w4[0].weight.group
+            group = w4[0].group
             h, x = self.input_layernorm.fused_q8(residual, delta, group)
             h, x = self.post_attention_layernorm.fused_q8(h, self.self_attn(x, position_embeddings, cache), group)
             return h, self.mlp(x, cache.error_word)

@@ -59,3 +59,25 @@ def test_a_refusal_leaves_the_model_as_it_was(why):
         assert layer.self_attn._w4 is None and layer.mlp._w4 is None
         for lin, w, v in zip(projections(layer), weights, values):
             assert lin.weight is w and torch.equal(w, v)
+
+
+def test_a_quantized_model_moves():
+    """To the host, where its products are refused, and back, where they are what they were."""
+    import copy
+
+    from lastkv_b200.contract import RMarinBackendContractError
+
+    model = build(attention_bias=True).quantize_projections_(release=True)
+    tokens = torch.arange(40, device="cuda")[None] % 512
+
+    @torch.no_grad()
+    def logits(m):
+        return m(tokens, m.new_cache(1, 40))[0]
+
+    want = logits(model)
+    assert torch.equal(logits(copy.deepcopy(model)), want)
+    cache = model.new_cache(1, 40)
+    model.cpu()
+    with pytest.raises(RMarinBackendContractError), torch.no_grad():
+        model.model.layers[0].mlp(torch.zeros((1, 1, 512), dtype=torch.bfloat16, device="cuda"), cache.error_word)
+    assert torch.equal(logits(model.cuda()), want)

@@ -28,7 +28,7 @@ def test_release_lets_every_projection_weight_go(monkeypatch, fused):
         """Frees the weights as QuantizedLinears.of does on the GPU."""
         for lin in linears:
             lin.weight = torch.nn.Parameter(lin.weight.new_empty((0, lin.in_features)), requires_grad=False)
-        return object()
+        return torch.nn.Identity()
 
     monkeypatch.setattr(hf.QuantizedLinears, "of", staticmethod(of))
     monkeypatch.setattr(hf.QuantizedLinears, "check", staticmethod(lambda linears, group: None))
