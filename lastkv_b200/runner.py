@@ -198,7 +198,11 @@ class GraphDecodeRunner:
             cache._pending = pending  # not the captured form: run it on its own
             cache.flush_commit()
             pending = None
-        self._prepare()
+        try:
+            self._prepare()
+        except Exception:
+            cache._pending = pending  # a refused step leaves the finished chunk's commit queued
+            raise
         if pending is not None:
             if self.plan is None:  # (the device plan makes the same lists)
                 self.c_raw.copy_(pending.raw_pages)
