@@ -596,7 +596,7 @@ def decode_gemm(x, weight, *, silu_mul: bool = False, out=None, error_word=None)
 # few comparisons and its messages are built only when one fails.
 
 Q8_GROUPS = (32, 64, 128)
-_BF16, _I8, _F32 = torch.bfloat16, torch.int8, torch.float32
+_BF16, _I8, _U8, _F32 = torch.bfloat16, torch.int8, torch.uint8, torch.float32
 
 
 class Q8Rows(NamedTuple):
@@ -773,11 +773,9 @@ def _w4_bytes(n: int, k: int, group: int) -> int:
 
 def _check_w4(weight, x) -> None:
     """The kernels read lkv_w4_bytes(n, k, group) bytes at ``packed``, whatever the tensor holds."""
-    if not isinstance(weight, W4Weight):
-        _fail("weight must be a W4Weight")
     packed, n, k, group = weight
     _check_group(group)
-    if packed.dtype != torch.uint8 or not packed.is_contiguous() or packed.numel() != _w4_bytes(n, k, group) \
+    if packed.dtype is not _U8 or not packed.is_contiguous() or packed.numel() != _w4_bytes(n, k, group) \
             or packed.numel() == 0:
         _fail(f"weight.packed must be the {_w4_bytes(n, k, group)} contiguous bytes that w4_pack lays out for "
               f"[{n}, {k}] in groups of {group}, got {packed.dtype} {tuple(packed.shape)}")
@@ -837,9 +835,16 @@ def w4_quantize(weight, group: int = 128) -> W4Weight:
 def w4_linear(x, weight: W4Weight, bias=None, *, out=None, error_word=None):
     """``x @ w.T (+ bias)`` for a 4-bit weight: x bf16 [..., k] or :class:`Q8Rows` of the
     weight's group; bf16 out [..., n], any number of rows (lkv_w4_linear, lkv_w4_linear_q8)."""
-    _check_w4(weight, x.q if type(x) is Q8Rows else x)
+    first = x[0] if type(x) is Q8Rows else x
+    if type(weight) is not W4Weight:
+        _fail("weight must be a W4Weight")
     packed, n, k, group = weight
-    if type(x) is Q8Rows:
+    dev = first.get_device()
+    # what _check_w4 looks at, in the cheapest form
+    if packed.dtype is not _U8 or packed.numel() != _w4_bytes(n, k, group) or packed.get_device() != dev or dev < 0 \
+            or not packed.is_contiguous():
+        _check_w4(weight, first)
+    if first is not x:
         _check_q8(x, "x")
         x2, scale, x_group, lead = x
         if x_group != group:
@@ -864,13 +869,14 @@ def w4_linear(x, weight: W4Weight, bias=None, *, out=None, error_word=None):
         if bias.dtype != _BF16 or not bias.is_cuda or bias.numel() != n or not bias.is_contiguous():
             _fail("bias must be CUDA bf16 [n]")
         b = bias.data_ptr()
-    err = _err_ptr(error_word)
+    err = None if error_word is None else _err_ptr(error_word)
+    stream = torch._C._cuda_getCurrentRawStream(dev)
     if scale is not None:
         st = _capi.lib().lkv_w4_linear_q8(x2.data_ptr(), x2.stride(0), scale.data_ptr(), scale.stride(0),
-                                          packed.data_ptr(), b, o2.data_ptr(), o_row, T, n, k, group, err, _stream())
+                                          packed.data_ptr(), b, o2.data_ptr(), o_row, T, n, k, group, err, stream)
     else:
         st = _capi.lib().lkv_w4_linear(x2.data_ptr(), x2.stride(0), packed.data_ptr(), b, o2.data_ptr(), o_row, T, n,
-                                       k, group, err, _stream())
+                                       k, group, err, stream)
     if st:
         _capi.check(st, "lkv_w4_linear" if scale is None else "lkv_w4_linear_q8")
     return out
