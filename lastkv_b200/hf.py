@@ -187,12 +187,18 @@ class QuantizedLinears(nn.Module):
                 lin.weight = nn.Parameter(lin.weight.new_empty((0, lin.in_features)), requires_grad=False)
         return cls(weight, bias, int8)
 
-    # From here on bf16 rows are the faster ones, int8 against bf16 at 28672 x 4096: 128 rows 50
-    # and 60 us, 192 rows 87 and 74 us, 2048 rows 540 and 460 us.
-    MANY_ROWS = 192
-
     def takes_int8(self, rows: int) -> bool:
-        return self.int8 and rows < self.MANY_ROWS
+        """Whether ``rows`` rows come as int8: up to as many as a group has columns, where those are
+        the faster ones.  int8 against bf16 rows, us:
+                         groups of 128             of 64                     of 32
+            rows         128         160           64          96            16          48
+            6144 x 4096  16.6 19.3   25.5 22.3     16.7 17.6   24.1 19.9     9.0  8.4    26.0 21.6
+            4096 x 4096  12.3 13.9   17.3 16.2     11.8 12.4   15.8 13.9     6.1  6.0    16.3 14.3
+            28672 x 4096 48.9 58.0   84.3 71.0     53.0 54.9   81.5 63.0     26.8 25.5   89.5 71.5
+            4096 x 14336 25.3 30.2   40.2 34.6     27.1 28.5   39.4 31.7     13.9 13.9   43.0 35.1
+        (groups of 32: 8 rows 5.9 against 6.5 and 17.7 against 20.5 us, 32 rows equal but for 6144 x
+        4096, 15.9 against 12.7 us)."""
+        return self.int8 and rows <= self.group
 
     def forward(self, x, error_word=None):
         """The projections of x: int8 rows, or bf16 [..., k], rounded to int8 rows first where those are taken."""
@@ -778,8 +784,8 @@ class LastKVForCausalLM(nn.Module):
         to 4 bits with a bf16 scale per ``group`` (32, 64 or 128) input columns and run on
         ``ops.w4_linear``, for decode steps and prefill alike.  ``activations``: ``"int8"``
         (the norms, SiLU-and-mul and the attention output leave int8 rows with a scale per
-        group) or ``"bf16"``; calls of ``QuantizedLinears.MANY_ROWS`` rows and more keep
-        bf16 activations either way.  Embedding, norms and LM head stay bf16.  Call it on a bf16
+        group) or ``"bf16"``; calls of more than ``group`` rows keep bf16 activations either
+        way, which are faster there.  Embedding, norms and LM head stay bf16.  Call it on a bf16
         CUDA model with its weights loaded; ``release`` frees the bf16 projection weights (the
         state dict then no longer holds them).  Later changes of the weights are not seen."""
         if activations not in ("int8", "bf16"):
