@@ -23,8 +23,8 @@
 // block takes one part of a row's columns (four neighbours per thread where the width allows
 // 16-byte stores), computes each once and stores it for its run of layers; few rows and
 // columns get more runs, so that the GPU is filled.  32 layers, chunks of 1024, tables of 512
-// columns: 8 decode rows 4.3 us (one run of layers 5.7), 64 rows 5.3 us (4-byte stores 6.5);
-// 64 spans in tables of 8192 columns 15.5 us, 4.4 TB/s of stores (4-byte stores 22.3).  The extra row fills the unused tokens
+// columns: 8 decode rows 4.0 us (one run of layers 5.7), 64 rows 5.2 us (4-byte stores 6.5);
+// 64 spans in tables of 8192 columns 16.2 us, 4.2 TB/s of stores (4-byte stores 22.3).  The extra row fills the unused tokens
 // and commit rows.  Every block scans the rows' lengths itself (a few KB from L2), which
 // costs less than a second launch.
 

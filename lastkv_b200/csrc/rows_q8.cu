@@ -101,10 +101,11 @@ struct NormQ8Params {
 // The weight is loaded once, beside the first row, and stays in registers.  (Rows of more than
 // 16384 columns, V = 8, leave no registers for either.)  It is read after the dependency wait
 // like the rows: it may be the previous kernel's output.
-// Bound by HBM for long rows, by the launch and one trip to memory for a few: with a residual,
-// 1 x 4096 1.8 us; 2048 x 4096 17.3 us (3.4 TB/s, 0.52 of the measured copy), 2048 x 8192 28.0,
-// 2048 x 16384 46.1 us (0.78), 512 x 32768 41.9 us.  A CTA per row instead of persistent ones:
-// 20.1, 43.4 and 62.8 us.
+// Bound by the launch and one trip to memory for a few rows (with a residual, 1 x 4096 1.9 us), by
+// HBM for long ones (2048 x 16384 43.2 us, 5.4 TB/s, 0.84 of the measured copy) and by issue slots
+// in between: 2048 x 4096 16.1 us (3.6 TB/s, 0.56; two thirds of the cycles issue), 2048 x 8192
+// 25.0, 512 x 32768 39.3 us.  A CTA per row instead of persistent ones: 20.1, 43.4 and 62.8 us for
+// 2048 rows of 4096, 8192 and 16384.
 template <int V, int THREADS>
 __global__ void __launch_bounds__(THREADS) rmsnorm_q8_kernel(const NormQ8Params p) {
   pdl_launch_dependents();
@@ -184,9 +185,9 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_q8_kernel(const NormQ8Params 
 
 // One warp per 256 columns of a row (whole groups), one 8-column vector per lane.  One pass;
 // SiLU 8 x 14336 1.7 us, 2048 x 14336 41 us (3.6 TB/s), plain 2048 x 4096 8.7 us (2.9 TB/s), 1000
-// x 1544 in groups of 32 3.1 us.  Bound by its instructions more than by memory: an IEEE division in
-// SiLU makes 46 us of the 41, an exact quotient by s in the rounding (two products and a rare
-// division) 11.0 of the 8.7.  Four chunks' loads in flight per warp: SiLU 2048 rows 1 us less,
+// x 1544 in groups of 32 3.1 us.  Bound by its instructions (85 and 75 % of the cycles issue, 336 and
+// 202 per 256 columns) more than by memory: an IEEE division in SiLU makes 46 us of the 41, an exact
+// quotient by s in the rounding (two products and a rare division) 11.0 of the 8.7.  Four chunks' loads in flight per warp: SiLU 2048 rows 1 us less,
 // 256 rows 8.4 against 6.7 us.
 // __fdividef: the quotient's last bits are far below the int8 step.  Its denominator has to stay
 // below 2^126; the test for gates past that costs 1.4 us of the 41.
@@ -228,8 +229,8 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// One 8-column vector per thread: 2048 x 4096 7.5 us (3.4 TB/s), 1000 x 1544 2.8 us; four
-// vectors in flight 8.5 and 4.1 us.
+// One 8-column vector per thread: 2048 x 4096 6.6 us (3.8 TB/s; 70 % of the cycles issue), 1000 x
+// 1544 2.7 us; four vectors in flight 8.5 and 4.1 us.
 __global__ void __launch_bounds__(256)
     dequantize_q8_kernel(const int8_t* __restrict__ q, int64_t q_row, const float* __restrict__ scale,
                          int64_t scale_row, __nv_bfloat16* __restrict__ out, int64_t out_row, int64_t rows, int cols,

@@ -195,11 +195,12 @@ __device__ __forceinline__ void add_group(float (&acc)[2][NT][4], const WeightBl
 // splits' sums (a cluster's CTAs, then one tile per CTA) over the cluster's, always in the
 // same order.  Without splits the CTAs are persistent over the row tiles.  Tokens past the
 // last read the last one's row (their sums are not stored).
-// What it waits for, before HBM, is the expansion of the codes and the products' dependent
-// steps (issue slots half used, four warps a scheduler) and, for small weights, the launch and
-// the memory's latency.  8 tokens, groups of 128, int8 / bf16 rows: 28672 x 4096 14.6 / 20.2 us
-// (4.2 / 3.0 TB/s of the 6.5 measured), 4096 x 14336 8.0 / 10.3 us, 4096 x 4096 3.6 / 4.3 us;
-// 1 token, 6144 x 4096 4.0 / 5.9 us.  Three CTAs per SM (85 registers) were no faster,
+// What it waits for, before HBM, with four warps a scheduler and half of the issue slots used:
+// int8 rows for the activations and their scales, loaded in the iteration that uses them (the
+// largest stall), bf16 rows for their 1.4 times as many instructions, most of them the expansion;
+// small weights for the launch and the memory's latency.  8 tokens, groups of 128, int8 / bf16
+// rows: 28672 x 4096 13.9 / 19.3 us (4.4 / 3.2 TB/s of the 6.5 measured), 4096 x 14336 7.8 / 10.3
+// us, 4096 x 4096 3.6 / 4.4 us; 1 token, 6144 x 4096 4.0 / 6.0 us.  Three CTAs per SM (85 registers) were no faster,
 // the round that 896 tiles begin on 296 CTAs costs 0.9 / 1.6 us.
 // Loads into registers instead of the ring: 15.9 / 23.3 us for the first.
 // kDepth: three blocks of 16 warps are 101 KB in flight per SM, above what the latency asks for

@@ -11,8 +11,8 @@
 // while the tensor core sums the next groups into the other buffers.  So
 // int8 x 4-bit group sums are exact and no weight is rounded, at the price of reading
 // 128 x TN sums from TMEM per group, which is what bounds it: 2048 tokens x 28672 x 4096 in
-// groups of 128 take 452 us with bf16 rows (1064 TFLOP/s, 0.64 of the measured bf16 peak) and
-// 536 us with int8 rows (897 TOP/s), whose sums need a second multiply-add each (timed without
+// groups of 128 take 455 us with bf16 rows (1057 TFLOP/s, 0.63 of the measured bf16 peak) and
+// 535 us with int8 rows (899 TOP/s), whose sums need a second multiply-add each (timed without
 // it, and without the conversion, 410 us); in groups of 64 and 32 (4096 x 4096) 77 -> 113 ->
 // 181 us and 85 -> 145 -> 263 us.  Weights s * c rounded to bf16 need no group sums (376 and
 // 59 us), but are off by up to 2^-8 each.  Four drain warpgroups, a second expanding one,
@@ -656,14 +656,15 @@ int w4_tile(const W4Args& a, int sms, cudaStream_t stream) {
   p.err = a.error_word;
   const int64_t row_tiles = (a.n + kM - 1) / kM;
   auto tiles = [&](int tn) { return row_tiles * ((a.tokens + tn - 1) / tn); };
-  // a power of two of splits, while every CTA of every cluster still has an SM and two blocks of k
+  // A power of two of splits, while every CTA still has an SM and two blocks of k.  (Clusters that
+  // the SMs' grouping leaves no room for run after the others; none waits for another.)
   auto splits = [&](int tn) {
     int s = 1;
     while (s < kMaxSplits && tiles(tn) * s * 2 <= sms && p.kblocks >= s * 4) s *= 2;
     return s;
   };
-  // Tokens of a tile: 256 take 1.85 (int8) or 1.35 (bf16) times a 128-token tile's time, which the
-  // rounds of tiles over the SMs may cost.  256 against 128, int8 / bf16 rows: 2048 tokens x 28672
+  // Tokens of a tile: 256 take 1.85 (int8) or 1.35 (bf16) times a 128-token tile's time in groups of
+  // 128 (groups of 32: 1.73 and 1.86), which the rounds of tiles over the SMs may cost.  256 against 128, int8 / bf16 rows: 2048 tokens x 28672
   // x 4096 (13 against 25 rounds) 540 / 460 against 561 / 670 us; 1024 x 6144 (2, 3) 86 / 73 against
   // 71 / 85 us; 384 x 6144 (1, 1) 45 / 38 against 26 / 31 us; 512 x 28672 (4, 7) 168 / 143 against
   // 159 / 191 us.

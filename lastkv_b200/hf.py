@@ -787,7 +787,10 @@ class LastKVForCausalLM(nn.Module):
         group) or ``"bf16"``; calls of more than ``group`` rows keep bf16 activations either
         way, which are faster there.  Embedding, norms and LM head stay bf16.  Call it on a bf16
         CUDA model with its weights loaded; ``release`` frees the bf16 projection weights (the
-        state dict then no longer holds them).  Later changes of the weights are not seen."""
+        state dict then no longer holds them); kept, they are in the state dict but in no call.
+        Prefill on 4-bit weights is slower than on bf16 ones: a server with memory for both
+        prefills with an unquantized copy of the model, on the same cache.  Later changes of the
+        weights are not seen."""
         if activations not in ("int8", "bf16"):
             raise RMarinBackendContractError(f"activations must be 'int8' or 'bf16', got {activations!r}")
         for layer in self.model.layers:  # all of them first: a refusal leaves the model as it was

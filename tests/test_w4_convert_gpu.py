@@ -81,3 +81,37 @@ def test_a_quantized_model_moves():
     with pytest.raises(RMarinBackendContractError), torch.no_grad():
         model.model.layers[0].mlp(torch.zeros((1, 1, 512), dtype=torch.bfloat16, device="cuda"), cache.error_word)
     assert torch.equal(logits(model.cuda()), want)
+
+
+def test_a_bf16_copy_prefills_for_the_quantized_model():
+    """One cache: the prompt by the model with bf16 weights, the tokens behind it by its 4-bit copy."""
+    import copy
+
+    from lastkv_b200.runner import GraphDecodeRunner
+
+    model = build().fuse_projections_()
+    small = copy.deepcopy(model).quantize_projections_(release=True)
+    prompt = torch.arange(120, device="cuda").view(2, 60)
+    tokens, pools = [], []
+    with torch.no_grad():
+        for graph in (False, True):
+            cache = small.new_cache(2, 80)
+            logits, _ = model(prompt, cache, logits_to_keep=1)
+            pools.append(cache.pool_k.clone())
+            ids = logits[:, -1].float().argmax(-1, keepdim=True)
+            out = [ids]
+            if graph:
+                runner = GraphDecodeRunner(small, cache, device_plan=True)
+                runner.ids.copy_(ids)
+                runner.capture()
+                out += [runner.step().clone() for _ in range(10)]
+            else:
+                for _ in range(10):
+                    logits, _ = small(out[-1], cache, logits_to_keep=1)
+                    out.append(logits[:, -1].float().argmax(-1, keepdim=True))
+            cache.check_errors()
+            tokens.append(torch.cat(out, 1))
+        alone = model.new_cache(2, 80)
+        model(prompt, alone)
+    assert torch.equal(tokens[0], tokens[1])
+    assert torch.equal(pools[0], alone.pool_k) and torch.equal(pools[1], alone.pool_k)
