@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs 
   const int last = r.p0 + r.n - 1;
   const int rec = max(0, last / a.chunk * a.chunk - a.chunk);
   const int ns = real ? rec / LKV_PAGE_SIZE : 0;
-  const int np = real ? (last + LKV_PAGE_SIZE - rec) / LKV_PAGE_SIZE : 0;
+  const int np = real ? (last - rec) / LKV_PAGE_SIZE + 1 : 0;  // (last + 16 may pass 2^31)
   const int32_t* src = a.src_table + (int64_t)(real ? r.slot : 0) * a.src_table_stride;
   const int64_t layer = (int64_t)a.batch * a.width;
   for (int j0 = gtid * VEC; j0 < a.width; j0 += gsize * VEC) {
