@@ -553,6 +553,99 @@ int lkv_cp_combine(const float* send, const uint64_t* peer_recv, int rank, int w
                    int64_t rows, int head_dim, int hq, const float* out_scale, void* out,
                    int64_t out_stride_tok, int32_t* error_word, void* stream);
 
+/* ------------------------------------------------------------------ 8-bit pages
+ * Older pages of a cache in 8 bits: for each (page, KV head) int8 codes of the
+ * keys and values and four fp32 scales, one for every 8 tokens of either; a code
+ * q stands for q * scale.
+ *   codes  : int8 [q8_pages, num_kv_heads, 2 (K, V), 16 * head_dim], each page's codes
+ *            in the order of the decode kernel's operands: with g = 0..7, c = 0..3,
+ *              K[8 h + g, 16 j + 8 t1 + 2 c + t0] at (j / 2) * 512 + (4 g + c) * 16
+ *                                                    + ((j % 2) * 2 + h) * 4 + 2 t0 + t1
+ *              V[8 h + 2 c + t, 16 k + 8 m + g]   at (k / 2) * 512 + (4 g + c) * 16
+ *                                                    + ((k % 2) * 2 + h) * 4 + 2 t + m
+ *   scales : fp32 [q8_pages, num_kv_heads, 4]: K of tokens 0-7, K of 8-15, V, V
+ * Both 16-byte aligned; head_dim 64 or 128.  The reference keeps bf16 history; the
+ * layout of a row (older pages, then recent ones) is the merged pool's.
+ *
+ * lkv_q8_quantize_pages: page pages[i] of a bf16 pool into 8-bit page out_pages[i], i < n:
+ *   scale = max|x| / 127, code = round-to-nearest-even(x / scale), zeros where the
+ *   scale is 0.  tokens (int32 [n], may be NULL: 16) counts the tokens that a page
+ *   holds; the rest become zeros and do not count for the scale.  A block of 8 tokens
+ *   that holds an infinity or a NaN has that scale and zero codes: its values are NaN.
+ *   No two out_pages may be the same.
+ * lkv_q8_dequantize_pages: the reverse, bf16(code * scale).
+ * Page ids outside the pools are skipped and recorded in error_word (may be NULL). */
+int lkv_q8_quantize_pages(const void* pool_k, const void* pool_v, int64_t num_pages, const int32_t* pages,
+                          const int32_t* tokens, int8_t* codes, float* scales, int64_t q8_pages,
+                          const int32_t* out_pages, int64_t n, int num_kv_heads, int head_dim,
+                          int32_t* error_word, void* stream);
+int lkv_q8_dequantize_pages(const int8_t* codes, const float* scales, int64_t q8_pages, const int32_t* pages,
+                            void* pool_k, void* pool_v, int64_t num_pages, const int32_t* out_pages, int64_t n,
+                            int num_kv_heads, int head_dim, int32_t* error_word, void* stream);
+
+/* lkv_decode_paged over such a cache: the first num_q8[b] (int32 [batch] on the device;
+ * NULL: all) block-table columns of row b are 8-bit pages, the rest pages of the
+ * bf16 pool (pool_k and pool_v may be NULL where there are none).  Either kind may hold
+ * the row's last token; keys from seq_k[b] on have no weight, whatever is there.  A row
+ * without keys gives zeros and an LSE of -inf.  Workspace, out, lse, out_scale as for
+ * lkv_decode_paged; flags: LKV_DECODE_L2_KEEP or 0.  Two calls whose work overlaps need
+ * two workspaces.  Everything is read after the launch's dependency wait. */
+int lkv_decode_paged_q8(const void* q, int64_t q_stride_tok, const int8_t* codes, const float* scales,
+                        int64_t q8_pages, const void* pool_k, const void* pool_v, int64_t num_pages,
+                        const int32_t* block_table, int64_t block_table_stride, const int32_t* num_q8,
+                        const int32_t* seq_k, void* out, int64_t out_stride_tok, float* lse,
+                        const float* out_scale, int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                        int max_pages_per_seq, float softmax_scale, void* workspace, size_t workspace_bytes,
+                        int flags, void* stream);
+
+/* Spans of tokens over such a cache, in two calls, so that layers which read the same
+ * older pages share the first:
+ * lkv_q8_stage_pages copies the codes (whole numbers, exact in bf16) of each row's
+ *   8-bit pages, columns below stage_width, to page b * stage_width + column of
+ *   stage_k / stage_v, bf16 [batch * stage_width, 16, num_kv_heads, head_dim].
+ * lkv_prefill_paged_q8 is lkv_prefill_paged with them: it reads the codes from the
+ *   stage and the scales by the block table's page ids.  A row with more 8-bit pages than
+ *   stage_width is recorded in error_word (may be NULL), its further ones read as zeros. */
+int lkv_q8_stage_pages(const int8_t* codes, const float* scales, int64_t q8_pages, const int32_t* block_table,
+                       int64_t block_table_stride, const int32_t* num_q8, const int32_t* seq_k, int batch,
+                       int max_pages_per_seq, void* stage_k, void* stage_v, int stage_width, int num_kv_heads,
+                       int head_dim, int32_t* error_word, void* stream);
+int lkv_prefill_paged_q8(const void* q, int64_t q_stride_tok, const void* stage_k, const void* stage_v,
+                         int stage_width, const float* scales, int64_t q8_pages, const void* pool_k,
+                         const void* pool_v, int64_t num_pages, const int32_t* block_table,
+                         int64_t block_table_stride, const int32_t* num_q8, const int32_t* seq_k,
+                         const int32_t* cu_seqlens_q, void* out, int64_t out_stride_tok, float* lse,
+                         const float* out_scale, int batch, int total_q, int max_q, int num_q_heads,
+                         int num_kv_heads, int head_dim, int max_pages_per_seq, int causal, float softmax_scale,
+                         int32_t* error_word, void* stream);
+
+/* ------------------------------------------------------------------ beam search
+ * lkv_reorder_pages: page dst_pages[i] = page src_pages[i] for all i < n <= 2048 at once (the
+ * lists may permute pages), in each of num_pools <= 8 pools (page_bytes[p], a multiple
+ * of 16, and num_pages[p] of each; host arrays) and, for layers > 1, at the ids plus
+ * l * layer_stride for every layer l (ids below layer_stride).  No two dst_pages may be the
+ * same.  The copies of LastKVCache.reorder_cache (llm/src/lastkv/llm/modeling.py:56-67).
+ *
+ * lkv_beam_select: with scores c [batch, beams] and logits x [batch * beams, vocab] (bf16, or
+ * fp32 with fp32 = 1; row stride in elements), the `select` largest
+ *   total[k, v] = c[k] + x[k, v] - log sum_u exp x[k, u]
+ * of each batch item, largest first; equal totals in the order of k * vocab + v (of one
+ * beam's, the larger logit first).  Totals are compared in 64 bits; a row's maximum and sum of exponentials are fp32.
+ * out_scores [batch, select]; out_rows: the row b * beams + k; out_tokens: v;
+ * out_finished (uint8, may be NULL): v == eos_token, or the beam was finished.
+ * finished (uint8 [batch, beams], may be NULL): such a beam goes on with eos_token alone, at
+ * its score.  A total that is not a number, and every total of a beam whose score or sum
+ * is not finite, counts as -inf.  select <= 32, select <= vocab, beams <= 64,
+ * batch * beams <= 65535.  The workspace (16-byte aligned) need not be cleared. */
+int lkv_reorder_pages(void* const* pools, const int64_t* page_bytes, const int64_t* num_pages, int num_pools,
+                      const int32_t* src_pages, const int32_t* dst_pages, int n, int layers,
+                      int64_t layer_stride, int32_t* error_word, void* stream);
+size_t lkv_beam_workspace_bytes(int64_t rows, int select);
+int lkv_beam_select(const void* logits, int64_t logits_row, int fp32, const float* scores,
+                    const uint8_t* finished, int64_t eos_token, int batch, int beams, int64_t vocab, int select,
+                    float* out_scores, int64_t* out_rows, int64_t* out_tokens, uint8_t* out_finished,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -597,6 +597,104 @@ int lkv_plan_step(const int32_t* num_computed, const int32_t* num_new, const int
   return lkv::plan_step(a, static_cast<cudaStream_t>(stream));
 }
 
+int lkv_q8_quantize_pages(const void* pool_k, const void* pool_v, int64_t num_pages, const int32_t* pages,
+                          const int32_t* tokens, int8_t* codes, float* scales, int64_t q8_pages,
+                          const int32_t* out_pages, int64_t n, int num_kv_heads, int head_dim, int32_t* error_word,
+                          void* stream) {
+  return lkv::quantise_pages(pool_k, pool_v, num_pages, pages, tokens, codes, scales, q8_pages, out_pages, n,
+                             num_kv_heads, head_dim, error_word, static_cast<cudaStream_t>(stream));
+}
+
+int lkv_q8_dequantize_pages(const int8_t* codes, const float* scales, int64_t q8_pages, const int32_t* pages,
+                            void* pool_k, void* pool_v, int64_t num_pages, const int32_t* out_pages, int64_t n,
+                            int num_kv_heads, int head_dim, int32_t* error_word, void* stream) {
+  return lkv::dequantise_pages(codes, scales, q8_pages, pages, pool_k, pool_v, num_pages, out_pages, n, num_kv_heads,
+                               head_dim, error_word, static_cast<cudaStream_t>(stream));
+}
+
+int lkv_q8_stage_pages(const int8_t* codes, const float* scales, int64_t q8_pages, const int32_t* block_table,
+                       int64_t block_table_stride, const int32_t* num_q8, const int32_t* seq_k, int batch,
+                       int max_pages_per_seq, void* stage_k, void* stage_v, int stage_width, int num_kv_heads,
+                       int head_dim, int32_t* error_word, void* stream) {
+  return lkv::stage_pages(codes, scales, q8_pages, block_table, block_table_stride, num_q8, seq_k, batch,
+                          max_pages_per_seq, stage_k, stage_v, stage_width, num_kv_heads, head_dim, error_word,
+                          static_cast<cudaStream_t>(stream));
+}
+
+int lkv_prefill_paged_q8(const void* q, int64_t q_stride_tok, const void* stage_k, const void* stage_v,
+                         int stage_width, const float* scales, int64_t q8_pages, const void* pool_k,
+                         const void* pool_v, int64_t num_pages, const int32_t* block_table,
+                         int64_t block_table_stride, const int32_t* num_q8, const int32_t* seq_k,
+                         const int32_t* cu_seqlens_q, void* out, int64_t out_stride_tok, float* lse,
+                         const float* out_scale, int batch, int total_q, int max_q, int num_q_heads,
+                         int num_kv_heads, int head_dim, int max_pages_per_seq, int causal, float softmax_scale,
+                         int32_t* error_word, void* stream) {
+  if (!stage_k && batch != 0 && total_q != 0) return LKV_ERR_INVALID_ARGUMENT;
+  lkv::PrefillArgs a{};
+  a.q = q;
+  a.q_stride_tok = q_stride_tok;
+  a.pool_k = pool_k;
+  a.pool_v = pool_v;
+  a.num_pages = num_pages;
+  a.block_table = block_table;
+  a.block_table_stride = block_table_stride;
+  a.seq_k = seq_k;
+  a.cu_q = cu_seqlens_q;
+  a.out = out;
+  a.out_stride_tok = out_stride_tok;
+  a.lse = lse;
+  a.out_scale = out_scale;
+  a.batch = batch;
+  a.total_q = total_q;
+  a.max_q = max_q;
+  a.num_q_heads = num_q_heads;
+  a.num_kv_heads = num_kv_heads;
+  a.head_dim = head_dim;
+  a.max_pages_per_seq = max_pages_per_seq;
+  a.causal = causal;
+  a.softmax_scale = softmax_scale;
+  a.error_word = error_word;
+  a.stream = stream;
+  a.stage_k = stage_k;
+  a.stage_v = stage_v;
+  a.stage_width = stage_width;
+  a.num_q8 = num_q8;
+  a.q8_scales = scales;
+  a.q8_pages = q8_pages;
+  return lkv::prefill_paged(a);
+}
+
+int lkv_decode_paged_q8(const void* q, int64_t q_stride_tok, const int8_t* codes, const float* scales,
+                        int64_t q8_pages, const void* pool_k, const void* pool_v, int64_t num_pages,
+                        const int32_t* block_table, int64_t block_table_stride, const int32_t* num_q8,
+                        const int32_t* seq_k, void* out, int64_t out_stride_tok, float* lse, const float* out_scale,
+                        int batch, int num_q_heads, int num_kv_heads, int head_dim, int max_pages_per_seq,
+                        float softmax_scale, void* workspace, size_t workspace_bytes, int flags, void* stream) {
+  return lkv::decode_paged_q8(lkv::DecodeQ8Args{q, q_stride_tok, codes, scales, q8_pages, pool_k, pool_v, num_pages,
+                                                block_table, block_table_stride, num_q8, seq_k, out, out_stride_tok,
+                                                lse, out_scale, batch, num_q_heads, num_kv_heads, head_dim,
+                                                max_pages_per_seq, softmax_scale, workspace, workspace_bytes, flags,
+                                                stream});
+}
+
+int lkv_reorder_pages(void* const* pools, const int64_t* page_bytes, const int64_t* num_pages, int num_pools,
+                      const int32_t* src_pages, const int32_t* dst_pages, int n, int layers, int64_t layer_stride,
+                      int32_t* error_word, void* stream) {
+  return lkv::reorder_pages(pools, page_bytes, num_pages, num_pools, src_pages, dst_pages, n, layers, layer_stride,
+                            error_word, static_cast<cudaStream_t>(stream));
+}
+
+size_t lkv_beam_workspace_bytes(int64_t rows, int select) { return lkv::beam_workspace_bytes(rows, select); }
+
+int lkv_beam_select(const void* logits, int64_t logits_row, int fp32, const float* scores, const uint8_t* finished,
+                    int64_t eos_token, int batch, int beams, int64_t vocab, int select, float* out_scores,
+                    int64_t* out_rows, int64_t* out_tokens, uint8_t* out_finished, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  return lkv::beam_select(logits, logits_row, fp32, scores, finished, eos_token, batch, beams, vocab, select,
+                          out_scores, out_rows, out_tokens, out_finished, workspace, workspace_bytes,
+                          static_cast<cudaStream_t>(stream));
+}
+
 int lkv_cp_combine_sizes(int64_t rows, int head_dim, int world, int64_t* send_floats, int64_t* recv_words) {
   if (rows < 1 || head_dim < 1 || world < 1 || world > lkv::kCpMaxRanks) return LKV_ERR_INVALID_ARGUMENT;
   if (send_floats) *send_floats = (rows * (head_dim + 1) + 3) / 4 * 4;

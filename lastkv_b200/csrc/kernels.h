@@ -45,10 +45,65 @@ struct PrefillArgs {
   int kv_splits = 1;
   float* part_o = nullptr;    // [kv_splits][total_q * num_q_heads][head_dim]
   float* part_lse = nullptr;  // [kv_splits][total_q * num_q_heads], natural log
+  // the first num_q8 pages of each row in 8 bits (null stage_k: none), staged by stage_pages at
+  // page row * stage_width + column
+  const void* stage_k = nullptr;
+  const void* stage_v = nullptr;
+  int stage_width = 0;
+  const int32_t* num_q8 = nullptr;  // [batch], or null: every page
+  const float* q8_scales = nullptr;
+  int64_t q8_pages = 0;
 };
 int prefill_paged(const PrefillArgs& a);
 int prefill_split_plan(int batch, int max_q, int num_q_heads, int num_kv_heads, int head_dim, int max_pages,
                        int causal, int* kv_splits);
+
+// 8-bit pages (pages_q8.cu): codes [pages][hkv][2][16 * d] in the kernels' order, scales [pages][hkv][4].
+int quantise_pages(const void* pool_k, const void* pool_v, int64_t pool_pages, const int32_t* pages,
+                   const int32_t* tokens, void* codes, float* scales, int64_t q8_pages, const int32_t* out_pages,
+                   int64_t n, int hkv, int d, int* err, cudaStream_t stream);
+int dequantise_pages(const void* codes, const float* scales, int64_t q8_pages, const int32_t* pages, void* pool_k,
+                     void* pool_v, int64_t pool_pages, const int32_t* out_pages, int64_t n, int hkv, int d, int* err,
+                     cudaStream_t stream);
+// The codes of the leading `width` columns of block tables as bf16, for prefill_paged.
+int stage_pages(const void* codes, const float* scales, int64_t q8_pages, const int32_t* bt, int64_t bt_stride,
+                const int32_t* num_q8, const int32_t* seq_k, int batch, int W, void* stage_k, void* stage_v, int width,
+                int hkv, int d, int* err, cudaStream_t stream);
+int reorder_pages(void* const* pools, const int64_t* page_bytes, const int64_t* pages, int num_pools,
+                  const int32_t* src, const int32_t* dst, int n, int layers, int64_t layer_stride, int* err,
+                  cudaStream_t stream);
+
+struct DecodeQ8Args {
+  const void* q;
+  int64_t q_stride_tok;
+  const void* codes;
+  const float* scales;
+  int64_t q8_pages;
+  const void* pool_k;  // or null: every page is in 8 bits
+  const void* pool_v;
+  int64_t num_pages;
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  const int32_t* num_q8;  // [batch] leading columns in 8 bits, or null: all
+  const int32_t* seq_k;
+  void* out;
+  int64_t out_stride_tok;
+  float* lse;
+  const float* out_scale;
+  int batch, num_q_heads, num_kv_heads, head_dim, max_pages_per_seq;
+  float softmax_scale;
+  void* workspace;
+  size_t workspace_bytes;
+  int flags;  // LKV_DECODE_L2_KEEP
+  void* stream;
+};
+int decode_paged_q8(const DecodeQ8Args& a);
+
+size_t beam_workspace_bytes(int64_t rows, int select);
+int beam_select(const void* logits, int64_t row_stride, int fp32, const float* scores, const uint8_t* finished,
+                int64_t eos, int batch, int beams, int64_t vocab, int select, float* out_scores, int64_t* out_rows,
+                int64_t* out_tokens, uint8_t* out_finished, void* workspace, size_t workspace_bytes,
+                cudaStream_t stream);
 
 struct DecodeArgs {
   const void* q;

@@ -1,0 +1,448 @@
+// Pages of a bf16 pool to 8 bits and back, and copies of whole pages (sm_100a).
+//
+//   quantise    per (page, KV head, keys or values, 8 tokens): s = max|x| / 127, q = rne(x / s)
+//               (zeros where s = 0); a block that holds an infinity or a NaN gets that scale and
+//               zeros, so its values are NaN.  Tokens past the page's count are zeros and do not
+//               count for the scale.
+//   dequantise  bf16(q * s), or (staging for the prefill kernel) the codes themselves, which are
+//               whole numbers up to 127 and exact in bf16.
+//   reorder     pages[dst[i]] = pages[src[i]] for all i at once, in several pools and layers.
+// All three read and write each byte once and are bound by HBM.
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "launch.cuh"
+#include "pages_q8.cuh"
+
+namespace lkv {
+
+namespace {
+
+constexpr int kWarps = 4;
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+struct QuantParams {
+  const __nv_bfloat16* pool[2];  // keys, values
+  int64_t pool_pages;
+  const int32_t* pages;
+  const int32_t* tokens;  // or null: 16
+  uint8_t* codes;
+  float* scales;
+  int64_t q8_pages;
+  const int32_t* out_pages;
+  int64_t n;
+  int hkv;
+  int* err;
+};
+
+// One warp per (page, head, keys or values).  Rows are loaded whole (16 bytes a lane), rounded in
+// registers, and put into the kernels' order through a byte tile in shared memory: rows of D + 16
+// bytes, so that neither the 8-byte stores nor the reads in operand order meet bank conflicts.
+template <int D>
+__global__ void __launch_bounds__(kWarps * 32) quantise_pages_kernel(const QuantParams p) {
+  constexpr int PITCH = D + 16;
+  constexpr int LANES = D / 8;       // lanes per row
+  constexpr int STEP = 32 / LANES;   // rows per load
+  constexpr int LOADS = 16 / STEP;   // the first half of them holds tokens 0-7
+  __shared__ __align__(16) uint8_t tile_all[kWarps][16 * PITCH];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * kWarps + warp;
+  if (item >= p.n * p.hkv * 2) return;
+  const int which = (int)(item & 1), hk = (int)((item >> 1) % p.hkv);
+  const int64_t n = (item >> 1) / p.hkv;
+  const int64_t src = p.pages[n], dst = p.out_pages[n];
+  if (src < 0 || src >= p.pool_pages || dst < 0 || dst >= p.q8_pages) {
+    if (lane == 0 && hk == 0) report_error(p.err, DEVERR_BAD_PAGE, 8, (int)(src < 0 || src >= p.pool_pages ? src : dst));
+    return;
+  }
+  const int valid = p.tokens ? min(max(p.tokens[n], 0), kPageTokens) : kPageTokens;
+  const __nv_bfloat16* base = (which ? p.pool[1] : p.pool[0]) + (src * kPageTokens * p.hkv + hk) * D;
+  const int64_t row_stride = (int64_t)p.hkv * D;
+  const int r0 = lane / LANES, col = (lane % LANES) * 8;
+  uint4 v[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int r = i * STEP + r0;
+    v[i] = r < valid ? __ldcs(reinterpret_cast<const uint4*>(base + r * row_stride + col)) : make_uint4(0, 0, 0, 0);
+  }
+  uint8_t* tile = tile_all[warp];
+  float scale[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float amax = 0.f;
+#pragma unroll
+    for (int i = h * LOADS / 2; i < (h + 1) * LOADS / 2; ++i) {
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) amax = max_nan(amax, max_nan(fabsf(bf16_lo(w[e])), fabsf(bf16_hi(w[e]))));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    scale[h] = amax / 127.0f;
+    const bool zero = !(amax < INFINITY) || scale[h] == 0.f;
+    // one division per block: x * (127 / max), rounded by the addition that puts the integer into the
+    // low byte of 1.5 * 2^23 + q; where the reciprocal would overflow, x / s
+    const bool tiny = amax < 1e-30f;
+    const float inv = tiny ? 0.f : 127.0f / amax;
+#pragma unroll
+    for (int i = h * LOADS / 2; i < (h + 1) * LOADS / 2; ++i) {
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      uint32_t q[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = bf16_lo(w[e]), b = bf16_hi(w[e]);
+        if (!tiny) {
+          q[2 * e] = __float_as_uint(fmaf(a, inv, 12582912.0f));
+          q[2 * e + 1] = __float_as_uint(fmaf(b, inv, 12582912.0f));
+        } else {
+          q[2 * e] = zero ? 0u : (uint32_t)max(-127, min(127, __float2int_rn(a / scale[h])));
+          q[2 * e + 1] = zero ? 0u : (uint32_t)max(-127, min(127, __float2int_rn(b / scale[h])));
+        }
+      }
+      uint2 packed;
+      packed.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+      packed.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
+      if (zero) packed = make_uint2(0, 0);
+      *reinterpret_cast<uint2*>(tile + (i * STEP + r0) * PITCH + col) = packed;
+    }
+  }
+  __syncwarp();
+  const int64_t block = dst * p.hkv + hk;
+  const int g = lane >> 2, c = lane & 3;
+  uint8_t* out = p.codes + (block * 2 + which) * 16 * D;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    uint32_t w[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int t = 2 * i + (x >> 1), h = x & 1;  // 16-column tile, row half
+      if (which == 0) {
+        const uint8_t* at = tile + (8 * h + g) * PITCH + 16 * t + 2 * c;
+        w[x] = __byte_perm(*reinterpret_cast<const uint16_t*>(at), *reinterpret_cast<const uint16_t*>(at + 8), 0x5140);
+      } else {
+        const uint8_t* at = tile + (8 * h + 2 * c) * PITCH + 16 * t + g;
+        w[x] = (uint32_t)at[0] | (uint32_t)at[8] << 8 | (uint32_t)at[PITCH] << 16 | (uint32_t)at[PITCH + 8] << 24;
+      }
+    }
+    *reinterpret_cast<uint4*>(out + i * 512 + lane * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if (lane == 0)
+    *reinterpret_cast<float2*>(p.scales + block * kScalesPerBlock + 2 * which) = make_float2(scale[0], scale[1]);
+}
+
+struct DequantParams {
+  const uint8_t* codes;
+  const float* scales;
+  int64_t q8_pages;
+  __nv_bfloat16* pool[2];
+  int64_t pool_pages;
+  int hkv;
+  int* err;
+  // a list of pages
+  const int32_t* pages;
+  const int32_t* out_pages;
+  int64_t n;
+  // or the leading columns of block tables: row b's column j becomes page b * width + j
+  const int32_t* bt;
+  int64_t bt_stride;
+  const int32_t* num_q8;  // or null: every column
+  const int32_t* seq_k;
+  int batch, W, width;
+};
+
+// Back to rows of bf16, one warp per (page, head, keys or values): the inverse of the above.
+// STAGE: the codes themselves (the prefill kernel applies the scales); where a scale is not finite
+// the keys are NaN, so that the tokens' scores are, and the values zero.
+template <int D, bool STAGE>
+__global__ void __launch_bounds__(kWarps * 32) dequantise_pages_kernel(const DequantParams p) {
+  constexpr int PITCH = D + 16;
+  constexpr int LANES = D / 8, STEP = 32 / LANES, LOADS = 16 / STEP;
+  __shared__ __align__(16) uint8_t tile_all[kWarps][16 * PITCH];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * kWarps + warp;
+  const int which = (int)(item & 1), hk = (int)((item >> 1) % p.hkv);
+  const int64_t n = (item >> 1) / p.hkv;
+  int64_t src, dst;
+  if constexpr (STAGE) {
+    const int b = (int)(n / p.width), j = (int)(n % p.width);
+    if (b >= p.batch) return;
+    const int pages = min((max(p.seq_k[b], 0) + kPageTokens - 1) / kPageTokens, p.W);
+    if (j >= (p.num_q8 ? min(p.num_q8[b], pages) : pages)) return;
+    src = p.bt[(int64_t)b * p.bt_stride + j];
+    dst = n;
+  } else {
+    if (n >= p.n) return;
+    src = p.pages[n];
+    dst = p.out_pages[n];
+  }
+  if (src < 0 || src >= p.q8_pages || dst < 0 || dst >= p.pool_pages) {
+    const bool bad_src = src < 0 || src >= p.q8_pages;
+    if (lane == 0 && hk == 0) report_error(p.err, DEVERR_BAD_PAGE, 9, (int)(bad_src ? src : dst));
+    if (!STAGE) return;
+  }
+  const bool have = src >= 0 && src < p.q8_pages;  // a staged page that is not there reads as zeros
+  const int g = lane >> 2, c = lane & 3;
+  const int64_t block = src * p.hkv + hk;
+  const uint8_t* in = p.codes + (block * 2 + which) * 16 * D;
+  uint8_t* tile = tile_all[warp];
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  uint4 v[D / 32];
+  if (have) s = *reinterpret_cast<const float4*>(p.scales + block * kScalesPerBlock);
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+    v[i] = have ? __ldcs(reinterpret_cast<const uint4*>(in + i * 512 + lane * 16)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int t = 2 * i + (x >> 1), h = x & 1;
+      if (which == 0) {
+        uint8_t* at = tile + (8 * h + g) * PITCH + 16 * t + 2 * c;
+        *reinterpret_cast<uint16_t*>(at) = (uint16_t)__byte_perm(w[x], 0, 0x4420);
+        *reinterpret_cast<uint16_t*>(at + 8) = (uint16_t)__byte_perm(w[x], 0, 0x4431);
+      } else {
+        uint8_t* at = tile + (8 * h + 2 * c) * PITCH + 16 * t + g;
+        at[0] = (uint8_t)w[x];
+        at[8] = (uint8_t)(w[x] >> 8);
+        at[PITCH] = (uint8_t)(w[x] >> 16);
+        at[PITCH + 8] = (uint8_t)(w[x] >> 24);
+      }
+    }
+  }
+  __syncwarp();
+  const float s0 = which ? s.z : s.x, s1 = which ? s.w : s.y;
+  // staged keys of tokens whose keys or values have a scale that is not finite
+  const bool bad0 = !(fabsf(s.x) < INFINITY) || !(fabsf(s.z) < INFINITY);
+  const bool bad1 = !(fabsf(s.y) < INFINITY) || !(fabsf(s.w) < INFINITY);
+  __nv_bfloat16* base = (which ? p.pool[1] : p.pool[0]) + (dst * kPageTokens * p.hkv + hk) * D;
+  const int64_t row_stride = (int64_t)p.hkv * D;
+  const int r0 = lane / LANES, col = (lane % LANES) * 8;
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int r = i * STEP + r0;
+    const uint2 q = *reinterpret_cast<const uint2*>(tile + r * PITCH + col);
+    uint32_t o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t w = (e & 2) ? q.y : q.x;
+      const float a = (float)(int8_t)(w >> ((e & 1) * 16)), b = (float)(int8_t)(w >> ((e & 1) * 16 + 8));
+      if constexpr (STAGE) {
+        o[e] = which == 0 && (r < 8 ? bad0 : bad1) ? 0x7fff7fffu : pack_bf16(a, b);
+      } else {
+        const float sc = r < 8 ? s0 : s1;
+        o[e] = pack_bf16(a * sc, b * sc);
+      }
+    }
+    *reinterpret_cast<uint4*>(base + r * row_stride + col) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+// ---------------------------------------------------------------- copies of pages
+
+constexpr int kMaxPools = 8;
+constexpr int kCopyThreads = 256, kCopyPerThread = 8;
+constexpr int kCopyVectors = kCopyThreads * kCopyPerThread;
+
+struct ReorderParams {
+  uint8_t* pool[kMaxPools];
+  int64_t page_bytes[kMaxPools];
+  int64_t pages[kMaxPools];
+  int64_t first_slice[kMaxPools + 1];  // slices of one layer, pool after pool
+  const int32_t* src;
+  const int32_t* dst;
+  int n, log_width;  // a slice: 1 << log_width 16-byte vectors of every listed page
+  int64_t layer_stride, id_limit;
+  int* err;
+};
+
+// A CTA moves the same slice of every listed page of one pool and layer: it reads all of them
+// into registers before it writes any, so the lists may permute pages among themselves.  Slices are as
+// wide as the registers allow (2048 vectors of 16 bytes over the list), up to 1 KB.
+__global__ void __launch_bounds__(kCopyThreads) reorder_pages_kernel(const ReorderParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t slice = blockIdx.x;
+  int pool = 0;
+  while (slice >= p.first_slice[pool + 1]) ++pool;
+  const int64_t layer = blockIdx.y;
+  const int width = 1 << p.log_width;
+  const int64_t v0 = (slice - p.first_slice[pool]) << p.log_width, vectors = p.page_bytes[pool] / 16;
+  const int64_t pages = p.pages[pool];
+  uint4* base = reinterpret_cast<uint4*>(p.pool[pool]);
+  uint4 v[kCopyPerThread];
+  int64_t to[kCopyPerThread];
+#pragma unroll
+  for (int i = 0; i < kCopyPerThread; ++i) {
+    const int e = i * kCopyThreads + threadIdx.x;
+    const int r = e >> p.log_width;
+    const int64_t at = v0 + (e & (width - 1));
+    to[i] = -1;
+    if (r < p.n && at < vectors) {
+      const int64_t s = p.src[r] + layer * p.layer_stride, d = p.dst[r] + layer * p.layer_stride;
+      // with several layers an id is one of a layer's pages, so no layer writes what another reads
+      auto bad = [&](int id, int64_t page) { return id < 0 || id >= p.id_limit || page >= pages; };
+      if (bad(p.src[r], s) || bad(p.dst[r], d)) {
+        if (at == 0) report_error(p.err, DEVERR_BAD_PAGE, 10, bad(p.src[r], s) ? p.src[r] : p.dst[r]);
+      } else if (s != d) {
+        to[i] = d * vectors + at;
+        v[i] = __ldcs(base + s * vectors + at);
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kCopyPerThread; ++i)
+    if (to[i] >= 0) base[to[i]] = v[i];
+}
+
+bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
+
+int check_pages(const void* pool_k, const void* pool_v, int64_t pool_pages, const void* codes, const void* scales,
+                int64_t q8_pages, int hkv, int d) {
+  if (d != 64 && d != 128) return LKV_ERR_UNSUPPORTED;
+  if (hkv < 1 || hkv > 256 || pool_pages < 0 || q8_pages < 0 || pool_pages > INT32_MAX || q8_pages > INT32_MAX)
+    return LKV_ERR_INVALID_ARGUMENT;
+  if (!pool_k || !pool_v || !codes || !scales) return LKV_ERR_INVALID_ARGUMENT;
+  if (misaligned(pool_k, 16) || misaligned(pool_v, 16) || misaligned(codes, 16) || misaligned(scales, 16))
+    return LKV_ERR_INVALID_ARGUMENT;
+  return LKV_OK;
+}
+
+}  // namespace
+
+int quantise_pages(const void* pool_k, const void* pool_v, int64_t pool_pages, const int32_t* pages,
+                   const int32_t* tokens, void* codes, float* scales, int64_t q8_pages, const int32_t* out_pages,
+                   int64_t n, int hkv, int d, int* err, cudaStream_t stream) {
+  const int st = check_pages(pool_k, pool_v, pool_pages, codes, scales, q8_pages, hkv, d);
+  if (st != LKV_OK) return st;
+  if (n < 0 || (n > 0 && (!pages || !out_pages))) return LKV_ERR_INVALID_ARGUMENT;
+  if (n == 0) return LKV_OK;
+  QuantParams p{};
+  p.pool[0] = static_cast<const __nv_bfloat16*>(pool_k);
+  p.pool[1] = static_cast<const __nv_bfloat16*>(pool_v);
+  p.pool_pages = pool_pages;
+  p.pages = pages;
+  p.tokens = tokens;
+  p.codes = static_cast<uint8_t*>(codes);
+  p.scales = scales;
+  p.q8_pages = q8_pages;
+  p.out_pages = out_pages;
+  p.n = n;
+  p.hkv = hkv;
+  p.err = err;
+  const int64_t blocks = (n * hkv * 2 + kWarps - 1) / kWarps;
+  if (n > INT32_MAX || blocks > INT32_MAX) return LKV_ERR_UNSUPPORTED;
+  const auto kern = d == 128 ? quantise_pages_kernel<128> : quantise_pages_kernel<64>;
+  return launch_pdl(kern, dim3((unsigned)blocks), dim3(kWarps * 32), 0, stream, p) == cudaSuccess ? LKV_OK
+                                                                                                  : LKV_ERR_CUDA;
+}
+
+namespace {
+int launch_dequantise(const DequantParams& p, int64_t n, int d, bool stage, cudaStream_t stream) {
+  const int64_t blocks = (n * p.hkv * 2 + kWarps - 1) / kWarps;
+  if (n > INT32_MAX || blocks > INT32_MAX) return LKV_ERR_UNSUPPORTED;
+  const auto kern = d == 128 ? (stage ? dequantise_pages_kernel<128, true> : dequantise_pages_kernel<128, false>)
+                             : (stage ? dequantise_pages_kernel<64, true> : dequantise_pages_kernel<64, false>);
+  return launch_pdl(kern, dim3((unsigned)blocks), dim3(kWarps * 32), 0, stream, p) == cudaSuccess ? LKV_OK
+                                                                                                  : LKV_ERR_CUDA;
+}
+}  // namespace
+
+int dequantise_pages(const void* codes, const float* scales, int64_t q8_pages, const int32_t* pages, void* pool_k,
+                     void* pool_v, int64_t pool_pages, const int32_t* out_pages, int64_t n, int hkv, int d, int* err,
+                     cudaStream_t stream) {
+  const int st = check_pages(pool_k, pool_v, pool_pages, codes, scales, q8_pages, hkv, d);
+  if (st != LKV_OK) return st;
+  if (n < 0 || (n > 0 && (!pages || !out_pages))) return LKV_ERR_INVALID_ARGUMENT;
+  if (n == 0) return LKV_OK;
+  DequantParams p{};
+  p.codes = static_cast<const uint8_t*>(codes);
+  p.scales = scales;
+  p.q8_pages = q8_pages;
+  p.pool[0] = static_cast<__nv_bfloat16*>(pool_k);
+  p.pool[1] = static_cast<__nv_bfloat16*>(pool_v);
+  p.pool_pages = pool_pages;
+  p.hkv = hkv;
+  p.err = err;
+  p.pages = pages;
+  p.out_pages = out_pages;
+  p.n = n;
+  return launch_dequantise(p, n, d, false, stream);
+}
+
+int stage_pages(const void* codes, const float* scales, int64_t q8_pages, const int32_t* bt, int64_t bt_stride,
+                const int32_t* num_q8, const int32_t* seq_k, int batch, int W, void* stage_k, void* stage_v, int width,
+                int hkv, int d, int* err, cudaStream_t stream) {
+  if (batch < 0 || W < 0 || width < 0 || width > W) return LKV_ERR_INVALID_ARGUMENT;
+  if (batch == 0 || width == 0) return LKV_OK;
+  const int64_t n = (int64_t)batch * width;
+  const int st = check_pages(stage_k, stage_v, n, codes, scales, q8_pages, hkv, d);
+  if (st != LKV_OK) return st;
+  if (!bt || !seq_k) return LKV_ERR_INVALID_ARGUMENT;
+  DequantParams p{};
+  p.codes = static_cast<const uint8_t*>(codes);
+  p.scales = scales;
+  p.q8_pages = q8_pages;
+  p.pool[0] = static_cast<__nv_bfloat16*>(stage_k);
+  p.pool[1] = static_cast<__nv_bfloat16*>(stage_v);
+  p.pool_pages = n;
+  p.hkv = hkv;
+  p.err = err;
+  p.bt = bt;
+  p.bt_stride = bt_stride;
+  p.num_q8 = num_q8;
+  p.seq_k = seq_k;
+  p.batch = batch;
+  p.W = W;
+  p.width = width;
+  return launch_dequantise(p, n, d, true, stream);
+}
+
+int reorder_pages(void* const* pools, const int64_t* page_bytes, const int64_t* pages, int num_pools,
+                  const int32_t* src, const int32_t* dst, int n, int layers, int64_t layer_stride, int* err,
+                  cudaStream_t stream) {
+  if (num_pools < 1 || num_pools > kMaxPools || !pools || !page_bytes || !pages) return LKV_ERR_INVALID_ARGUMENT;
+  if (n < 0 || layers < 0 || layer_stride < 0 || (n > 0 && (!src || !dst))) return LKV_ERR_INVALID_ARGUMENT;
+  if (n > kCopyVectors || layers > 65535) return LKV_ERR_UNSUPPORTED;
+  if (layers > 1 && (layer_stride < 1 || layer_stride > INT32_MAX)) return LKV_ERR_INVALID_ARGUMENT;
+  for (int i = 0; i < num_pools; ++i)
+    if (!pools[i] || misaligned(pools[i], 16) || page_bytes[i] < 16 || page_bytes[i] % 16 || pages[i] < 1)
+      return LKV_ERR_INVALID_ARGUMENT;
+  if (n == 0 || layers == 0) return LKV_OK;
+  ReorderParams p{};
+  p.src = src;
+  p.dst = dst;
+  p.n = n;
+  p.layer_stride = layer_stride;
+  p.id_limit = layers > 1 ? layer_stride : (int64_t)INT32_MAX + 1;
+  p.err = err;
+  while (p.log_width < 6 && (n << (p.log_width + 1)) <= kCopyVectors) ++p.log_width;
+  int64_t slices = 0;
+  for (int i = 0; i < num_pools; ++i) {
+    p.pool[i] = static_cast<uint8_t*>(pools[i]);
+    p.page_bytes[i] = page_bytes[i];
+    p.pages[i] = pages[i];
+    p.first_slice[i] = slices;
+    slices += (page_bytes[i] / 16 + (1 << p.log_width) - 1) >> p.log_width;
+  }
+  for (int i = num_pools; i <= kMaxPools; ++i) p.first_slice[i] = slices;
+  if (slices > INT32_MAX) return LKV_ERR_UNSUPPORTED;
+  return launch_pdl(reorder_pages_kernel, dim3((unsigned)slices, (unsigned)layers), dim3(kCopyThreads), 0, stream, p) ==
+                 cudaSuccess
+             ? LKV_OK
+             : LKV_ERR_CUDA;
+}
+
+}  // namespace lkv

@@ -45,6 +45,14 @@
 // a quarter of its exponentials on the FMA pipe (ex2_poly2) and the rest on the
 // SFU, and stores P in 32-key chunks as they are ready.
 //
+// Older pages in 8 bits (Q8): a row's first num_q8 pages come from a staged copy of their int8
+// codes as bf16 (dequantise_pages_kernel: whole numbers up to 127, exact), so the MMAs run as they
+// do on bf16 pages, and the scales, one for every 8 keys, are applied in fp32 in the softmax.  A
+// key scale k multiplies a group's scores: it goes into the maximum once per group and into the
+// FFMA in front of the exponential.  A value scale v multiplies the weights that PV takes,
+// p v = 2^(s - m + log2 v): it goes into that FFMA's addend, and a group's sum of them times 1 / v is
+// its part of the row's sum.  No instruction per key is added.  Pages in bf16 have scales of one.
+//
 // Key splits (non-causal calls, S > 1): blockIdx.z = sequence * S + split and
 // a CTA covers its split's share of the key blocks, writing the normalised
 // fp32 partial and natural-log LSE of its rows; merge_partials_kernel then
@@ -55,6 +63,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -94,7 +103,17 @@ struct PrefillParams {
   float* part_lse;       // S > 1: natural-log LSE [S][rows]
   int64_t part_rows;     // rows per split
   int tma_out;           // S == 1 and the output map is valid: full tiles leave by TMA stores
+  // Q8: staged pages b * stage_width + column, their scales by the block table's page ids
+  const int32_t* num_q8;  // or null: every page
+  const float* q8_scales;
+  int64_t q8_pages;
+  int stage_width;
+  int has_pool;
 };
+
+// Value scales below this are taken as this in the weights (their codes are then zero, or the
+// products below 2^-53 of anything else): 1 / v stays finite.
+constexpr float kMinValueScale = 8.6736174e-19f;  // 2^-60
 
 template <int D>
 struct PrefillCfg {
@@ -111,6 +130,12 @@ struct PrefillCfg {
   // At least 120 KB so a second CTA never shares the SM (each CTA holds all 512 TMEM columns).
   static constexpr int SMEM_BYTES =
       (1024 + OFF_BAR + BAR_BYTES) > 120 * 1024 ? (1024 + OFF_BAR + BAR_BYTES) : 120 * 1024;
+  // Q8: after the barriers, per softmax warp the scales of a block's 16 groups of 8 keys: key scale x
+  // softmax scale, log2 of the value scale, 1 / value scale
+  static constexpr int OFF_SCALE = OFF_BAR + 256;
+  static constexpr int SCALE_BYTES = 8 * 3 * 16 * 4;
+  static constexpr int SMEM_Q8 = 1024 + OFF_SCALE + SCALE_BYTES > SMEM_BYTES ? 1024 + OFF_SCALE + SCALE_BYTES : SMEM_BYTES;
+  static_assert(SMEM_Q8 <= 227 * 1024, "shared memory");
   static constexpr uint32_t IDESC_S = umma_idesc_bf16(kBM, kBN, 0, 0);
   static constexpr uint32_t IDESC_PV = umma_idesc_bf16(kBM, D, 0, 1);
   static constexpr uint32_t COL_S = 0;        // + tile * kBN
@@ -128,11 +153,19 @@ struct Bars {
   int fail;
 };
 
-template <int D, int GROUP>
+static_assert(sizeof(Bars) <= 256, "the scales begin behind the barriers");
+
+struct StageMaps {
+  CUtensorMap k, v;  // Q8: the staged pages
+};
+struct NoStageMaps {};
+
+template <int D, int GROUP, bool Q8>
 __global__ void __launch_bounds__(kThreads, 1)
     prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                            const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmo,
-                           const PrefillParams p) {
+                           const PrefillParams p,
+                           const __grid_constant__ std::conditional_t<Q8, StageMaps, NoStageMaps> stage) {
   using Cfg = PrefillCfg<D>;
   constexpr int TOK = kBM / GROUP;  // tokens per tile
   extern __shared__ uint8_t smem_raw[];
@@ -178,6 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
   const int npages = min((n + kPageTok - 1) / kPageTok, p.W);
+  const int nh = Q8 ? (p.num_q8 ? min(max(p.num_q8[b], 0), npages) : npages) : 0;  // pages in 8 bits
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, 1);
@@ -244,13 +278,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int pg = pg0; pg < pg0 + npg; ++pg) {
           const int pi = (j0 + j) * kPagesPerBlock + pg;
           int pid = (int)p.num_pages;  // past the pool: TMA fills zeros
-          if (pi < npages) {
+          const CUtensorMap* from = map;
+          if (Q8 && pi < nh) {
+            if constexpr (Q8) from = is_k ? &stage.k : &stage.v;
+            // a page without a place in the stage reads as zeros
+            pid = pi < p.stage_width ? b * p.stage_width + pi : p.B * p.stage_width;
+            if (is_k && pi >= p.stage_width) report_error(p.err, DEVERR_BAD_PAGE, 4, pi);
+          } else if (pi < npages) {
             pid = btrow[pi];
-            if (is_k && (pid < 0 || (int64_t)pid >= p.num_pages)) report_error(p.err, DEVERR_BAD_PAGE, 4, pid);
+            const bool bad = pid < 0 || (int64_t)pid >= p.num_pages || (Q8 && !p.has_pool);
+            if (is_k && bad) report_error(p.err, DEVERR_BAD_PAGE, 4, pid);
+            if (Q8 && bad) pid = (int)p.num_pages;
           }
 #pragma unroll
           for (int h = 0; h < Cfg::HALVES; ++h)
-            tma_load_4d(dst + h * Cfg::KV_HALF + pg * (kPageTok * 128), map, &full[s], h * 64, hk, 0, pid);
+            tma_load_4d(dst + h * Cfg::KV_HALF + pg * (kPageTok * 128), from, &full[s], h * 64, hk, 0, pid);
         }
       }
     }
@@ -326,8 +368,32 @@ __global__ void __launch_bounds__(kThreads, 1)
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     const float sl2 = p.scale_log2;
+    float* group_scale = reinterpret_cast<float*>(smem + Cfg::OFF_SCALE) + warp * 48;  // Q8
+    // Q8: lane 4 i + c has scale c (keys 0-7, 8-15, values 0-7, 8-15) of page i of a block, read a block ahead
+    auto scale_of = [&](int j) {
+      const int pi = (j0 + j) * kPagesPerBlock + (lane >> 2);
+      if (j >= nb || pi >= nh || pi >= p.stage_width) return 1.f;
+      const int pid = btrow[pi];
+      if (pid < 0 || (int64_t)pid >= p.q8_pages) return 1.f;
+      return __ldg(p.q8_scales + ((int64_t)pid * p.Hkv + hk) * 4 + (lane & 3));
+    };
+    float next_scale = Q8 ? scale_of(0) : 1.f;
     // Wait results are made warp-uniform: tcgen05.ld/st below are warp-collective.
     for (int j = 0; j < nb; ++j) {
+      if constexpr (Q8) {
+        float f = next_scale;
+        next_scale = scale_of(j + 1);
+        if (!(fabsf(f) < INFINITY)) f = 1.f;  // the staged keys are NaN there
+        const int at = (lane >> 2) * 2 + (lane & 1);
+        if (lane & 2) {
+          f = fmaxf(f, kMinValueScale);
+          group_scale[16 + at] = log2f(f);
+          group_scale[32 + at] = 1.f / f;
+        } else {
+          group_scale[at] = fmaxf(f, 1e-37f) * sl2;  // codes of zero: not -inf * 0 where they are masked
+        }
+        __syncwarp();
+      }
       ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[t], j & 1));
       tc_fence_after();
       if (!ok) break;
@@ -349,6 +415,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < kBN; ++e)
           if (key0 + e > lim) x[e] = -INFINITY;
       }
+      float mx;
+      if constexpr (Q8) {
+        float gm[16];
+#pragma unroll
+        for (int g = 0; g < 16; ++g) {
+          const float* y = x + 8 * g;
+          gm[g] = fmaxf(fmax3f(fmax3f(y[0], y[1], y[2]), y[3], y[4]), fmax3f(y[5], y[6], y[7])) * group_scale[g];
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) gm[g] = fmaxf(fmax3f(gm[g], gm[g + 4], gm[g + 8]), gm[g + 12]);
+        mx = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
+      } else {
       // 8 independent partial maxima (short dependency chains, three-input max), then a tree
       float mp[8];
 #pragma unroll
@@ -357,8 +435,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int e = 8; e + 16 <= kBN - 8; e += 16)
 #pragma unroll
         for (int u = 0; u < 8; ++u) mp[u] = fmax3f(mp[u], x[e + u], x[e + 8 + u]);
-      float mx = fmaxf(fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])), fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7])));
+      mx = fmaxf(fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])), fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7])));
       mx *= sl2;  // scale > 0, so max commutes with it
+      }
       float alpha = 1.f;
       if (mx > m + kRescaleLog2) {
         alpha = (m == -INFINITY) ? 0.f : ex2_approx(m - mx);
@@ -374,6 +453,24 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int c = 0; c < kBN / 32; ++c) {
         uint32_t pc[16];
+        if constexpr (Q8) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float kf = group_scale[4 * c + g], add = group_scale[16 + 4 * c + g] + neg_mref;
+            const float2 kfv = make_float2(kf, kf), addv = make_float2(add, add);
+            float2 gs = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int e = c * 32 + g * 8 + 2 * q;
+              const float2 a = __ffma2_rn(make_float2(x[e], x[e + 1]), kfv, addv);
+              const float2 pv = q == (g & 1) ? ex2_poly2(a) : make_float2(ex2_approx(a.x), ex2_approx(a.y));
+              gs = __fadd2_rn(gs, pv);
+              pc[g * 4 + q] = pack_bf16(pv.x, pv.y);
+            }
+            const float inv = group_scale[32 + 4 * c + g];
+            sp[g] = __ffma2_rn(gs, make_float2(inv, inv), sp[g]);
+          }
+        } else {
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
           const int e = c * 32 + 2 * q;
@@ -381,6 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float2 pv = (q & 7) < 2 ? ex2_poly2(a) : make_float2(ex2_approx(a.x), ex2_approx(a.y));
           sp[q & 3] = __fadd2_rn(sp[q & 3], pv);
           pc[q] = pack_bf16(pv.x, pv.y);
+        }
         }
         tmem_st16(lane_base + col_s + c * 16, pc);
       }
@@ -493,22 +591,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kWarpMma) tmem_dealloc(tmem, 512);
 }
 
-template <int D, int GROUP>
+template <int D, int GROUP, bool Q8, typename Stage>
 int launch_prefill(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to,
-                   const PrefillParams& prm, int max_q, cudaStream_t stream) {
+                   const Stage& stage, const PrefillParams& prm, int max_q, cudaStream_t stream) {
   using Cfg = PrefillCfg<D>;
   constexpr int TOK = kTiles * kBM / GROUP;  // query tokens per CTA
+  constexpr int smem = Q8 ? Cfg::SMEM_Q8 : Cfg::SMEM_BYTES;
   static bool attr_done[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !attr_done[dev]) {
-    if (cudaFuncSetAttribute(prefill_tcgen05_kernel<D, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             Cfg::SMEM_BYTES) != cudaSuccess)
+    if (cudaFuncSetAttribute(prefill_tcgen05_kernel<D, GROUP, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+        cudaSuccess)
       return LKV_ERR_CUDA;
     attr_done[dev] = true;
   }
   dim3 grid((max_q + TOK - 1) / TOK, prm.Hkv, prm.B * prm.S);
-  prefill_tcgen05_kernel<D, GROUP><<<grid, kThreads, Cfg::SMEM_BYTES, stream>>>(tq, tk, tv, to, prm);
+  prefill_tcgen05_kernel<D, GROUP, Q8><<<grid, kThreads, smem, stream>>>(tq, tk, tv, to, prm, stage);
   return cudaGetLastError() == cudaSuccess ? LKV_OK : LKV_ERR_CUDA;
 }
 
@@ -521,12 +620,16 @@ int prefill_paged(const PrefillArgs& a) {
   if (group != 1 && group != 2 && group != 4 && group != 8) return LKV_ERR_UNSUPPORTED;
   if (a.batch < 0 || a.total_q < 0 || a.max_q < 0 || a.max_pages_per_seq < 0) return LKV_ERR_INVALID_ARGUMENT;
   if (a.batch == 0 || a.total_q == 0 || a.max_q == 0) return LKV_OK;
-  if (!a.q || !a.pool_k || !a.pool_v || !a.block_table || !a.seq_k || !a.cu_q || !a.out)
+  const bool q8 = a.stage_k != nullptr;
+  const bool pool = a.pool_k && a.pool_v && a.num_pages > 0;
+  if (!a.q || (!pool && !q8) || !a.block_table || !a.seq_k || !a.cu_q || !a.out) return LKV_ERR_INVALID_ARGUMENT;
+  if (q8 && (!a.stage_v || !a.q8_scales || a.stage_width < 1 || (int64_t)a.stage_width * a.batch >= INT32_MAX ||
+             a.q8_pages < 0 || a.kv_splits > 1))
     return LKV_ERR_INVALID_ARGUMENT;
   if ((reinterpret_cast<uintptr_t>(a.q) & 15) || ((a.q_stride_tok * 2) & 15)) return LKV_ERR_INVALID_ARGUMENT;
   if ((reinterpret_cast<uintptr_t>(a.out) & 15) || ((a.out_stride_tok * 2) & 15)) return LKV_ERR_INVALID_ARGUMENT;
   if (a.batch > 65535 || a.num_kv_heads > 65535) return LKV_ERR_UNSUPPORTED;
-  if (!a.error_word) return LKV_ERR_INVALID_ARGUMENT;
+  if (!a.error_word && !q8) return LKV_ERR_INVALID_ARGUMENT;
   const int S = a.kv_splits < 1 ? 1 : a.kv_splits;
   if (S > 1) {
     // key splits need a non-causal call (every query sees the same key range)
@@ -537,10 +640,23 @@ int prefill_paged(const PrefillArgs& a) {
   CUtensorMap tq, tk, tv;
   int st = make_query_tensor_map(&tq, a.q, a.total_q, a.q_stride_tok, a.num_q_heads, a.head_dim, group);
   if (st != LKV_OK) return st;
-  st = make_pool_tensor_map(&tk, a.pool_k, a.num_pages, a.num_kv_heads, a.head_dim);
-  if (st != LKV_OK) return st;
-  st = make_pool_tensor_map(&tv, a.pool_v, a.num_pages, a.num_kv_heads, a.head_dim);
-  if (st != LKV_OK) return st;
+  StageMaps stage;
+  if (q8) {
+    const int64_t staged = (int64_t)a.stage_width * a.batch;
+    st = make_pool_tensor_map(&stage.k, a.stage_k, staged, a.num_kv_heads, a.head_dim);
+    if (st != LKV_OK) return st;
+    st = make_pool_tensor_map(&stage.v, a.stage_v, staged, a.num_kv_heads, a.head_dim);
+    if (st != LKV_OK) return st;
+  }
+  if (pool) {
+    st = make_pool_tensor_map(&tk, a.pool_k, a.num_pages, a.num_kv_heads, a.head_dim);
+    if (st != LKV_OK) return st;
+    st = make_pool_tensor_map(&tv, a.pool_v, a.num_pages, a.num_kv_heads, a.head_dim);
+    if (st != LKV_OK) return st;
+  } else {  // no bf16 pages: keys past a row's end read as zeros past the stage
+    tk = stage.k;
+    tv = stage.v;
+  }
   // The output has the query's [token][head][dim] geometry: full tiles are stored
   // a warp's 32 rows at a time (unused when the map cannot be built).
   CUtensorMap to;
@@ -562,7 +678,8 @@ int prefill_paged(const PrefillArgs& a) {
   prm.Hq = a.num_q_heads;
   prm.Hkv = a.num_kv_heads;
   prm.W = a.max_pages_per_seq;
-  prm.num_pages = a.num_pages;
+  // (ids past the map's end read as zeros)
+  prm.num_pages = pool ? a.num_pages : (int64_t)a.stage_width * a.batch;
   prm.causal = a.causal ? 1 : 0;
   prm.scale_log2 = a.softmax_scale * 1.4426950408889634f;
   prm.S = S;
@@ -570,9 +687,17 @@ int prefill_paged(const PrefillArgs& a) {
   prm.part_lse = a.part_lse;
   prm.part_rows = (int64_t)a.total_q * a.num_q_heads;
   prm.tma_out = tma_out;
+  prm.num_q8 = a.num_q8;
+  prm.q8_scales = a.q8_scales;
+  prm.q8_pages = a.q8_pages;
+  prm.stage_width = a.stage_width;
+  prm.has_pool = pool;
   cudaStream_t stream = static_cast<cudaStream_t>(a.stream);
   int rc = LKV_OK;
-#define LKV_PF(DD, GG) rc = launch_prefill<DD, GG>(tq, tk, tv, to, prm, a.max_q, stream); break
+#define LKV_PF(DD, GG)                                                                        \
+  rc = q8 ? launch_prefill<DD, GG, true>(tq, tk, tv, to, stage, prm, a.max_q, stream)          \
+          : launch_prefill<DD, GG, false>(tq, tk, tv, to, NoStageMaps{}, prm, a.max_q, stream); \
+  break
   if (a.head_dim == 128) {
     switch (group) {
       case 1: LKV_PF(128, 1);

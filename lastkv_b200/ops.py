@@ -1032,3 +1032,352 @@ def cp_combine(send, recv_ptrs, rank: int, world: int, state, rows: int, head_di
                                     _ptr(out_scale), out.data_ptr(), out.stride(0), _ptr(error_word), _stream())
     _capi.check(st, "lkv_cp_combine")
     return out
+
+
+# ------------------------------------------------------------------ 8-bit pages
+
+_I32, _I64, _BOOL = torch.int32, torch.int64, torch.bool
+
+
+def _here(t, what: str) -> None:
+    """A call runs on the current device's stream, so its tensors have to be there."""
+    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+        _fail(f"{what} must be on the current CUDA device, got {t.device}")
+
+
+def _ints(t, n: int, what: str) -> int:
+    """Address of at least n int32 on the device."""
+    if t.dtype != _I32 or t.numel() < n or not t.is_contiguous():
+        _fail(f"{what} must be contiguous CUDA int32 [>= {n}], got {t.dtype} {tuple(t.shape)}")
+    _here(t, what)
+    return t.data_ptr()
+
+
+class PagesQ8(NamedTuple):
+    """Pages of 16 tokens' keys and values in 8 bits, with an fp32 scale for every 8 tokens of a
+    head: ``codes`` int8 [pages, Hkv, 2 (K, V), 16 * D] in the kernels' order (``from_codes`` and
+    ``to_codes`` translate) and ``scales`` fp32 [pages, Hkv, 4] (K of tokens 0-7, K of 8-15, V, V)."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @property
+    def num_pages(self) -> int:
+        return self.codes.shape[0]
+
+    @property
+    def num_kv_heads(self) -> int:
+        return self.codes.shape[1]
+
+    @property
+    def head_dim(self) -> int:
+        return self.codes.shape[3] // PAGE_SIZE
+
+    @classmethod
+    def empty(cls, num_pages: int, num_kv_heads: int, head_dim: int, device="cuda") -> "PagesQ8":
+        """Pages of zeros."""
+        require_heads(num_kv_heads, num_kv_heads, head_dim)
+        return cls(torch.zeros((num_pages, num_kv_heads, 2, PAGE_SIZE * head_dim), dtype=_I8, device=device),
+                   torch.zeros((num_pages, num_kv_heads, 4), dtype=_F32, device=device))
+
+    @classmethod
+    def from_codes(cls, k, v, k_scale, v_scale) -> "PagesQ8":
+        """From codes int8 [pages, 16, Hkv, D] and scales fp32 [pages, 2, Hkv] of K and V."""
+        _require(k.dtype == _I8 and v.dtype == _I8 and k.dim() == 4 and k.shape == v.shape
+                 and k.shape[1] == PAGE_SIZE and k.shape[3] in (64, 128), "codes must be int8 [pages, 16, Hkv, 64 or 128]")
+        n, _, h, d = k.shape
+        _require(all(s.dtype == _F32 and s.shape == (n, 2, h) for s in (k_scale, v_scale)),
+                 "scales must be fp32 [pages, 2, Hkv]")
+        codes = torch.empty((n, h, 2, PAGE_SIZE * d), dtype=_I8, device=k.device)
+        # [page, h, g, head, j / 2, j % 2, t1, c, t0] -> [page, head, j / 2, g, c, j % 2, h, t0, t1]
+        codes[:, :, 0] = k.view(n, 2, 8, h, d // 32, 2, 2, 4, 2).permute(0, 3, 4, 2, 7, 5, 1, 8, 6).reshape(n, h, -1)
+        # [page, h, c, t, head, k / 2, k % 2, m, g] -> [page, head, k / 2, g, c, k % 2, h, t, m]
+        codes[:, :, 1] = v.view(n, 2, 4, 2, h, d // 32, 2, 2, 8).permute(0, 4, 5, 8, 2, 6, 1, 3, 7).reshape(n, h, -1)
+        return cls(codes, torch.cat((k_scale, v_scale), 1).transpose(1, 2).contiguous())
+
+    def to_codes(self):
+        """(k, v, k_scale, v_scale) as ``from_codes`` takes them."""
+        n, h, d = self.num_pages, self.num_kv_heads, self.head_dim
+        k = self.codes[:, :, 0].view(n, h, d // 32, 8, 4, 2, 2, 2, 2).permute(0, 6, 3, 1, 2, 5, 8, 4, 7)
+        v = self.codes[:, :, 1].view(n, h, d // 32, 8, 4, 2, 2, 2, 2).permute(0, 6, 4, 7, 1, 2, 5, 8, 3)
+        return (k.reshape(n, PAGE_SIZE, h, d), v.reshape(n, PAGE_SIZE, h, d), *self.token_scales())
+
+    def token_scales(self):
+        """Views (k_scale, v_scale) [pages, 2, Hkv] of the scales."""
+        return self.scales[..., :2].transpose(1, 2), self.scales[..., 2:].transpose(1, 2)
+
+
+def _check_pages_q8(c) -> None:
+    if type(c) is not PagesQ8:
+        _fail("the 8-bit pages must be PagesQ8")
+    codes, scales = c
+    if codes.dtype != _I8 or codes.dim() != 4 or codes.shape[2] != 2 or codes.shape[3] not in (1024, 2048) \
+            or not codes.is_contiguous():
+        _fail("PagesQ8.codes must be contiguous int8 [pages, Hkv, 2, 16 * D] with D 64 or 128")
+    if scales.dtype != _F32 or scales.shape != (codes.shape[0], codes.shape[1], 4) or not scales.is_contiguous():
+        _fail("PagesQ8.scales must be contiguous fp32 [pages, Hkv, 4]")
+    _here(codes, "PagesQ8.codes")
+    _here(scales, "PagesQ8.scales")
+
+
+def _check_both(pool_k, pool_v, c) -> None:
+    _check_pool(pool_k, pool_v)
+    _here(pool_k, "pool_k")
+    _here(pool_v, "pool_v")
+    if pool_k.shape[2] != c.num_kv_heads or pool_k.shape[3] != c.head_dim:
+        _fail(f"pools of {pool_k.shape[2]} heads x {pool_k.shape[3]} against 8-bit pages of {c.num_kv_heads} x {c.head_dim}")
+
+
+@_traced
+def quantize_pages(pool_k, pool_v, pages, cache: PagesQ8, out_pages, *, tokens=None, error_word=None) -> None:
+    """Pages ``pages[i]`` of a bf16 pool into 8-bit pages ``out_pages[i]`` (int32 [n] on the device;
+    lkv_q8_quantize_pages).  ``tokens`` int32 [n]: how many tokens of each page count (the rest
+    become zeros); None: 16.  No two ``out_pages`` may be the same."""
+    _check_pages_q8(cache)
+    _check_both(pool_k, pool_v, cache)
+    n = pages.numel()
+    if out_pages.numel() != n or (tokens is not None and tokens.numel() != n):
+        _fail("pages, out_pages and tokens must have the same length")
+    st = _capi.lib().lkv_q8_quantize_pages(
+        pool_k.data_ptr(), pool_v.data_ptr(), pool_k.shape[0], _ints(pages, n, "pages"),
+        None if tokens is None else _ints(tokens, n, "tokens"), cache.codes.data_ptr(), cache.scales.data_ptr(),
+        cache.num_pages, _ints(out_pages, n, "out_pages"), n, cache.num_kv_heads, cache.head_dim, _err_ptr(error_word),
+        _stream())
+    if st:
+        _capi.check(st, "lkv_q8_quantize_pages")
+
+
+@_traced
+def dequantize_pages(cache: PagesQ8, pages, pool_k, pool_v, out_pages, *, error_word=None) -> None:
+    """8-bit pages ``pages[i]`` into pages ``out_pages[i]`` of a bf16 pool, bf16(code * scale)."""
+    _check_pages_q8(cache)
+    _check_both(pool_k, pool_v, cache)
+    n = pages.numel()
+    if out_pages.numel() != n:
+        _fail("pages and out_pages must have the same length")
+    st = _capi.lib().lkv_q8_dequantize_pages(
+        cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_pages, _ints(pages, n, "pages"), pool_k.data_ptr(),
+        pool_v.data_ptr(), pool_k.shape[0], _ints(out_pages, n, "out_pages"), n, cache.num_kv_heads, cache.head_dim,
+        _err_ptr(error_word), _stream())
+    if st:
+        _capi.check(st, "lkv_q8_dequantize_pages")
+
+
+def _check_attend(q, cache, block_table, seq_k, num_q8, pool_k, pool_v, B, out, out_scale, lse, max_pages):
+    """What decode and prefill over 8-bit pages check alike; (width, out)."""
+    _check_pages_q8(cache)
+    if q.dim() != 3 or q.dtype != _BF16 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
+        _fail("q must be bf16 [rows, Hq, D] rows")
+    _here(q, "q")
+    T, Hq, D = q.shape
+    require_heads(Hq, cache.num_kv_heads, D)
+    if D != cache.head_dim:
+        _fail(f"head_dim {D} of q against {cache.head_dim} of the 8-bit pages")
+    if (pool_k is None) != (pool_v is None):
+        _fail("pool_k and pool_v come together")
+    if pool_k is not None:
+        _check_both(pool_k, pool_v, cache)
+    if block_table.dtype != _I32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.shape[0] < B:
+        _fail("block_table must be int32 [>= B, W] with unit column stride")
+    _here(block_table, "block_table")
+    W = block_table.shape[1] if max_pages is None else int(max_pages)
+    if not 0 <= W <= block_table.shape[1]:
+        _fail("max_pages exceeds block_table width")
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=_BF16, device=q.device)
+    elif out.dtype != _BF16 or out.shape != (T, Hq, D) or out.stride(2) != 1 or out.stride(1) != D \
+            or (T > 1 and out.stride(0) < Hq * D):
+        _fail("out must be bf16 [rows, Hq, D] rows")
+    _here(out, "out")
+    if out_scale is not None:
+        if out_scale.dtype != _F32 or out_scale.numel() != Hq or not out_scale.is_contiguous():
+            _fail("out_scale must be fp32 [Hq]")
+        _here(out_scale, "out_scale")
+    if lse is not None:
+        if lse.dtype != _F32 or lse.numel() != T * Hq or not lse.is_contiguous():
+            _fail("lse must be contiguous fp32 [rows, Hq]")
+        _here(lse, "lse")
+    return W, out
+
+
+def _row_stride(t) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+@_traced
+def decode_paged_q8(q, cache: PagesQ8, block_table, seq_k, *, num_q8=None, pool_k=None, pool_v=None,
+                    softmax_scale=None, out=None, lse=None, out_scale=None, workspace: Workspace | None = None,
+                    max_pages: int | None = None, l2_keep: bool = False):
+    """One query token per sequence over a cache whose older pages are in 8 bits (lkv_decode_paged_q8).
+
+    q [B, Hq, D] bf16 (row-strided views allowed); block_table int32 [B, W]: the first ``num_q8[b]``
+    (int32 [B]; None: all) columns are pages of ``cache``, the rest pages of ``pool_k`` / ``pool_v``;
+    seq_k int32 [B].  Returns out [B, Hq, D] bf16.  ``lse`` (fp32 [B, Hq]) receives the log-sum-exp.
+    Calls that overlap need a workspace each.
+    """
+    B, Hq, D = q.shape if q.dim() == 3 else _fail("q must be bf16 [rows, Hq, D] rows")
+    W, out = _check_attend(q, cache, block_table, seq_k, num_q8, pool_k, pool_v, B, out, out_scale, lse, max_pages)
+    if workspace is None:
+        workspace = Workspace.for_decode(B, Hq, D, W, device=q.device)
+    _here(workspace.buf, "workspace")
+    st = _capi.lib().lkv_decode_paged_q8(
+        q.data_ptr(), _row_stride(q), cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_pages, _ptr(pool_k),
+        _ptr(pool_v), 0 if pool_k is None else pool_k.shape[0], block_table.data_ptr(), block_table.stride(0),
+        None if num_q8 is None else _ints(num_q8, B, "num_q8"), _ints(seq_k, B, "seq_k"), out.data_ptr(),
+        _row_stride(out), _ptr(lse), _ptr(out_scale), B, Hq, cache.num_kv_heads, D, W,
+        D ** -0.5 if softmax_scale is None else float(softmax_scale), workspace.ptr(), workspace.nbytes,
+        DECODE_L2_KEEP if l2_keep else 0, _stream())
+    if st:
+        _capi.check(st, "lkv_decode_paged_q8")
+    return out
+
+
+class StageQ8(NamedTuple):
+    """Workspace of ``prefill_paged_q8``: the codes of each row's 8-bit pages as bf16, page
+    ``row * width + column`` of ``k`` and ``v`` [batch * width, 16, Hkv, D]."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    width: int
+
+    @classmethod
+    def empty(cls, batch: int, width: int, num_kv_heads: int, head_dim: int, device="cuda") -> "StageQ8":
+        """For ``batch`` rows of at most ``width`` 8-bit pages."""
+        width = max(int(width), 1)
+        k, v = (torch.empty((max(batch, 1) * width, PAGE_SIZE, num_kv_heads, head_dim), dtype=_BF16, device=device)
+                for _ in range(2))
+        return cls(k, v, width)
+
+
+@_traced
+def prefill_paged_q8(q, cache: PagesQ8, block_table, seq_k, cu_q, max_q: int, *, num_q8=None, pool_k=None,
+                     pool_v=None, causal=True, softmax_scale=None, out=None, lse=None, out_scale=None,
+                     stage: StageQ8 | None = None, staged: bool = False, error_word=None,
+                     max_pages: int | None = None):
+    """``prefill_paged`` over a cache whose older pages are in 8 bits (lkv_prefill_paged_q8).
+
+    The arguments of ``prefill_paged``, with the pages as in ``decode_paged_q8``.  The 8-bit pages'
+    codes are first copied to ``stage`` as bf16 (lkv_q8_stage_pages); ``staged=True`` says that an
+    earlier call with the same rows and pages did that (the layers of one step), and skips it.
+    A row may have at most ``stage.width`` 8-bit pages.
+    """
+    B = cu_q.numel() - 1
+    if B < 0:
+        _fail("cu_q must be int32 [B + 1]")
+    W, out = _check_attend(q, cache, block_table, seq_k, num_q8, pool_k, pool_v, B, out, out_scale, lse, max_pages)
+    T, Hq, D = q.shape
+    if stage is None:
+        if staged:
+            _fail("staged=True needs the stage of the earlier call")
+        stage = StageQ8.empty(B, W, cache.num_kv_heads, D, device=q.device)
+    _check_both(stage.k, stage.v, cache)
+    width = min(stage.width, W)
+    if stage.width < 1 or stage.k.shape[0] < B * stage.width:
+        _fail(f"the stage holds {stage.k.shape[0]} pages, {B} rows of {stage.width} were asked for")
+    args = (block_table.data_ptr(), block_table.stride(0), None if num_q8 is None else _ints(num_q8, B, "num_q8"),
+            _ints(seq_k, B, "seq_k"))
+    err, cu = _err_ptr(error_word), _ints(cu_q, B + 1, "cu_q")
+    if not staged:
+        st = _capi.lib().lkv_q8_stage_pages(
+            cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_pages, *args, B, W, stage.k.data_ptr(),
+            stage.v.data_ptr(), width, cache.num_kv_heads, D, err, _stream())
+        if st:
+            _capi.check(st, "lkv_q8_stage_pages")
+    st = _capi.lib().lkv_prefill_paged_q8(
+        q.data_ptr(), _row_stride(q), stage.k.data_ptr(), stage.v.data_ptr(), max(width, 1), cache.scales.data_ptr(),
+        cache.num_pages, _ptr(pool_k), _ptr(pool_v), 0 if pool_k is None else pool_k.shape[0], *args, cu,
+        out.data_ptr(), _row_stride(out), _ptr(lse), _ptr(out_scale), B, T, int(max_q), Hq, cache.num_kv_heads, D, W,
+        int(bool(causal)), D ** -0.5 if softmax_scale is None else float(softmax_scale), err, _stream())
+    if st:
+        _capi.check(st, "lkv_prefill_paged_q8")
+    return out
+
+
+# ------------------------------------------------------------------ beam search
+
+
+@_traced
+def reorder_pages(pools, src_pages, dst_pages, *, layers: int = 1, layer_stride: int = 0, error_word=None) -> None:
+    """``pool[dst_pages[i]] = pool[src_pages[i]]`` for all i at once, in every pool (lkv_reorder_pages).
+
+    pools: up to 8 contiguous tensors whose first dimension is the page (16-byte pages and up); the
+    lists (int32 [n] on the device, n <= 2048) may permute pages among themselves.  With ``layers``
+    the same is done at the ids plus ``l * layer_stride`` for each layer l, ids below ``layer_stride``.
+    No two ``dst_pages`` may be the same.
+    """
+    pools = (pools,) if isinstance(pools, torch.Tensor) else tuple(pools)
+    n = src_pages.numel()
+    if dst_pages.numel() != n:
+        _fail("src_pages and dst_pages must have the same length")
+    if not 1 <= len(pools) <= 8:
+        _fail(f"reorder_pages takes 1 to 8 pools, got {len(pools)}")
+    for t in pools:
+        if t.dim() < 1 or not t.is_contiguous():
+            _fail("pools must be contiguous, the page their first dimension")
+        _here(t, "a pool")
+    sizes = [t[0].numel() * t.element_size() if t.shape[0] else 0 for t in pools]
+    N = len(pools)
+    st = _capi.lib().lkv_reorder_pages(
+        (ctypes.c_void_p * N)(*(t.data_ptr() for t in pools)), (ctypes.c_int64 * N)(*sizes),
+        (ctypes.c_int64 * N)(*(t.shape[0] for t in pools)), N, _ints(src_pages, n, "src_pages"),
+        _ints(dst_pages, n, "dst_pages"), n, int(layers), int(layer_stride), _err_ptr(error_word), _stream())
+    if st:
+        _capi.check(st, "lkv_reorder_pages")
+
+
+class BeamChoice(NamedTuple):
+    """The candidates that ``beam_select`` chose, [B, select] each, best first."""
+
+    scores: torch.Tensor    # fp32 totals
+    rows: torch.Tensor      # int64: the row b * K + beam that a candidate continues
+    tokens: torch.Tensor    # int64
+    finished: torch.Tensor  # bool: the end token, now or before
+
+    @classmethod
+    def empty(cls, batch: int, select: int, device="cuda") -> "BeamChoice":
+        return cls(*(torch.empty((batch, select), dtype=t, device=device) for t in (_F32, _I64, _I64, _BOOL)))
+
+
+@_traced
+def beam_select(logits, scores, *, select: int | None = None, finished=None, eos_token: int | None = None,
+                out: BeamChoice | None = None) -> BeamChoice:
+    """The ``select`` (default: as many as beams) best continuations of each batch item (lkv_beam_select).
+
+    logits [B * K, V] bf16 or fp32 rows (any row stride); scores fp32 [B, K], the beams' summed
+    log-probabilities.  Candidates are ordered by ``scores + log_softmax(logits)``, equal ones by beam
+    and token.  ``finished`` bool [B, K]: such a beam continues with ``eos_token`` alone, at its score.
+    ``out``: buffers to write (a captured step's).
+    """
+    if scores.dtype != _F32 or scores.dim() != 2 or not scores.is_contiguous():
+        _fail("scores must be contiguous CUDA fp32 [B, K]")
+    _here(scores, "scores")
+    B, K = scores.shape
+    if logits.dtype not in (_BF16, _F32) or logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[0] != B * K:
+        _fail(f"logits must be bf16 or fp32 [{B * K}, V] rows")
+    _here(logits, "logits")
+    n = K if select is None else int(select)
+    if not (1 <= n <= 32 and n <= logits.shape[1] and 1 <= K <= 64 and B * K <= 65535):
+        _fail(f"beam_select takes 1 to 32 candidates of at least as many tokens, 1 to 64 beams and 65535 rows, got "
+              f"select {n}, {K} beams, {tuple(logits.shape)}")
+    eos = -1 if eos_token is None else int(eos_token)
+    if finished is not None:
+        if finished.dtype != _BOOL or finished.shape != (B, K) or not finished.is_contiguous():
+            _fail(f"finished must be contiguous bool [{B}, {K}]")
+        _here(finished, "finished")
+        if not 0 <= eos < logits.shape[1]:
+            _fail("finished beams need an eos_token of the vocabulary")
+    if out is None:
+        out = BeamChoice.empty(B, n, scores.device)
+    for t, like in zip(out, (_F32, _I64, _I64, _BOOL)):
+        if t.dtype != like or t.shape != (B, n) or not t.is_contiguous():
+            _fail(f"out must be a BeamChoice of contiguous [{B}, {n}] tensors")
+        _here(t, "out")
+    nbytes = _capi.lib().lkv_beam_workspace_bytes(B * K, n)
+    work = torch.empty(nbytes, dtype=_U8, device=scores.device)
+    st = _capi.lib().lkv_beam_select(
+        logits.data_ptr(), logits.stride(0), int(logits.dtype == _F32), scores.data_ptr(), _ptr(finished), eos, B, K,
+        logits.shape[1], n, out.scores.data_ptr(), out.rows.data_ptr(), out.tokens.data_ptr(), out.finished.data_ptr(),
+        work.data_ptr(), nbytes, _stream())
+    if st:
+        _capi.check(st, "lkv_beam_select")
+    return out
