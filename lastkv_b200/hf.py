@@ -24,7 +24,9 @@ Dense layers (projections, MLP, norms, embedding, LM head) are plain torch
 from __future__ import annotations
 
 import math
+from contextlib import contextmanager
 from dataclasses import dataclass, field
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -305,12 +307,31 @@ class PagedLastKVCache:
     sequence at ``ring_base[l] + b * ring_pages`` holding K and V / s_l.
     ``seen_tokens``, ``get_seq_length`` and ``reorder_cache`` keep the
     reference's meaning (modeling.py:56-67).
+
+    ``history="int8"`` (bf16 caches): the shared history is held in 8 bits (``q8``, an
+    ``ops.PagesQ8``), half its memory and of what a decode step reads of it.  A chunk's raw K and V
+    go to a ring of 2C tokens per sequence in front of the layers' rings and are rounded to 8 bits
+    when the chunk is finished, a scale for every 8 tokens of a head; the previous and current
+    chunk stay bf16, and so does the blend.
+
+    After ``reorder_cache`` rows share the pages that their common tokens filled (``src_table``,
+    ``ring_table``): a page is written by one row and read by any, and every row writes its own
+    pages, those of a cache that was never reordered.
     """
 
+    #: bf16 copies of 8-bit pages that a prefill call may hold at once (``history="int8"``); rows beyond
+    #: that are taken in turns
+    stage_bytes = 2 << 30
+
     def __init__(self, config: LastKVConfig, batch: int, max_tokens: int, device=None, *, page_order=None,
-                 dtype=torch.bfloat16):
+                 dtype=torch.bfloat16, history: str | None = None):
         if dtype not in (torch.bfloat16, torch.float32):
             raise RMarinBackendContractError("the paged cache holds bf16 or fp32 keys and values")
+        if history not in (None, "int8"):
+            raise RMarinBackendContractError(f"history must be None or 'int8', got {history!r}")
+        if history is not None and dtype != torch.bfloat16:
+            raise RMarinBackendContractError("a history in 8 bits needs a bf16 cache")
+        self.history = history
         self.dtype = dtype
         self.num_layers = config.num_hidden_layers
         self.chunk_size = config.chunk_size
@@ -326,17 +347,24 @@ class PagedLastKVCache:
         self.pages_per_seq = -(-max_tokens // PAGE_SIZE)
         self.ring_pages = 2 * C // PAGE_SIZE
         self.ring_tokens = 2 * C
-        self.src_pages = batch * self.pages_per_seq
+        shared = batch * self.pages_per_seq
         self.ring_stride = self.ring_pages * batch + 1
+        # pages in front of the layers' rings: the shared history, or with an 8-bit one the raw ring
+        self.src_pages = shared if history is None else self.ring_stride
         self.num_pages = self.src_pages + self.num_layers * self.ring_stride
         shape = (self.num_pages, PAGE_SIZE, self.hkv, self.d)
         self.pool_k = torch.zeros(shape, dtype=dtype, device=device)
         self.pool_v = torch.zeros(shape, dtype=dtype, device=device)
-        order = np.arange(self.src_pages) if page_order is None else np.asarray(page_order)
-        if sorted(order.tolist()) != list(range(self.src_pages)):
+        self.q8 = None if history is None else ops.PagesQ8.empty(shared, self.hkv, self.d, device=device)
+        order = np.arange(shared) if page_order is None else np.asarray(page_order)
+        if sorted(order.tolist()) != list(range(shared)):
             raise RMarinBackendContractError("page_order must permute the shared pages")
         self.src_table = order.reshape(batch, self.pages_per_seq).astype(np.int32)
+        self._own_src = self.src_table  # the pages that each row writes (src_table_dev on the device)
         self.src_table_dev = torch.from_numpy(self.src_table).to(device)
+        self._own_ring = np.arange(batch * self.ring_pages, dtype=np.int32).reshape(batch, self.ring_pages)
+        self.ring_table = self._own_ring.copy()  # relative to a layer's ring
+        self._rows = np.arange(batch)  # the rows that spans are planned for (only_rows)
         self.ring_base = self.src_pages + np.arange(self.num_layers) * self.ring_stride
         self.ring_base_dev = torch.from_numpy(self.ring_base.astype(np.int32)).to(device)
         self.error_word = torch.zeros(4, dtype=torch.int32, device=device)
@@ -362,6 +390,9 @@ class PagedLastKVCache:
         self.flush_commit()
         B, L, P = self.batch, self.num_layers, PAGE_SIZE
         pps = -(-max_tokens // P)
+        if self.q8 is not None:
+            self._reserve_q8(max_tokens, pps)
+            return
         src_pages = B * pps
         num_pages = src_pages + L * self.ring_stride
         table = np.arange(src_pages, dtype=np.int32).reshape(B, pps)
@@ -381,7 +412,7 @@ class PagedLastKVCache:
         self.pages_per_seq = pps
         self.src_pages = src_pages
         self.num_pages = num_pages
-        self.src_table = table
+        self.src_table = self._own_src = table
         self.src_table_dev = torch.from_numpy(table).to(self.device)
         self.ring_base = ring_base
         self.ring_base_dev = torch.from_numpy(ring_base.astype(np.int32)).to(self.device)
@@ -389,25 +420,108 @@ class PagedLastKVCache:
             self.workspace = ops.Workspace.for_decode(B, self._hq, self.d, pps + self.ring_pages, device=self.device)
         self._meta = None
 
+    def _reserve_q8(self, max_tokens: int, pps: int) -> None:
+        """``reserve`` of an 8-bit history: new 8-bit pages in sequence order, the rings as they are."""
+        B = self.batch
+        table = np.arange(B * pps, dtype=np.int32).reshape(B, pps)
+        old = torch.from_numpy(self.src_table.reshape(-1).astype(np.int64)).to(self.device)
+        new = torch.from_numpy(table[:, : self.pages_per_seq].reshape(-1).astype(np.int64)).to(self.device)
+        grown = ops.PagesQ8.empty(B * pps, self.hkv, self.d, device=self.device)
+        for a, b in zip(grown, self.q8):
+            a[new] = b.index_select(0, old)
+        self.q8 = grown
+        self.max_tokens, self.pages_per_seq = max_tokens, pps
+        self.src_table = self._own_src = table
+        self.src_table_dev = torch.from_numpy(table).to(self.device)
+        self.workspace = ops.Workspace.for_decode(B, self._hq, self.d, pps + self.ring_pages, device=self.device)
+        self._meta = None
+
     # -- reference API
     def get_seq_length(self, layer_idx=0):
         return self.seen_tokens
 
     def reorder_cache(self, beam_idx):
-        """Reorder sequences (beam search): gather shared pages and rings by beam index."""
+        """Reorder sequences (beam search): row b goes on as row ``beam_idx[b]`` was.
+
+        Rows share the pages that are full; the page that is being written is copied, for the rows that
+        change, in the history and in every layer's ring (``ops.reorder_pages``)."""
+        idx = torch.as_tensor(beam_idx).to("cpu").long().numpy().reshape(-1)
+        if idx.shape[0] != self.batch or (idx.size and (idx.min() < 0 or idx.max() >= self.batch)):
+            raise RMarinBackendContractError(f"beam_idx must name {self.batch} of the cache's rows")
         self.flush_commit()
-        idx = beam_idx.to("cpu").long().numpy()
-        src_old = self.src_table[idx].reshape(-1)
-        src_new = self.src_table.reshape(-1)
-        ring_old = (idx[:, None] * self.ring_pages + np.arange(self.ring_pages)[None]).reshape(-1)
-        ring_new = (np.arange(self.batch)[:, None] * self.ring_pages + np.arange(self.ring_pages)[None]).reshape(-1)
-        old = [src_old] + [self.ring_base[l] + ring_old for l in range(self.num_layers)]
-        new = [src_new] + [self.ring_base[l] + ring_new for l in range(self.num_layers)]
-        o = torch.from_numpy(np.concatenate(old)).to(self.device)
-        n = torch.from_numpy(np.concatenate(new)).to(self.device)
-        for pool in (self.pool_k, self.pool_v):
-            pool[n] = pool.index_select(0, o)
+        C, P, RP = self.chunk_size, PAGE_SIZE, self.ring_pages
+        full = self.seen_tokens // P
+        old_src, old_ring = self.src_table, self.ring_table
+        # the history's finished pages; an 8-bit one has those of finished chunks
+        done = full if self.q8 is None else self.committed // P
+        self.src_table = np.concatenate((old_src[idx, :done], self._own_src[:, done:]), axis=1)
+        # the rings' pages that the next span reads
+        live = np.arange(max(0, self.seen_tokens // C * C - C) // P, full) % RP
+        self.ring_table = self._own_ring.copy()
+        self.ring_table[:, live] = old_ring[idx][:, live]
+        if self.seen_tokens % P:
+            self._copy_pages(old_ring[idx, full % RP], self._own_ring[:, full % RP], ring=True)
+            if self.q8 is None:
+                self._copy_pages(old_src[idx, full], self._own_src[:, full], ring=False)
         self._meta = None
+
+    def _copy_pages(self, src, dst, *, ring: bool) -> None:
+        """Pages src[i] to dst[i], all at once: relative pages of every layer's ring (and of the raw one), or
+        shared pages."""
+        layers, pools = 1, (self.pool_k, self.pool_v)
+        if not ring and self.q8 is not None:
+            pools = tuple(self.q8)
+        elif ring:
+            layers = self.num_layers + (self.q8 is not None)
+            first = 0 if self.q8 is not None else self.src_pages
+            pools = self.pool_k[first:], self.pool_v[first:]
+        keep = src != dst
+        s, d = (torch.from_numpy(np.ascontiguousarray(t[keep], dtype=np.int32)).to(self.device) for t in (src, dst))
+        if not s.numel():
+            return
+        if self.device.type == "cuda" and s.numel() <= 2048:
+            ops.reorder_pages(pools, s, d, layers=layers, layer_stride=self.ring_stride if layers > 1 else 0,
+                              error_word=self.error_word)
+            return
+        at = (torch.arange(layers, device=self.device) * self.ring_stride)[:, None]
+        for p in pools:
+            p[at + d.long()] = p[at + s.long()]
+
+    @property
+    def shared(self) -> bool:
+        """Whether rows read pages of one another (after ``reorder_cache``)."""
+        return not (np.array_equal(self.src_table, self._own_src) and np.array_equal(self.ring_table, self._own_ring))
+
+    def unshare_(self) -> None:
+        """Copy what rows share to pages of their own, so that row b's pages are those of a cache that was never
+        reordered (as a device-side step plan takes them)."""
+        if not self.shared:
+            return
+        self.flush_commit()
+        for ring, table, own in ((True, self.ring_table, self._own_ring), (False, self.src_table, self._own_src)):
+            # a column's pages are shared among its rows alone, so whole columns can be copied at once
+            columns = np.flatnonzero((table != own).any(0))
+            step = max(1, 2048 // self.batch)
+            for i in range(0, len(columns), step):
+                at = columns[i:i + step]
+                self._copy_pages(table[:, at].reshape(-1), own[:, at].reshape(-1), ring=ring)
+        self.ring_table, self.src_table = self._own_ring.copy(), self._own_src
+        self._meta = None
+
+    @contextmanager
+    def only_rows(self, rows):
+        """Spans inside the block are those of ``rows`` alone, in that order (a prompt that several rows will go on
+        from); the other rows' contents are then stale until ``reorder_cache`` gives them one of these."""
+        rows = np.asarray(rows, dtype=np.int64).reshape(-1)
+        if not rows.size or rows.min() < 0 or rows.max() >= self.batch or len(set(rows.tolist())) != rows.size:
+            raise RMarinBackendContractError(f"rows must name different rows of the {self.batch}")
+        self.flush_commit()
+        before, self._rows, self._meta = self._rows, rows, None
+        try:
+            yield self
+        finally:
+            self.flush_commit()
+            self._rows, self._meta = before, None
 
     # -- per-span metadata (shared by all layers of one chunk piece)
     def plan_host(self, n_new: int) -> dict:
@@ -424,22 +538,26 @@ class PagedLastKVCache:
         nsrc = rec // P
         window = last + 1 - rec
         npages = -(-window // P)
-        first = (rec // P) % self.ring_pages
-        B = self.batch
+        RP, rows = self.ring_pages, self._rows
+        # pages that this span begins: their columns hold pages that no span reads any more
+        begun = np.arange(-(-start // P), last // P + 1) % RP
+        self.ring_table[:, begun] = self._own_ring[:, begun]
         W = nsrc + npages
-        bt = np.zeros((B, W), np.int32)
-        for b in range(B):
-            bt[b, :nsrc] = self.src_table[b, :nsrc]
-            bt[b, nsrc:] = b * self.ring_pages + (first + np.arange(npages)) % self.ring_pages
+        bt = np.zeros((len(rows), W), np.int32)
+        bt[:, :nsrc] = self.src_table[rows, :nsrc]
+        bt[:, nsrc:] = self.ring_table[rows][:, (rec // P + np.arange(npages)) % RP]
         pos = start + np.arange(n_new)
-        ring_tok = (np.arange(B)[:, None] * self.ring_tokens + (pos % self.ring_tokens)[None, :]).reshape(-1)
-        src_tok = (self.src_table[:, pos // P] * P + (pos % P)[None, :]).reshape(-1)
+        ring_tok = (self.ring_table[rows][:, pos // P % RP].astype(np.int64) * P + (pos % P)[None, :]).reshape(-1)
+        if self.q8 is None:
+            src_tok = (self.src_table[rows][:, pos // P].astype(np.int64) * P + (pos % P)[None, :]).reshape(-1)
+        else:
+            src_tok = ring_tok  # the raw ring, in front of the layers' rings
         return {"bt": bt, "nsrc": nsrc, "W": W, "seq_k": last + 1, "ring_tok": ring_tok.astype(np.int64),
                 "src_tok": src_tok.astype(np.int64)}
 
     def plan(self, n_new: int):
         h = self.plan_host(n_new)
-        B, dev = self.batch, self.device
+        B, dev = len(self._rows), self.device
         # block tables are padded to the maximum width, so the decode kernel's
         # split plan is the same at every position (and in captured graphs)
         w_max = self.pages_per_seq + self.ring_pages
@@ -448,7 +566,7 @@ class PagedLastKVCache:
         bt_d = torch.from_numpy(bt).to(dev)
         nsrc_d = torch.full((B,), h["nsrc"], dtype=torch.int32, device=dev)
         meta = {
-            "n": n_new, "W": w_max,
+            "n": n_new, "W": w_max, "nsrc": nsrc_d, "older": h["nsrc"],
             "bt_all": ops.build_layer_block_tables(bt_d, nsrc_d, self.ring_base_dev),
             "seq_k": torch.full((B,), h["seq_k"], dtype=torch.int32, device=dev),
             "cu_q": torch.arange(0, (B + 1) * n_new, n_new, dtype=torch.int32, device=dev),
@@ -476,10 +594,17 @@ class PagedLastKVCache:
         if end != self.committed + C:
             raise RMarinBackendContractError("boundary commits must be contiguous and exactly one chunk")
         pages = np.arange((end - C) // P, end // P)
-        raw = self.src_table[:, pages]
-        ring_first = ((end - C) % self.ring_tokens) // P
-        ring = (self.ring_base[0] + np.arange(self.batch)[:, None] * self.ring_pages
-                + ring_first + np.arange(C // P)[None, :])
+        ring = self.ring_table[self._rows][:, pages % self.ring_pages]
+        raw = self.src_table[self._rows][:, pages] if self.q8 is None else ring
+        if self.q8 is not None:  # the finished chunk in 8 bits, each row to its own pages
+            out = self._own_src[self._rows][:, pages]
+            lists = [torch.from_numpy(np.ascontiguousarray(t.reshape(-1), dtype=np.int32)).to(self.device)
+                     for t in (raw, out)]
+            ops.quantize_pages(self.pool_k, self.pool_v, lists[0], self.q8, lists[1], error_word=self.error_word)
+        _, once = np.unique(ring.reshape(-1), return_index=True)
+        if once.size < ring.size:  # rows share pages: each is blended once
+            raw, ring = (t.reshape(-1)[np.sort(once)][:, None] for t in (raw, ring))
+        ring = self.ring_base[0] + ring
         raw_d = torch.from_numpy(np.ascontiguousarray(raw, dtype=np.int32)).to(self.device)
         ring_d = torch.from_numpy(np.ascontiguousarray(ring, dtype=np.int32)).to(self.device)
         self.flush_commit()
@@ -501,6 +626,32 @@ class PagedLastKVCache:
         if c is not None:
             ops.blend_chunk(c.pool_k, c.pool_v, c.raw_pages, c.ring_pages, c.ring_layer_stride, c.alpha,
                             error_word=self.error_word)
+
+    def attend_q8(self, q, layer: int, meta: dict, out_scale):
+        """A layer's attention over the 8-bit history and its bf16 ring: one token or a span for every row."""
+        bt, seq_k, n = meta["bt_all"][layer], meta["seq_k"], meta["n"]
+        kw = dict(num_q8=meta["nsrc"], pool_k=self.pool_k, pool_v=self.pool_v, out_scale=out_scale,
+                  max_pages=meta["W"])
+        if n == 1:
+            return ops.decode_paged_q8(q, self.q8, bt, seq_k, workspace=self.workspace, l2_keep=True, **kw)
+        if not meta["older"]:  # the first two chunks
+            return ops.prefill_paged(q, self.pool_k, self.pool_v, bt, seq_k, meta["cu_q"], n, out_scale=out_scale,
+                                     error_word=self.error_word, max_pages=meta["W"])
+        B, width = seq_k.numel(), meta["older"]
+        if "stage" not in meta:
+            page = 2 * 2 * PAGE_SIZE * self.hkv * self.d
+            meta["stage_rows"] = min(B, max(1, self.stage_bytes // (width * page)))
+            meta["stage"] = ops.StageQ8.empty(meta["stage_rows"], width, self.hkv, self.d, device=self.device)
+        step = meta["stage_rows"]
+        # all rows at once: the layers of a span read the same copy
+        staged, meta["staged"] = meta.get("staged", False) and step == B, True
+        out = torch.empty_like(q)
+        for b in range(0, B, step):
+            e = min(B, b + step)
+            ops.prefill_paged_q8(q[b * n:e * n], self.q8, bt[b:e], seq_k[b:e], meta["cu_q"][: e - b + 1], n,
+                                 out=out[b * n:e * n], stage=meta["stage"], staged=staged, error_word=self.error_word,
+                                 **(kw | {"num_q8": meta["nsrc"][b:e]}))
+        return out
 
     def check_errors(self):
         e = self.error_word.cpu().tolist()
@@ -637,6 +788,8 @@ class LastKVAttention(nn.Module):
         if kv_dtype == torch.float32:  # decode and spans alike (lkv_attention_paged_f32)
             out = ops.attention_paged_f32(q_out, cache.pool_k, cache.pool_v, bt, meta["seq_k"], meta["cu_q"],
                                           out_scale=out_scale, error_word=cache.error_word, max_pages=meta["W"])
+        elif cache.q8 is not None:
+            out = cache.attend_q8(q_out, self.layer_idx, meta, out_scale)
         elif L == 1:
             out = ops.decode_paged(q_out, cache.pool_k, cache.pool_v, bt, meta["seq_k"], out_scale=out_scale,
                                    workspace=cache.workspace, max_pages=meta["W"],
@@ -760,6 +913,14 @@ class LastKVModel(nn.Module):
         return cached[1]
 
 
+class Beams(NamedTuple):
+    """Beam search's result, each prompt's best beam first."""
+
+    sequences: torch.Tensor  # int64 [B, K, prompt + new tokens]
+    scores: torch.Tensor     # fp32 [B, K], summed log-probabilities of the new tokens
+    finished: torch.Tensor   # bool [B, K]
+
+
 class LastKVForCausalLM(nn.Module):
     """``CustomRecurrentMarinAKV254ReuseKVForCausalLM`` (modeling.py:215-293) on the B200 path."""
 
@@ -801,7 +962,8 @@ class LastKVForCausalLM(nn.Module):
 
     def new_cache(self, batch: int, max_tokens: int, **kw) -> PagedLastKVCache:
         """A paged cache for this model: fp32 keys and values for an fp32 model (the
-        reference's fp32 arithmetic end to end), bf16 otherwise."""
+        reference's fp32 arithmetic end to end), bf16 otherwise.  ``history="int8"``
+        holds the shared history of a bf16 cache in 8 bits (``PagedLastKVCache``)."""
         kw.setdefault("dtype", torch.float32 if self.lm_head.weight.dtype == torch.float32 else torch.bfloat16)
         return PagedLastKVCache(self.config, batch, max_tokens, device=self.lm_head.weight.device, **kw)
 
@@ -826,6 +988,40 @@ class LastKVForCausalLM(nn.Module):
             logits, _ = self(nxt, cache, logits_to_keep=1)
             nxt = logits[:, -1].float().argmax(-1, keepdim=True)
         return torch.cat(out, dim=1)
+
+    @torch.no_grad()
+    def generate_beam(self, prompt, num_beams: int, max_new_tokens: int, *, eos_token: int | None = None,
+                      cache: PagedLastKVCache | None = None) -> "Beams":
+        """Beam search: ``num_beams`` continuations of every prompt [B, P] by their summed log-probabilities.
+
+        The prompts run once each; their beams share what they have in common (``reorder_cache``).
+        A beam that has ended with ``eos_token`` keeps its score and repeats it.  ``cache``: an empty one of
+        B * num_beams rows (``new_cache``; with ``history="int8"``, say)."""
+        B, P = prompt.shape
+        K = num_beams
+        cache = cache or self.new_cache(B * K, P + max_new_tokens)
+        if cache.batch != B * K or cache.seen_tokens:
+            raise RMarinBackendContractError(f"beam search needs an empty cache of {B * K} rows")
+        if max_new_tokens < 1:
+            raise RMarinBackendContractError("beam search adds at least one token")
+        with cache.only_rows(np.arange(B) * K):
+            logits, _ = self(prompt, cache, logits_to_keep=1)
+        # every prompt's K best first tokens, then all beams as copies of their prompt's row
+        best = ops.beam_select(logits[:, -1], torch.zeros((B, 1), device=prompt.device), select=K, eos_token=eos_token)
+        cache.reorder_cache(np.arange(B * K) // K * K)
+        out = torch.cat((prompt.repeat_interleave(K, 0), best.tokens.view(-1, 1)), 1)
+        rows = None
+        for _ in range(max_new_tokens - 1):
+            if eos_token is not None and bool(best.finished.all()):
+                break
+            if rows is not None:
+                cache.reorder_cache(rows)
+            logits, _ = self(best.tokens.view(-1, 1), cache, logits_to_keep=1)
+            best = ops.beam_select(logits[:, -1], best.scores, eos_token=eos_token,
+                                   finished=best.finished if eos_token is not None else None)
+            rows = best.rows.view(-1)
+            out = torch.cat((out[rows], best.tokens.view(-1, 1)), 1)
+        return Beams(out.view(B, K, -1), best.scores, best.finished)
 
     def load_reference_state_dict(self, state: dict, strict: bool = True):
         """Load the reference's tensor names (strict, as modeling.py:243-249 requires)."""

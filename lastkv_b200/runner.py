@@ -12,6 +12,11 @@ a second graph, captured with that fused launch over static page lists,
 replays for the step after each boundary.  All sequences of the batch advance
 together (equal positions), as in ``generate``.
 
+With ``beams=K`` the captured step ends in beam search's selection instead of the argmax
+(``ops.beam_select``): K rows of the cache continue each prompt, and after each step the
+host reorders the cache by the rows that were chosen, which is a table update and a copy
+of the pages being written.
+
 With ``device_plan=True`` the prologue runs inside the graph as well
 (``ops.StepPlan``): the tables, slots, positions and commit lists of a step are
 built on the device from the lengths there, which the step advances itself, so a
@@ -20,6 +25,9 @@ step is one graph launch and copies nothing from the host.
 
 from __future__ import annotations
 
+from contextlib import nullcontext
+
+import numpy as np
 import torch
 
 from . import ops
@@ -30,9 +38,19 @@ from .hf import LastKVForCausalLM, PagedLastKVCache
 class GraphDecodeRunner:
     NSETS = 4
 
-    def __init__(self, model: LastKVForCausalLM, cache: PagedLastKVCache, *, device_plan: bool = False):
+    def __init__(self, model: LastKVForCausalLM, cache: PagedLastKVCache, *, device_plan: bool = False,
+                 beams: int | None = None, eos_token: int | None = None):
+        if device_plan and (cache.q8 is not None or beams is not None):
+            raise RMarinBackendContractError("a step planned on the device takes a bf16 history and greedy rows")
+        if beams is not None and (beams < 1 or cache.batch % beams):
+            raise RMarinBackendContractError(f"{cache.batch} rows are not prompts of {beams} beams each")
         self.model, self.cache = model, cache
         dev = cache.device
+        self.beams, self.eos_token = beams, eos_token
+        if beams is not None:  # the step's candidates, and what the next one starts from
+            self.choice = ops.BeamChoice.empty(cache.batch // beams, beams, device=dev)
+            self.scores = torch.zeros((cache.batch // beams, beams), dtype=torch.float32, device=dev)
+            self.finished = torch.zeros_like(self.choice.finished)
         B, L = cache.batch, cache.num_layers
         self.B, self.L = B, L
         self.W = cache.pages_per_seq + cache.ring_pages
@@ -125,7 +143,7 @@ class GraphDecodeRunner:
         pages of every layer, so those decodes load pages after their wait."""
         self.cache._meta = {"n": 1, "W": self.W, "bt_all": self.bt_all, "seq_k": self.seq_k, "cu_q": self.cu_q,
                             "local_pos": self.local_pos, "ring_tok": self.ring_tok, "src_slot": self.src_slot,
-                            "tables_ready": tables_ready}
+                            "nsrc": self.nsrc, "tables_ready": tables_ready}
 
     def _body(self):
         m = self.model.model
@@ -135,19 +153,35 @@ class GraphDecodeRunner:
         hidden = m.embed_tokens(self.ids)
         pe = m.rotary_emb(hidden, self.pos)
         logits = self.model.lm_head(m.run_layers(hidden, pe, self.cache)[:, -1])
-        if logits.dtype == torch.bfloat16 and logits.shape[-1] % 8 == 0:
+        if self.beams is not None:
+            ops.beam_select(logits, self.scores, finished=self.finished if self.eos_token is not None else None,
+                            eos_token=self.eos_token, out=self.choice)
+            self._take_choice()
+        elif logits.dtype == torch.bfloat16 and logits.shape[-1] % 8 == 0:
             ops.argmax_rows(logits, out=self.ids.view(-1))  # torch.argmax order, one launch
         else:
             self.ids.copy_(logits.float().argmax(-1, keepdim=True))
         if self.plan is not None:
             self.computed.add_(self.new_tokens)
 
+    def _take_choice(self):
+        """The chosen candidates are what the next step starts from."""
+        self.ids.copy_(self.choice.tokens.view(-1, 1))
+        self.scores.copy_(self.choice.scores)
+        self.finished.copy_(self.choice.finished)
+
     def capture(self):
         """Capture one decode step at the current position (the warm-up runs do not advance),
         and for bf16 caches the same step with a boundary commit fused into layer 0's append."""
         cache = self.cache
         cache.flush_commit()
-        saved = self.ids.clone()
+        state = (self.ids, self.scores, self.finished) if self.beams is not None else (self.ids,)
+        saved = [t.clone() for t in state]
+
+        def restore():  # what the warm-up steps started from
+            for t, was in zip(state, saved):
+                t.copy_(was)
+
         self._prepare()
         fused = cache.fuse_commit
         empty = torch.zeros((0, self.c_raw.shape[1]), dtype=torch.int32, device=self.ids.device)
@@ -155,7 +189,7 @@ class GraphDecodeRunner:
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
             for i in range(3 if fused else 2):
-                self.ids.copy_(saved)
+                restore()
                 if self.plan is not None:
                     self.computed.fill_(cache.seen_tokens)
                 self._fresh_meta()
@@ -164,7 +198,7 @@ class GraphDecodeRunner:
                                                 self.alpha)
                 self._body()
         torch.cuda.current_stream().wait_stream(s)
-        self.ids.copy_(saved)
+        restore()
         self._fresh_meta()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
@@ -181,16 +215,20 @@ class GraphDecodeRunner:
             finally:
                 cache._pending = None
             self.graph_commit = gc
-        self.ids.copy_(saved)
+        restore()
         if self.plan is not None:
             self.computed.fill_(cache.seen_tokens)
             self._computed_host = cache.seen_tokens
 
     def step(self):
-        """One greedy token for every sequence; returns the device tensor of new ids [B, 1]."""
+        """One token for every sequence; returns the device tensor of new ids [B, 1].  With beams, row
+        ``b * K + i`` is then prompt b's beam i, best first: ``choice`` holds their scores and the rows that
+        they continue, by which the cache has been reordered."""
         if self.graph is None:
             raise RMarinBackendContractError("capture() must run before step()")
         cache = self.cache
+        if self.plan is not None:
+            cache.unshare_()  # the device plan's rows have pages of their own
         pending = cache.take_commit()
         if pending is not None and (self.graph_commit is None or pending.pool_k is not cache.pool_k
                                     or pending.alpha is not self.alpha
@@ -216,15 +254,27 @@ class GraphDecodeRunner:
         cache._meta = None
         if cache.seen_tokens % cache.chunk_size == 0:
             cache.commit(self.alpha)
+        if self.beams is not None:
+            cache.reorder_cache(self.choice.rows)
         return self.ids
 
     @torch.no_grad()
     def prefill(self, prompt: torch.Tensor, call_tokens: int) -> torch.Tensor:
         """Eager chunked prefill in calls of ``call_tokens`` (split at chunk boundaries inside);
-        sets the first generated token into the static id buffer."""
-        logits = None
-        for start in range(0, prompt.shape[1], call_tokens):
-            logits, _ = self.model(prompt[:, start:start + call_tokens], self.cache, logits_to_keep=1)
+        sets the first generated token into the static id buffer.  With beams, ``prompt`` has a row
+        for each prompt, whose K best first tokens its beams begin with."""
+        logits, rows = None, None
+        if self.beams is not None:
+            rows = np.arange(0, self.B, self.beams)
+        with nullcontext() if rows is None else self.cache.only_rows(rows):
+            for start in range(0, prompt.shape[1], call_tokens):
+                logits, _ = self.model(prompt[:, start:start + call_tokens], self.cache, logits_to_keep=1)
+        if rows is not None:
+            ops.beam_select(logits[:, -1], self.scores.new_zeros((len(rows), 1)), select=self.beams,
+                            eos_token=self.eos_token, out=self.choice)
+            self._take_choice()
+            self.cache.reorder_cache(np.repeat(rows, self.beams))
+            return self.ids
         self.ids.copy_(logits[:, -1].float().argmax(-1, keepdim=True))
         return self.ids
 
