@@ -554,10 +554,10 @@ int lkv_cp_combine(const float* send, const uint64_t* peer_recv, int rank, int w
                    int64_t out_stride_tok, int32_t* error_word, void* stream);
 
 /* ------------------------------------------------------------------ 8-bit pages
- * Older pages of a cache in 8 bits: for each (page, KV head) int8 codes of the
- * keys and values and four fp32 scales, one for every 8 tokens of either; a code
- * q stands for q * scale.
- *   codes  : int8 [q8_pages, num_kv_heads, 2 (K, V), 16 * head_dim], each page's codes
+ * Older pages of a cache in 8 bits: for each (page, KV head) codes of the keys and
+ * values, whole numbers from -127 to 127, and four fp32 scales, one for every 8 tokens of
+ * either; a code q stands for q * scale.
+ *   codes  : uint8 [q8_pages, num_kv_heads, 2 (K, V), 16 * head_dim], q + 128, each page's
  *            in the order of the decode kernel's operands: with g = 0..7, c = 0..3,
  *              K[8 h + g, 16 j + 8 t1 + 2 c + t0] at (j / 2) * 512 + (4 g + c) * 16
  *                                                    + ((j % 2) * 2 + h) * 4 + 2 t0 + t1
@@ -576,10 +576,10 @@ int lkv_cp_combine(const float* send, const uint64_t* peer_recv, int rank, int w
  * lkv_q8_dequantize_pages: the reverse, bf16(code * scale).
  * Page ids outside the pools are skipped and recorded in error_word (may be NULL). */
 int lkv_q8_quantize_pages(const void* pool_k, const void* pool_v, int64_t num_pages, const int32_t* pages,
-                          const int32_t* tokens, int8_t* codes, float* scales, int64_t q8_pages,
+                          const int32_t* tokens, uint8_t* codes, float* scales, int64_t q8_pages,
                           const int32_t* out_pages, int64_t n, int num_kv_heads, int head_dim,
                           int32_t* error_word, void* stream);
-int lkv_q8_dequantize_pages(const int8_t* codes, const float* scales, int64_t q8_pages, const int32_t* pages,
+int lkv_q8_dequantize_pages(const uint8_t* codes, const float* scales, int64_t q8_pages, const int32_t* pages,
                             void* pool_k, void* pool_v, int64_t num_pages, const int32_t* out_pages, int64_t n,
                             int num_kv_heads, int head_dim, int32_t* error_word, void* stream);
 
@@ -588,9 +588,10 @@ int lkv_q8_dequantize_pages(const int8_t* codes, const float* scales, int64_t q8
  * bf16 pool (pool_k and pool_v may be NULL where there are none).  Either kind may hold
  * the row's last token; keys from seq_k[b] on have no weight, whatever is there.  A row
  * without keys gives zeros and an LSE of -inf.  Workspace, out, lse, out_scale as for
- * lkv_decode_paged; flags: LKV_DECODE_L2_KEEP or 0.  Two calls whose work overlaps need
+ * lkv_decode_paged (lkv_decode_workspace_bytes; a smaller one makes the work's parts
+ * fewer); flags: LKV_DECODE_L2_KEEP or 0.  Two calls whose work overlaps need
  * two workspaces.  Everything is read after the launch's dependency wait. */
-int lkv_decode_paged_q8(const void* q, int64_t q_stride_tok, const int8_t* codes, const float* scales,
+int lkv_decode_paged_q8(const void* q, int64_t q_stride_tok, const uint8_t* codes, const float* scales,
                         int64_t q8_pages, const void* pool_k, const void* pool_v, int64_t num_pages,
                         const int32_t* block_table, int64_t block_table_stride, const int32_t* num_q8,
                         const int32_t* seq_k, void* out, int64_t out_stride_tok, float* lse,
@@ -606,7 +607,7 @@ int lkv_decode_paged_q8(const void* q, int64_t q_stride_tok, const int8_t* codes
  * lkv_prefill_paged_q8 is lkv_prefill_paged with them: it reads the codes from the
  *   stage and the scales by the block table's page ids.  A row with more 8-bit pages than
  *   stage_width is recorded in error_word (may be NULL), its further ones read as zeros. */
-int lkv_q8_stage_pages(const int8_t* codes, const float* scales, int64_t q8_pages, const int32_t* block_table,
+int lkv_q8_stage_pages(const uint8_t* codes, const float* scales, int64_t q8_pages, const int32_t* block_table,
                        int64_t block_table_stride, const int32_t* num_q8, const int32_t* seq_k, int batch,
                        int max_pages_per_seq, void* stage_k, void* stage_v, int stage_width, int num_kv_heads,
                        int head_dim, int32_t* error_word, void* stream);

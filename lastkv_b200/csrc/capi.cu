@@ -598,21 +598,21 @@ int lkv_plan_step(const int32_t* num_computed, const int32_t* num_new, const int
 }
 
 int lkv_q8_quantize_pages(const void* pool_k, const void* pool_v, int64_t num_pages, const int32_t* pages,
-                          const int32_t* tokens, int8_t* codes, float* scales, int64_t q8_pages,
+                          const int32_t* tokens, uint8_t* codes, float* scales, int64_t q8_pages,
                           const int32_t* out_pages, int64_t n, int num_kv_heads, int head_dim, int32_t* error_word,
                           void* stream) {
   return lkv::quantise_pages(pool_k, pool_v, num_pages, pages, tokens, codes, scales, q8_pages, out_pages, n,
                              num_kv_heads, head_dim, error_word, static_cast<cudaStream_t>(stream));
 }
 
-int lkv_q8_dequantize_pages(const int8_t* codes, const float* scales, int64_t q8_pages, const int32_t* pages,
+int lkv_q8_dequantize_pages(const uint8_t* codes, const float* scales, int64_t q8_pages, const int32_t* pages,
                             void* pool_k, void* pool_v, int64_t num_pages, const int32_t* out_pages, int64_t n,
                             int num_kv_heads, int head_dim, int32_t* error_word, void* stream) {
   return lkv::dequantise_pages(codes, scales, q8_pages, pages, pool_k, pool_v, num_pages, out_pages, n, num_kv_heads,
                                head_dim, error_word, static_cast<cudaStream_t>(stream));
 }
 
-int lkv_q8_stage_pages(const int8_t* codes, const float* scales, int64_t q8_pages, const int32_t* block_table,
+int lkv_q8_stage_pages(const uint8_t* codes, const float* scales, int64_t q8_pages, const int32_t* block_table,
                        int64_t block_table_stride, const int32_t* num_q8, const int32_t* seq_k, int batch,
                        int max_pages_per_seq, void* stage_k, void* stage_v, int stage_width, int num_kv_heads,
                        int head_dim, int32_t* error_word, void* stream) {
@@ -664,7 +664,7 @@ int lkv_prefill_paged_q8(const void* q, int64_t q_stride_tok, const void* stage_
   return lkv::prefill_paged(a);
 }
 
-int lkv_decode_paged_q8(const void* q, int64_t q_stride_tok, const int8_t* codes, const float* scales,
+int lkv_decode_paged_q8(const void* q, int64_t q_stride_tok, const uint8_t* codes, const float* scales,
                         int64_t q8_pages, const void* pool_k, const void* pool_v, int64_t num_pages,
                         const int32_t* block_table, int64_t block_table_stride, const int32_t* num_q8,
                         const int32_t* seq_k, void* out, int64_t out_stride_tok, float* lse, const float* out_scale,

@@ -822,11 +822,15 @@ int launch_group(const CUtensorMap& tmk, const CUtensorMap& tmv, DecodeParams pr
 // [rows, D] and LSE [rows] in fp32, plus 256 bytes for the o area's alignment.
 size_t decode_split_bytes(int64_t rows, int d) { return (size_t)rows * (size_t)(d + 1) * sizeof(float) + 256; }
 
+constexpr int64_t kQ8Cuts = 320;  // two CTAs on each of 160 SMs
+
 size_t decode_workspace_bytes(int batch, int hq, int d, int max_pages) {
   const int64_t rows = (int64_t)std::max(batch, 0) * std::max(hq, 0);
   const int s = std::min(kMaxSplits, std::max(1, max_pages / 4));
-  // s splits of decode_paged's per-split layout (o and lse of every row + 256 bytes of alignment slack)
-  return kWorkspaceHeader + (size_t)s * decode_split_bytes(rows, std::max(d, 64));
+  // s splits of decode_paged's per-split layout (o and lse of every row + 256 bytes of alignment slack), and for
+  // decode_paged_q8 a piece of 8 heads for each of its CTAs' cuts and the rows' first slots
+  return kWorkspaceHeader + (size_t)s * decode_split_bytes(rows, std::max(d, 64)) +
+         decode_split_bytes(kQ8Cuts * 8, std::max(d, 64)) + ((size_t)std::max(batch, 0) + 1) * sizeof(int64_t) + 256;
 }
 
 int decode_paged(const DecodeArgs& a) {

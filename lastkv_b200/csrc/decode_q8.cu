@@ -1,24 +1,33 @@
 // Split-KV decode over a cache whose older pages are held in 8 bits (sm_100a).
 //
-// Row b attends to seq_k[b] keys: its first num_q8[b] block-table columns are pages of int8 codes
-// with scales (pages_q8.cuh), the rest pages of the bf16 pool.  Per KV head, with the GQA group's
-// query heads folded into one tile,
-//     S^T[16 keys, 8 heads] = K[16, D] Q^T        (mma m16n8k16, bf16 operands, fp32 sums)
+// Row b attends to seq_k[b] keys: its first num_q8[b] block-table columns are 8-bit pages
+// (pages_q8.cuh), the rest pages of the bf16 pool.  Per KV head, with the GQA group's query heads
+// folded into one tile of 8 columns,
+//     S^T[16 keys, 8 heads] = K[16, D] Q^T          (mma m16n8k16, fp32 sums)
 //     s = S * key scale * softmax scale,  online softmax in fp32
 //     O^T[D, 8 heads] += V^T[D, 16] (p * value scale)^T
-// A code is a whole number up to 127 and exact in bf16, so the 8-bit pages' products are as exact
-// as those of bf16 keys; the scales (one per 8 tokens, the rows of an accumulator) multiply fp32
-// scores and weights.  p * scale is rounded to bf16, as decode_splitkv_kernel rounds p.
+// The scales belong to 8 tokens, the rows of an accumulator, and never touch the codes.  The codes
+// are whole numbers up to 127 and enter the products as f16, exactly: a byte q + 128 becomes 1024 +
+// 128 + q by one byte permutation that puts it under f16's exponent byte, and one subtraction
+// takes the 1152 off (bf16, with 7 bits of mantissa, took 3.5 instructions for two codes instead of 2).
+// - Q: a row's heads are divided by a power of two that brings their largest value to 1 .. 2 and rounded to
+//   f16: exact but for values below 2^-17 of the largest, which are rounded at 2^-25 of it.
+// - p * value scale: with t = s + log2(value scale) and M its running maximum, the product is 2^(t - M)
+//   whatever the scales are, in 0 .. 1; times 2^15 it uses f16's whole range, 11 bits down to
+//   2^-29 of the largest and 2^-40 of it as the smallest step.  A token's part of the sum of weights is that
+//   number (in fp32) divided by the value scale.
+// bf16 pages keep bf16 operands, and the same M with a value scale of 1.
 //
-// Bound by HBM: an 8-bit page is half a bf16 page's bytes.  Work is cut into slots of equal bytes,
-// one bf16 page or two 8-bit pages; an item is a (row, KV head, split) with its share of the
-// slots.  The grid is persistent, CTA c taking items c, c + grid, ...: a producer warp fills a
-// ring of STAGES x NW slots (a lane per copy: half a bf16 page by TMA, an 8-bit page's codes and
-// its scales by two bulk copies), NW consumer warps take one slot of a stage each.  A consumer lane
-// finds its operands of an 8-bit page in 16-byte pieces and turns them to bf16 in registers, 3.5
-// instructions per two codes.  The splits' normalised partials are joined by merge_partials.
+// Bound by HBM: an 8-bit page is half a bf16 page's bytes.  Work is counted in slots of equal bytes, one bf16
+// page or two 8-bit pages of one KV head.  The rows' slots lie end to end, (row, head) after
+// (row, head), and every CTA takes the same number of them, so ragged rows cost no balance; a
+// (row, head)'s part within a CTA is a piece, whose normalised partial goes to the workspace, and
+// join_pieces_kernel joins each row's pieces.  Per CTA one warp fills a ring of slots (an 8-bit page's codes and
+// scales by two bulk copies, a bf16 page's halves by TMA), 7 warps take the slots in turn.
 
 #include <math.h>
+
+#include <cuda_fp16.h>
 
 #include <algorithm>
 #include <climits>
@@ -48,30 +57,34 @@ struct DecodeQ8Params {
   int64_t out_stride_tok;
   float* lse;              // natural log [B, Hq] or null
   const float* out_scale;  // [Hq] or null
-  float* part_o;           // S > 1: [S][B * Hq][D]
-  float* part_lse;         // S > 1: natural log [S][B * Hq]
+  float* part_o;           // [pieces][GROUP][D], normalised
+  float* part_lse;         // [pieces][GROUP], natural log
+  int64_t* first_slot;     // [B + 1]: the rows' first slots, written for join_pieces_kernel
   int* err;
-  int B, Hq, Hkv, W, S;
+  int B, Hq, Hkv, W;
+  int whole;  // 1: the workspace holds one piece per (row, head): CTAs take whole ones
   float scale_log2;
   int keep_pages;  // leading columns that stay in L2
 };
 
+constexpr int kNW = 7;  // consumer warps: with the producer 16 warps on an SM, 128 registers for a thread
+constexpr int kThreads = (kNW + 1) * 32;
+constexpr int kLeastSlots = kNW;  // of a CTA that has any: a slot for each warp
+
 template <int D>
 struct Q8Cfg {
-  static constexpr int NW = 4;                           // consumer warps
-  static constexpr int STAGES = D == 128 ? 3 : 6;        // 96 KB of slots: two CTAs per SM
+  static constexpr int RING = D == 128 ? 11 : 22;         // 88 KB of slots: two CTAs per SM
   static constexpr int HALVES = D / 64;
-  static constexpr int TILE_BYTES = kPageTokens * 128;   // 16 rows x 64 bf16
+  static constexpr int TILE_BYTES = kPageTokens * 128;    // 16 rows x 64 bf16
   static constexpr int CODE_BYTES = 2 * kPageTokens * D;  // keys and values of an 8-bit page
-  static constexpr int SLOT_BYTES = 2 * CODE_BYTES;      // two 8-bit pages, or one bf16 page
-  static constexpr int STAGE_BYTES = NW * SLOT_BYTES;
-  static constexpr int SCALE_BYTES = STAGES * NW * 2 * 16;
+  static constexpr int SLOT_BYTES = 2 * CODE_BYTES;       // two 8-bit pages, or one bf16 page
   static constexpr int OSTRIDE = D + 4;
-  static constexpr int OFF_SCALE = STAGES * STAGE_BYTES;
-  static constexpr int OFF_MERGE = OFF_SCALE + SCALE_BYTES;
-  // merge area: o [NW][4 heads][OSTRIDE], then m and l [NW][8]
-  static constexpr int OFF_BAR = OFF_MERGE + NW * 4 * OSTRIDE * 4 + 2 * NW * 8 * 4;
-  static constexpr int SMEM_BYTES = 1024 + OFF_BAR + 2 * STAGES * 8 + 16;
+  static constexpr int OFF_SCALE = RING * SLOT_BYTES;     // two pages' scales per slot
+  static constexpr int OFF_Q = OFF_SCALE + RING * 32;     // bf16 Q operands of the current piece
+  // join area: o [kNW][4 heads][OSTRIDE], then m and l [kNW][8]
+  static constexpr int OFF_JOIN = OFF_Q + (D / 16) * 32 * 8;
+  static constexpr int OFF_BAR = OFF_JOIN + kNW * 4 * OSTRIDE * 4 + 2 * kNW * 8 * 4;
+  static constexpr int SMEM_BYTES = 1024 + OFF_BAR + 2 * RING * 8 + 64;
 };
 
 __device__ __forceinline__ float max_over_rows(float v) {  // over the 8 lanes that share lane & 3
@@ -86,118 +99,247 @@ __device__ __forceinline__ float sum_over_rows(float v) {
   return v + __shfl_xor_sync(0xffffffffu, v, 16);
 }
 
+// D = A(16x16, row) * B(16x8, col) + D, f16 inputs, fp32 accumulate.
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ float lg2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Value scales below this count as this in the weights (codes of zero, or products that no sum of others
+// would keep): its reciprocal is finite.
+constexpr float kMinValueScale = 8.6736174e-19f;  // 2^-60
+constexpr float kWeightLog2 = 15.f;               // weights of the products are times 2^15
+
+// The slots of row b.
+struct Row {
+  int n, npages, nh, hs, slots;  // keys, pages, 8-bit pages, their slots, all slots of a head
+};
+__device__ __forceinline__ Row row_of(const DecodeQ8Params& p, int b) {
+  Row r;
+  r.n = max(0, p.seq_k[b]);
+  r.npages = min((int)(((int64_t)r.n + kPageTokens - 1) / kPageTokens), p.W);
+  r.n = min(r.n, r.npages * kPageTokens);
+  r.nh = p.num_q8 ? min(max(p.num_q8[b], 0), r.npages) : r.npages;
+  r.hs = (r.nh + 1) / 2;
+  r.slots = r.hs + r.npages - r.nh;
+  return r;
+}
+
+// What a CTA takes: pieces from slot `at` of (row b, head hk) on, `left` slots in all (whole: `left` (row, head)s).
+struct Share {
+  int b, hk, at, piece;
+  int64_t left;
+};
+
+// A piece: slots [s0, s1) of (row b, head hk).
+struct Piece {
+  Row r;
+  int b, hk, s0, s1, id;
+};
+
+// The next piece of a share; false where it ends.  Every warp walks its copy of the share.
+__device__ __forceinline__ bool next_piece(const DecodeQ8Params& p, Share& s, Piece& x) {
+  if (s.left <= 0 || s.b >= p.B) return false;
+  x.r = row_of(p, s.b);
+  if (!p.whole)
+    while (x.r.slots == 0) {  // rows without keys have no pieces, but their places among them
+      s.piece += p.Hkv;
+      if (++s.b >= p.B) return false;
+      x.r = row_of(p, s.b);
+    }
+  x.b = s.b;
+  x.hk = s.hk;
+  x.id = s.piece;
+  x.s0 = s.at;
+  x.s1 = p.whole ? x.r.slots : (int)min((int64_t)x.r.slots, s.at + s.left);
+  s.left -= p.whole ? 1 : x.s1 - x.s0;
+  s.at = 0;
+  ++s.piece;
+  if (++s.hk == p.Hkv) {
+    s.hk = 0;
+    ++s.b;
+  }
+  return true;
+}
+
+// All threads: the CTA's share.  Piece u of the (row, head)s in order, cut at CTA c's first slot, is piece u + c.
+__device__ Share share_of(const DecodeQ8Params& p, int64_t* sm, int* sm_row) {
+  Share s{};
+  const int64_t units = (int64_t)p.B * p.Hkv;
+  if (p.whole) {
+    const int64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+    s.b = (int)(u0 / p.Hkv);
+    s.hk = (int)(u0 % p.Hkv);
+    s.piece = (int)u0;
+    s.left = u1 - u0;
+    return s;
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int WARPS = kThreads / 32;
+  int64_t mine = 0;
+  for (int b = threadIdx.x; b < p.B; b += kThreads) mine += row_of(p, b).slots;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) sm[warp] = mine;
+  if (threadIdx.x == 0) *sm_row = -1;
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < WARPS; ++w) total += sm[w];
+  total *= p.Hkv;
+  const int64_t per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kLeastSlots);
+  const int64_t first = per * blockIdx.x;
+  if (first >= total && blockIdx.x != 0) return s;
+  // the row that holds the first slot (CTA 0 goes through all rows, for join_pieces_kernel)
+  int64_t before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+    const int b = b0 + threadIdx.x;
+    const int64_t here = b < p.B ? (int64_t)row_of(p, b).slots * p.Hkv : 0;
+    int64_t sum = here;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    __syncthreads();  // sm is read
+    if (lane == 31) sm[warp] = sum;
+    __syncthreads();
+    int64_t start = before + sum - here;
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) start += sm[w];
+      before += sm[w];
+    }
+    if (blockIdx.x == 0 && b < p.B) {
+      p.first_slot[b] = start;
+      if (b == p.B - 1) p.first_slot[p.B] = per;
+    }
+    if (here > 0 && start <= first && first < start + here) {
+      *sm_row = b;
+      sm[WARPS] = start;
+    }
+    if (blockIdx.x != 0 && before > first) break;  // the same for all threads
+  }
+  __syncthreads();
+  if (first >= total) return s;
+  s.b = *sm_row;
+  const Row r = row_of(p, s.b);
+  const int64_t off = first - sm[WARPS];
+  s.hk = (int)(off / r.slots);
+  s.at = (int)(off % r.slots);
+  s.piece = s.b * p.Hkv + s.hk + blockIdx.x;
+  s.left = min(per, total - first);
+  return s;
+}
+
 template <int D, int GROUP>
-__global__ void __launch_bounds__((Q8Cfg<D>::NW + 1) * 32, 2)
+__global__ void __launch_bounds__(kThreads, 2)
     decode_q8_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                      const DecodeQ8Params p) {
   using Cfg = Q8Cfg<D>;
-  constexpr int NW = Cfg::NW, STAGES = Cfg::STAGES, KT = D / 16;
+  constexpr int RING = Cfg::RING, KT = D / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* mo = reinterpret_cast<float*>(smem + Cfg::OFF_MERGE);
-  float* mm = mo + NW * 4 * Cfg::OSTRIDE;
-  float* ml = mm + NW * 8;
+  float* jo = reinterpret_cast<float*>(smem + Cfg::OFF_JOIN);
+  float* jm = jo + kNW * 4 * Cfg::OSTRIDE;
+  float* jl = jm + kNW * 8;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
-  uint64_t* empty = full + STAGES;
-  volatile int* fail_flag = reinterpret_cast<volatile int*>(empty + STAGES);
+  uint64_t* empty = full + RING;
+  volatile int* fail_flag = reinterpret_cast<volatile int*>(empty + RING);
+  __shared__ int64_t sm_sum[kThreads / 32 + 1];
+  __shared__ int sm_row;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < RING; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], NW);
+      mbar_init(&empty[s], 1);
     }
     *fail_flag = 0;
     fence_barrier_init();
   }
   __syncthreads();
   pdl_wait();
+  Share share = share_of(p, sm_sum, &sm_row);
+  Piece x;
+  uint32_t gs = 0;  // slots of this CTA's earlier pieces: slot k of a piece has ring place (gs + k) % RING
 
-  struct Item {
-    int b, hk, split, n, npages, nh, hs, s0, s1, n_iter;
-  };
-  const int n_items = p.S * p.Hkv * p.B;
-  auto item_at = [&](int i) {
-    Item it;
-    it.split = i % p.S;
-    it.hk = (i / p.S) % p.Hkv;
-    it.b = i / (p.S * p.Hkv);
-    it.n = max(0, p.seq_k[it.b]);
-    it.npages = min((int)(((int64_t)it.n + kPageTokens - 1) / kPageTokens), p.W);
-    it.n = min(it.n, it.npages * kPageTokens);
-    it.nh = p.num_q8 ? min(max(p.num_q8[it.b], 0), it.npages) : it.npages;
-    it.hs = (it.nh + 1) / 2;  // slots of 8-bit pages, then one per bf16 page
-    const int slots = it.hs + it.npages - it.nh;
-    const int per = (slots + p.S - 1) / p.S;
-    it.s0 = min(slots, it.split * per);
-    it.s1 = min(slots, it.s0 + per);
-    it.n_iter = (it.s1 - it.s0 + NW - 1) / NW;
-    return it;
-  };
-
-  if (warp == NW) {
+  if (warp == kNW) {
     // ------------------------------------------------------------ producer
-    // Lane 2 w + u copies half u of consumer warp w's slot: an 8-bit page (its codes and scales), or
-    // the keys (u = 0) or values (u = 1) of a bf16 page.
+    // Lane 2 i + u copies half u of the i-th slot of a group of 16: an 8-bit page (its codes and scales), or the
+    // keys (u = 0) or values (u = 1) of a bf16 page.
     if (p.pool_pages && lane == 0) {
       tma_prefetch_desc(&tmk);
       tma_prefetch_desc(&tmv);
     }
     const uint64_t pol_first = policy_evict_first(), pol_last = policy_evict_last();
-    const int w = lane >> 1, u = lane & 1;
-    uint32_t gs = 0;
+    const int u = lane & 1;
     bool ok = true;
-    for (int i = blockIdx.x; ok && i < n_items; i += gridDim.x) {
-      const Item it = item_at(i);
-      const int32_t* row = p.bt + (int64_t)it.b * p.bt_stride;
-      // this lane's page of step k: its block-table column (-1: none) and id, read a step ahead
+    while (ok && next_piece(p, share, x)) {
+      const int32_t* row = p.bt + (int64_t)x.b * p.bt_stride;
+      const int count = x.s1 - x.s0;
+      // this lane's block-table column of the group from slot k on (-1: none), and its page, read a group ahead
       auto column = [&](int k) {
-        const int sl = it.s0 + k * NW + w;
-        if (lane >= 2 * NW || k >= it.n_iter || sl >= it.s1) return -1;
-        if (sl >= it.hs) return it.nh + sl - it.hs;
-        return 2 * sl + u < it.nh ? 2 * sl + u : -1;
+        const int sl = x.s0 + k + (lane >> 1);
+        if (sl >= x.s1) return -1;
+        if (sl >= x.r.hs) return x.r.nh + sl - x.r.hs;
+        return 2 * sl + u < x.r.nh ? 2 * sl + u : -1;
       };
       int col = column(0);
       int id = col >= 0 ? __ldg(row + col) : 0;
-      for (int k = 0; k < it.n_iter; ++k, ++gs) {
+      for (int k0 = 0; ok && k0 < count; k0 += 16) {
         const int c = col, pid = id;
-        col = column(k + 1);
+        col = column(k0 + 16);
         if (col >= 0) id = __ldg(row + col);
-        const int s = (int)(gs % STAGES);
-        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((gs / STAGES) & 1u) ^ 1u));
-        if (!ok) break;
-        const bool q8 = c >= 0 && c < it.nh;
+        const bool q8 = c >= 0 && c < x.r.nh;
         const bool bad = c >= 0 && (pid < 0 || (int64_t)pid >= (q8 ? p.q8_pages : p.pool_pages));
-        uint8_t* dst = smem + s * Cfg::STAGE_BYTES + w * Cfg::SLOT_BYTES + u * Cfg::CODE_BYTES;
-        float* sc = reinterpret_cast<float*>(smem + Cfg::OFF_SCALE + (s * NW + w) * 32 + u * 16);
-        uint32_t bytes = 0;
-        if (c >= 0 && !bad) bytes = Cfg::CODE_BYTES + (q8 ? 16 : 0);
-        if (bad) {
-          // a page that is not there reads as zeros: scales of zero over whatever codes are there,
-          // or zeros in the place of bf16 rows
-          report_error(p.err, DEVERR_BAD_PAGE, 11, pid);
-          if (q8) {
-            *reinterpret_cast<float4*>(sc) = make_float4(0.f, 0.f, 0.f, 0.f);
-          } else {
-            for (int e = 0; e < Cfg::CODE_BYTES; e += 16) *reinterpret_cast<uint4*>(dst + e) = make_uint4(0, 0, 0, 0);
+        const uint32_t bytes = c >= 0 && !bad ? Cfg::CODE_BYTES + (q8 ? 16 : 0) : 0;
+        const uint32_t both = bytes + __shfl_xor_sync(0xffffffffu, bytes, 1);
+        const uint64_t pol = c < p.keep_pages ? pol_last : pol_first;
+        const int64_t block = (int64_t)pid * p.Hkv + x.hk;
+        for (int i = 0; i < min(16, count - k0); ++i, ++gs) {
+          const int s = (int)(gs % RING);
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((gs / RING) & 1u) ^ 1u));
+          if (!ok) break;
+          const bool mine = (lane >> 1) == i;
+          uint8_t* dst = smem + s * Cfg::SLOT_BYTES + u * Cfg::CODE_BYTES;
+          float* sc = reinterpret_cast<float*>(smem + Cfg::OFF_SCALE + s * 32 + u * 16);
+          if (mine && bad) {
+            // a page that is not there reads as zeros: scales of zero over whatever codes are there, or
+            // zeros in the place of bf16 rows
+            report_error(p.err, DEVERR_BAD_PAGE, 11, pid);
+            if (q8) {
+              *reinterpret_cast<float4*>(sc) = make_float4(0.f, 0.f, 0.f, 0.f);
+            } else {
+              for (int e = 0; e < Cfg::CODE_BYTES; e += 16) *reinterpret_cast<uint4*>(dst + e) = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before later copies to the same place
           }
-          // before later copies into the same place
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
-        const uint32_t total = __reduce_add_sync(0xffffffffu, bytes);
-        __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(&full[s], total);
-        __syncwarp();
-        if (bytes) {
-          const uint64_t pol = c < p.keep_pages ? pol_last : pol_first;
-          if (q8) {
-            const int64_t block = (int64_t)pid * p.Hkv + it.hk;
-            bulk_load_hint(dst, p.codes + block * Cfg::CODE_BYTES, Cfg::CODE_BYTES, &full[s], pol);
-            bulk_load(sc, p.scales + block * kScalesPerBlock, 16, &full[s]);
-          } else {
+          __syncwarp();
+          if (mine && u == 0) mbar_arrive_expect_tx(&full[s], both);
+          __syncwarp();
+          if (mine && bytes) {
+            if (q8) {
+              bulk_load_hint(dst, p.codes + block * Cfg::CODE_BYTES, Cfg::CODE_BYTES, &full[s], pol);
+              bulk_load(sc, p.scales + block * kScalesPerBlock, 16, &full[s]);
+            } else {
 #pragma unroll
-            for (int h = 0; h < Cfg::HALVES; ++h)
-              tma_load_4d_hint(dst + h * Cfg::TILE_BYTES, u ? &tmv : &tmk, &full[s], h * 64, it.hk, 0, pid, pol);
+              for (int h = 0; h < Cfg::HALVES; ++h)
+                tma_load_4d_hint(dst + h * Cfg::TILE_BYTES, u ? &tmv : &tmk, &full[s], h * 64, x.hk, 0, pid, pol);
+            }
           }
         }
       }
@@ -205,7 +347,7 @@ __global__ void __launch_bounds__((Q8Cfg<D>::NW + 1) * 32, 2)
     if (!ok) {
       // a consumer never gave a slot back: wait (again with a limit) for the copies in flight
       if (lane == 0) report_error(p.err, DEVERR_WAIT_TIMEOUT, 11, (int)gs);
-      for (uint32_t x = gs > STAGES ? gs - STAGES : 0; x < gs; ++x) mbar_wait(&full[x % STAGES], (x / STAGES) & 1u);
+      for (uint32_t y = gs > RING ? gs - RING : 0; y < gs; ++y) mbar_wait(&full[y % RING], (y / RING) & 1u);
     }
     return;
   }
@@ -214,28 +356,44 @@ __global__ void __launch_bounds__((Q8Cfg<D>::NW + 1) * 32, 2)
   const int g = lane >> 2, c = lane & 3;
   const uint32_t k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_chunk_hi = lane >> 4;
   const uint32_t v_row = (lane & 7) + (lane >> 4) * 8, v_chunk_hi = (lane >> 3) & 1;
-  uint32_t gs = 0;
+  uint2* sq = reinterpret_cast<uint2*>(smem + Cfg::OFF_Q) + lane;  // [KT][32]: the same for every warp
   bool failed = false;
 
-  for (int i = blockIdx.x; i < n_items; i += gridDim.x) {
-    const Item it = item_at(i);
+  while (next_piece(p, share, x)) {
+    // Q as f16 with a power of two per head, and (once per CTA) as it is for the bf16 pages
     uint32_t qf[KT][2];
+    float q0, q1;  // what a score of heads 2 c and 2 c + 1 is multiplied by: their powers and the softmax scale
     {
       const bool valid = g < GROUP;
-      const __nv_bfloat16* qrow =
-          p.q + (int64_t)it.b * p.q_stride_tok + (int64_t)(it.hk * GROUP + (valid ? g : 0)) * D;
+      const __nv_bfloat16* qrow = p.q + (int64_t)x.b * p.q_stride_tok + (int64_t)(x.hk * GROUP + (valid ? g : 0)) * D;
+      float top = 0.f;
 #pragma unroll
       for (int j = 0; j < KT; ++j) {
-        const int d0 = 16 * j + 2 * c;
-        qf[j][0] = valid ? *reinterpret_cast<const uint32_t*>(qrow + d0) : 0u;
-        qf[j][1] = valid ? *reinterpret_cast<const uint32_t*>(qrow + d0 + 8) : 0u;
+        qf[j][0] = valid ? *reinterpret_cast<const uint32_t*>(qrow + 16 * j + 2 * c) : 0u;
+        qf[j][1] = valid ? *reinterpret_cast<const uint32_t*>(qrow + 16 * j + 2 * c + 8) : 0u;
+        if (warp == j % kNW) sq[j * 32] = make_uint2(qf[j][0], qf[j][1]);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) top = fmaxf(top, fmaxf(fabsf(bf16_lo(qf[j][t])), fabsf(bf16_hi(qf[j][t]))));
       }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^e <= top < 2^(e + 1), within the powers whose reciprocals are ordinary numbers
+      const int e = min(max((int)(__float_as_uint(top) >> 23), 2), 252);
+      const float down = __uint_as_float((uint32_t)(254 - e) << 23), up = __uint_as_float((uint32_t)e << 23);
+#pragma unroll
+      for (int j = 0; j < KT; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) qf[j][t] = pack_f16(bf16_lo(qf[j][t]) * down, bf16_hi(qf[j][t]) * down);
+      q0 = __shfl_sync(0xffffffffu, up, 8 * c) * p.scale_log2;
+      q1 = __shfl_sync(0xffffffffu, up, 8 * c + 4) * p.scale_log2;
     }
+    asm volatile("bar.sync 1, %0;" ::"n"(kNW * 32));  // sq is written
     float o[KT][4];
 #pragma unroll
     for (int k = 0; k < KT; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    // raises the running maxima to the new scores' and rescales what is summed so far
+    // raises the running maxima to those of the new scores and rescales what is summed so far; r0, r1: what a
+    // weight's exponent has to lose
     auto raise = [&](float t0, float t1, float& r0, float& r1) {
       const float n0 = fmaxf(m0, max_over_rows(t0)), n1 = fmaxf(m1, max_over_rows(t1));
       if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
@@ -252,25 +410,27 @@ __global__ void __launch_bounds__((Q8Cfg<D>::NW + 1) * 32, 2)
           o[k][3] *= a1;
         }
       }
-      r0 = m0 == -INFINITY ? 0.f : m0;  // no score above -inf: weights of zero, not NaN
-      r1 = m1 == -INFINITY ? 0.f : m1;
+      r0 = (m0 == -INFINITY ? 0.f : m0) - kWeightLog2;  // no score above -inf: weights of zero, not NaN
+      r1 = (m1 == -INFINITY ? 0.f : m1) - kWeightLog2;
     };
 
-    for (int k = 0; k < it.n_iter; ++k, ++gs) {
-      const int s = (int)(gs % STAGES);
-      if (!mbar_wait(&full[s], (gs / STAGES) & 1u)) {
-        if (lane == 0) report_error(p.err, DEVERR_WAIT_TIMEOUT, 11, 1000000 + (int)gs);
+    const int count = x.s1 - x.s0;
+    for (int k = warp; k < count; k += kNW) {
+      const uint32_t at = gs + k;
+      const int s = (int)(at % RING);
+      if (!mbar_wait(&full[s], (at / RING) & 1u)) {
+        if (lane == 0) report_error(p.err, DEVERR_WAIT_TIMEOUT, 11, 1000000 + (int)at);
         failed = true;
         break;
       }
-      const int sl = it.s0 + k * NW + warp;
-      uint8_t* slot = smem + s * Cfg::STAGE_BYTES + warp * Cfg::SLOT_BYTES;
-      if (sl < it.s1 && sl < it.hs) {
+      const int sl = x.s0 + k;
+      uint8_t* slot = smem + s * Cfg::SLOT_BYTES;
+      if (sl < x.r.hs) {
         // ------------------------------------------ two 8-bit pages (or the last one): 32 keys
-        const float4* scp = reinterpret_cast<const float4*>(smem + Cfg::OFF_SCALE + (s * NW + warp) * 32);
-        const bool two = 2 * sl + 1 < it.nh;
-        const int left = min(it.n, it.nh * kPageTokens) - 2 * sl * kPageTokens;  // 8-bit keys from here on, >= 1
-        float sc[2][4], pv[2][4];
+        const float4* scp = reinterpret_cast<const float4*>(smem + Cfg::OFF_SCALE + s * 32);
+        const bool two = 2 * sl + 1 < x.r.nh;
+        const int left = min(x.r.n, x.r.nh * kPageTokens) - 2 * sl * kPageTokens;  // 8-bit keys from here on, >= 1
+        float sc[2][4], iv[2][2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float sd[4] = {0.f, 0.f, 0.f, 0.f};
@@ -278,35 +438,36 @@ __global__ void __launch_bounds__((Q8Cfg<D>::NW + 1) * 32, 2)
           if (e == 0 || two) {
             const uint8_t* kt = slot + e * Cfg::CODE_BYTES + lane * 16;
 #pragma unroll
-            for (int x = 0; x < KT / 2; ++x) {
-              const uint4 v = *reinterpret_cast<const uint4*>(kt + x * 512);
+            for (int y = 0; y < KT / 2; ++y) {
+              const uint4 v = *reinterpret_cast<const uint4*>(kt + y * 512);
               uint32_t a0, a1, a2, a3;
-              codes_to_bf16(v.x, a0, a2);
-              codes_to_bf16(v.y, a1, a3);
-              mma_bf16_16816(sc[e], a0, a1, a2, a3, qf[2 * x][0], qf[2 * x][1]);
-              codes_to_bf16(v.z, a0, a2);
-              codes_to_bf16(v.w, a1, a3);
-              mma_bf16_16816(sd, a0, a1, a2, a3, qf[2 * x + 1][0], qf[2 * x + 1][1]);
+              codes_to_f16(v.x, a0, a2);
+              codes_to_f16(v.y, a1, a3);
+              mma_f16_16816(sc[e], a0, a1, a2, a3, qf[2 * y][0], qf[2 * y][1]);
+              codes_to_f16(v.z, a0, a2);
+              codes_to_f16(v.w, a1, a3);
+              mma_f16_16816(sd, a0, a1, a2, a3, qf[2 * y + 1][0], qf[2 * y + 1][1]);
             }
           }
-          const float4 f = two || e == 0 ? scp[e] : make_float4(0.f, 0.f, 0.f, 0.f);
-          const float k0 = f.x * p.scale_log2, k1 = f.y * p.scale_log2;
-          sc[e][0] = (sc[e][0] + sd[0]) * k0;
-          sc[e][1] = (sc[e][1] + sd[1]) * k0;
-          sc[e][2] = (sc[e][2] + sd[2]) * k1;
-          sc[e][3] = (sc[e][3] + sd[3]) * k1;
-          pv[e][0] = pv[e][1] = f.z;
-          pv[e][2] = pv[e][3] = f.w;
+          float4 f = two || e == 0 ? scp[e] : make_float4(0.f, 0.f, 1.f, 1.f);
+          // blocks past the row's end: whatever their scales hold
+          if (16 * e >= left) f.x = 0.f, f.z = 1.f;
+          if (16 * e + 8 >= left) f.y = 0.f, f.w = 1.f;
+          const float v0 = f.z < kMinValueScale ? kMinValueScale : f.z, v1 = f.w < kMinValueScale ? kMinValueScale : f.w;
+          const float g0 = lg2_approx(v0), g1 = lg2_approx(v1);
+          iv[e][0] = __fdividef(1.f, v0);
+          iv[e][1] = __fdividef(1.f, v1);
+          sc[e][0] = fmaf(sc[e][0] + sd[0], f.x * q0, g0);
+          sc[e][1] = fmaf(sc[e][1] + sd[1], f.x * q1, g0);
+          sc[e][2] = fmaf(sc[e][2] + sd[2], f.y * q0, g1);
+          sc[e][3] = fmaf(sc[e][3] + sd[3], f.y * q1, g1);
         }
-        if (left < 32) {  // keys past the row's end: no weight, whatever they and their scales hold
+        if (left < 32) {  // keys past the row's end have no weight
 #pragma unroll
           for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if (16 * e + g + (x & 2) * 4 >= left) {
-                sc[e][x] = -INFINITY;
-                pv[e][x] = 0.f;
-              }
+            for (int y = 0; y < 4; ++y)
+              if (16 * e + g + (y & 2) * 4 >= left) sc[e][y] = -INFINITY;
         }
         float r0, r1;
         raise(fmaxf(fmaxf(sc[0][0], sc[0][2]), fmaxf(sc[1][0], sc[1][2])),
@@ -314,31 +475,30 @@ __global__ void __launch_bounds__((Q8Cfg<D>::NW + 1) * 32, 2)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float w = ex2_approx(sc[e][x] - (x & 1 ? r1 : r0));
-            if (x & 1) l1 += w;
-            else l0 += w;
-            pv[e][x] *= w;
+          for (int y = 0; y < 4; ++y) {
+            sc[e][y] = ex2_approx(sc[e][y] - (y & 1 ? r1 : r0));
+            if (y & 1) l1 = fmaf(sc[e][y], iv[e][y >> 1], l1);
+            else l0 = fmaf(sc[e][y], iv[e][y >> 1], l0);
           }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           if (e == 1 && !two) break;
-          const uint32_t pb0 = movmatrix_trans(pack_bf16(pv[e][0], pv[e][1]));
-          const uint32_t pb1 = movmatrix_trans(pack_bf16(pv[e][2], pv[e][3]));
+          const uint32_t pb0 = movmatrix_trans(pack_f16(sc[e][0], sc[e][1]));
+          const uint32_t pb1 = movmatrix_trans(pack_f16(sc[e][2], sc[e][3]));
           const uint8_t* vt = slot + e * Cfg::CODE_BYTES + kPageTokens * D + lane * 16;
 #pragma unroll
-          for (int x = 0; x < KT / 2; ++x) {
-            const uint4 v = *reinterpret_cast<const uint4*>(vt + x * 512);
+          for (int y = 0; y < KT / 2; ++y) {
+            const uint4 v = *reinterpret_cast<const uint4*>(vt + y * 512);
             uint32_t a0, a1, a2, a3;
-            codes_to_bf16(v.x, a0, a1);
-            codes_to_bf16(v.y, a2, a3);
-            mma_bf16_16816(o[2 * x], a0, a1, a2, a3, pb0, pb1);
-            codes_to_bf16(v.z, a0, a1);
-            codes_to_bf16(v.w, a2, a3);
-            mma_bf16_16816(o[2 * x + 1], a0, a1, a2, a3, pb0, pb1);
+            codes_to_f16(v.x, a0, a1);
+            codes_to_f16(v.y, a2, a3);
+            mma_f16_16816(o[2 * y], a0, a1, a2, a3, pb0, pb1);
+            codes_to_f16(v.z, a0, a1);
+            codes_to_f16(v.w, a2, a3);
+            mma_f16_16816(o[2 * y + 1], a0, a1, a2, a3, pb0, pb1);
           }
         }
-      } else if (sl < it.s1) {
+      } else {
         // ------------------------------------------ one bf16 page: 16 keys
         uint8_t* vt = slot + Cfg::CODE_BYTES;
         const uint32_t kbase = smem_u32(slot), vbase = smem_u32(vt);
@@ -347,21 +507,22 @@ __global__ void __launch_bounds__((Q8Cfg<D>::NW + 1) * 32, 2)
         for (int j = 0; j < KT; ++j) {
           uint32_t a0, a1, a2, a3;
           ldmatrix_x4(a0, a1, a2, a3, kbase + (j >> 2) * Cfg::TILE_BYTES + swz128(k_row, 2 * (j & 3) + k_chunk_hi));
-          if (j & 1) mma_bf16_16816(sd, a0, a1, a2, a3, qf[j][0], qf[j][1]);
-          else mma_bf16_16816(sc, a0, a1, a2, a3, qf[j][0], qf[j][1]);
+          const uint2 b = sq[j * 32];
+          if (j & 1) mma_bf16_16816(sd, a0, a1, a2, a3, b.x, b.y);
+          else mma_bf16_16816(sc, a0, a1, a2, a3, b.x, b.y);
         }
-        const int left = it.n - (it.nh + sl - it.hs) * kPageTokens;  // >= 1
+        const int left = x.r.n - (x.r.nh + sl - x.r.hs) * kPageTokens;  // >= 1
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          sc[x] = g + (x & 2) * 4 < left ? (sc[x] + sd[x]) * p.scale_log2 : -INFINITY;
+        for (int y = 0; y < 4; ++y)
+          sc[y] = g + (y & 2) * 4 < left ? (sc[y] + sd[y]) * p.scale_log2 : -INFINITY;
         float r0, r1;
         raise(fmaxf(sc[0], sc[2]), fmaxf(sc[1], sc[3]), r0, r1);
-        const float p00 = ex2_approx(sc[0] - r0), p01 = ex2_approx(sc[1] - r1);
-        const float p10 = ex2_approx(sc[2] - r0), p11 = ex2_approx(sc[3] - r1);
-        l0 += p00 + p10;
-        l1 += p01 + p11;
-        const uint32_t pb0 = movmatrix_trans(pack_bf16(p00, p01));
-        const uint32_t pb1 = movmatrix_trans(pack_bf16(p10, p11));
+#pragma unroll
+        for (int y = 0; y < 4; ++y) sc[y] = ex2_approx(sc[y] - (y & 1 ? r1 : r0));
+        l0 += sc[0] + sc[2];
+        l1 += sc[1] + sc[3];
+        const uint32_t pb0 = movmatrix_trans(pack_bf16(sc[0], sc[1]));
+        const uint32_t pb1 = movmatrix_trans(pack_bf16(sc[2], sc[3]));
         if (left < kPageTokens) {  // rows past the end may hold NaN: 0 * NaN would reach O
           const int per = (kPageTokens - left) * 8;
           for (int e = lane; e < per * Cfg::HALVES; e += 32) {
@@ -373,33 +534,34 @@ __global__ void __launch_bounds__((Q8Cfg<D>::NW + 1) * 32, 2)
           __syncwarp();
         }
 #pragma unroll
-        for (int x = 0; x < KT; ++x) {
+        for (int y = 0; y < KT; ++y) {
           uint32_t a0, a1, a2, a3;
           ldmatrix_x4_trans(a0, a1, a2, a3,
-                            vbase + (x >> 2) * Cfg::TILE_BYTES + swz128(v_row, 2 * (x & 3) + v_chunk_hi));
-          mma_bf16_16816(o[x], a0, a1, a2, a3, pb0, pb1);
+                            vbase + (y >> 2) * Cfg::TILE_BYTES + swz128(v_row, 2 * (y & 3) + v_chunk_hi));
+          mma_bf16_16816(o[y], a0, a1, a2, a3, pb0, pb1);
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
     }
+    gs += count;
 
-    // ------------------------------------------------------------ item merge
+    // ------------------------------------------------------------ the piece's partial
     // Only consumer warps write the failure flag, and only before this barrier.
     l0 = sum_over_rows(l0);
     l1 = sum_over_rows(l1);
     if (failed && lane == 0) *fail_flag = 1;
     if (g == 0) {
-      mm[warp * 8 + 2 * c] = m0;
-      mm[warp * 8 + 2 * c + 1] = m1;
-      ml[warp * 8 + 2 * c] = l0;
-      ml[warp * 8 + 2 * c + 1] = l1;
+      jm[warp * 8 + 2 * c] = m0;
+      jm[warp * 8 + 2 * c + 1] = m1;
+      jl[warp * 8 + 2 * c] = l0;
+      jl[warp * 8 + 2 * c + 1] = l1;
     }
     // four heads at a time: thread (g, c) holds heads 2c and 2c + 1
 #pragma unroll
     for (int hc = 0; hc < (GROUP + 3) / 4; ++hc) {
       if ((c >> 1) == hc) {
-        float* w0 = mo + (warp * 4 + 2 * c - 4 * hc) * Cfg::OSTRIDE;
+        float* w0 = jo + (warp * 4 + 2 * c - 4 * hc) * Cfg::OSTRIDE;
         float* w1 = w0 + Cfg::OSTRIDE;
 #pragma unroll
         for (int k = 0; k < KT; ++k) {
@@ -409,42 +571,94 @@ __global__ void __launch_bounds__((Q8Cfg<D>::NW + 1) * 32, 2)
           w1[16 * k + g + 8] = o[k][3];
         }
       }
-      asm volatile("bar.sync 1, %0;" ::"n"(NW * 32));
+      asm volatile("bar.sync 1, %0;" ::"n"(kNW * 32));
       if (*fail_flag) return;  // the same for all consumer warps
       constexpr int HC = GROUP < 4 ? GROUP : 4;
-      for (int idx = threadIdx.x; idx < HC * D; idx += NW * 32) {
+      for (int idx = threadIdx.x; idx < HC * D; idx += kNW * 32) {
         const int hl = idx / D, d = idx % D, h = 4 * hc + hl;
         float M = -INFINITY;
 #pragma unroll
-        for (int v = 0; v < NW; ++v) M = fmaxf(M, mm[v * 8 + h]);
+        for (int v = 0; v < kNW; ++v) M = fmaxf(M, jm[v * 8 + h]);
         float L = 0.f, acc = 0.f;
 #pragma unroll
-        for (int v = 0; v < NW; ++v) {
-          const float f = mm[v * 8 + h] == M ? 1.f : exp2f(mm[v * 8 + h] - M);
-          L += ml[v * 8 + h] * f;
-          acc += mo[(v * 4 + hl) * Cfg::OSTRIDE + d] * f;
+        for (int v = 0; v < kNW; ++v) {
+          const float f = jm[v * 8 + h] == M ? 1.f : exp2f(jm[v * 8 + h] - M);
+          L += jl[v * 8 + h] * f;
+          acc += jo[(v * 4 + hl) * Cfg::OSTRIDE + d] * f;
         }
-        const float val = L == 0.f ? 0.f : acc / L;  // no key: zeros; a NaN stays one
-        float lse = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
-        if (p.S > 1 && L != L) lse = INFINITY;  // so that the merge does not pass a NaN part over
-        const int hq = it.hk * GROUP + h;
-        const int64_t row = (int64_t)it.b * p.Hq + hq;
-        if (p.S == 1) {
-          const float f = p.out_scale ? p.out_scale[hq] : 1.f;
-          p.out[(int64_t)it.b * p.out_stride_tok + (int64_t)hq * D + d] = __float2bfloat16_rn(val * f);
-          if (p.lse && d == 0) p.lse[row] = lse;
-        } else {
-          const int64_t at = (int64_t)it.split * p.B * p.Hq + row;
-          p.part_o[at * D + d] = val;
-          if (d == 0) p.part_lse[at] = lse;
-        }
+        const int64_t at = (int64_t)x.id * GROUP + h;
+        p.part_o[at * D + d] = L == 0.f ? 0.f : acc / L;  // no key: zeros; a NaN stays one
+        if (d == 0) p.part_lse[at] = L == 0.f ? -INFINITY : (M + log2f(L) - kWeightLog2) * 0.6931471805599453f;
       }
-      asm volatile("bar.sync 1, %0;" ::"n"(NW * 32));  // the area is rewritten
+      asm volatile("bar.sync 1, %0;" ::"n"(kNW * 32));  // the area is rewritten
     }
   }
 }
 
-constexpr int kMaxSplits = 32;
+// One warp per (row, query head): the exact join of its pieces, times out_scale.
+template <int D>
+__global__ void __launch_bounds__(128) join_pieces_kernel(const DecodeQ8Params p, int group) {
+  constexpr int PER = D / 32;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= (int64_t)p.B * p.Hq) return;
+  const int b = (int)(row / p.Hq), h = (int)(row % p.Hq), hk = h / group;
+  const int unit = b * p.Hkv + hk;
+  int64_t first = unit;
+  int count = 1;
+  if (!p.whole) {
+    const int slots = row_of(p, b).slots;
+    const int64_t per = p.first_slot[p.B], from = p.first_slot[b] + (int64_t)hk * slots;
+    first = unit + from / per;
+    count = slots ? (int)((from + slots - 1) / per - from / per) + 1 : 0;
+  }
+  const float* o = p.part_o + (first * group + h % group) * D + lane * PER;
+  const float* lse = p.part_lse + first * group + h % group;
+  float M = -INFINITY, L = 0.f, acc[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+  constexpr int C = 8;  // pieces whose parts are requested together
+  for (int i0 = 0; i0 < count; i0 += C) {
+    float v[C][PER], ls[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const bool have = i0 + i < count;
+      ls[i] = have ? __ldcg(lse + (int64_t)(i0 + i) * group) : -INFINITY;
+      const float* src = o + (int64_t)(have ? i0 + i : i0) * group * D;
+      if constexpr (PER == 4) {
+        const float4 t = __ldcg(reinterpret_cast<const float4*>(src));
+        v[i][0] = t.x, v[i][1] = t.y, v[i][2] = t.z, v[i][3] = t.w;
+      } else {
+        const float2 t = __ldcg(reinterpret_cast<const float2*>(src));
+        v[i][0] = t.x, v[i][1] = t.y;
+      }
+    }
+    float top = M;
+#pragma unroll
+    for (int i = 0; i < C; ++i) top = fmaxf(top, ls[i]);
+    const float keep = M == top ? 1.f : exp2f((M - top) * 1.4426950408889634f);
+    M = top;
+    L *= keep;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] *= keep;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      if (ls[i] == -INFINITY) continue;  // no keys
+      const float w = ls[i] == M ? 1.f : exp2f((ls[i] - M) * 1.4426950408889634f);  // NaN where ls is
+      L += w;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) acc[e] = fmaf(w, v[i][e], acc[e]);
+    }
+  }
+  const float f = L == 0.f ? 0.f : (p.out_scale ? p.out_scale[h] : 1.f) / L;
+  __nv_bfloat16* dst = p.out + (int64_t)b * p.out_stride_tok + (int64_t)h * D + lane * PER;
+#pragma unroll
+  for (int e = 0; e < PER; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16(acc[e] * f, acc[e + 1] * f);
+  if (p.lse && lane == 0) p.lse[row] = L == 0.f ? -INFINITY : M + logf(L);
+}
+
 constexpr double kL2KeepFraction = 0.25;  // as decode_paged keeps
 constexpr int kL2KeepMaxBatch = 16;
 
@@ -464,8 +678,7 @@ int occupancy(int dev) {
     const auto kern = decode_q8_kernel<D, GROUP>;
     int occ = 0, sms = 0, l2 = 0;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Q8Cfg<D>::SMEM_BYTES) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, (Q8Cfg<D>::NW + 1) * 32, Q8Cfg<D>::SMEM_BYTES) !=
-            cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, kThreads, Q8Cfg<D>::SMEM_BYTES) != cudaSuccess ||
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
         cudaDeviceGetAttribute(&l2, cudaDevAttrL2CacheSize, dev) != cudaSuccess || occ < 1)
       return -1;
@@ -476,39 +689,45 @@ int occupancy(int dev) {
   return info.occ[di][gi];
 }
 
-// Splits for the persistent grid: the busiest CTA's slots, plus a slot's time per item for its
-// merge, the ring's fill, and the merge launch where there are splits.
-int choose_splits(int units, int slots, int ctas, int smax) {
-  int best = 1;
-  int64_t best_cost = INT64_MAX;
-  smax = std::min(smax, std::max(1, slots / 4));
-  for (int s = 1; s <= smax; ++s) {
-    const int64_t per_cta = ((int64_t)units * s + ctas - 1) / ctas;
-    const int64_t cost = per_cta * ((slots + s - 1) / s + 1) + 6 + (s > 1 ? 2 : 0);
-    if (cost < best_cost) {
-      best_cost = cost;
-      best = s;
-    }
-  }
-  return best;
-}
-
 template <int D, int GROUP>
-int launch_q8(const CUtensorMap& tmk, const CUtensorMap& tmv, DecodeQ8Params& prm, int smax, int dev, int keep,
-              cudaStream_t stream) {
+int launch_q8(const CUtensorMap& tmk, const CUtensorMap& tmv, DecodeQ8Params& prm, uint8_t* ws, size_t ws_bytes,
+              int dev, int keep, cudaStream_t stream) {
   const int occ = occupancy<D, GROUP>(dev);
   if (occ < 0) return LKV_ERR_CUDA;
-  const int ctas = g_dev[dev].sms * occ;
-  // the host does not know how many of a row's pages are in 8 bits: as if all were
-  prm.S = choose_splits(prm.B * prm.Hkv, (prm.W + 1) / 2, ctas, smax);
   if (keep && prm.B <= kL2KeepMaxBatch) {
     const double page_bytes = (double)prm.Hkv * Q8Cfg<D>::CODE_BYTES;
     prm.keep_pages = (int)std::min<double>(prm.W, kL2KeepFraction * g_dev[dev].l2 / (page_bytes * prm.B));
   }
-  const int64_t items = (int64_t)prm.S * prm.Hkv * prm.B;
-  if (items > INT_MAX) return LKV_ERR_UNSUPPORTED;
-  return launch_pdl(decode_q8_kernel<D, GROUP>, dim3((unsigned)std::min<int64_t>(items, ctas)),
-                    dim3((Q8Cfg<D>::NW + 1) * 32), Q8Cfg<D>::SMEM_BYTES, stream, tmk, tmv, prm) == cudaSuccess
+  // A CTA for every kLeastSlots slots that the tables have room for, up to two per SM.  A cut makes a piece
+  // more, which the workspace has to hold: first the rows' first slots, then the pieces' lse, then their o.
+  const int64_t units = (int64_t)prm.B * prm.Hkv;
+  int64_t ctas = std::min<int64_t>((int64_t)g_dev[dev].sms * occ,
+                                   std::max<int64_t>(1, units * prm.W / kLeastSlots));
+  const size_t piece_bytes = (size_t)GROUP * (D + 1) * sizeof(float), slack = 512;
+  const size_t table = ((size_t)prm.B + 1) * sizeof(int64_t);
+  const int64_t room = ws_bytes > table + slack ? (int64_t)((ws_bytes - table - slack) / piece_bytes) : 0;
+  int64_t pieces = units + ctas - 1;
+  if (room < pieces) {
+    // fewer cuts, or (with fewer CTAs than whole (row, head)s would keep busy) none
+    pieces = std::max(room, units);
+    const int64_t cut = pieces - units + 1;
+    prm.whole = cut < std::min(ctas, units);
+    ctas = prm.whole ? std::min(ctas, units) : cut;
+    if (prm.whole) pieces = units;
+  }
+  const size_t skip = prm.whole ? 0 : (table + 255) & ~size_t(255);
+  prm.first_slot = reinterpret_cast<int64_t*>(ws);
+  prm.part_lse = reinterpret_cast<float*>(ws + skip);
+  const size_t lse_bytes = ((size_t)pieces * GROUP * sizeof(float) + 255) & ~size_t(255);
+  prm.part_o = reinterpret_cast<float*>(ws + skip + lse_bytes);
+  if (skip + lse_bytes + (size_t)pieces * GROUP * D * sizeof(float) > ws_bytes) return LKV_ERR_WORKSPACE;
+  if (pieces > INT_MAX) return LKV_ERR_UNSUPPORTED;
+  if (launch_pdl(decode_q8_kernel<D, GROUP>, dim3((unsigned)ctas), dim3(kThreads), Q8Cfg<D>::SMEM_BYTES, stream, tmk,
+                 tmv, prm) != cudaSuccess)
+    return LKV_ERR_CUDA;
+  const int64_t rows = (int64_t)prm.B * prm.Hq;
+  return launch_pdl(join_pieces_kernel<D>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, prm, GROUP) ==
+                 cudaSuccess
              ? LKV_OK
              : LKV_ERR_CUDA;
 }
@@ -524,7 +743,7 @@ int decode_paged_q8(const DecodeQ8Args& a) {
   if (a.batch < 0 || a.max_pages_per_seq < 0 || a.max_pages_per_seq > INT_MAX / kPageTokens)
     return LKV_ERR_INVALID_ARGUMENT;
   if (a.batch == 0) return LKV_OK;
-  if ((int64_t)a.batch * a.num_kv_heads > INT_MAX / kMaxSplits) return LKV_ERR_UNSUPPORTED;
+  if ((int64_t)a.batch * a.num_q_heads > INT_MAX / 2) return LKV_ERR_UNSUPPORTED;
   if (!a.q || !a.codes || !a.scales || !a.block_table || !a.seq_k || !a.out) return LKV_ERR_INVALID_ARGUMENT;
   if (a.q8_pages < 0 || a.q8_pages > INT32_MAX || a.num_pages < 0 || a.num_pages > INT32_MAX)
     return LKV_ERR_INVALID_ARGUMENT;
@@ -546,10 +765,6 @@ int decode_paged_q8(const DecodeQ8Args& a) {
     st = make_pool_tensor_map(&tmv, a.pool_v, a.num_pages, a.num_kv_heads, a.head_dim);
     if (st != LKV_OK) return st;
   }
-  const int64_t rows = (int64_t)a.batch * a.num_q_heads;
-  // after the error header: the splits' lse, then (256-byte aligned) their o
-  const size_t per_split = (size_t)rows * (a.head_dim + 1) * sizeof(float) + 256;
-  const int smax = (int)std::min<size_t>(kMaxSplits, (a.workspace_bytes - kWorkspaceHeader) / per_split);
   DecodeQ8Params prm{};
   prm.q = static_cast<const __nv_bfloat16*>(a.q);
   prm.q_stride_tok = a.q_stride_tok;
@@ -565,10 +780,6 @@ int decode_paged_q8(const DecodeQ8Args& a) {
   prm.out_stride_tok = a.out_stride_tok;
   prm.lse = a.lse;
   prm.out_scale = a.out_scale;
-  uint8_t* ws = static_cast<uint8_t*>(a.workspace) + kWorkspaceHeader;
-  prm.part_lse = reinterpret_cast<float*>(ws);
-  prm.part_o =
-      reinterpret_cast<float*>(ws + (((size_t)rows * std::max(smax, 1) * sizeof(float) + 255) & ~size_t(255)));
   prm.err = static_cast<int*>(a.workspace);
   prm.B = a.batch;
   prm.Hq = a.num_q_heads;
@@ -577,8 +788,9 @@ int decode_paged_q8(const DecodeQ8Args& a) {
   prm.scale_log2 = a.softmax_scale * 1.4426950408889634f;
   cudaStream_t stream = static_cast<cudaStream_t>(a.stream);
   const int keep = a.flags & LKV_DECODE_L2_KEEP;
-  int st = LKV_ERR_UNSUPPORTED;
-#define LKV_Q8(DD, GG) st = launch_q8<DD, GG>(tmk, tmv, prm, std::max(smax, 1), dev, keep, stream); break
+  uint8_t* ws = static_cast<uint8_t*>(a.workspace) + kWorkspaceHeader;
+  const size_t ws_bytes = a.workspace_bytes - kWorkspaceHeader;
+#define LKV_Q8(DD, GG) return launch_q8<DD, GG>(tmk, tmv, prm, ws, ws_bytes, dev, keep, stream)
   if (a.head_dim == 128) {
     switch (group) {
       case 1: LKV_Q8(128, 1);
@@ -595,9 +807,6 @@ int decode_paged_q8(const DecodeQ8Args& a) {
     }
   }
 #undef LKV_Q8
-  if (st != LKV_OK || prm.S == 1) return st;
-  return merge_partials(prm.part_o, prm.part_lse, prm.S, rows, a.head_dim, a.num_q_heads, rows * a.head_dim, rows,
-                        a.out_scale, a.out, a.lse, stream, a.out_stride_tok);
 }
 
 }  // namespace lkv

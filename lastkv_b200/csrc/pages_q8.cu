@@ -89,8 +89,8 @@ __global__ void __launch_bounds__(kWarps * 32) quantise_pages_kernel(const Quant
     for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     scale[h] = amax / 127.0f;
     const bool zero = !(amax < INFINITY) || scale[h] == 0.f;
-    // one division per block: x * (127 / max), rounded by the addition that puts the integer into the
-    // low byte of 1.5 * 2^23 + q; where the reciprocal would overflow, x / s
+    // one division per block: x * (127 / max), rounded by the addition that puts q + 128 into the low
+    // byte of 1.5 * 2^23 + 128 + q; where the reciprocal would overflow, x / s
     const bool tiny = amax < 1e-30f;
     const float inv = tiny ? 0.f : 127.0f / amax;
 #pragma unroll
@@ -101,17 +101,17 @@ __global__ void __launch_bounds__(kWarps * 32) quantise_pages_kernel(const Quant
       for (int e = 0; e < 4; ++e) {
         const float a = bf16_lo(w[e]), b = bf16_hi(w[e]);
         if (!tiny) {
-          q[2 * e] = __float_as_uint(fmaf(a, inv, 12582912.0f));
-          q[2 * e + 1] = __float_as_uint(fmaf(b, inv, 12582912.0f));
+          q[2 * e] = __float_as_uint(fmaf(a, inv, 12583040.0f));
+          q[2 * e + 1] = __float_as_uint(fmaf(b, inv, 12583040.0f));
         } else {
-          q[2 * e] = zero ? 0u : (uint32_t)max(-127, min(127, __float2int_rn(a / scale[h])));
-          q[2 * e + 1] = zero ? 0u : (uint32_t)max(-127, min(127, __float2int_rn(b / scale[h])));
+          q[2 * e] = (uint32_t)(128 + max(-127, min(127, __float2int_rn(a / scale[h]))));
+          q[2 * e + 1] = (uint32_t)(128 + max(-127, min(127, __float2int_rn(b / scale[h]))));
         }
       }
       uint2 packed;
       packed.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
       packed.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
-      if (zero) packed = make_uint2(0, 0);
+      if (zero) packed = make_uint2(0x80808080u, 0x80808080u);
       *reinterpret_cast<uint2*>(tile + (i * STEP + r0) * PITCH + col) = packed;
     }
   }
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kWarps * 32) dequantise_pages_kernel(const Deq
   if (have) s = *reinterpret_cast<const float4*>(p.scales + block * kScalesPerBlock);
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
-    v[i] = have ? __ldcs(reinterpret_cast<const uint4*>(in + i * 512 + lane * 16)) : make_uint4(0, 0, 0, 0);
+    v[i] = have ? __ldcs(reinterpret_cast<const uint4*>(in + i * 512 + lane * 16)) : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) {
     const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
@@ -237,7 +237,8 @@ __global__ void __launch_bounds__(kWarps * 32) dequantise_pages_kernel(const Deq
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t w = (e & 2) ? q.y : q.x;
-      const float a = (float)(int8_t)(w >> ((e & 1) * 16)), b = (float)(int8_t)(w >> ((e & 1) * 16 + 8));
+      const uint32_t two = w >> ((e & 1) * 16);
+      const float a = (float)((int)(two & 255u) - 128), b = (float)((int)(two >> 8 & 255u) - 128);
       if constexpr (STAGE) {
         o[e] = which == 0 && (r < 8 ? bad0 : bad1) ? 0x7fff7fffu : pack_bf16(a, b);
       } else {

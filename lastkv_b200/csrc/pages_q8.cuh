@@ -1,8 +1,8 @@
 // Pages of keys and values in 8 bits: the layout that the kernels share.
 //
-// A page holds 16 tokens.  For every (page, KV head) there is one block of 2 x 16 x D int8 codes
-// (keys, then values) and four fp32 scales: keys of tokens 0-7 and 8-15, values of tokens 0-7 and
-// 8-15.  A code q stands for q * scale.  The codes lie in the order in which the 32 lanes of a warp
+// A page holds 16 tokens.  For every (page, KV head) there is one block of 2 x 16 x D codes (keys,
+// then values), whole numbers from -127 to 127 held in a byte as q + 128, and four fp32 scales: keys
+// of tokens 0-7 and 8-15, values of tokens 0-7 and 8-15.  A code q stands for q * scale.  The codes lie in the order in which the 32 lanes of a warp
 // take them as operands of mma m16n8k16, so a lane's 16-byte loads need no shuffles and meet no
 // bank conflicts; with lane = 4 g + c:
 //   keys    row r = 8 h + g, column d = 16 j + 8 t1 + 2 c + t0:
@@ -12,6 +12,8 @@
 // Either way a 32-bit word holds two operand registers: bytes 0 and 2, and bytes 1 and 3.
 #pragma once
 
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 
 namespace lkv {
@@ -19,19 +21,15 @@ namespace lkv {
 constexpr int kPageTokens = 16;
 constexpr int kScalesPerBlock = 4;  // fp32: keys 0-7, keys 8-15, values 0-7, values 8-15
 
-// Two pairs of int8 codes as bf16 pairs: bytes 0 and 2 of w in lo, bytes 1 and 3 in hi.  Exact: with
-// low = the code's seven low bits, 0x4300 | low is 128 + low and 0x4300 | sign bit is 128 or 256 in
-// bf16, whose difference is the code.  Seven instructions for four codes.
-__device__ __forceinline__ void codes_to_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  constexpr uint32_t kOne = 0x43004300u;
-  auto pair = [](uint32_t v) {
-    const uint32_t a = (v & 0x007f007fu) | kOne, b = (v & 0x00800080u) | kOne;
-    const __nv_bfloat162 d =
-        __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&d);
-  };
-  lo = pair(w);
-  hi = pair(w >> 8);
+// Four codes as two pairs of f16: bytes 0 and 2 of w in lo, bytes 1 and 3 in hi.  Exact: the byte q + 128 under
+// f16's 0x64 is 1024 + 128 + q.
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t a = __byte_perm(w, 0x64646464u, 0x4240), b = __byte_perm(w, 0x64646464u, 0x4341);
+  const __half2 off = __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
+  const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+  lo = *reinterpret_cast<const uint32_t*>(&x);
+  hi = *reinterpret_cast<const uint32_t*>(&y);
 }
 
 }  // namespace lkv

@@ -1055,8 +1055,9 @@ def _ints(t, n: int, what: str) -> int:
 
 class PagesQ8(NamedTuple):
     """Pages of 16 tokens' keys and values in 8 bits, with an fp32 scale for every 8 tokens of a
-    head: ``codes`` int8 [pages, Hkv, 2 (K, V), 16 * D] in the kernels' order (``from_codes`` and
-    ``to_codes`` translate) and ``scales`` fp32 [pages, Hkv, 4] (K of tokens 0-7, K of 8-15, V, V)."""
+    head: ``codes`` uint8 [pages, Hkv, 2 (K, V), 16 * D], each the code plus 128 and in the kernels'
+    order (``from_codes`` and ``to_codes`` translate), and ``scales`` fp32 [pages, Hkv, 4] (K of tokens 0-7,
+    K of 8-15, V, V)."""
 
     codes: torch.Tensor
     scales: torch.Tensor
@@ -1077,7 +1078,7 @@ class PagesQ8(NamedTuple):
     def empty(cls, num_pages: int, num_kv_heads: int, head_dim: int, device="cuda") -> "PagesQ8":
         """Pages of zeros."""
         require_heads(num_kv_heads, num_kv_heads, head_dim)
-        return cls(torch.zeros((num_pages, num_kv_heads, 2, PAGE_SIZE * head_dim), dtype=_I8, device=device),
+        return cls(torch.full((num_pages, num_kv_heads, 2, PAGE_SIZE * head_dim), 128, dtype=_U8, device=device),
                    torch.zeros((num_pages, num_kv_heads, 4), dtype=_F32, device=device))
 
     @classmethod
@@ -1093,13 +1094,14 @@ class PagesQ8(NamedTuple):
         codes[:, :, 0] = k.view(n, 2, 8, h, d // 32, 2, 2, 4, 2).permute(0, 3, 4, 2, 7, 5, 1, 8, 6).reshape(n, h, -1)
         # [page, h, c, t, head, k / 2, k % 2, m, g] -> [page, head, k / 2, g, c, k % 2, h, t, m]
         codes[:, :, 1] = v.view(n, 2, 4, 2, h, d // 32, 2, 2, 8).permute(0, 4, 5, 8, 2, 6, 1, 3, 7).reshape(n, h, -1)
-        return cls(codes, torch.cat((k_scale, v_scale), 1).transpose(1, 2).contiguous())
+        return cls(codes.view(_U8).bitwise_xor_(128), torch.cat((k_scale, v_scale), 1).transpose(1, 2).contiguous())
 
     def to_codes(self):
         """(k, v, k_scale, v_scale) as ``from_codes`` takes them."""
         n, h, d = self.num_pages, self.num_kv_heads, self.head_dim
-        k = self.codes[:, :, 0].view(n, h, d // 32, 8, 4, 2, 2, 2, 2).permute(0, 6, 3, 1, 2, 5, 8, 4, 7)
-        v = self.codes[:, :, 1].view(n, h, d // 32, 8, 4, 2, 2, 2, 2).permute(0, 6, 4, 7, 1, 2, 5, 8, 3)
+        codes = self.codes.bitwise_xor(128).view(_I8)
+        k = codes[:, :, 0].view(n, h, d // 32, 8, 4, 2, 2, 2, 2).permute(0, 6, 3, 1, 2, 5, 8, 4, 7)
+        v = codes[:, :, 1].view(n, h, d // 32, 8, 4, 2, 2, 2, 2).permute(0, 6, 4, 7, 1, 2, 5, 8, 3)
         return (k.reshape(n, PAGE_SIZE, h, d), v.reshape(n, PAGE_SIZE, h, d), *self.token_scales())
 
     def token_scales(self):
@@ -1111,9 +1113,9 @@ def _check_pages_q8(c) -> None:
     if type(c) is not PagesQ8:
         _fail("the 8-bit pages must be PagesQ8")
     codes, scales = c
-    if codes.dtype != _I8 or codes.dim() != 4 or codes.shape[2] != 2 or codes.shape[3] not in (1024, 2048) \
+    if codes.dtype != _U8 or codes.dim() != 4 or codes.shape[2] != 2 or codes.shape[3] not in (1024, 2048) \
             or not codes.is_contiguous():
-        _fail("PagesQ8.codes must be contiguous int8 [pages, Hkv, 2, 16 * D] with D 64 or 128")
+        _fail("PagesQ8.codes must be contiguous uint8 [pages, Hkv, 2, 16 * D] with D 64 or 128")
     if scales.dtype != _F32 or scales.shape != (codes.shape[0], codes.shape[1], 4) or not scales.is_contiguous():
         _fail("PagesQ8.scales must be contiguous fp32 [pages, Hkv, 4]")
     _here(codes, "PagesQ8.codes")

@@ -106,7 +106,7 @@ def test_8_bit_history_lays_out_its_raw_ring_in_front():
     h = cache.plan_host(2)
     assert h["nsrc"] == 2 and h["bt"][1, :2].tolist() == [7, 8]  # two finished chunks back: one chunk older
     codes = cache.q8.codes
-    codes.copy_(torch.randint(-127, 128, codes.shape).to(torch.int8))
+    codes.copy_(torch.randint(1, 256, codes.shape).to(torch.uint8))
     was = [cache.q8.codes[cache.src_table[b]].clone() for b in range(2)]
     cache.reserve(300)
     assert cache.q8.num_pages == 2 * 19

@@ -171,7 +171,7 @@ def test_pages_past_4_gib():
     hkv, d = 8, 128
     page = hkv * 2 * 16 * d
     pages = 2 ** 32 // page + 64
-    codes = torch.zeros((pages, hkv, 2, 16 * d), dtype=torch.int8, device="cuda")
+    codes = torch.zeros((pages, hkv, 2, 16 * d), dtype=torch.uint8, device="cuda")
     scales = torch.zeros((pages, hkv, 4), device="cuda")
     t = random_cache(21, [500], [32], hkv, d, extra=0)
     small = _cache(t)

@@ -21,13 +21,14 @@ def test_codes_layout_round_trip(d):
     assert (c.num_pages, c.num_kv_heads, c.head_dim) == (n, h, d)
     for a, b in zip(c.to_codes(), (k, v, ks, vs)):
         assert torch.equal(a, b)
+    raw = c.codes.int() - 128
     for r in range(16):
         for x in range(d):  # the order that include/lastkv_b200.h gives
             half, tile = r // 8, x // 16
             at = tile // 2 * 512 + (4 * (r % 8) + x // 2 % 4) * 16 + (tile % 2 * 2 + half) * 4 + 2 * (x % 2) + x // 8 % 2
-            assert torch.equal(c.codes[:, :, 0, at], k[:, r, :, x])
+            assert torch.equal(raw[:, :, 0, at], k[:, r, :, x].int())
             at = tile // 2 * 512 + (4 * (x % 8) + r // 2 % 4) * 16 + (tile % 2 * 2 + half) * 4 + 2 * (r % 2) + x // 8 % 2
-            assert torch.equal(c.codes[:, :, 1, at], v[:, r, :, x])
+            assert torch.equal(raw[:, :, 1, at], v[:, r, :, x].int())
     assert torch.equal(c.scales[..., 0], ks[:, 0]) and torch.equal(c.scales[..., 3], vs[:, 1])
 
 

@@ -113,7 +113,7 @@ def test_pages_outside_the_pools_are_skipped():
     err = torch.zeros(4, dtype=torch.int32, device="cuda")
     ops.quantize_pages(k, v, _ids(0, 4, -1, 2, 1), cache, _ids(0, 1, 1, 3, 2), error_word=err)
     assert err[0] == 2 and err[1] == 8
-    assert bool((cache.codes[1] == 0).all()) and bool((cache.scales[1] == 0).all())
+    assert bool((cache.codes[1] == 128).all()) and bool((cache.scales[1] == 0).all())
     _check_codes(k[[0, 1]], cache.to_codes()[0][[0, 2]], cache.to_codes()[2][[0, 2]])
     err.zero_()
     back = torch.full_like(k, 7.0), torch.full_like(v, 7.0)
