@@ -23,7 +23,7 @@
 // (row, head), and every CTA takes the same number of them, so ragged rows cost no balance; a
 // (row, head)'s part within a CTA is a piece, whose normalised partial goes to the workspace, and
 // join_pieces_kernel joins each row's pieces.  Per CTA one warp fills a ring of slots (an 8-bit page's codes and
-// scales by two bulk copies, a bf16 page's halves by TMA), 7 warps take the slots in turn.
+// scales by two bulk copies, a bf16 page's halves by TMA), 6 warps take the slots in turn.
 
 #include <math.h>
 
@@ -67,13 +67,19 @@ struct DecodeQ8Params {
   int keep_pages;  // leading columns that stay in L2
 };
 
-constexpr int kNW = 7;  // consumer warps: with the producer 16 warps on an SM, 128 registers for a thread
+constexpr int kNW = 6;  // consumer warps: with the producer 14 warps on an SM, 128 registers for a thread
 constexpr int kThreads = (kNW + 1) * 32;
 constexpr int kLeastSlots = kNW;  // of a CTA that has any: a slot for each warp
 
 template <int D>
 struct Q8Cfg {
-  static constexpr int RING = D == 128 ? 11 : 22;         // 88 KB of slots: two CTAs per SM
+  // 96 KB of slots: two CTAs per SM.  A multiple of the warps, so that a ring place is always the same warp's: two
+  // warps could wait for two different copies into one place with the same barrier parity.
+  static constexpr int RING = D == 128 ? 12 : 24;
+  static_assert(RING % kNW == 0, "a ring place belongs to one warp");
+  // Slots that the producer waits for and copies at once, a lane per half: one after another they took it
+  // 600 cycles each, more than a slot's time at the memory's rate.
+  static constexpr int BATCH = RING / 3;
   static constexpr int HALVES = D / 64;
   static constexpr int TILE_BYTES = kPageTokens * 128;    // 16 rows x 64 bf16
   static constexpr int CODE_BYTES = 2 * kPageTokens * D;  // keys and values of an 8-bit page
@@ -81,9 +87,9 @@ struct Q8Cfg {
   static constexpr int OSTRIDE = D + 4;
   static constexpr int OFF_SCALE = RING * SLOT_BYTES;     // two pages' scales per slot
   static constexpr int OFF_Q = OFF_SCALE + RING * 32;     // bf16 Q operands of the current piece
-  // join area: o [kNW][4 heads][OSTRIDE], then m and l [kNW][8]
+  // join area: o [kNW][2 heads][OSTRIDE], then m and l [kNW][8]
   static constexpr int OFF_JOIN = OFF_Q + (D / 16) * 32 * 8;
-  static constexpr int OFF_BAR = OFF_JOIN + kNW * 4 * OSTRIDE * 4 + 2 * kNW * 8 * 4;
+  static constexpr int OFF_BAR = OFF_JOIN + kNW * 2 * OSTRIDE * 4 + 2 * kNW * 8 * 4;
   static constexpr int SMEM_BYTES = 1024 + OFF_BAR + 2 * RING * 8 + 64;
 };
 
@@ -177,7 +183,8 @@ __device__ __forceinline__ bool next_piece(const DecodeQ8Params& p, Share& s, Pi
   return true;
 }
 
-// All threads: the CTA's share.  Piece u of the (row, head)s in order, cut at CTA c's first slot, is piece u + c.
+// The CTA's share, called by all threads.  Piece u of the (row, head)s in order, cut at CTA c's first slot, is
+// piece u + c.
 __device__ Share share_of(const DecodeQ8Params& p, int64_t* sm, int* sm_row) {
   Share s{};
   const int64_t units = (int64_t)p.B * p.Hkv;
@@ -190,56 +197,75 @@ __device__ Share share_of(const DecodeQ8Params& p, int64_t* sm, int* sm_row) {
     return s;
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  constexpr int WARPS = kThreads / 32;
-  int64_t mine = 0;
-  for (int b = threadIdx.x; b < p.B; b += kThreads) mine += row_of(p, b).slots;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) sm[warp] = mine;
-  if (threadIdx.x == 0) *sm_row = -1;
-  __syncthreads();
-  int64_t total = 0;
-  for (int w = 0; w < WARPS; ++w) total += sm[w];
-  total *= p.Hkv;
-  const int64_t per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kLeastSlots);
-  const int64_t first = per * blockIdx.x;
-  if (first >= total && blockIdx.x != 0) return s;
-  // the row that holds the first slot (CTA 0 goes through all rows, for join_pieces_kernel)
-  int64_t before = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
-    const int b = b0 + threadIdx.x;
-    const int64_t here = b < p.B ? (int64_t)row_of(p, b).slots * p.Hkv : 0;
-    int64_t sum = here;
+  auto prefix = [lane](int64_t v) {  // inclusive, over the warp
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += up;
+      const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += up;
     }
-    __syncthreads();  // sm is read
-    if (lane == 31) sm[warp] = sum;
+    return v;
+  };
+  int64_t total, per, first, start;  // start: the first slot of the row that holds the CTA's first
+  if (p.B <= 32) {  // every warp for itself
+    const int64_t here = lane < p.B ? (int64_t)row_of(p, lane).slots * p.Hkv : 0;
+    const int64_t upto = prefix(here);
+    total = __shfl_sync(0xffffffffu, upto, 31);
+    per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kLeastSlots);
+    first = per * blockIdx.x;
+    if (blockIdx.x == 0 && warp == 0) {
+      if (lane < p.B) p.first_slot[lane] = upto - here;
+      if (lane == 0) p.first_slot[p.B] = per;
+    }
+    if (first >= total) return s;
+    s.b = __ffs(__ballot_sync(0xffffffffu, upto > first)) - 1;
+    start = __shfl_sync(0xffffffffu, upto - here, s.b);
+  } else {
+    constexpr int WARPS = kThreads / 32;
+    int64_t mine = 0;
+    for (int b = threadIdx.x; b < p.B; b += kThreads) mine += row_of(p, b).slots;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) sm[warp] = mine;
     __syncthreads();
-    int64_t start = before + sum - here;
-    for (int w = 0; w < WARPS; ++w) {
-      if (w < warp) start += sm[w];
-      before += sm[w];
+    total = 0;
+    for (int w = 0; w < WARPS; ++w) total += sm[w];
+    total *= p.Hkv;
+    per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kLeastSlots);
+    first = per * blockIdx.x;
+    if (first >= total && blockIdx.x != 0) return s;
+    // CTA 0 goes through all rows, for join_pieces_kernel
+    int64_t before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+      const int b = b0 + threadIdx.x;
+      const int64_t here = b < p.B ? (int64_t)row_of(p, b).slots * p.Hkv : 0;
+      const int64_t upto = prefix(here);
+      __syncthreads();  // sm is read
+      if (lane == 31) sm[warp] = upto;
+      __syncthreads();
+      int64_t at = before + upto - here;
+      for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) at += sm[w];
+        before += sm[w];
+      }
+      if (blockIdx.x == 0 && b < p.B) {
+        p.first_slot[b] = at;
+        if (b == p.B - 1) p.first_slot[p.B] = per;
+      }
+      if (here > 0 && at <= first && first < at + here) {
+        *sm_row = b;
+        sm[WARPS] = at;
+      }
+      if (blockIdx.x != 0 && before > first) break;  // the same for all threads
     }
-    if (blockIdx.x == 0 && b < p.B) {
-      p.first_slot[b] = start;
-      if (b == p.B - 1) p.first_slot[p.B] = per;
-    }
-    if (here > 0 && start <= first && first < start + here) {
-      *sm_row = b;
-      sm[WARPS] = start;
-    }
-    if (blockIdx.x != 0 && before > first) break;  // the same for all threads
+    __syncthreads();
+    if (first >= total) return s;
+    s.b = *sm_row;
+    start = sm[WARPS];
   }
-  __syncthreads();
-  if (first >= total) return s;
-  s.b = *sm_row;
-  const Row r = row_of(p, s.b);
-  const int64_t off = first - sm[WARPS];
-  s.hk = (int)(off / r.slots);
-  s.at = (int)(off % r.slots);
+  const int slots = row_of(p, s.b).slots;
+  const int64_t off = first - start;
+  s.hk = (int)(off / slots);
+  s.at = (int)(off % slots);
   s.piece = s.b * p.Hkv + s.hk + blockIdx.x;
   s.left = min(per, total - first);
   return s;
@@ -254,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* jo = reinterpret_cast<float*>(smem + Cfg::OFF_JOIN);
-  float* jm = jo + kNW * 4 * Cfg::OSTRIDE;
+  float* jm = jo + kNW * 2 * Cfg::OSTRIDE;
   float* jl = jm + kNW * 8;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
   uint64_t* empty = full + RING;
@@ -310,11 +336,13 @@ __global__ void __launch_bounds__(kThreads, 2)
         const uint32_t both = bytes + __shfl_xor_sync(0xffffffffu, bytes, 1);
         const uint64_t pol = c < p.keep_pages ? pol_last : pol_first;
         const int64_t block = (int64_t)pid * p.Hkv + x.hk;
-        for (int i = 0; i < min(16, count - k0); ++i, ++gs) {
-          const int s = (int)(gs % RING);
-          ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((gs / RING) & 1u) ^ 1u));
+        for (int i0 = 0; i0 < min(16, count - k0); i0 += Cfg::BATCH) {
+          const int i = (lane >> 1) - i0;
+          const bool mine = i >= 0 && i < Cfg::BATCH && c >= 0;
+          const uint32_t at = gs + max(i, 0);
+          const int s = (int)(at % RING);
+          ok = __all_sync(0xffffffffu, !mine || mbar_wait(&empty[s], ((at / RING) & 1u) ^ 1u));
           if (!ok) break;
-          const bool mine = (lane >> 1) == i;
           uint8_t* dst = smem + s * Cfg::SLOT_BYTES + u * Cfg::CODE_BYTES;
           float* sc = reinterpret_cast<float*>(smem + Cfg::OFF_SCALE + s * 32 + u * 16);
           if (mine && bad) {
@@ -341,6 +369,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 tma_load_4d_hint(dst + h * Cfg::TILE_BYTES, u ? &tmv : &tmk, &full[s], h * 64, x.hk, 0, pid, pol);
             }
           }
+          gs += min(Cfg::BATCH, count - k0 - i0);
         }
       }
     }
@@ -415,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     };
 
     const int count = x.s1 - x.s0;
-    for (int k = warp; k < count; k += kNW) {
+    for (int k = (warp + kNW - (int)(gs % kNW)) % kNW; k < count; k += kNW) {
       const uint32_t at = gs + k;
       const int s = (int)(at % RING);
       if (!mbar_wait(&full[s], (at / RING) & 1u)) {
@@ -557,11 +586,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       jl[warp * 8 + 2 * c] = l0;
       jl[warp * 8 + 2 * c + 1] = l1;
     }
-    // four heads at a time: thread (g, c) holds heads 2c and 2c + 1
+    // two heads at a time: thread (g, c) holds heads 2c and 2c + 1
 #pragma unroll
-    for (int hc = 0; hc < (GROUP + 3) / 4; ++hc) {
-      if ((c >> 1) == hc) {
-        float* w0 = jo + (warp * 4 + 2 * c - 4 * hc) * Cfg::OSTRIDE;
+    for (int hc = 0; hc < (GROUP + 1) / 2; ++hc) {
+      if (c == hc) {
+        float* w0 = jo + warp * 2 * Cfg::OSTRIDE;
         float* w1 = w0 + Cfg::OSTRIDE;
 #pragma unroll
         for (int k = 0; k < KT; ++k) {
@@ -573,9 +602,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       asm volatile("bar.sync 1, %0;" ::"n"(kNW * 32));
       if (*fail_flag) return;  // the same for all consumer warps
-      constexpr int HC = GROUP < 4 ? GROUP : 4;
+      constexpr int HC = GROUP < 2 ? GROUP : 2;
       for (int idx = threadIdx.x; idx < HC * D; idx += kNW * 32) {
-        const int hl = idx / D, d = idx % D, h = 4 * hc + hl;
+        const int hl = idx / D, d = idx % D, h = 2 * hc + hl;
         float M = -INFINITY;
 #pragma unroll
         for (int v = 0; v < kNW; ++v) M = fmaxf(M, jm[v * 8 + h]);
@@ -584,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int v = 0; v < kNW; ++v) {
           const float f = jm[v * 8 + h] == M ? 1.f : exp2f(jm[v * 8 + h] - M);
           L += jl[v * 8 + h] * f;
-          acc += jo[(v * 4 + hl) * Cfg::OSTRIDE + d] * f;
+          acc += jo[(v * 2 + hl) * Cfg::OSTRIDE + d] * f;
         }
         const int64_t at = (int64_t)x.id * GROUP + h;
         p.part_o[at * D + d] = L == 0.f ? 0.f : acc / L;  // no key: zeros; a NaN stays one
@@ -595,14 +624,17 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
-// One warp per (row, query head): the exact join of its pieces, times out_scale.
-template <int D>
-__global__ void __launch_bounds__(128) join_pieces_kernel(const DecodeQ8Params p, int group) {
+// The exact join of a (row, query head)'s pieces, times out_scale.  WARPS warps take a row's pieces by turns: one
+// where there are many rows, with few pieces each, 8 where there are few.
+template <int D, int WARPS>
+__global__ void __launch_bounds__(256) join_pieces_kernel(const DecodeQ8Params p, int group) {
   constexpr int PER = D / 32;
+  __shared__ float part[WARPS > 1 ? 8 : 1][D + 2];
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = WARPS > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 8 + warp;
+  const int turn = WARPS > 1 ? warp : 0;
   if (row >= (int64_t)p.B * p.Hq) return;
   const int b = (int)(row / p.Hq), h = (int)(row % p.Hq), hk = h / group;
   const int unit = b * p.Hkv + hk;
@@ -620,13 +652,15 @@ __global__ void __launch_bounds__(128) join_pieces_kernel(const DecodeQ8Params p
 #pragma unroll
   for (int e = 0; e < PER; ++e) acc[e] = 0.f;
   constexpr int C = 8;  // pieces whose parts are requested together
-  for (int i0 = 0; i0 < count; i0 += C) {
+  auto weight = [&M](float ls) { return ls == M ? 1.f : exp2f((ls - M) * 1.4426950408889634f); };
+  for (int i0 = turn; i0 < count; i0 += C * WARPS) {
     float v[C][PER], ls[C];
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      const bool have = i0 + i < count;
-      ls[i] = have ? __ldcg(lse + (int64_t)(i0 + i) * group) : -INFINITY;
-      const float* src = o + (int64_t)(have ? i0 + i : i0) * group * D;
+      const int at = i0 + i * WARPS;
+      const bool have = at < count;
+      ls[i] = have ? __ldcg(lse + (int64_t)at * group) : -INFINITY;
+      const float* src = o + (int64_t)(have ? at : i0) * group * D;
       if constexpr (PER == 4) {
         const float4 t = __ldcg(reinterpret_cast<const float4*>(src));
         v[i][0] = t.x, v[i][1] = t.y, v[i][2] = t.z, v[i][3] = t.w;
@@ -646,10 +680,28 @@ __global__ void __launch_bounds__(128) join_pieces_kernel(const DecodeQ8Params p
 #pragma unroll
     for (int i = 0; i < C; ++i) {
       if (ls[i] == -INFINITY) continue;  // no keys
-      const float w = ls[i] == M ? 1.f : exp2f((ls[i] - M) * 1.4426950408889634f);  // NaN where ls is
+      const float w = weight(ls[i]);     // NaN where ls is
       L += w;
 #pragma unroll
       for (int e = 0; e < PER; ++e) acc[e] = fmaf(w, v[i][e], acc[e]);
+    }
+  }
+  if constexpr (WARPS > 1) {
+#pragma unroll
+    for (int e = 0; e < PER; ++e) part[warp][lane * PER + e] = acc[e];
+    if (lane == 0) part[warp][D] = M, part[warp][D + 1] = L;
+    __syncthreads();
+    if (warp != 0) return;
+    M = -INFINITY;
+    L = 0.f;
+    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, part[w][D]);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+    for (int w = 0; w < WARPS; ++w) {
+      const float f = weight(part[w][D]);
+      L += part[w][D + 1] * f;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) acc[e] = fmaf(part[w][lane * PER + e], f, acc[e]);
     }
   }
   const float f = L == 0.f ? 0.f : (p.out_scale ? p.out_scale[h] : 1.f) / L;
@@ -726,7 +778,9 @@ int launch_q8(const CUtensorMap& tmk, const CUtensorMap& tmv, DecodeQ8Params& pr
                  tmv, prm) != cudaSuccess)
     return LKV_ERR_CUDA;
   const int64_t rows = (int64_t)prm.B * prm.Hq;
-  return launch_pdl(join_pieces_kernel<D>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, prm, GROUP) ==
+  const bool few = !prm.whole && rows <= 4 * g_dev[dev].sms;
+  const auto join = few ? join_pieces_kernel<D, 8> : join_pieces_kernel<D, 1>;
+  return launch_pdl(join, dim3((unsigned)(few ? rows : (rows + 7) / 8)), dim3(256), 0, stream, prm, GROUP) ==
                  cudaSuccess
              ? LKV_OK
              : LKV_ERR_CUDA;
