@@ -830,7 +830,7 @@ size_t decode_workspace_bytes(int batch, int hq, int d, int max_pages) {
   // s splits of decode_paged's per-split layout (o and lse of every row + 256 bytes of alignment slack), and for
   // decode_paged_q8 a piece of 8 heads for each of its CTAs' cuts and the rows' first slots
   return kWorkspaceHeader + (size_t)s * decode_split_bytes(rows, std::max(d, 64)) +
-         decode_split_bytes(kQ8Cuts * 8, std::max(d, 64)) + ((size_t)std::max(batch, 0) + 1) * sizeof(int64_t) + 256;
+         decode_split_bytes(kQ8Cuts * 8, std::max(d, 64)) + ((size_t)std::max(batch, 0) + 1) * sizeof(int) + 256;
 }
 
 int decode_paged(const DecodeArgs& a) {

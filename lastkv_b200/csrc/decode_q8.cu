@@ -59,7 +59,7 @@ struct DecodeQ8Params {
   const float* out_scale;  // [Hq] or null
   float* part_o;           // [pieces][GROUP][D], normalised
   float* part_lse;         // [pieces][GROUP], natural log
-  int64_t* first_slot;     // [B + 1]: the rows' first slots, written for join_pieces_kernel
+  int* first_slot;         // [B + 1]: the rows' first slots and the slots per CTA, written for join_pieces_kernel
   int* err;
   int B, Hq, Hkv, W;
   int whole;  // 1: the workspace holds one piece per (row, head): CTAs take whole ones
@@ -120,6 +120,14 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// 16 bytes to shared memory, and this thread's arrival on a barrier once its copies so far are there.
+__device__ __forceinline__ void async_copy16(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void async_copy_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 __device__ __forceinline__ float lg2_approx(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -148,8 +156,7 @@ __device__ __forceinline__ Row row_of(const DecodeQ8Params& p, int b) {
 
 // What a CTA takes: pieces from slot `at` of (row b, head hk) on, `left` slots in all (whole: `left` (row, head)s).
 struct Share {
-  int b, hk, at, piece;
-  int64_t left;
+  int b, hk, at, piece, left;
 };
 
 // A piece: slots [s0, s1) of (row b, head hk).
@@ -172,7 +179,7 @@ __device__ __forceinline__ bool next_piece(const DecodeQ8Params& p, Share& s, Pi
   x.hk = s.hk;
   x.id = s.piece;
   x.s0 = s.at;
-  x.s1 = p.whole ? x.r.slots : (int)min((int64_t)x.r.slots, s.at + s.left);
+  x.s1 = p.whole ? x.r.slots : min(x.r.slots, s.at + s.left);
   s.left -= p.whole ? 1 : x.s1 - x.s0;
   s.at = 0;
   ++s.piece;
@@ -184,35 +191,38 @@ __device__ __forceinline__ bool next_piece(const DecodeQ8Params& p, Share& s, Pi
 }
 
 // The CTA's share, called by all threads.  Piece u of the (row, head)s in order, cut at CTA c's first slot, is
-// piece u + c.
-__device__ Share share_of(const DecodeQ8Params& p, int64_t* sm, int* sm_row) {
+// piece u + c.  (All slots together are below 2^31: the host checks the tables' size.)
+__device__ Share share_of(const DecodeQ8Params& p, int* sm, int* sm_row) {
   Share s{};
-  const int64_t units = (int64_t)p.B * p.Hkv;
+  const unsigned cta = blockIdx.x, ctas = gridDim.x;
   if (p.whole) {
-    const int64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+    const unsigned units = (unsigned)p.B * p.Hkv;
+    const unsigned u0 = (unsigned)((uint64_t)units * cta / ctas), u1 = (unsigned)((uint64_t)units * (cta + 1) / ctas);
     s.b = (int)(u0 / p.Hkv);
     s.hk = (int)(u0 % p.Hkv);
     s.piece = (int)u0;
-    s.left = u1 - u0;
+    s.left = (int)(u1 - u0);
     return s;
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto prefix = [lane](int64_t v) {  // inclusive, over the warp
+  auto prefix = [lane](int v) {  // inclusive, over the warp
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
+      const int up = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v += up;
     }
     return v;
   };
-  int64_t total, per, first, start;  // start: the first slot of the row that holds the CTA's first
+  auto share = [ctas](int all) { return max((int)(((unsigned)all + ctas - 1) / ctas), kLeastSlots); };
+  int total, per, start;   // start: the first slot of the row that holds the CTA's first
+  int64_t first;
   if (p.B <= 32) {  // every warp for itself
-    const int64_t here = lane < p.B ? (int64_t)row_of(p, lane).slots * p.Hkv : 0;
-    const int64_t upto = prefix(here);
+    const int here = lane < p.B ? row_of(p, lane).slots * p.Hkv : 0;
+    const int upto = prefix(here);
     total = __shfl_sync(0xffffffffu, upto, 31);
-    per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kLeastSlots);
-    first = per * blockIdx.x;
-    if (blockIdx.x == 0 && warp == 0) {
+    per = share(total);
+    first = (int64_t)per * cta;
+    if (cta == 0 && warp == 0) {
       if (lane < p.B) p.first_slot[lane] = upto - here;
       if (lane == 0) p.first_slot[p.B] = per;
     }
@@ -221,33 +231,32 @@ __device__ Share share_of(const DecodeQ8Params& p, int64_t* sm, int* sm_row) {
     start = __shfl_sync(0xffffffffu, upto - here, s.b);
   } else {
     constexpr int WARPS = kThreads / 32;
-    int64_t mine = 0;
+    int mine = 0;
     for (int b = threadIdx.x; b < p.B; b += kThreads) mine += row_of(p, b).slots;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    mine = __reduce_add_sync(0xffffffffu, mine);
     if (lane == 0) sm[warp] = mine;
     __syncthreads();
     total = 0;
     for (int w = 0; w < WARPS; ++w) total += sm[w];
     total *= p.Hkv;
-    per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kLeastSlots);
-    first = per * blockIdx.x;
-    if (first >= total && blockIdx.x != 0) return s;
+    per = share(total);
+    first = (int64_t)per * cta;
+    if (first >= total && cta != 0) return s;
     // CTA 0 goes through all rows, for join_pieces_kernel
-    int64_t before = 0;
+    int before = 0;
     for (int b0 = 0; b0 < p.B; b0 += kThreads) {
       const int b = b0 + threadIdx.x;
-      const int64_t here = b < p.B ? (int64_t)row_of(p, b).slots * p.Hkv : 0;
-      const int64_t upto = prefix(here);
+      const int here = b < p.B ? row_of(p, b).slots * p.Hkv : 0;
+      const int upto = prefix(here);
       __syncthreads();  // sm is read
       if (lane == 31) sm[warp] = upto;
       __syncthreads();
-      int64_t at = before + upto - here;
+      int at = before + upto - here;
       for (int w = 0; w < WARPS; ++w) {
         if (w < warp) at += sm[w];
         before += sm[w];
       }
-      if (blockIdx.x == 0 && b < p.B) {
+      if (cta == 0 && b < p.B) {
         p.first_slot[b] = at;
         if (b == p.B - 1) p.first_slot[p.B] = per;
       }
@@ -255,19 +264,18 @@ __device__ Share share_of(const DecodeQ8Params& p, int64_t* sm, int* sm_row) {
         *sm_row = b;
         sm[WARPS] = at;
       }
-      if (blockIdx.x != 0 && before > first) break;  // the same for all threads
+      if (cta != 0 && before > first) break;  // the same for all threads
     }
     __syncthreads();
     if (first >= total) return s;
     s.b = *sm_row;
     start = sm[WARPS];
   }
-  const int slots = row_of(p, s.b).slots;
-  const int64_t off = first - start;
+  const unsigned slots = row_of(p, s.b).slots, off = (unsigned)((int)first - start);
   s.hk = (int)(off / slots);
   s.at = (int)(off % slots);
-  s.piece = s.b * p.Hkv + s.hk + blockIdx.x;
-  s.left = min(per, total - first);
+  s.piece = s.b * p.Hkv + s.hk + (int)cta;
+  s.left = min(per, total - (int)first);
   return s;
 }
 
@@ -285,13 +293,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
   uint64_t* empty = full + RING;
   volatile int* fail_flag = reinterpret_cast<volatile int*>(empty + RING);
-  __shared__ int64_t sm_sum[kThreads / 32 + 1];
+  __shared__ int sm_sum[kThreads / 32 + 1];
   __shared__ int sm_row;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < RING; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], 3);  // the expected bytes, and the scales of both halves
       mbar_init(&empty[s], 1);
     }
     *fail_flag = 0;
@@ -332,13 +340,13 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (col >= 0) id = __ldg(row + col);
         const bool q8 = c >= 0 && c < x.r.nh;
         const bool bad = c >= 0 && (pid < 0 || (int64_t)pid >= (q8 ? p.q8_pages : p.pool_pages));
-        const uint32_t bytes = c >= 0 && !bad ? Cfg::CODE_BYTES + (q8 ? 16 : 0) : 0;
+        const uint32_t bytes = c >= 0 && !bad ? Cfg::CODE_BYTES : 0;
         const uint32_t both = bytes + __shfl_xor_sync(0xffffffffu, bytes, 1);
         const uint64_t pol = c < p.keep_pages ? pol_last : pol_first;
         const int64_t block = (int64_t)pid * p.Hkv + x.hk;
         for (int i0 = 0; i0 < min(16, count - k0); i0 += Cfg::BATCH) {
           const int i = (lane >> 1) - i0;
-          const bool mine = i >= 0 && i < Cfg::BATCH && c >= 0;
+          const bool mine = i >= 0 && i < Cfg::BATCH && k0 + i0 + i < count;
           const uint32_t at = gs + max(i, 0);
           const int s = (int)(at % RING);
           ok = __all_sync(0xffffffffu, !mine || mbar_wait(&empty[s], ((at / RING) & 1u) ^ 1u));
@@ -359,10 +367,17 @@ __global__ void __launch_bounds__(kThreads, 2)
           __syncwarp();
           if (mine && u == 0) mbar_arrive_expect_tx(&full[s], both);
           __syncwarp();
+          if (mine) {
+            if (bytes && q8) {  // the scales by a plain asynchronous copy: all lanes' in one instruction
+              async_copy16(sc, p.scales + block * kScalesPerBlock);
+              async_copy_arrive(&full[s]);
+            } else {
+              mbar_arrive(&full[s]);
+            }
+          }
           if (mine && bytes) {
             if (q8) {
               bulk_load_hint(dst, p.codes + block * Cfg::CODE_BYTES, Cfg::CODE_BYTES, &full[s], pol);
-              bulk_load(sc, p.scales + block * kScalesPerBlock, 16, &full[s]);
             } else {
 #pragma unroll
               for (int h = 0; h < Cfg::HALVES; ++h)
@@ -576,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     gs += count;
 
     // ------------------------------------------------------------ the piece's partial
-    // Only consumer warps write the failure flag, and only before this barrier.
+    // Only consumer warps write the failure flag, and only before the first barrier.
     l0 = sum_over_rows(l0);
     l1 = sum_over_rows(l1);
     if (failed && lane == 0) *fail_flag = 1;
@@ -586,6 +601,16 @@ __global__ void __launch_bounds__(kThreads, 2)
       jl[warp * 8 + 2 * c] = l0;
       jl[warp * 8 + 2 * c + 1] = l1;
     }
+    asm volatile("bar.sync 1, %0;" ::"n"(kNW * 32));
+    if (*fail_flag) return;  // the same for all consumer warps
+    // every warp brings its sums to the maximum of all of them
+    auto factor = [&](int h, float own) {
+      float M = jm[h];
+#pragma unroll
+      for (int v = 1; v < kNW; ++v) M = fmaxf(M, jm[v * 8 + h]);
+      return own == M ? 1.f : ex2_approx(own - M);
+    };
+    const float f0 = factor(2 * c, m0), f1 = factor(2 * c + 1, m1);
     // two heads at a time: thread (g, c) holds heads 2c and 2c + 1
 #pragma unroll
     for (int hc = 0; hc < (GROUP + 1) / 2; ++hc) {
@@ -594,29 +619,32 @@ __global__ void __launch_bounds__(kThreads, 2)
         float* w1 = w0 + Cfg::OSTRIDE;
 #pragma unroll
         for (int k = 0; k < KT; ++k) {
-          w0[16 * k + g] = o[k][0];
-          w1[16 * k + g] = o[k][1];
-          w0[16 * k + g + 8] = o[k][2];
-          w1[16 * k + g + 8] = o[k][3];
+          w0[16 * k + g] = o[k][0] * f0;
+          w1[16 * k + g] = o[k][1] * f1;
+          w0[16 * k + g + 8] = o[k][2] * f0;
+          w1[16 * k + g + 8] = o[k][3] * f1;
         }
       }
       asm volatile("bar.sync 1, %0;" ::"n"(kNW * 32));
-      if (*fail_flag) return;  // the same for all consumer warps
       constexpr int HC = GROUP < 2 ? GROUP : 2;
-      for (int idx = threadIdx.x; idx < HC * D; idx += kNW * 32) {
-        const int hl = idx / D, d = idx % D, h = 2 * hc + hl;
-        float M = -INFINITY;
+      for (int idx = threadIdx.x; idx < HC * D / 2; idx += kNW * 32) {
+        const int hl = idx / (D / 2), d = idx % (D / 2) * 2, h = 2 * hc + hl;
+        float M = jm[h];
 #pragma unroll
-        for (int v = 0; v < kNW; ++v) M = fmaxf(M, jm[v * 8 + h]);
-        float L = 0.f, acc = 0.f;
+        for (int v = 1; v < kNW; ++v) M = fmaxf(M, jm[v * 8 + h]);
+        float L = 0.f;
+        float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
         for (int v = 0; v < kNW; ++v) {
-          const float f = jm[v * 8 + h] == M ? 1.f : exp2f(jm[v * 8 + h] - M);
-          L += jl[v * 8 + h] * f;
-          acc += jo[(v * 2 + hl) * Cfg::OSTRIDE + d] * f;
+          const float m = jm[v * 8 + h];
+          L = fmaf(jl[v * 8 + h], m == M ? 1.f : ex2_approx(m - M), L);
+          const float2 part = *reinterpret_cast<const float2*>(jo + (v * 2 + hl) * Cfg::OSTRIDE + d);
+          acc.x += part.x;
+          acc.y += part.y;
         }
         const int64_t at = (int64_t)x.id * GROUP + h;
-        p.part_o[at * D + d] = L == 0.f ? 0.f : acc / L;  // no key: zeros; a NaN stays one
+        const float inv = L == 0.f ? 0.f : 1.f / L;  // no key: zeros; a NaN stays one
+        *reinterpret_cast<float2*>(p.part_o + at * D + d) = make_float2(acc.x * inv, acc.y * inv);
         if (d == 0) p.part_lse[at] = L == 0.f ? -INFINITY : (M + log2f(L) - kWeightLog2) * 0.6931471805599453f;
       }
       asm volatile("bar.sync 1, %0;" ::"n"(kNW * 32));  // the area is rewritten
@@ -642,9 +670,10 @@ __global__ void __launch_bounds__(256) join_pieces_kernel(const DecodeQ8Params p
   int count = 1;
   if (!p.whole) {
     const int slots = row_of(p, b).slots;
-    const int64_t per = p.first_slot[p.B], from = p.first_slot[b] + (int64_t)hk * slots;
-    first = unit + from / per;
-    count = slots ? (int)((from + slots - 1) / per - from / per) + 1 : 0;
+    const unsigned per = p.first_slot[p.B], from = p.first_slot[b] + hk * slots;
+    const int cta = (int)(from / per);
+    first = unit + cta;
+    count = slots ? (int)((from + slots - 1) / per) - cta + 1 : 0;
   }
   const float* o = p.part_o + (first * group + h % group) * D + lane * PER;
   const float* lse = p.part_lse + first * group + h % group;
@@ -756,7 +785,7 @@ int launch_q8(const CUtensorMap& tmk, const CUtensorMap& tmv, DecodeQ8Params& pr
   int64_t ctas = std::min<int64_t>((int64_t)g_dev[dev].sms * occ,
                                    std::max<int64_t>(1, units * prm.W / kLeastSlots));
   const size_t piece_bytes = (size_t)GROUP * (D + 1) * sizeof(float), slack = 512;
-  const size_t table = ((size_t)prm.B + 1) * sizeof(int64_t);
+  const size_t table = ((size_t)prm.B + 1) * sizeof(int);
   const int64_t room = ws_bytes > table + slack ? (int64_t)((ws_bytes - table - slack) / piece_bytes) : 0;
   int64_t pieces = units + ctas - 1;
   if (room < pieces) {
@@ -768,7 +797,7 @@ int launch_q8(const CUtensorMap& tmk, const CUtensorMap& tmv, DecodeQ8Params& pr
     if (prm.whole) pieces = units;
   }
   const size_t skip = prm.whole ? 0 : (table + 255) & ~size_t(255);
-  prm.first_slot = reinterpret_cast<int64_t*>(ws);
+  prm.first_slot = reinterpret_cast<int*>(ws);
   prm.part_lse = reinterpret_cast<float*>(ws + skip);
   const size_t lse_bytes = ((size_t)pieces * GROUP * sizeof(float) + 255) & ~size_t(255);
   prm.part_o = reinterpret_cast<float*>(ws + skip + lse_bytes);
@@ -797,7 +826,9 @@ int decode_paged_q8(const DecodeQ8Args& a) {
   if (a.batch < 0 || a.max_pages_per_seq < 0 || a.max_pages_per_seq > INT_MAX / kPageTokens)
     return LKV_ERR_INVALID_ARGUMENT;
   if (a.batch == 0) return LKV_OK;
-  if ((int64_t)a.batch * a.num_q_heads > INT_MAX / 2) return LKV_ERR_UNSUPPORTED;
+  // slots are counted in 32 bits
+  if ((int64_t)a.batch * a.num_q_heads > INT_MAX / 2 ||
+      (int64_t)a.batch * a.num_kv_heads * a.max_pages_per_seq > INT_MAX) return LKV_ERR_UNSUPPORTED;
   if (!a.q || !a.codes || !a.scales || !a.block_table || !a.seq_k || !a.out) return LKV_ERR_INVALID_ARGUMENT;
   if (a.q8_pages < 0 || a.q8_pages > INT32_MAX || a.num_pages < 0 || a.num_pages > INT32_MAX)
     return LKV_ERR_INVALID_ARGUMENT;
