@@ -62,7 +62,7 @@ struct DecodeQ8Params {
   int* first_slot;         // [B + 1]: the rows' first slots and the slots per CTA, written for join_pieces_kernel
   int* err;
   int B, Hq, Hkv, W;
-  int whole;  // 1: the workspace holds one piece per (row, head): CTAs take whole ones
+  int whole;  // 1: CTAs take whole (row, head)s and write the result themselves
   float scale_log2;
   int keep_pages;  // leading columns that stay in L2
 };
@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     };
     const float f0 = factor(2 * c, m0), f1 = factor(2 * c + 1, m1);
     // two heads at a time: thread (g, c) holds heads 2c and 2c + 1
-#pragma unroll
+#pragma unroll 1
     for (int hc = 0; hc < (GROUP + 1) / 2; ++hc) {
       if (c == hc) {
         float* w0 = jo + warp * 2 * Cfg::OSTRIDE;
@@ -642,10 +642,19 @@ __global__ void __launch_bounds__(kThreads, 2)
           acc.x += part.x;
           acc.y += part.y;
         }
-        const int64_t at = (int64_t)x.id * GROUP + h;
         const float inv = L == 0.f ? 0.f : 1.f / L;  // no key: zeros; a NaN stays one
-        *reinterpret_cast<float2*>(p.part_o + at * D + d) = make_float2(acc.x * inv, acc.y * inv);
-        if (d == 0) p.part_lse[at] = L == 0.f ? -INFINITY : (M + log2f(L) - kWeightLog2) * 0.6931471805599453f;
+        const float lse = L == 0.f ? -INFINITY : (M + log2f(L) - kWeightLog2) * 0.6931471805599453f;
+        if (p.whole) {  // the result
+          const int hq = x.hk * GROUP + h;
+          const float f = p.out_scale ? p.out_scale[hq] * inv : inv;
+          *reinterpret_cast<uint32_t*>(p.out + (int64_t)x.b * p.out_stride_tok + (int64_t)hq * D + d) =
+              pack_bf16(acc.x * f, acc.y * f);
+          if (p.lse && d == 0) p.lse[(int64_t)x.b * p.Hq + hq] = lse;
+        } else {
+          const int64_t at = (int64_t)x.id * GROUP + h;
+          *reinterpret_cast<float2*>(p.part_o + at * D + d) = make_float2(acc.x * inv, acc.y * inv);
+          if (d == 0) p.part_lse[at] = lse;
+        }
       }
       asm volatile("bar.sync 1, %0;" ::"n"(kNW * 32));  // the area is rewritten
     }
@@ -665,16 +674,10 @@ __global__ void __launch_bounds__(256) join_pieces_kernel(const DecodeQ8Params p
   const int turn = WARPS > 1 ? warp : 0;
   if (row >= (int64_t)p.B * p.Hq) return;
   const int b = (int)(row / p.Hq), h = (int)(row % p.Hq), hk = h / group;
-  const int unit = b * p.Hkv + hk;
-  int64_t first = unit;
-  int count = 1;
-  if (!p.whole) {
-    const int slots = row_of(p, b).slots;
-    const unsigned per = p.first_slot[p.B], from = p.first_slot[b] + hk * slots;
-    const int cta = (int)(from / per);
-    first = unit + cta;
-    count = slots ? (int)((from + slots - 1) / per) - cta + 1 : 0;
-  }
+  const int slots = row_of(p, b).slots;
+  const unsigned per = p.first_slot[p.B], from = p.first_slot[b] + hk * slots;
+  const int cta = (int)(from / per), count = slots ? (int)((from + slots - 1) / per) - cta + 1 : 0;
+  const int64_t first = b * p.Hkv + hk + cta;
   const float* o = p.part_o + (first * group + h % group) * D + lane * PER;
   const float* lse = p.part_lse + first * group + h % group;
   float M = -INFINITY, L = 0.f, acc[PER];
@@ -779,35 +782,37 @@ int launch_q8(const CUtensorMap& tmk, const CUtensorMap& tmv, DecodeQ8Params& pr
     const double page_bytes = (double)prm.Hkv * Q8Cfg<D>::CODE_BYTES;
     prm.keep_pages = (int)std::min<double>(prm.W, kL2KeepFraction * g_dev[dev].l2 / (page_bytes * prm.B));
   }
-  // A CTA for every kLeastSlots slots that the tables have room for, up to two per SM.  A cut makes a piece
-  // more, which the workspace has to hold: first the rows' first slots, then the pieces' lse, then their o.
-  const int64_t units = (int64_t)prm.B * prm.Hkv;
-  int64_t ctas = std::min<int64_t>((int64_t)g_dev[dev].sms * occ,
-                                   std::max<int64_t>(1, units * prm.W / kLeastSlots));
+  // A CTA for every kLeastSlots slots that the tables have room for, up to two per SM.
+  const int64_t units = (int64_t)prm.B * prm.Hkv, full = (int64_t)g_dev[dev].sms * occ;
+  int64_t ctas = std::min<int64_t>(full, std::max<int64_t>(1, units * prm.W / kLeastSlots));
+  // Short rows are not cut: without pieces there is no join launch, which costs what a CTA takes for about 40
+  // slots (4 us).  The host knows the tables' width alone; `slots` is a row's as if a half of a mixed
+  // table's pages were in 8 bits.
+  const int64_t slots = prm.pool_pages ? (3ll * prm.W + 3) / 4 : (prm.W + 1) / 2;
+  const int64_t uncut = (units + full - 1) / full * slots, cut = std::max<int64_t>(kLeastSlots, units * slots / full);
+  prm.whole = slots <= 64 && uncut - cut <= 40;
+  // A cut makes a piece more, which the workspace has to hold: first the rows' first slots, then the pieces' lse,
+  // then their o.
   const size_t piece_bytes = (size_t)GROUP * (D + 1) * sizeof(float), slack = 512;
   const size_t table = ((size_t)prm.B + 1) * sizeof(int);
   const int64_t room = ws_bytes > table + slack ? (int64_t)((ws_bytes - table - slack) / piece_bytes) : 0;
-  int64_t pieces = units + ctas - 1;
-  if (room < pieces) {
+  if (room < units + ctas - 1) {
     // fewer cuts, or (with fewer CTAs than whole (row, head)s would keep busy) none
-    pieces = std::max(room, units);
-    const int64_t cut = pieces - units + 1;
-    prm.whole = cut < std::min(ctas, units);
-    ctas = prm.whole ? std::min(ctas, units) : cut;
-    if (prm.whole) pieces = units;
+    ctas = std::min(ctas, room - units + 1);
+    if (ctas < std::min(full, units)) prm.whole = 1;
   }
-  const size_t skip = prm.whole ? 0 : (table + 255) & ~size_t(255);
+  if (prm.whole) ctas = std::min(full, units);
+  const size_t skip = (table + 255) & ~size_t(255);
+  const size_t lse_bytes = ((size_t)(units + ctas - 1) * GROUP * sizeof(float) + 255) & ~size_t(255);
   prm.first_slot = reinterpret_cast<int*>(ws);
   prm.part_lse = reinterpret_cast<float*>(ws + skip);
-  const size_t lse_bytes = ((size_t)pieces * GROUP * sizeof(float) + 255) & ~size_t(255);
   prm.part_o = reinterpret_cast<float*>(ws + skip + lse_bytes);
-  if (skip + lse_bytes + (size_t)pieces * GROUP * D * sizeof(float) > ws_bytes) return LKV_ERR_WORKSPACE;
-  if (pieces > INT_MAX) return LKV_ERR_UNSUPPORTED;
   if (launch_pdl(decode_q8_kernel<D, GROUP>, dim3((unsigned)ctas), dim3(kThreads), Q8Cfg<D>::SMEM_BYTES, stream, tmk,
                  tmv, prm) != cudaSuccess)
     return LKV_ERR_CUDA;
+  if (prm.whole) return LKV_OK;
   const int64_t rows = (int64_t)prm.B * prm.Hq;
-  const bool few = !prm.whole && rows <= 4 * g_dev[dev].sms;
+  const bool few = rows <= 4 * g_dev[dev].sms;
   const auto join = few ? join_pieces_kernel<D, 8> : join_pieces_kernel<D, 1>;
   return launch_pdl(join, dim3((unsigned)(few ? rows : (rows + 7) / 8)), dim3(256), 0, stream, prm, GROUP) ==
                  cudaSuccess
