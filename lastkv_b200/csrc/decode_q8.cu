@@ -20,8 +20,8 @@
 //
 // Bound by HBM: an 8-bit page is half a bf16 page's bytes.  Work is counted in slots of equal bytes, one bf16
 // page or two 8-bit pages of one KV head.  The rows' slots lie end to end, (row, head) after
-// (row, head), and every CTA takes the same number of them, so ragged rows cost no balance; a
-// (row, head)'s part within a CTA is a piece, whose normalised partial goes to the workspace, and
+// (row, head), each behind the places of what a (row, head) costs by itself, and every CTA takes the same number
+// of places, so ragged rows cost no balance; a (row, head)'s part within a CTA is a piece, whose normalised partial goes to the workspace, and
 // join_pieces_kernel joins each row's pieces.  Per CTA one warp fills a ring of slots (an 8-bit page's codes and
 // scales by two bulk copies, a bf16 page's halves by TMA), 6 warps take the slots in turn.
 
@@ -59,7 +59,7 @@ struct DecodeQ8Params {
   const float* out_scale;  // [Hq] or null
   float* part_o;           // [pieces][GROUP][D], normalised
   float* part_lse;         // [pieces][GROUP], natural log
-  int* first_slot;         // [B + 1]: the rows' first slots and the slots per CTA, written for join_pieces_kernel
+  int* first_place;        // [B + 1]: the rows' first places and the places per CTA, written for join_pieces_kernel
   int* err;
   int B, Hq, Hkv, W;
   int whole;  // 1: CTAs take whole (row, head)s and write the result themselves
@@ -154,8 +154,15 @@ __device__ __forceinline__ Row row_of(const DecodeQ8Params& p, int b) {
   return r;
 }
 
-// What a CTA takes: pieces from slot `at` of (row b, head hk) on, `left` slots in all (whole: `left` (row, head)s).
+// What a (row, head) costs besides its slots, in slots: its Q, the join of the warps, the partial.
+constexpr int kPieceCost = 6;
+
+// A (row, head)'s places in the order that CTAs share: kPieceCost of its own, then one per slot.
+__device__ __forceinline__ int places(const Row& r) { return r.slots ? r.slots + kPieceCost : 0; }
+
+// What a CTA takes: `left` places from place `at` of (row b, head hk) on (whole: `left` (row, head)s).
 struct Share {
+  Row r;  // of row b
   int b, hk, at, piece, left;
 };
 
@@ -167,31 +174,35 @@ struct Piece {
 
 // The next piece of a share; false where it ends.  Every warp walks its copy of the share.
 __device__ __forceinline__ bool next_piece(const DecodeQ8Params& p, Share& s, Piece& x) {
-  if (s.left <= 0 || s.b >= p.B) return false;
-  x.r = row_of(p, s.b);
-  if (!p.whole)
-    while (x.r.slots == 0) {  // rows without keys have no pieces, but their places among them
-      s.piece += p.Hkv;
-      if (++s.b >= p.B) return false;
-      x.r = row_of(p, s.b);
-    }
-  x.b = s.b;
-  x.hk = s.hk;
-  x.id = s.piece;
-  x.s0 = s.at;
-  x.s1 = p.whole ? x.r.slots : min(x.r.slots, s.at + s.left);
-  s.left -= p.whole ? 1 : x.s1 - x.s0;
-  s.at = 0;
-  ++s.piece;
-  if (++s.hk == p.Hkv) {
+  if (s.left <= 0) return false;
+  if (s.hk == p.Hkv) {
     s.hk = 0;
-    ++s.b;
+    do {
+      if (++s.b >= p.B) return false;
+      s.r = row_of(p, s.b);
+      if (s.r.slots == 0 && !p.whole) s.piece += p.Hkv;  // no pieces, but their places among them
+    } while (s.r.slots == 0 && !p.whole);
   }
-  return true;
+  x.r = s.r;
+  x.b = s.b;
+  x.hk = s.hk++;
+  x.id = s.piece++;
+  if (p.whole) {
+    x.s0 = 0;
+    x.s1 = s.r.slots;
+    --s.left;
+    return true;
+  }
+  const int take = min(s.left, s.r.slots + kPieceCost - s.at);
+  x.s0 = max(0, s.at - kPieceCost);
+  x.s1 = s.at + take - kPieceCost;
+  s.left -= take;
+  s.at = 0;
+  return x.s1 > x.s0;  // a share that ends before a (row, head)'s first slot ends there
 }
 
-// The CTA's share, called by all threads.  Piece u of the (row, head)s in order, cut at CTA c's first slot, is
-// piece u + c.  (All slots together are below 2^31: the host checks the tables' size.)
+// The CTA's share, called by all threads.  Piece u of the (row, head)s in order, cut at CTA c's first place, is
+// piece u + c.  (All places together are below 2^31: the host checks the tables' size.)
 __device__ Share share_of(const DecodeQ8Params& p, int* sm, int* sm_row) {
   Share s{};
   const unsigned cta = blockIdx.x, ctas = gridDim.x;
@@ -202,6 +213,7 @@ __device__ Share share_of(const DecodeQ8Params& p, int* sm, int* sm_row) {
     s.hk = (int)(u0 % p.Hkv);
     s.piece = (int)u0;
     s.left = (int)(u1 - u0);
+    s.r = row_of(p, s.b);
     return s;
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -213,26 +225,34 @@ __device__ Share share_of(const DecodeQ8Params& p, int* sm, int* sm_row) {
     }
     return v;
   };
-  auto share = [ctas](int all) { return max((int)(((unsigned)all + ctas - 1) / ctas), kLeastSlots); };
-  int total, per, start;   // start: the first slot of the row that holds the CTA's first
+  auto share = [ctas](int all) {
+    return max((int)(((unsigned)all + ctas - 1) / ctas), kLeastSlots + kPieceCost);
+  };
+  int total, per, start;  // start: the first place of the row that holds the CTA's first
   int64_t first;
   if (p.B <= 32) {  // every warp for itself
-    const int here = lane < p.B ? row_of(p, lane).slots * p.Hkv : 0;
-    const int upto = prefix(here);
+    Row r{};
+    if (lane < p.B) r = row_of(p, lane);
+    const int here = places(r) * p.Hkv, upto = prefix(here);
     total = __shfl_sync(0xffffffffu, upto, 31);
     per = share(total);
     first = (int64_t)per * cta;
     if (cta == 0 && warp == 0) {
-      if (lane < p.B) p.first_slot[lane] = upto - here;
-      if (lane == 0) p.first_slot[p.B] = per;
+      if (lane < p.B) p.first_place[lane] = upto - here;
+      if (lane == 0) p.first_place[p.B] = per;
     }
     if (first >= total) return s;
     s.b = __ffs(__ballot_sync(0xffffffffu, upto > first)) - 1;
     start = __shfl_sync(0xffffffffu, upto - here, s.b);
+    s.r.n = __shfl_sync(0xffffffffu, r.n, s.b);
+    s.r.npages = __shfl_sync(0xffffffffu, r.npages, s.b);
+    s.r.nh = __shfl_sync(0xffffffffu, r.nh, s.b);
+    s.r.hs = (s.r.nh + 1) / 2;
+    s.r.slots = s.r.hs + s.r.npages - s.r.nh;
   } else {
     constexpr int WARPS = kThreads / 32;
     int mine = 0;
-    for (int b = threadIdx.x; b < p.B; b += kThreads) mine += row_of(p, b).slots;
+    for (int b = threadIdx.x; b < p.B; b += kThreads) mine += places(row_of(p, b));
     mine = __reduce_add_sync(0xffffffffu, mine);
     if (lane == 0) sm[warp] = mine;
     __syncthreads();
@@ -246,7 +266,7 @@ __device__ Share share_of(const DecodeQ8Params& p, int* sm, int* sm_row) {
     int before = 0;
     for (int b0 = 0; b0 < p.B; b0 += kThreads) {
       const int b = b0 + threadIdx.x;
-      const int here = b < p.B ? row_of(p, b).slots * p.Hkv : 0;
+      const int here = b < p.B ? places(row_of(p, b)) * p.Hkv : 0;
       const int upto = prefix(here);
       __syncthreads();  // sm is read
       if (lane == 31) sm[warp] = upto;
@@ -257,8 +277,8 @@ __device__ Share share_of(const DecodeQ8Params& p, int* sm, int* sm_row) {
         before += sm[w];
       }
       if (cta == 0 && b < p.B) {
-        p.first_slot[b] = at;
-        if (b == p.B - 1) p.first_slot[p.B] = per;
+        p.first_place[b] = at;
+        if (b == p.B - 1) p.first_place[p.B] = per;
       }
       if (here > 0 && at <= first && first < at + here) {
         *sm_row = b;
@@ -270,10 +290,11 @@ __device__ Share share_of(const DecodeQ8Params& p, int* sm, int* sm_row) {
     if (first >= total) return s;
     s.b = *sm_row;
     start = sm[WARPS];
+    s.r = row_of(p, s.b);
   }
-  const unsigned slots = row_of(p, s.b).slots, off = (unsigned)((int)first - start);
-  s.hk = (int)(off / slots);
-  s.at = (int)(off % slots);
+  const unsigned unit = s.r.slots + kPieceCost, off = (unsigned)((int)first - start);
+  s.hk = (int)(off / unit);
+  s.at = (int)(off % unit);
   s.piece = s.b * p.Hkv + s.hk + (int)cta;
   s.left = min(per, total - (int)first);
   return s;
@@ -412,9 +433,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       const __nv_bfloat16* qrow = p.q + (int64_t)x.b * p.q_stride_tok + (int64_t)(x.hk * GROUP + (valid ? g : 0)) * D;
       float top = 0.f;
 #pragma unroll
-      for (int j = 0; j < KT; ++j) {
+      for (int j = 0; j < KT; ++j) {  // all loads before the first store, which they could not pass
         qf[j][0] = valid ? *reinterpret_cast<const uint32_t*>(qrow + 16 * j + 2 * c) : 0u;
         qf[j][1] = valid ? *reinterpret_cast<const uint32_t*>(qrow + 16 * j + 2 * c + 8) : 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < KT; ++j) {
         if (warp == j % kNW) sq[j * 32] = make_uint2(qf[j][0], qf[j][1]);
 #pragma unroll
         for (int t = 0; t < 2; ++t) top = fmaxf(top, fmaxf(fabsf(bf16_lo(qf[j][t])), fabsf(bf16_hi(qf[j][t]))));
@@ -675,7 +699,8 @@ __global__ void __launch_bounds__(256) join_pieces_kernel(const DecodeQ8Params p
   if (row >= (int64_t)p.B * p.Hq) return;
   const int b = (int)(row / p.Hq), h = (int)(row % p.Hq), hk = h / group;
   const int slots = row_of(p, b).slots;
-  const unsigned per = p.first_slot[p.B], from = p.first_slot[b] + hk * slots;
+  const unsigned per = p.first_place[p.B];
+  const unsigned from = p.first_place[b] + hk * (slots + kPieceCost) + kPieceCost;  // the first slot's place
   const int cta = (int)(from / per), count = slots ? (int)((from + slots - 1) / per) - cta + 1 : 0;
   const int64_t first = b * p.Hkv + hk + cta;
   const float* o = p.part_o + (first * group + h % group) * D + lane * PER;
@@ -791,7 +816,7 @@ int launch_q8(const CUtensorMap& tmk, const CUtensorMap& tmv, DecodeQ8Params& pr
   const int64_t slots = prm.pool_pages ? (3ll * prm.W + 3) / 4 : (prm.W + 1) / 2;
   const int64_t uncut = (units + full - 1) / full * slots, cut = std::max<int64_t>(kLeastSlots, units * slots / full);
   prm.whole = slots <= 64 && uncut - cut <= 40;
-  // A cut makes a piece more, which the workspace has to hold: first the rows' first slots, then the pieces' lse,
+  // A cut makes a piece more, which the workspace has to hold: first the rows' first places, then the pieces' lse,
   // then their o.
   const size_t piece_bytes = (size_t)GROUP * (D + 1) * sizeof(float), slack = 512;
   const size_t table = ((size_t)prm.B + 1) * sizeof(int);
@@ -804,7 +829,7 @@ int launch_q8(const CUtensorMap& tmk, const CUtensorMap& tmv, DecodeQ8Params& pr
   if (prm.whole) ctas = std::min(full, units);
   const size_t skip = (table + 255) & ~size_t(255);
   const size_t lse_bytes = ((size_t)(units + ctas - 1) * GROUP * sizeof(float) + 255) & ~size_t(255);
-  prm.first_slot = reinterpret_cast<int*>(ws);
+  prm.first_place = reinterpret_cast<int*>(ws);
   prm.part_lse = reinterpret_cast<float*>(ws + skip);
   prm.part_o = reinterpret_cast<float*>(ws + skip + lse_bytes);
   if (launch_pdl(decode_q8_kernel<D, GROUP>, dim3((unsigned)ctas), dim3(kThreads), Q8Cfg<D>::SMEM_BYTES, stream, tmk,
@@ -833,7 +858,7 @@ int decode_paged_q8(const DecodeQ8Args& a) {
   if (a.batch == 0) return LKV_OK;
   // slots are counted in 32 bits
   if ((int64_t)a.batch * a.num_q_heads > INT_MAX / 2 ||
-      (int64_t)a.batch * a.num_kv_heads * a.max_pages_per_seq > INT_MAX) return LKV_ERR_UNSUPPORTED;
+      (int64_t)a.batch * a.num_kv_heads * (a.max_pages_per_seq + kPieceCost) > INT_MAX) return LKV_ERR_UNSUPPORTED;
   if (!a.q || !a.codes || !a.scales || !a.block_table || !a.seq_k || !a.out) return LKV_ERR_INVALID_ARGUMENT;
   if (a.q8_pages < 0 || a.q8_pages > INT32_MAX || a.num_pages < 0 || a.num_pages > INT32_MAX)
     return LKV_ERR_INVALID_ARGUMENT;
