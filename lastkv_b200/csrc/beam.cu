@@ -7,16 +7,18 @@
 // Within a beam they are ordered as its logits are, so one pass over the logits in their own type
 // finds each row's `select` largest together with its maximum and sum of exponentials (fp32):
 //
-//   beam_rows    A CTA takes a stretch of a row in tiles of 8192 values, 32 in each thread's
-//                registers.  It keeps the stretch's best `select` as sorted 64-bit keys (the value as
+//   beam_rows    A CTA takes a stretch of a row in tiles of 4096 or 8192 values, 16 or 32 in
+//                each thread's registers.  It keeps the stretch's best `select` as sorted 64-bit keys (the value as
 //                an ordered integer, then the complement of the index, so that no two are equal) and
-//                collects what beats the last of them.  A tile with too many such values (the first
-//                one) first raises the bar to a key that at least `select` of its values reach: the
-//                select-th largest of a warp's 32 lane maxima, in the warp where that is largest, or
-//                the (select / 8)-th, in the warp where it is least.  If still too many pass, the
-//                tile's best are taken out one by one.
-//   beam_merge   A CTA per batch item joins each row's stretches, then the rows: lists are sorted, so a
-//                candidate's rank is a sum of binary searches.
+//                collects the values above the last of them: later tiles mostly hold none, so that a
+//                comparison per value is what selection costs.  A tile with too many (the first one)
+//                first finds a bar that at least `select` of its values reach: the select-th largest of a
+//                warp's 32 lane maxima, in the warp where that is largest, or the (select / 8)-th, in the
+//                warp where it is least.  Of values equal to the bar, where they are too many (a masked
+//                vocabulary), the first ones are taken; if still too many lie above it, the tile's best are
+//                taken out one by one.
+//   beam_merge   A CTA per batch item joins each row's stretches two by two, then the rows: lists are
+//                sorted, so a candidate's rank is its place in its own list and a binary search in the other.
 //
 // Bound by HBM for many rows and by two launches for few.
 
@@ -33,8 +35,9 @@ namespace lkv {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kPer = 32;                 // values per thread and tile
-constexpr int kTile = kThreads * kPer;   // 8192
+// Values per thread and tile: 32 (tiles of 8192), or 16 where that leaves SMs without a tile.  4 rows of 128256:
+// 12.2 us with 32, 10.4 with 16.
+constexpr int kPerMany = 32, kPerFew = 16;
 constexpr int kMaxSelect = 32;
 constexpr int kMaxBeams = 64;
 constexpr int kCandidates = 1024;        // a tile's values over the bar
@@ -57,6 +60,19 @@ __device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
   return k;
 }
 
+// The lanes' values sorted from the largest: lane r has the r-th (bitonic).
+__device__ __forceinline__ uint32_t warp_sort(uint32_t v, int lane) {
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, v, j);
+      const bool larger = ((lane & k) == 0) == ((lane & j) == 0);  // the place that keeps the larger one
+      v = larger ? max(v, other) : min(v, other);
+    }
+  return v;
+}
+
 struct RowsParams {
   const void* logits;
   int64_t row_stride;
@@ -68,54 +84,81 @@ struct RowsParams {
   float2* sums;    // [rows][stretches]: maximum, sum of exp(x - maximum)
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) beam_rows_kernel(const RowsParams p) {
+template <typename T, int kPer>
+__global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(const RowsParams p) {
+  constexpr int kTile = kThreads * kPer;
   constexpr int VE = 16 / sizeof(T);  // values per 16-byte load
   __shared__ uint64_t cand[kCandidates + kMaxSelect];
   __shared__ uint64_t best[2][kMaxSelect];
-  __shared__ uint64_t warp_key[kWarps], warp_eighth[kWarps];
+  __shared__ uint64_t warp_key[kWarps];
+  __shared__ float warp_bar[kWarps], warp_eighth[kWarps];
   __shared__ float2 warp_sum[kWarps];
-  __shared__ int count;
+  __shared__ int counts[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents();
   pdl_wait();
   const int64_t row = blockIdx.y;
   const int n = p.select;
+  const int64_t out = row * p.stretches + blockIdx.x;
+  if (p.finished && p.finished[row]) {
+    // one candidate of total 0 + score; behind it the first tokens, at -inf
+    if (tid < n) {
+      const uint32_t eos = (uint32_t)p.eos, low = ordered(-INFINITY);
+      const uint32_t i = tid == 0 ? eos : (uint32_t)(tid - 1) + ((uint32_t)(tid - 1) >= eos ? 1u : 0u);
+      p.keys[out * n + tid] =
+          blockIdx.x == 0 ? (uint64_t)(tid == 0 ? ordered(0.f) : low) << 32 | (0xffffffffu - i) : 0;
+    }
+    if (tid == 0) p.sums[out] = make_float2(0.f, 1.f);
+    return;
+  }
   const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
   // tiles start at 16-byte boundaries, so a row's first may begin before it
   const int lead = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  const bool done = p.finished && p.finished[row];
   const int64_t first = (int64_t)blockIdx.x * p.tiles_per;
   int cur = 0;
   if (tid < n) best[0][tid] = 0;
+  if (tid < 2) counts[tid] = 0;
+  __syncthreads();
   float m = -INFINITY, sum = 0.f;
   for (int64_t t = first; t < first + p.tiles_per; ++t) {
     const int64_t base = t * kTile - lead;
     if (base >= p.V) break;
     float v[kPer];
     // the index of v[e]: base + (e / VE * kThreads + tid) * VE + e % VE
-    auto index = [&](int e) { return base + (int64_t)(e / VE * kThreads + tid) * VE + e % VE; };
-    auto inside = [&](int64_t i) { return i >= 0 && i < p.V; };
+    auto place = [&](int e) { return (e / VE * kThreads + tid) * VE + e % VE; };
+    const bool whole = base >= 0 && base + kTile <= p.V;
+    if (whole) {
+      const uint4* at = reinterpret_cast<const uint4*>(x + base) + tid;
+      uint4 w[kPer / VE];
 #pragma unroll
-    for (int i = 0; i < kPer / VE; ++i) {
-      const int64_t at = index(i * VE);
-      if (done) {
+      for (int i = 0; i < kPer / VE; ++i) w[i] = __ldcs(at + i * kThreads);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) v[i * VE + e] = at + e == p.eos ? 0.f : -INFINITY;
-      } else if (at >= 0 && at + VE <= p.V) {
-        const uint4 w = __ldcs(reinterpret_cast<const uint4*>(x + at));
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+      for (int i = 0; i < kPer / VE; ++i) {
+        const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
           if constexpr (sizeof(T) == 2) v[i * VE + e] = e & 1 ? bf16_hi(u[e / 2]) : bf16_lo(u[e / 2]);
           else v[i * VE + e] = __uint_as_float(u[e]);
         }
-      } else {
+      }
+    } else {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) v[i * VE + e] = inside(at + e) ? (float)x[at + e] : -INFINITY;
+      for (int i = 0; i < kPer / VE; ++i) {
+        const int64_t at = base + place(i * VE);
+        if (at >= 0 && at + VE <= p.V) {
+          const uint4 w = __ldcs(reinterpret_cast<const uint4*>(x + at));
+          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            if constexpr (sizeof(T) == 2) v[i * VE + e] = e & 1 ? bf16_hi(u[e / 2]) : bf16_lo(u[e / 2]);
+            else v[i * VE + e] = __uint_as_float(u[e]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < VE; ++e) v[i * VE + e] = at + e >= 0 && at + e < p.V ? (float)x[at + e] : -INFINITY;
+        }
       }
     }
-    const bool whole = base >= 0 && base + kTile <= p.V;
     // the thread's maximum and sum, over all its tiles; a NaN stays in the sum
     float top = v[0];
 #pragma unroll
@@ -123,132 +166,175 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(const RowsParams p)
     const float nm = fmaxf(m, top);
     if (nm != -INFINITY) {
       if (nm != m) sum *= exp2f((m - nm) * kLog2e);
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) sum += ex2_approx((v[e] - nm) * kLog2e);
+      for (int e = 0; e < kPer; ++e) part[e & 3] += ex2_approx((v[e] - nm) * kLog2e);
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
       m = nm;
     } else {
 #pragma unroll
       for (int e = 0; e < kPer; ++e) sum = v[e] == v[e] ? sum : NAN;
     }
-    auto key = [&](int e) -> uint64_t {
-      const int64_t i = index(e);
-      return whole || inside(i) ? (uint64_t)ordered(v[e]) << 32 | (0xffffffffu - (uint32_t)i) : 0;
+    auto key = [&](int e) -> uint64_t {  // 0 outside the row (below its start the index wraps around)
+      const uint32_t i = (uint32_t)base + (uint32_t)place(e);
+      return i < (uint32_t)p.V ? (uint64_t)ordered(v[e]) << 32 | ~i : 0;
     };
-    __syncthreads();  // best[cur] is written; count and cand are free
-    uint64_t bar = best[cur][n - 1] + 1;  // the least key that is worth collecting
-    if (tid == 0) count = 0;
-    // a first look, at the values' high words alone: most tiles after a stretch's first hold nothing
-    const bool any = ordered(top) >= (uint32_t)(bar >> 32);
-    if (!__syncthreads_or(any)) continue;
-    int mine = 0;
-    if (any) {
+    // Values above the list's last: an equal one, of a later index, comes behind it.  (A NaN, which counts as
+    // -inf, is not below anything; its key tells.)
+    const uint64_t last = best[cur][n - 1];
+    const bool empty = last == 0;
+    const float list_bar = empty ? -INFINITY : from_ordered((uint32_t)(last >> 32));
+    const bool some = empty || top > list_bar;
+    if (!__syncthreads_or(some)) continue;
+    float bar = list_bar;
+    bool equal = false;  // whether values equal to the bar count
+    // A bar that at least n of the tile's values reach.
+    auto tile_bar = [&] {
+      const uint32_t sorted = warp_sort(ordered(top), lane);
+      if (lane == n - 1) warp_bar[warp] = from_ordered(sorted);
+      if (lane == (n + kWarps - 1) / kWarps - 1) warp_eighth[warp] = from_ordered(sorted);
+      __syncthreads();
+      float least = warp_eighth[0], most = warp_bar[0];
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) mine += key(e) >= bar;
+      for (int w = 1; w < kWarps; ++w) {
+        most = fmaxf(most, warp_bar[w]);
+        least = fminf(least, warp_eighth[w]);
+      }
+      return fmaxf(most, least);
+    };
+    // Collects the values above (or equal to) the bar behind the entries that are there.  (The order does not
+    // matter: keys are ranked below.)
+    auto collect = [&] {
+      uint32_t mask = 0;
+      if (!(top < bar)) {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) mask |= (uint32_t)(equal ? !(v[e] < bar) : v[e] > bar) << e;
+      }
+      if (mask) {
+        int at = atomicAdd(&counts[0], __popc(mask));
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+          if (mask >> e & 1) {
+            if (at < kCandidates) cand[at] = key(e);
+            ++at;
+          }
+      }
+      __syncthreads();
+      return counts[0];
+    };
+    if (empty) {
+      bar = tile_bar();
+      equal = true;
     }
-    if (mine) atomicAdd(&count, mine);
-    __syncthreads();
-    int total = count;
+    int total = collect();
     if (total > kCandidates) {
-      uint64_t big = 0;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) big = max_key(big, key(e));
-      int rank = 0;
-      for (int l = 0; l < 32; ++l) {
-        const uint64_t other = __shfl_sync(0xffffffffu, big, l);
-        rank += other > big || (other == big && l < lane);
+      // too many: count what lies above a bar of the tile's own, and on it
+      if (!empty) {
+        const float own = tile_bar();
+        if (own > list_bar) bar = own, equal = true;
       }
-      if (rank == n - 1) warp_key[warp] = big;
-      if (rank == (n + kWarps - 1) / kWarps - 1) warp_eighth[warp] = big;
+      __syncthreads();  // counts are read
+      if (tid < 2) counts[tid] = 0;
       __syncthreads();
-      uint64_t least = warp_eighth[0];
-      for (int w = 0; w < kWarps; ++w) {
-        bar = max_key(bar, warp_key[w]);
-        least = min(least, warp_eighth[w]);
-      }
-      bar = max_key(bar, least);
-      if (tid == 0) count = 0;
-      __syncthreads();
-      mine = 0;
-      if (big >= bar) {
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) mine += key(e) >= bar;
-      }
-      if (mine) atomicAdd(&count, mine);
-      __syncthreads();
-      total = count;
-    }
-    __syncthreads();  // count is read
-    if (total <= kCandidates) {
-      if (tid == 0) count = 0;
-      __syncthreads();
-      if (mine) {
-        int at = atomicAdd(&count, mine);  // the order of the list does not matter: keys are ranked below
+      int above = 0, level = 0;
+      if (!(top < bar)) {
 #pragma unroll
         for (int e = 0; e < kPer; ++e) {
-          const uint64_t k = key(e);
-          if (k >= bar) cand[at++] = k;
+          above += v[e] > bar;
+          level += equal && !(v[e] < bar) && !(v[e] > bar);
         }
       }
-    } else {
-      // the tile's best, one after another
-      uint64_t last = ~0ull;
-      for (int r = 0; r < n; ++r) {
-        uint64_t big = 0;
+      above = __reduce_add_sync(0xffffffffu, above);
+      level = __reduce_add_sync(0xffffffffu, level);
+      if (lane == 0 && above) atomicAdd(&counts[0], above);
+      if (lane == 0 && level) atomicAdd(&counts[1], level);
+      __syncthreads();
+      above = counts[0];
+      level = counts[1];
+      __syncthreads();
+      if (tid < 2) counts[tid] = 0;
+      if (above > kCandidates - kMaxSelect) {
+        // the tile's best, one after another
+        uint64_t before = ~0ull;
+        for (int r = 0; r < n; ++r) {
+          uint64_t big = 0;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          const uint64_t k = key(e);
-          if (k < last) big = max_key(big, k);
+          for (int e = 0; e < kPer; ++e) {
+            const uint64_t k = key(e);
+            if (k < before) big = max_key(big, k);
+          }
+          big = warp_max_key(big);
+          if (lane == 0) warp_key[warp] = big;
+          __syncthreads();
+          big = warp_key[0];
+          for (int w = 1; w < kWarps; ++w) big = max_key(big, warp_key[w]);
+          if (tid == 0) cand[r] = big;
+          before = big;
+          __syncthreads();
         }
-        big = warp_max_key(big);
-        if (lane == 0) warp_key[warp] = big;
+        total = n;
+      } else {
+        if (above + level > kCandidates) {
+          // the first of the values equal to the bar (a NaN counts as -inf)
+          equal = false;
+          int64_t after = -1;
+          for (int r = 0; r < n; ++r) {
+            uint32_t next = 0xffffffffu;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+              const int64_t i = base + place(e);
+              const float y = v[e] == v[e] ? v[e] : -INFINITY;
+              if (y == bar && i > after && i < p.V) next = min(next, (uint32_t)i);
+            }
+            next = __reduce_min_sync(0xffffffffu, next);
+            if (lane == 0) warp_key[warp] = next;
+            __syncthreads();
+            for (int w = 0; w < kWarps; ++w) next = min(next, (uint32_t)warp_key[w]);
+            if (tid == 0) cand[r] = next == 0xffffffffu ? 0 : (uint64_t)ordered(bar) << 32 | (0xffffffffu - next);
+            after = next;
+            __syncthreads();
+          }
+          if (tid == 0) counts[0] = n;
+        }
         __syncthreads();
-        big = warp_key[0];
-        for (int w = 1; w < kWarps; ++w) big = max_key(big, warp_key[w]);
-        if (tid == 0) cand[r] = big;
-        last = big;
-        __syncthreads();
+        total = min(collect(), kCandidates);
       }
-      total = n;
     }
+    // the new list: every entry of the old one and of the collected ones finds its rank among all
     if (tid < n) {
+      cand[total + tid] = best[cur][tid];
       best[cur ^ 1][tid] = 0;
     }
     __syncthreads();
-    // the new best: every entry of the old list and of the collected ones finds its rank among all
-    if (tid < n) cand[total + tid] = best[cur][tid];
-    __syncthreads();
+    if (tid < 2) counts[tid] = 0;
     const int all = total + n;
     for (int a = tid; a < all; a += kThreads) {
       const uint64_t k = cand[a];
       if (k == 0) continue;
       int rank = 0;
+#pragma unroll 4
       for (int b = 0; b < all; ++b) rank += cand[b] > k;
       if (rank < n) best[cur ^ 1][rank] = k;
     }
+    __syncthreads();
     cur ^= 1;
   }
-  // the stretch's maximum and sum: warps, then the CTA, in a fixed order
-  auto join = [](float2 a, float2 b) {
-    const float t = fmaxf(a.x, b.x);
-    if (t == -INFINITY) return make_float2(t, a.y + b.y);
-    return make_float2(t, (a.x == t ? a.y : a.y * exp2f((a.x - t) * kLog2e)) +
-                              (b.x == t ? b.y : b.y * exp2f((b.x - t) * kLog2e)));
+  // the stretch's maximum and sum: the warps', then the CTA's, in a fixed order
+  auto join = [lane](float2 ms, int lanes) {
+    float t = ms.x;
+    for (int o = lanes / 2; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+    float y = ms.x == t ? ms.y : ms.y * ex2_approx((ms.x - t) * kLog2e);  // (t = -inf: y is 0, or a NaN)
+    for (int o = lanes / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+    return make_float2(t, y);
   };
-  float2 ms = make_float2(m, sum);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float2 other = make_float2(__shfl_xor_sync(0xffffffffu, ms.x, o), __shfl_xor_sync(0xffffffffu, ms.y, o));
-    ms = lane & o ? join(other, ms) : join(ms, other);  // the same operands in both lanes' order
-  }
-  if (lane == 0) warp_sum[warp] = ms;
+  const float2 mine = join(make_float2(m, sum), 32);
+  if (lane == 0) warp_sum[warp] = mine;
   __syncthreads();
-  const int64_t at = row * p.stretches + blockIdx.x;
-  if (tid == 0) {
-    ms = warp_sum[0];
-    for (int w = 1; w < kWarps; ++w) ms = join(ms, warp_sum[w]);
-    p.sums[at] = ms;
+  if (warp == 0) {
+    const float2 all = join(warp_sum[lane % kWarps], kWarps);
+    if (lane == 0) p.sums[out] = all;
   }
-  if (tid < n) p.keys[at * n + tid] = best[cur][tid];
+  if (tid < n) p.keys[out * n + tid] = best[cur][tid];
 }
 
 struct MergeParams {
@@ -258,28 +344,27 @@ struct MergeParams {
   const uint8_t* finished;
   int64_t V, eos;
   int K, select, stretches;
-  int rows_per_pass;  // rows whose keys fit in shared memory at once
+  int log_n, log_lists;  // select and stretches, rounded up to powers of two
+  int rows_per_pass;     // rows whose keys fit in shared memory at once
   float* out_scores;
   int64_t* out_rows;
   int64_t* out_tokens;
   uint8_t* out_finished;
 };
 
-// How many of the n keys, sorted from the largest, are larger than k.
+// How many of the n keys (a power of two), sorted from the largest, are larger than k.
 __device__ __forceinline__ int larger(const uint64_t* list, int n, uint64_t k) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (list[mid] > k) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
+  int at = 0;
+  for (int step = n >> 1; step > 0; step >>= 1)
+    if (list[at + step - 1] > k) at += step;
+  return at + (list[at] > k);
 }
 
 constexpr int kMergeThreads = 512;
 
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const MergeParams p) {
-  extern __shared__ uint64_t keys[];  // [rows_per_pass][stretches][select]
+  // [rows_per_pass][1 << log_lists][1 << log_n], padded with zeros, then as much again for half as many lists
+  extern __shared__ uint64_t keys[];
   // A total is (x - top) + norm: the maximum is taken off first, so that rows of values like a type's
   // lowest keep their sums' logarithms and their scores.  norm NaN: every total of the row is -inf.
   __shared__ double tops[kMaxBeams], norm[kMaxBeams];
@@ -288,36 +373,60 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const MergePa
   const int b = blockIdx.x, n = p.select, K = p.K, S = p.stretches, tid = threadIdx.x;
   pdl_launch_dependents();
   pdl_wait();
-  for (int k = tid; k < K; k += kMergeThreads) {
-    const int64_t row = (int64_t)b * K + k;
-    float top = -INFINITY;
-    double sum = 0;
-    for (int s = 0; s < S; ++s) top = fmaxf(top, p.sums[row * S + s].x);
-    for (int s = 0; s < S; ++s) {
-      const float2 ms = p.sums[row * S + s];
-      if (ms.x == -INFINITY) sum += ms.y;  // 0, or a NaN
-      else sum += (double)ms.y * (ms.x == top ? 1.0 : (double)expf(ms.x - top));
+  auto row_norms = [&] {
+    for (int k = tid >> 5; k < K; k += kMergeThreads / 32) {  // a warp per row, two stretches per lane
+      const int64_t row = (int64_t)b * K + k;
+      const int lane = tid & 31;
+      const float2 none = make_float2(-INFINITY, 0.f);
+      const float2 a = lane < S ? p.sums[row * S + lane] : none, c = lane + 32 < S ? p.sums[row * S + lane + 32] : none;
+      float top = fmaxf(a.x, c.x);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      // a stretch of -inf alone adds 0, or a NaN
+      auto part = [top](float2 ms) {
+        return ms.x == -INFINITY || ms.x == top ? (double)ms.y : (double)ms.y * (double)expf(ms.x - top);
+      };
+      double sum = part(a) + part(c);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) {
+        const bool done = p.finished && p.finished[row];
+        const double score = (double)p.scores[row], rest = done ? 0.0 : log(sum);
+        tops[k] = done ? 0.0 : (double)top;
+        norm[k] = fabs(score) < INFINITY && fabs(tops[k]) < INFINITY && fabs(rest) < INFINITY ? score - rest : NAN;
+      }
     }
-    const bool done = p.finished && p.finished[row];
-    const double c = (double)p.scores[row], rest = done ? 0.0 : log(sum);
-    tops[k] = done ? 0.0 : (double)top;
-    norm[k] = fabs(c) < INFINITY && fabs(tops[k]) < INFINITY && fabs(rest) < INFINITY ? c - rest : NAN;
-  }
+  };
   for (int k0 = 0; k0 < K; k0 += p.rows_per_pass) {
-    const int rows = min(p.rows_per_pass, K - k0), per = S * n;
-    const uint64_t* in = p.keys + ((int64_t)b * K + k0) * per;
+    const int rows = min(p.rows_per_pass, K - k0);
+    const uint64_t* in = p.keys + ((int64_t)b * K + k0) * S * n;
+    const int log_n = p.log_n, pad = 1 << log_n;
+    uint64_t* from = keys;
+    uint64_t* to = keys + ((int64_t)p.rows_per_pass << (p.log_lists + log_n));
     __syncthreads();
-    for (int i = tid; i < rows * per; i += kMergeThreads) keys[i] = in[i];
+    for (int i = tid; i < rows << (p.log_lists + log_n); i += kMergeThreads) {
+      const int at = i & (pad - 1), list = i >> log_n, s = list & ((1 << p.log_lists) - 1), r = list >> p.log_lists;
+      from[i] = at < n && s < S ? in[(r * S + s) * n + at] : 0;
+    }
+    if (k0 == 0) row_norms();
     __syncthreads();
-    for (int i = tid; i < rows * per; i += kMergeThreads) {
-      const uint64_t k = keys[i];
-      if (k == 0) continue;
-      const int r = i / per, s = i % per / n;
-      int rank = i % n;
-      const uint64_t* row = keys + r * per;
-      for (int o = 0; o < S && rank < n; ++o)
-        if (o != s) rank += larger(row + o * n, n, k);
-      if (rank >= n) continue;
+    // lists 2 s and 2 s + 1 become list s, until a row has one
+    for (int log_lists = p.log_lists; log_lists > 0; --log_lists) {
+      for (int i = tid; i < rows << (log_lists + log_n); i += kMergeThreads) {
+        const int list = i >> log_n;
+        const uint64_t k = from[i];
+        const int rank = (i & (pad - 1)) + larger(from + ((list ^ 1) << log_n), pad, k);
+        // (zeros, past a list's end, come behind both lists' others, some of them to the same places)
+        if (rank < pad) to[((list >> 1) << log_n) + rank] = k;
+      }
+      __syncthreads();
+      uint64_t* t = from;
+      from = to;
+      to = t;
+    }
+    for (int i = tid; i < rows * n; i += kMergeThreads) {
+      const int r = i / n, rank = i - r * n;
+      const uint64_t k = from[(r << log_n) + rank];
       const double c = norm[k0 + r];
       const double t = ((double)from_ordered((uint32_t)(k >> 32)) - tops[k0 + r]) + c;
       const bool alive = c == c;
@@ -354,13 +463,16 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const MergePa
 
 struct Split {
   int stretches, tiles_per;
+  bool few;
 };
-// About four CTAs per SM over all rows, whole tiles each.
+// About two CTAs per SM over all rows, whole tiles each: a stretch's first tile costs as much as four others.
 Split split_rows(int64_t rows, int64_t V, int sms) {
-  const int64_t tiles = (V + 7 + kTile - 1) / kTile;
-  int64_t s = std::min<int64_t>({tiles, (int64_t)kMaxStretches, std::max<int64_t>(1, 4ll * sms / rows)});
+  const int64_t large = kThreads * kPerMany, small = kThreads * kPerFew;
+  const bool few = rows * ((V + 7 + large - 1) / large) <= sms;
+  const int64_t tile = few ? small : large, tiles = (V + 7 + tile - 1) / tile;
+  const int64_t s = std::min<int64_t>({tiles, (int64_t)kMaxStretches, std::max<int64_t>(1, 2ll * sms / rows)});
   const int64_t per = (tiles + s - 1) / s;
-  return {(int)((tiles + per - 1) / per), (int)per};
+  return {(int)((tiles + per - 1) / per), (int)per, few};
 }
 
 constexpr int kMergeSmem = 128 * 1024;
@@ -406,7 +518,8 @@ int beam_select(const void* logits, int64_t row_stride, int fp32, const float* s
   r.sums = static_cast<float2*>(workspace);
   r.keys = reinterpret_cast<uint64_t*>(r.sums + entries);
   const dim3 grid((unsigned)sp.stretches, (unsigned)rows);
-  const auto kern = fp32 ? beam_rows_kernel<float> : beam_rows_kernel<__nv_bfloat16>;
+  const auto kern = fp32 ? (sp.few ? beam_rows_kernel<float, kPerFew> : beam_rows_kernel<float, kPerMany>)
+                         : (sp.few ? beam_rows_kernel<__nv_bfloat16, kPerFew> : beam_rows_kernel<__nv_bfloat16, kPerMany>);
   if (launch_pdl(kern, grid, dim3(kThreads), 0, stream, r) != cudaSuccess) return LKV_ERR_CUDA;
   MergeParams m{};
   m.keys = r.keys;
@@ -422,7 +535,9 @@ int beam_select(const void* logits, int64_t row_stride, int fp32, const float* s
   m.out_rows = out_rows;
   m.out_tokens = out_tokens;
   m.out_finished = out_finished;
-  const int row_bytes = sp.stretches * select * (int)sizeof(uint64_t);  // at most 16 KB
+  while (1 << m.log_n < select) ++m.log_n;
+  while (1 << m.log_lists < sp.stretches) ++m.log_lists;
+  const int row_bytes = (3 << (m.log_n + m.log_lists)) / 2 * (int)sizeof(uint64_t) + (int)sizeof(uint64_t);  // 24 KB at most
   m.rows_per_pass = std::min(beams, kMergeSmem / row_bytes);
   const int smem = m.rows_per_pass * row_bytes;
   static bool attr_done[64] = {false};
