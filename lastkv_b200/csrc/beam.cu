@@ -7,16 +7,16 @@
 // Within a beam they are ordered as its logits are, so one pass over the logits in their own type
 // finds each row's `select` largest together with its maximum and sum of exponentials (fp32):
 //
-//   beam_rows    A CTA takes a stretch of a row in tiles of 4096 or 8192 values, 16 or 32 in
-//                each thread's registers.  It keeps the stretch's best `select` as sorted 64-bit keys (the value as
-//                an ordered integer, then the complement of the index, so that no two are equal) and
-//                collects the values above the last of them: later tiles mostly hold none, so that a
-//                comparison per value is what selection costs.  A tile with too many (the first one)
-//                first finds a bar that at least `select` of its values reach: the select-th largest of a
-//                warp's 32 lane maxima, in the warp where that is largest, or the (select / 8)-th, in the
-//                warp where it is least.  Of values equal to the bar, where they are too many (a masked
-//                vocabulary), the first ones are taken; if still too many lie above it, the tile's best are
-//                taken out one by one.
+//   beam_rows    A CTA takes a stretch of a row; its warps take pieces of 32 x 16 bytes by turns, each for
+//                itself.  A warp keeps its best 32 as sorted 64-bit keys, one per lane (the value as an
+//                ordered integer, then the complement of the index, so that no two are equal), and puts the
+//                few values that may be among the stretch's best into their places one by one; for the rest
+//                selection costs a comparison of a lane's maximum.  What they are held against is a bar
+//                that at least `select` values of the stretch reach: the select-th largest of the four best
+//                of every warp, which the warps leave in shared memory as they rise, at first by their
+//                lanes' maxima.  (How old those are that a warp finds does not change the result, only how
+//                many values it looks at.)
+//                At the end the warps' lists are merged two by two (bitonic).
 //   beam_merge   A CTA per batch item joins each row's stretches two by two, then the rows: lists are
 //                sorted, so a candidate's rank is its place in its own list and a binary search in the other.
 //
@@ -35,12 +35,9 @@ namespace lkv {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-// Values per thread and tile: 32 (tiles of 8192), or 16 where that leaves SMs without a tile.  4 rows of 128256:
-// 12.2 us with 32, 10.4 with 16.
-constexpr int kPerMany = 32, kPerFew = 16;
+constexpr int kGroupValues = 16;  // a lane's values that are loaded together, one group ahead
 constexpr int kMaxSelect = 32;
 constexpr int kMaxBeams = 64;
-constexpr int kCandidates = 1024;        // a tile's values over the bar
 constexpr int kMaxStretches = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -54,11 +51,6 @@ __device__ __forceinline__ float from_ordered(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 __device__ __forceinline__ uint64_t max_key(uint64_t a, uint64_t b) { return a > b ? a : b; }
-__device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) k = max_key(k, __shfl_xor_sync(0xffffffffu, k, o));
-  return k;
-}
 
 // The lanes' values sorted from the largest: lane r has the r-th (bitonic).
 __device__ __forceinline__ uint32_t warp_sort(uint32_t v, int lane) {
@@ -73,28 +65,38 @@ __device__ __forceinline__ uint32_t warp_sort(uint32_t v, int lane) {
   return v;
 }
 
+// The 32 largest of two sorted lists, one key of each per lane, sorted: the second is given reversed, so that the
+// larger of each lane's pair are the 32 largest and form a bitonic sequence.
+__device__ __forceinline__ uint64_t merge_lists(uint64_t a, uint64_t b_reversed, int lane) {
+  uint64_t v = max_key(a, b_reversed);
+#pragma unroll
+  for (int j = 16; j > 0; j >>= 1) {
+    const uint64_t other = __shfl_xor_sync(0xffffffffu, v, j);
+    v = (lane & j) == 0 ? max_key(v, other) : (v < other ? v : other);
+  }
+  return v;
+}
+
 struct RowsParams {
   const void* logits;
   int64_t row_stride;
   int64_t V;
   const uint8_t* finished;  // [rows] or null
   int64_t eos;
-  int select, stretches, tiles_per;
+  int select, stretches;
+  int pieces_per;  // of a stretch: kWarps x 32 x 16 bytes each
   uint64_t* keys;  // [rows][stretches][select], sorted, 0 past the last
   float2* sums;    // [rows][stretches]: maximum, sum of exp(x - maximum)
 };
 
-template <typename T, int kPer>
-__global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(const RowsParams p) {
-  constexpr int kTile = kThreads * kPer;
-  constexpr int VE = 16 / sizeof(T);  // values per 16-byte load
-  __shared__ uint64_t cand[kCandidates + kMaxSelect];
-  __shared__ uint64_t best[2][kMaxSelect];
-  __shared__ uint64_t warp_key[kWarps];
-  __shared__ float warp_bar[kWarps], warp_eighth[kWarps];
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4) beam_rows_kernel(const RowsParams p) {
+  constexpr int VE = 16 / sizeof(T);  // values of a lane's 16 bytes
+  constexpr int kGroup = kGroupValues / VE;
+  __shared__ uint64_t lists[kWarps][32];
   __shared__ float2 warp_sum[kWarps];
-  __shared__ int counts[2];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __shared__ volatile uint32_t known[kWarps * 4];  // ordered values: each warp's best four so far, at least
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
   pdl_wait();
   const int64_t row = blockIdx.y;
@@ -102,224 +104,133 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(const RowsParams
   const int64_t out = row * p.stretches + blockIdx.x;
   if (p.finished && p.finished[row]) {
     // one candidate of total 0 + score; behind it the first tokens, at -inf
-    if (tid < n) {
+    const int i = threadIdx.x;
+    if (i < n) {
       const uint32_t eos = (uint32_t)p.eos, low = ordered(-INFINITY);
-      const uint32_t i = tid == 0 ? eos : (uint32_t)(tid - 1) + ((uint32_t)(tid - 1) >= eos ? 1u : 0u);
-      p.keys[out * n + tid] =
-          blockIdx.x == 0 ? (uint64_t)(tid == 0 ? ordered(0.f) : low) << 32 | (0xffffffffu - i) : 0;
+      const uint32_t token = i == 0 ? eos : (uint32_t)(i - 1) + ((uint32_t)(i - 1) >= eos ? 1u : 0u);
+      p.keys[out * n + i] = blockIdx.x == 0 ? (uint64_t)(i == 0 ? ordered(0.f) : low) << 32 | ~token : 0;
     }
-    if (tid == 0) p.sums[out] = make_float2(0.f, 1.f);
+    if (i == 0) p.sums[out] = make_float2(0.f, 1.f);
     return;
   }
   const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
-  // tiles start at 16-byte boundaries, so a row's first may begin before it
+  // pieces start at 16-byte boundaries, so a row's first may begin before it
   const int lead = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  const int64_t first = (int64_t)blockIdx.x * p.tiles_per;
-  int cur = 0;
-  if (tid < n) best[0][tid] = 0;
-  if (tid < 2) counts[tid] = 0;
-  __syncthreads();
-  float m = -INFINITY, sum = 0.f;
-  for (int64_t t = first; t < first + p.tiles_per; ++t) {
-    const int64_t base = t * kTile - lead;
-    if (base >= p.V) break;
-    float v[kPer];
-    // the index of v[e]: base + (e / VE * kThreads + tid) * VE + e % VE
-    auto place = [&](int e) { return (e / VE * kThreads + tid) * VE + e % VE; };
-    const bool whole = base >= 0 && base + kTile <= p.V;
-    if (whole) {
-      const uint4* at = reinterpret_cast<const uint4*>(x + base) + tid;
-      uint4 w[kPer / VE];
+  // piece j of this warp: 32 lanes x VE values from index first + j * kWarps * 32 * VE on
+  constexpr uint32_t kStep = kWarps * 32 * VE;
+  const int64_t first = ((int64_t)blockIdx.x * p.pieces_per * kWarps + warp) * (32 * VE) + lane * VE - lead;
+  // a lane's 16 bytes lie in the row where its first index, in 32 bits, is below this (one below the row's start wraps)
+  const uint32_t inside = p.V >= VE ? (uint32_t)(p.V - VE) + 1 : 0;
+  auto load = [&](uint4 (&w)[kGroup], int j0) {  // returns which pieces are there
+    uint32_t there = 0;
 #pragma unroll
-      for (int i = 0; i < kPer / VE; ++i) w[i] = __ldcs(at + i * kThreads);
+    for (int j = 0; j < kGroup; ++j) {
+      const uint32_t i = (uint32_t)first + (uint32_t)(j0 + j) * kStep;
+      if (j0 + j < p.pieces_per && i < inside) {
+        w[j] = __ldcs(reinterpret_cast<const uint4*>(x + i));
+        there |= 1u << j;
+      }
+    }
+    return there;
+  };
+  float m = -INFINITY, sum = 0.f;  // this lane's
+  uint64_t list = 0, last = 0;     // lane r: the warp's r-th best key; the select-th
+  float bar = -INFINITY;           // what may be among the stretch's best is above it
+  bool all = true;                 // not even that is known: fewer than select values so far
+  // A bar from what the warps have left in shared memory and this one's own list.  Values equal to another warp's
+  // may come before them: that bar is the next value below.
+  static_assert(kWarps * 4 == 32, "one of the known values for each lane");
+  auto raise = [&] {
+    uint32_t below = max(__shfl_sync(0xffffffffu, warp_sort(known[lane], lane), n - 1), 1u) - 1;
+    if (below == 0x7fffffffu) --below;  // -0, which is no less than 0
+    const uint32_t at = max(below, (uint32_t)(last >> 32));
+    all = at < ordered(-INFINITY);
+    bar = all ? -INFINITY : from_ordered(at);
+  };
+  uint4 w[kGroup];
+  uint32_t there = load(w, 0);
+  for (int j0 = 0; j0 < p.pieces_per; j0 += kGroup) {
+    if (j0 && first - lane * VE + (int64_t)j0 * kStep >= p.V) break;  // the same for the warp
+    float v[kGroup][VE], tops[kGroup];
+    float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < kPer / VE; ++i) {
-        const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+    for (int j = 0; j < kGroup; ++j) {
+      if (there >> j & 1) {
+        const uint32_t u[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
-          if constexpr (sizeof(T) == 2) v[i * VE + e] = e & 1 ? bf16_hi(u[e / 2]) : bf16_lo(u[e / 2]);
-          else v[i * VE + e] = __uint_as_float(u[e]);
+          if constexpr (sizeof(T) == 2) v[j][e] = e & 1 ? bf16_hi(u[e / 2]) : bf16_lo(u[e / 2]);
+          else v[j][e] = __uint_as_float(u[e]);
         }
+      } else {
+        const uint32_t i = (uint32_t)first + (uint32_t)(j0 + j) * kStep;
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+          v[j][e] = j0 + j < p.pieces_per && i + e < (uint32_t)p.V ? (float)x[i + e] : -INFINITY;
       }
-    } else {
+      tops[j] = v[j][0];
 #pragma unroll
-      for (int i = 0; i < kPer / VE; ++i) {
-        const int64_t at = base + place(i * VE);
-        if (at >= 0 && at + VE <= p.V) {
-          const uint4 w = __ldcs(reinterpret_cast<const uint4*>(x + at));
-          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            if constexpr (sizeof(T) == 2) v[i * VE + e] = e & 1 ? bf16_hi(u[e / 2]) : bf16_lo(u[e / 2]);
-            else v[i * VE + e] = __uint_as_float(u[e]);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < VE; ++e) v[i * VE + e] = at + e >= 0 && at + e < p.V ? (float)x[at + e] : -INFINITY;
-        }
-      }
+      for (int e = 1; e < VE; ++e) tops[j] = fmaxf(tops[j], v[j][e]);
+      top = fmaxf(top, tops[j]);
     }
-    // the thread's maximum and sum, over all its tiles; a NaN stays in the sum
-    float top = v[0];
-#pragma unroll
-    for (int e = 1; e < kPer; ++e) top = fmaxf(top, v[e]);
+    there = load(w, j0 + kGroup);
+    // maximum and sum; a NaN stays in the sum
     const float nm = fmaxf(m, top);
     if (nm != -INFINITY) {
-      if (nm != m) sum *= exp2f((m - nm) * kLog2e);
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) part[e & 3] += ex2_approx((v[e] - nm) * kLog2e);
-      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      if (nm != m) sum *= ex2_approx((m - nm) * kLog2e);
       m = nm;
+#pragma unroll
+      for (int j = 0; j < kGroup; ++j) {
+        float part = 0.f;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) part += ex2_approx((v[j][e] - nm) * kLog2e);
+        sum += part;
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) sum = v[e] == v[e] ? sum : NAN;
+      for (int j = 0; j < kGroup; ++j)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) sum = v[j][e] == v[j][e] ? sum : NAN;
     }
-    auto key = [&](int e) -> uint64_t {  // 0 outside the row (below its start the index wraps around)
-      const uint32_t i = (uint32_t)base + (uint32_t)place(e);
-      return i < (uint32_t)p.V ? (uint64_t)ordered(v[e]) << 32 | ~i : 0;
-    };
-    // Values above the list's last: an equal one, of a later index, comes behind it.  (A NaN, which counts as
-    // -inf, is not below anything; its key tells.)
-    const uint64_t last = best[cur][n - 1];
-    const bool empty = last == 0;
-    const float list_bar = empty ? -INFINITY : from_ordered((uint32_t)(last >> 32));
-    const bool some = empty || top > list_bar;
-    if (!__syncthreads_or(some)) continue;
-    float bar = list_bar;
-    bool equal = false;  // whether values equal to the bar count
-    // A bar that at least n of the tile's values reach.
-    auto tile_bar = [&] {
+    // the warp's best
+    if (j0 == 0) {
       const uint32_t sorted = warp_sort(ordered(top), lane);
-      if (lane == n - 1) warp_bar[warp] = from_ordered(sorted);
-      if (lane == (n + kWarps - 1) / kWarps - 1) warp_eighth[warp] = from_ordered(sorted);
-      __syncthreads();
-      float least = warp_eighth[0], most = warp_bar[0];
-#pragma unroll
-      for (int w = 1; w < kWarps; ++w) {
-        most = fmaxf(most, warp_bar[w]);
-        least = fminf(least, warp_eighth[w]);
-      }
-      return fmaxf(most, least);
-    };
-    // Collects the values above (or equal to) the bar behind the entries that are there.  (The order does not
-    // matter: keys are ranked below.)
-    auto collect = [&] {
-      uint32_t mask = 0;
-      if (!(top < bar)) {
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) mask |= (uint32_t)(equal ? !(v[e] < bar) : v[e] > bar) << e;
-      }
-      if (mask) {
-        int at = atomicAdd(&counts[0], __popc(mask));
-#pragma unroll
-        for (int e = 0; e < kPer; ++e)
-          if (mask >> e & 1) {
-            if (at < kCandidates) cand[at] = key(e);
-            ++at;
-          }
-      }
-      __syncthreads();
-      return counts[0];
-    };
-    if (empty) {
-      bar = tile_bar();
-      equal = true;
+      if (lane < 4) known[warp * 4 + lane] = sorted;
+      asm volatile("bar.sync 1, %0;" ::"n"(kThreads));
     }
-    int total = collect();
-    if (total > kCandidates) {
-      // too many: count what lies above a bar of the tile's own, and on it
-      if (!empty) {
-        const float own = tile_bar();
-        if (own > list_bar) bar = own, equal = true;
-      }
-      __syncthreads();  // counts are read
-      if (tid < 2) counts[tid] = 0;
-      __syncthreads();
-      int above = 0, level = 0;
-      if (!(top < bar)) {
+    if (!__any_sync(0xffffffffu, all || top > bar)) continue;
+    raise();
+    if (!__any_sync(0xffffffffu, all || top > bar)) continue;
+    bool changed = false;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          above += v[e] > bar;
-          level += equal && !(v[e] < bar) && !(v[e] > bar);
+    for (int j = 0; j < kGroup; ++j) {
+      if (!__any_sync(0xffffffffu, all || tops[j] > bar)) continue;
+      const uint32_t i0 = (uint32_t)first + (uint32_t)(j0 + j) * kStep;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float y = v[j][e];
+        if (!__any_sync(0xffffffffu, all || y > bar)) continue;
+        const uint32_t i = i0 + e;
+        const bool valid = (all || y > bar) && i < (uint32_t)p.V && j0 + j < p.pieces_per;
+        const uint64_t key = valid ? (uint64_t)ordered(y) << 32 | ~i : 0;
+        uint32_t who = __ballot_sync(0xffffffffu, key > last);
+        changed |= who != 0;
+        while (who) {
+          const uint64_t k = __shfl_sync(0xffffffffu, key, __ffs(who) - 1);
+          const int place = __popc(__ballot_sync(0xffffffffu, list > k));
+          const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
+          list = lane < place ? list : lane == place ? k : up;
+          last = __shfl_sync(0xffffffffu, list, n - 1);
+          who &= who - 1;
+          who &= __ballot_sync(0xffffffffu, key > last);
         }
       }
-      above = __reduce_add_sync(0xffffffffu, above);
-      level = __reduce_add_sync(0xffffffffu, level);
-      if (lane == 0 && above) atomicAdd(&counts[0], above);
-      if (lane == 0 && level) atomicAdd(&counts[1], level);
-      __syncthreads();
-      above = counts[0];
-      level = counts[1];
-      __syncthreads();
-      if (tid < 2) counts[tid] = 0;
-      if (above > kCandidates - kMaxSelect) {
-        // the tile's best, one after another
-        uint64_t before = ~0ull;
-        for (int r = 0; r < n; ++r) {
-          uint64_t big = 0;
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) {
-            const uint64_t k = key(e);
-            if (k < before) big = max_key(big, k);
-          }
-          big = warp_max_key(big);
-          if (lane == 0) warp_key[warp] = big;
-          __syncthreads();
-          big = warp_key[0];
-          for (int w = 1; w < kWarps; ++w) big = max_key(big, warp_key[w]);
-          if (tid == 0) cand[r] = big;
-          before = big;
-          __syncthreads();
-        }
-        total = n;
-      } else {
-        if (above + level > kCandidates) {
-          // the first of the values equal to the bar (a NaN counts as -inf)
-          equal = false;
-          int64_t after = -1;
-          for (int r = 0; r < n; ++r) {
-            uint32_t next = 0xffffffffu;
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-              const int64_t i = base + place(e);
-              const float y = v[e] == v[e] ? v[e] : -INFINITY;
-              if (y == bar && i > after && i < p.V) next = min(next, (uint32_t)i);
-            }
-            next = __reduce_min_sync(0xffffffffu, next);
-            if (lane == 0) warp_key[warp] = next;
-            __syncthreads();
-            for (int w = 0; w < kWarps; ++w) next = min(next, (uint32_t)warp_key[w]);
-            if (tid == 0) cand[r] = next == 0xffffffffu ? 0 : (uint64_t)ordered(bar) << 32 | (0xffffffffu - next);
-            after = next;
-            __syncthreads();
-          }
-          if (tid == 0) counts[0] = n;
-        }
-        __syncthreads();
-        total = min(collect(), kCandidates);
-      }
     }
-    // the new list: every entry of the old one and of the collected ones finds its rank among all
-    if (tid < n) {
-      cand[total + tid] = best[cur][tid];
-      best[cur ^ 1][tid] = 0;
+    if (changed) {
+      if (lane < 4) known[warp * 4 + lane] = max(known[warp * 4 + lane], (uint32_t)(list >> 32));
     }
-    __syncthreads();
-    if (tid < 2) counts[tid] = 0;
-    const int all = total + n;
-    for (int a = tid; a < all; a += kThreads) {
-      const uint64_t k = cand[a];
-      if (k == 0) continue;
-      int rank = 0;
-#pragma unroll 4
-      for (int b = 0; b < all; ++b) rank += cand[b] > k;
-      if (rank < n) best[cur ^ 1][rank] = k;
-    }
-    __syncthreads();
-    cur ^= 1;
   }
-  // the stretch's maximum and sum: the warps', then the CTA's, in a fixed order
+  // the stretch's list, maximum and sum: the warps', then the CTA's, in a fixed order
   auto join = [lane](float2 ms, int lanes) {
     float t = ms.x;
     for (int o = lanes / 2; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
@@ -329,12 +240,17 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(const RowsParams
   };
   const float2 mine = join(make_float2(m, sum), 32);
   if (lane == 0) warp_sum[warp] = mine;
-  __syncthreads();
+#pragma unroll
+  for (int half = kWarps / 2; half > 0; half >>= 1) {
+    if (warp >= half && warp < 2 * half) lists[warp][lane] = list;
+    __syncthreads();
+    if (warp < half) list = merge_lists(list, lists[warp + half][31 - lane], lane);
+  }
   if (warp == 0) {
     const float2 all = join(warp_sum[lane % kWarps], kWarps);
     if (lane == 0) p.sums[out] = all;
+    if (lane < n) p.keys[out * n + lane] = list;
   }
-  if (tid < n) p.keys[out * n + tid] = best[cur][tid];
 }
 
 struct MergeParams {
@@ -384,14 +300,17 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const MergePa
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       // a stretch of -inf alone adds 0, or a NaN
       auto part = [top](float2 ms) {
-        return ms.x == -INFINITY || ms.x == top ? (double)ms.y : (double)ms.y * (double)expf(ms.x - top);
+        return ms.x == -INFINITY || ms.x == top ? (double)ms.y : (double)(ms.y * ex2_approx((ms.x - top) * kLog2e));
       };
       double sum = part(a) + part(c);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (lane == 0) {
         const bool done = p.finished && p.finished[row];
-        const double score = (double)p.scores[row], rest = done ? 0.0 : log(sum);
+        // log(f 2^e) = e log 2 + log f with f in 1 .. 2, whose logarithm fp32 has to 2^-24
+        const int e = ilogb(sum);
+        const double score = (double)p.scores[row];
+        const double rest = done ? 0.0 : e * 0.6931471805599453 + (double)logf((float)scalbn(sum, -e));
         tops[k] = done ? 0.0 : (double)top;
         norm[k] = fabs(score) < INFINITY && fabs(tops[k]) < INFINITY && fabs(rest) < INFINITY ? score - rest : NAN;
       }
@@ -462,17 +381,14 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const MergePa
 }
 
 struct Split {
-  int stretches, tiles_per;
-  bool few;
+  int stretches, pieces;
 };
-// About two CTAs per SM over all rows, whole tiles each: a stretch's first tile costs as much as four others.
-Split split_rows(int64_t rows, int64_t V, int sms) {
-  const int64_t large = kThreads * kPerMany, small = kThreads * kPerFew;
-  const bool few = rows * ((V + 7 + large - 1) / large) <= sms;
-  const int64_t tile = few ? small : large, tiles = (V + 7 + tile - 1) / tile;
-  const int64_t s = std::min<int64_t>({tiles, (int64_t)kMaxStretches, std::max<int64_t>(1, 2ll * sms / rows)});
-  const int64_t per = (tiles + s - 1) / s;
-  return {(int)((tiles + per - 1) / per), (int)per, few};
+// Stretches for about three CTAs per SM over all rows, of two pieces for each warp at least.
+Split split_rows(int64_t rows, int64_t V, int elem, int sms) {
+  const int64_t piece = kThreads * 16 / elem, pieces = (V + 16 / elem - 1 + piece - 1) / piece;
+  const int64_t s = std::min<int64_t>({(pieces + 1) / 2, (int64_t)kMaxStretches, std::max<int64_t>(1, 3ll * sms / rows)});
+  const int64_t per = (pieces + s - 1) / s;
+  return {(int)((pieces + per - 1) / per), (int)per};
 }
 
 constexpr int kMergeSmem = 128 * 1024;
@@ -501,7 +417,7 @@ int beam_select(const void* logits, int64_t row_stride, int fp32, const float* s
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return LKV_ERR_CUDA;
-  const Split sp = split_rows(rows, vocab, sms);
+  const Split sp = split_rows(rows, vocab, fp32 ? 4 : 2, sms);
   const size_t entries = (size_t)rows * sp.stretches;
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
       workspace_bytes < entries * (select * sizeof(uint64_t) + sizeof(float2)))
@@ -514,12 +430,11 @@ int beam_select(const void* logits, int64_t row_stride, int fp32, const float* s
   r.eos = eos;
   r.select = select;
   r.stretches = sp.stretches;
-  r.tiles_per = sp.tiles_per;
+  r.pieces_per = sp.pieces;
   r.sums = static_cast<float2*>(workspace);
   r.keys = reinterpret_cast<uint64_t*>(r.sums + entries);
   const dim3 grid((unsigned)sp.stretches, (unsigned)rows);
-  const auto kern = fp32 ? (sp.few ? beam_rows_kernel<float, kPerFew> : beam_rows_kernel<float, kPerMany>)
-                         : (sp.few ? beam_rows_kernel<__nv_bfloat16, kPerFew> : beam_rows_kernel<__nv_bfloat16, kPerMany>);
+  const auto kern = fp32 ? beam_rows_kernel<float> : beam_rows_kernel<__nv_bfloat16>;
   if (launch_pdl(kern, grid, dim3(kThreads), 0, stream, r) != cudaSuccess) return LKV_ERR_CUDA;
   MergeParams m{};
   m.keys = r.keys;
