@@ -260,7 +260,7 @@ struct MergeParams {
   const uint8_t* finished;
   int64_t V, eos;
   int K, select, stretches;
-  int log_n, log_lists;  // select and stretches, rounded up to powers of two
+  int log_n, log_lists, log_beams;  // select, stretches and beams, rounded up to powers of two
   int rows_per_pass;     // rows whose keys fit in shared memory at once
   float* out_scores;
   int64_t* out_rows;
@@ -276,7 +276,47 @@ __device__ __forceinline__ int larger(const uint64_t* list, int n, uint64_t k) {
   return at + (list[at] > k);
 }
 
+// A total as an integer of the same order, above 0.
+__device__ __forceinline__ uint64_t ordered(double x) {
+  const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);
+  return b >> 63 ? ~b : b | 1ull << 63;
+}
+__device__ __forceinline__ double from_ordered(uint64_t k) {
+  return __longlong_as_double((long long)(k >> 63 ? k & ~(1ull << 63) : ~k));
+}
+
 constexpr int kMergeThreads = 512;
+
+// Lists of 1 << log_n entries, sorted from the largest, two by two into half as many, until there is one for
+// each 1 << log_lists; of equal entries the earlier list's come first (k + 1 in its place in the search).  Where a
+// payload goes with the keys it moves along.  Returns with `from` the result's place.
+template <bool PAYLOAD>
+__device__ __forceinline__ void merge_rounds(uint64_t*& from, uint64_t*& to, uint32_t*& pay, uint32_t*& pay_to, int groups,
+                                             int log_lists, int log_n) {
+  const int pad = 1 << log_n;
+  for (; log_lists > 0; --log_lists) {
+    for (int i = threadIdx.x; i < groups << (log_lists + log_n); i += kMergeThreads) {
+      const int list = i >> log_n;
+      const uint64_t k = from[i];
+      // an equal entry of the list before comes first: it counts as larger
+      const int rank = (i & (pad - 1)) + larger(from + ((list ^ 1) << log_n), pad, PAYLOAD && (list & 1) && k ? k - 1 : k);
+      // (zeros, past a list's end, come behind both lists' others, some of them to the same places)
+      if (rank < pad) {
+        to[((list >> 1) << log_n) + rank] = k;
+        if (PAYLOAD) pay_to[((list >> 1) << log_n) + rank] = pay[i];
+      }
+    }
+    __syncthreads();
+    uint64_t* t = from;
+    from = to;
+    to = t;
+    if (PAYLOAD) {
+      uint32_t* u = pay;
+      pay = pay_to;
+      pay_to = u;
+    }
+  }
+}
 
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const MergeParams p) {
   // [rows_per_pass][1 << log_lists][1 << log_n], padded with zeros, then as much again for half as many lists
@@ -284,99 +324,95 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const MergePa
   // A total is (x - top) + norm: the maximum is taken off first, so that rows of values like a type's
   // lowest keep their sums' logarithms and their scores.  norm NaN: every total of the row is -inf.
   __shared__ double tops[kMaxBeams], norm[kMaxBeams];
-  __shared__ double total[kMaxBeams * kMaxSelect];
+  __shared__ uint64_t total[kMaxBeams * kMaxSelect * 3 / 2];  // ordered totals: a list of 1 << log_n for each beam
+  __shared__ uint32_t from_where[kMaxBeams * kMaxSelect * 3 / 2];  // the beam and the place in its list
   __shared__ uint32_t token[kMaxBeams * kMaxSelect];
   const int b = blockIdx.x, n = p.select, K = p.K, S = p.stretches, tid = threadIdx.x;
+  const int log_n = p.log_n, pad = 1 << log_n;
   pdl_launch_dependents();
   pdl_wait();
-  auto row_norms = [&] {
-    for (int k = tid >> 5; k < K; k += kMergeThreads / 32) {  // a warp per row, two stretches per lane
-      const int64_t row = (int64_t)b * K + k;
-      const int lane = tid & 31;
-      const float2 none = make_float2(-INFINITY, 0.f);
-      const float2 a = lane < S ? p.sums[row * S + lane] : none, c = lane + 32 < S ? p.sums[row * S + lane + 32] : none;
-      float top = fmaxf(a.x, c.x);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      // a stretch of -inf alone adds 0, or a NaN
-      auto part = [top](float2 ms) {
-        return ms.x == -INFINITY || ms.x == top ? (double)ms.y : (double)(ms.y * ex2_approx((ms.x - top) * kLog2e));
-      };
-      double sum = part(a) + part(c);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0) {
-        const bool done = p.finished && p.finished[row];
-        // log(f 2^e) = e log 2 + log f with f in 1 .. 2, whose logarithm fp32 has to 2^-24
-        const int e = ilogb(sum);
-        const double score = (double)p.scores[row];
-        const double rest = done ? 0.0 : e * 0.6931471805599453 + (double)logf((float)scalbn(sum, -e));
-        tops[k] = done ? 0.0 : (double)top;
-        norm[k] = fabs(score) < INFINITY && fabs(tops[k]) < INFINITY && fabs(rest) < INFINITY ? score - rest : NAN;
-      }
-    }
-  };
+  const int lane = tid & 31;
+  const float2 none = make_float2(-INFINITY, 0.f);
+  auto sums_at = [&](int k, int s) { return k < K && s < S ? __ldcg(p.sums + ((int64_t)b * K + k) * S + s) : none; };
+  float2 a = sums_at(tid >> 5, lane), c = sums_at(tid >> 5, lane + 32);  // a warp per row, two stretches per lane
+  for (int i = tid; i < 1 << (p.log_beams + log_n); i += kMergeThreads) total[i] = 0;
   for (int k0 = 0; k0 < K; k0 += p.rows_per_pass) {
     const int rows = min(p.rows_per_pass, K - k0);
     const uint64_t* in = p.keys + ((int64_t)b * K + k0) * S * n;
-    const int log_n = p.log_n, pad = 1 << log_n;
     uint64_t* from = keys;
     uint64_t* to = keys + ((int64_t)p.rows_per_pass << (p.log_lists + log_n));
+    uint32_t* unused = nullptr;
     __syncthreads();
-    for (int i = tid; i < rows << (p.log_lists + log_n); i += kMergeThreads) {
-      const int at = i & (pad - 1), list = i >> log_n, s = list & ((1 << p.log_lists) - 1), r = list >> p.log_lists;
-      from[i] = at < n && s < S ? in[(r * S + s) * n + at] : 0;
-    }
-    if (k0 == 0) row_norms();
-    __syncthreads();
-    // lists 2 s and 2 s + 1 become list s, until a row has one
-    for (int log_lists = p.log_lists; log_lists > 0; --log_lists) {
-      for (int i = tid; i < rows << (log_lists + log_n); i += kMergeThreads) {
-        const int list = i >> log_n;
-        const uint64_t k = from[i];
-        const int rank = (i & (pad - 1)) + larger(from + ((list ^ 1) << log_n), pad, k);
-        // (zeros, past a list's end, come behind both lists' others, some of them to the same places)
-        if (rank < pad) to[((list >> 1) << log_n) + rank] = k;
+    const int entries = rows << (p.log_lists + log_n);
+    for (int i0 = tid; i0 < entries; i0 += 8 * kMergeThreads) {  // eight loads in flight
+      uint64_t k[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = i0 + j * kMergeThreads;
+        const int at = i & (pad - 1), list = i >> log_n, s = list & ((1 << p.log_lists) - 1), r = list >> p.log_lists;
+        const bool there = i < entries && at < n && s < S;
+        k[j] = __ldcg(in + (there ? (r * S + s) * n + at : 0));
+        if (!there) k[j] = 0;
       }
-      __syncthreads();
-      uint64_t* t = from;
-      from = to;
-      to = t;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (i0 + j * kMergeThreads < entries) from[i0 + j * kMergeThreads] = k[j];
     }
-    for (int i = tid; i < rows * n; i += kMergeThreads) {
-      const int r = i / n, rank = i - r * n;
-      const uint64_t k = from[(r << log_n) + rank];
-      const double c = norm[k0 + r];
-      const double t = ((double)from_ordered((uint32_t)(k >> 32)) - tops[k0 + r]) + c;
-      const bool alive = c == c;
+    if (k0 == 0) {
+      for (int k = tid >> 5; k < K; k += kMergeThreads / 32) {
+        const int64_t row = (int64_t)b * K + k;
+        float top = fmaxf(a.x, c.x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        // a stretch of -inf alone adds 0, or a NaN
+        auto part = [top](float2 ms) {
+          return ms.x == -INFINITY || ms.x == top ? (double)ms.y : (double)(ms.y * ex2_approx((ms.x - top) * kLog2e));
+        };
+        double sum = part(a) + part(c);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) {
+          const bool done = p.finished && p.finished[row];
+          // log(f 2^e) = e log 2 + log f with f in 1 .. 2, whose logarithm fp32 has to 2^-24
+          const int e = ilogb(sum);
+          const double score = (double)p.scores[row];
+          const double rest = done ? 0.0 : e * 0.6931471805599453 + (double)logf((float)scalbn(sum, -e));
+          tops[k] = done ? 0.0 : (double)top;
+          norm[k] = fabs(score) < INFINITY && fabs(tops[k]) < INFINITY && fabs(rest) < INFINITY ? score - rest : NAN;
+        }
+        a = sums_at(k + kMergeThreads / 32, lane);
+        c = sums_at(k + kMergeThreads / 32, lane + 32);
+      }
+    }
+    __syncthreads();
+    merge_rounds<false>(from, to, unused, unused, rows, p.log_lists, log_n);
+    for (int i = tid; i < rows << log_n; i += kMergeThreads) {
+      const int k = k0 + (i >> log_n), rank = i & (pad - 1);
+      if (rank >= n) continue;
+      const uint64_t key = from[i];
+      const double t = ((double)from_ordered((uint32_t)(key >> 32)) - tops[k]) + norm[k];
+      const bool alive = norm[k] == norm[k];
       // all totals of a row without a finite score or sum are -inf: its first tokens, in their order
-      total[(k0 + r) * n + rank] = alive && t == t ? t : -INFINITY;
-      token[(k0 + r) * n + rank] = alive ? 0xffffffffu - (uint32_t)k : (uint32_t)rank;
+      const int at = (k << log_n) + rank;
+      total[at] = ordered(alive && t == t ? t : -INFINITY);
+      from_where[at] = (uint32_t)at;
+      token[k * n + rank] = alive ? 0xffffffffu - (uint32_t)key : (uint32_t)rank;
     }
   }
   __syncthreads();
-  for (int i = tid; i < K * n; i += kMergeThreads) {
-    const int k = i / n;
-    const double t = total[i];
-    int rank = i % n;
-    for (int o = 0; o < K && rank < n; ++o) {
-      if (o == k) continue;
-      // entries of row o that come before (t, k): larger, or equal and of an earlier row
-      const double* list = total + o * n;
-      int lo = 0, hi = n;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (list[mid] > t || (list[mid] == t && o < k)) lo = mid + 1;
-        else hi = mid;
-      }
-      rank += lo;
-    }
-    if (rank >= n) continue;
-    const int64_t row = (int64_t)b * K + k, at = (int64_t)b * n + rank;
-    p.out_scores[at] = (float)t;
+  uint64_t* from = total;
+  uint64_t* to = total + (1 << (p.log_beams + log_n));
+  uint32_t* pay = from_where;
+  uint32_t* pay_to = from_where + (1 << (p.log_beams + log_n));
+  merge_rounds<true>(from, to, pay, pay_to, 1, p.log_beams, log_n);
+  if (tid < n) {
+    const int k = (int)(pay[tid] >> log_n);
+    const uint32_t v = token[k * n + (pay[tid] & (pad - 1))];
+    const int64_t row = (int64_t)b * K + k, at = (int64_t)b * n + tid;
+    p.out_scores[at] = (float)from_ordered(from[tid]);
     p.out_rows[at] = row;
-    p.out_tokens[at] = token[i];
-    if (p.out_finished) p.out_finished[at] = (int64_t)token[i] == p.eos || (p.finished && p.finished[row]);
+    p.out_tokens[at] = v;
+    if (p.out_finished) p.out_finished[at] = (int64_t)v == p.eos || (p.finished && p.finished[row]);
   }
 }
 
@@ -452,6 +488,7 @@ int beam_select(const void* logits, int64_t row_stride, int fp32, const float* s
   m.out_finished = out_finished;
   while (1 << m.log_n < select) ++m.log_n;
   while (1 << m.log_lists < sp.stretches) ++m.log_lists;
+  while (1 << m.log_beams < beams) ++m.log_beams;
   const int row_bytes = (3 << (m.log_n + m.log_lists)) / 2 * (int)sizeof(uint64_t) + (int)sizeof(uint64_t);  // 24 KB at most
   m.rows_per_pass = std::min(beams, kMergeSmem / row_bytes);
   const int smem = m.rows_per_pass * row_bytes;
