@@ -599,21 +599,16 @@ int lkv_decode_paged_q8(const void* q, int64_t q_stride_tok, const uint8_t* code
                         int max_pages_per_seq, float softmax_scale, void* workspace, size_t workspace_bytes,
                         int flags, void* stream);
 
-/* Spans of tokens over such a cache, in two calls, so that layers which read the same
- * older pages share the first:
- * lkv_q8_stage_pages copies the codes (whole numbers, exact in bf16) of each row's
- *   8-bit pages, columns below stage_width, to page b * stage_width + column of
- *   stage_k / stage_v, bf16 [batch * stage_width, 16, num_kv_heads, head_dim].
- * lkv_prefill_paged_q8 is lkv_prefill_paged with them: it reads the codes from the
- *   stage and the scales by the block table's page ids.  A row with more 8-bit pages than
- *   stage_width is recorded in error_word (may be NULL), its further ones read as zeros. */
-int lkv_q8_stage_pages(const uint8_t* codes, const float* scales, int64_t q8_pages, const int32_t* block_table,
-                       int64_t block_table_stride, const int32_t* num_q8, const int32_t* seq_k, int batch,
-                       int max_pages_per_seq, void* stage_k, void* stage_v, int stage_width, int num_kv_heads,
-                       int head_dim, int32_t* error_word, void* stream);
-int lkv_prefill_paged_q8(const void* q, int64_t q_stride_tok, const void* stage_k, const void* stage_v,
-                         int stage_width, const float* scales, int64_t q8_pages, const void* pool_k,
-                         const void* pool_v, int64_t num_pages, const int32_t* block_table,
+/* lkv_prefill_paged (spans of tokens) over such a cache.  It first copies the codes (whole
+ * numbers, exact in bf16) of each row's 8-bit pages, columns below stage_width, to
+ * page b * stage_width + column of stage_k / stage_v, bf16 [batch * stage_width, 16,
+ * num_kv_heads, head_dim], whose contents need not be kept; staged = 1: an earlier call with
+ * the same rows and pages did that (layers that read the same older pages) and the
+ * call reads the copy.  A row with more 8-bit pages than stage_width is recorded in
+ * error_word (may be NULL), its further ones read as zeros. */
+int lkv_prefill_paged_q8(const void* q, int64_t q_stride_tok, const uint8_t* codes, const float* scales,
+                         int64_t q8_pages, void* stage_k, void* stage_v, int stage_width, int staged,
+                         const void* pool_k, const void* pool_v, int64_t num_pages, const int32_t* block_table,
                          int64_t block_table_stride, const int32_t* num_q8, const int32_t* seq_k,
                          const int32_t* cu_seqlens_q, void* out, int64_t out_stride_tok, float* lse,
                          const float* out_scale, int batch, int total_q, int max_q, int num_q_heads,

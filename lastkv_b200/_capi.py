@@ -64,8 +64,7 @@ _SIGNATURES = {
     "lkv_w4_linear_q8": (I32, [P, I64, P, I64, P, P, P, I64, I64, I64, I64, I32, P, P]),
     "lkv_q8_quantize_pages": (I32, [P, P, I64, P, P, P, P, I64, P, I64, I32, I32, P, P]),
     "lkv_q8_dequantize_pages": (I32, [P, P, I64, P, P, P, I64, P, I64, I32, I32, P, P]),
-    "lkv_q8_stage_pages": (I32, [P, P, I64, P, I64, P, P, I32, I32, P, P, I32, I32, I32, P, P]),
-    "lkv_prefill_paged_q8": (I32, [P, I64, P, P, I32, P, I64, P, P, I64, P, I64, P, P, P, P, I64, P, P,
+    "lkv_prefill_paged_q8": (I32, [P, I64, P, P, I64, P, P, I32, I32, P, P, I64, P, I64, P, P, P, P, I64, P, P,
                                    I32, I32, I32, I32, I32, I32, I32, I32, F32, P, P]),
     "lkv_decode_paged_q8": (I32, [P, I64, P, P, I64, P, P, I64, P, I64, P, P, P, I64, P, P,
                                   I32, I32, I32, I32, I32, F32, P, SZ, I32, P]),

@@ -612,24 +612,14 @@ int lkv_q8_dequantize_pages(const uint8_t* codes, const float* scales, int64_t q
                                head_dim, error_word, static_cast<cudaStream_t>(stream));
 }
 
-int lkv_q8_stage_pages(const uint8_t* codes, const float* scales, int64_t q8_pages, const int32_t* block_table,
-                       int64_t block_table_stride, const int32_t* num_q8, const int32_t* seq_k, int batch,
-                       int max_pages_per_seq, void* stage_k, void* stage_v, int stage_width, int num_kv_heads,
-                       int head_dim, int32_t* error_word, void* stream) {
-  return lkv::stage_pages(codes, scales, q8_pages, block_table, block_table_stride, num_q8, seq_k, batch,
-                          max_pages_per_seq, stage_k, stage_v, stage_width, num_kv_heads, head_dim, error_word,
-                          static_cast<cudaStream_t>(stream));
-}
-
-int lkv_prefill_paged_q8(const void* q, int64_t q_stride_tok, const void* stage_k, const void* stage_v,
-                         int stage_width, const float* scales, int64_t q8_pages, const void* pool_k,
-                         const void* pool_v, int64_t num_pages, const int32_t* block_table,
+int lkv_prefill_paged_q8(const void* q, int64_t q_stride_tok, const uint8_t* codes, const float* scales,
+                         int64_t q8_pages, void* stage_k, void* stage_v, int stage_width, int staged,
+                         const void* pool_k, const void* pool_v, int64_t num_pages, const int32_t* block_table,
                          int64_t block_table_stride, const int32_t* num_q8, const int32_t* seq_k,
                          const int32_t* cu_seqlens_q, void* out, int64_t out_stride_tok, float* lse,
                          const float* out_scale, int batch, int total_q, int max_q, int num_q_heads,
                          int num_kv_heads, int head_dim, int max_pages_per_seq, int causal, float softmax_scale,
                          int32_t* error_word, void* stream) {
-  if (!stage_k && batch != 0 && total_q != 0) return LKV_ERR_INVALID_ARGUMENT;
   lkv::PrefillArgs a{};
   a.q = q;
   a.q_stride_tok = q_stride_tok;
@@ -661,7 +651,7 @@ int lkv_prefill_paged_q8(const void* q, int64_t q_stride_tok, const void* stage_
   a.num_q8 = num_q8;
   a.q8_scales = scales;
   a.q8_pages = q8_pages;
-  return lkv::prefill_paged(a);
+  return lkv::prefill_paged_q8(a, codes, staged != 0);
 }
 
 int lkv_decode_paged_q8(const void* q, int64_t q_stride_tok, const uint8_t* codes, const float* scales,

@@ -47,14 +47,16 @@ struct PrefillArgs {
   float* part_lse = nullptr;  // [kv_splits][total_q * num_q_heads], natural log
   // the first num_q8 pages of each row in 8 bits (null stage_k: none), staged by stage_pages at
   // page row * stage_width + column
-  const void* stage_k = nullptr;
-  const void* stage_v = nullptr;
+  void* stage_k = nullptr;
+  void* stage_v = nullptr;
   int stage_width = 0;
   const int32_t* num_q8 = nullptr;  // [batch], or null: every page
   const float* q8_scales = nullptr;
   int64_t q8_pages = 0;
 };
 int prefill_paged(const PrefillArgs& a);
+// With 8-bit pages: stages their codes first, unless that is done.
+int prefill_paged_q8(const PrefillArgs& a, const void* codes, bool staged);
 int prefill_split_plan(int batch, int max_q, int num_q_heads, int num_kv_heads, int head_dim, int max_pages,
                        int causal, int* kv_splits);
 

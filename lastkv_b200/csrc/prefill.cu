@@ -613,13 +613,19 @@ int launch_prefill(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorM
 
 }  // namespace
 
-int prefill_paged(const PrefillArgs& a) {
+namespace {
+// LKV_OK, or why the arguments are refused; *empty: there is nothing to do.
+int check_args(const PrefillArgs& a, bool* empty) {
+  *empty = false;
   if (a.head_dim != 64 && a.head_dim != 128) return LKV_ERR_UNSUPPORTED;
   if (a.num_kv_heads <= 0 || a.num_q_heads <= 0 || a.num_q_heads % a.num_kv_heads) return LKV_ERR_INVALID_ARGUMENT;
   const int group = a.num_q_heads / a.num_kv_heads;
   if (group != 1 && group != 2 && group != 4 && group != 8) return LKV_ERR_UNSUPPORTED;
   if (a.batch < 0 || a.total_q < 0 || a.max_q < 0 || a.max_pages_per_seq < 0) return LKV_ERR_INVALID_ARGUMENT;
-  if (a.batch == 0 || a.total_q == 0 || a.max_q == 0) return LKV_OK;
+  if (a.batch == 0 || a.total_q == 0 || a.max_q == 0) {
+    *empty = true;
+    return LKV_OK;
+  }
   const bool q8 = a.stage_k != nullptr;
   const bool pool = a.pool_k && a.pool_v && a.num_pages > 0;
   if (!a.q || (!pool && !q8) || !a.block_table || !a.seq_k || !a.cu_q || !a.out) return LKV_ERR_INVALID_ARGUMENT;
@@ -636,9 +642,33 @@ int prefill_paged(const PrefillArgs& a) {
     if (a.causal || S > kMaxKvSplits || (int64_t)a.batch * S > 65535) return LKV_ERR_UNSUPPORTED;
     if (!a.part_o || !a.part_lse || (reinterpret_cast<uintptr_t>(a.part_o) & 15)) return LKV_ERR_INVALID_ARGUMENT;
   }
+  return LKV_OK;
+}
+}  // namespace
+
+int prefill_paged_q8(const PrefillArgs& a, const void* codes, bool staged) {
+  bool empty;
+  const int st = check_args(a, &empty);
+  if (st != LKV_OK || empty) return st;
+  if (!a.stage_k) return LKV_ERR_INVALID_ARGUMENT;
+  if (!staged) {
+    const int rc = stage_pages(codes, a.q8_scales, a.q8_pages, a.block_table, a.block_table_stride, a.num_q8, a.seq_k,
+                               a.batch, a.max_pages_per_seq, a.stage_k, a.stage_v, a.stage_width, a.num_kv_heads,
+                               a.head_dim, a.error_word, static_cast<cudaStream_t>(a.stream));
+    if (rc != LKV_OK) return rc;
+  }
+  return prefill_paged(a);
+}
+
+int prefill_paged(const PrefillArgs& a) {
+  bool empty;
+  int st = check_args(a, &empty);
+  if (st != LKV_OK || empty) return st;
+  const int group = a.num_q_heads / a.num_kv_heads, S = a.kv_splits < 1 ? 1 : a.kv_splits;
+  const bool q8 = a.stage_k != nullptr, pool = a.pool_k && a.pool_v && a.num_pages > 0;
 
   CUtensorMap tq, tk, tv;
-  int st = make_query_tensor_map(&tq, a.q, a.total_q, a.q_stride_tok, a.num_q_heads, a.head_dim, group);
+  st = make_query_tensor_map(&tq, a.q, a.total_q, a.q_stride_tok, a.num_q_heads, a.head_dim, group);
   if (st != LKV_OK) return st;
   StageMaps stage;
   if (q8) {

@@ -1037,19 +1037,32 @@ def cp_combine(send, recv_ptrs, rank: int, world: int, state, rows: int, head_di
 # ------------------------------------------------------------------ 8-bit pages
 
 _I32, _I64, _BOOL = torch.int32, torch.int64, torch.bool
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _here(t, what: str) -> None:
-    """A call runs on the current device's stream, so its tensors have to be there."""
-    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+def _device_of(t, what: str) -> int:
+    """The current device, which a call's first tensor has to be on: it runs on that device's stream."""
+    dev = t.get_device()
+    if dev < 0 or dev != torch._C._cuda_getDevice():
         _fail(f"{what} must be on the current CUDA device, got {t.device}")
+    return dev
 
 
-def _ints(t, n: int, what: str) -> int:
-    """Address of at least n int32 on the device."""
-    if t.dtype != _I32 or t.numel() < n or not t.is_contiguous():
-        _fail(f"{what} must be contiguous CUDA int32 [>= {n}], got {t.dtype} {tuple(t.shape)}")
-    _here(t, what)
+def _ints(t, n: int, dev: int, what: str) -> int:
+    """Address of at least n int32 on the call's device."""
+    if t.dtype is not _I32 or t.numel() < n or not t.is_contiguous() or t.get_device() != dev:
+        _fail(f"{what} must be contiguous int32 [>= {n}] on the call's CUDA device, got {t.dtype} {tuple(t.shape)} on "
+              f"{t.device}")
+    return t.data_ptr()
+
+
+def _floats(t, n: int, dev: int, what: str):
+    """Address of n fp32 on the call's device, None for none."""
+    if t is None:
+        return None
+    if t.dtype is not _F32 or t.numel() != n or not t.is_contiguous() or t.get_device() != dev:
+        _fail(f"{what} must be contiguous fp32 of {n} values on the call's CUDA device, got {t.dtype} "
+              f"{tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
@@ -1106,28 +1119,41 @@ class PagesQ8(NamedTuple):
 
     def token_scales(self):
         """Views (k_scale, v_scale) [pages, 2, Hkv] of the scales."""
-        return self.scales[..., :2].transpose(1, 2), self.scales[..., 2:].transpose(1, 2)
+        s = self.scales
+        n, h, _ = s.shape
+        page, head, one = s.stride()
+        at = s.storage_offset()
+        return s.as_strided((n, 2, h), (page, one, head), at), s.as_strided((n, 2, h), (page, one, head), at + 2 * one)
 
 
-def _check_pages_q8(c) -> None:
+def _pages_q8(c, dev: int):
+    """(codes' address, scales' address, pages, Hkv, D) of checked 8-bit pages."""
     if type(c) is not PagesQ8:
         _fail("the 8-bit pages must be PagesQ8")
     codes, scales = c
-    if codes.dtype != _U8 or codes.dim() != 4 or codes.shape[2] != 2 or codes.shape[3] not in (1024, 2048) \
-            or not codes.is_contiguous():
-        _fail("PagesQ8.codes must be contiguous uint8 [pages, Hkv, 2, 16 * D] with D 64 or 128")
-    if scales.dtype != _F32 or scales.shape != (codes.shape[0], codes.shape[1], 4) or not scales.is_contiguous():
-        _fail("PagesQ8.scales must be contiguous fp32 [pages, Hkv, 4]")
-    _here(codes, "PagesQ8.codes")
-    _here(scales, "PagesQ8.scales")
+    n, h, two, last = codes.shape if codes.dim() == 4 else (0, 0, 0, 0)
+    if codes.dtype is not _U8 or two != 2 or (last != 2048 and last != 1024) or not codes.is_contiguous() \
+            or codes.get_device() != dev:
+        _fail("PagesQ8.codes must be contiguous uint8 [pages, Hkv, 2, 16 * D] with D 64 or 128 on the call's CUDA device")
+    if scales.dtype is not _F32 or scales.shape != (n, h, 4) or not scales.is_contiguous() \
+            or scales.get_device() != dev:
+        _fail("PagesQ8.scales must be contiguous fp32 [pages, Hkv, 4] on the call's CUDA device")
+    return codes.data_ptr(), scales.data_ptr(), n, h, last // PAGE_SIZE
 
 
-def _check_both(pool_k, pool_v, c) -> None:
-    _check_pool(pool_k, pool_v)
-    _here(pool_k, "pool_k")
-    _here(pool_v, "pool_v")
-    if pool_k.shape[2] != c.num_kv_heads or pool_k.shape[3] != c.head_dim:
-        _fail(f"pools of {pool_k.shape[2]} heads x {pool_k.shape[3]} against 8-bit pages of {c.num_kv_heads} x {c.head_dim}")
+def _pools(pool_k, pool_v, h: int, d: int, dev: int):
+    """(addresses of K and V, pages) of a checked bf16 pool of h heads, None for none."""
+    if pool_k is None and pool_v is None:
+        return None, None, 0
+    if pool_k is None or pool_v is None:
+        _fail("pool_k and pool_v come together")
+    shape = pool_k.shape
+    if pool_k.dtype is not _BF16 or pool_v.dtype is not _BF16 or pool_v.shape != shape \
+            or shape[1:] != (PAGE_SIZE, h, d) or not pool_k.is_contiguous() or not pool_v.is_contiguous() \
+            or pool_k.get_device() != dev or pool_v.get_device() != dev:
+        _fail(f"pools must be equal contiguous bf16 [pages, {PAGE_SIZE}, {h}, {d}] on the call's CUDA device (the heads "
+              f"of the 8-bit pages), got {pool_k.dtype} {tuple(shape)}")
+    return pool_k.data_ptr(), pool_v.data_ptr(), shape[0]
 
 
 @_traced
@@ -1135,16 +1161,15 @@ def quantize_pages(pool_k, pool_v, pages, cache: PagesQ8, out_pages, *, tokens=N
     """Pages ``pages[i]`` of a bf16 pool into 8-bit pages ``out_pages[i]`` (int32 [n] on the device;
     lkv_q8_quantize_pages).  ``tokens`` int32 [n]: how many tokens of each page count (the rest
     become zeros); None: 16.  No two ``out_pages`` may be the same."""
-    _check_pages_q8(cache)
-    _check_both(pool_k, pool_v, cache)
+    dev = _device_of(pool_k, "pool_k")
+    codes, scales, q8_pages, h, d = _pages_q8(cache, dev)
+    k, v, num = _pools(pool_k, pool_v, h, d, dev)
     n = pages.numel()
     if out_pages.numel() != n or (tokens is not None and tokens.numel() != n):
         _fail("pages, out_pages and tokens must have the same length")
     st = _capi.lib().lkv_q8_quantize_pages(
-        pool_k.data_ptr(), pool_v.data_ptr(), pool_k.shape[0], _ints(pages, n, "pages"),
-        None if tokens is None else _ints(tokens, n, "tokens"), cache.codes.data_ptr(), cache.scales.data_ptr(),
-        cache.num_pages, _ints(out_pages, n, "out_pages"), n, cache.num_kv_heads, cache.head_dim, _err_ptr(error_word),
-        _stream())
+        k, v, num, _ints(pages, n, dev, "pages"), None if tokens is None else _ints(tokens, n, dev, "tokens"), codes,
+        scales, q8_pages, _ints(out_pages, n, dev, "out_pages"), n, h, d, _err_ptr(error_word), _raw_stream(dev))
     if st:
         _capi.check(st, "lkv_q8_quantize_pages")
 
@@ -1152,58 +1177,58 @@ def quantize_pages(pool_k, pool_v, pages, cache: PagesQ8, out_pages, *, tokens=N
 @_traced
 def dequantize_pages(cache: PagesQ8, pages, pool_k, pool_v, out_pages, *, error_word=None) -> None:
     """8-bit pages ``pages[i]`` into pages ``out_pages[i]`` of a bf16 pool, bf16(code * scale)."""
-    _check_pages_q8(cache)
-    _check_both(pool_k, pool_v, cache)
+    dev = _device_of(pool_k, "pool_k")
+    codes, scales, q8_pages, h, d = _pages_q8(cache, dev)
+    k, v, num = _pools(pool_k, pool_v, h, d, dev)
     n = pages.numel()
     if out_pages.numel() != n:
         _fail("pages and out_pages must have the same length")
     st = _capi.lib().lkv_q8_dequantize_pages(
-        cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_pages, _ints(pages, n, "pages"), pool_k.data_ptr(),
-        pool_v.data_ptr(), pool_k.shape[0], _ints(out_pages, n, "out_pages"), n, cache.num_kv_heads, cache.head_dim,
-        _err_ptr(error_word), _stream())
+        codes, scales, q8_pages, _ints(pages, n, dev, "pages"), k, v, num, _ints(out_pages, n, dev, "out_pages"), n, h,
+        d, _err_ptr(error_word), _raw_stream(dev))
     if st:
         _capi.check(st, "lkv_q8_dequantize_pages")
 
 
-def _check_attend(q, cache, block_table, seq_k, num_q8, pool_k, pool_v, B, out, out_scale, lse, max_pages):
-    """What decode and prefill over 8-bit pages check alike; (width, out)."""
-    _check_pages_q8(cache)
-    if q.dim() != 3 or q.dtype != _BF16 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
-        _fail("q must be bf16 [rows, Hq, D] rows")
-    _here(q, "q")
-    T, Hq, D = q.shape
-    require_heads(Hq, cache.num_kv_heads, D)
-    if D != cache.head_dim:
-        _fail(f"head_dim {D} of q against {cache.head_dim} of the 8-bit pages")
-    if (pool_k is None) != (pool_v is None):
-        _fail("pool_k and pool_v come together")
-    if pool_k is not None:
-        _check_both(pool_k, pool_v, cache)
-    if block_table.dtype != _I32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.shape[0] < B:
-        _fail("block_table must be int32 [>= B, W] with unit column stride")
-    _here(block_table, "block_table")
-    W = block_table.shape[1] if max_pages is None else int(max_pages)
-    if not 0 <= W <= block_table.shape[1]:
-        _fail("max_pages exceeds block_table width")
+def _rows_hd(t, name: str, dev: int):
+    """(T, Hq, D, row stride) of bf16 rows of packed heads."""
+    if t.dim() != 3 or t.dtype is not _BF16 or t.get_device() != dev:
+        _fail(f"{name} must be bf16 [rows, Hq, D] on the call's CUDA device")
+    T, H, D = t.shape
+    row, head, one = t.stride()
+    if one != 1 or (head != D and H > 1):
+        _fail(f"{name} must be rows of packed heads")
+    return T, H, D, row if T > 1 else H * D
+
+
+def _attend_args(q, cache, block_table, seq_k, num_q8, pool_k, pool_v, B, out, out_scale, lse, max_pages):
+    """What decode and prefill over 8-bit pages check alike: the calls' arguments by their place."""
+    dev = _device_of(q, "q")
+    T, Hq, D, q_row = _rows_hd(q, "q", dev)
+    codes, scales, q8_pages, h, d = _pages_q8(cache, dev)
+    if D != d or Hq not in (h, 2 * h, 4 * h, 8 * h):
+        require_heads(Hq, h, D)
+        _fail(f"head_dim {D} of q against {d} of the 8-bit pages")
+    k, v, num = _pools(pool_k, pool_v, h, d, dev)
+    if block_table.dtype is not _I32 or block_table.dim() != 2 or block_table.stride(1) != 1 \
+            or block_table.shape[0] < B or block_table.get_device() != dev:
+        _fail("block_table must be int32 [>= B, W] with unit column stride on the call's CUDA device")
+    W = block_table.shape[1]
+    if max_pages is not None:
+        if not 0 <= max_pages <= W:
+            _fail("max_pages exceeds block_table width")
+        W = int(max_pages)
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=_BF16, device=q.device)
-    elif out.dtype != _BF16 or out.shape != (T, Hq, D) or out.stride(2) != 1 or out.stride(1) != D \
-            or (T > 1 and out.stride(0) < Hq * D):
-        _fail("out must be bf16 [rows, Hq, D] rows")
-    _here(out, "out")
-    if out_scale is not None:
-        if out_scale.dtype != _F32 or out_scale.numel() != Hq or not out_scale.is_contiguous():
-            _fail("out_scale must be fp32 [Hq]")
-        _here(out_scale, "out_scale")
-    if lse is not None:
-        if lse.dtype != _F32 or lse.numel() != T * Hq or not lse.is_contiguous():
-            _fail("lse must be contiguous fp32 [rows, Hq]")
-        _here(lse, "lse")
-    return W, out
-
-
-def _row_stride(t) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+        out, o_row = q.new_empty((T, Hq, D)), Hq * D
+    else:
+        if out.shape != (T, Hq, D):
+            _fail("out must be bf16 [rows, Hq, D] as q is")
+        o_row = _rows_hd(out, "out", dev)[3]
+        if T > 1 and o_row < Hq * D:
+            _fail("out's rows overlap")
+    return (dev, T, Hq, D, q_row, codes, scales, q8_pages, h, k, v, num, block_table.data_ptr(), block_table.stride(0),
+            None if num_q8 is None else _ints(num_q8, B, dev, "num_q8"), _ints(seq_k, B, dev, "seq_k"), W, out, o_row,
+            _floats(out_scale, Hq, dev, "out_scale"), _floats(lse, T * Hq, dev, "lse"))
 
 
 @_traced
@@ -1217,18 +1242,17 @@ def decode_paged_q8(q, cache: PagesQ8, block_table, seq_k, *, num_q8=None, pool_
     seq_k int32 [B].  Returns out [B, Hq, D] bf16.  ``lse`` (fp32 [B, Hq]) receives the log-sum-exp.
     Calls that overlap need a workspace each.
     """
-    B, Hq, D = q.shape if q.dim() == 3 else _fail("q must be bf16 [rows, Hq, D] rows")
-    W, out = _check_attend(q, cache, block_table, seq_k, num_q8, pool_k, pool_v, B, out, out_scale, lse, max_pages)
+    (dev, B, Hq, D, q_row, codes, scales, q8_pages, h, k, v, num, table, t_row, nq8, seq, W, out, o_row, f,
+     l) = _attend_args(q, cache, block_table, seq_k, num_q8, pool_k, pool_v, q.shape[0], out, out_scale, lse, max_pages)
     if workspace is None:
         workspace = Workspace.for_decode(B, Hq, D, W, device=q.device)
-    _here(workspace.buf, "workspace")
+    buf = workspace.buf
+    if buf.get_device() != dev:
+        _fail(f"workspace must be on the call's CUDA device, got {buf.device}")
     st = _capi.lib().lkv_decode_paged_q8(
-        q.data_ptr(), _row_stride(q), cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_pages, _ptr(pool_k),
-        _ptr(pool_v), 0 if pool_k is None else pool_k.shape[0], block_table.data_ptr(), block_table.stride(0),
-        None if num_q8 is None else _ints(num_q8, B, "num_q8"), _ints(seq_k, B, "seq_k"), out.data_ptr(),
-        _row_stride(out), _ptr(lse), _ptr(out_scale), B, Hq, cache.num_kv_heads, D, W,
-        D ** -0.5 if softmax_scale is None else float(softmax_scale), workspace.ptr(), workspace.nbytes,
-        DECODE_L2_KEEP if l2_keep else 0, _stream())
+        q.data_ptr(), q_row, codes, scales, q8_pages, k, v, num, table, t_row, nq8, seq, out.data_ptr(), o_row, l, f, B,
+        Hq, h, D, W, D ** -0.5 if softmax_scale is None else softmax_scale, buf.data_ptr(), workspace.nbytes,
+        DECODE_L2_KEEP if l2_keep else 0, _raw_stream(dev))
     if st:
         _capi.check(st, "lkv_decode_paged_q8")
     return out
@@ -1259,43 +1283,37 @@ def prefill_paged_q8(q, cache: PagesQ8, block_table, seq_k, cu_q, max_q: int, *,
     """``prefill_paged`` over a cache whose older pages are in 8 bits (lkv_prefill_paged_q8).
 
     The arguments of ``prefill_paged``, with the pages as in ``decode_paged_q8``.  The 8-bit pages'
-    codes are first copied to ``stage`` as bf16 (lkv_q8_stage_pages); ``staged=True`` says that an
+    codes are first copied to ``stage`` as bf16; ``staged=True`` says that an
     earlier call with the same rows and pages did that (the layers of one step), and skips it.
     A row may have at most ``stage.width`` 8-bit pages.
     """
     B = cu_q.numel() - 1
     if B < 0:
         _fail("cu_q must be int32 [B + 1]")
-    W, out = _check_attend(q, cache, block_table, seq_k, num_q8, pool_k, pool_v, B, out, out_scale, lse, max_pages)
-    T, Hq, D = q.shape
+    (dev, T, Hq, D, q_row, codes, scales, q8_pages, h, k, v, num, table, t_row, nq8, seq, W, out, o_row, f,
+     l) = _attend_args(q, cache, block_table, seq_k, num_q8, pool_k, pool_v, B, out, out_scale, lse, max_pages)
     if stage is None:
         if staged:
             _fail("staged=True needs the stage of the earlier call")
-        stage = StageQ8.empty(B, W, cache.num_kv_heads, D, device=q.device)
-    _check_both(stage.k, stage.v, cache)
-    width = min(stage.width, W)
-    if stage.width < 1 or stage.k.shape[0] < B * stage.width:
-        _fail(f"the stage holds {stage.k.shape[0]} pages, {B} rows of {stage.width} were asked for")
-    args = (block_table.data_ptr(), block_table.stride(0), None if num_q8 is None else _ints(num_q8, B, "num_q8"),
-            _ints(seq_k, B, "seq_k"))
-    err, cu = _err_ptr(error_word), _ints(cu_q, B + 1, "cu_q")
-    if not staged:
-        st = _capi.lib().lkv_q8_stage_pages(
-            cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_pages, *args, B, W, stage.k.data_ptr(),
-            stage.v.data_ptr(), width, cache.num_kv_heads, D, err, _stream())
-        if st:
-            _capi.check(st, "lkv_q8_stage_pages")
+        stage = StageQ8.empty(B, W, h, D, device=q.device)
+    sk, sv, pages = _pools(stage.k, stage.v, h, D, dev)
+    if stage.width < 1 or pages < B * stage.width:
+        _fail(f"the stage holds {pages} pages, {B} rows of {stage.width} were asked for")
     st = _capi.lib().lkv_prefill_paged_q8(
-        q.data_ptr(), _row_stride(q), stage.k.data_ptr(), stage.v.data_ptr(), max(width, 1), cache.scales.data_ptr(),
-        cache.num_pages, _ptr(pool_k), _ptr(pool_v), 0 if pool_k is None else pool_k.shape[0], *args, cu,
-        out.data_ptr(), _row_stride(out), _ptr(lse), _ptr(out_scale), B, T, int(max_q), Hq, cache.num_kv_heads, D, W,
-        int(bool(causal)), D ** -0.5 if softmax_scale is None else float(softmax_scale), err, _stream())
+        q.data_ptr(), q_row, codes, scales, q8_pages, sk, sv, max(min(stage.width, W), 1), int(staged), k, v, num, table,
+        t_row, nq8, seq, _ints(cu_q, B + 1, dev, "cu_q"), out.data_ptr(), o_row, l, f, B, T, int(max_q), Hq, h, D, W,
+        int(bool(causal)), D ** -0.5 if softmax_scale is None else softmax_scale, _err_ptr(error_word),
+        _raw_stream(dev))
     if st:
         _capi.check(st, "lkv_prefill_paged_q8")
     return out
 
 
 # ------------------------------------------------------------------ beam search
+
+
+_PTRS = [ctypes.c_void_p * n for n in range(9)]
+_SIZES = [ctypes.c_int64 * n for n in range(9)]
 
 
 @_traced
@@ -1313,16 +1331,16 @@ def reorder_pages(pools, src_pages, dst_pages, *, layers: int = 1, layer_stride:
         _fail("src_pages and dst_pages must have the same length")
     if not 1 <= len(pools) <= 8:
         _fail(f"reorder_pages takes 1 to 8 pools, got {len(pools)}")
-    for t in pools:
-        if t.dim() < 1 or not t.is_contiguous():
-            _fail("pools must be contiguous, the page their first dimension")
-        _here(t, "a pool")
-    sizes = [t[0].numel() * t.element_size() if t.shape[0] else 0 for t in pools]
-    N = len(pools)
+    dev, N = _device_of(pools[0], "a pool"), len(pools)
+    ptrs, sizes, counts = _PTRS[N](), _SIZES[N](), _SIZES[N]()
+    for i, t in enumerate(pools):
+        if t.dim() < 1 or not t.is_contiguous() or t.get_device() != dev:
+            _fail("pools must be contiguous on the call's CUDA device, the page their first dimension")
+        ptrs[i], counts[i] = t.data_ptr(), t.shape[0]
+        sizes[i] = t.nbytes // t.shape[0] if t.shape[0] else 0
     st = _capi.lib().lkv_reorder_pages(
-        (ctypes.c_void_p * N)(*(t.data_ptr() for t in pools)), (ctypes.c_int64 * N)(*sizes),
-        (ctypes.c_int64 * N)(*(t.shape[0] for t in pools)), N, _ints(src_pages, n, "src_pages"),
-        _ints(dst_pages, n, "dst_pages"), n, int(layers), int(layer_stride), _err_ptr(error_word), _stream())
+        ptrs, sizes, counts, N, _ints(src_pages, n, dev, "src_pages"), _ints(dst_pages, n, dev, "dst_pages"), n,
+        layers, layer_stride, _err_ptr(error_word), _raw_stream(dev))
     if st:
         _capi.check(st, "lkv_reorder_pages")
 
@@ -1340,6 +1358,11 @@ class BeamChoice(NamedTuple):
         return cls(*(torch.empty((batch, select), dtype=t, device=device) for t in (_F32, _I64, _I64, _BOOL)))
 
 
+@functools.lru_cache(maxsize=None)
+def _beam_row_bytes(select: int) -> int:
+    return _capi.lib().lkv_beam_workspace_bytes(1, select)
+
+
 @_traced
 def beam_select(logits, scores, *, select: int | None = None, finished=None, eos_token: int | None = None,
                 out: BeamChoice | None = None) -> BeamChoice:
@@ -1350,36 +1373,41 @@ def beam_select(logits, scores, *, select: int | None = None, finished=None, eos
     and token.  ``finished`` bool [B, K]: such a beam continues with ``eos_token`` alone, at its score.
     ``out``: buffers to write (a captured step's).
     """
-    if scores.dtype != _F32 or scores.dim() != 2 or not scores.is_contiguous():
+    if scores.dtype is not _F32 or scores.dim() != 2 or not scores.is_contiguous():
         _fail("scores must be contiguous CUDA fp32 [B, K]")
-    _here(scores, "scores")
+    dev = _device_of(scores, "scores")
     B, K = scores.shape
-    if logits.dtype not in (_BF16, _F32) or logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[0] != B * K:
-        _fail(f"logits must be bf16 or fp32 [{B * K}, V] rows")
-    _here(logits, "logits")
-    n = K if select is None else int(select)
-    if not (1 <= n <= 32 and n <= logits.shape[1] and 1 <= K <= 64 and B * K <= 65535):
+    if logits.dim() != 2 or logits.dtype is not _BF16 and logits.dtype is not _F32 or logits.get_device() != dev:
+        _fail("logits must be bf16 or fp32 [B * K, V] rows on the call's CUDA device")
+    rows, V = logits.shape
+    row, one = logits.stride()
+    if rows != B * K or (one != 1 and V > 1):
+        _fail(f"logits must be [{B * K}, V] rows with unit column stride, got {tuple(logits.shape)}")
+    n = K if select is None else select
+    if not (1 <= n <= 32 and n <= V and 1 <= K <= 64 and rows <= 65535):
         _fail(f"beam_select takes 1 to 32 candidates of at least as many tokens, 1 to 64 beams and 65535 rows, got "
               f"select {n}, {K} beams, {tuple(logits.shape)}")
-    eos = -1 if eos_token is None else int(eos_token)
+    eos, done = -1 if eos_token is None else eos_token, None
     if finished is not None:
-        if finished.dtype != _BOOL or finished.shape != (B, K) or not finished.is_contiguous():
-            _fail(f"finished must be contiguous bool [{B}, {K}]")
-        _here(finished, "finished")
-        if not 0 <= eos < logits.shape[1]:
+        if finished.dtype is not _BOOL or finished.shape != (B, K) or not finished.is_contiguous() \
+                or finished.get_device() != dev:
+            _fail(f"finished must be contiguous bool [{B}, {K}] on the call's CUDA device")
+        if not 0 <= eos < V:
             _fail("finished beams need an eos_token of the vocabulary")
+        done = finished.data_ptr()
     if out is None:
-        out = BeamChoice.empty(B, n, scores.device)
-    for t, like in zip(out, (_F32, _I64, _I64, _BOOL)):
-        if t.dtype != like or t.shape != (B, n) or not t.is_contiguous():
-            _fail(f"out must be a BeamChoice of contiguous [{B}, {n}] tensors")
-        _here(t, "out")
-    nbytes = _capi.lib().lkv_beam_workspace_bytes(B * K, n)
-    work = torch.empty(nbytes, dtype=_U8, device=scores.device)
+        ids = scores.new_empty((2, B, n), dtype=_I64)
+        out = BeamChoice(scores.new_empty((B, n)), *ids.unbind(0), scores.new_empty((B, n), dtype=_BOOL))
+    else:
+        for t, like in zip(out, (_F32, _I64, _I64, _BOOL)):
+            if t.dtype is not like or t.shape != (B, n) or not t.is_contiguous() or t.get_device() != dev:
+                _fail(f"out must be a BeamChoice of contiguous [{B}, {n}] tensors on the call's CUDA device")
+    nbytes = rows * _beam_row_bytes(n)
+    work = scores.new_empty(nbytes, dtype=_U8)
     st = _capi.lib().lkv_beam_select(
-        logits.data_ptr(), logits.stride(0), int(logits.dtype == _F32), scores.data_ptr(), _ptr(finished), eos, B, K,
-        logits.shape[1], n, out.scores.data_ptr(), out.rows.data_ptr(), out.tokens.data_ptr(), out.finished.data_ptr(),
-        work.data_ptr(), nbytes, _stream())
+        logits.data_ptr(), row, logits.dtype is _F32, scores.data_ptr(), done, eos, B, K, V, n,
+        out.scores.data_ptr(), out.rows.data_ptr(), out.tokens.data_ptr(), out.finished.data_ptr(), work.data_ptr(),
+        nbytes, _raw_stream(dev))
     if st:
         _capi.check(st, "lkv_beam_select")
     return out

@@ -93,10 +93,6 @@ def test_page_calls_check_their_arguments_on_the_host():
     assert back(a, a, 4, a, a, a, 4, a, 1, 300, 64, None, None) == 1
     assert back(a, a + 4, 4, a, a, a, 4, a, 1, 2, 64, None, None) == 1
     assert back(a, a, 4, None, a, a, 4, None, 0, 2, 64, None, None) == 0
-    stage = lib.lkv_q8_stage_pages
-    assert stage(a, a, 4, a, 2, None, a, 1, 2, a, a, 3, 2, 64, None, None) == 1  # wider than the table
-    assert stage(a, a, 4, None, 2, None, a, 1, 2, a, a, 2, 2, 64, None, None) == 1
-    assert stage(a, a, 4, a, 2, None, a, 0, 2, a, a, 2, 2, 64, None, None) == 0
     pools, sizes, counts = (ctypes.c_void_p * 1)(a), (ctypes.c_int64 * 1)(64), (ctypes.c_int64 * 1)(4)
     move = lib.lkv_reorder_pages
     assert move(pools, sizes, counts, 0, a, a, 1, 1, 0, None, None) == 1
@@ -126,12 +122,14 @@ def test_attention_calls_check_their_arguments_on_the_host():
     assert decode(width=-1) == 1 and decode(batch=-1) == 1
     assert decode(batch=0) == 0
 
-    def prefill(stage=a, width=2, scales=a, q=a, q_row=256, batch=1, total=1, d=64, hq=4):
-        return lib.lkv_prefill_paged_q8(q, q_row, stage, stage, width, scales, 4, None, None, 0, a, 2, None, a, a, a,
-                                        256, None, None, batch, total, 1, hq, 2, d, 2, 1, 1.0, None, None)
+    def prefill(stage=a, width=2, codes=a, scales=a, q=a, q_row=256, batch=1, total=1, d=64, hq=4, staged=0):
+        return lib.lkv_prefill_paged_q8(q, q_row, codes, scales, 4, stage, stage, width, staged, None, None, 0, a, 2,
+                                        None, a, a, a, 256, None, None, batch, total, 1, hq, 2, d, 2, 1, 1.0, None,
+                                        None)
 
     assert prefill(d=96) == 2 and prefill(hq=6) == 2
     assert prefill(stage=None) == 1 and prefill(width=0) == 1 and prefill(scales=None) == 1
+    assert prefill(codes=None) == 1 and prefill(codes=a + 8) == 1 and prefill(width=3) == 1  # wider than the table
     assert prefill(q=a + 4) == 1 and prefill(q_row=252) == 1
     assert prefill(batch=0) == 0 and prefill(total=0) == 0
 
