@@ -605,7 +605,10 @@ int lkv_decode_paged_q8(const void* q, int64_t q_stride_tok, const uint8_t* code
  * num_kv_heads, head_dim], whose contents need not be kept; staged = 1: an earlier call with
  * the same rows and pages did that (layers that read the same older pages) and the
  * call reads the copy.  A row with more 8-bit pages than stage_width is recorded in
- * error_word (may be NULL), its further ones read as zeros. */
+ * error_word (may be NULL), its further ones read as zeros.
+ * kv_splits > 1 (at most 8; lkv_prefill_q8_split_plan gives a good number): as for
+ * lkv_prefill_paged_split, with part_o fp32 [kv_splits, total_q * num_q_heads, head_dim] and
+ * part_lse fp32 [kv_splits, total_q * num_q_heads]; causal calls take it too. */
 int lkv_prefill_paged_q8(const void* q, int64_t q_stride_tok, const uint8_t* codes, const float* scales,
                          int64_t q8_pages, void* stage_k, void* stage_v, int stage_width, int staged,
                          const void* pool_k, const void* pool_v, int64_t num_pages, const int32_t* block_table,
@@ -613,7 +616,9 @@ int lkv_prefill_paged_q8(const void* q, int64_t q_stride_tok, const uint8_t* cod
                          const int32_t* cu_seqlens_q, void* out, int64_t out_stride_tok, float* lse,
                          const float* out_scale, int batch, int total_q, int max_q, int num_q_heads,
                          int num_kv_heads, int head_dim, int max_pages_per_seq, int causal, float softmax_scale,
-                         int32_t* error_word, void* stream);
+                         int kv_splits, float* part_o, float* part_lse, int32_t* error_word, void* stream);
+int lkv_prefill_q8_split_plan(int batch, int max_q, int total_q, int num_q_heads, int num_kv_heads, int head_dim,
+                              int max_pages_per_seq, int* kv_splits);
 
 /* ------------------------------------------------------------------ beam search
  * lkv_reorder_pages: page dst_pages[i] = page src_pages[i] for all i < n <= 2048 at once (the

@@ -65,7 +65,8 @@ _SIGNATURES = {
     "lkv_q8_quantize_pages": (I32, [P, P, I64, P, P, P, P, I64, P, I64, I32, I32, P, P]),
     "lkv_q8_dequantize_pages": (I32, [P, P, I64, P, P, P, I64, P, I64, I32, I32, P, P]),
     "lkv_prefill_paged_q8": (I32, [P, I64, P, P, I64, P, P, I32, I32, P, P, I64, P, I64, P, P, P, P, I64, P, P,
-                                   I32, I32, I32, I32, I32, I32, I32, I32, F32, P, P]),
+                                   I32, I32, I32, I32, I32, I32, I32, I32, F32, I32, P, P, P, P]),
+    "lkv_prefill_q8_split_plan": (I32, [I32, I32, I32, I32, I32, I32, I32, P]),
     "lkv_decode_paged_q8": (I32, [P, I64, P, P, I64, P, P, I64, P, I64, P, P, P, I64, P, P,
                                   I32, I32, I32, I32, I32, F32, P, SZ, I32, P]),
     "lkv_reorder_pages": (I32, [P, P, P, I32, P, P, I32, I32, I64, P, P]),

@@ -619,7 +619,7 @@ int lkv_prefill_paged_q8(const void* q, int64_t q_stride_tok, const uint8_t* cod
                          const int32_t* cu_seqlens_q, void* out, int64_t out_stride_tok, float* lse,
                          const float* out_scale, int batch, int total_q, int max_q, int num_q_heads,
                          int num_kv_heads, int head_dim, int max_pages_per_seq, int causal, float softmax_scale,
-                         int32_t* error_word, void* stream) {
+                         int kv_splits, float* part_o, float* part_lse, int32_t* error_word, void* stream) {
   lkv::PrefillArgs a{};
   a.q = q;
   a.q_stride_tok = q_stride_tok;
@@ -651,7 +651,16 @@ int lkv_prefill_paged_q8(const void* q, int64_t q_stride_tok, const uint8_t* cod
   a.num_q8 = num_q8;
   a.q8_scales = scales;
   a.q8_pages = q8_pages;
+  a.kv_splits = kv_splits;
+  a.part_o = part_o;
+  a.part_lse = part_lse;
   return lkv::prefill_paged_q8(a, codes, staged != 0);
+}
+
+int lkv_prefill_q8_split_plan(int batch, int max_q, int total_q, int num_q_heads, int num_kv_heads, int head_dim,
+                              int max_pages_per_seq, int* kv_splits) {
+  return lkv::prefill_q8_split_plan(batch, max_q, total_q, num_q_heads, num_kv_heads, head_dim, max_pages_per_seq,
+                                    kv_splits);
 }
 
 int lkv_decode_paged_q8(const void* q, int64_t q_stride_tok, const uint8_t* codes, const float* scales,

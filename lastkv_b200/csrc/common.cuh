@@ -288,6 +288,13 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
+// log2 on the SFU (lg2.approx.ftz.f32).
+__device__ __forceinline__ float lg2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // max(a, b, c) in one instruction (sm_100 three-input max.f32).
 __device__ __forceinline__ float fmax3f(float a, float b, float c) {
   float d;

@@ -128,12 +128,6 @@ __device__ __forceinline__ void async_copy_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-__device__ __forceinline__ float lg2_approx(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Value scales below this count as this in the weights (codes of zero, or products that no sum of others
 // would keep): its reciprocal is finite.
 constexpr float kMinValueScale = 8.6736174e-19f;  // 2^-60

@@ -57,6 +57,8 @@ struct PrefillArgs {
 int prefill_paged(const PrefillArgs& a);
 // With 8-bit pages: stages their codes first, unless that is done.
 int prefill_paged_q8(const PrefillArgs& a, const void* codes, bool staged);
+int prefill_q8_split_plan(int batch, int max_q, int total_q, int num_q_heads, int num_kv_heads, int head_dim,
+                          int max_pages, int* kv_splits);
 int prefill_split_plan(int batch, int max_q, int num_q_heads, int num_kv_heads, int head_dim, int max_pages,
                        int causal, int* kv_splits);
 

@@ -369,26 +369,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     const float sl2 = p.scale_log2;
     float* group_scale = reinterpret_cast<float*>(smem + Cfg::OFF_SCALE) + warp * 48;  // Q8
-    // Q8: lane 4 i + c has scale c (keys 0-7, 8-15, values 0-7, 8-15) of page i of a block, read a block ahead
-    auto scale_of = [&](int j) {
+    const float4* gs4 = reinterpret_cast<const float4*>(group_scale);
+    // Q8: lane 4 i + c has scale c (keys 0-7, 8-15, values 0-7, 8-15) of page i of a block.  It is read a block
+    // ahead, and the page's id two, so that neither is waited for.
+    auto page_of = [&](int j) {
       const int pi = (j0 + j) * kPagesPerBlock + (lane >> 2);
-      if (j >= nb || pi >= nh || pi >= p.stage_width) return 1.f;
-      const int pid = btrow[pi];
-      if (pid < 0 || (int64_t)pid >= p.q8_pages) return 1.f;
-      return __ldg(p.q8_scales + ((int64_t)pid * p.Hkv + hk) * 4 + (lane & 3));
+      return j < nb && pi < nh && pi < p.stage_width ? btrow[pi] : -1;
     };
-    float next_scale = Q8 ? scale_of(0) : 1.f;
+    auto scale_of = [&](int pid) {
+      return pid >= 0 && (int64_t)pid < p.q8_pages
+                 ? __ldg(p.q8_scales + ((int64_t)pid * p.Hkv + hk) * 4 + (lane & 3)) : 1.f;
+    };
+    float next_scale = Q8 ? scale_of(page_of(0)) : 1.f;
+    int next_page = Q8 ? page_of(1) : 0;
     // Wait results are made warp-uniform: tcgen05.ld/st below are warp-collective.
     for (int j = 0; j < nb; ++j) {
       if constexpr (Q8) {
         float f = next_scale;
-        next_scale = scale_of(j + 1);
+        next_scale = scale_of(next_page);
+        next_page = page_of(j + 2);
         if (!(fabsf(f) < INFINITY)) f = 1.f;  // the staged keys are NaN there
         const int at = (lane >> 2) * 2 + (lane & 1);
         if (lane & 2) {
           f = fmaxf(f, kMinValueScale);
-          group_scale[16 + at] = log2f(f);
-          group_scale[32 + at] = 1.f / f;
+          group_scale[16 + at] = lg2_approx(f);
+          group_scale[32 + at] = __fdividef(1.f, f);
         } else {
           group_scale[at] = fmaxf(f, 1e-37f) * sl2;  // codes of zero: not -inf * 0 where they are masked
         }
@@ -417,14 +422,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       float mx;
       if constexpr (Q8) {
-        float gm[16];
+        float gm[4];
 #pragma unroll
-        for (int g = 0; g < 16; ++g) {
-          const float* y = x + 8 * g;
-          gm[g] = fmaxf(fmax3f(fmax3f(y[0], y[1], y[2]), y[3], y[4]), fmax3f(y[5], y[6], y[7])) * group_scale[g];
+        for (int c = 0; c < 4; ++c) {
+          const float4 kf = gs4[c];
+          auto top8 = [&x](int e) {
+            return fmaxf(fmax3f(fmax3f(x[e], x[e + 1], x[e + 2]), x[e + 3], x[e + 4]), fmax3f(x[e + 5], x[e + 6], x[e + 7]));
+          };
+          gm[c] = fmaxf(fmax3f(top8(32 * c) * kf.x, top8(32 * c + 8) * kf.y, top8(32 * c + 16) * kf.z),
+                        top8(32 * c + 24) * kf.w);
         }
-#pragma unroll
-        for (int g = 0; g < 4; ++g) gm[g] = fmaxf(fmax3f(gm[g], gm[g + 4], gm[g + 8]), gm[g + 12]);
         mx = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
       } else {
       // 8 independent partial maxima (short dependency chains, three-input max), then a tree
@@ -454,9 +461,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = 0; c < kBN / 32; ++c) {
         uint32_t pc[16];
         if constexpr (Q8) {
+          const float4 kf4 = gs4[c], lv4 = gs4[4 + c], iv4 = gs4[8 + c];
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const float kf = group_scale[4 * c + g], add = group_scale[16 + 4 * c + g] + neg_mref;
+            const float kf = (&kf4.x)[g], add = (&lv4.x)[g] + neg_mref;
             const float2 kfv = make_float2(kf, kf), addv = make_float2(add, add);
             float2 gs = make_float2(0.f, 0.f);
 #pragma unroll
@@ -467,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               gs = __fadd2_rn(gs, pv);
               pc[g * 4 + q] = pack_bf16(pv.x, pv.y);
             }
-            const float inv = group_scale[32 + 4 * c + g];
+            const float inv = (&iv4.x)[g];
             sp[g] = __ffma2_rn(gs, make_float2(inv, inv), sp[g]);
           }
         } else {
@@ -630,7 +638,7 @@ int check_args(const PrefillArgs& a, bool* empty) {
   const bool pool = a.pool_k && a.pool_v && a.num_pages > 0;
   if (!a.q || (!pool && !q8) || !a.block_table || !a.seq_k || !a.cu_q || !a.out) return LKV_ERR_INVALID_ARGUMENT;
   if (q8 && (!a.stage_v || !a.q8_scales || a.stage_width < 1 || (int64_t)a.stage_width * a.batch >= INT32_MAX ||
-             a.q8_pages < 0 || a.kv_splits > 1))
+             a.q8_pages < 0))
     return LKV_ERR_INVALID_ARGUMENT;
   if ((reinterpret_cast<uintptr_t>(a.q) & 15) || ((a.q_stride_tok * 2) & 15)) return LKV_ERR_INVALID_ARGUMENT;
   if ((reinterpret_cast<uintptr_t>(a.out) & 15) || ((a.out_stride_tok * 2) & 15)) return LKV_ERR_INVALID_ARGUMENT;
@@ -638,8 +646,9 @@ int check_args(const PrefillArgs& a, bool* empty) {
   if (!a.error_word && !q8) return LKV_ERR_INVALID_ARGUMENT;
   const int S = a.kv_splits < 1 ? 1 : a.kv_splits;
   if (S > 1) {
-    // key splits need a non-causal call (every query sees the same key range)
-    if (a.causal || S > kMaxKvSplits || (int64_t)a.batch * S > 65535) return LKV_ERR_UNSUPPORTED;
+    // key splits need a non-causal call (every query sees the same key range); with 8-bit pages, where the
+    // older keys are most of a span's, causal ones take them too
+    if ((a.causal && !q8) || S > kMaxKvSplits || (int64_t)a.batch * S > 65535) return LKV_ERR_UNSUPPORTED;
     if (!a.part_o || !a.part_lse || (reinterpret_cast<uintptr_t>(a.part_o) & 15)) return LKV_ERR_INVALID_ARGUMENT;
   }
   return LKV_OK;
@@ -749,6 +758,40 @@ int prefill_paged(const PrefillArgs& a) {
   return merge_partials(a.part_o, a.part_lse, S, prm.part_rows, a.head_dim, a.num_q_heads,
                         prm.part_rows * a.head_dim, prm.part_rows, a.out_scale, a.out, a.lse, stream,
                         a.out_stride_tok);
+}
+
+// Key splits of a call over 8-bit pages, causal or not: what the waves of CTAs take, in blocks (about 1.5 us), with
+// the start and end of a CTA as 2.5 of them, and the merge launch as as many, besides the partials' way through memory.
+// Short spans gain from them, long ones lose (us at 1 / 2 / 3 / 4 / 6 / 8 splits): one row of 8 tokens over 8192 keys
+// 105 / 61 / 46 / 38 / 31 / 27; four of 128 over 2048 42 / 35 / 29 / 27 / 34 / 33; two of 1024 over 8192 235 / 287 /
+// 304 / 306 / 347 / 394.
+int prefill_q8_split_plan(int batch, int max_q, int total_q, int num_q_heads, int num_kv_heads, int head_dim,
+                          int max_pages, int* kv_splits) {
+  if (!kv_splits) return LKV_ERR_INVALID_ARGUMENT;
+  *kv_splits = 1;
+  if (num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads) return LKV_ERR_INVALID_ARGUMENT;
+  if (head_dim != 64 && head_dim != 128) return LKV_ERR_UNSUPPORTED;
+  if (batch <= 0 || max_q <= 0 || max_pages <= 0) return LKV_OK;
+  const int group = num_q_heads / num_kv_heads;
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
+    return LKV_ERR_CUDA;
+  const int64_t tok_per_cta = (int64_t)kTiles * kBM / group;
+  const int64_t ctas = (max_q + tok_per_cta - 1) / tok_per_cta * num_kv_heads * batch;
+  const int64_t blocks = ((int64_t)max_pages * kPageTok + kBN - 1) / kBN;
+  const double split_us = 2.0 * total_q * num_q_heads * head_dim * 4 / 5e6;  // a partial written and read
+  double best = 1e30;
+  for (int s = 1; s <= kMaxKvSplits; ++s) {
+    if (s > 1 && (s > blocks || (int64_t)batch * s > 65535)) break;
+    const double waves = (double)((ctas * s + sms - 1) / sms);
+    const double cost = waves * ((double)((blocks + s - 1) / s) + 2.5) + (s > 1 ? 2.5 + s * split_us / 1.5 : 0.0);
+    if (cost < best - 1e-9) {
+      best = cost;
+      *kv_splits = s;
+    }
+  }
+  return LKV_OK;
 }
 
 // Key splits for a non-causal call: with one CTA per SM, a grid of C CTAs runs

@@ -1275,17 +1275,27 @@ class StageQ8(NamedTuple):
         return cls(k, v, width)
 
 
+@functools.lru_cache(maxsize=4096)
+def _q8_splits(dev: int, batch: int, max_q: int, total_q: int, hq: int, hkv: int, d: int, width: int) -> int:
+    """Key splits of a call of this size on device `dev` (lkv_prefill_q8_split_plan)."""
+    s = ctypes.c_int(1)
+    _capi.check(_capi.lib().lkv_prefill_q8_split_plan(batch, max_q, total_q, hq, hkv, d, width, ctypes.byref(s)),
+                "lkv_prefill_q8_split_plan")
+    return s.value
+
+
 @_traced
 def prefill_paged_q8(q, cache: PagesQ8, block_table, seq_k, cu_q, max_q: int, *, num_q8=None, pool_k=None,
                      pool_v=None, causal=True, softmax_scale=None, out=None, lse=None, out_scale=None,
                      stage: StageQ8 | None = None, staged: bool = False, error_word=None,
-                     max_pages: int | None = None):
+                     max_pages: int | None = None, kv_splits: int | None = None, partials=None):
     """``prefill_paged`` over a cache whose older pages are in 8 bits (lkv_prefill_paged_q8).
 
     The arguments of ``prefill_paged``, with the pages as in ``decode_paged_q8``.  The 8-bit pages'
     codes are first copied to ``stage`` as bf16; ``staged=True`` says that an
     earlier call with the same rows and pages did that (the layers of one step), and skips it.
-    A row may have at most ``stage.width`` 8-bit pages.
+    A row may have at most ``stage.width`` 8-bit pages.  ``kv_splits`` and ``partials`` as for
+    ``prefill_paged`` (causal calls may split their keys too).
     """
     B = cu_q.numel() - 1
     if B < 0:
@@ -1299,11 +1309,24 @@ def prefill_paged_q8(q, cache: PagesQ8, block_table, seq_k, cu_q, max_q: int, *,
     sk, sv, pages = _pools(stage.k, stage.v, h, D, dev)
     if stage.width < 1 or pages < B * stage.width:
         _fail(f"the stage holds {pages} pages, {B} rows of {stage.width} were asked for")
+    if kv_splits is None:
+        kv_splits = _q8_splits(dev, B, int(max_q), T, Hq, h, D, W)
+    part_o = part_lse = None
+    if kv_splits > 1:
+        if partials is None:
+            partials = (q.new_empty((kv_splits, T * Hq, D), dtype=_F32), q.new_empty((kv_splits, T * Hq), dtype=_F32))
+        o, e = partials
+        if o.dtype is not _F32 or o.dim() != 3 or o.shape[0] < kv_splits or o.shape[1:] != (T * Hq, D) \
+                or not o.is_contiguous() or o.get_device() != dev or e.dtype is not _F32 or e.dim() != 2 \
+                or e.shape[0] < kv_splits or e.shape[1] != T * Hq or not e.is_contiguous() or e.get_device() != dev:
+            _fail(f"partials must be contiguous fp32 [>= {kv_splits}, {T * Hq}, {D}] and [>= {kv_splits}, {T * Hq}] on the "
+                  "call's CUDA device")
+        part_o, part_lse = o.data_ptr(), e.data_ptr()
     st = _capi.lib().lkv_prefill_paged_q8(
         q.data_ptr(), q_row, codes, scales, q8_pages, sk, sv, max(min(stage.width, W), 1), int(staged), k, v, num, table,
         t_row, nq8, seq, _ints(cu_q, B + 1, dev, "cu_q"), out.data_ptr(), o_row, l, f, B, T, int(max_q), Hq, h, D, W,
-        int(bool(causal)), D ** -0.5 if softmax_scale is None else softmax_scale, _err_ptr(error_word),
-        _raw_stream(dev))
+        int(bool(causal)), D ** -0.5 if softmax_scale is None else softmax_scale, kv_splits, part_o, part_lse,
+        _err_ptr(error_word), _raw_stream(dev))
     if st:
         _capi.check(st, "lkv_prefill_paged_q8")
     return out

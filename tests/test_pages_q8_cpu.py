@@ -122,15 +122,16 @@ def test_attention_calls_check_their_arguments_on_the_host():
     assert decode(width=-1) == 1 and decode(batch=-1) == 1
     assert decode(batch=0) == 0
 
-    def prefill(stage=a, width=2, codes=a, scales=a, q=a, q_row=256, batch=1, total=1, d=64, hq=4, staged=0):
+    def prefill(stage=a, width=2, codes=a, scales=a, q=a, q_row=256, batch=1, total=1, d=64, hq=4, staged=0, splits=1):
         return lib.lkv_prefill_paged_q8(q, q_row, codes, scales, 4, stage, stage, width, staged, None, None, 0, a, 2,
-                                        None, a, a, a, 256, None, None, batch, total, 1, hq, 2, d, 2, 1, 1.0, None,
-                                        None)
+                                        None, a, a, a, 256, None, None, batch, total, 1, hq, 2, d, 2, 1, 1.0, splits, None,
+                                        None, None, None)
 
     assert prefill(d=96) == 2 and prefill(hq=6) == 2
     assert prefill(stage=None) == 1 and prefill(width=0) == 1 and prefill(scales=None) == 1
     assert prefill(codes=None) == 1 and prefill(codes=a + 8) == 1 and prefill(width=3) == 1  # wider than the table
     assert prefill(q=a + 4) == 1 and prefill(q_row=252) == 1
+    assert prefill(splits=2) == 1 and prefill(splits=9) == 2  # no partials; too many
     assert prefill(batch=0) == 0 and prefill(total=0) == 0
 
 

@@ -76,6 +76,21 @@ def test_stage_shared_by_calls_and_wider_than_needed():
     assert torch.equal(a, _run(t, q, cu, stage=narrow))
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("splits", [2, 3, 8])
+def test_splits_of_the_keys(causal, splits):
+    """Splits that end inside both kinds of pages, splits without a key that a token sees, rows of a single block."""
+    t, q, cu = _case(13, [700, 40, 333, 1], [130, 40, 300, 1], [30, 1, 4, 0], 4, 2, 64)
+    lse = torch.empty((471, 4), dtype=torch.float32, device="cuda")
+    one = torch.empty_like(lse)
+    out = _run(t, q, cu, causal=causal, kv_splits=splits, lse=lse)
+    _check(t, q, cu, out, causal)
+    _run(t, q, cu, causal=causal, kv_splits=1, lse=one)
+    assert float((lse - one).abs().max()) <= 4 * POLY  # both have their weights' errors
+    work = torch.empty((9, 471 * 4, 64), device="cuda"), torch.empty((9, 471 * 4), device="cuda")
+    assert torch.equal(out, _run(t, q, cu, causal=causal, kv_splits=splits, partials=work))
+
+
 def test_a_row_with_more_pages_than_the_stage_is_reported():
     t, q, cu = _case(7, [400, 90], [64, 10], [20, 3], 4, 2, 64)
     err = torch.zeros(4, dtype=torch.int32, device="cuda")
@@ -143,6 +158,10 @@ def test_refusals():
         _run(t, q, cu, stage=ops.StageQ8.empty(1, 3, 2, 64)._replace(width=4))
     with pytest.raises(Refused, match="heads"):
         _run(t, q, cu, stage=ops.StageQ8.empty(1, 3, 1, 64))
+    with pytest.raises(Refused, match="partials"):
+        _run(t, q, cu, kv_splits=2, partials=(torch.empty((2, 40, 64), device="cuda"), torch.empty(2, 39, device="cuda")))
+    with pytest.raises(Refused, match="unsupported"):
+        _run(t, q, cu, kv_splits=9)
     with pytest.raises(Refused, match="cu_q"):
         _run(t, q, cu.long())
     with pytest.raises(Refused, match="together"):
