@@ -42,16 +42,41 @@ struct QuantParams {
   int* err;
 };
 
-// One warp per (page, head, keys or values).  Rows are loaded whole (16 bytes a lane), rounded in
-// registers, and put into the kernels' order through a byte tile in shared memory: rows of D + 16
-// bytes, so that neither the 8-byte stores nor the reads in operand order meet bank conflicts.
+// A lane holds two rows (tokens 2p and 2p + 1) of one 16-column tile, so that every 4-byte word of the
+// operand order is made in registers: 8 words per row pair, one of each of 4 column pairs x 2 rows for
+// keys, of 8 columns for values.  They reach the order of memory through shared memory, word (tile t,
+// row half h, g, c) at the place below: 16-byte vectors of (t & 1, h), which lane 4g + c reads.  The
+// gaps and exclusive ors keep a warp's stores of one word on 32 banks.
 template <int D>
-__global__ void __launch_bounds__(kWarps * 32) quantise_pages_kernel(const QuantParams p) {
-  constexpr int PITCH = D + 16;
-  constexpr int LANES = D / 8;       // lanes per row
-  constexpr int STEP = 32 / LANES;   // rows per load
-  constexpr int LOADS = 16 / STEP;   // the first half of them holds tokens 0-7
-  __shared__ __align__(16) uint8_t tile_all[kWarps][16 * PITCH];
+struct Words {
+  static constexpr int TILES = D / 16;
+  static constexpr int PAIRS = 32 / TILES;  // row pairs per pass over the lanes
+  static constexpr int PASSES = 8 / PAIRS;
+  static constexpr int COUNT = D / 32 * 144;
+  __device__ static int vector(int t2, int g, int c) { return t2 * 144 + g * 16 + ((c ^ (g >> 1)) * 4); }
+  __device__ static int at(int t, int h, int g, int c) {
+    return vector(t >> 1, g, c) + (((t & 1) * 2 + h) ^ (t >> 2));
+  }
+};
+
+__device__ __forceinline__ uint32_t abs_max2(uint32_t a, uint32_t b) {  // |bf16| pairs, NaN stays
+  uint32_t d;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a & 0x7fff7fffu), "r"(b & 0x7fff7fffu));
+  return d;
+}
+
+__device__ __forceinline__ void load_tile_row(uint32_t (&v)[8], const __nv_bfloat16* at) {
+  const uint4 a = __ldg(reinterpret_cast<const uint4*>(at)), b = __ldg(reinterpret_cast<const uint4*>(at) + 1);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+
+// One warp per (page, head, keys or values).  4096 pages of 8 heads of 128 (403 MB moved): 65-67 us, 6.0-6.2 TB/s,
+// so HBM bounds it; a byte tile in shared memory and bf16 maxima one by one were issue-bound at 85.
+// 64 wide: 41 us, 5.0 TB/s (a warp has 2 KB to read there, and starts and ends cost as much).
+template <int D>
+__global__ void __launch_bounds__(kWarps * 32, 8) quantise_pages_kernel(const QuantParams p) {
+  using W = Words<D>;
+  __shared__ __align__(16) uint32_t words_all[kWarps][W::COUNT];
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -67,76 +92,83 @@ __global__ void __launch_bounds__(kWarps * 32) quantise_pages_kernel(const Quant
   const int valid = p.tokens ? min(max(p.tokens[n], 0), kPageTokens) : kPageTokens;
   const __nv_bfloat16* base = (which ? p.pool[1] : p.pool[0]) + (src * kPageTokens * p.hkv + hk) * D;
   const int64_t row_stride = (int64_t)p.hkv * D;
-  const int r0 = lane / LANES, col = (lane % LANES) * 8;
-  uint4 v[LOADS];
+  const int t = lane % W::TILES, pair0 = lane / W::TILES;
+  uint32_t v[W::PASSES][2][8];
 #pragma unroll
-  for (int i = 0; i < LOADS; ++i) {
-    const int r = i * STEP + r0;
-    v[i] = r < valid ? __ldcs(reinterpret_cast<const uint4*>(base + r * row_stride + col)) : make_uint4(0, 0, 0, 0);
-  }
-  uint8_t* tile = tile_all[warp];
-  float scale[2];
+  for (int i = 0; i < W::PASSES; ++i)
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float amax = 0.f;
+    for (int e = 0; e < 2; ++e) {
+      const int r = 2 * (i * W::PAIRS + pair0) + e;
+      if (r < valid) {
+        load_tile_row(v[i][e], base + r * row_stride + t * 16);
+      } else {
 #pragma unroll
-    for (int i = h * LOADS / 2; i < (h + 1) * LOADS / 2; ++i) {
-      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) amax = max_nan(amax, max_nan(fabsf(bf16_lo(w[e])), fabsf(bf16_hi(w[e]))));
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    scale[h] = amax / 127.0f;
-    const bool zero = !(amax < INFINITY) || scale[h] == 0.f;
-    // one division per block: x * (127 / max), rounded by the addition that puts q + 128 into the low
-    // byte of 1.5 * 2^23 + 128 + q; where the reciprocal would overflow, x / s
-    const bool tiny = amax < 1e-30f;
-    const float inv = tiny ? 0.f : 127.0f / amax;
-#pragma unroll
-    for (int i = h * LOADS / 2; i < (h + 1) * LOADS / 2; ++i) {
-      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-      uint32_t q[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float a = bf16_lo(w[e]), b = bf16_hi(w[e]);
-        if (!tiny) {
-          q[2 * e] = __float_as_uint(fmaf(a, inv, 12583040.0f));
-          q[2 * e + 1] = __float_as_uint(fmaf(b, inv, 12583040.0f));
-        } else {
-          q[2 * e] = (uint32_t)(128 + max(-127, min(127, __float2int_rn(a / scale[h]))));
-          q[2 * e + 1] = (uint32_t)(128 + max(-127, min(127, __float2int_rn(b / scale[h]))));
-        }
+        for (int x = 0; x < 8; ++x) v[i][e][x] = 0;
       }
-      uint2 packed;
-      packed.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
-      packed.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
-      if (zero) packed = make_uint2(0x80808080u, 0x80808080u);
-      *reinterpret_cast<uint2*>(tile + (i * STEP + r0) * PITCH + col) = packed;
+    }
+  uint32_t* words = words_all[warp];
+  float scales[W::PASSES];
+#pragma unroll
+  for (int i = 0; i < W::PASSES; ++i) {
+    const int pair = i * W::PAIRS + pair0, h = pair >> 2, c0 = pair & 3;
+    uint32_t m2 = 0;
+#pragma unroll
+    for (int x = 0; x < 16; ++x) m2 = abs_max2(m2, v[i][x >> 3][x & 7]);
+#pragma unroll
+    for (int o = 2 * W::TILES; o > 0; o >>= 1) m2 = abs_max2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
+    const float amax = max_nan(bf16_lo(m2), bf16_hi(m2));
+    const float scale = amax / 127.0f;
+    scales[i] = scale;
+    // one division per block: x * (127 / max), rounded by the addition that puts q + 128 into the low
+    // byte of 1.5 * 2^23 + 128 + q
+    float inv = 127.0f / amax;
+    if (!(amax >= 1e-30f && amax < INFINITY)) {  // the reciprocal overflows: times 2^96 on both sides; or all zeros
+      const bool zero = !(amax < INFINITY) || scale == 0.f;
+      inv = zero ? 0.f : 1.0f / (scale * 0x1p96f);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const uint32_t w = v[i][e][x];
+          v[i][e][x] = zero ? 0u : pack_bf16(bf16_lo(w) * 0x1p96f, bf16_hi(w) * 0x1p96f);
+        }
+    }
+    auto codes = [&](uint32_t w) {
+      return __ffma2_rn(make_float2(bf16_lo(w), bf16_hi(w)), make_float2(inv, inv),
+                        make_float2(12583040.0f, 12583040.0f));
+    };
+    auto word = [](float a, float b, float c, float d) {
+      return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040),
+                         __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
+    };
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {  // columns 2x, 2x + 1, 2x + 8 and 2x + 9
+      const float2 a0 = codes(v[i][0][x]), a8 = codes(v[i][0][x + 4]);
+      const float2 b0 = codes(v[i][1][x]), b8 = codes(v[i][1][x + 4]);
+      if (which == 0) {
+        words[W::at(t, h, 2 * c0, x)] = word(a0.x, a8.x, a0.y, a8.y);
+        words[W::at(t, h, 2 * c0 + 1, x)] = word(b0.x, b8.x, b0.y, b8.y);
+      } else {
+        words[W::at(t, h, 2 * x, c0)] = word(a0.x, a8.x, b0.x, b8.x);
+        words[W::at(t, h, 2 * x + 1, c0)] = word(a0.y, a8.y, b0.y, b8.y);
+      }
     }
   }
   __syncwarp();
   const int64_t block = dst * p.hkv + hk;
-  const int g = lane >> 2, c = lane & 3;
   uint8_t* out = p.codes + (block * 2 + which) * 16 * D;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) {
-    uint32_t w[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int t = 2 * i + (x >> 1), h = x & 1;  // 16-column tile, row half
-      if (which == 0) {
-        const uint8_t* at = tile + (8 * h + g) * PITCH + 16 * t + 2 * c;
-        w[x] = __byte_perm(*reinterpret_cast<const uint16_t*>(at), *reinterpret_cast<const uint16_t*>(at + 8), 0x5140);
-      } else {
-        const uint8_t* at = tile + (8 * h + 2 * c) * PITCH + 16 * t + g;
-        w[x] = (uint32_t)at[0] | (uint32_t)at[8] << 8 | (uint32_t)at[PITCH] << 16 | (uint32_t)at[PITCH + 8] << 24;
-      }
-    }
-    *reinterpret_cast<uint4*>(out + i * 512 + lane * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    uint4 w = *reinterpret_cast<const uint4*>(words + W::vector(i, lane >> 2, lane & 3));
+    if (i & 2) w = make_uint4(w.y, w.x, w.w, w.z);
+    *reinterpret_cast<uint4*>(out + i * 512 + lane * 16) = w;
   }
-  if (lane == 0)
-    *reinterpret_cast<float2*>(p.scales + block * kScalesPerBlock + 2 * which) = make_float2(scale[0], scale[1]);
+  if constexpr (W::PASSES == 2) {
+    if (lane == 0)
+      *reinterpret_cast<float2*>(p.scales + block * kScalesPerBlock + 2 * which) = make_float2(scales[0], scales[1]);
+  } else {
+    if (lane % 16 == 0) p.scales[block * kScalesPerBlock + 2 * which + lane / 16] = scales[0];
+  }
 }
 
 struct DequantParams {
@@ -159,7 +191,10 @@ struct DequantParams {
   int batch, W, width;
 };
 
-// Back to rows of bf16, one warp per (page, head, keys or values): the inverse of the above.
+// Back to rows of bf16, one warp per (page, head, keys or values), through a byte tile in shared memory:
+// rows of D + 16 bytes, so that whole 16-byte pieces of a row are written (words made in registers as
+// above, which would write rows in pieces of half a sector, took 9.4 us where this takes 8.0).  4096 pages
+// of 8 heads of 128: 67 us, 6.0 TB/s; 64 wide: 37 us, 5.4 TB/s.
 // STAGE: the codes themselves (the prefill kernel applies the scales); where a scale is not finite
 // the keys are NaN, so that the tokens' scores are, and the values zero.
 template <int D, bool STAGE>
