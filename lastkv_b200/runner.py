@@ -72,6 +72,7 @@ class GraphDecodeRunner:
                     "pos": torch.zeros((1, 1), dtype=torch.int64).pin_memory(),
                     "done": None} for _ in range(self.NSETS)]
         self._set = 0
+        self._captured = None  # the cache's memory that the graphs read and write
         self.graph = None
         self.graph_commit = None  # the step after a chunk boundary (bf16 caches)
         self.alpha = model.model.blend_alpha(cache.dtype)
@@ -175,6 +176,7 @@ class GraphDecodeRunner:
         and for bf16 caches the same step with a boundary commit fused into layer 0's append."""
         cache = self.cache
         cache.flush_commit()
+        self._captured = cache.pool_k, cache.q8, self.W
         state = (self.ids, self.scores, self.finished) if self.beams is not None else (self.ids,)
         saved = [t.clone() for t in state]
 
@@ -227,6 +229,9 @@ class GraphDecodeRunner:
         if self.graph is None:
             raise RMarinBackendContractError("capture() must run before step()")
         cache = self.cache
+        pool, q8, width = self._captured
+        if cache.pool_k is not pool or cache.q8 is not q8 or cache.pages_per_seq + cache.ring_pages != width:
+            raise RMarinBackendContractError("the cache has grown since the step was captured")
         if self.plan is not None:
             cache.unshare_()  # the device plan's rows have pages of their own
         pending = cache.take_commit()

@@ -218,6 +218,26 @@ def test_device_planned_steps_after_a_reorder():
     assert torch.equal(runs[0], runs[1])
 
 
+@pytest.mark.parametrize("history", [None, "int8"])
+def test_a_captured_step_is_refused_after_the_cache_has_grown(history):
+    """The graphs hold the addresses of the memory that they were captured over."""
+    model = _model(torch.bfloat16)
+    cache = model.new_cache(2, 100, history=history)
+    runner = GraphDecodeRunner(model, cache)
+    with torch.no_grad():
+        runner.prefill(_prompt(2, 40), 64)
+        runner.capture()
+        first = runner.step().clone()
+        cache.reserve(110)  # the same number of pages
+        with pytest.raises(Refused, match="grown"):
+            runner.step()
+        again = GraphDecodeRunner(model, cache)
+        again.ids.copy_(first)
+        again.capture()
+        again.step()
+    cache.check_errors()
+
+
 def test_refused_calls():
     model = _model(torch.bfloat16)
     cache = model.new_cache(4, 64, history="int8")
