@@ -128,9 +128,9 @@ __device__ __forceinline__ void async_copy_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// Value scales below this count as this in the weights (codes of zero, or products that no sum of others
-// would keep): its reciprocal is finite.
-constexpr float kMinValueScale = 8.6736174e-19f;  // 2^-60
+// Value scales below this count as this: the sum of weights, times their reciprocals, stays finite for
+// rows of 2^20 keys and more (2^15 * 2^90 * 2^20).
+constexpr float kMinValueScale = 8.0779357e-28f;  // 2^-90
 constexpr float kWeightLog2 = 15.f;               // weights of the products are times 2^15
 
 // The slots of row b.

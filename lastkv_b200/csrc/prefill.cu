@@ -111,9 +111,9 @@ struct PrefillParams {
   int has_pool;
 };
 
-// Value scales below this are taken as this in the weights (their codes are then zero, or the
-// products below 2^-53 of anything else): 1 / v stays finite.
-constexpr float kMinValueScale = 8.6736174e-19f;  // 2^-60
+// Value scales below this are taken as this in the weights: the sum of weights, times their reciprocals,
+// stays finite for rows of 2^20 keys and more.
+constexpr float kMinValueScale = 8.0779357e-28f;  // 2^-90
 
 template <int D>
 struct PrefillCfg {

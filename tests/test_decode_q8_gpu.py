@@ -141,6 +141,17 @@ def test_large_scores_and_zero_blocks():
     _check(t, q, out)
 
 
+@pytest.mark.parametrize("lens", [[300, 90], [9000, 20]])
+@pytest.mark.parametrize("power", [-80, 90])
+def test_values_of_any_size(lens, power):
+    """Scales from 2^-90 up: the weights carry them, the sum of weights does not."""
+    t = random_cache(27, lens, [10000, 10000], 2, 128)
+    t["vs"] *= 2.0 ** power
+    q = _q(8, 2, 4, 128)
+    out = ops.decode_paged_q8(q, _cache(t), t["table"], t["seq_k"], num_q8=t["num_q8"])
+    _check(t, q, out)
+
+
 def test_pages_that_are_not_there_read_as_zeros():
     hkv, d = 2, 128
     t = random_cache(19, [100, 100], [4, 4], hkv, d)

@@ -131,6 +131,13 @@ def test_zero_scales_and_scales_far_apart():
     _check(t, q, cu, _run(t, q, cu))
 
 
+@pytest.mark.parametrize("power", [-80, 90])
+def test_values_of_any_size(power):
+    t, q, cu = _case(13, [700, 90], [70, 20], [99, 99], 4, 2, 128)
+    t["vs"] *= 2.0 ** power
+    _check(t, q, cu, _run(t, q, cu))
+
+
 def test_strides_lse_and_scales():
     t, q0, cu = _case(11, [90, 33], [50, 33], [4, 1], 8, 4, 64)
     wide = torch.zeros((83, 2, 8, 64), dtype=torch.bfloat16, device="cuda")
