@@ -20,11 +20,14 @@
 //   beam_merge   A CTA per batch item joins each row's stretches two by two, then the rows: lists are
 //                sorted, so a candidate's rank is its place in its own list and a binary search in the other.
 //
-// Bound by HBM for many rows and by two launches for few.
+// Bound by HBM for many rows and by the latencies of two launches, a CTA's few steps over its stretch and the join's
+// rounds for few: 4 rows of 128256 bf16 logits take 8.7 us, 128 rows of 50001 in fp32 (25.6 MB) 22, 512 of
+// 32000 in bf16 (32.8 MB) 25.
 
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -261,7 +264,6 @@ struct MergeParams {
   int64_t V, eos;
   int K, select, stretches;
   int log_n, log_lists, log_beams;  // select, stretches and beams, rounded up to powers of two
-  int rows_per_pass;     // rows whose keys fit in shared memory at once
   float* out_scores;
   int64_t* out_rows;
   int64_t* out_tokens;
@@ -319,7 +321,7 @@ __device__ __forceinline__ void merge_rounds(uint64_t*& from, uint64_t*& to, uin
 }
 
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const MergeParams p) {
-  // [rows_per_pass][1 << log_lists][1 << log_n], padded with zeros, then as much again for half as many lists
+  // [K][1 << log_lists][1 << log_n], padded with zeros, then as much again for half as many lists
   extern __shared__ uint64_t keys[];
   // A total is (x - top) + norm: the maximum is taken off first, so that rows of values like a type's
   // lowest keep their sums' logarithms and their scores.  norm NaN: every total of the row is -inf.
@@ -336,68 +338,61 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const MergePa
   auto sums_at = [&](int k, int s) { return k < K && s < S ? __ldcg(p.sums + ((int64_t)b * K + k) * S + s) : none; };
   float2 a = sums_at(tid >> 5, lane), c = sums_at(tid >> 5, lane + 32);  // a warp per row, two stretches per lane
   for (int i = tid; i < 1 << (p.log_beams + log_n); i += kMergeThreads) total[i] = 0;
-  for (int k0 = 0; k0 < K; k0 += p.rows_per_pass) {
-    const int rows = min(p.rows_per_pass, K - k0);
-    const uint64_t* in = p.keys + ((int64_t)b * K + k0) * S * n;
-    uint64_t* from = keys;
-    uint64_t* to = keys + ((int64_t)p.rows_per_pass << (p.log_lists + log_n));
-    uint32_t* unused = nullptr;
-    __syncthreads();
-    const int entries = rows << (p.log_lists + log_n);
-    for (int i0 = tid; i0 < entries; i0 += 8 * kMergeThreads) {  // eight loads in flight
-      uint64_t k[8];
+  const int entries = K << (p.log_lists + log_n);
+  const uint64_t* in = p.keys + (int64_t)b * K * S * n;
+  uint64_t* lists = keys;
+  uint64_t* lists_to = keys + entries;
+  uint32_t* unused = nullptr;
+  for (int i0 = tid; i0 < entries; i0 += 8 * kMergeThreads) {  // eight loads in flight
+    uint64_t k[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = i0 + j * kMergeThreads;
-        const int at = i & (pad - 1), list = i >> log_n, s = list & ((1 << p.log_lists) - 1), r = list >> p.log_lists;
-        const bool there = i < entries && at < n && s < S;
-        k[j] = __ldcg(in + (there ? (r * S + s) * n + at : 0));
-        if (!there) k[j] = 0;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (i0 + j * kMergeThreads < entries) from[i0 + j * kMergeThreads] = k[j];
+    for (int j = 0; j < 8; ++j) {
+      const int i = i0 + j * kMergeThreads;
+      const int at = i & (pad - 1), list = i >> log_n, s = list & ((1 << p.log_lists) - 1), r = list >> p.log_lists;
+      const bool there = i < entries && at < n && s < S;
+      k[j] = __ldcg(in + (there ? (r * S + s) * n + at : 0));
+      if (!there) k[j] = 0;
     }
-    if (k0 == 0) {
-      for (int k = tid >> 5; k < K; k += kMergeThreads / 32) {
-        const int64_t row = (int64_t)b * K + k;
-        float top = fmaxf(a.x, c.x);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        // a stretch of -inf alone adds 0, or a NaN
-        auto part = [top](float2 ms) {
-          return ms.x == -INFINITY || ms.x == top ? (double)ms.y : (double)(ms.y * ex2_approx((ms.x - top) * kLog2e));
-        };
-        double sum = part(a) + part(c);
+    for (int j = 0; j < 8; ++j)
+      if (i0 + j * kMergeThreads < entries) lists[i0 + j * kMergeThreads] = k[j];
+  }
+  for (int k = tid >> 5; k < K; k += kMergeThreads / 32) {
+    const int64_t row = (int64_t)b * K + k;
+    float top = fmaxf(a.x, c.x);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) {
-          const bool done = p.finished && p.finished[row];
-          // log(f 2^e) = e log 2 + log f with f in 1 .. 2, whose logarithm fp32 has to 2^-24
-          const int e = ilogb(sum);
-          const double score = (double)p.scores[row];
-          const double rest = done ? 0.0 : e * 0.6931471805599453 + (double)logf((float)scalbn(sum, -e));
-          tops[k] = done ? 0.0 : (double)top;
-          norm[k] = fabs(score) < INFINITY && fabs(tops[k]) < INFINITY && fabs(rest) < INFINITY ? score - rest : NAN;
-        }
-        a = sums_at(k + kMergeThreads / 32, lane);
-        c = sums_at(k + kMergeThreads / 32, lane + 32);
-      }
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // a stretch of -inf alone adds 0, or a NaN
+    auto part = [top](float2 ms) {
+      return ms.x == -INFINITY || ms.x == top ? (double)ms.y : (double)(ms.y * ex2_approx((ms.x - top) * kLog2e));
+    };
+    double sum = part(a) + part(c);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) {
+      const bool done = p.finished && p.finished[row];
+      // log(f 2^e) = e log 2 + log f with f in 1 .. 2, whose logarithm fp32 has to 2^-24
+      const int e = ilogb(sum);
+      const double score = (double)p.scores[row];
+      const double rest = done ? 0.0 : e * 0.6931471805599453 + (double)logf((float)scalbn(sum, -e));
+      tops[k] = done ? 0.0 : (double)top;
+      norm[k] = fabs(score) < INFINITY && fabs(tops[k]) < INFINITY && fabs(rest) < INFINITY ? score - rest : NAN;
     }
-    __syncthreads();
-    merge_rounds<false>(from, to, unused, unused, rows, p.log_lists, log_n);
-    for (int i = tid; i < rows << log_n; i += kMergeThreads) {
-      const int k = k0 + (i >> log_n), rank = i & (pad - 1);
-      if (rank >= n) continue;
-      const uint64_t key = from[i];
-      const double t = ((double)from_ordered((uint32_t)(key >> 32)) - tops[k]) + norm[k];
-      const bool alive = norm[k] == norm[k];
-      // all totals of a row without a finite score or sum are -inf: its first tokens, in their order
-      const int at = (k << log_n) + rank;
-      total[at] = ordered(alive && t == t ? t : -INFINITY);
-      from_where[at] = (uint32_t)at;
-      token[k * n + rank] = alive ? 0xffffffffu - (uint32_t)key : (uint32_t)rank;
-    }
+    a = sums_at(k + kMergeThreads / 32, lane);
+    c = sums_at(k + kMergeThreads / 32, lane + 32);
+  }
+  __syncthreads();
+  merge_rounds<false>(lists, lists_to, unused, unused, K, p.log_lists, log_n);
+  for (int i = tid; i < K << log_n; i += kMergeThreads) {
+    const int k = i >> log_n, rank = i & (pad - 1);
+    if (rank >= n) continue;
+    const uint64_t key = lists[i];
+    const double t = ((double)from_ordered((uint32_t)(key >> 32)) - tops[k]) + norm[k];
+    const bool alive = norm[k] == norm[k];
+    // all totals of a row without a finite score or sum are -inf: its first tokens, in their order
+    total[i] = ordered(alive && t == t ? t : -INFINITY);
+    from_where[i] = (uint32_t)i;
+    token[k * n + rank] = alive ? 0xffffffffu - (uint32_t)key : (uint32_t)rank;
   }
   __syncthreads();
   uint64_t* from = total;
@@ -419,15 +414,22 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const MergePa
 struct Split {
   int stretches, pieces;
 };
-// Stretches for about three CTAs per SM over all rows, of two pieces for each warp at least.
-Split split_rows(int64_t rows, int64_t V, int elem, int sms) {
+constexpr int kMergeSmem = 128 * 1024;
+// What the join holds of a row: `lists` lists of 1 << log_n keys, and half as many of the next round.
+int64_t join_bytes(int64_t lists, int log_n) { return ((3 * lists << log_n) / 2 + 1) * (int64_t)sizeof(uint64_t); }
+
+// Stretches for four CTAs per SM over all rows, all at once (16 items of 8 beams over 50001 tokens: 22.0 us, with
+// three 23.6, with six 25.8), of two pieces for each warp at least, and no more than the join can hold of
+// all beams at once (16 beams over 200000 tokens, the 32 best:
+// 33 us; in several passes 42 to 66).
+Split split_rows(int64_t rows, int beams, int log_n, int64_t V, int elem, int sms) {
   const int64_t piece = kThreads * 16 / elem, pieces = (V + 16 / elem - 1 + piece - 1) / piece;
-  const int64_t s = std::min<int64_t>({(pieces + 1) / 2, (int64_t)kMaxStretches, std::max<int64_t>(1, 3ll * sms / rows)});
+  int64_t most = kMaxStretches;
+  while (most > 1 && beams * join_bytes(most, log_n) > kMergeSmem) most /= 2;
+  const int64_t s = std::min<int64_t>({(pieces + 1) / 2, most, std::max<int64_t>(1, 4ll * sms / rows)});
   const int64_t per = (pieces + s - 1) / s;
   return {(int)((pieces + per - 1) / per), (int)per};
 }
-
-constexpr int kMergeSmem = 128 * 1024;
 
 }  // namespace
 
@@ -453,7 +455,9 @@ int beam_select(const void* logits, int64_t row_stride, int fp32, const float* s
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return LKV_ERR_CUDA;
-  const Split sp = split_rows(rows, vocab, fp32 ? 4 : 2, sms);
+  MergeParams m{};
+  while (1 << m.log_n < select) ++m.log_n;
+  const Split sp = split_rows(rows, beams, m.log_n, vocab, fp32 ? 4 : 2, sms);
   const size_t entries = (size_t)rows * sp.stretches;
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
       workspace_bytes < entries * (select * sizeof(uint64_t) + sizeof(float2)))
@@ -472,7 +476,6 @@ int beam_select(const void* logits, int64_t row_stride, int fp32, const float* s
   const dim3 grid((unsigned)sp.stretches, (unsigned)rows);
   const auto kern = fp32 ? beam_rows_kernel<float> : beam_rows_kernel<__nv_bfloat16>;
   if (launch_pdl(kern, grid, dim3(kThreads), 0, stream, r) != cudaSuccess) return LKV_ERR_CUDA;
-  MergeParams m{};
   m.keys = r.keys;
   m.sums = r.sums;
   m.scores = scores;
@@ -486,13 +489,10 @@ int beam_select(const void* logits, int64_t row_stride, int fp32, const float* s
   m.out_rows = out_rows;
   m.out_tokens = out_tokens;
   m.out_finished = out_finished;
-  while (1 << m.log_n < select) ++m.log_n;
   while (1 << m.log_lists < sp.stretches) ++m.log_lists;
   while (1 << m.log_beams < beams) ++m.log_beams;
-  const int row_bytes = (3 << (m.log_n + m.log_lists)) / 2 * (int)sizeof(uint64_t) + (int)sizeof(uint64_t);  // 24 KB at most
-  m.rows_per_pass = std::min(beams, kMergeSmem / row_bytes);
-  const int smem = m.rows_per_pass * row_bytes;
-  static bool attr_done[64] = {false};
+  const int64_t smem = beams * join_bytes(1ll << m.log_lists, m.log_n);  // kMergeSmem at most (split_rows)
+  static std::atomic<bool> attr_done[64];
   if (dev >= 0 && dev < 64 && !attr_done[dev]) {
     if (cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMergeSmem) != cudaSuccess)
       return LKV_ERR_CUDA;
