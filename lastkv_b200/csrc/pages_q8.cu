@@ -5,7 +5,7 @@
 //               zeros, so its values are NaN.  Tokens past the page's count are zeros and do not
 //               count for the scale.
 //   dequantise  bf16(q * s), or (staging for the prefill kernel) the codes themselves, which are
-//               whole numbers up to 127 and exact in bf16.
+//               whole numbers up to 127 and exact in bf16 (keys) and f16 (values).
 //   reorder     pages[dst[i]] = pages[src[i]] for all i at once, in several pools and layers.
 // All three read and write each byte once and are bound by HBM.
 
@@ -195,7 +195,7 @@ struct DequantParams {
 // rows of D + 16 bytes, so that whole 16-byte pieces of a row are written (words made in registers as
 // above, which would write rows in pieces of half a sector, took 9.4 us where this takes 8.0).  4096 pages
 // of 8 heads of 128: 67 us, 6.0 TB/s; 64 wide: 37 us, 5.4 TB/s.
-// STAGE: the codes themselves (the prefill kernel applies the scales); where a scale is not finite
+// STAGE: the codes themselves, keys in bf16 and values in f16 (the prefill kernel applies the scales); where a scale is not finite
 // the keys are NaN, so that the tokens' scores are, and the values zero.
 template <int D, bool STAGE>
 __global__ void __launch_bounds__(kWarps * 32) dequantise_pages_kernel(const DequantParams p) {
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kWarps * 32) dequantise_pages_kernel(const Deq
       const uint32_t two = w >> ((e & 1) * 16);
       const float a = (float)((int)(two & 255u) - 128), b = (float)((int)(two >> 8 & 255u) - 128);
       if constexpr (STAGE) {
-        o[e] = which == 0 && (r < 8 ? bad0 : bad1) ? 0x7fff7fffu : pack_bf16(a, b);
+        o[e] = which ? pack_f16(a, b) : (r < 8 ? bad0 : bad1) ? 0x7fff7fffu : pack_bf16(a, b);
       } else {
         const float sc = r < 8 ? s0 : s1;
         o[e] = pack_bf16(a * sc, b * sc);

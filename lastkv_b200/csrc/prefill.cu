@@ -46,12 +46,20 @@
 // SFU, and stores P in 32-key chunks as they are ready.
 //
 // Older pages in 8 bits (Q8): a row's first num_q8 pages come from a staged copy of their int8
-// codes as bf16 (dequantise_pages_kernel: whole numbers up to 127, exact), so the MMAs run as they
-// do on bf16 pages, and the scales, one for every 8 keys, are applied in fp32 in the softmax.  A
-// key scale k multiplies a group's scores: it goes into the maximum once per group and into the
-// FFMA in front of the exponential.  A value scale v multiplies the weights that PV takes,
-// p v = 2^(s - m + log2 v): it goes into that FFMA's addend, and a group's sum of them times 1 / v is
-// its part of the row's sum.  No instruction per key is added.  Pages in bf16 have scales of one.
+// codes (dequantise_pages_kernel: whole numbers up to 127, exact in bf16 and f16), and the scales, one for
+// every 8 keys, are applied in fp32 in the softmax.  A key scale k multiplies a group's scores: it goes into
+// the maximum once per group and into the FFMA in front of the exponential.  A value scale v multiplies the
+// weights that PV takes, p v = 2^(s + log2 v - m): it goes into that FFMA's addend (and into the maximum, so
+// that f16 holds them), and a group's sum of them times 1 / v is its part of the row's sum.  No instruction per
+// key is added.  Pages in bf16 have scales of one.
+// A page is one step of PV, 16 keys, so its type is chosen page by page: staged pages have values and weights in
+// f16, times 2^7, whose rounding is lost in the output's (bf16 weights are not 1 where the largest is, as they are
+// without scales, and took the error from 1.0 to 1.4, in short rows 1.7, times the output's rounding); bf16
+// pages bf16 weights, and where they are most of the row a second bf16 term with what the first leaves out,
+// in S's other columns.  That term in every row cost 11 % of a call with a quarter of its keys in bf16.
+// Two spans of 1024 tokens, 32 heads of 128 over 8, against 8192 keys and half of that: 232 us with the
+// staging, 223 without (prefill_paged: 182).  The softmax of a block bounds it, as there, with the scales'
+// loads and products in its chain: without them 200.
 //
 // Key splits (non-causal calls, S > 1): blockIdx.z = sequence * S + split and
 // a CTA covers its split's share of the key blocks, writing the normalised
@@ -67,6 +75,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "pages_q8.cuh"
 #include "tcgen05.cuh"
 
 namespace lkv {
@@ -82,6 +91,10 @@ constexpr int kWarpK = 8, kWarpV = 9, kWarpK2 = 10, kWarpMma = 11;
 constexpr int kThreads = 12 * 32;
 constexpr int kStagesK = 2, kStagesV = 3;
 constexpr float kRescaleLog2 = 8.0f;
+constexpr float kWeightLog2 = 7.0f;  // Q8: weights are times 2^7, so that f16 has 2^15 for the largest
+// Q8: registers of a softmax thread, and of the others, of the 168 that each was launched with (8 warps gain
+// what 4 lose).  Two spans of 1024 tokens over 8192 keys: 223 us, with 168 each 239.
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 constexpr int kMaxKvSplits = 8;
 
 struct PrefillParams {
@@ -138,6 +151,7 @@ struct PrefillCfg {
   static_assert(SMEM_Q8 <= 227 * 1024, "shared memory");
   static constexpr uint32_t IDESC_S = umma_idesc_bf16(kBM, kBN, 0, 0);
   static constexpr uint32_t IDESC_PV = umma_idesc_bf16(kBM, D, 0, 1);
+  static constexpr uint32_t IDESC_PV_F16 = umma_idesc_f16(kBM, D, 0, 1);
   static constexpr uint32_t COL_S = 0;        // + tile * kBN
   static constexpr uint32_t COL_O = 2 * kBN;  // + tile * D
 };
@@ -212,6 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const int npages = min((n + kPageTok - 1) / kPageTok, p.W);
   const int nh = Q8 ? (p.num_q8 ? min(max(p.num_q8[b], 0), npages) : npages) : 0;  // pages in 8 bits
+  const bool two_terms = Q8 && npages - nh > nh;  // of the weights of bf16 pages
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, 1);
@@ -245,118 +260,134 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sV = smem + Cfg::OFF_V;
   const int32_t* btrow = p.bt + (int64_t)b * p.bt_stride;
 
-  if (warp == kWarpK || warp == kWarpK2 || warp == kWarpV) {
-    // ------------------------------------------------------------ producers
-    if (lane == 0) {
-      const bool is_k = warp != kWarpV;
-      const int stages = is_k ? kStagesK : kStagesV;
-      const CUtensorMap* map = is_k ? &tmk : &tmv;
-      const int pg0 = warp == kWarpK2 ? kPagesPerBlock / 2 : 0;
-      const int npg = is_k ? kPagesPerBlock / 2 : kPagesPerBlock;
-      tma_prefetch_desc(map);
-      if (!is_k) {
-        tma_prefetch_desc(&tmq);
-        mbar_arrive_expect_tx(&bars->q_full, ntiles * Cfg::Q_BYTES);
-        for (int t = 0; t < ntiles; ++t)
+  if (warp >= kTiles * 4) {
+    if constexpr (Q8) regs_dec<kOtherRegs>();
+    if (warp != kWarpMma) {
+      // ------------------------------------------------------------ producers
+      if (lane == 0) {
+        const bool is_k = warp != kWarpV;
+        const int stages = is_k ? kStagesK : kStagesV;
+        const CUtensorMap* map = is_k ? &tmk : &tmv;
+        const int pg0 = warp == kWarpK2 ? kPagesPerBlock / 2 : 0;
+        const int npg = is_k ? kPagesPerBlock / 2 : kPagesPerBlock;
+        tma_prefetch_desc(map);
+        if (!is_k) {
+          tma_prefetch_desc(&tmq);
+          mbar_arrive_expect_tx(&bars->q_full, ntiles * Cfg::Q_BYTES);
+          for (int t = 0; t < ntiles; ++t)
 #pragma unroll
-          for (int h = 0; h < Cfg::HALVES; ++h)
-            tma_load_3d(sQ + t * Cfg::Q_BYTES + h * Cfg::Q_HALF, &tmq, &bars->q_full, h * 64, hk * GROUP,
-                        q0 + t0 + t * TOK);
-      }
-      uint64_t* full = is_k ? bars->k_full : bars->v_full;
-      uint64_t* empty = is_k ? bars->k_empty : bars->v_empty;
-      uint8_t* ring = is_k ? sK : sV;
-      for (int j = 0; j < nb; ++j) {
-        const int s = j % stages;
-        if (!mbar_wait(&empty[s], ((j / stages) & 1) ^ 1)) {
-          report_error(p.err, DEVERR_WAIT_TIMEOUT, 4, j);
-          bars->fail = 1;
-          break;
+            for (int h = 0; h < Cfg::HALVES; ++h)
+              tma_load_3d(sQ + t * Cfg::Q_BYTES + h * Cfg::Q_HALF, &tmq, &bars->q_full, h * 64, hk * GROUP,
+                          q0 + t0 + t * TOK);
         }
-        mbar_arrive_expect_tx(&full[s], npg * (Cfg::KV_BYTES / kPagesPerBlock));
-        uint8_t* dst = ring + s * Cfg::KV_BYTES;
-        for (int pg = pg0; pg < pg0 + npg; ++pg) {
-          const int pi = (j0 + j) * kPagesPerBlock + pg;
-          int pid = (int)p.num_pages;  // past the pool: TMA fills zeros
-          const CUtensorMap* from = map;
-          if (Q8 && pi < nh) {
-            if constexpr (Q8) from = is_k ? &stage.k : &stage.v;
-            // a page without a place in the stage reads as zeros
-            pid = pi < p.stage_width ? b * p.stage_width + pi : p.B * p.stage_width;
-            if (is_k && pi >= p.stage_width) report_error(p.err, DEVERR_BAD_PAGE, 4, pi);
-          } else if (pi < npages) {
-            pid = btrow[pi];
-            const bool bad = pid < 0 || (int64_t)pid >= p.num_pages || (Q8 && !p.has_pool);
-            if (is_k && bad) report_error(p.err, DEVERR_BAD_PAGE, 4, pid);
-            if (Q8 && bad) pid = (int)p.num_pages;
+        uint64_t* full = is_k ? bars->k_full : bars->v_full;
+        uint64_t* empty = is_k ? bars->k_empty : bars->v_empty;
+        uint8_t* ring = is_k ? sK : sV;
+        for (int j = 0; j < nb; ++j) {
+          const int s = j % stages;
+          if (!mbar_wait(&empty[s], ((j / stages) & 1) ^ 1)) {
+            report_error(p.err, DEVERR_WAIT_TIMEOUT, 4, j);
+            bars->fail = 1;
+            break;
           }
+          mbar_arrive_expect_tx(&full[s], npg * (Cfg::KV_BYTES / kPagesPerBlock));
+          uint8_t* dst = ring + s * Cfg::KV_BYTES;
+          for (int pg = pg0; pg < pg0 + npg; ++pg) {
+            const int pi = (j0 + j) * kPagesPerBlock + pg;
+            int pid = (int)p.num_pages;  // past the pool: TMA fills zeros
+            const CUtensorMap* from = map;
+            if (Q8 && pi < nh) {
+              if constexpr (Q8) from = is_k ? &stage.k : &stage.v;
+              // a page without a place in the stage reads as zeros
+              pid = pi < p.stage_width ? b * p.stage_width + pi : p.B * p.stage_width;
+              if (is_k && pi >= p.stage_width) report_error(p.err, DEVERR_BAD_PAGE, 4, pi);
+            } else if (pi < npages) {
+              pid = btrow[pi];
+              const bool bad = pid < 0 || (int64_t)pid >= p.num_pages || (Q8 && !p.has_pool);
+              if (is_k && bad) report_error(p.err, DEVERR_BAD_PAGE, 4, pid);
+              if (Q8 && bad) pid = (int)p.num_pages;
+            }
 #pragma unroll
-          for (int h = 0; h < Cfg::HALVES; ++h)
-            tma_load_4d(dst + h * Cfg::KV_HALF + pg * (kPageTok * 128), from, &full[s], h * 64, hk, 0, pid);
+            for (int h = 0; h < Cfg::HALVES; ++h)
+              tma_load_4d(dst + h * Cfg::KV_HALF + pg * (kPageTok * 128), from, &full[s], h * 64, hk, 0, pid);
+          }
         }
       }
-    }
-  } else if (warp == kWarpMma) {
-    // ------------------------------------------------------------ MMA issuer
-    const bool leader = elect_one();
-    // Descriptors of each operand's first 16-element K slice; the slices and
-    // ring stages are constant offsets (16-byte units) from them.
-    const uint64_t qd = umma_sdesc_sw128(smem_u32(sQ), 16, 1024);
-    const uint64_t kd = umma_sdesc_sw128(smem_u32(sK), 16, 1024);
-    const uint64_t vd = umma_sdesc_sw128(smem_u32(sV), Cfg::KV_HALF, 1024);
-    auto issue_s = [&](int t, int j) {
-      const uint64_t kb = kd + (uint64_t)(((j % kStagesK) * Cfg::KV_BYTES) >> 4);
-      const uint64_t qb = qd + (uint64_t)((t * Cfg::Q_BYTES) >> 4);
+    } else {
+      // ------------------------------------------------------------ MMA issuer
+      const bool leader = elect_one();
+      // Descriptors of each operand's first 16-element K slice; the slices and
+      // ring stages are constant offsets (16-byte units) from them.
+      const uint64_t qd = umma_sdesc_sw128(smem_u32(sQ), 16, 1024);
+      const uint64_t kd = umma_sdesc_sw128(smem_u32(sK), 16, 1024);
+      const uint64_t vd = umma_sdesc_sw128(smem_u32(sV), Cfg::KV_HALF, 1024);
+      auto issue_s = [&](int t, int j) {
+        const uint64_t kb = kd + (uint64_t)(((j % kStagesK) * Cfg::KV_BYTES) >> 4);
+        const uint64_t qb = qd + (uint64_t)((t * Cfg::Q_BYTES) >> 4);
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const uint32_t oq = ((ks >> 2) * Cfg::Q_HALF + (ks & 3) * 32) >> 4;
-        const uint32_t okv = ((ks >> 2) * Cfg::KV_HALF + (ks & 3) * 32) >> 4;
-        if (leader) umma_bf16_ss(tmem + Cfg::COL_S + t * kBN, qb + oq, kb + okv, Cfg::IDESC_S, ks > 0 ? 1u : 0u);
-      }
-      if (leader) umma_commit(&bars->s_full[t]);
-    };
-    auto issue_pv = [&](int t, int j) {
-      const uint64_t vb = vd + (uint64_t)(((j % kStagesV) * Cfg::KV_BYTES) >> 4);
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t oq = ((ks >> 2) * Cfg::Q_HALF + (ks & 3) * 32) >> 4;
+          const uint32_t okv = ((ks >> 2) * Cfg::KV_HALF + (ks & 3) * 32) >> 4;
+          if (leader) umma_bf16_ss(tmem + Cfg::COL_S + t * kBN, qb + oq, kb + okv, Cfg::IDESC_S, ks > 0 ? 1u : 0u);
+        }
+        if (leader) umma_commit(&bars->s_full[t]);
+      };
+      auto issue_pv = [&](int t, int j) {
+        const uint64_t vb = vd + (uint64_t)(((j % kStagesV) * Cfg::KV_BYTES) >> 4);
+        if constexpr (Q8) {  // a page, 16 keys, is one step: f16 weights and codes, or two bf16 terms of the weights
+          const int staged = nh - (j0 + j) * kPagesPerBlock;
+          const uint32_t d = tmem + Cfg::COL_O + t * D, w = tmem + Cfg::COL_S + t * kBN;
 #pragma unroll
-      for (int ks = 0; ks < kBN / 16; ++ks)
-        if (leader)
-          umma_bf16_ts(tmem + Cfg::COL_O + t * D, tmem + Cfg::COL_S + t * kBN + ks * 8,
-                       vb + (uint64_t)((ks * (kPageTok * 128)) >> 4), Cfg::IDESC_PV, (j > 0 || ks > 0) ? 1u : 0u);
-      if (leader) umma_commit(&bars->pv_done[t]);
-    };
-    // Wait results are made warp-uniform so the whole warp leaves together.
-    bool ok = __all_sync(0xffffffffu, mbar_wait(&bars->q_full, 0));
-    for (int j = 0; ok && j <= nb; ++j) {
-      // PV_A(j-1), S_A(j), PV_B(j-1), S_B(j)
-      if (j < nb) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars->k_full[j % kStagesK], (j / kStagesK) & 1));
-        tc_fence_after();
-        if (!ok) break;
-      }
-      if (j > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_full[(j - 1) % kStagesV], ((j - 1) / kStagesV) & 1));
-        if (!ok) break;
-      }
-      for (int t = 0; t < ntiles; ++t) {
-        if (j > 0) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_full[t], (j - 1) & 1));
+          for (int ks = 0; ks < kBN / 16; ++ks) {
+            const uint64_t v = vb + (uint64_t)((ks * (kPageTok * 128)) >> 4);
+            const bool f16 = ks < staged;
+            if (leader) umma_bf16_ts(d, w + ks * 8, v, f16 ? Cfg::IDESC_PV_F16 : Cfg::IDESC_PV, (j > 0 || ks > 0) ? 1u : 0u);
+            if (leader && !f16 && two_terms) umma_bf16_ts(d, w + kBN / 2 + ks * 8, v, Cfg::IDESC_PV, 1u);
+          }
+        } else {
+#pragma unroll
+          for (int ks = 0; ks < kBN / 16; ++ks)
+            if (leader)
+              umma_bf16_ts(tmem + Cfg::COL_O + t * D, tmem + Cfg::COL_S + t * kBN + ks * 8,
+                           vb + (uint64_t)((ks * (kPageTok * 128)) >> 4), Cfg::IDESC_PV, (j > 0 || ks > 0) ? 1u : 0u);
+        }
+        if (leader) umma_commit(&bars->pv_done[t]);
+      };
+      // Wait results are made warp-uniform so the whole warp leaves together.
+      bool ok = __all_sync(0xffffffffu, mbar_wait(&bars->q_full, 0));
+      for (int j = 0; ok && j <= nb; ++j) {
+        // PV_A(j-1), S_A(j), PV_B(j-1), S_B(j)
+        if (j < nb) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->k_full[j % kStagesK], (j / kStagesK) & 1));
           tc_fence_after();
           if (!ok) break;
-          issue_pv(t, j - 1);
         }
-        if (j < nb) issue_s(t, j);
+        if (j > 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_full[(j - 1) % kStagesV], ((j - 1) / kStagesV) & 1));
+          if (!ok) break;
+        }
+        for (int t = 0; t < ntiles; ++t) {
+          if (j > 0) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_full[t], (j - 1) & 1));
+            tc_fence_after();
+            if (!ok) break;
+            issue_pv(t, j - 1);
+          }
+          if (j < nb) issue_s(t, j);
+        }
+        if (!ok) break;
+        if (leader) {
+          if (j < nb) umma_commit(&bars->k_empty[j % kStagesK]);
+          if (j > 0) umma_commit(&bars->v_empty[(j - 1) % kStagesV]);
+        }
       }
-      if (!ok) break;
-      if (leader) {
-        if (j < nb) umma_commit(&bars->k_empty[j % kStagesK]);
-        if (j > 0) umma_commit(&bars->v_empty[(j - 1) % kStagesV]);
+      if (!ok && leader) {
+        report_error(p.err, DEVERR_WAIT_TIMEOUT, 4, 100);
+        bars->fail = 1;
       }
-    }
-    if (!ok && leader) {
-      report_error(p.err, DEVERR_WAIT_TIMEOUT, 4, 100);
-      bars->fail = 1;
     }
   } else if ((warp >> 2) < ntiles) {
+    if constexpr (Q8) regs_inc<kSoftmaxRegs>();
     // ------------------------------------------------------------ softmax (rows)
     const int t = warp >> 2;                       // tile
     const int r = (warp & 3) * 32 + lane;          // TMEM lane = row within the tile
@@ -425,70 +456,94 @@ __global__ void __launch_bounds__(kThreads, 1)
         float gm[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const float4 kf = gs4[c];
+          const float4 kf = gs4[c], lv = gs4[4 + c];
           auto top8 = [&x](int e) {
             return fmaxf(fmax3f(fmax3f(x[e], x[e + 1], x[e + 2]), x[e + 3], x[e + 4]), fmax3f(x[e + 5], x[e + 6], x[e + 7]));
           };
-          gm[c] = fmaxf(fmax3f(top8(32 * c) * kf.x, top8(32 * c + 8) * kf.y, top8(32 * c + 16) * kf.z),
-                        top8(32 * c + 24) * kf.w);
+          gm[c] = fmaxf(fmax3f(fmaf(top8(32 * c), kf.x, lv.x), fmaf(top8(32 * c + 8), kf.y, lv.y),
+                               fmaf(top8(32 * c + 16), kf.z, lv.z)),
+                        fmaf(top8(32 * c + 24), kf.w, lv.w));
         }
         mx = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
       } else {
-      // 8 independent partial maxima (short dependency chains, three-input max), then a tree
-      float mp[8];
+        // 8 independent partial maxima (short dependency chains, three-input max), then a tree
+        float mp[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) mp[u] = fmaxf(x[u], x[kBN - 8 + u]);
+        for (int u = 0; u < 8; ++u) mp[u] = fmaxf(x[u], x[kBN - 8 + u]);
 #pragma unroll
-      for (int e = 8; e + 16 <= kBN - 8; e += 16)
+        for (int e = 8; e + 16 <= kBN - 8; e += 16)
 #pragma unroll
-        for (int u = 0; u < 8; ++u) mp[u] = fmax3f(mp[u], x[e + u], x[e + 8 + u]);
-      mx = fmaxf(fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])), fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7])));
-      mx *= sl2;  // scale > 0, so max commutes with it
+          for (int u = 0; u < 8; ++u) mp[u] = fmax3f(mp[u], x[e + u], x[e + 8 + u]);
+        mx = fmaxf(fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])), fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7])));
+        mx *= sl2;  // scale > 0, so max commutes with it
       }
       float alpha = 1.f;
       if (mx > m + kRescaleLog2) {
         alpha = (m == -INFINITY) ? 0.f : ex2_approx(m - mx);
         m = mx;
       }
-      const float neg_mref = (m == -INFINITY) ? 0.f : -m;
+      const float neg_mref = (m == -INFINITY) ? 0.f : (Q8 ? kWeightLog2 : 0.f) - m;
       const float2 sl2v = make_float2(sl2, sl2), negm = make_float2(neg_mref, neg_mref);
       float2 sp[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       // P(j) (bf16 pairs) over the first 64 columns of this tile's S, which is fully
       // read: 16 columns per 32 keys, stored as each chunk is ready.  f32x2 FFMA /
       // FADD halve the issue slots of the scale-and-subtract and the sums; pairs 0
       // and 1 of every 8 take their exponentials on the FMA pipe, the rest on the SFU.
+      if constexpr (Q8) {
+        const int staged = nh - (j0 + j) * kPagesPerBlock;  // pages of this block in 8 bits
+        // the weights as PV takes them: f16, or (MIXED: pages from `staged` on) bf16, with TWO what that leaves out
+        auto weights = [&](auto mixed, auto two) {
+          constexpr bool MIXED = decltype(mixed)::value, TWO = decltype(two)::value;
 #pragma unroll
-      for (int c = 0; c < kBN / 32; ++c) {
-        uint32_t pc[16];
-        if constexpr (Q8) {
-          const float4 kf4 = gs4[c], lv4 = gs4[4 + c], iv4 = gs4[8 + c];
+          for (int c = 0; c < kBN / 32; ++c) {
+            uint32_t pc[16], rest[TWO ? 16 : 1];
+            const float4 kf4 = gs4[c], lv4 = gs4[4 + c], iv4 = gs4[8 + c];
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const float kf = (&kf4.x)[g], add = (&lv4.x)[g] + neg_mref;
-            const float2 kfv = make_float2(kf, kf), addv = make_float2(add, add);
-            float2 gs = make_float2(0.f, 0.f);
+            for (int g = 0; g < 4; ++g) {
+              const float kf = (&kf4.x)[g], add = (&lv4.x)[g] + neg_mref;
+              const float2 kfv = make_float2(kf, kf), addv = make_float2(add, add);
+              float2 gs = make_float2(0.f, 0.f), pv[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int e = c * 32 + g * 8 + 2 * q;
-              const float2 a = __ffma2_rn(make_float2(x[e], x[e + 1]), kfv, addv);
-              const float2 pv = q == (g & 1) ? ex2_poly2(a) : make_float2(ex2_approx(a.x), ex2_approx(a.y));
-              gs = __fadd2_rn(gs, pv);
-              pc[g * 4 + q] = pack_bf16(pv.x, pv.y);
+              for (int q = 0; q < 4; ++q) {
+                const int e = c * 32 + g * 8 + 2 * q;
+                const float2 a = __ffma2_rn(make_float2(x[e], x[e + 1]), kfv, addv);
+                pv[q] = q == (g & 1) ? ex2_poly2(a) : make_float2(ex2_approx(a.x), ex2_approx(a.y));
+                gs = __fadd2_rn(gs, pv[q]);
+              }
+              const bool f16 = !MIXED || 2 * c + (g >> 1) < staged;
+#pragma unroll
+              for (int q = 0; q < 4; ++q) pc[g * 4 + q] = f16 ? pack_f16(pv[q].x, pv[q].y) : pack_bf16(pv[q].x, pv[q].y);
+              if constexpr (TWO) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  const uint32_t hi = pc[g * 4 + q];
+                  rest[g * 4 + q] = pack_bf16(pv[q].x - bf16_lo(hi), pv[q].y - bf16_hi(hi));
+                }
+              }
+              const float inv = (&iv4.x)[g];
+              sp[g] = __ffma2_rn(gs, make_float2(inv, inv), sp[g]);
             }
-            const float inv = (&iv4.x)[g];
-            sp[g] = __ffma2_rn(gs, make_float2(inv, inv), sp[g]);
+            tmem_st16(lane_base + col_s + c * 16, pc);
+            if constexpr (TWO) tmem_st16(lane_base + col_s + kBN / 2 + c * 16, rest);
           }
-        } else {
+        };
+        if (staged >= kPagesPerBlock) weights(std::false_type{}, std::false_type{});
+        else if (two_terms) weights(std::true_type{}, std::true_type{});
+        else weights(std::true_type{}, std::false_type{});
+      } else {
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          const int e = c * 32 + 2 * q;
-          const float2 a = __ffma2_rn(make_float2(x[e], x[e + 1]), sl2v, negm);
-          const float2 pv = (q & 7) < 2 ? ex2_poly2(a) : make_float2(ex2_approx(a.x), ex2_approx(a.y));
-          sp[q & 3] = __fadd2_rn(sp[q & 3], pv);
-          pc[q] = pack_bf16(pv.x, pv.y);
+        for (int c = 0; c < kBN / 32; ++c) {
+          uint32_t pc[16];
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            const int e = c * 32 + 2 * q;
+            const float2 a = __ffma2_rn(make_float2(x[e], x[e + 1]), sl2v, negm);
+            const float2 pv = (q & 7) < 2 ? ex2_poly2(a) : make_float2(ex2_approx(a.x), ex2_approx(a.y));
+            sp[q & 3] = __fadd2_rn(sp[q & 3], pv);
+            pc[q] = pack_bf16(pv.x, pv.y);
+          }
+          tmem_st16(lane_base + col_s + c * 16, pc);
         }
-        }
-        tmem_st16(lane_base + col_s + c * 16, pc);
       }
       const float sum = ((sp[0].x + sp[0].y) + (sp[1].x + sp[1].y)) + ((sp[2].x + sp[2].y) + (sp[3].x + sp[3].y));
       l = l * alpha + sum;
@@ -531,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int hq = hk * GROUP + r % GROUP;
       const bool valid = tok < Lq;
       const float inv = l > 0.f ? 1.f / l : 0.f;
-      const float lse_e = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+      const float lse_e = l > 0.f ? (m + log2f(l) - (Q8 ? kWeightLog2 : 0.f)) * 0.6931471805599453f : -INFINITY;
       const int64_t row = (int64_t)(q0 + (valid ? tok : 0)) * p.Hq + hq;
       if (p.S > 1) {
         // this split's normalised partial (fp32) and its natural-log LSE

@@ -102,6 +102,17 @@ __device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[2][8]) {
                : "memory");
 }
 
+// Registers of this warpgroup's threads from here on (every warp of it comes by): what some give, others may
+// take, of those that the block was launched with.
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // ---------------------------------------------------------------- UMMA
 
 // D[tmem] (+)= A[smem desc] * B[smem desc], kind::f16 (bf16 in, fp32 accumulate).
@@ -150,6 +161,11 @@ __host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N, int a_mn_ma
          | ((uint32_t)b_mn_major << 16)   // B major (0 = K, 1 = MN)
          | ((uint32_t)(N >> 3) << 17)     // N / 8
          | ((uint32_t)(M >> 4) << 24);    // M / 16
+}
+
+// The same with f16 A/B.
+__host__ __device__ constexpr uint32_t umma_idesc_f16(int M, int N, int a_mn_major, int b_mn_major) {
+  return umma_idesc_bf16(M, N, a_mn_major, b_mn_major) & ~(1u << 7) & ~(1u << 10);  // A, B format 0: f16
 }
 
 // Instruction descriptor of kind::i8: signed A/B, int32 D, dense, both operands K-major.

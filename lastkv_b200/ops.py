@@ -1141,14 +1141,14 @@ def _pages_q8(c, dev: int):
     return codes.data_ptr(), scales.data_ptr(), n, h, last // PAGE_SIZE
 
 
-def _pools(pool_k, pool_v, h: int, d: int, dev: int):
-    """(addresses of K and V, pages) of a checked bf16 pool of h heads, None for none."""
+def _pools(pool_k, pool_v, h: int, d: int, dev: int, v_type=_BF16):
+    """(addresses of K and V, pages) of a checked bf16 pool (values of v_type) of h heads, None for none."""
     if pool_k is None and pool_v is None:
         return None, None, 0
     if pool_k is None or pool_v is None:
         _fail("pool_k and pool_v come together")
     shape = pool_k.shape
-    if pool_k.dtype is not _BF16 or pool_v.dtype is not _BF16 or pool_v.shape != shape \
+    if pool_k.dtype is not _BF16 or pool_v.dtype is not v_type or pool_v.shape != shape \
             or shape[1:] != (PAGE_SIZE, h, d) or not pool_k.is_contiguous() or not pool_v.is_contiguous() \
             or pool_k.get_device() != dev or pool_v.get_device() != dev:
         _fail(f"pools must be equal contiguous bf16 [pages, {PAGE_SIZE}, {h}, {d}] on the call's CUDA device (the heads "
@@ -1259,8 +1259,8 @@ def decode_paged_q8(q, cache: PagesQ8, block_table, seq_k, *, num_q8=None, pool_
 
 
 class StageQ8(NamedTuple):
-    """Workspace of ``prefill_paged_q8``: the codes of each row's 8-bit pages as bf16, page
-    ``row * width + column`` of ``k`` and ``v`` [batch * width, 16, Hkv, D]."""
+    """Workspace of ``prefill_paged_q8``: the codes of each row's 8-bit pages, page ``row * width + column``
+    of ``k`` (bf16) and ``v`` (fp16) [batch * width, 16, Hkv, D]."""
 
     k: torch.Tensor
     v: torch.Tensor
@@ -1270,8 +1270,8 @@ class StageQ8(NamedTuple):
     def empty(cls, batch: int, width: int, num_kv_heads: int, head_dim: int, device="cuda") -> "StageQ8":
         """For ``batch`` rows of at most ``width`` 8-bit pages."""
         width = max(int(width), 1)
-        k, v = (torch.empty((max(batch, 1) * width, PAGE_SIZE, num_kv_heads, head_dim), dtype=_BF16, device=device)
-                for _ in range(2))
+        k, v = (torch.empty((max(batch, 1) * width, PAGE_SIZE, num_kv_heads, head_dim), dtype=t, device=device)
+                for t in (_BF16, torch.float16))
         return cls(k, v, width)
 
 
@@ -1306,7 +1306,7 @@ def prefill_paged_q8(q, cache: PagesQ8, block_table, seq_k, cu_q, max_q: int, *,
         if staged:
             _fail("staged=True needs the stage of the earlier call")
         stage = StageQ8.empty(B, W, h, D, device=q.device)
-    sk, sv, pages = _pools(stage.k, stage.v, h, D, dev)
+    sk, sv, pages = _pools(stage.k, stage.v, h, D, dev, torch.float16)
     if stage.width < 1 or pages < B * stage.width:
         _fail(f"the stage holds {pages} pages, {B} rows of {stage.width} were asked for")
     if kv_splits is None:
