@@ -637,7 +637,8 @@ int lkv_prefill_q8_split_plan(int batch, int max_q, int total_q, int num_q_heads
  * finished (uint8 [batch, beams], may be NULL): such a beam goes on with eos_token alone, at
  * its score.  A total that is not a number, and every total of a beam whose score or sum
  * is not finite, counts as -inf.  select <= 32, select <= vocab, beams <= 64,
- * batch * beams <= 65535.  The workspace (16-byte aligned) need not be cleared. */
+ * batch * beams <= 65535.  With select = beams, out_scores and out_finished may be scores and
+ * finished themselves.  The workspace (16-byte aligned) need not be cleared. */
 int lkv_reorder_pages(void* const* pools, const int64_t* page_bytes, const int64_t* num_pages, int num_pools,
                       const int32_t* src_pages, const int32_t* dst_pages, int n, int layers,
                       int64_t layer_stride, int32_t* error_word, void* stream);

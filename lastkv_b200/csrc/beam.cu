@@ -329,6 +329,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const MergePa
   __shared__ uint64_t total[kMaxBeams * kMaxSelect * 3 / 2];  // ordered totals: a list of 1 << log_n for each beam
   __shared__ uint32_t from_where[kMaxBeams * kMaxSelect * 3 / 2];  // the beam and the place in its list
   __shared__ uint32_t token[kMaxBeams * kMaxSelect];
+  __shared__ bool ended[kMaxBeams];  // read before anything is written: the outputs may be the inputs' buffers
   const int b = blockIdx.x, n = p.select, K = p.K, S = p.stretches, tid = threadIdx.x;
   const int log_n = p.log_n, pad = 1 << log_n;
   pdl_launch_dependents();
@@ -375,6 +376,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const MergePa
       const int e = ilogb(sum);
       const double score = (double)p.scores[row];
       const double rest = done ? 0.0 : e * 0.6931471805599453 + (double)logf((float)scalbn(sum, -e));
+      ended[k] = done;
       tops[k] = done ? 0.0 : (double)top;
       norm[k] = fabs(score) < INFINITY && fabs(tops[k]) < INFINITY && fabs(rest) < INFINITY ? score - rest : NAN;
     }
@@ -407,7 +409,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const MergePa
     p.out_scores[at] = (float)from_ordered(from[tid]);
     p.out_rows[at] = row;
     p.out_tokens[at] = v;
-    if (p.out_finished) p.out_finished[at] = (int64_t)v == p.eos || (p.finished && p.finished[row]);
+    if (p.out_finished) p.out_finished[at] = (int64_t)v == p.eos || ended[k];
   }
 }
 

@@ -69,7 +69,7 @@ int quantise_pages(const void* pool_k, const void* pool_v, int64_t pool_pages, c
 int dequantise_pages(const void* codes, const float* scales, int64_t q8_pages, const int32_t* pages, void* pool_k,
                      void* pool_v, int64_t pool_pages, const int32_t* out_pages, int64_t n, int hkv, int d, int* err,
                      cudaStream_t stream);
-// The codes of the leading `width` columns of block tables as bf16, for prefill_paged.
+// The codes of the leading `width` columns of block tables (keys as bf16, values as f16), for prefill_paged.
 int stage_pages(const void* codes, const float* scales, int64_t q8_pages, const int32_t* bt, int64_t bt_stride,
                 const int32_t* num_q8, const int32_t* seq_k, int batch, int W, void* stage_k, void* stage_v, int width,
                 int hkv, int d, int* err, cudaStream_t stream);

@@ -1394,7 +1394,7 @@ def beam_select(logits, scores, *, select: int | None = None, finished=None, eos
     logits [B * K, V] bf16 or fp32 rows (any row stride); scores fp32 [B, K], the beams' summed
     log-probabilities.  Candidates are ordered by ``scores + log_softmax(logits)``, equal ones by beam
     and token.  ``finished`` bool [B, K]: such a beam continues with ``eos_token`` alone, at its score.
-    ``out``: buffers to write (a captured step's).
+    ``out``: buffers to write (a captured step's); its scores and finished may be the call's own.
     """
     if scores.dtype is not _F32 or scores.dim() != 2 or not scores.is_contiguous():
         _fail("scores must be contiguous CUDA fp32 [B, K]")

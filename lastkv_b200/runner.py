@@ -47,14 +47,12 @@ class GraphDecodeRunner:
         self.model, self.cache = model, cache
         dev = cache.device
         self.beams, self.eos_token = beams, eos_token
-        if beams is not None:  # the step's candidates, and what the next one starts from
-            self.choice = ops.BeamChoice.empty(cache.batch // beams, beams, device=dev)
-            self.scores = torch.zeros((cache.batch // beams, beams), dtype=torch.float32, device=dev)
-            self.finished = torch.zeros_like(self.choice.finished)
+        if beams is not None:  # the step's candidates, in whose place the next one's are written
+            self.choice = ops.BeamChoice(*(t.zero_() for t in ops.BeamChoice.empty(cache.batch // beams, beams, device=dev)))
         B, L = cache.batch, cache.num_layers
         self.B, self.L = B, L
         self.W = cache.pages_per_seq + cache.ring_pages
-        self.ids = torch.zeros((B, 1), dtype=torch.int64, device=dev)
+        self.ids = torch.zeros((B, 1), dtype=torch.int64, device=dev) if beams is None else self.choice.tokens.view(B, 1)
         self.pos = torch.zeros((1, 1), dtype=torch.int64, device=dev)
         self.bt = torch.zeros((B, self.W), dtype=torch.int32, device=dev)
         self.nsrc = torch.zeros(B, dtype=torch.int32, device=dev)
@@ -155,9 +153,8 @@ class GraphDecodeRunner:
         pe = m.rotary_emb(hidden, self.pos)
         logits = self.model.lm_head(m.run_layers(hidden, pe, self.cache)[:, -1])
         if self.beams is not None:
-            ops.beam_select(logits, self.scores, finished=self.finished if self.eos_token is not None else None,
-                            eos_token=self.eos_token, out=self.choice)
-            self._take_choice()
+            ops.beam_select(logits, self.choice.scores, eos_token=self.eos_token, out=self.choice,
+                            finished=self.choice.finished if self.eos_token is not None else None)
         elif logits.dtype == torch.bfloat16 and logits.shape[-1] % 8 == 0:
             ops.argmax_rows(logits, out=self.ids.view(-1))  # torch.argmax order, one launch
         else:
@@ -165,19 +162,13 @@ class GraphDecodeRunner:
         if self.plan is not None:
             self.computed.add_(self.new_tokens)
 
-    def _take_choice(self):
-        """The chosen candidates are what the next step starts from."""
-        self.ids.copy_(self.choice.tokens.view(-1, 1))
-        self.scores.copy_(self.choice.scores)
-        self.finished.copy_(self.choice.finished)
-
     def capture(self):
         """Capture one decode step at the current position (the warm-up runs do not advance),
         and for bf16 caches the same step with a boundary commit fused into layer 0's append."""
         cache = self.cache
         cache.flush_commit()
         self._captured = cache.pool_k, cache.q8, self.W
-        state = (self.ids, self.scores, self.finished) if self.beams is not None else (self.ids,)
+        state = tuple(self.choice) if self.beams is not None else (self.ids,)
         saved = [t.clone() for t in state]
 
         def restore():  # what the warm-up steps started from
@@ -275,9 +266,8 @@ class GraphDecodeRunner:
             for start in range(0, prompt.shape[1], call_tokens):
                 logits, _ = self.model(prompt[:, start:start + call_tokens], self.cache, logits_to_keep=1)
         if rows is not None:
-            ops.beam_select(logits[:, -1], self.scores.new_zeros((len(rows), 1)), select=self.beams,
+            ops.beam_select(logits[:, -1], self.choice.scores.new_zeros((len(rows), 1)), select=self.beams,
                             eos_token=self.eos_token, out=self.choice)
-            self._take_choice()
             self.cache.reorder_cache(np.repeat(rows, self.beams))
             return self.ids
         self.ids.copy_(logits[:, -1].float().argmax(-1, keepdim=True))

@@ -205,6 +205,18 @@ def test_captured_steps():
             assert torch.equal(o.rows.cpu(), rows) and torch.equal(o.tokens.cpu(), tokens)
 
 
+@pytest.mark.parametrize("B,K", [(1, 1), (3, 7), (5, 32)])
+def test_results_in_the_place_of_scores_and_finished(B, K):
+    g = torch.Generator().manual_seed(B)
+    logits = torch.randn((B * K, 3001), generator=g).cuda()
+    scores, done = -torch.rand((B, K), generator=g).cuda() * 5, (torch.rand((B, K), generator=g) < 0.4).cuda()
+    want = ops.beam_select(logits, scores, finished=done, eos_token=9)
+    out = ops.BeamChoice.empty(B, K)._replace(scores=scores, finished=done)
+    ops.beam_select(logits, scores, finished=done, eos_token=9, out=out)
+    for a, b in zip(out, want):
+        assert torch.equal(a, b)
+
+
 def test_same_result_every_time():
     x, s = _logits(15, 32, 128256).bfloat16(), _scores(16, 4, 8)
     first = ops.beam_select(x, s, select=16)
