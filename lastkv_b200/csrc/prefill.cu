@@ -57,9 +57,9 @@
 // without scales, and took the error from 1.0 to 1.4, in short rows 1.7, times the output's rounding); bf16
 // pages bf16 weights, and where they are most of the row a second bf16 term with what the first leaves out,
 // in S's other columns.  That term in every row cost 11 % of a call with a quarter of its keys in bf16.
-// Two spans of 1024 tokens, 32 heads of 128 over 8, against 8192 keys and half of that: 232 us with the
-// staging, 223 without (prefill_paged: 182).  The softmax of a block bounds it, as there, with the scales'
-// loads and products in its chain: without them 200.
+// Two spans of 1024 tokens, 32 heads of 128 over 8, against 8192 keys and half of that: 221 us with the
+// staging, 212 without (prefill_paged: 182).  The softmax of a block bounds it, as there, with the scales in its
+// chain.
 //
 // Key splits (non-causal calls, S > 1): blockIdx.z = sequence * S + split and
 // a CTA covers its split's share of the key blocks, writing the normalised
@@ -93,7 +93,8 @@ constexpr int kStagesK = 2, kStagesV = 3;
 constexpr float kRescaleLog2 = 8.0f;
 constexpr float kWeightLog2 = 7.0f;  // Q8: weights are times 2^7, so that f16 has 2^15 for the largest
 // Q8: registers of a softmax thread, and of the others, of the 168 that each was launched with (8 warps gain
-// what 4 lose).  Two spans of 1024 tokens over 8192 keys: 223 us, with 168 each 239.
+// what 4 lose).  Two spans of 1024 tokens over 8192 keys: 223 us, with 168 each 239; the scales of a block then fit
+// into registers before its scores are waited for: 212.
 constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 constexpr int kMaxKvSplits = 8;
 
@@ -400,7 +401,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     const float sl2 = p.scale_log2;
     float* group_scale = reinterpret_cast<float*>(smem + Cfg::OFF_SCALE) + warp * 48;  // Q8
-    const float4* gs4 = reinterpret_cast<const float4*>(group_scale);
+    auto load4 = [](const float* p) {
+      const uint4 v = ld_shared16(p);
+      return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+    };
     // Q8: lane 4 i + c has scale c (keys 0-7, 8-15, values 0-7, 8-15) of page i of a block.  It is read a block
     // ahead, and the page's id two, so that neither is waited for.
     auto page_of = [&](int j) {
@@ -415,6 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int next_page = Q8 ? page_of(1) : 0;
     // Wait results are made warp-uniform: tcgen05.ld/st below are warp-collective.
     for (int j = 0; j < nb; ++j) {
+      float4 kf[4], lv[4];  // Q8
       if constexpr (Q8) {
         float f = next_scale;
         next_scale = scale_of(next_page);
@@ -429,6 +434,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           group_scale[at] = fmaxf(f, 1e-37f) * sl2;  // codes of zero: not -inf * 0 where they are masked
         }
         __syncwarp();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {  // those of the 16 groups, before the scores are waited for
+          kf[c] = load4(group_scale + 4 * c);
+          lv[c] = load4(group_scale + 16 + 4 * c);
+        }
       }
       ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[t], j & 1));
       tc_fence_after();
@@ -456,13 +466,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         float gm[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const float4 kf = gs4[c], lv = gs4[4 + c];
           auto top8 = [&x](int e) {
             return fmaxf(fmax3f(fmax3f(x[e], x[e + 1], x[e + 2]), x[e + 3], x[e + 4]), fmax3f(x[e + 5], x[e + 6], x[e + 7]));
           };
-          gm[c] = fmaxf(fmax3f(fmaf(top8(32 * c), kf.x, lv.x), fmaf(top8(32 * c + 8), kf.y, lv.y),
-                               fmaf(top8(32 * c + 16), kf.z, lv.z)),
-                        fmaf(top8(32 * c + 24), kf.w, lv.w));
+          gm[c] = fmaxf(fmax3f(fmaf(top8(32 * c), kf[c].x, lv[c].x), fmaf(top8(32 * c + 8), kf[c].y, lv[c].y),
+                               fmaf(top8(32 * c + 16), kf[c].z, lv[c].z)),
+                        fmaf(top8(32 * c + 24), kf[c].w, lv[c].w));
         }
         mx = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
       } else {
@@ -497,16 +506,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int c = 0; c < kBN / 32; ++c) {
             uint32_t pc[16], rest[TWO ? 16 : 1];
-            const float4 kf4 = gs4[c], lv4 = gs4[4 + c], iv4 = gs4[8 + c];
+            const float4 iv = load4(group_scale + 32 + 4 * c);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-              const float kf = (&kf4.x)[g], add = (&lv4.x)[g] + neg_mref;
-              const float2 kfv = make_float2(kf, kf), addv = make_float2(add, add);
+              const float scale = (&kf[c].x)[g], add = (&lv[c].x)[g] + neg_mref;
+              const float2 scalev = make_float2(scale, scale), addv = make_float2(add, add);
               float2 gs = make_float2(0.f, 0.f), pv[4];
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 const int e = c * 32 + g * 8 + 2 * q;
-                const float2 a = __ffma2_rn(make_float2(x[e], x[e + 1]), kfv, addv);
+                const float2 a = __ffma2_rn(make_float2(x[e], x[e + 1]), scalev, addv);
                 pv[q] = q == (g & 1) ? ex2_poly2(a) : make_float2(ex2_approx(a.x), ex2_approx(a.y));
                 gs = __fadd2_rn(gs, pv[q]);
               }
@@ -520,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   rest[g * 4 + q] = pack_bf16(pv[q].x - bf16_lo(hi), pv[q].y - bf16_hi(hi));
                 }
               }
-              const float inv = (&iv4.x)[g];
+              const float inv = (&iv.x)[g];
               sp[g] = __ffma2_rn(gs, make_float2(inv, inv), sp[g]);
             }
             tmem_st16(lane_base + col_s + c * 16, pc);
