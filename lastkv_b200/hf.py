@@ -999,6 +999,8 @@ class LastKVForCausalLM(nn.Module):
         B * num_beams rows (``new_cache``; with ``history="int8"``, say)."""
         B, P = prompt.shape
         K = num_beams
+        if not 1 <= K <= 32 or P < 1:
+            raise RMarinBackendContractError("beam search needs a prompt of one token at least, and a beam (32 at most)")
         cache = cache or self.new_cache(B * K, P + max_new_tokens)
         if cache.batch != B * K or cache.seen_tokens:
             raise RMarinBackendContractError(f"beam search needs an empty cache of {B * K} rows")

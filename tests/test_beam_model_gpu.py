@@ -249,5 +249,11 @@ def test_refused_calls():
         GraphDecodeRunner(model, cache, beams=3)
     with pytest.raises(Refused, match="rows"):
         model.generate_beam(_prompt(3, 4), 2, 5, cache=cache)
+    with pytest.raises(Refused, match="a beam"):
+        model.generate_beam(_prompt(2, 4), 0, 5)
+    with pytest.raises(Refused, match="32 at most"):
+        model.generate_beam(_prompt(1, 4), 33, 5)
+    with pytest.raises(Refused, match="a prompt"):
+        model.generate_beam(_prompt(2, 0), 2, 5)
     with pytest.raises(Refused, match="at least one"):
         model.generate_beam(_prompt(2, 4), 2, 0, cache=cache)
