@@ -217,7 +217,7 @@ int lkv_prefill_split_plan(int batch, int max_q, int num_q_heads, int num_kv_hea
  *   o_parts   fp32, part p at o_parts + p * o_part_stride: [rows, head_dim]
  *             (normalised partial outputs)
  *   lse_parts fp32, part p at lse_parts + p * lse_part_stride: [rows]
- *             (natural log, -inf = empty)
+ *             (natural log, -inf = empty; NaN makes the merged row and its LSE NaN)
  *   out       bf16 [rows, head_dim] = out_scale[row % num_q_heads] * merged
  *   lse_out   fp32 [rows] (optional)
  * rows = tokens * num_q_heads; strides in elements, 0 = packed (rows * head_dim,

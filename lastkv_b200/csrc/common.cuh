@@ -309,6 +309,13 @@ __device__ __forceinline__ float fmax3f(float a, float b, float c) {
   return d;
 }
 
+// max(a, b), NaN where either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 // Two 2^x on the FMA pipe (f32x2), for softmax exponentials moved off the SFU.
 // Range reduction x = j + f with j = round(x), f in [-0.5, 0.5]: adding
 // 1.5 * 2^23 rounds x to an integer held in the low mantissa bits of t; then

@@ -81,7 +81,7 @@ __device__ __forceinline__ void cp_merge_row(const uint64_t* slot_base, int64_t 
             to2;
   float M = my_ls;
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+  for (int off = 16; off > 0; off >>= 1) M = max_nan(M, __shfl_xor_sync(0xffffffffu, M, off));
   float acc[PER];
 #pragma unroll
   for (int e = 0; e < PER; ++e) acc[e] = 0.f;
@@ -113,7 +113,7 @@ __device__ __forceinline__ void cp_merge_row(const uint64_t* slot_base, int64_t 
       }
     }
   }
-  const float inv = L > 0.f ? 1.f / L : 0.f;
+  const float inv = L == 0.f ? 0.f : 1.f / L;
   const int h = (int)(row % Hq);
   const int64_t tok = row / Hq;
   const float sc = (out_scale ? out_scale[h] : 1.f) * inv;

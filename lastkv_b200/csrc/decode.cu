@@ -84,7 +84,8 @@ constexpr int kMaxTouched = 32;
 //   part s of the row: o at o_base + s * o_step (D floats), LSE at lse_base + s * lse_step
 //   to2 converts the stored LSE to log2 units.  Returns this lane's D / 32
 //   weighted sums in acc (unnormalised), their normaliser in inv (1 / sum of
-//   weights, 0 when empty) and the log2 LSE in lse2.
+//   weights, 0 when empty) and the log2 LSE in lse2.  A part whose LSE is NaN makes
+//   all three NaN.
 template <int D>
 __device__ __forceinline__ void merge_row_parts(const float* o_base, int64_t o_step, const float* lse_base,
                                                 int64_t lse_step, int S, float to2, int lane,
@@ -116,7 +117,7 @@ __device__ __forceinline__ void merge_row_parts(const float* o_base, int64_t o_s
   const float my_ls = lane < S ? __ldcg(lse_base + lane * lse_step) * to2 : -INFINITY;
   float M = my_ls;
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+  for (int off = 16; off > 0; off >>= 1) M = max_nan(M, __shfl_xor_sync(0xffffffffu, M, off));
 #pragma unroll
   for (int e = 0; e < PER; ++e) acc[e] = 0.f;
   float L = 0.f;
@@ -141,8 +142,8 @@ __device__ __forceinline__ void merge_row_parts(const float* o_base, int64_t o_s
       }
     }
   }
-  inv = L > 0.f ? 1.f / L : 0.f;
-  lse2 = L > 0.f ? M + log2f(L) : -INFINITY;
+  inv = L == 0.f ? 0.f : 1.f / L;
+  lse2 = L == 0.f ? -INFINITY : M + log2f(L);
 }
 
 // Context parallel: merge one row's S split partials (merge_partials_kernel's
@@ -661,9 +662,9 @@ __global__ void __launch_bounds__(128) merge_partials_kernel(const MergeParams p
   } else {
     // general path (more than 32 parts): the same arithmetic, one part at a time
     float M = -INFINITY;
-    for (int s = lane; s < p.S; s += 32) M = fmaxf(M, lse_at(s));
+    for (int s = lane; s < p.S; s += 32) M = max_nan(M, lse_at(s));
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    for (int off = 16; off > 0; off >>= 1) M = max_nan(M, __shfl_xor_sync(0xffffffffu, M, off));
 #pragma unroll
     for (int e = 0; e < PER; ++e) acc[e] = 0.f;
     float L = 0.f;
@@ -678,8 +679,8 @@ __global__ void __launch_bounds__(128) merge_partials_kernel(const MergeParams p
         for (int e = 0; e < PER; ++e) acc[e] += w * src[e];
       }
     }
-    inv = L > 0.f ? 1.f / L : 0.f;
-    lse2 = L > 0.f ? M + log2f(L) : -INFINITY;
+    inv = L == 0.f ? 0.f : 1.f / L;
+    lse2 = L == 0.f ? -INFINITY : M + log2f(L);
   }
   const int h = (int)(row % p.Hq);
   const int64_t tok = row / p.Hq;

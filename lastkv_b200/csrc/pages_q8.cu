@@ -22,12 +22,6 @@ namespace {
 
 constexpr int kWarps = 4;
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-
 struct QuantParams {
   const __nv_bfloat16* pool[2];  // keys, values
   int64_t pool_pages;

@@ -594,8 +594,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ok) {
       const int hq = hk * GROUP + r % GROUP;
       const bool valid = tok < Lq;
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      const float lse_e = l > 0.f ? (m + log2f(l) - (Q8 ? kWeightLog2 : 0.f)) * 0.6931471805599453f : -INFINITY;
+      // no key that this row sees: zeros (the sum is not 0 beside rows that see some: ex2_poly2's 2^-125 for each
+      // masked key); a sum that is not a number stays one, in the LSE too, by which the splits are merged
+      const bool none = l == 0.f || (m == -INFINITY && l == l);
+      const float inv = none ? 0.f : 1.f / l;
+      const float lse_e = none ? -INFINITY : (m + log2f(l) - (Q8 ? kWeightLog2 : 0.f)) * 0.6931471805599453f;
       const int64_t row = (int64_t)(q0 + (valid ? tok : 0)) * p.Hq + hq;
       if (p.S > 1) {
         // this split's normalised partial (fp32) and its natural-log LSE
