@@ -848,7 +848,8 @@ int decode_paged_q8(const DecodeQ8Args& a) {
   // slots are counted in 32 bits
   if ((int64_t)a.batch * a.num_q_heads > INT_MAX / 2 ||
       (int64_t)a.batch * a.num_kv_heads * (a.max_pages_per_seq + kPieceCost) > INT_MAX) return LKV_ERR_UNSUPPORTED;
-  if (!a.q || !a.codes || !a.scales || !a.block_table || !a.seq_k || !a.out) return LKV_ERR_INVALID_ARGUMENT;
+  if (!a.q || !a.codes || !a.scales || (!a.block_table && a.max_pages_per_seq) || !a.seq_k || !a.out)
+    return LKV_ERR_INVALID_ARGUMENT;
   if (a.q8_pages < 0 || a.q8_pages > INT32_MAX || a.num_pages < 0 || a.num_pages > INT32_MAX)
     return LKV_ERR_INVALID_ARGUMENT;
   auto off = [](const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; };

@@ -197,12 +197,12 @@ struct DequantParams {
   const int32_t* pages;
   const int32_t* out_pages;
   int64_t n;
-  // or the leading columns of block tables: row b's column j becomes page b * width + j
+  // or the `columns` leading ones of block tables: row b's column j becomes page b * width + j
   const int32_t* bt;
   int64_t bt_stride;
   const int32_t* num_q8;  // or null: every column
   const int32_t* seq_k;
-  int batch, W, width;
+  int batch, W, width, columns;
 };
 
 // Back to rows of bf16, one warp per (page, head, keys or values), through a byte tile in shared memory:
@@ -224,12 +224,12 @@ __global__ void __launch_bounds__(kWarps * 32) dequantise_pages_kernel(const Deq
   const int64_t n = (item >> 1) / p.hkv;
   int64_t src, dst;
   if constexpr (STAGE) {
-    const int b = (int)(n / p.width), j = (int)(n % p.width);
+    const int b = (int)(n / p.columns), j = (int)(n % p.columns);
     if (b >= p.batch) return;
     const int pages = min((max(p.seq_k[b], 0) + kPageTokens - 1) / kPageTokens, p.W);
     if (j >= (p.num_q8 ? min(p.num_q8[b], pages) : pages)) return;
     src = p.bt[(int64_t)b * p.bt_stride + j];
-    dst = n;
+    dst = (int64_t)b * p.width + j;
   } else {
     if (n >= p.n) return;
     src = p.pages[n];
@@ -448,10 +448,10 @@ int dequantise_pages(const void* codes, const float* scales, int64_t q8_pages, c
 int stage_pages(const void* codes, const float* scales, int64_t q8_pages, const int32_t* bt, int64_t bt_stride,
                 const int32_t* num_q8, const int32_t* seq_k, int batch, int W, void* stage_k, void* stage_v, int width,
                 int hkv, int d, int* err, cudaStream_t stream) {
-  if (batch < 0 || W < 0 || width < 0 || width > W) return LKV_ERR_INVALID_ARGUMENT;
-  if (batch == 0 || width == 0) return LKV_OK;
-  const int64_t n = (int64_t)batch * width;
-  const int st = check_pages(stage_k, stage_v, n, codes, scales, q8_pages, hkv, d);
+  if (batch < 0 || W < 0 || width < 0) return LKV_ERR_INVALID_ARGUMENT;
+  const int columns = std::min(width, W);
+  if (batch == 0 || columns == 0) return LKV_OK;
+  const int st = check_pages(stage_k, stage_v, (int64_t)batch * width, codes, scales, q8_pages, hkv, d);
   if (st != LKV_OK) return st;
   if (!bt || !seq_k) return LKV_ERR_INVALID_ARGUMENT;
   DequantParams p{};
@@ -460,7 +460,7 @@ int stage_pages(const void* codes, const float* scales, int64_t q8_pages, const 
   p.q8_pages = q8_pages;
   p.pool[0] = static_cast<__nv_bfloat16*>(stage_k);
   p.pool[1] = static_cast<__nv_bfloat16*>(stage_v);
-  p.pool_pages = n;
+  p.pool_pages = (int64_t)batch * width;
   p.hkv = hkv;
   p.err = err;
   p.bt = bt;
@@ -470,7 +470,8 @@ int stage_pages(const void* codes, const float* scales, int64_t q8_pages, const 
   p.batch = batch;
   p.W = W;
   p.width = width;
-  return launch_dequantise(p, n, d, true, stream);
+  p.columns = columns;
+  return launch_dequantise(p, (int64_t)batch * columns, d, true, stream);
 }
 
 int reorder_pages(void* const* pools, const int64_t* page_bytes, const int64_t* pages, int num_pools,

@@ -703,7 +703,8 @@ int check_args(const PrefillArgs& a, bool* empty) {
   }
   const bool q8 = a.stage_k != nullptr;
   const bool pool = a.pool_k && a.pool_v && a.num_pages > 0;
-  if (!a.q || (!pool && !q8) || !a.block_table || !a.seq_k || !a.cu_q || !a.out) return LKV_ERR_INVALID_ARGUMENT;
+  if (!a.q || (!pool && !q8) || (!a.block_table && a.max_pages_per_seq) || !a.seq_k || !a.cu_q || !a.out)
+    return LKV_ERR_INVALID_ARGUMENT;
   if (q8 && (!a.stage_v || !a.q8_scales || a.stage_width < 1 || (int64_t)a.stage_width * a.batch >= INT32_MAX ||
              a.q8_pages < 0))
     return LKV_ERR_INVALID_ARGUMENT;
