@@ -1292,8 +1292,9 @@ def prefill_paged_q8(q, cache: PagesQ8, block_table, seq_k, cu_q, max_q: int, *,
     """``prefill_paged`` over a cache whose older pages are in 8 bits (lkv_prefill_paged_q8).
 
     The arguments of ``prefill_paged``, with the pages as in ``decode_paged_q8``.  The 8-bit pages'
-    codes are first copied to ``stage`` as bf16; ``staged=True`` says that an
-    earlier call with the same rows and pages did that (the layers of one step), and skips it.
+    codes are first copied to ``stage``; ``staged=True`` says that an earlier call with the same rows and
+    pages and this stage did that (the layers of one step; its ``max_pages`` may differ, as long as it saw the
+    8-bit pages), and skips it.
     A row may have at most ``stage.width`` 8-bit pages.  ``kv_splits`` and ``partials`` as for
     ``prefill_paged`` (causal calls may split their keys too).
     """
@@ -1323,7 +1324,7 @@ def prefill_paged_q8(q, cache: PagesQ8, block_table, seq_k, cu_q, max_q: int, *,
                   "call's CUDA device")
         part_o, part_lse = o.data_ptr(), e.data_ptr()
     st = _capi.lib().lkv_prefill_paged_q8(
-        q.data_ptr(), q_row, codes, scales, q8_pages, sk, sv, max(min(stage.width, W), 1), int(staged), k, v, num, table,
+        q.data_ptr(), q_row, codes, scales, q8_pages, sk, sv, stage.width, int(staged), k, v, num, table,
         t_row, nq8, seq, _ints(cu_q, B + 1, dev, "cu_q"), out.data_ptr(), o_row, l, f, B, T, int(max_q), Hq, h, D, W,
         int(bool(causal)), D ** -0.5 if softmax_scale is None else softmax_scale, kv_splits, part_o, part_lse,
         _err_ptr(error_word), _raw_stream(dev))

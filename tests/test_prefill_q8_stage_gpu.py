@@ -37,6 +37,21 @@ def _check(t, q, cu, out):
         assert_within(out[c[b]:c[b + 1]], ref, bound, f"row {b}")
 
 
+@pytest.mark.parametrize("first,second", [(60, 25), (25, 60), (None, 25), (25, None)])
+@pytest.mark.parametrize("width", [20, 33, 70])
+def test_calls_of_other_widths_share_a_stage(first, second, width):
+    """A table with room behind its rows, of which two calls see different numbers of columns."""
+    t, q, cu, cache = _case()
+    wide = torch.full((3, 60), -5, dtype=torch.int32, device="cuda")
+    wide[:, :25] = t["table"][:, :25]
+    small = dict(t, table=wide)
+    stage = ops.StageQ8.empty(3, width, 2, 64)
+    a = _call(small, q, cu, cache, stage=stage, max_pages=first)
+    _check(t, q, cu, a)
+    b = _call(small, q, cu, cache, stage=stage, max_pages=second, staged=True)
+    assert torch.equal(a, b)
+
+
 def test_a_table_without_columns():
     t, q, cu, cache = _case()
     empty = torch.zeros(3, dtype=torch.int32, device="cuda")
