@@ -15,7 +15,8 @@
 // - p * value scale: with t = s + log2(value scale) and M its running maximum, the product is 2^(t - M)
 //   whatever the scales are, in 0 .. 1; times 2^15 it uses f16's whole range, 11 bits down to
 //   2^-29 of the largest and 2^-40 of it as the smallest step.  A token's part of the sum of weights is that
-//   number (in fp32) divided by the value scale.
+//   number (in fp32) divided by the value scale; the scales of a row may lie 2^90 apart (zero aside), further the
+//   number flushes to 0 for tokens that still count.
 // bf16 pages keep bf16 operands, and the same M with a value scale of 1.
 //
 // Bound by HBM: an 8-bit page is half a bf16 page's bytes.  Work is counted in slots of equal bytes, one bf16
@@ -123,9 +124,11 @@ __device__ __forceinline__ void async_copy_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// Value scales below this count as this: the sum of weights, times their reciprocals, stays finite for
-// rows of 2^20 keys and more (2^15 * 2^90 * 2^20).
+// Value scales below this are taken as this in the maximum: the sum of weights, times their reciprocals, stays finite for
+// rows of 2^20 keys and more (2^15 * 2^90 * 2^20).  Blocks of zeros are such, beside scales of any size: their
+// weights times the scale would be below fp32's least from scales of 2^51 on, so the sum takes 2^(s - M) for them.
 constexpr float kMinValueScale = 8.0779357e-28f;  // 2^-90
+constexpr float kMinValueScaleLog2 = -90.f;
 constexpr float kWeightLog2 = 15.f;               // weights of the products are times 2^15
 
 // The slots of row b.
@@ -488,6 +491,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const bool two = 2 * sl + 1 < x.r.nh;
         const int left = min(x.r.n, x.r.nh * kPageTokens) - 2 * sl * kPageTokens;  // 8-bit keys from here on, >= 1
         float sc[2][4], iv[2][2];
+        bool tiny = false;  // a value scale below kMinValueScale, the same for the warp
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float sd[4] = {0.f, 0.f, 0.f, 0.f};
@@ -510,10 +514,12 @@ __global__ void __launch_bounds__(kThreads, 2)
           // blocks past the row's end: whatever their scales hold
           if (16 * e >= left) f.x = 0.f, f.z = 1.f;
           if (16 * e + 8 >= left) f.y = 0.f, f.w = 1.f;
-          const float v0 = f.z < kMinValueScale ? kMinValueScale : f.z, v1 = f.w < kMinValueScale ? kMinValueScale : f.w;
+          const bool t0 = f.z < kMinValueScale, t1 = f.w < kMinValueScale;
+          tiny |= t0 || t1;
+          const float v0 = t0 ? kMinValueScale : f.z, v1 = t1 ? kMinValueScale : f.w;
           const float g0 = lg2_approx(v0), g1 = lg2_approx(v1);
-          iv[e][0] = __fdividef(1.f, v0);
-          iv[e][1] = __fdividef(1.f, v1);
+          iv[e][0] = t0 ? 0.f : __fdividef(1.f, v0);
+          iv[e][1] = t1 ? 0.f : __fdividef(1.f, v1);
           sc[e][0] = fmaf(sc[e][0] + sd[0], f.x * q0, g0);
           sc[e][1] = fmaf(sc[e][1] + sd[1], f.x * q1, g0);
           sc[e][2] = fmaf(sc[e][2] + sd[2], f.y * q0, g1);
@@ -529,6 +535,21 @@ __global__ void __launch_bounds__(kThreads, 2)
         float r0, r1;
         raise(fmaxf(fmaxf(sc[0][0], sc[0][2]), fmaxf(sc[1][0], sc[1][2])),
               fmaxf(fmaxf(sc[0][1], sc[0][3]), fmaxf(sc[1][1], sc[1][3])), r0, r1);
+        if (tiny) {  // those blocks' weights in the sum, by themselves (2^105 at most: M is no less than s - 90)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 v = *reinterpret_cast<const float2*>(&scp[e].z);  // (keys that are not there have scores of -inf)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const float w = ex2_approx(sc[e][y] - kMinValueScaleLog2 - (y & 1 ? r1 : r0));
+              const float own = y & 2 ? v.y : v.x;
+              if (own < kMinValueScale) {
+                (y & 1 ? l1 : l0) += w;
+                sc[e][y] += lg2_approx(own) - kMinValueScaleLog2;  // the product's weight, of its own scale: 0 for 0
+              }
+            }
+          }
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll

@@ -1,0 +1,63 @@
+"""Blocks of zeros beside large values: their tokens keep their weight, and only theirs."""
+
+import pytest
+import torch
+
+from lastkv_b200 import ops
+from tests.q8_helpers import FP32_HALF_STEP, assert_within, attention, random_cache, row_keys
+
+pytestmark = pytest.mark.gpu
+
+
+def _check_lse(lse, q, k, weight_error=0.0, causal_from=None):
+    """Log-sum-exps [L, Hq] of one row: a weight's relative error is one of the sum's, a score's (a sum of D products,
+    and its scaling) one of its exponential's; the sum itself has n roundings, the logarithm's last steps some of its size."""
+    n, D = k.shape[0], q.shape[2]
+    k = k.repeat_interleave(q.shape[1] // k.shape[1], 1)
+    x = torch.einsum("lhd,nhd->lhn", q.double(), k) * D ** -0.5
+    off = torch.einsum("lhd,nhd->lhn", q.double().abs(), k.abs()).amax(-1) * D ** -0.5
+    if causal_from is not None:
+        late = torch.arange(n, device=x.device)[None] > causal_from + torch.arange(x.shape[0], device=x.device)[:, None]
+        x = x.masked_fill(late[:, None], float("-inf"))
+    want = torch.logsumexp(x, -1)
+    # the largest value scale goes through the running maximum and back: 128 at most as its logarithm
+    tol = 2 * weight_error + (4 * D * off + 2 * n + 4 * want.abs() + 4 * 128) * FP32_HALF_STEP
+    assert bool(((lse.double() - want).abs() <= tol).all()), float((lse.double() - want).abs().max())
+
+
+def _cache(seed, lens, num_q8, power, d, low=0.0):
+    """Values of about 2^power, every third half page of value scale `low`."""
+    t = random_cache(seed, lens, num_q8, 2, d)
+    t["vs"] *= 2.0 ** power
+    t["pool_v"] = (t["pool_v"].float() * 2.0 ** power).bfloat16()
+    half = torch.arange(t["vs"].shape[0] * 2, device="cuda").view(-1, 2) % 3 == 1
+    t["vs"] = torch.where(half[..., None], low, t["vs"]).contiguous()
+    return t
+
+
+@pytest.mark.parametrize("power", [20, 40, 60, 90])
+@pytest.mark.parametrize("lens,num_q8", [([300, 90], [9999, 9999]), ([9000, 20], [9999, 1]), ([700, 40], [20, 2])])
+def test_single_tokens(power, lens, num_q8):
+    t = _cache(51, lens, num_q8, power, 128)
+    q = torch.randn((2, 4, 128), generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    cache = ops.PagesQ8.from_codes(t["k"], t["v"], t["ks"], t["vs"])
+    lse = torch.empty((2, 4), device="cuda")
+    out = ops.decode_paged_q8(q, cache, t["table"], t["seq_k"], num_q8=t["num_q8"], pool_k=t["pool_k"],
+                              pool_v=t["pool_v"], lse=lse)
+    for b in range(2):
+        k, v = row_keys(t, b)
+        ref, bound = attention(q[b:b + 1], k, v, 128 ** -0.5)
+        assert_within(out[b:b + 1], ref, bound, f"row {b}")
+        _check_lse(lse[b:b + 1], q[b:b + 1], k)
+
+
+def test_a_row_of_zero_blocks():
+    """Nothing but zeros as values: zeros, and the log-sum-exp of the scores."""
+    t = random_cache(53, [200], [9999], 2, 64)
+    t["vs"].zero_()
+    q = torch.randn((1, 4, 64), generator=torch.Generator().manual_seed(4)).bfloat16().cuda()
+    cache = ops.PagesQ8.from_codes(t["k"], t["v"], t["ks"], t["vs"])
+    lse = torch.empty(q.shape[:2], device="cuda")
+    out = ops.decode_paged_q8(q, cache, t["table"], t["seq_k"], lse=lse)
+    assert bool((out == 0).all())
+    _check_lse(lse, q, row_keys(t, 0)[0])
