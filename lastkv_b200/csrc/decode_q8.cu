@@ -545,7 +545,8 @@ __global__ void __launch_bounds__(kThreads, 2)
               const float own = y & 2 ? v.y : v.x;
               if (own < kMinValueScale) {
                 (y & 1 ? l1 : l0) += w;
-                sc[e][y] += lg2_approx(own) - kMinValueScaleLog2;  // the product's weight, of its own scale: 0 for 0
+                // the product's weight, of its own scale: 0 for 0, and for what lies behind the row's end
+                sc[e][y] = own > 0.f ? sc[e][y] + (lg2_approx(own) - kMinValueScaleLog2) : -INFINITY;
               }
             }
           }

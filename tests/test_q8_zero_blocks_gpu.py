@@ -61,3 +61,19 @@ def test_a_row_of_zero_blocks():
     out = ops.decode_paged_q8(q, cache, t["table"], t["seq_k"], lse=lse)
     assert bool((out == 0).all())
     _check_lse(lse, q, row_keys(t, 0)[0])
+
+
+@pytest.mark.parametrize("behind", [-1.0, float("-inf"), float("nan"), 1e-40])
+def test_what_lies_behind_a_zero_block(behind):
+    """A zero block before the row's end, whatever the scales of the blocks behind it hold; an odd number of pages, so
+    that the last one has no neighbour."""
+    t = random_cache(54, [20, 72, 200], [9999] * 3, 2, 64)
+    q = torch.randn((3, 4, 64), generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+    for b, column, half in ((0, 1, 0), (1, 4, 0), (2, 12, 0)):  # the row's last tokens
+        t["vs"][int(t["table"][b, column]), half] = 0
+        t["vs"][int(t["table"][b, column]), 1 - half] = behind
+    cache = ops.PagesQ8.from_codes(t["k"], t["v"], t["ks"], t["vs"])
+    out = ops.decode_paged_q8(q, cache, t["table"], t["seq_k"])
+    for b in range(3):
+        ref, bound = attention(q[b:b + 1], *row_keys(t, b), 64 ** -0.5)
+        assert_within(out[b:b + 1], ref, bound, f"row {b}")
