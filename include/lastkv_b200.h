@@ -587,8 +587,9 @@ int lkv_q8_dequantize_pages(const uint8_t* codes, const float* scales, int64_t q
  * NULL: all) block-table columns of row b are 8-bit pages, the rest pages of the
  * bf16 pool (pool_k and pool_v may be NULL where there are none).  Either kind may hold
  * the row's last token; keys from seq_k[b] on have no weight, whatever is there.  A row
- * without keys gives zeros and an LSE of -inf.  A value scale below 2^-90 counts as 2^-90
- * (in the prefill too).  Workspace, out, lse, out_scale as for
+ * without keys gives zeros and an LSE of -inf.  The value scales of a row may lie 2^90 apart
+ * (in the prefill too); zeros, and scales below 2^-90, which lose bits there, beside any.
+ * Workspace, out, lse, out_scale as for
  * lkv_decode_paged (lkv_decode_workspace_bytes; a smaller one makes the work's parts
  * fewer); flags: LKV_DECODE_L2_KEEP or 0.  Two calls whose work overlaps need
  * two workspaces.  Everything is read after the launch's dependency wait. */

@@ -324,7 +324,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // (Remez exchange, restated in tests/test_exp2_poly_cpu.py): max relative error
 // 7.5e-5, far below the bf16 rounding (2^-9) applied to softmax weights.
 // Inputs are clamped at -125 (2^-125 instead of the SFU's flush to zero; a
-// masked -inf therefore yields 2^-125, a weight 1e-38 below any visible key's).
+// masked -inf therefore yields 2^-125, a weight 1e-38 below any visible key's where
+// nothing multiplies the weights again; a sum of such weights alone is not 0).
 constexpr float kExp2C0 = 0.99992806f, kExp2C1 = 0.69326097f, kExp2C2 = 0.24261113f, kExp2C3 = 0.05517167f;
 
 __device__ __forceinline__ float2 ex2_poly2(float2 x) {

@@ -124,12 +124,7 @@ __device__ __forceinline__ void async_copy_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// Value scales below this are taken as this in the maximum: the sum of weights, times their reciprocals, stays finite for
-// rows of 2^20 keys and more (2^15 * 2^90 * 2^20).  Blocks of zeros are such, beside scales of any size: their
-// weights times the scale would be below fp32's least from scales of 2^51 on, so the sum takes 2^(s - M) for them.
-constexpr float kMinValueScale = 8.0779357e-28f;  // 2^-90
-constexpr float kMinValueScaleLog2 = -90.f;
-constexpr float kWeightLog2 = 15.f;               // weights of the products are times 2^15
+constexpr float kWeightLog2 = 15.f;  // weights of the products are times 2^15
 
 // The slots of row b.
 struct Row {
@@ -518,8 +513,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           tiny |= t0 || t1;
           const float v0 = t0 ? kMinValueScale : f.z, v1 = t1 ? kMinValueScale : f.w;
           const float g0 = lg2_approx(v0), g1 = lg2_approx(v1);
-          iv[e][0] = t0 ? 0.f : __fdividef(1.f, v0);
-          iv[e][1] = t1 ? 0.f : __fdividef(1.f, v1);
+          iv[e][0] = __fdividef(1.f, v0);
+          iv[e][1] = __fdividef(1.f, v1);
           sc[e][0] = fmaf(sc[e][0] + sd[0], f.x * q0, g0);
           sc[e][1] = fmaf(sc[e][1] + sd[1], f.x * q1, g0);
           sc[e][2] = fmaf(sc[e][2] + sd[2], f.y * q0, g1);
@@ -540,13 +535,16 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int e = 0; e < 2; ++e) {
             const float2 v = *reinterpret_cast<const float2*>(&scp[e].z);  // (keys that are not there have scores of -inf)
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const float w = ex2_approx(sc[e][y] - kMinValueScaleLog2 - (y & 1 ? r1 : r0));
-              const float own = y & 2 ? v.y : v.x;
+            for (int h = 0; h < 2; ++h) {
+              const float own = h ? v.y : v.x;
               if (own < kMinValueScale) {
-                (y & 1 ? l1 : l0) += w;
+                l0 += ex2_approx(sc[e][2 * h] - kMinValueScaleLog2 - r0);  // 2^(s - M)
+                l1 += ex2_approx(sc[e][2 * h + 1] - kMinValueScaleLog2 - r1);
+                iv[e][h] = 0.f;
                 // the product's weight, of its own scale: 0 for 0, and for what lies behind the row's end
-                sc[e][y] = own > 0.f ? sc[e][y] + (lg2_approx(own) - kMinValueScaleLog2) : -INFINITY;
+                const float less = own > 0.f ? lg2_approx(own) - kMinValueScaleLog2 : -INFINITY;
+                sc[e][2 * h] += less;
+                sc[e][2 * h + 1] += less;
               }
             }
           }

@@ -277,6 +277,9 @@ __global__ void __launch_bounds__(kWarps * 32) dequantise_pages_kernel(const Deq
   const bool bad1 = !(fabsf(s.y) < INFINITY) || !(fabsf(s.w) < INFINITY);
   __nv_bfloat16* base = (which ? p.pool[1] : p.pool[0]) + (dst * kPageTokens * p.hkv + hk) * D;
   const int64_t row_stride = (int64_t)p.hkv * D;
+  // staged values of blocks whose scale the prefill kernel takes as kMinValueScale: times what is missing (0 for 0, and
+  // for whatever lies behind a row's end)
+  const float v0 = fminf(fmaxf(s0 * 0x1p90f, 0.f), 1.f), v1 = fminf(fmaxf(s1 * 0x1p90f, 0.f), 1.f);
   const int r0 = lane / LANES, col = (lane % LANES) * 8;
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
@@ -289,7 +292,8 @@ __global__ void __launch_bounds__(kWarps * 32) dequantise_pages_kernel(const Deq
       const uint32_t two = w >> ((e & 1) * 16);
       const float a = (float)((int)(two & 255u) - 128), b = (float)((int)(two >> 8 & 255u) - 128);
       if constexpr (STAGE) {
-        o[e] = which ? pack_f16(a, b) : (r < 8 ? bad0 : bad1) ? 0x7fff7fffu : pack_bf16(a, b);
+        const float v = r < 8 ? v0 : v1;
+        o[e] = which ? pack_f16(a * v, b * v) : (r < 8 ? bad0 : bad1) ? 0x7fff7fffu : pack_bf16(a, b);
       } else {
         const float sc = r < 8 ? s0 : s1;
         o[e] = pack_bf16(a * sc, b * sc);

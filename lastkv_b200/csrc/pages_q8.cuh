@@ -21,6 +21,12 @@ namespace lkv {
 constexpr int kPageTokens = 16;
 constexpr int kScalesPerBlock = 4;  // fp32: keys 0-7, keys 8-15, values 0-7, values 8-15
 
+// Value scales below this are taken as this in the softmax's maximum: the sum of weights, times their reciprocals, stays
+// finite for rows of 2^20 keys and more (2^15 * 2^90 * 2^20).  Blocks of zeros are such, beside scales of any size: their
+// weights times the scale would be below fp32's least from scales of 2^51 on, so the sum takes them without it.
+constexpr float kMinValueScale = 8.0779357e-28f;  // 2^-90
+constexpr float kMinValueScaleLog2 = -90.f;
+
 // Four codes as two pairs of f16: bytes 0 and 2 of w in lo, bytes 1 and 3 in hi.  Exact: the byte q + 128 under
 // f16's 0x64 is 1024 + 128 + q.
 __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {

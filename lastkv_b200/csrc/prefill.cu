@@ -125,10 +125,6 @@ struct PrefillParams {
   int has_pool;
 };
 
-// Value scales below this are taken as this in the weights: the sum of weights, times their reciprocals,
-// stays finite for rows of 2^20 keys and more.
-constexpr float kMinValueScale = 8.0779357e-28f;  // 2^-90
-
 template <int D>
 struct PrefillCfg {
   static constexpr int HALVES = D / 64;
@@ -420,16 +416,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Wait results are made warp-uniform: tcgen05.ld/st below are warp-collective.
     for (int j = 0; j < nb; ++j) {
       float4 kf[4], lv[4];  // Q8
+      uint32_t tiny = 0;    // Q8: the lanes whose value scale is below kMinValueScale
       if constexpr (Q8) {
         float f = next_scale;
         next_scale = scale_of(next_page);
         next_page = page_of(j + 2);
         if (!(fabsf(f) < INFINITY)) f = 1.f;  // the staged keys are NaN there
         const int at = (lane >> 2) * 2 + (lane & 1);
+        const bool small = (lane & 2) && f < kMinValueScale;
+        tiny = __ballot_sync(0xffffffffu, small);
         if (lane & 2) {
-          f = fmaxf(f, kMinValueScale);
+          if (small) f = kMinValueScale;
           group_scale[16 + at] = lg2_approx(f);
-          group_scale[32 + at] = __fdividef(1.f, f);
+          group_scale[32 + at] = small ? 0.f : __fdividef(1.f, f);
         } else {
           group_scale[at] = fmaxf(f, 1e-37f) * sl2;  // codes of zero: not -inf * 0 where they are masked
         }
@@ -536,6 +535,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             if constexpr (TWO) tmem_st16(lane_base + col_s + kBN / 2 + c * 16, rest);
           }
         };
+        if (tiny) {
+          // those groups' weights in the sum, by themselves (2^105 at most: m is no less than s - 98), from the scores as
+          // they still are in TMEM: code in the path of x cost every call 2 %, with heads of 64 9 %
+#pragma unroll 1
+          for (uint32_t left = tiny; left; left &= left - 1) {
+            const int at = __ffs(left) - 1, g = (at >> 2) * 2 + (at & 1);
+            uint32_t raw[8];
+            tmem_ld8(lane_base + col_s + 8 * g, raw);
+            tmem_wait_ld();
+            const float scale = group_scale[g];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (key0 + 8 * g + e <= lim) sp[0].x += ex2_approx(fmaf(__uint_as_float(raw[e]), scale, neg_mref));
+          }
+        }
         if (staged >= kPagesPerBlock) weights(std::false_type{}, std::false_type{});
         else if (two_terms) weights(std::true_type{}, std::true_type{});
         else weights(std::true_type{}, std::false_type{});

@@ -8,6 +8,8 @@ from tests.q8_helpers import FP32_HALF_STEP, assert_within, attention, random_ca
 
 pytestmark = pytest.mark.gpu
 
+POLY = 7.5e-5  # the relative error of the exponentials that a polynomial takes
+
 
 def _check_lse(lse, q, k, weight_error=0.0, causal_from=None):
     """Log-sum-exps [L, Hq] of one row: a weight's relative error is one of the sum's, a score's (a sum of D products,
@@ -51,16 +53,44 @@ def test_single_tokens(power, lens, num_q8):
         _check_lse(lse[b:b + 1], q[b:b + 1], k)
 
 
-def test_a_row_of_zero_blocks():
+@pytest.mark.parametrize("power", [20, 40, 60, 90])
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("d", [64, 128])
+def test_spans(power, splits, d):
+    """Causal spans that end inside a block, so that most blocks have keys that a token does not see."""
+    t = _cache(52, [700, 90, 333], [9999, 9999, 12], power, d)
+    cu = torch.tensor([0, 70, 90, 390], dtype=torch.int32, device="cuda")
+    q = torch.randn((390, 4, d), generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    cache = ops.PagesQ8.from_codes(t["k"], t["v"], t["ks"], t["vs"])
+    lse = torch.empty((390, 4), device="cuda")
+    out = ops.prefill_paged_q8(q, cache, t["table"], t["seq_k"], cu, 300, num_q8=t["num_q8"], pool_k=t["pool_k"],
+                               pool_v=t["pool_v"], kv_splits=splits, lse=lse)
+    c = cu.tolist()
+    for b in range(3):
+        k, v = row_keys(t, b)
+        span = q[c[b]:c[b + 1]]
+        n, L = k.shape[0], span.shape[0]
+        ref, bound = attention(span, k, v, d ** -0.5, n - L, POLY)
+        assert_within(out[c[b]:c[b + 1]], ref, bound, f"row {b}")
+        _check_lse(lse[c[b]:c[b + 1]], span, k, POLY, n - L)
+
+
+@pytest.mark.parametrize("span", [False, True])
+def test_a_row_of_zero_blocks(span):
     """Nothing but zeros as values: zeros, and the log-sum-exp of the scores."""
     t = random_cache(53, [200], [9999], 2, 64)
     t["vs"].zero_()
-    q = torch.randn((1, 4, 64), generator=torch.Generator().manual_seed(4)).bfloat16().cuda()
+    q = torch.randn((2 if span else 1, 4, 64), generator=torch.Generator().manual_seed(4)).bfloat16().cuda()
     cache = ops.PagesQ8.from_codes(t["k"], t["v"], t["ks"], t["vs"])
     lse = torch.empty(q.shape[:2], device="cuda")
-    out = ops.decode_paged_q8(q, cache, t["table"], t["seq_k"], lse=lse)
+    if span:
+        cu = torch.tensor([0, 2], dtype=torch.int32, device="cuda")
+        out = ops.prefill_paged_q8(q, cache, t["table"], t["seq_k"], cu, 2, causal=False, lse=lse)
+    else:
+        out = ops.decode_paged_q8(q, cache, t["table"], t["seq_k"], lse=lse)
+    k, _ = row_keys(t, 0)
     assert bool((out == 0).all())
-    _check_lse(lse, q, row_keys(t, 0)[0])
+    _check_lse(lse, q, k, POLY)
 
 
 @pytest.mark.parametrize("behind", [-1.0, float("-inf"), float("nan"), 1e-40])
@@ -73,7 +103,9 @@ def test_what_lies_behind_a_zero_block(behind):
         t["vs"][int(t["table"][b, column]), half] = 0
         t["vs"][int(t["table"][b, column]), 1 - half] = behind
     cache = ops.PagesQ8.from_codes(t["k"], t["v"], t["ks"], t["vs"])
-    out = ops.decode_paged_q8(q, cache, t["table"], t["seq_k"])
-    for b in range(3):
-        ref, bound = attention(q[b:b + 1], *row_keys(t, b), 64 ** -0.5)
-        assert_within(out[b:b + 1], ref, bound, f"row {b}")
+    cu = torch.arange(4, dtype=torch.int32, device="cuda")
+    for out in (ops.decode_paged_q8(q, cache, t["table"], t["seq_k"]),
+                ops.prefill_paged_q8(q, cache, t["table"], t["seq_k"], cu, 1)):
+        for b in range(3):
+            ref, bound = attention(q[b:b + 1], *row_keys(t, b), 64 ** -0.5, None, POLY)
+            assert_within(out[b:b + 1], ref, bound, f"row {b}")
