@@ -452,11 +452,13 @@ __global__ void __launch_bounds__(kThreads, 2)
     auto raise = [&](float t0, float t1, float& r0, float& r1) {
       const float n0 = fmaxf(m0, max_over_rows(t0)), n1 = fmaxf(m1, max_over_rows(t1));
       if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
-        const float a0 = m0 == n0 ? 1.f : ex2_approx(m0 - n0), a1 = m1 == n1 ? 1.f : ex2_approx(m1 - n1);
+        // (the sums in two steps: they may be 2^105, of zero blocks, so that a factor below fp32's least still counts)
+        const float h0 = m0 == n0 ? 1.f : ex2_approx(0.5f * (m0 - n0)), h1 = m1 == n1 ? 1.f : ex2_approx(0.5f * (m1 - n1));
+        const float a0 = h0 * h0, a1 = h1 * h1;
         m0 = n0;
         m1 = n1;
-        l0 *= a0;
-        l1 *= a1;
+        l0 = l0 * h0 * h0;
+        l1 = l1 * h1 * h1;
 #pragma unroll
         for (int k = 0; k < KT; ++k) {
           o[k][0] *= a0;
@@ -669,8 +671,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
         for (int v = 0; v < kNW; ++v) {
-          const float m = jm[v * 8 + h];
-          L = fmaf(jl[v * 8 + h], m == M ? 1.f : ex2_approx(m - M), L);
+          const float m = jm[v * 8 + h], half = m == M ? 1.f : ex2_approx(0.5f * (m - M));
+          L = fmaf(jl[v * 8 + h] * half, half, L);
           const float2 part = *reinterpret_cast<const float2*>(jo + (v * 2 + hl) * Cfg::OSTRIDE + d);
           acc.x += part.x;
           acc.y += part.y;

@@ -171,6 +171,46 @@ struct StageMaps {
 };
 struct NoStageMaps {};
 
+// Q8: a sum against a maximum larger by -`by`.  In two steps: it may be 2^105, so that one below fp32's least still counts.
+__device__ __forceinline__ float lowered(float l, float by) {
+  const float half = ex2_approx(0.5f * by);
+  return l * half * half;
+}
+
+// Q8: the weights of a block's groups of keys with value scales below kMinValueScale (`tiny`: their lanes) in a row's
+// sum, by themselves and before the block's others, against a maximum raised to what those groups have in it (so
+// 2^105 at most): the row's m, l and what O loses by that.  The scores are in TMEM still.  A call, and where no scores
+// are held in registers: the same code between them and their exponentials cost every call 2-9 %, in line here 5 %
+// with heads of 64 (this 2.5).
+__device__ __noinline__ float3 sum_zero_groups(uint32_t tiny, uint32_t scores, const float* group_scale, int last,
+                                               float m, float l) {
+  float alpha0 = 1.f;
+  auto each = [&](auto take) {
+#pragma unroll 1
+    for (uint32_t left = tiny; left; left &= left - 1) {
+      const int at = __ffs(left) - 1, g = (at >> 2) * 2 + (at & 1);
+      uint32_t raw[8];
+      tmem_ld8(scores + 8 * g, raw);
+      tmem_wait_ld();
+      const float scale = group_scale[g];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (8 * g + e <= last) take(__uint_as_float(raw[e]) * scale);
+    }
+  };
+  float top = -INFINITY;
+  each([&](float t) { top = fmaxf(top, t); });
+  top += kMinValueScaleLog2;
+  if (top > m + kRescaleLog2) {
+    alpha0 = (m == -INFINITY) ? 0.f : ex2_approx(m - top);
+    l = lowered(l, m - top);
+    m = top;
+  }
+  const float ref = kWeightLog2 - (m == -INFINITY ? 0.f : m);
+  each([&](float t) { l += ex2_approx(t + ref); });
+  return make_float3(m, l, alpha0);
+}
+
 template <int D, int GROUP, bool Q8>
 __global__ void __launch_bounds__(kThreads, 1)
     prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
@@ -442,6 +482,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[t], j & 1));
       tc_fence_after();
       if (!ok) break;
+      const int key0 = (j0 + j) * kBN;
+      float alpha0 = 1.f;  // what O has lost before its block's maximum
+      if constexpr (Q8) {
+        if (__builtin_expect(tiny != 0, 0)) {
+          const float3 r = sum_zero_groups(tiny, lane_base + col_s, group_scale, lim - key0, m, l);
+          m = r.x;
+          l = r.y;
+          alpha0 = r.z;
+        }
+      }
       // raw scores; the softmax scale is folded into one FFMA per element below
       float x[kBN];
       {
@@ -454,7 +504,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e) x[c * 32 + e] = __uint_as_float(raw[c][e]);
       }
-      const int key0 = (j0 + j) * kBN;
       if (key0 + kBN - 1 > lim) {
 #pragma unroll
         for (int e = 0; e < kBN; ++e)
@@ -488,6 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float alpha = 1.f;
       if (mx > m + kRescaleLog2) {
         alpha = (m == -INFINITY) ? 0.f : ex2_approx(m - mx);
+        if constexpr (Q8) l = lowered(l, m - mx);
         m = mx;
       }
       const float neg_mref = (m == -INFINITY) ? 0.f : (Q8 ? kWeightLog2 : 0.f) - m;
@@ -508,6 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float4 iv = load4(group_scale + 32 + 4 * c);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
+              const bool f16 = !MIXED || 2 * c + (g >> 1) < staged;
               const float scale = (&kf[c].x)[g], add = (&lv[c].x)[g] + neg_mref;
               const float2 scalev = make_float2(scale, scale), addv = make_float2(add, add);
               float2 gs = make_float2(0.f, 0.f), pv[4];
@@ -518,7 +569,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 pv[q] = q == (g & 1) ? ex2_poly2(a) : make_float2(ex2_approx(a.x), ex2_approx(a.y));
                 gs = __fadd2_rn(gs, pv[q]);
               }
-              const bool f16 = !MIXED || 2 * c + (g >> 1) < staged;
 #pragma unroll
               for (int q = 0; q < 4; ++q) pc[g * 4 + q] = f16 ? pack_f16(pv[q].x, pv[q].y) : pack_bf16(pv[q].x, pv[q].y);
               if constexpr (TWO) {
@@ -535,21 +585,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             if constexpr (TWO) tmem_st16(lane_base + col_s + kBN / 2 + c * 16, rest);
           }
         };
-        if (tiny) {
-          // those groups' weights in the sum, by themselves (2^105 at most: m is no less than s - 98), from the scores as
-          // they still are in TMEM: code in the path of x cost every call 2 %, with heads of 64 9 %
-#pragma unroll 1
-          for (uint32_t left = tiny; left; left &= left - 1) {
-            const int at = __ffs(left) - 1, g = (at >> 2) * 2 + (at & 1);
-            uint32_t raw[8];
-            tmem_ld8(lane_base + col_s + 8 * g, raw);
-            tmem_wait_ld();
-            const float scale = group_scale[g];
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (key0 + 8 * g + e <= lim) sp[0].x += ex2_approx(fmaf(__uint_as_float(raw[e]), scale, neg_mref));
-          }
-        }
         if (staged >= kPagesPerBlock) weights(std::false_type{}, std::false_type{});
         else if (two_terms) weights(std::true_type{}, std::true_type{});
         else weights(std::true_type{}, std::false_type{});
@@ -569,7 +604,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       const float sum = ((sp[0].x + sp[0].y) + (sp[1].x + sp[1].y)) + ((sp[2].x + sp[2].y) + (sp[3].x + sp[3].y));
-      l = l * alpha + sum;
+      l = Q8 ? l + sum : l * alpha + sum;
+      if constexpr (Q8) alpha *= alpha0;
       if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
         // O holds blocks < j once PV(j-1) is complete; rescale it in TMEM
         ok = __all_sync(0xffffffffu, mbar_wait(&bars->pv_done[t], (j - 1) & 1));

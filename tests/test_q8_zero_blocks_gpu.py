@@ -109,3 +109,27 @@ def test_what_lies_behind_a_zero_block(behind):
         for b in range(3):
             ref, bound = attention(q[b:b + 1], *row_keys(t, b), 64 ** -0.5, None, POLY)
             assert_within(out[b:b + 1], ref, bound, f"row {b}")
+
+
+@pytest.mark.parametrize("power", [0, 30, 50, 90])
+@pytest.mark.parametrize("zeros", ["first", "last"])
+def test_pages_of_zeros_and_pages_of_large_values(power, zeros):
+    """Hundreds of keys whose values are zeros, before or behind those whose values are not."""
+    n, d = 1600, 64
+    t = random_cache(55, [n], [9999], 2, d)
+    t["vs"] *= 2.0 ** power
+    pages = t["table"][0].long()
+    t["vs"][pages[:60] if zeros == "first" else pages[-60:]] = 0
+    q = torch.randn((3, 4, d), generator=torch.Generator().manual_seed(6)).bfloat16().cuda()
+    cache = ops.PagesQ8.from_codes(t["k"], t["v"], t["ks"], t["vs"])
+    k, v = row_keys(t, 0)
+    ref, bound = attention(q, k, v, d ** -0.5, None, POLY)
+    lse = torch.empty((3, 4), device="cuda")
+    out = ops.decode_paged_q8(q, cache, t["table"].expand(3, -1), t["seq_k"].expand(3).contiguous(), lse=lse)
+    assert_within(out, ref, bound, "tokens")
+    _check_lse(lse, q, k)
+    cu = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    for splits in (1, 3):
+        out = ops.prefill_paged_q8(q, cache, t["table"], t["seq_k"], cu, 3, causal=False, kv_splits=splits, lse=lse)
+        assert_within(out, ref, bound, f"span in {splits} parts")
+        _check_lse(lse, q, k, POLY)
