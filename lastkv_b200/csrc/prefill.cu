@@ -51,7 +51,8 @@
 // the maximum once per group and into the FFMA in front of the exponential.  A value scale v multiplies the
 // weights that PV takes, p v = 2^(s + log2 v - m): it goes into that FFMA's addend (and into the maximum, so
 // that f16 holds them), and a group's sum of them times 1 / v is its part of the row's sum.  No instruction per
-// key is added.  Pages in bf16 have scales of one.
+// key is added.  Pages in bf16 have scales of one; in a block of both kinds they count in the maximum with the
+// scale of its 8-bit values, if that is smaller: their weights are bf16, which holds what is above f16's range.
 // A page is one step of PV, 16 keys, so its type is chosen page by page: staged pages have values and weights in
 // f16, times 2^7, whose rounding is lost in the output's (bf16 weights are not 1 where the largest is, as they are
 // without scales, and took the error from 1.0 to 1.4, in short rows 1.7, times the output's rounding); bf16
@@ -91,6 +92,7 @@ constexpr int kWarpK = 8, kWarpV = 9, kWarpK2 = 10, kWarpMma = 11;
 constexpr int kThreads = 12 * 32;
 constexpr int kStagesK = 2, kStagesV = 3;
 constexpr float kRescaleLog2 = 8.0f;
+constexpr float kLeastPageScale = 0x1p-60f;  // Q8: bf16 pages' weights are 2^75 at most
 constexpr float kWeightLog2 = 7.0f;  // Q8: weights are times 2^7, so that f16 has 2^15 for the largest
 // Q8: registers of a softmax thread, and of the others, of the 168 that each was launched with (8 warps gain
 // what 4 lose).  Two spans of 1024 tokens over 8192 keys: 223 us, with 168 each 239; the scales of a block then fit
@@ -463,12 +465,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         next_page = page_of(j + 2);
         if (!(fabsf(f) < INFINITY)) f = 1.f;  // the staged keys are NaN there
         const int at = (lane >> 2) * 2 + (lane & 1);
+        const int here = nh - (j0 + j) * kPagesPerBlock;  // pages of this block in 8 bits
+        if (here > 0 && here < kPagesPerBlock) {
+          // both kinds: its bf16 pages count in the maximum with the scale of its 8-bit values, if that is below 1
+          float top = (lane & 2) && (lane >> 2) < here ? f : 0.f;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          if ((lane & 2) && (lane >> 2) >= here && top >= kMinValueScale) f = fminf(fmaxf(top, kLeastPageScale), 1.f);
+        }
         const bool small = (lane & 2) && f < kMinValueScale;
         tiny = __ballot_sync(0xffffffffu, small);
         if (lane & 2) {
           if (small) f = kMinValueScale;
           group_scale[16 + at] = lg2_approx(f);
-          group_scale[32 + at] = small ? 0.f : __fdividef(1.f, f);
+          group_scale[32 + at] = small ? 0.f : (lane >> 2) < here ? __fdividef(1.f, f) : 1.f;
         } else {
           group_scale[at] = fmaxf(f, 1e-37f) * sl2;  // codes of zero: not -inf * 0 where they are masked
         }
@@ -559,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
               const bool f16 = !MIXED || 2 * c + (g >> 1) < staged;
-              const float scale = (&kf[c].x)[g], add = (&lv[c].x)[g] + neg_mref;
+              const float scale = (&kf[c].x)[g], add = (f16 ? (&lv[c].x)[g] : 0.f) + neg_mref;
               const float2 scalev = make_float2(scale, scale), addv = make_float2(add, add);
               float2 gs = make_float2(0.f, 0.f), pv[4];
 #pragma unroll
