@@ -299,9 +299,83 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sV = smem + Cfg::OFF_V;
   const int32_t* btrow = p.bt + (int64_t)b * p.bt_stride;
 
-  if (warp >= kTiles * 4) {
+  auto issue = [&] {
+    // ------------------------------------------------------------ MMA issuer
+    const bool leader = elect_one();
+    // Descriptors of each operand's first 16-element K slice; the slices and
+    // ring stages are constant offsets (16-byte units) from them.
+    const uint64_t qd = umma_sdesc_sw128(smem_u32(sQ), 16, 1024);
+    const uint64_t kd = umma_sdesc_sw128(smem_u32(sK), 16, 1024);
+    const uint64_t vd = umma_sdesc_sw128(smem_u32(sV), Cfg::KV_HALF, 1024);
+    auto issue_s = [&](int t, int j) {
+      const uint64_t kb = kd + (uint64_t)(((j % kStagesK) * Cfg::KV_BYTES) >> 4);
+      const uint64_t qb = qd + (uint64_t)((t * Cfg::Q_BYTES) >> 4);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const uint32_t oq = ((ks >> 2) * Cfg::Q_HALF + (ks & 3) * 32) >> 4;
+        const uint32_t okv = ((ks >> 2) * Cfg::KV_HALF + (ks & 3) * 32) >> 4;
+        if (leader) umma_bf16_ss(tmem + Cfg::COL_S + t * kBN, qb + oq, kb + okv, Cfg::IDESC_S, ks > 0 ? 1u : 0u);
+      }
+      if (leader) umma_commit(&bars->s_full[t]);
+    };
+    auto issue_pv = [&](int t, int j) {
+      const uint64_t vb = vd + (uint64_t)(((j % kStagesV) * Cfg::KV_BYTES) >> 4);
+      if constexpr (Q8) {  // a page, 16 keys, is one step: f16 weights and codes, or two bf16 terms of the weights
+        const int staged = nh - (j0 + j) * kPagesPerBlock;
+        const uint32_t d = tmem + Cfg::COL_O + t * D, w = tmem + Cfg::COL_S + t * kBN;
+#pragma unroll
+        for (int ks = 0; ks < kBN / 16; ++ks) {
+          const uint64_t v = vb + (uint64_t)((ks * (kPageTok * 128)) >> 4);
+          const bool f16 = ks < staged;
+          if (leader) umma_bf16_ts(d, w + ks * 8, v, f16 ? Cfg::IDESC_PV_F16 : Cfg::IDESC_PV, (j > 0 || ks > 0) ? 1u : 0u);
+          if (leader && !f16 && two_terms) umma_bf16_ts(d, w + kBN / 2 + ks * 8, v, Cfg::IDESC_PV, 1u);
+        }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < kBN / 16; ++ks)
+          if (leader)
+            umma_bf16_ts(tmem + Cfg::COL_O + t * D, tmem + Cfg::COL_S + t * kBN + ks * 8,
+                         vb + (uint64_t)((ks * (kPageTok * 128)) >> 4), Cfg::IDESC_PV, (j > 0 || ks > 0) ? 1u : 0u);
+      }
+      if (leader) umma_commit(&bars->pv_done[t]);
+    };
+    // Wait results are made warp-uniform so the whole warp leaves together.
+    bool ok = __all_sync(0xffffffffu, mbar_wait(&bars->q_full, 0));
+    for (int j = 0; ok && j <= nb; ++j) {
+      // PV_A(j-1), S_A(j), PV_B(j-1), S_B(j)
+      if (j < nb) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->k_full[j % kStagesK], (j / kStagesK) & 1));
+        tc_fence_after();
+        if (!ok) break;
+      }
+      if (j > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_full[(j - 1) % kStagesV], ((j - 1) / kStagesV) & 1));
+        if (!ok) break;
+      }
+      for (int t = 0; t < ntiles; ++t) {
+        if (j > 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_full[t], (j - 1) & 1));
+          tc_fence_after();
+          if (!ok) break;
+          issue_pv(t, j - 1);
+        }
+        if (j < nb) issue_s(t, j);
+      }
+      if (!ok) break;
+      if (leader) {
+        if (j < nb) umma_commit(&bars->k_empty[j % kStagesK]);
+        if (j > 0) umma_commit(&bars->v_empty[(j - 1) % kStagesV]);
+      }
+    }
+    if (!ok && leader) {
+      report_error(p.err, DEVERR_WAIT_TIMEOUT, 4, 100);
+      bars->fail = 1;
+    }
+  };
+  // (the bf16 kernel's roles lie side by side: nested as in the other one, they cost it 0.5 %)
+  if (Q8 ? warp >= kTiles * 4 : warp == kWarpK || warp == kWarpK2 || warp == kWarpV) {
     if constexpr (Q8) regs_dec<kOtherRegs>();
-    if (warp != kWarpMma) {
+    if (!Q8 || warp != kWarpMma) {
       // ------------------------------------------------------------ producers
       if (lane == 0) {
         const bool is_k = warp != kWarpV;
@@ -342,9 +416,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (is_k && pi >= p.stage_width) report_error(p.err, DEVERR_BAD_PAGE, 4, pi);
             } else if (pi < npages) {
               pid = btrow[pi];
-              const bool bad = pid < 0 || (int64_t)pid >= p.num_pages || (Q8 && !p.has_pool);
-              if (is_k && bad) report_error(p.err, DEVERR_BAD_PAGE, 4, pid);
-              if (Q8 && bad) pid = (int)p.num_pages;
+              // (only the K producers check it: with the checks in front of every V copy, too, spans over bf16 pages
+              // took 4-7 % longer; ids outside the map read as zeros by themselves)
+              if (is_k && (pid < 0 || (int64_t)pid >= p.num_pages || (Q8 && !p.has_pool)))
+                report_error(p.err, DEVERR_BAD_PAGE, 4, pid);
+              if (Q8 && !p.has_pool) pid = (int)p.num_pages;
             }
 #pragma unroll
             for (int h = 0; h < Cfg::HALVES; ++h)
@@ -353,78 +429,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     } else {
-      // ------------------------------------------------------------ MMA issuer
-      const bool leader = elect_one();
-      // Descriptors of each operand's first 16-element K slice; the slices and
-      // ring stages are constant offsets (16-byte units) from them.
-      const uint64_t qd = umma_sdesc_sw128(smem_u32(sQ), 16, 1024);
-      const uint64_t kd = umma_sdesc_sw128(smem_u32(sK), 16, 1024);
-      const uint64_t vd = umma_sdesc_sw128(smem_u32(sV), Cfg::KV_HALF, 1024);
-      auto issue_s = [&](int t, int j) {
-        const uint64_t kb = kd + (uint64_t)(((j % kStagesK) * Cfg::KV_BYTES) >> 4);
-        const uint64_t qb = qd + (uint64_t)((t * Cfg::Q_BYTES) >> 4);
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t oq = ((ks >> 2) * Cfg::Q_HALF + (ks & 3) * 32) >> 4;
-          const uint32_t okv = ((ks >> 2) * Cfg::KV_HALF + (ks & 3) * 32) >> 4;
-          if (leader) umma_bf16_ss(tmem + Cfg::COL_S + t * kBN, qb + oq, kb + okv, Cfg::IDESC_S, ks > 0 ? 1u : 0u);
-        }
-        if (leader) umma_commit(&bars->s_full[t]);
-      };
-      auto issue_pv = [&](int t, int j) {
-        const uint64_t vb = vd + (uint64_t)(((j % kStagesV) * Cfg::KV_BYTES) >> 4);
-        if constexpr (Q8) {  // a page, 16 keys, is one step: f16 weights and codes, or two bf16 terms of the weights
-          const int staged = nh - (j0 + j) * kPagesPerBlock;
-          const uint32_t d = tmem + Cfg::COL_O + t * D, w = tmem + Cfg::COL_S + t * kBN;
-#pragma unroll
-          for (int ks = 0; ks < kBN / 16; ++ks) {
-            const uint64_t v = vb + (uint64_t)((ks * (kPageTok * 128)) >> 4);
-            const bool f16 = ks < staged;
-            if (leader) umma_bf16_ts(d, w + ks * 8, v, f16 ? Cfg::IDESC_PV_F16 : Cfg::IDESC_PV, (j > 0 || ks > 0) ? 1u : 0u);
-            if (leader && !f16 && two_terms) umma_bf16_ts(d, w + kBN / 2 + ks * 8, v, Cfg::IDESC_PV, 1u);
-          }
-        } else {
-#pragma unroll
-          for (int ks = 0; ks < kBN / 16; ++ks)
-            if (leader)
-              umma_bf16_ts(tmem + Cfg::COL_O + t * D, tmem + Cfg::COL_S + t * kBN + ks * 8,
-                           vb + (uint64_t)((ks * (kPageTok * 128)) >> 4), Cfg::IDESC_PV, (j > 0 || ks > 0) ? 1u : 0u);
-        }
-        if (leader) umma_commit(&bars->pv_done[t]);
-      };
-      // Wait results are made warp-uniform so the whole warp leaves together.
-      bool ok = __all_sync(0xffffffffu, mbar_wait(&bars->q_full, 0));
-      for (int j = 0; ok && j <= nb; ++j) {
-        // PV_A(j-1), S_A(j), PV_B(j-1), S_B(j)
-        if (j < nb) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&bars->k_full[j % kStagesK], (j / kStagesK) & 1));
-          tc_fence_after();
-          if (!ok) break;
-        }
-        if (j > 0) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_full[(j - 1) % kStagesV], ((j - 1) / kStagesV) & 1));
-          if (!ok) break;
-        }
-        for (int t = 0; t < ntiles; ++t) {
-          if (j > 0) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_full[t], (j - 1) & 1));
-            tc_fence_after();
-            if (!ok) break;
-            issue_pv(t, j - 1);
-          }
-          if (j < nb) issue_s(t, j);
-        }
-        if (!ok) break;
-        if (leader) {
-          if (j < nb) umma_commit(&bars->k_empty[j % kStagesK]);
-          if (j > 0) umma_commit(&bars->v_empty[(j - 1) % kStagesV]);
-        }
-      }
-      if (!ok && leader) {
-        report_error(p.err, DEVERR_WAIT_TIMEOUT, 4, 100);
-        bars->fail = 1;
-      }
+      issue();
     }
+  } else if (!Q8 && warp == kWarpMma) {
+    issue();
   } else if ((warp >> 2) < ntiles) {
     if constexpr (Q8) regs_inc<kSoftmaxRegs>();
     // ------------------------------------------------------------ softmax (rows)
@@ -550,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (Q8) l = lowered(l, m - mx);
         m = mx;
       }
-      const float neg_mref = (m == -INFINITY) ? 0.f : (Q8 ? kWeightLog2 : 0.f) - m;
+      const float neg_mref = (m == -INFINITY) ? 0.f : Q8 ? kWeightLog2 - m : -m;
       const float2 sl2v = make_float2(sl2, sl2), negm = make_float2(neg_mref, neg_mref);
       float2 sp[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       // P(j) (bf16 pairs) over the first 64 columns of this tile's S, which is fully
