@@ -913,6 +913,15 @@ class LastKVModel(nn.Module):
         return cached[1]
 
 
+def check_beams(beams: int, eos_token: int | None, vocab: int) -> None:
+    """Refuse what the selection (``ops.beam_select``) does not serve, before anything runs."""
+    if not 1 <= beams <= min(32, vocab):
+        raise RMarinBackendContractError(f"beam search needs a beam ({min(32, vocab)} at most with {vocab} tokens), "
+                                         f"got {beams}")
+    if eos_token is not None and not 0 <= eos_token < vocab:
+        raise RMarinBackendContractError(f"eos_token {eos_token} is not one of {vocab} tokens")
+
+
 class Beams(NamedTuple):
     """Beam search's result, each prompt's best beam first."""
 
@@ -999,8 +1008,9 @@ class LastKVForCausalLM(nn.Module):
         B * num_beams rows (``new_cache``; with ``history="int8"``, say)."""
         B, P = prompt.shape
         K = num_beams
-        if not 1 <= K <= 32 or P < 1:
-            raise RMarinBackendContractError("beam search needs a prompt of one token at least, and a beam (32 at most)")
+        check_beams(K, eos_token, self.config.vocab_size)
+        if P < 1:
+            raise RMarinBackendContractError("beam search needs a prompt of one token at least")
         cache = cache or self.new_cache(B * K, P + max_new_tokens)
         if cache.batch != B * K or cache.seen_tokens:
             raise RMarinBackendContractError(f"beam search needs an empty cache of {B * K} rows")

@@ -32,7 +32,7 @@ import torch
 
 from . import ops
 from .contract import PAGE_SIZE, RMarinBackendContractError
-from .hf import LastKVForCausalLM, PagedLastKVCache
+from .hf import LastKVForCausalLM, PagedLastKVCache, check_beams
 
 
 class GraphDecodeRunner:
@@ -42,7 +42,9 @@ class GraphDecodeRunner:
                  beams: int | None = None, eos_token: int | None = None):
         if device_plan and (cache.q8 is not None or beams is not None):
             raise RMarinBackendContractError("a step planned on the device takes a bf16 history and greedy rows")
-        if beams is not None and (beams < 1 or cache.batch % beams):
+        if beams is not None:
+            check_beams(beams, eos_token, model.config.vocab_size)
+        if beams is not None and cache.batch % beams:
             raise RMarinBackendContractError(f"{cache.batch} rows are not prompts of {beams} beams each")
         self.model, self.cache = model, cache
         dev = cache.device
@@ -259,6 +261,8 @@ class GraphDecodeRunner:
         """Eager chunked prefill in calls of ``call_tokens`` (split at chunk boundaries inside);
         sets the first generated token into the static id buffer.  With beams, ``prompt`` has a row
         for each prompt, whose K best first tokens its beams begin with."""
+        if prompt.shape[1] < 1:
+            raise RMarinBackendContractError("a prefill needs a prompt of one token at least")
         logits, rows = None, None
         if self.beams is not None:
             rows = np.arange(0, self.B, self.beams)
