@@ -364,6 +364,7 @@ class PagedLastKVCache:
         self.src_table_dev = torch.from_numpy(self.src_table).to(device)
         self._own_ring = np.arange(batch * self.ring_pages, dtype=np.int32).reshape(batch, self.ring_pages)
         self.ring_table = self._own_ring.copy()  # relative to a layer's ring
+        self._reordered = False  # whether rows may read pages of one another (``shared``)
         self._rows = np.arange(batch)  # the rows that spans are planned for (only_rows)
         self.ring_base = self.src_pages + np.arange(self.num_layers) * self.ring_stride
         self.ring_base_dev = torch.from_numpy(self.ring_base.astype(np.int32)).to(device)
@@ -449,6 +450,7 @@ class PagedLastKVCache:
         if idx.shape[0] != self.batch or (idx.size and (idx.min() < 0 or idx.max() >= self.batch)):
             raise RMarinBackendContractError(f"beam_idx must name {self.batch} of the cache's rows")
         self.flush_commit()
+        self._reordered = True
         C, P, RP = self.chunk_size, PAGE_SIZE, self.ring_pages
         full = self.seen_tokens // P
         old_src, old_ring = self.src_table, self.ring_table
@@ -490,7 +492,10 @@ class PagedLastKVCache:
     @property
     def shared(self) -> bool:
         """Whether rows read pages of one another (after ``reorder_cache``)."""
-        return not (np.array_equal(self.src_table, self._own_src) and np.array_equal(self.ring_table, self._own_ring))
+        if self._reordered:
+            self._reordered = not (np.array_equal(self.src_table, self._own_src)
+                                   and np.array_equal(self.ring_table, self._own_ring))
+        return self._reordered
 
     def unshare_(self) -> None:
         """Copy what rows share to pages of their own, so that row b's pages are those of a cache that was never
