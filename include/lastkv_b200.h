@@ -165,7 +165,8 @@ int lkv_decode_plan(int batch, int num_q_heads, int num_kv_heads, int head_dim, 
  * causal = 0 it is the non-causal block attention of the Wan path
  * (videogen/src/lastkv/videogen/attention.py:9-32).
  *   q / out      bf16 [total_q, num_q_heads, head_dim] rows (16-byte aligned)
- *   cu_seqlens_q int32 [batch + 1] query offsets; max_q >= every span length
+ *   cu_seqlens_q int32 [batch + 1] query offsets; max_q >= every span length; out and
+ *                lse keep their rows of tokens in front of the first and behind the last
  *   seq_k        int32 [batch] keys per sequence (>= its span when causal);
  *                query i of a span of Lq attends keys [0, seq_k - Lq + i]
  *   out_scale    fp32 [num_q_heads] or NULL (folds s_l)

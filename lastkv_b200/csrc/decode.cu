@@ -633,6 +633,8 @@ struct MergeParams {
   float* lse_out;        // natural log [rows] or null
   float* out_f32;        // fp32 normalised [rows, D] instead of bf16 (partial of partials) or null
   float* out_lse_f32;    // natural log [rows] for out_f32 mode
+  const int32_t* cu;     // rows of tokens in front of cu[0] or from cu[batch] on stay as they are, or null: none
+  int batch;
 };
 
 template <int D>
@@ -643,6 +645,7 @@ __global__ void __launch_bounds__(128) merge_partials_kernel(const MergeParams p
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 4 + warp;
   if (row >= p.rows) return;
+  if (p.cu && (row < (int64_t)p.cu[0] * p.Hq || row >= (int64_t)p.cu[p.batch] * p.Hq)) return;  // no span's
   const float to2 = p.lse_log2 ? 1.f : 1.4426950408889634f;
   auto lse_at = [&](int s) -> float {
     const int64_t i = p.split_major ? (int64_t)s * p.lse_part_stride + row : row * p.S + s;
@@ -991,7 +994,7 @@ int decode_plan(int batch, int hq, int hkv, int d, int max_pages, size_t workspa
 
 int merge_partials(const float* o_parts, const float* lse_parts, int num_parts, int64_t rows, int head_dim, int hq,
                    int64_t o_part_stride, int64_t lse_part_stride, const float* out_scale, void* out,
-                   float* lse_out, cudaStream_t stream, int64_t out_stride_tok) {
+                   float* lse_out, cudaStream_t stream, int64_t out_stride_tok, const int32_t* cu, int batch) {
   if (head_dim != 64 && head_dim != 128) return LKV_ERR_UNSUPPORTED;
   if (num_parts < 1 || rows < 0 || hq < 1 || rows % hq) return LKV_ERR_INVALID_ARGUMENT;
   if (rows == 0) return LKV_OK;
@@ -1018,6 +1021,8 @@ int merge_partials(const float* o_parts, const float* lse_parts, int num_parts, 
   if (out_stride_tok < (int64_t)hq * head_dim || (out_stride_tok & 1)) return LKV_ERR_INVALID_ARGUMENT;
   mp.out_stride_tok = out_stride_tok;
   mp.lse_out = lse_out;
+  mp.cu = cu;
+  mp.batch = batch;
   const unsigned blocks = (unsigned)((rows + 3) / 4);
   const cudaError_t e = head_dim == 128 ? launch_pdl(merge_partials_kernel<128>, dim3(blocks), dim3(128), 0, stream, mp)
                                          : launch_pdl(merge_partials_kernel<64>, dim3(blocks), dim3(128), 0, stream, mp);

@@ -145,9 +145,11 @@ int noalloc_scratch_prepare();
 int decode_paged(const DecodeArgs& a);
 int decode_plan(int batch, int hq, int hkv, int d, int max_pages, size_t workspace_bytes, int partial, int* splits,
                 int* launches);
+// cu [batch + 1] (or null): tokens in front of its first and from its last value on are left as they are.
 int merge_partials(const float* o_parts, const float* lse_parts, int num_parts, int64_t rows, int head_dim, int hq,
                    int64_t o_part_stride, int64_t lse_part_stride, const float* out_scale, void* out,
-                   float* lse_out, cudaStream_t stream, int64_t out_stride_tok = 0);
+                   float* lse_out, cudaStream_t stream, int64_t out_stride_tok = 0, const int32_t* cu = nullptr,
+                   int batch = 0);
 
 struct AppendArgs {
   const void* q;

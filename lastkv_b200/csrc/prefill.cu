@@ -893,7 +893,7 @@ int prefill_paged(const PrefillArgs& a) {
   // exact LSE merge of the splits into out (x out_scale) and lse
   return merge_partials(a.part_o, a.part_lse, S, prm.part_rows, a.head_dim, a.num_q_heads,
                         prm.part_rows * a.head_dim, prm.part_rows, a.out_scale, a.out, a.lse, stream,
-                        a.out_stride_tok);
+                        a.out_stride_tok, a.cu_q, a.batch);
 }
 
 // Key splits of a call over 8-bit pages, causal or not: what the waves of CTAs take, in blocks (about 1.5 us), with
