@@ -569,8 +569,8 @@ int lkv_cp_combine(const float* send, const uint64_t* peer_recv, int rank, int w
  * layout of a row (older pages, then recent ones) is the merged pool's.
  *
  * lkv_q8_quantize_pages: page pages[i] of a bf16 pool into 8-bit page out_pages[i], i < n:
- *   scale = max|x| / 127, code = round-to-nearest-even(x / scale), zeros where the
- *   scale is 0.  tokens (int32 [n], may be NULL: 16) counts the tokens that a page
+ *   scale = max|x| / 127, code = round-to-nearest-even(x / scale), both quotients in fp32,
+ *   zeros where the scale is 0.  tokens (int32 [n], may be NULL: 16) counts the tokens that a page
  *   holds; the rest become zeros and do not count for the scale.  A block of 8 tokens
  *   that holds an infinity or a NaN has that scale and zero codes: its values are NaN.
  *   No two out_pages may be the same.

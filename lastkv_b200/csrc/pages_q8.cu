@@ -1,7 +1,7 @@
 // Pages of a bf16 pool to 8 bits and back, and copies of whole pages (sm_100a).
 //
-//   quantise    per (page, KV head, keys or values, 8 tokens): s = max|x| / 127 in fp32, q = rne(x / s)
-//               of that s (zeros where s = 0); a block that holds an infinity or a NaN gets that scale and
+//   quantise    per (page, KV head, keys or values, 8 tokens): s = max|x| / 127 and q = rne(x / s) in
+//               fp32 arithmetic (zeros where s = 0); a block that holds an infinity or a NaN gets that scale and
 //               zeros, so its values are NaN.  Tokens past the page's count are zeros and do not
 //               count for the scale.
 //   dequantise  bf16(q * s), or (staging for the prefill kernel) the codes themselves, which are
@@ -113,29 +113,20 @@ __global__ void __launch_bounds__(kWarps * 32, 8) quantise_pages_kernel(const Qu
     const float amax = max_nan(bf16_lo(m2), bf16_hi(m2));
     const float scale = amax / 127.0f;
     scales[i] = scale;
-    // The code is rne(x / scale) of the stored scale, by one division per block: x * inv with inv = 127 / max, rounded
-    // by the addition that puts q + 128 into the low byte of 1.5 * 2^23 + 128 + q.  A bf16 x comes closer than 2^-17
-    // to a place half way between two codes only where 127 x / max is one; but for x = max / 2, at 63.5, both
-    // roundings are exact there.  So it is enough that max / 2 goes to the side that the scale's rounding puts it
-    // on (64 from 63.5 on): inv is one step from the nearest where that one goes to the other side.
+    // The code is the fp32 quotient x / scale rounded to nearest even, by two divisions per block: x * inv with
+    // inv = 127 / max, rounded by the addition that puts q + 128 into the low byte of 1.5 * 2^23 + 128 + q.  A bf16 x
+    // comes closer than 2^-17 to a place half way between two codes only where 127 x / max is one; but for
+    // x = max / 2, at 63.5, the scale and inv are exact there.  So it is enough that max / 2 goes to the side that its
+    // quotient is on (64 from 63.5 on): inv is one step from the nearest where that one goes to the other side.
     float inv = 127.0f / amax;
     {
-      const bool up = fmaf(-127.0f, scale, amax) >= 0.f, inv_up = fmaf(amax, inv, -127.0f) >= 0.f;  // both exact
+      const bool up = 0.5f * amax / scale >= 63.5f, inv_up = fmaf(amax, inv, -127.0f) >= 0.f;  // (the latter exact)
       if (up != inv_up) inv = __uint_as_float(__float_as_uint(inv) + (up ? 1u : ~0u));
     }
     if (!(amax >= 1e-30f && amax < INFINITY)) {
-      // scales with few bits, or none, or not finite: the codes themselves take the values' place.  Times 2^96 all
-      // numbers are ordinary ones, and a quotient's remainder is exact.
+      // scales with few bits, or none, or not finite: the codes themselves take the values' place
       const bool zero = !(amax < INFINITY) || scale == 0.f;
-      const float s96 = scale * 0x1p96f;
-      auto code = [&](float x) {
-        if (zero) return 0.f;
-        x *= 0x1p96f;
-        float q = rintf(x / s96);
-        const float r2 = 2.f * fmaf(-q, s96, x), past = fabsf(r2) - s96;  // twice what is left, against a whole step
-        if (past > 0.f || (past == 0.f && fmodf(q, 2.f) != 0.f)) q += copysignf(1.f, r2);
-        return q;
-      };
+      auto code = [&](float x) { return zero ? 0.f : rintf(x / scale); };
       inv = 1.f;
 #pragma unroll 1
       for (int e = 0; e < 2; ++e)
