@@ -12,19 +12,20 @@
 // takes the 1152 off (bf16, with 7 bits of mantissa, took 3.5 instructions for two codes instead of 2).
 // - Q: a row's heads are divided by a power of two that brings their largest value to 1 .. 2 and rounded to
 //   f16: exact but for values below 2^-17 of the largest, which are rounded at 2^-25 of it.
-// - p * value scale: with t = s + log2(value scale) and M its running maximum, the product is 2^(t - M)
-//   whatever the scales are, in 0 .. 1; times 2^15 it uses f16's whole range, 11 bits down to
+// - p * value scale: with t = s + log2(value scale) and M its running maximum, the product is 2^(t - M),
+//   in 0 .. 1; times 2^15 it uses f16's whole range, 11 bits down to
 //   2^-29 of the largest and 2^-40 of it as the smallest step.  A token's part of the sum of weights is that
 //   number (in fp32) divided by the value scale; the scales of a row may lie 2^90 apart (zero aside), further the
 //   number flushes to 0 for tokens that still count.
-// bf16 pages keep bf16 operands, and the same M with a value scale of 1.
+// bf16 pages keep bf16 operands, and the same M with a value scale of 1 (a slot has pages of one kind, and a row's
+// 8-bit ones come first: their products are in the fp32 sums before a larger M).
 //
 // Bound by HBM: an 8-bit page is half a bf16 page's bytes.  Work is counted in slots of equal bytes, one bf16
 // page or two 8-bit pages of one KV head.  The rows' slots lie end to end, (row, head) after
 // (row, head), each behind the places of what a (row, head) costs by itself, and every CTA takes the same number
 // of places, so ragged rows cost no balance; a (row, head)'s part within a CTA is a piece, whose normalised partial goes to the workspace, and
-// join_pieces_kernel joins each row's pieces.  Per CTA one warp fills a ring of slots (an 8-bit page's codes and
-// scales by two bulk copies, a bf16 page's halves by TMA), 6 warps take the slots in turn.
+// join_pieces_kernel joins each row's pieces.  Per CTA one warp fills a ring of slots (an 8-bit page's codes by
+// a bulk copy and its scales by cp.async, a bf16 page's halves by TMA), 6 warps take the slots in turn.
 
 #include <math.h>
 

@@ -62,7 +62,7 @@
 // staging, 212 without (prefill_paged: 182).  The softmax of a block bounds it, as there, with the scales in its
 // chain.
 //
-// Key splits (non-causal calls, S > 1): blockIdx.z = sequence * S + split and
+// Key splits (non-causal calls and those over 8-bit pages, S > 1): blockIdx.z = sequence * S + split and
 // a CTA covers its split's share of the key blocks, writing the normalised
 // fp32 partial and natural-log LSE of its rows; merge_partials_kernel then
 // combines the splits exactly.  With one CTA per SM, this fills the last wave

@@ -311,16 +311,16 @@ class PagedLastKVCache:
     ``history="int8"`` (bf16 caches): the shared history is held in 8 bits (``q8``, an
     ``ops.PagesQ8``), half its memory and of what a decode step reads of it.  A chunk's raw K and V
     go to a ring of 2C tokens per sequence in front of the layers' rings and are rounded to 8 bits
-    when the chunk is finished, a scale for every 8 tokens of a head; the previous and current
-    chunk stay bf16, and so does the blend.
+    when the chunk is finished, a scale for every 8 tokens of a head, by every row to pages of its own;
+    the previous and current chunk stay bf16, and so does the blend.
 
     After ``reorder_cache`` rows share the pages that their common tokens filled (``src_table``,
     ``ring_table``): a page is written by one row and read by any, and every row writes its own
     pages, those of a cache that was never reordered.
     """
 
-    #: bf16 copies of 8-bit pages that a prefill call may hold at once (``history="int8"``); rows beyond
-    #: that are taken in turns
+    #: bytes of staged 8-bit pages (``ops.StageQ8``: keys in bf16, values in fp16) that a prefill call may hold at
+    #: once (``history="int8"``); rows beyond that are taken in turns
     stage_bytes = 2 << 30
 
     def __init__(self, config: LastKVConfig, batch: int, max_tokens: int, device=None, *, page_order=None,
