@@ -58,8 +58,8 @@
 // without scales, and took the error from 1.0 to 1.4, in short rows 1.7, times the output's rounding); bf16
 // pages bf16 weights, and where they are most of the row a second bf16 term with what the first leaves out,
 // in S's other columns.  That term in every row cost 11 % of a call with a quarter of its keys in bf16.
-// Two spans of 1024 tokens, 32 heads of 128 over 8, against 8192 keys and half of that: 221 us with the
-// staging, 212 without (prefill_paged: 182).  The softmax of a block bounds it, as there, with the scales in its
+// Two spans of 1024 tokens, 32 heads of 128 over 8, against 8192 keys and half of that: 219 us with the
+// staging, 209 without (prefill_paged: 167).  The softmax of a block bounds it, as there, with the scales in its
 // chain.
 //
 // Key splits (non-causal calls and those over 8-bit pages, S > 1): blockIdx.z = sequence * S + split and
@@ -95,8 +95,8 @@ constexpr float kRescaleLog2 = 8.0f;
 constexpr float kLeastPageScale = 0x1p-60f;  // Q8: bf16 pages' weights are 2^75 at most
 constexpr float kWeightLog2 = 7.0f;  // Q8: weights are times 2^7, so that f16 has 2^15 for the largest
 // Q8: registers of a softmax thread, and of the others, of the 168 that each was launched with (8 warps gain
-// what 4 lose).  Two spans of 1024 tokens over 8192 keys: 223 us, with 168 each 239; the scales of a block then fit
-// into registers before its scores are waited for: 212.
+// what 4 lose).  Two spans of 1024 tokens over 8192 keys, without the staging: 223 us, with 168 each 239; the scales of
+// a block then fit into registers before its scores are waited for: 212, now 209 (4 bytes spilled with heads of 128).
 constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 constexpr int kMaxKvSplits = 8;
 
