@@ -607,9 +607,10 @@ int lkv_decode_paged_q8(const void* q, int64_t q_stride_tok, const uint8_t* code
  * page b * stage_width + column of stage_k (bf16) and stage_v (fp16) [batch * stage_width,
  * 16, num_kv_heads, head_dim], whose contents need not be kept; staged = 1: an earlier call with
  * the same rows, pages and stage_width did that (layers that read the same older pages) and
- * the call reads the copy.  stage_width >= 1 may be above the table's columns.  A row with more
- * 8-bit pages than stage_width is recorded in error_word (may be NULL), its further ones
- * read as zeros.
+ * the call reads the copy; staged = 2: as 0, for a stage that may be wider than the table's
+ * max_pages_per_seq columns, which 0 refuses (its rows lie stage_width apart all the same).
+ * stage_width >= 1.  A row with more 8-bit pages than stage_width is recorded in
+ * error_word (may be NULL), its further ones read as zeros.
  * kv_splits > 1 (at most 8; lkv_prefill_q8_split_plan gives a good number): as for
  * lkv_prefill_paged_split, with part_o fp32 [kv_splits, total_q * num_q_heads, head_dim] and
  * part_lse fp32 [kv_splits, total_q * num_q_heads]; causal calls take it too. */

@@ -654,7 +654,7 @@ int lkv_prefill_paged_q8(const void* q, int64_t q_stride_tok, const uint8_t* cod
   a.kv_splits = kv_splits;
   a.part_o = part_o;
   a.part_lse = part_lse;
-  return lkv::prefill_paged_q8(a, codes, staged != 0);
+  return lkv::prefill_paged_q8(a, codes, staged);
 }
 
 int lkv_prefill_q8_split_plan(int batch, int max_q, int total_q, int num_q_heads, int num_kv_heads, int head_dim,

@@ -55,8 +55,9 @@ struct PrefillArgs {
   int64_t q8_pages = 0;
 };
 int prefill_paged(const PrefillArgs& a);
-// With 8-bit pages: stages their codes first, unless that is done.
-int prefill_paged_q8(const PrefillArgs& a, const void* codes, bool staged);
+// With 8-bit pages: stages their codes first (staged 0, or 2 where the stage may be wider than the table), unless that
+// is done (1).
+int prefill_paged_q8(const PrefillArgs& a, const void* codes, int staged);
 int prefill_q8_split_plan(int batch, int max_q, int total_q, int num_q_heads, int num_kv_heads, int head_dim,
                           int max_pages, int* kv_splits);
 int prefill_split_plan(int batch, int max_q, int num_q_heads, int num_kv_heads, int head_dim, int max_pages,

@@ -791,12 +791,13 @@ int check_args(const PrefillArgs& a, bool* empty) {
 }
 }  // namespace
 
-int prefill_paged_q8(const PrefillArgs& a, const void* codes, bool staged) {
+int prefill_paged_q8(const PrefillArgs& a, const void* codes, int staged) {
   bool empty;
   const int st = check_args(a, &empty);
   if (st != LKV_OK || empty) return st;
   if (!a.stage_k) return LKV_ERR_INVALID_ARGUMENT;
-  if (!staged) {
+  if (staged == 0 && a.stage_width > a.max_pages_per_seq) return LKV_ERR_INVALID_ARGUMENT;
+  if (staged == 0 || staged == 2) {
     const int rc = stage_pages(codes, a.q8_scales, a.q8_pages, a.block_table, a.block_table_stride, a.num_q8, a.seq_k,
                                a.batch, a.max_pages_per_seq, a.stage_k, a.stage_v, a.stage_width, a.num_kv_heads,
                                a.head_dim, a.error_word, static_cast<cudaStream_t>(a.stream));

@@ -1324,7 +1324,7 @@ def prefill_paged_q8(q, cache: PagesQ8, block_table, seq_k, cu_q, max_q: int, *,
                   "call's CUDA device")
         part_o, part_lse = o.data_ptr(), e.data_ptr()
     st = _capi.lib().lkv_prefill_paged_q8(
-        q.data_ptr(), q_row, codes, scales, q8_pages, sk, sv, stage.width, int(staged), k, v, num, table,
+        q.data_ptr(), q_row, codes, scales, q8_pages, sk, sv, stage.width, 1 if staged else 2, k, v, num, table,
         t_row, nq8, seq, _ints(cu_q, B + 1, dev, "cu_q"), out.data_ptr(), o_row, l, f, B, T, int(max_q), Hq, h, D, W,
         int(bool(causal)), D ** -0.5 if softmax_scale is None else softmax_scale, kv_splits, part_o, part_lse,
         _err_ptr(error_word), _raw_stream(dev))
